@@ -71,6 +71,14 @@ def _init_cuda():
     _cuda = torch._C
 
 
+def check_device(t) -> None:
+    """Refuse a tensor of another GPU than the current one, whose stream the launch would go to."""
+    if _cuda is None:
+        _init_cuda()
+    if t.get_device() != _cuda._cuda_getDevice():
+        raise ValueError(f"the tensor is on {t.device}, the current GPU is cuda:{_cuda._cuda_getDevice()}")
+
+
 def _block_here(t) -> bool:
     """One block of memory on the current GPU, whose current stream a clear may go to."""
     if not (t.is_cuda and t.is_contiguous()):

@@ -25,6 +25,7 @@ CU_SOURCES = [
     "ops/ops.cu",
     "ops/attention.cu",
     "ops/attention_noalloc.cu",
+    "ops/rotary.cu",
     "comm/p2p.cu",
 ]
 CPP_SOURCES = ["bindings.cpp"]

@@ -19,6 +19,7 @@
 #include "gemm/sm100_gemm.h"
 #include "ops/attention.h"
 #include "ops/ops.h"
+#include "ops/rotary.h"
 
 namespace py = pybind11;
 using namespace msb;
@@ -531,6 +532,12 @@ void py_attention_bwd(uint64_t qkv, uint64_t out, uint64_t dout, uint64_t lse, u
                       seq, heads, causal, scale, P<uint32_t>(status), S(stream)), "attention_bwd");
 }
 
+void py_rotary(uint64_t x, uint64_t y, int64_t ldx, int64_t ldy, uint64_t positions, uint64_t turns, int tokens, int seq, int kv, int group,
+               int head_dim, int rot_dim, int half, float sign, float factor, uint64_t stream) {
+  check(rotary({P<void>(x), P<void>(y), ldx, ldy, P<int64_t>(positions), P<uint64_t>(turns), tokens, seq, kv, group, head_dim, rot_dim,
+                half, sign, factor}, S(stream)), "rotary");
+}
+
 void memset_zero(uint64_t ptr, size_t bytes, uint64_t stream) {
   check(cudaMemsetAsync(P<void>(ptr), 0, bytes,
                         reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream))),
@@ -673,6 +680,8 @@ PYBIND11_MODULE(_C, m) {
       MSB_DIRECT("attention_fwd", py_attention_fwd, "qkv, out, lse, batch, seq, heads, causal, scale, status, stream"),
       MSB_DIRECT("attention_bwd", py_attention_bwd, "qkv, out, dout, lse, dqkv, dq_acc, delta, batch, seq, heads, causal, scale, "
                  "status, stream"),
+      MSB_DIRECT("rotary", py_rotary, "x, y, ldx, ldy, positions, turns, tokens, seq, kv, group, head_dim, rot_dim, half, sign, factor, "
+                 "stream"),
       {nullptr, nullptr, 0, nullptr}};
 #undef MSB_DIRECT
   if (PyModule_AddFunctions(m.ptr(), direct_calls) != 0) throw py::error_already_set();

@@ -10,6 +10,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
+from .rotary import Rotary, RotaryConfig, rotary_qkv  # noqa: F401  (ops of this module's callers)
 
 GELU_K0 = 0.7978845608028654
 GELU_K1 = 0.044715
