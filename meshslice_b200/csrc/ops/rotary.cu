@@ -157,7 +157,8 @@ cudaError_t rotary(const RotaryArgs& a, cudaStream_t stream) {
   w.per_cta = per < spread ? per : spread;
   if (w.per_cta > kMaxTokens) w.per_cta = kMaxTokens;
   const unsigned grid = (unsigned)((a.tokens + w.per_cta - 1) / w.per_cta);
-  return launch_dependent(a.half ? rotary_kernel<true> : rotary_kernel<false>, grid, kThreads, 0, stream, w);
+  auto kernel = a.half ? rotary_kernel<true> : rotary_kernel<false>;
+  return launch_dependent(kernel, grid, kThreads, 0, stream, w);
 }
 
 }  // namespace msb
