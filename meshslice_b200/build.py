@@ -26,6 +26,7 @@ CU_SOURCES = [
     "ops/attention.cu",
     "ops/attention_noalloc.cu",
     "ops/rotary.cu",
+    "ops/distill.cu",
     "comm/p2p.cu",
 ]
 CPP_SOURCES = ["bindings.cpp"]

@@ -18,6 +18,7 @@
 #include "comm/p2p.h"
 #include "gemm/sm100_gemm.h"
 #include "ops/attention.h"
+#include "ops/distill.h"
 #include "ops/ops.h"
 #include "ops/rotary.h"
 
@@ -538,6 +539,15 @@ void py_rotary(uint64_t x, uint64_t y, int64_t ldx, int64_t ldy, uint64_t positi
                 half, sign, factor}, S(stream)), "rotary");
 }
 
+// step: 0 whole rows, 1 statistics of a slice, 2 gradient of a slice
+void py_distill(int step, uint64_t logits, int64_t ld, uint64_t grad, int64_t ldg, uint64_t ids, uint64_t values, int values_bf16,
+                uint64_t targets, int rows, int cols, int col_offset, int vocab, int top, float temperature, float hard, float scale,
+                uint64_t loss, uint64_t stats, uint64_t stream) {
+  const DistillArgs a{P<void>(logits), P<void>(grad), ld, ldg, P<int64_t>(ids), P<void>(values), values_bf16, P<int64_t>(targets), rows,
+                      cols, col_offset, vocab, top, temperature, hard, scale, P<float>(loss), P<float>(stats)};
+  check(step == 0 ? distill_row(a, S(stream)) : step == 1 ? distill_partial(a, S(stream)) : distill_grad(a, S(stream)), "distill");
+}
+
 void memset_zero(uint64_t ptr, size_t bytes, uint64_t stream) {
   check(cudaMemsetAsync(P<void>(ptr), 0, bytes,
                         reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream))),
@@ -617,6 +627,8 @@ PYBIND11_MODULE(_C, m) {
   m.def("ln_grid", &ln_grid, py::arg("backward"), py::arg("rows"), py::arg("cols") = 0,
         "CTAs of the LayerNorm kernels in a row exchange for a row count and local width (0: forward, 1: backward)");
   m.attr("CE_ROW_COLS") = ce_row_cols();
+  m.attr("DISTILL_ROW_COLS") = distill_row_cols();
+  m.attr("DISTILL_TOP") = kDistillTop;
   m.def("ce_grid", &ce_grid, "CTAs of the cross-entropy kernels in a row exchange for a row count");
   m.def("cast_f32_to_bf16", [](uint64_t in, uint64_t out, int64_t n, int accumulate, uint64_t stream) {
     check(cast_f32_to_bf16(P<float>(in), P<void>(out), n, accumulate, S(stream)), "cast_f32_to_bf16");
@@ -682,6 +694,8 @@ PYBIND11_MODULE(_C, m) {
                  "status, stream"),
       MSB_DIRECT("rotary", py_rotary, "x, y, ldx, ldy, positions, turns, tokens, seq, kv, group, head_dim, rot_dim, half, sign, factor, "
                  "stream"),
+      MSB_DIRECT("distill", py_distill, "step, logits, ld, grad, ldg, ids, values, values_bf16, targets, rows, cols, col_offset, vocab, "
+                 "top, temperature, hard, scale, loss, stats, stream"),
       {nullptr, nullptr, 0, nullptr}};
 #undef MSB_DIRECT
   if (PyModule_AddFunctions(m.ptr(), direct_calls) != 0) throw py::error_already_set();

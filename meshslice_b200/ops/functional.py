@@ -10,7 +10,8 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from .rotary import Rotary, RotaryConfig, rotary_qkv  # noqa: F401  (ops of this module's callers)
+from .distill import distill_grad, distill_loss_grad, distill_partial  # noqa: F401  (ops of this module's callers)
+from .rotary import Rotary, RotaryConfig, rotary_qkv  # noqa: F401
 
 GELU_K0 = 0.7978845608028654
 GELU_K1 = 0.044715

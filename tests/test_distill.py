@@ -1,0 +1,255 @@
+"""Distillation loss and gradient: CPU formulation and kernels against the definition in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from meshslice_b200.ops import functional as F
+from meshslice_b200.ops.distill import distill_rescale
+
+
+def definition(z, ids, values, targets, vocab, T, w):
+    """(loss, d loss / d z, sum of the absolute parts of the loss, of the gradient) in 64 bits, row by row.  Not for NaN."""
+    n, cols = z.shape
+    loss, grad = torch.zeros(n, dtype=torch.float64), torch.zeros(n, cols, dtype=torch.float64)
+    size, parts = torch.ones(n, dtype=torch.float64), torch.zeros(n, cols, dtype=torch.float64)
+    for r in range(n):
+        x = z[r, :vocab].double()
+        kept = [(int(i), float(v)) for i, v in zip(ids[r], values[r]) if 0 <= int(i) < vocab and float(v) != -math.inf]
+        if kept and w != 1.0:
+            e = torch.softmax(torch.tensor([v for _, v in kept], dtype=torch.float64) / T, 0)
+            p = torch.zeros(vocab, dtype=torch.float64)
+            for (i, _), q in zip(kept, e):
+                p[i] += q
+            logq = torch.log_softmax(x / T, 0)
+            # entries of one id are one event each with that token's probability under the student
+            terms = [q * (q.log() - logq[i]) for (i, _), q in zip(kept, e) if q > 0]
+            loss[r] += (1 - w) * T * T * sum(terms)
+            size[r] += T * T * (1 + (e * e.clamp_min(1e-300).log()).sum().abs() + torch.logsumexp(x / T, 0).abs() + x.max().abs()) \
+                + T * (p * torch.where(p > 0, (x - x.max()).abs(), 0.0)).sum()
+            grad[r, :vocab] += (1 - w) * T * (logq.exp() - p)
+            parts[r, :vocab] += (1 - w) * T * (logq.exp() + p)
+        y = -1 if targets is None else int(targets[r])
+        if 0 <= y < vocab and w != 0.0:
+            logq = torch.log_softmax(x, 0)
+            loss[r] -= w * logq[y]
+            size[r] += torch.logsumexp(x, 0).abs() + (x[y] - x.max()).abs() + x.max().abs()
+            hot = torch.zeros(vocab, dtype=torch.float64)
+            hot[y] = 1
+            grad[r, :vocab] += w * (logq.exp() - hot)
+            parts[r, :vocab] += w * (logq.exp() + hot)
+    return loss, grad, size, parts
+
+
+def data(rows, vocab, cols, top, missing=False, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    z = (torch.randn(rows, cols, generator=g) * 2).bfloat16()
+    ids = torch.stack([torch.randperm(vocab, generator=g)[:top] for _ in range(rows)]) if top else torch.zeros(rows, 0, dtype=torch.int64)
+    values = torch.randn(rows, top, generator=g) * 3
+    targets = torch.randint(0, vocab, (rows,), generator=g)
+    if missing:
+        ids[0::3, top // 2:] = -1
+        ids[1::4] = vocab
+        values[2::5, : top // 2 + 1] = -math.inf
+        targets[1::3] = -1
+    elif top:
+        targets[::2] = ids[::2, 0]                     # labels among the entries
+    return z, ids, values, targets
+
+
+def check(got, want, scale, bits=20):
+    """Loss: exponentials are 2^-22 off, sums and logarithms 2^-23 a step: 2^-19 of the absolute parts.  Gradient: half a unit of
+    bf16 (2^-8), and of its parts 2^-17: the exponent (z - m) / T, up to 2^5, is rounded to 24 bits."""
+    loss, grad = got
+    wl, wg, size, parts = want
+    assert ((loss.double().cpu() - wl).abs() <= 2.0 ** -19 * size).all()
+    bound = 2.0 ** -8 * wg.abs() * scale + 2.0 ** -17 * parts * scale + 1e-37
+    assert ((grad.double().cpu() - wg * scale).abs() <= bound).all()
+
+
+SETTINGS = [(1.0, 0.0), (1.0, 0.3), (2.0, 0.0), (2.0, 0.5), (0.7, 1.0), (4.0, 0.1)]
+SIZES = [(1, 1, 8, 1), (5, 203, 208, 9), (17, 1000, 1024, 33), (3, 9, 16, 9), (2, 40, 40, 0)]
+
+
+def run(dev, size, T, w, missing, values_dtype=torch.float32, use_targets=True, in_place=False):
+    rows, vocab, cols, top = size
+    z, ids, values, targets = data(rows, vocab, cols, top, missing)
+    values = values.to(values_dtype)
+    t = targets if use_targets else None
+    want = definition(z, ids, values, t, vocab, T, w)
+    a = [x.to(dev) if x is not None else None for x in (z, ids, values, t)]
+    got = F.distill_loss_grad(a[0], a[1], a[2], vocab, 0.25, temperature=T, targets=a[3], hard_weight=w, out=a[0] if in_place else None)
+    check(got, want, 0.25)
+    assert got[1][:, vocab:].count_nonzero() == 0
+    if in_place:
+        assert got[1] is a[0]
+    else:
+        assert torch.equal(a[0].cpu(), z)
+    return got
+
+
+@pytest.mark.parametrize("missing", [False, True])
+@pytest.mark.parametrize("T,w", SETTINGS)
+@pytest.mark.parametrize("size", SIZES)
+def test_cpu(size, T, w, missing):
+    run("cpu", size, T, w, missing)
+
+
+def slices(z, ids, values, targets, vocab, T, w, cuts, scale):
+    """Loss and gradient by way of the statistics of column slices, as a mesh row computes them."""
+    parts = [z[:, a:b].contiguous() for a, b in zip(cuts, cuts[1:])]
+    st = [F.distill_partial(p, ids, values, a, vocab, T, targets) for p, a in zip(parts, cuts)]
+    gmax = torch.stack([s[:, 0] for s in st]).amax(0)
+    total = sum(distill_rescale(s, gmax, T) for s in st)
+    total[:, 0] = gmax
+    got = [F.distill_grad(p, ids, values, a, vocab, scale, total, T, targets, w) for p, a in zip(parts, cuts)]
+    for other in got[1:]:
+        assert torch.equal(other[0], got[0][0])
+    return got[0][0], torch.cat([g for _, g in got], 1)
+
+
+@pytest.mark.parametrize("T,w", SETTINGS)
+def test_cpu_slices(T, w):
+    z, ids, values, targets = data(11, 203, 256, 9, True)
+    got = slices(z, ids, values, targets, 203, T, w, [0, 64, 128, 208, 256], 0.5)
+    check(got, definition(z, ids, values, targets, 203, T, w), 0.5)
+
+
+def test_gradient_against_differences():
+    """Central differences of the definition's loss in 64 bits against the formulation's gradient (fp32 logits: no rounding to bf16)."""
+    z, ids, values, targets = data(2, 20, 24, 5)
+    z = z.float()
+    for T, w in SETTINGS:
+        _, grad = F.distill_loss_grad(z, ids, values, 20, 1.0, temperature=T, targets=targets, hard_weight=w)
+        for c in range(20):
+            d = torch.zeros_like(z, dtype=torch.float64)
+            d[:, c] = 1e-4
+            up, down = (definition(z.double() + s * d, ids, values, targets, 20, T, w)[0] for s in (1, -1))
+            assert ((up - down) / 2e-4 - grad[:, c].double()).abs().max() < 1e-5
+
+
+def test_duplicates_and_ignored_rows():
+    """An id that occurs twice takes both probabilities; a row without entries and label is zero whatever its logits are."""
+    z, ids, values, targets = data(3, 50, 56, 6)
+    ids[:, 3] = ids[:, 0]
+    want = definition(z, ids, values, targets, 50, 2.0, 0.5)
+    check(F.distill_loss_grad(z, ids, values, 50, 1.0, 2.0, targets, 0.5), want, 1.0)
+    z[1] = float("nan")
+    ids[1], targets[1] = -1, -1
+    loss, grad = F.distill_loss_grad(z, ids, values, 50, 1.0, 2.0, targets, 0.5)
+    assert loss[1] == 0 and grad[1].count_nonzero() == 0 and torch.isfinite(grad).all()
+
+
+def refusals(dev):
+    z, ids, values, targets = (t.to(dev) for t in data(4, 50, 56, 6))
+    ok = dict(vocab=50, scale=1.0)
+    for args, kw in (((z, ids.int(), values), {}), ((z, ids[:2], values), {}), ((z, ids, values.double()), {}), ((z, ids, values[:, :3]), {}),
+                     ((z, ids, values), dict(hard_weight=0.5)), ((z, ids, values), dict(hard_weight=1.5, targets=targets)),
+                     ((z, ids, values), dict(temperature=0.0)), ((z, ids, values), dict(temperature=float("inf"))),
+                     ((z, ids, values), dict(vocab=57)), ((z, ids, values), dict(vocab=0)), ((z, ids, values), dict(targets=targets.int())),
+                     ((z, ids, values), dict(targets=targets[:2])), ((z[0], ids, values), {}), ((z, ids, values), dict(out=z.float()))):
+        with pytest.raises(ValueError):
+            F.distill_loss_grad(*args, **{**ok, **kw})
+    with pytest.raises(ValueError):
+        F.distill_grad(z, ids, values, 0, 50, 1.0, torch.zeros(4, 3, device=dev))
+    with pytest.raises(ValueError):
+        F.distill_partial(z, ids, values, -8, 50)
+
+
+def test_refusals():
+    refusals("cpu")
+
+
+# ---------------------------------------------------------------------------------------------- on a GPU
+@pytest.mark.gpu
+@pytest.mark.parametrize("missing", [False, True])
+@pytest.mark.parametrize("T,w", SETTINGS)
+@pytest.mark.parametrize("size", SIZES + [(7, 5003, 5008, 128), (3, 30011, 30016, 64)])
+def test_kernel(size, T, w, missing):
+    run("cuda", size, T, w, missing)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kw", [dict(in_place=True), dict(values_dtype=torch.bfloat16), dict(use_targets=False)])
+def test_kernel_forms(kw):
+    for size in ((9, 1003, 1008, 20), (2, 110001, 110008, 5)):
+        for T, w in ((1.0, 0.0), (2.0, 0.0)) if "use_targets" in kw else ((1.0, 0.5), (3.0, 0.5)):
+            run("cuda", size, T, w, True, **kw)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,w", SETTINGS)
+def test_kernel_slices(T, w):
+    z, ids, values, targets = (t.cuda() for t in data(11, 2003, 2048, 37, True))
+    want = definition(*(t.cpu() for t in (z, ids, values, targets)), 2003, T, w)
+    check(slices(z, ids, values, targets, 2003, T, w, [0, 512, 1024, 2008, 2048], 0.5), want, 0.5)
+    check(slices(z, ids, values, targets, 2003, T, w, [0, 2048], 0.5), want, 0.5)
+
+
+@pytest.mark.gpu
+def test_kernel_many_entries_and_duplicates():
+    z, ids, values, targets = data(3, 3000, 3000, 1024)
+    ids[:, 900:] = ids[:, 100:224]
+    want = definition(z, ids, values, targets, 3000, 1.5, 0.2)
+    a = [t.cuda() for t in (z, ids, values, targets)]
+    got = F.distill_loss_grad(a[0], a[1], a[2], 3000, 1.0, 1.5, a[3], 0.2)
+    check(got, want, 1.0)
+    again = F.distill_loss_grad(a[0], a[1], a[2], 3000, 1.0, 1.5, a[3], 0.2)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.gpu
+def test_kernel_ignored_rows_infinities_and_nan():
+    """Rows that nothing is learnt from are zero; -inf logits have probability 0; a NaN shows in its own row alone."""
+    for vocab in (1000, 104000):
+        z, ids, values, targets = (t.cuda() for t in data(6, vocab, vocab, 6))
+        z[0] = float("nan")
+        ids[0], targets[0] = -1, -1
+        z[1, 100:] = -math.inf
+        ids[1], targets[1] = torch.arange(6, device="cuda"), 7
+        z[2, 5] = float("nan")
+        values[3, 2] = float("nan")
+        want = definition(*(t[[1, 4, 5]].cpu() for t in (z, ids, values, targets)), vocab, 2.0, 0.5)
+        loss, grad = F.distill_loss_grad(z, ids, values, vocab, 1.0, 2.0, targets, 0.5)
+        assert loss[0] == 0 and grad[0].count_nonzero() == 0
+        check((loss[[1, 4, 5]], grad[[1, 4, 5]]), want, 1.0)
+        assert grad[1, 100:].count_nonzero() == 0
+        assert loss[2].isnan() and loss[3].isnan() and grad[2].isnan().any() and grad[3].isnan().any()
+
+
+@pytest.mark.gpu
+def test_kernel_strides_and_alignment():
+    z, ids, values, targets = (t.cuda() for t in data(7, 203, 208, 9, True))
+    a = (203, 0.5, 2.0, targets, 0.5)
+    want = F.distill_loss_grad(z, ids, values, *a)
+    wide = torch.zeros(7, 240, dtype=torch.bfloat16, device="cuda")
+    for at in (0, 8, 3):
+        cut = wide[:, at:at + 208].copy_(z)
+        got = F.distill_loss_grad(cut, ids.T.contiguous().T, values.T.contiguous().T, *a)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        for to in (0, 16, 1):
+            out = torch.zeros(7, 250, dtype=torch.bfloat16, device="cuda")
+            got = F.distill_loss_grad(cut, ids, values, *a, out=out[:, to:to + 208])
+            assert torch.equal(got[1], want[1]) and torch.equal(out[:, to:to + 208], want[1])
+            assert out[:, :to].count_nonzero() == 0 and out[:, to + 208:].count_nonzero() == 0
+        got = F.distill_loss_grad(cut, ids, values, *a, out=cut)
+        assert torch.equal(cut, want[1])
+    block = torch.zeros(8, 208, dtype=torch.bfloat16, device="cuda")
+    block[:7].copy_(z)
+    assert torch.equal(F.distill_loss_grad(block[:7], ids, values, *a, out=block[1:])[1], want[1])
+    empty = F.distill_loss_grad(z[:0], ids[:0], values[:0], 203, 0.5, 2.0, targets[:0], 0.5)
+    assert empty[0].shape == (0,) and empty[1].shape == (0, 208)
+
+
+@pytest.mark.gpu
+def test_kernel_refusals():
+    refusals("cuda")
+    z, ids, values, _ = (t.cuda() for t in data(4, 50, 56, 6))
+    with pytest.raises(ValueError):
+        F.distill_loss_grad(z.float(), ids, values, 50, 1.0)
+    with pytest.raises(ValueError):
+        F.distill_loss_grad(z[:, :51], ids, values, 50, 1.0)
+    with pytest.raises(ValueError):
+        F.distill_loss_grad(z, ids.cpu(), values, 50, 1.0)
+    with pytest.raises(ValueError):
+        F.distill_loss_grad(z, ids.repeat(1, 200), values.repeat(1, 200), 50, 1.0)
