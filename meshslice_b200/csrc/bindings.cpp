@@ -21,6 +21,7 @@
 #include "ops/distill.h"
 #include "ops/ops.h"
 #include "ops/rotary.h"
+#include "ops/window_decode.h"
 
 namespace py = pybind11;
 using namespace msb;
@@ -548,6 +549,12 @@ void py_distill(int step, uint64_t logits, int64_t ld, uint64_t grad, int64_t ld
   check(step == 0 ? distill_row(a, S(stream)) : step == 1 ? distill_partial(a, S(stream)) : distill_grad(a, S(stream)), "distill");
 }
 
+void py_window_decode(uint64_t qkv, int64_t ld, uint64_t k, uint64_t v, uint64_t positions, uint64_t out, int batch, int kv, int group,
+                      int window, int sinks, float scale, uint64_t parts, uint64_t counters, int splits, uint64_t stream) {
+  check(window_decode({P<void>(qkv), ld, P<void>(k), P<void>(v), P<int64_t>(positions), P<void>(out), batch, kv, group, window, sinks,
+                       scale, P<float>(parts), P<uint32_t>(counters)}, splits, S(stream)), "window_decode");
+}
+
 void memset_zero(uint64_t ptr, size_t bytes, uint64_t stream) {
   check(cudaMemsetAsync(P<void>(ptr), 0, bytes,
                         reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream))),
@@ -629,6 +636,8 @@ PYBIND11_MODULE(_C, m) {
   m.attr("CE_ROW_COLS") = ce_row_cols();
   m.attr("DISTILL_ROW_COLS") = distill_row_cols();
   m.attr("DISTILL_TOP") = kDistillTop;
+  m.attr("WINDOW_DECODE_PART") = kWindowDecodePart;
+  m.def("window_decode_splits", &window_decode_splits, "splits of a sequence's slots: batch, kv, group, slots, SMs");
   m.def("ce_grid", &ce_grid, "CTAs of the cross-entropy kernels in a row exchange for a row count");
   m.def("cast_f32_to_bf16", [](uint64_t in, uint64_t out, int64_t n, int accumulate, uint64_t stream) {
     check(cast_f32_to_bf16(P<float>(in), P<void>(out), n, accumulate, S(stream)), "cast_f32_to_bf16");
@@ -696,6 +705,8 @@ PYBIND11_MODULE(_C, m) {
                  "stream"),
       MSB_DIRECT("distill", py_distill, "step, logits, ld, grad, ldg, ids, values, values_bf16, targets, rows, cols, col_offset, vocab, "
                  "top, temperature, hard, scale, loss, stats, stream"),
+      MSB_DIRECT("window_decode", py_window_decode, "qkv, ld, k, v, positions, out, batch, kv, group, window, sinks, scale, parts, "
+                 "counters, splits, stream"),
       {nullptr, nullptr, 0, nullptr}};
 #undef MSB_DIRECT
   if (PyModule_AddFunctions(m.ptr(), direct_calls) != 0) throw py::error_already_set();

@@ -1,0 +1,288 @@
+// Attention of single tokens over the ring cache of a windowed model.
+#include "window_decode.h"
+
+#include <cuda_bf16.h>
+
+#include "../common/pdl.cuh"
+#include "../common/ptx.cuh"
+
+namespace msb {
+
+namespace {
+
+constexpr int kD = 128;
+constexpr int kWarps = 4;
+constexpr int kKeys = 16;                          // slots of a tile: one warp's step
+constexpr int kTile = kKeys * kD * 2;              // 4 KiB, of K or of V
+constexpr int kStages = 3;
+constexpr int kHeads = 16;                         // query heads of a CTA: rows of a matrix fragment
+constexpr int kSmem = kWarps * kStages * 2 * kTile;
+constexpr int kPart = kWindowDecodePart;           // floats of a split: O, m, l
+static_assert(kPart == kHeads * (kD + 2), "what a split leaves");
+constexpr float kLog2e = 1.4426950408889634f;
+static_assert(kWarps * kHeads * (kD + 2) * 4 <= kSmem, "the warps' results take the place of the tiles");
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  // what is not there is filled with zeros: the cache may hold anything beyond the last position
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+__device__ __forceinline__ void load4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// c[16 x 8] += a[16 x 16] b[16 x 8]
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A CTA works on a run of slots of one (sequence, key/value head, 16 of its query heads); each warp on every fourth tile of 16
+// slots, with running maximum and sum of its own, through a ring that it fills itself (cp.async; no barrier).  The query heads
+// are the rows of the matrix fragments, so that all heads of a group share a pass over K and V.  mma.sync: a token's products are a
+// sixth of what that path does beside the memory, and the operands come as rows of any number and origin.
+// The token's own k and v are taken from `qkv` in place of their slot, which the CTA that has it writes.
+// Splits of a sequence are joined, in their order, by the CTA that finishes last.
+// kWide: more than 8 query heads (rows 8 to 15 of the fragments are in use).
+template <bool kWide>
+__global__ void __launch_bounds__(kWarps * 32)
+window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int per_split) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ uint32_t last;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int passes = (a.group + kHeads - 1) / kHeads;
+  const int split = blockIdx.x, h = blockIdx.y / passes, g0 = (blockIdx.y - h * passes) * kHeads, b = blockIdx.z;
+  const int heads = min(kHeads, a.group - g0), slots = a.sinks + a.window;
+  grid_trigger();
+  grid_wait();
+  const int64_t pos = a.positions[b];
+  const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(a.qkv) + b * a.ld + (int64_t)h * (a.group + 2) * kD;
+  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.out) + ((int64_t)(b * a.kv + h) * a.group + g0) * kD;
+  if (pos < 0) {
+    if (split == 0)
+      for (int i = threadIdx.x; i < heads * kD / 8; i += kWarps * 32) reinterpret_cast<uint4*>(out)[i] = make_uint4(0u, 0u, 0u, 0u);
+    return;
+  }
+  const int held = pos < slots ? (int)pos + 1 : slots;
+  const int own = pos < a.sinks ? (int)pos : a.sinks + (int)((pos - a.sinks) % a.window);
+  const int s0 = split * per_split, s1 = min(held, s0 + per_split);
+  if (s0 >= held) return;
+  const int64_t base = ((int64_t)b * a.kv + h) * slots * kD;
+  __nv_bfloat16 *ck = reinterpret_cast<__nv_bfloat16*>(a.k) + base, *cv = reinterpret_cast<__nv_bfloat16*>(a.v) + base;
+  const __nv_bfloat16 *nk = row + a.group * kD, *nv = nk + kD;
+  if (g0 == 0 && own >= s0 && own < s1 && threadIdx.x < 32) {
+    const int i = threadIdx.x & 15;
+    const uint4 u = reinterpret_cast<const uint4*>(threadIdx.x < 16 ? nk : nv)[i];
+    reinterpret_cast<uint4*>((threadIdx.x < 16 ? ck : cv) + (int64_t)own * kD)[i] = u;
+  }
+
+  const int tiles = (s1 - s0 + kKeys - 1) / kKeys;
+  const uint32_t ring = smem_u32(smem) + warp * kStages * 2 * kTile;
+  auto fetch = [&](int tile, int stage) {
+    if (tile < tiles) {
+      const uint32_t at = ring + stage * 2 * kTile;
+      // 16 lanes a row; chunk c of row r lies at c ^ (r % 8): fragments are read without conflicts
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 2 + (lane >> 4), c = lane & 15, slot = s0 + tile * kKeys + r;
+        const bool there = slot < s1;
+        const int64_t off = (int64_t)(there ? slot : s0) * kD + c * 8;
+        const uint32_t to = at + r * 256 + ((c ^ (r & 7)) << 4);
+        copy16(to, slot == own ? nk + c * 8 : ck + off, there);
+        copy16(to + kTile, slot == own ? nv + c * 8 : cv + off, there);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(warp + i * kWarps, i);
+  // query heads as A fragments: rows lane / 4 and + 8, columns 2 (lane % 4) and + 8 of each 16
+  uint32_t q[8][4];
+#pragma unroll
+  for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = (lane >> 2) + (i & 1) * 8, col = ks * 16 + (i >> 1) * 8 + (lane & 3) * 2;
+      q[ks][i] = (kWide || !(i & 1)) && r < heads ? *reinterpret_cast<const uint32_t*>(row + (g0 + r) * kD + col) : 0u;
+    }
+  float o[16][4] = {};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  const float sl2 = a.scale * kLog2e;
+  int stage = 0;
+  for (int tile = warp; tile < tiles; tile += kWarps) {
+    fetch(tile + (kStages - 1) * kWarps, stage == 0 ? kStages - 1 : stage - 1);
+    copy_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t at = ring + stage * 2 * kTile;
+    float s[2][4] = {};
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) {
+      uint32_t kb[4];
+      const int r = (lane & 7) + (lane >> 4) * 8, c = ks * 2 + ((lane >> 3) & 1);
+      load4(kb, at + r * 256 + ((c ^ (r & 7)) << 4));
+      mma(s[0], q[ks], kb[0], kb[1]);
+      mma(s[1], q[ks], kb[2], kb[3]);
+    }
+    // scores in the log2 domain; slots beyond the last one see nothing
+    const int left = s1 - s0 - tile * kKeys;
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = n * 8 + (lane & 3) * 2 + (i & 1);
+        s[n][i] = key < left ? s[n][i] * sl2 : -INFINITY;
+      }
+    float up[2];
+    bool grown = false;
+#pragma unroll
+    for (int r = 0; r < (kWide ? 2 : 1); ++r) {
+      float t = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
+      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
+      up[r] = fmaxf(m[r], t);                      // a tile has a slot in it: finite unless a score is not
+      grown |= up[r] > m[r];
+    }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int r = 0; r < (kWide ? 2 : 1); ++r) {
+        const float f = up[r] > m[r] ? exp2_ftz(m[r] - up[r]) : 1.f;
+        l[r] *= f;
+        m[r] = up[r];
+#pragma unroll
+        for (int n = 0; n < 16; ++n) {
+          o[n][2 * r] *= f;
+          o[n][2 * r + 1] *= f;
+        }
+      }
+    }
+    uint32_t p[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int r = 0; r < (kWide ? 2 : 1); ++r) {
+        const float x = exp2_ftz(s[n][2 * r] - m[r]), y = exp2_ftz(s[n][2 * r + 1] - m[r]);
+        l[r] += x + y;
+        p[n * 2 + r] = pack(x, y);
+      }
+#pragma unroll
+    for (int c = 0; c < 16; c += 2) {
+      uint32_t vb[4];
+      const int r = lane & 15, cc = c + (lane >> 4);
+      load4_trans(vb, at + kTile + r * 256 + ((cc ^ (r & 7)) << 4));
+      mma(o[c], p, vb[0], vb[1]);
+      mma(o[c + 1], p, vb[2], vb[3]);
+    }
+    __syncwarp();                                  // the stage has been read
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+  }
+  copy_wait<0>();
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+  }
+  // the warps' results: O [warp][head][128], m and l [warp][head]
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(smem);
+  float *sm = so + kWarps * kHeads * kD, *sl = sm + kWarps * kHeads;
+#pragma unroll
+  for (int r = 0; r < (kWide ? 2 : 1); ++r) {
+    const int head = (lane >> 2) + r * 8;
+    float* to = so + (warp * kHeads + head) * kD + (lane & 3) * 2;
+#pragma unroll
+    for (int n = 0; n < 16; ++n) *reinterpret_cast<float2*>(to + n * 8) = make_float2(o[n][2 * r], o[n][2 * r + 1]);
+    if ((lane & 3) == 0) {
+      sm[warp * kHeads + head] = m[r];
+      sl[warp * kHeads + head] = l[r];
+    }
+  }
+  __syncthreads();
+  const int live = (held + per_split - 1) / per_split;
+  const int64_t unit = ((int64_t)b * gridDim.y + blockIdx.y);
+  const int d = threadIdx.x;                       // one feature per thread
+  static_assert(kWarps * 32 == kD, "a thread per feature");
+  float* part = a.parts + (unit * splits + split) * kPart;
+  for (int head = 0; head < heads; ++head) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kHeads + head]);
+    float sum = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float mw = sm[w * kHeads + head], f = w < tiles ? exp2_ftz(mw - top) : 0.f;   // a warp without a tile has nothing
+      sum += f * sl[w * kHeads + head];
+      acc += f * so[(w * kHeads + head) * kD + d];
+    }
+    if (live == 1) {
+      out[head * kD + d] = __float2bfloat16(acc / sum);
+    } else {
+      part[head * kD + d] = acc;
+      if (d == 0) {
+        part[kHeads * kD + head] = top;
+        part[kHeads * kD + kHeads + head] = sum;
+      }
+    }
+  }
+  if (live == 1) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const uint32_t before = atomicAdd(a.counters + unit, 1u);
+    last = before + 1 == (uint32_t)live;
+    if (last) a.counters[unit] = 0;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  const float* parts = a.parts + unit * splits * kPart;
+  for (int head = 0; head < heads; ++head) {
+    float top = -INFINITY;
+    for (int s = 0; s < live; ++s) top = fmaxf(top, __ldcg(parts + s * kPart + kHeads * kD + head));
+    float sum = 0.f, acc = 0.f;
+    for (int s = 0; s < live; ++s) {
+      const float f = exp2_ftz(__ldcg(parts + s * kPart + kHeads * kD + head) - top);
+      sum += f * __ldcg(parts + s * kPart + kHeads * kD + kHeads + head);
+      acc += f * __ldcg(parts + s * kPart + head * kD + d);
+    }
+    out[head * kD + d] = __float2bfloat16(acc / sum);
+  }
+}
+
+}  // namespace
+
+int window_decode_splits(int batch, int kv, int group, int slots, int sms) {
+  const int64_t units = (int64_t)batch * kv * ((group + kHeads - 1) / kHeads);
+  const int64_t most = (slots + kWarps * kKeys - 1) / (kWarps * kKeys);        // a tile for every warp
+  const int64_t want = ((int64_t)sms * 4 + units - 1) / units;
+  return (int)(want < most ? want : most);
+}
+
+cudaError_t window_decode(const WindowDecodeArgs& a, int splits, cudaStream_t stream) {
+  const auto off = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) != 0; };
+  if (a.batch <= 0 || a.kv <= 0 || a.group <= 0 || a.window <= 0 || a.sinks < 0 || splits <= 0) return cudaErrorInvalidValue;
+  if (off(a.qkv) || off(a.k) || off(a.v) || off(a.out) || a.ld % 8) return cudaErrorInvalidValue;
+  const int64_t slots = (int64_t)a.sinks + a.window, rows = (int64_t)a.kv * ((a.group + kHeads - 1) / kHeads);
+  if (slots > 1 << 30 || rows > 65535 || a.batch > 65535) return cudaErrorInvalidValue;
+  const int steps = kWarps * kKeys, per = (int)((slots + splits - 1) / splits + steps - 1) / steps * steps;
+  auto kernel = a.group > 8 ? window_decode_kernel<true> : window_decode_kernel<false>;
+  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(kernel, dim3((unsigned)splits, (unsigned)rows, (unsigned)a.batch), kWarps * 32, kSmem, stream, a, splits, per);
+}
+
+}  // namespace msb

@@ -1,0 +1,117 @@
+"""Causal attention within a window that keeps the first tokens visible, on rows of grouped heads (per key/value head
+[q_0 | .. | q_group-1 | k | v]): query i sees key j <= i where i - j < window or j < sinks.  Native kernels for CUDA tensors, fp32
+formulation for CPU tensors."""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from .. import _native
+from . import rows
+
+HEAD_DIM = 128          # of the kernels
+
+
+def _width(qkv, kv_heads: int, group: int, batch_rows: Optional[int]) -> int:
+    """Features per head of ``qkv`` [batch_rows, kv_heads * (group + 2) * D]."""
+    if kv_heads < 1 or group < 1:
+        raise ValueError(f"attention needs kv_heads >= 1 and group >= 1 (got {kv_heads}, {group})")
+    per = kv_heads * (group + 2)
+    if qkv.dim() != 2 or qkv.shape[1] % per or qkv.shape[1] == 0 or (batch_rows is not None and qkv.shape[0] != batch_rows):
+        raise ValueError(f"attention needs rows [{'tokens' if batch_rows is None else batch_rows}, kv_heads * (group + 2) * head_dim] with "
+                         f"kv_heads * (group + 2) = {per} (got {tuple(qkv.shape)})")
+    return qkv.shape[1] // per
+
+
+# ----------------------------------------------------------------------------------------------
+# single tokens over a cache of fixed size
+# ----------------------------------------------------------------------------------------------
+class WindowCache:
+    """Keys and values [batch, kv_heads, sinks + window, head_dim] of what the next token of each sequence sees: position p lies in
+    slot p below ``sinks`` and in slot sinks + (p - sinks) % window from there on.  Whatever a slot holds before its first position
+    is stored is never used."""
+
+    def __init__(self, k, v, window: int, sinks: int = 0):
+        if window < 1 or sinks < 0:
+            raise ValueError(f"a cache needs window >= 1 and sinks >= 0 (got {window}, {sinks})")
+        if k.dim() != 4 or k.shape[2] != window + sinks or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
+            raise ValueError(f"keys and values must both be [batch, kv_heads, {window + sinks}, head_dim] (got {tuple(k.shape)} {k.dtype} "
+                             f"and {tuple(v.shape)} {v.dtype})")
+        if k.is_cuda:
+            if k.dtype != torch.bfloat16 or k.shape[3] != HEAD_DIM:
+                raise ValueError(f"the kernel needs a bf16 cache with head_dim {HEAD_DIM} (got {k.dtype}, {k.shape[3]})")
+            if not (k.is_contiguous() and v.is_contiguous()) or k.data_ptr() % 16 or v.data_ptr() % 16:
+                raise ValueError("the kernel needs contiguous caches on 16-byte boundaries")
+        self.k, self.v, self.window, self.sinks = k, v, window, sinks
+        self._work = {}
+
+    @classmethod
+    def new(cls, batch: int, kv_heads: int, window: int, sinks: int = 0, head_dim: int = HEAD_DIM, dtype=torch.bfloat16, device=None):
+        k, v = (torch.zeros(batch, kv_heads, sinks + window, head_dim, dtype=dtype, device=device) for _ in range(2))
+        return cls(k, v, window, sinks)
+
+    def slots(self, positions):
+        return torch.where(positions < self.sinks, positions, self.sinks + (positions - self.sinks) % self.window)
+
+    def fill(self, qkv, seq: int, group: int = 1):
+        """Keys and values of the first ``seq`` tokens of every sequence, as far as later tokens see them; ``qkv`` [batch * seq, ...]."""
+        batch, kv = self.k.shape[:2]
+        D = _width(qkv, kv, group, batch * seq)
+        if D != self.k.shape[3]:
+            raise ValueError(f"the cache holds {self.k.shape[3]} features per head, the rows {D}")
+        pos = torch.arange(seq, device=qkv.device)
+        pos = torch.cat([pos[: self.sinks], pos[max(self.sinks, seq - self.window):]])
+        x = qkv.reshape(batch, seq, kv, group + 2, D)[:, pos]
+        at = self.slots(pos)
+        self.k[:, :, at] = x[:, :, :, group].transpose(1, 2)
+        self.v[:, :, at] = x[:, :, :, group + 1].transpose(1, 2)
+
+    def workspace(self, group: int):
+        """(splits, partial results, counters) of the decoding kernel, laid out once."""
+        if group not in self._work:
+            batch, kv, slots = self.k.shape[:3]
+            C = _native.load()
+            sms = torch.cuda.get_device_properties(self.k.device).multi_processor_count
+            splits = C.window_decode_splits(batch, kv, group, slots, sms)
+            units = batch * kv * -(-group // 16)
+            parts = torch.empty(units * splits * C.WINDOW_DECODE_PART if splits > 1 else 0, dtype=torch.float32, device=self.k.device)
+            counters = torch.zeros(units, dtype=torch.int32, device=self.k.device)
+            self._work[group] = (splits, parts, counters)
+        return self._work[group]
+
+
+def window_attention_decode(qkv, cache: WindowCache, positions, group: int = 1):
+    """Attention of one token per sequence, ``qkv`` [batch, kv_heads * (group + 2) * D], at ``positions`` (int64 [batch]) over what
+    it sees, itself included.  Stores its key and value in the cache.  A negative position is an idle sequence: nothing is
+    stored, its output is zero.  Returns [batch, kv_heads * group * D]."""
+    batch, kv, slots, D = cache.k.shape
+    if _width(qkv, kv, group, batch) != D:
+        raise ValueError(f"the cache holds {D} features per head, the rows {qkv.shape[1] // (kv * (group + 2))}")
+    if positions.shape != (batch,) or positions.dtype != torch.int64 or positions.device != qkv.device:
+        raise ValueError(f"positions must be int64 [{batch}] beside the rows (got {positions.dtype} {tuple(positions.shape)} on "
+                         f"{positions.device})")
+    if qkv.dtype != cache.k.dtype or qkv.device != cache.k.device:
+        raise ValueError(f"rows are {qkv.dtype} on {qkv.device}, the cache {cache.k.dtype} on {cache.k.device}")
+    if qkv.is_cuda:
+        _native.check_device(qkv)
+        out = torch.empty(batch, kv * group * D, dtype=qkv.dtype, device=qkv.device)
+        if batch:
+            x, positions = rows.as_aligned(qkv), positions.contiguous()
+            splits, parts, counters = cache.workspace(group)
+            _native.load().window_decode(x.data_ptr(), rows.pitch(x), cache.k.data_ptr(), cache.v.data_ptr(), positions.data_ptr(),
+                                         out.data_ptr(), batch, kv, group, cache.window, cache.sinks, 1.0 / math.sqrt(D),
+                                         parts.data_ptr(), counters.data_ptr(), splits, _native.stream_ptr())
+        return out
+    x = qkv.view(batch, kv, group + 2, D)
+    out = torch.zeros(batch, kv, group, D, dtype=torch.float32)
+    for b, p in enumerate(positions.tolist()):
+        if p < 0:
+            continue
+        s = p if p < cache.sinks else cache.sinks + (p - cache.sinks) % cache.window
+        cache.k[b, :, s], cache.v[b, :, s] = x[b, :, group], x[b, :, group + 1]
+        held = min(p + 1, slots)
+        w = torch.softmax(x[b, :, :group].float() @ cache.k[b, :, :held].float().transpose(-1, -2) / math.sqrt(D), -1)
+        out[b] = w @ cache.v[b, :, :held].float()
+    return out.view(batch, -1).to(qkv.dtype)
