@@ -239,6 +239,11 @@ cudaError_t launch_sm100_gemm2(Gemm2Args& args, int problems, int tile_n, int sm
 int make_tensor_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                        uint64_t pitch_bytes, uint32_t box_inner, uint32_t box_outer, int swizzle_bytes = 128);
 
+// Tensor map of a contiguous bf16 [batch, seq, cols]: boxes of box_rows x box_cols (64: 128-byte swizzle, 32: 64-byte) end with their
+// sequence: rows beyond it are read as zeros and not written.
+int make_tensor_map_seq(CUtensorMap* map, const void* base, uint64_t cols, uint64_t seq, uint64_t batch, uint32_t box_cols,
+                        uint32_t box_rows);
+
 // Tensor map of an output matrix [rows, cols] with row pitch `ld` elements: boxes of 32 rows x 128 bytes, 128-byte
 // swizzle.  Returns non-zero where TMA cannot address it (base or pitch not a multiple of 16 bytes).
 int make_tensor_map_out(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, bool fp32);
