@@ -27,6 +27,7 @@ CU_SOURCES = [
     "ops/attention_noalloc.cu",
     "ops/rotary.cu",
     "ops/distill.cu",
+    "ops/window_attention.cu",
     "ops/window_decode.cu",
     "comm/p2p.cu",
 ]

@@ -21,6 +21,7 @@
 #include "ops/distill.h"
 #include "ops/ops.h"
 #include "ops/rotary.h"
+#include "ops/window_attention.h"
 #include "ops/window_decode.h"
 
 namespace py = pybind11;
@@ -555,6 +556,17 @@ void py_window_decode(uint64_t qkv, int64_t ld, uint64_t k, uint64_t v, uint64_t
                        scale, P<float>(parts), P<uint32_t>(counters)}, splits, S(stream)), "window_decode");
 }
 
+void py_window_attention_fwd(uint64_t qkv, uint64_t out, uint64_t lse, int batch, int seq, int kv, int group, int window, int sinks,
+                             float scale, uint64_t status, uint64_t stream) {
+  check(window_attention_fwd(P<void>(qkv), P<void>(out), P<float>(lse), {batch, seq, kv, group, window, sinks, scale},
+                             P<uint32_t>(status), S(stream)), "window_attention_fwd");
+}
+void py_window_attention_bwd(uint64_t qkv, uint64_t out, uint64_t dout, uint64_t lse, uint64_t dqkv, uint64_t scratch, int batch, int seq,
+                             int kv, int group, int window, int sinks, float scale, uint64_t status, uint64_t stream) {
+  check(window_attention_bwd(P<void>(qkv), P<void>(out), P<void>(dout), P<float>(lse), P<void>(dqkv), P<float>(scratch),
+                             {batch, seq, kv, group, window, sinks, scale}, P<uint32_t>(status), S(stream)), "window_attention_bwd");
+}
+
 void memset_zero(uint64_t ptr, size_t bytes, uint64_t stream) {
   check(cudaMemsetAsync(P<void>(ptr), 0, bytes,
                         reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream))),
@@ -637,6 +649,9 @@ PYBIND11_MODULE(_C, m) {
   m.attr("DISTILL_ROW_COLS") = distill_row_cols();
   m.attr("DISTILL_TOP") = kDistillTop;
   m.attr("WINDOW_DECODE_PART") = kWindowDecodePart;
+  m.def("window_attention_scratch", [](int batch, int seq, int kv, int group, int window, int sinks) {
+    return window_attention_scratch({batch, seq, kv, group, window, sinks, 1.f});
+  }, "fp32 values of the backward pass's scratch");
   m.def("window_decode_splits", &window_decode_splits, "splits of a sequence's slots: batch, kv, group, slots, SMs");
   m.def("ce_grid", &ce_grid, "CTAs of the cross-entropy kernels in a row exchange for a row count");
   m.def("cast_f32_to_bf16", [](uint64_t in, uint64_t out, int64_t n, int accumulate, uint64_t stream) {
@@ -707,6 +722,10 @@ PYBIND11_MODULE(_C, m) {
                  "top, temperature, hard, scale, loss, stats, stream"),
       MSB_DIRECT("window_decode", py_window_decode, "qkv, ld, k, v, positions, out, batch, kv, group, window, sinks, scale, parts, "
                  "counters, splits, stream"),
+      MSB_DIRECT("window_attention_fwd", py_window_attention_fwd, "qkv, out, lse, batch, seq, kv, group, window, sinks, scale, status, "
+                 "stream"),
+      MSB_DIRECT("window_attention_bwd", py_window_attention_bwd, "qkv, out, dout, lse, dqkv, scratch, batch, seq, kv, group, window, "
+                 "sinks, scale, status, stream"),
       {nullptr, nullptr, 0, nullptr}};
 #undef MSB_DIRECT
   if (PyModule_AddFunctions(m.ptr(), direct_calls) != 0) throw py::error_already_set();

@@ -1,0 +1,1198 @@
+// Window attention with first tokens that stay visible, forward and backward, on tcgen05: the kernels of attention.cu over lists of
+// key blocks instead of prefixes, for shared key/value heads and sequences that end inside a tile.
+//
+// A query block's list holds the blocks of the first tokens and those of its window; blocks between them are never loaded.  A key block
+// is streamed by the query blocks of its window, or by all later ones where it holds a first token, of every query head of its group:
+// shared heads add up in tensor memory.  Tensor maps end with their sequence (three dimensions), so rows beyond it are zeros when
+// read, and left alone when written.
+// All waits are bounded; a timeout records a code in `status` and the CTA leaves.
+#include "window_attention.h"
+
+#include <cuda_bf16.h>
+
+#include "../common/f32x2.cuh"
+#include "../common/pdl.cuh"
+#include "../common/ptx.cuh"
+#include "../gemm/sm100_gemm.h"  // make_tensor_map_seq
+#include "attention_tiles.cuh"
+
+namespace msb {
+
+namespace {
+
+constexpr uint32_t kErrWindow = 40;
+
+struct WinArgs {
+  int batch, seq, kv, group, heads;   // heads = kv * group
+  int window, sinks;                  // 1 <= window <= seq, 0 <= sinks <= seq
+  float scale;
+  float* lse;
+  int tiles_per_item;                 // query tiles that a CTA works on at a time (1 or 2)
+  uint32_t* status;
+  uint64_t timeout_ns;
+};
+
+// First columns of a query head and of a key head (values follow).
+template <class A>
+__device__ __forceinline__ int col_q(const A& a, int h) {
+  const int kv = h / a.group;
+  return (kv * (a.group + 2) + h - kv * a.group) * kD;
+}
+template <class A>
+__device__ __forceinline__ int col_k(const A& a, int kv) { return (kv * (a.group + 2) + a.group) * kD; }
+// First key block of query block i's window, blocks that hold first tokens.
+template <class A>
+__device__ __forceinline__ int window_block(const A& a, int i) { return max(0, i * kBlk - a.window + 1) / kBlk; }
+template <class A>
+__device__ __forceinline__ int sink_blocks(const A& a) { return (a.sinks + kBlk - 1) / kBlk; }
+
+// n low bits, for any n.
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
+
+__device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int b) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(col), "r"(row), "r"(b)
+      : "memory");
+}
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int b) {
+  load_half(dst, map, bar, col, row, b);
+  load_half(dst + kHalf, map, bar, col + 64, row, b);
+}
+// A warp's staged box on its way, if it begins inside the sequence: every lane's writes are visible to the copy engine before lane
+// 0 starts it.
+__device__ __forceinline__ void warp_store_box(const CUtensorMap* map, const void* stage, int col, int row, int b, int seq) {
+  fence_proxy_async_smem();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0 && row < seq) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(map), "r"(smem_u32(stage)), "r"(col), "r"(row), "r"(b) : "memory");
+    bulk_commit();
+  }
+}
+
+// ==========================================================================================
+// forward
+// ==========================================================================================
+// Roles and tensor memory as in attn_fwd2_kernel: producer, MMA issuer, a softmax warpgroup for each of two neighbouring query
+// tiles.  Both tiles walk one list of key blocks through the same K / V rings; each leaves out what it does not see.
+constexpr int kFwdWarpStage = 32 * 128;   // output staging per softmax warp: 32 rows x 64 columns
+constexpr size_t kFwdSmem = 6 * kTile + 8 * kFwdWarpStage + 256 + 1024;
+constexpr int kFwdThreads = 384;
+// registers per thread: 384 threads launch with 168; warps 0-3 give up what the softmax warps take
+constexpr int kFwdRegsLow = 96, kFwdRegsHigh = 200;
+static_assert(kFwdRegsLow + 2 * kFwdRegsHigh <= 3 * 168, "register shares exceed what the CTA is launched with");
+
+// One or two neighbouring tiles (tile 0 the later one, block hi) of a head, and the list of key blocks that either sees: `ns` blocks
+// with first tokens, then from `lo` to hi.  Tile 0 sees all but entry `skip` (the window of tile 1 begins a block earlier, or not),
+// tile 1 all but the last, which is tile 0's diagonal.
+struct FwdItem {
+  int b, h, hi, two, ns, lo, n, skip;
+  __device__ __forceinline__ int block(int x) const { return x < ns ? x : lo + x - ns; }
+  __device__ __forceinline__ bool uses(int t, int x) const { return t == 0 ? x != skip : two && x + 1 < n; }
+  __device__ __forceinline__ int first(int t) const { return t == 0 && skip == 0 ? 1 : 0; }
+  __device__ __forceinline__ int last(int t) const { return t == 0 ? n - 1 : n - 2; }
+  __device__ __forceinline__ int next(int t, int x) const { return t == 0 && x + 1 == skip ? x + 2 : x + 1; }
+};
+__device__ __forceinline__ FwdItem fwd_item(const WinArgs& a, uint32_t x, uint32_t y, uint32_t z, int group) {
+  FwdItem w;
+  const int bh = (int)z * group + (int)x, nblk = (a.seq + kBlk - 1) / kBlk;
+  w.b = bh / a.heads;
+  w.h = bh - w.b * a.heads;
+  w.hi = nblk - 1 - (int)y * a.tiles_per_item;
+  w.two = a.tiles_per_item == 2 && w.hi > 0 ? 1 : 0;
+  w.ns = min(sink_blocks(a), w.hi + 1);
+  const int lo0 = window_block(a, w.hi);
+  w.lo = max(w.ns, w.two ? window_block(a, w.hi - 1) : lo0);
+  w.n = w.ns + max(0, w.hi + 1 - w.lo);
+  w.skip = w.lo < lo0 ? w.ns : -1;
+  return w;
+}
+
+__global__ void __launch_bounds__(kFwdThreads, 1)
+window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_out,
+                 const __grid_constant__ WinArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  uint8_t* sQ = smem;                 // [2] tiles
+  uint8_t* sK = smem + 2 * kTile;     // [2] stages
+  uint8_t* sV = smem + 4 * kTile;     // [2] stages
+  uint8_t* sO = smem + 6 * kTile;     // [8] warps
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sO + 8 * kFwdWarpStage);
+  uint8_t* clc_resp = reinterpret_cast<uint8_t*>(bars);   // 16 bytes
+  uint64_t* clc_full = bars + 2;
+  uint64_t* clc_empty = bars + 3;
+  uint64_t* q_full = bars + 4;        // all [2] from here
+  uint64_t* q_empty = bars + 6;
+  uint64_t* k_full = bars + 8;
+  uint64_t* k_empty = bars + 10;
+  uint64_t* v_full = bars + 12;
+  uint64_t* v_empty = bars + 14;
+  uint64_t* s_full = bars + 16;
+  uint64_t* o_done = bars + 18;
+  uint64_t* p_ready = bars + 20;      // [2 * tile + part]: columns [0,96) / [96,128) of P
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint64_t tmo = a.timeout_ns;
+  const int group = gridDim.x;
+
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_qkv);
+    mbar_init(clc_full, 1);
+    mbar_init(clc_empty, 10);         // producer and MMA thread, 8 softmax warps
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(q_full + i, 1);
+      mbar_init(q_empty + i, 1);
+      mbar_init(k_full + i, 1);
+      mbar_init(k_empty + i, 1);
+      mbar_init(v_full + i, 1);
+      mbar_init(v_empty + i, 1);
+      mbar_init(s_full + i, 1);
+      mbar_init(o_done + i, 1);
+      mbar_init(p_ready + 2 * i, 128);
+      mbar_init(p_ready + 2 * i + 1, 128);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_trigger();
+  grid_wait();
+
+  // The next item as the producer got it: false when there is none (or on a timeout).
+  uint32_t clc_phase = 0;
+  auto next_item = [&](FwdItem& w) -> bool {
+    uint32_t x, y, z;
+    if (!mbar_wait(clc_full, clc_phase, 8 * tmo)) {
+      report(a.status, kErrWindow + 6, 0, 0);
+      return false;
+    }
+    clc_phase ^= 1;
+    const bool more = clc_read(clc_resp, x, y, z);
+    fence_proxy_async_smem();         // this read before the next response overwrites it
+    if (more) w = fwd_item(a, x, y, z, group);
+    return more;
+  };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFwdRegsLow));
+    FwdItem w = fwd_item(a, blockIdx.x, blockIdx.y, blockIdx.z, group);
+    if (warp == 0 && elect_one()) {
+      uint32_t c = 0;                 // K / V tiles loaded so far
+      uint32_t qc[2] = {0, 0};        // Q tiles loaded so far
+      bool ok = true, more = true;
+      while (ok && more) {
+        const int colq = col_q(a, w.h), colk = col_k(a, w.h / a.group);
+        for (int t = 0; t < 1 + w.two && ok; ++t) {
+          if (!(ok = mbar_wait(q_empty + t, (qc[t] & 1) ^ 1, 8 * tmo))) break;
+          ++qc[t];
+          mbar_expect_tx(q_full + t, kTile);
+          load_tile(sQ + t * kTile, &tm_qkv, q_full + t, colq, (w.hi - t) * kBlk, w.b);
+        }
+        for (int x = 0; x < w.n && ok; ++x, ++c) {
+          const uint32_t st = c & 1, ph = ((c >> 1) & 1) ^ 1;
+          const int krow = w.block(x) * kBlk;
+          if (!(ok = mbar_wait(k_empty + st, ph, 8 * tmo))) break;
+          mbar_expect_tx(k_full + st, kTile);
+          load_tile(sK + st * kTile, &tm_qkv, k_full + st, colk, krow, w.b);
+          if (!(ok = mbar_wait(v_empty + st, ph, 8 * tmo))) break;
+          mbar_expect_tx(v_full + st, kTile);
+          load_tile(sV + st * kTile, &tm_qkv, v_full + st, colk + kD, krow, w.b);
+        }
+        // Only now, with the item's last loads on their way, ask for the next item: a CTA that took one item ahead
+        // would hold it back from a CTA that is free sooner.
+        if (ok && (ok = mbar_wait(clc_empty, clc_phase ^ 1, 8 * tmo))) {
+          mbar_expect_tx(clc_full, 16);
+          clc_try_cancel(clc_resp, clc_full);
+          more = next_item(w);
+          mbar_arrive(clc_empty);
+        }
+        if (!ok) report(a.status, kErrWindow + 1, w.hi, c);
+      }
+    } else if (warp == 1 && elect_one()) {
+      const uint32_t idesc_s = make_idesc_bf16(128, 128, 0, 0);
+      const uint32_t idesc_pv = make_idesc_bf16(128, 128, 0, 1);
+      const uint64_t dq = desc_kmajor(smem_u32(sQ), 0), dk = desc_kmajor(smem_u32(sK), 0);
+      const uint64_t dv = desc_mnmajor(smem_u32(sV), 0);
+      constexpr uint64_t kTileOff = (uint64_t)(kTile >> 4);
+      uint32_t base = 0;              // K / V tiles of the items before this one
+      uint32_t qc[2] = {0, 0}, pc[2] = {0, 0};
+      bool ok = true, more = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code, uint32_t d) -> bool {
+        if (mbar_wait(bar, parity, 8 * tmo)) {
+          tc_fence_after_sync();
+          return true;
+        }
+        report(a.status, kErrWindow + code, d, base);
+        return false;
+      };
+      // Scores of tile t against entry x of the list.  The later tile that uses an entry gives its K back: tile 1 where both do (it
+      // leaves out none but the last, and its turn comes after tile 0's).
+      auto issue_s = [&](int t, int x) -> bool {
+        const uint32_t at = base + x;
+        if (!wait(k_full + (at & 1), (at >> 1) & 1, 3, t)) return false;
+        const uint64_t dqt = dq + t * kTileOff, dkt = dk + (at & 1) * kTileOff;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t off = (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4);
+          umma_f16(tmem + t * 128, dqt + off, dkt + off, idesc_s, k != 0);
+        }
+        umma_commit(s_full + t);
+        if (x == w.last(t)) umma_commit(q_empty + t);
+        if (t == 1 || !w.uses(1, x)) umma_commit(k_empty + (at & 1));
+        return true;
+      };
+      while (ok && more) {
+        for (int t = 0; t < 1 + w.two && ok; ++t) {
+          ok = wait(q_full + t, qc[t] & 1, 2, t);
+          ++qc[t];
+          if (ok) ok = issue_s(t, w.first(t));
+        }
+        for (int x = 0; x < w.n && ok; ++x) {
+          const uint32_t at = base + x;
+          if (!(ok = wait(v_full + (at & 1), (at >> 1) & 1, 4, 2))) break;
+          const uint64_t dvs = dv + (at & 1) * kTileOff;
+          for (int t = 0; t < 2; ++t) {
+            if (!w.uses(t, x)) continue;
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (ok) ok = wait(p_ready + 2 * t + half, pc[t] & 1, 4, t);
+              if (ok) {
+#pragma unroll
+                for (int k = half * 6; k < 6 + half * 2; ++k)   // 16 bf16 of a row of P = 8 TMEM columns per step
+                  umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, dvs + (uint64_t)((k * 2048) >> 4), idesc_pv,
+                              x != w.first(t) || k != 0);
+              }
+            }
+            if (!ok) break;
+            ++pc[t];
+            if (t == 1 || !w.uses(1, x)) umma_commit(v_empty + (at & 1));
+            if (x == w.last(t)) umma_commit(o_done + t);
+            else if (!(ok = issue_s(t, w.next(t, x)))) break;
+          }
+        }
+        if (ok) {
+          base += w.n;
+          more = next_item(w);
+          mbar_arrive(clc_empty);
+        }
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFwdRegsHigh));
+    // ---------------- softmax / output: one thread per query row ----------------
+    const int t = (warp >> 2) - 1;            // this warpgroup's tile
+    const int q4 = warp & 3;
+    const int row = q4 * 32 + lane;           // row inside the tile == TMEM lane
+    const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
+    const uint32_t ts = tmem + t * 128 + lane_off, to = tmem + 256 + t * 128 + lane_off;
+    const float sl2 = a.scale * kLog2e;
+    const uint64_t sl2x2 = f32x2(sl2, sl2);
+    uint8_t* stage = sO + (warp - 4) * kFwdWarpStage;
+    uint32_t sc = 0, oc = 0;                  // S tiles / outputs of this tile so far
+    bool ok = true, more = true;
+    FwdItem w = fwd_item(a, blockIdx.x, blockIdx.y, blockIdx.z, group);
+    while (more) {
+      const bool live = t == 0 || w.two;
+      const int i_blk = w.hi - t, query = i_blk * kBlk + row;
+      float m_used = -INFINITY, l = 0.f;
+      bool first = true;
+      for (int x = 0; x < w.n && live; ++x) {
+        if (!w.uses(t, x)) continue;
+        if (!warp_wait(s_full + t, sc & 1, 8 * tmo)) {
+          if (lane == 0) report(a.status, kErrWindow + 5, x, t);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        ++sc;
+        const int key0 = w.block(x) * kBlk;
+        // only blocks on the diagonal and on the window's edge, and far ones with first tokens, carry mask arithmetic
+        const bool masked = key0 == i_blk * kBlk || (i_blk * kBlk + kBlk - 1 - key0 >= a.window && key0 + kBlk > a.sinks);
+        uint32_t r[4][32];
+        float mc[4];
+        // the whole row with one wait: four loads in flight
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32(ts + c * 32, r[c]);
+        tmem_ld_wait();
+        if (masked) {
+          const int below = query - key0 + 1;                          // keys of this block up to the query
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t seen = low_bits(below - c * 32) & (~low_bits(below - a.window - c * 32) | low_bits(a.sinks - key0 - c * 32));
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!(seen >> i & 1)) r[c][i] = 0xff800000u;             // -inf
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float m0 = __uint_as_float(r[c][0]), m1 = __uint_as_float(r[c][1]);
+#pragma unroll
+          for (int i = 2; i + 3 < 32; i += 4) {
+            m0 = max3(m0, __uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1]));
+            m1 = max3(m1, __uint_as_float(r[c][i + 2]), __uint_as_float(r[c][i + 3]));
+          }
+          mc[c] = max3(fmaxf(m0, m1), __uint_as_float(r[c][30]), __uint_as_float(r[c][31]));
+        }
+        const float m_blk = fmaxf(fmaxf(mc[0], mc[1]), fmaxf(mc[2], mc[3])) * sl2;
+        if (first) {
+          first = false;
+          m_used = m_blk;
+        } else {
+          // these scores are complete, hence the P V before them is too: O may be rescaled in place
+          const float m_new = fmaxf(m_used, m_blk);
+          const bool need = (m_new - m_used) > 8.0f;
+          if (__any_sync(0xffffffffu, need)) {
+            const float alpha = need ? exp2f(m_used - m_new) : 1.0f;
+            if (need) {
+              l *= alpha;
+              m_used = m_new;
+            }
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t o[32];
+              tmem_ld_32x32(to + c * 32, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+              tmem_st_32x32(to + c * 32, o);
+            }
+          }
+        }
+        // (a row that has seen nothing yet: all its scores are -inf, and -inf - 0 gives the probability 0 that -inf + inf would not)
+        const float m_here = m_used == -INFINITY ? 0.f : m_used;
+        const uint64_t neg_m = f32x2(-m_here, -m_here);
+        uint64_t sum[4];
+        auto add_quarter = [&](int c) {
+          sum[c] = f32x2(__uint_as_float(r[c][0]), __uint_as_float(r[c][1]));
+#pragma unroll
+          for (int i = 2; i < 32; i += 2)
+            sum[c] = add2(sum[c], f32x2(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])));
+        };
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            float x0, x1;
+            split(fma2(f32x2(__uint_as_float(r[c][i]), __uint_as_float(r[c][i + 1])), sl2x2, neg_m), x0, x1);
+            x0 = fast_exp2(x0);
+            x1 = fast_exp2(x1);
+            r[c][i] = __float_as_uint(x0);
+            r[c][i + 1] = __float_as_uint(x1);
+            pk[i >> 1] = pack_bf16(x0, x1);
+          }
+          // P columns [32c, 32c+32) as bf16 = TMEM columns [16c, 16c+16): over S columns already read
+          tmem_st_32x16(ts + c * 16, pk);
+          if (c < 2) add_quarter(c);
+          if (c >= 2) {
+            tmem_st_wait();
+            tc_fence_before_sync();
+            mbar_arrive(p_ready + 2 * t + c - 2);
+          }
+        }
+        // the row's sum; its second half is off the chain that the products wait for
+        add_quarter(2);
+        add_quarter(3);
+        float s0, s1;
+        split(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), s0, s1);
+        l += s0 + s1;
+      }
+      if (ok && live) {
+        if (!warp_wait(o_done + t, oc & 1, 8 * tmo)) {
+          if (lane == 0) report(a.status, kErrWindow + 7, t, 0);
+          ok = false;
+        }
+        ++oc;
+      }
+      if (!ok) break;
+      if (live) {
+        tc_fence_after_sync();
+        const float inv = 1.0f / l;
+        // The warp's 32 rows leave through shared memory, 64 columns at a time, as TMA stores: nothing here waits for
+        // the memory system (with plain stores a warp stalls when all SMs write their items at the same time).
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          uint32_t o[2][32];
+          tmem_ld_32x32(to + half * 64, o[0]);
+          tmem_ld_32x32(to + half * 64 + 32, o[1]);
+          warp_stage_free();
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              uint4 u;
+              u.x = pack_bf16(__uint_as_float(o[c][q * 8 + 0]) * inv, __uint_as_float(o[c][q * 8 + 1]) * inv);
+              u.y = pack_bf16(__uint_as_float(o[c][q * 8 + 2]) * inv, __uint_as_float(o[c][q * 8 + 3]) * inv);
+              u.z = pack_bf16(__uint_as_float(o[c][q * 8 + 4]) * inv, __uint_as_float(o[c][q * 8 + 5]) * inv);
+              u.w = pack_bf16(__uint_as_float(o[c][q * 8 + 6]) * inv, __uint_as_float(o[c][q * 8 + 7]) * inv);
+              *reinterpret_cast<uint4*>(stage + lane * 128 + (((c * 4 + q) ^ (lane & 7)) << 4)) = u;   // 128-byte swizzle
+            }
+          warp_store_box(&tm_out, stage, w.h * kD + half * 64, i_blk * kBlk + q4 * 32, w.b, a.seq);
+        }
+        if (query < a.seq) a.lse[((int64_t)w.b * a.heads + w.h) * a.seq + query] = m_used * kLn2 + logf(l);
+      }
+      more = next_item(w);
+      __syncwarp();                              // every lane has read the response
+      if (lane == 0) mbar_arrive(clc_empty);
+    }
+    if (lane == 0) bulk_wait_all<0>();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// ==========================================================================================
+// backward
+// ==========================================================================================
+// delta[b, h, s] = -rowsum(dO * O) * scale and lse2[b, h, s] = -lse * log2(e), of sequences padded to whole tiles: rows beyond the end
+// get 0 and -inf, so that their probabilities are 0.  16 lanes with a 16-byte vector each take one head of kDeltaRows tokens.
+constexpr int kDeltaRows = 4;
+__global__ void __launch_bounds__(256)
+window_delta_kernel(const uint4* out, const uint4* dout, float* delta, uint32_t groups, uint32_t seq, uint32_t padded,
+                    uint32_t heads, const float* lse, float* lse2, float scale) {
+  grid_wait();
+  grid_trigger();
+  const uint32_t sub = threadIdx.x & 15;
+  const uint32_t w = blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4);   // (sequence, group of tokens, head)
+  const uint32_t tg = w / heads, h = w - tg * heads, per = padded / kDeltaRows, b = tg / per, s0 = (tg - b * per) * kDeltaRows;
+  uint4 o[kDeltaRows], d[kDeltaRows];
+#pragma unroll
+  for (int i = 0; i < kDeltaRows; ++i) {
+    o[i] = d[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (w < groups && s0 + i < seq) {
+      const int64_t at = (((int64_t)b * seq + s0 + i) * heads + h) * 16 + sub;
+      o[i] = ld_stream(out + at);
+      d[i] = ld_stream(dout + at);
+    }
+  }
+  float mine = 0.f;                      // the sum of row `sub`
+#pragma unroll
+  for (int i = 0; i < kDeltaRows; ++i) {
+    const uint32_t ov[4] = {o[i].x, o[i].y, o[i].z, o[i].w}, dv[4] = {d[i].x, d[i].y, d[i].z, d[i].w};
+    float s = 0.f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      s += __uint_as_float(ov[k] << 16) * __uint_as_float(dv[k] << 16) +
+           __uint_as_float(ov[k] & 0xffff0000u) * __uint_as_float(dv[k] & 0xffff0000u);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+    if (sub == i) mine = s;
+  }
+  if (w < groups && sub < kDeltaRows) {
+    const int64_t row = (int64_t)b * heads + h;
+    const uint32_t s = s0 + sub;
+    delta[row * padded + s] = -mine * scale;
+    lse2[row * padded + s] = s < seq ? -lse[row * seq + s] * kLog2e : -INFINITY;
+  }
+}
+
+// Key-major items accumulate dV and dK of 128 keys over the query blocks that see them, of every head of the group; query-major
+// items dQ of 128 queries over their list of key blocks.  Roles, rings and tensor memory as in attn_bwd2_kernel.
+constexpr int kBwdWarps = 16;               // element-wise warps
+constexpr int kBwdCols = kBlk * 4 / kBwdWarps;   // columns of a row per element-wise thread
+constexpr int kBwdStage = 32 * kBwdCols * 2;     // output staging per element-wise warp
+constexpr int kStatBytes = kBlk * 4;        // lse2 or delta of 128 queries
+constexpr int kBwdAlignSlack = 256;
+constexpr size_t kBwdBars = 7 * kTile + 5 * kStatBytes;   // where the barriers are
+constexpr size_t kBwdSmem = kBwdBars + 256 + kBwdAlignSlack;
+static_assert(kBwdWarps * kBwdStage == kTile, "an item's staged output takes the place of a tile");
+static_assert(kBwdSmem <= 232448, "shared memory of a CTA");
+constexpr int kBwdThreads = 96 + 32 * kBwdWarps;
+
+struct WinBwdArgs {
+  const float* lse2;    // -lse * log2(e)          (written by window_delta_kernel)
+  const float* delta;   // -rowsum(dO * O) * scale (written by window_delta_kernel)
+  uint32_t items;       // item i < items is key-major, items + i query-major
+  int key_group, query_group;   // rows of items (sequence, head) that are dealt together
+  int batch, seq, kv, group, heads, window, sinks;
+  float scale;
+  uint32_t* status;
+  uint64_t timeout_ns;
+};
+__device__ __forceinline__ int64_t stat_at(const WinBwdArgs& a, int b, int h, int blk) {
+  const int nblk = (a.seq + kBlk - 1) / kBlk;
+  return (((int64_t)b * a.heads + h) * nblk + blk) * kBlk;
+}
+
+struct Streamed {
+  int h, blk;           // query head and block of a streamed tile
+};
+struct BwdItem {
+  int b, h, blk, n_it;  // sequence, key head (key-major) or query head, owned block, streamed blocks
+  int i0, per;          // key-major: first query block, query blocks of a head; query-major: blocks with first tokens, first of the window
+  template <bool kKeyMajor>
+  __device__ __forceinline__ Streamed streamed(const WinBwdArgs& a, int it) const {
+    Streamed s;
+    if (kKeyMajor) {
+      const int m = it / per;
+      s.h = h * a.group + m;
+      s.blk = i0 + it - m * per;
+    } else {
+      s.h = h;
+      s.blk = it < i0 ? it : per + it - i0;
+    }
+    return s;
+  }
+};
+template <bool kKeyMajor>
+__device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) {
+  BwdItem w;
+  const int nblk = (a.seq + kBlk - 1) / kBlk, group = kKeyMajor ? a.key_group : a.query_group, heads = kKeyMajor ? a.kv : a.heads;
+  const uint32_t i = kKeyMajor ? item : item - a.items, row = i / (uint32_t)group;
+  const int bh = (int)(row / (uint32_t)nblk) * group + (int)(i - row * (uint32_t)group), y = (int)(row % (uint32_t)nblk);
+  w.b = bh / heads;
+  w.h = bh - w.b * heads;
+  // the longest items of a group first: key block 0, the last query block
+  w.blk = kKeyMajor ? y : nblk - 1 - y;
+  if (kKeyMajor) {
+    const int last = w.blk * kBlk < a.sinks ? nblk - 1 : min(nblk - 1, (w.blk * kBlk + kBlk - 1 + a.window - 1) / kBlk);
+    w.i0 = w.blk;
+    w.per = last - w.blk + 1;
+    w.n_it = w.per * a.group;
+  } else {
+    w.i0 = min(sink_blocks(a), w.blk + 1);
+    w.per = max(w.i0, window_block(a, w.blk));
+    w.n_it = w.i0 + max(0, w.blk + 1 - w.per);
+  }
+  return w;
+}
+
+// A CTA's run of items of one kind, from `item` on, until cluster launch control has none left or one of the other kind (the
+// response stays in shared memory).  False after a timeout.  At its end every copy and every tcgen05 operation has arrived
+// where it was announced, so the barriers can be set up anew for the next run.
+// kKeyMajor = true:  resident tiles K, V (this item's 128 keys), streamed Q, dO; accumulators dV, dK.
+//                    TMEM lanes = keys, columns = queries: lse / delta vary along the columns.
+// kKeyMajor = false: resident tiles Q, dO (this item's 128 queries), streamed K, V; accumulator dQ.
+//                    TMEM lanes = queries, columns = keys: lse / delta are per thread.
+template <bool kKeyMajor>
+__device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const CUtensorMap& tm_dqkv,
+                                              const WinBwdArgs& a, uint8_t* smem, uint32_t tmem, uint32_t item) {
+  uint8_t* sR0 = smem;                      // resident: K (key-major) or Q
+  uint8_t* sR1 = smem + kTile;              // resident: V (key-major) or dO
+  // Streamed tiles, a ring each.  Q / K is read by the first and the last product of a block, dO (key-major) by the
+  // second and third, V (query-major) by the second alone.
+  constexpr uint32_t kRing0 = 3, kRing1 = 2;
+  uint8_t* sS0 = smem + 2 * kTile;          // Q or K
+  uint8_t* sS1 = smem + 5 * kTile;          // dO or V; between items the stage of an item's last block takes its output
+  // key-major: lse2 travels with Q, delta with dO.  delta(i+2) takes the slot of delta(i): its producer waits for dS(i).
+  float* sLse = reinterpret_cast<float*>(smem + 7 * kTile);   // [3][128]
+  float* sDelta = sLse + 3 * kBlk;                            // [2][128]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBwdBars);   // up to 30: the tensor-memory address is behind them
+  uint8_t* clc_resp = reinterpret_cast<uint8_t*>(bars);   // 16 bytes
+  uint64_t* clc_full = bars + 2;
+  uint64_t* clc_empty = bars + 3;
+  uint64_t* res_full = bars + 4;            // [2] resident tiles: the one that S reads, the one that dP reads
+  uint64_t* res_empty = bars + 6;           // [2]
+  uint64_t* full0 = bars + 8;               // [3] rings
+  uint64_t* empty0 = bars + 11;             // [3]
+  uint64_t* full1 = bars + 14;              // [2]
+  uint64_t* empty1 = bars + 16;             // [2]
+  uint64_t* s_full = bars + 18;
+  uint64_t* s_free = bars + 19;             // query-major: S is in registers
+  uint64_t* dp_full = bars + 20;            // [2] (key-major uses [0] only)
+  uint64_t* ds_ready = bars + 22;           // [2] dS is in TMEM, even and odd blocks
+  uint64_t* p_ready = bars + 24;            // [2] key-major: the first / second 16 columns of every warp's P^T
+  uint64_t* acc_done = bars + 26;           // [2] key-major: dV / dK; query-major: [1] dQ
+  uint64_t* out_read = bars + 28;           // [2] the copy engine has read the output staged in a stage of ring 1
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint64_t tmo = a.timeout_ns;
+
+  if (threadIdx.x == 0) {
+    mbar_init(clc_full, 1);
+    mbar_init(clc_empty, 3 + kBwdWarps);    // producers and MMA thread, element-wise warps
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(full0 + i, 1);
+      mbar_init(empty0 + i, 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, kBwdWarps);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(res_full + i, 1);
+      mbar_init(res_empty + i, 1);
+      mbar_init(full1 + i, 1);
+      mbar_init(empty1 + i, 1);
+      mbar_init(dp_full + i, 1);
+      mbar_init(ds_ready + i, kBwdWarps);
+      mbar_init(p_ready + i, kBwdWarps);
+      mbar_init(acc_done + i, 1);
+      mbar_init(out_read + i, kBwdWarps);
+    }
+    mbar_fence_init();
+  }
+  __syncthreads();
+  // key-major:   S^T [0,128)  dP^T [128,256)  dV [256,384)  dK [384,512)
+  // query-major: S [0,128)  dP buffers [128,256) [256,384)  dQ [384,512)
+  const uint32_t t_dp = tmem + 128;
+  const auto dp_buf = [](uint32_t q) -> uint32_t { return kKeyMajor ? 0 : q & 1; };         // of streamed block q
+  const auto dp_phase = [](uint32_t q) -> uint32_t { return (kKeyMajor ? q : q >> 1) & 1; };
+  const uint32_t t_acc0 = tmem + (kKeyMajor ? 256 : 384), t_acc1 = tmem + 384;
+
+  BwdItem w = bwd_item<kKeyMajor>(a, item);
+  bool ok = true;
+  // The next item as the producer got it: false when there is none of this kind (or on a timeout).
+  uint32_t items = 0;                       // items finished by this thread
+  auto next_item = [&]() -> bool {
+    uint32_t x, y, z;
+    if (!mbar_wait(clc_full, items & 1, 8 * tmo)) {
+      report(a.status, kErrWindow + 18, items, 0);
+      ok = false;
+      return false;
+    }
+    ++items;
+    const bool more = clc_read(clc_resp, x, y, z) && (x < a.items) == kKeyMajor;
+    fence_proxy_async_smem();               // this read before the next response overwrites it
+    if (more) w = bwd_item<kKeyMajor>(a, x);
+    return more;
+  };
+  uint32_t g = 0;                           // streamed blocks so far: stages and phases of the rings and the hand-overs
+
+  if (warp == 0) {
+    // resident tile of S, ring of Q or K, next items
+    if (elect_one()) {
+      bool more = true;
+      while (ok && more) {
+        // the resident tile of S first, then the item's first streamed tile: S needs no more
+        for (int it = -1; it < w.n_it && ok; ++it) {
+          if (it < 0) {
+            if (!(ok = mbar_wait(res_empty, (items & 1) ^ 1, 8 * tmo))) break;
+            mbar_expect_tx(res_full, kTile);
+            load_tile(sR0, &tm_qkv, res_full, kKeyMajor ? col_k(a, w.h) : col_q(a, w.h), w.blk * kBlk, w.b);           // K or Q
+            continue;
+          }
+          const uint32_t st = g % kRing0;
+          const Streamed s = w.template streamed<kKeyMajor>(a, it);
+          if (!(ok = mbar_wait(empty0 + st, ((g / kRing0) & 1) ^ 1, 8 * tmo))) break;
+          mbar_expect_tx(full0 + st, kTile + (kKeyMajor ? kStatBytes : 0));
+          load_tile(sS0 + st * kTile, &tm_qkv, full0 + st, kKeyMajor ? col_q(a, s.h) : col_k(a, s.h / a.group), s.blk * kBlk, w.b);
+          if (kKeyMajor) bulk_g2s(sLse + st * kBlk, a.lse2 + stat_at(a, w.b, s.h, s.blk), kStatBytes, full0 + st);
+          ++g;
+        }
+        if (ok && (ok = mbar_wait(clc_empty, (items & 1) ^ 1, 8 * tmo))) {
+          mbar_expect_tx(clc_full, 16);
+          clc_try_cancel(clc_resp, clc_full);
+          more = next_item();
+          mbar_arrive(clc_empty);
+        }
+      }
+      // what is still under way (a timeout above is reported here too)
+      for (uint32_t q = g; q < g + kRing0 && ok; ++q) ok = mbar_wait(empty0 + q % kRing0, ((q / kRing0) & 1) ^ 1, 8 * tmo);
+      ok = ok && mbar_wait(res_empty, (items & 1) ^ 1, 8 * tmo);
+      if (!ok) report(a.status, kErrWindow + 11, w.blk, g);
+    }
+  } else if (warp == 2 + kBwdWarps) {
+    // resident tile of dP, ring of dO or V: by a thread of its own, because a stage of one ring is often free long before one of the other
+    if (elect_one()) {
+      bool more = true;
+      uint32_t outs[2] = {0, 0};              // outputs staged in either stage so far
+      bool staged[2] = {false, false};        // the last user of the stage was an item's output
+      while (ok && more) {
+        if ((ok = mbar_wait(res_empty + 1, (items & 1) ^ 1, 8 * tmo))) {
+          mbar_expect_tx(res_full + 1, kTile);
+          if (kKeyMajor) load_tile(sR1, &tm_qkv, res_full + 1, col_k(a, w.h) + kD, w.blk * kBlk, w.b);     // V
+          else load_tile(sR1, &tm_do, res_full + 1, w.h * kD, w.blk * kBlk, w.b);                            // dO
+        }
+        for (int it = 0; it < w.n_it && ok; ++it, ++g) {
+          const uint32_t st = g % kRing1;
+          const Streamed s = w.template streamed<kKeyMajor>(a, it);
+          if (!(ok = mbar_wait(empty1 + st, ((g / kRing1) & 1) ^ 1, 8 * tmo))) break;
+          if (staged[st] && !(ok = mbar_wait(out_read + st, (outs[st] - 1) & 1, 8 * tmo))) break;
+          staged[st] = false;
+          mbar_expect_tx(full1 + st, kTile + (kKeyMajor ? kStatBytes : 0));
+          if (kKeyMajor) {
+            load_tile(sS1 + st * kTile, &tm_do, full1 + st, s.h * kD, s.blk * kBlk, w.b);                                // dO
+            if (g > 1 && !(ok = mbar_wait(ds_ready + st, ((g - 2) >> 1) & 1, 8 * tmo))) break;
+            bulk_g2s(sDelta + st * kBlk, a.delta + stat_at(a, w.b, s.h, s.blk), kStatBytes, full1 + st);
+          } else {
+            load_tile(sS1 + st * kTile, &tm_qkv, full1 + st, col_k(a, s.h / a.group) + kD, s.blk * kBlk, w.b);                  // V
+          }
+        }
+        if (ok) {
+          const uint32_t st = (g - 1) % kRing1;
+          staged[st] = true;
+          ++outs[st];
+        }
+        if (ok) {
+          more = next_item();
+          mbar_arrive(clc_empty);
+        }
+      }
+      for (uint32_t q = g; q < g + kRing1 && ok; ++q) ok = mbar_wait(empty1 + q % kRing1, ((q / kRing1) & 1) ^ 1, 8 * tmo);
+      ok = ok && mbar_wait(res_empty + 1, (items & 1) ^ 1, 8 * tmo);
+      if (!ok) report(a.status, kErrWindow + 11, w.blk, g);
+    }
+  } else if (warp == 1) {
+    if (elect_one()) {
+      const uint32_t id_s = make_idesc_bf16(128, 128, 0, 0);      // A K-major (smem) * B K-major
+      const uint32_t id_g = make_idesc_bf16(128, 128, 0, 1);      // A (TMEM) * B MN-major
+      // descriptors of the first k-step of each operand; the others are these plus constants
+      const uint64_t dr0 = desc_kmajor(smem_u32(sR0), 0), dr1 = desc_kmajor(smem_u32(sR1), 0);
+      const uint64_t ds0k = desc_kmajor(smem_u32(sS0), 0), ds1k = desc_kmajor(smem_u32(sS1), 0);
+      const uint64_t ds0m = desc_mnmajor(smem_u32(sS0), 0), ds1m = desc_mnmajor(smem_u32(sS1), 0);
+      constexpr uint64_t kStageOff = (uint64_t)(kTile >> 4);
+      bool more = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, uint32_t code) -> bool {
+        if (mbar_wait(bar, parity, 8 * tmo)) {
+          tc_fence_after_sync();
+          return true;
+        }
+        report(a.status, kErrWindow + code, g, items);
+        return false;
+      };
+      // S (or S^T) / dP (or dP^T) of streamed block number q, once its tile is there and the block before is out of S (key-major:
+      // the products that read its P^T were issued before)
+      auto issue_s = [&](uint32_t q) -> bool {
+        const uint32_t st = q % kRing0;
+        if (!kKeyMajor && q > 0 && !wait(s_free, (q - 1) & 1, 19)) return false;
+        if (!wait(full0 + st, (q / kRing0) & 1, 13)) return false;
+        const uint64_t tile = ds0k + st * kStageOff;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t off = (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4);
+          umma_f16(tmem, dr0 + off, tile + off, id_s, k != 0);
+        }
+        umma_commit(s_full);
+        return true;
+      };
+      auto issue_dp = [&](uint32_t q) -> bool {
+        const uint32_t st = q % kRing1;
+        if (!wait(full1 + st, (q / kRing1) & 1, 13)) return false;
+        const uint64_t tile = ds1k + st * kStageOff;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const uint64_t off = (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4);
+          umma_f16(t_dp + dp_buf(q) * 128, dr1 + off, tile + off, id_s, k != 0);
+        }
+        umma_commit(dp_full + dp_buf(q));
+        if (!kKeyMajor) umma_commit(empty1 + st);         // V has no other reader
+        return true;
+      };
+      // The first blocks of an item also wait for its resident tiles.  An item's last products of either kind free them.
+      auto first_s = [&](uint32_t q) -> bool {
+        if (!(wait(res_full, items & 1, 12) && issue_s(q))) return false;
+        if (w.n_it == 1) umma_commit(res_empty);
+        return true;
+      };
+      auto first_dp = [&](uint32_t q) -> bool {
+        if (!(wait(res_full + 1, items & 1, 12) && issue_dp(q))) return false;
+        if (w.n_it == 1) umma_commit(res_empty + 1);
+        return true;
+      };
+      // acc += (P or dS in TMEM at `src`: a warp's columns packed from its first column) * streamed tile; the k-steps
+      // of the first / second 16 columns of every warp
+      auto issue_grad = [&](uint32_t acc, uint32_t src, uint64_t tile, int part, bool first) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          umma_f16_ts(acc, src + i * kBwdCols + part * 8, tile + (uint64_t)(((2 * i + part) * 2048) >> 4), id_g,
+                      !(first && i == 0));
+      };
+      // Blocks follow one another across items: the next item's first S is issued where the next block's would be, and its
+      // first dP behind this item's last product.
+      ok = first_s(g) && first_dp(g);
+      while (ok && more) {
+        const int n = w.n_it;
+        for (int it = 0; it < n && ok; ++it, ++g) {
+          const bool last = it + 1 == n;
+          const uint32_t st0 = g % kRing0, st1 = g % kRing1;
+          if (kKeyMajor) {
+            // dV += P^T dO (contraction over the queries)
+            if (!(ok = wait(p_ready, g & 1, 14))) break;
+            issue_grad(t_acc0, tmem, ds1m + st1 * kStageOff, 0, it == 0);
+            if (!(ok = wait(p_ready + 1, g & 1, 14))) break;
+            issue_grad(t_acc0, tmem, ds1m + st1 * kStageOff, 1, false);
+            umma_commit(empty1 + st1);
+            if (last) umma_commit(acc_done);
+          }
+          if (!last) {
+            if (!(ok = issue_s(g + 1))) break;
+            if (it + 2 == n) umma_commit(res_empty);
+            if (!kKeyMajor) {
+              if (!(ok = issue_dp(g + 1))) break;
+              if (it + 2 == n) umma_commit(res_empty + 1);
+            }
+          } else {
+            more = next_item();                           // w is the next item's from here on
+            mbar_arrive(clc_empty);
+            if (more && !(ok = first_s(g + 1))) break;
+          }
+          if (!(ok = wait(ds_ready + (g & 1), (g >> 1) & 1, 14))) break;
+          const uint32_t acc = kKeyMajor ? t_acc1 : t_acc0, ds = t_dp + dp_buf(g) * 128;
+          issue_grad(acc, ds, ds0m + st0 * kStageOff, 0, it == 0);     // dK += dS^T Q / dQ += dS K
+          issue_grad(acc, ds, ds0m + st0 * kStageOff, 1, false);
+          umma_commit(empty0 + st0);
+          if (last) umma_commit(acc_done + 1);
+          if (last) {
+            if (more && !(ok = first_dp(g + 1))) break;
+          } else if (kKeyMajor) {
+            if (!(ok = issue_dp(g + 1))) break;
+            if (it + 2 == n) umma_commit(res_empty + 1);
+          }
+        }
+      }
+    }
+  } else {
+    const int q4 = warp & 3;
+    const int part = (warp - 2) >> 2;                     // which kBwdCols of the 128 columns
+    const int row = q4 * 32 + lane;                       // TMEM lane: key (key-major) or query
+    const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
+    const uint64_t sl2 = f32x2(a.scale * kLog2e, a.scale * kLog2e), sc2 = f32x2(a.scale, a.scale);
+    bool more = true;
+    while (more) {
+      const int me = w.blk * kBlk + row;                  // query-major: this lane's query
+      const int me0 = w.blk * kBlk + q4 * 32 + (lane >> 2);   // key-major: the first of this thread's keys
+      uint64_t my_lse2 = 0, my_delta = 0;
+      if (!kKeyMajor) {
+        const int64_t at = stat_at(a, w.b, w.h, w.blk) + row;
+        my_lse2 = f32x2(a.lse2[at], a.lse2[at]);
+        my_delta = f32x2(a.delta[at], a.delta[at]);
+      }
+      for (int it = 0; it < w.n_it; ++it, ++g) {
+        const uint32_t ts = tmem + lane_off + part * kBwdCols, tdp = ts + 128 + dp_buf(g) * 128;
+        const int c0 = w.template streamed<kKeyMajor>(a, it).blk * kBlk + part * kBwdCols;   // first streamed index of this thread's columns
+        const uint32_t st0 = g % kRing0;
+        // key-major: lse2 / delta of this thread's columns
+        const float* my_lse = sLse + st0 * kBlk + part * kBwdCols + (lane & 3) * 2;
+        const float* my_dlt = sDelta + (g & 1) * kBlk + part * kBwdCols + (lane & 3) * 2;
+        // only pairs on the diagonal or the window's edge, and far ones with first tokens among the keys, pay for the mask
+        const bool masked = kKeyMajor ? c0 < me0 + 24 || (c0 + kBwdCols - 1 - me0 >= a.window && me0 + 24 >= a.sinks)
+                                      : c0 + kBwdCols - 1 > me || (me - c0 >= a.window && c0 + kBwdCols > a.sinks);
+        float e[kBwdCols];                                // P of this thread's columns
+        // ---- phase 1: P = exp2(S * scale * log2(e) - lse2) ----
+        // (key-major: lse2 comes with Q and delta with dO, whose barriers order them for this thread)
+        if (!warp_wait(s_full, g & 1, 8 * tmo) || (kKeyMajor && !warp_wait(full0 + st0, (g / kRing0) & 1, 8 * tmo))) {
+          if (lane == 0) report(a.status, kErrWindow + 15, it, 0);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        {
+          uint32_t rs[kBwdCols];
+          if (kKeyMajor) {
+            tmem_ld_16x32_frag(ts, rs);
+            tmem_ld_16x32_frag(ts + (16u << 16), rs + 16);
+          } else {
+            tmem_ld_32x32(ts, rs);
+          }
+          tmem_ld_wait();
+          if (!kKeyMajor) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(s_free);           // the next block's S may be computed
+          }
+          uint64_t st[4] = {my_lse2, my_lse2, my_lse2, my_lse2};
+          if (kKeyMajor) {
+#pragma unroll
+            for (int n = 0; n < 4; ++n) st[n] = *reinterpret_cast<const uint64_t*>(my_lse + n * 8);
+          }
+          // key-major: columns of a fragment are in groups n of 8, elements 4 n + {0, 1} of this thread's first row of a
+          // lane half, + {2, 3} of its second; by halves of 16 columns, so that P^T can be handed over in two parts
+#pragma unroll
+          for (int hp = 0; hp < 2; ++hp) {
+#pragma unroll
+            for (int i = 0; i < kBwdCols / 2; i += 2) {
+              const int k = kKeyMajor ? (i >> 3) * 16 + hp * 8 + (i & 7) : hp * 16 + i;
+              split(fma2(f32x2(__uint_as_float(rs[k]), __uint_as_float(rs[k + 1])), sl2, st[(k >> 2) & 3]), e[k], e[k + 1]);
+              e[k] = fast_exp2(e[k]);
+              e[k + 1] = fast_exp2(e[k + 1]);
+            }
+            if (masked) {
+#pragma unroll
+              for (int i = 0; i < kBwdCols / 2; ++i) {
+                const int k = kKeyMajor ? (i >> 3) * 16 + hp * 8 + (i & 7) : hp * 16 + i;
+                if (kKeyMajor) {
+                  const int key = me0 + (k >> 4) * 16 + (k >> 1 & 1) * 8, query = c0 + (k >> 2 & 3) * 8 + (lane & 3) * 2 + (k & 1);
+                  if (key > query || (query - key >= a.window && key >= a.sinks)) e[k] = 0.f;
+                } else if (c0 + k > me || (me - c0 - k >= a.window && c0 + k >= a.sinks)) {
+                  e[k] = 0.f;
+                }
+              }
+            }
+            if (kKeyMajor) {
+              // P^T over this warp's own S^T columns, packed from the first: the products that read the first 16
+              // run under the exponentials of the second
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t pk[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pk[i] = pack_bf16(e[h * 16 + hp * 8 + 2 * i], e[h * 16 + hp * 8 + 2 * i + 1]);
+                tmem_st_16x16_frag(ts + hp * 8 + ((h * 16u) << 16), pk);
+              }
+              tmem_st_wait();
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(p_ready + hp);
+            }
+          }
+        }
+        // ---- phase 2: dS = P * (dP * scale - delta * scale) ----
+        if (!warp_wait(dp_full + dp_buf(g), dp_phase(g), 8 * tmo) ||
+            (kKeyMajor && !warp_wait(full1 + (g & 1), (g >> 1) & 1, 8 * tmo))) {
+          if (lane == 0) report(a.status, kErrWindow + 16, it, 0);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        {
+          uint32_t rp[kBwdCols], dk[16];
+          uint64_t st[4] = {my_delta, my_delta, my_delta, my_delta};
+          if (kKeyMajor) {
+            tmem_ld_16x32_frag(tdp, rp);
+            tmem_ld_16x32_frag(tdp + (16u << 16), rp + 16);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) st[n] = *reinterpret_cast<const uint64_t*>(my_dlt + n * 8);
+          } else {
+            tmem_ld_32x32(tdp, rp);
+          }
+          tmem_ld_wait();
+#pragma unroll
+          for (int k = 0; k < kBwdCols; k += 2) {
+            float g0, g1;
+            split(mul2(f32x2(e[k], e[k + 1]),
+                       fma2(f32x2(__uint_as_float(rp[k]), __uint_as_float(rp[k + 1])), sc2, st[(k >> 2) & 3])), g0, g1);
+            dk[k >> 1] = pack_bf16(g0, g1);
+          }
+          // dS over this thread's own dP columns
+          if (kKeyMajor) {
+            tmem_st_16x32_frag(tdp, dk);
+            tmem_st_16x32_frag(tdp + (16u << 16), dk + 8);
+          } else {
+            tmem_st_32x16(tdp, dk);
+          }
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ds_ready + (g & 1));
+        }
+      }
+      if (!ok) break;
+      // Accumulators -> bf16 rows of dqkv: a warp's 32 rows x kBwdCols columns leave through shared memory as a TMA store
+      // (with plain stores the warps stall for 4000 cycles when all SMs write their items at the same time).
+      const int col = (kKeyMajor ? col_k(a, w.h) : col_q(a, w.h)) + part * kBwdCols, orow = w.blk * kBlk + q4 * 32, ob = w.b;
+      const uint32_t phase = items & 1;
+      const uint32_t out_st = (g - 1) & 1;
+      uint8_t* stage = sS1 + out_st * kTile + (warp - 2) * kBwdStage;   // where the item's last dO or V was
+      more = next_item();                        // w is the next item's from here on
+      __syncwarp();                              // every lane has read the response: the one after may be asked for now
+      if (lane == 0) mbar_arrive(clc_empty);
+#pragma unroll 1
+      for (int which = kKeyMajor ? 0 : 1; which < 2; ++which) {
+        if (!warp_wait(acc_done + which, phase, 8 * tmo)) {
+          if (lane == 0) report(a.status, kErrWindow + 17, which, 0);
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        // key-major: acc0 = dV, acc1 = dK;  query-major: acc0 = dQ
+        uint32_t r[kBwdCols];
+        tmem_ld_32x32((kKeyMajor && which ? t_acc1 : t_acc0) + lane_off + part * kBwdCols, r);
+        warp_stage_free();
+        tmem_ld_wait();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          uint4 v;
+          v.x = pack_bf16(__uint_as_float(r[q * 8 + 0]), __uint_as_float(r[q * 8 + 1]));
+          v.y = pack_bf16(__uint_as_float(r[q * 8 + 2]), __uint_as_float(r[q * 8 + 3]));
+          v.z = pack_bf16(__uint_as_float(r[q * 8 + 4]), __uint_as_float(r[q * 8 + 5]));
+          v.w = pack_bf16(__uint_as_float(r[q * 8 + 6]), __uint_as_float(r[q * 8 + 7]));
+          *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) = v;   // 64-byte swizzle
+        }
+        warp_store_box(&tm_dqkv, stage, col + (kKeyMajor && which == 0 ? kD : 0), orow, ob, a.seq);
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        bulk_wait_read<0>();
+        mbar_arrive(out_read + out_st);          // the stage may take a tile again
+      }
+      tc_fence_before_sync();                    // the accumulators are read before the next P / dS is announced
+      __syncwarp();
+    }
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  const bool all = __syncthreads_and(ok) != 0;
+  tc_fence_after_sync();
+  if (threadIdx.x == 0 && all)
+    for (int i = 2; i < 30; ++i) mbar_inval(bars + i);
+  return all;
+}
+
+// A grid of key-major items, of query-major ones, or of both, all key-major items first; a CTA of both kinds changes when cluster
+// launch control gives it an item of the other one, in that order at most once; nothing depends on that.
+template <bool kKey, bool kQuery>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+window_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
+                 const __grid_constant__ CUtensorMap tm_dqkv, const __grid_constant__ WinBwdArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~static_cast<uintptr_t>(1023));
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  // the base is 1024-byte aligned in practice; there is no room for the full slack of an arbitrary one
+  if (smem - smem_raw > kBwdAlignSlack) {
+    grid_wait();
+    if (threadIdx.x == 0) report(a.status, kErrWindow + 10, 0, 0);
+    return;
+  }
+  uint8_t* clc_resp = smem + kBwdBars;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kBwdBars + 30 * 8);
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&tm_qkv);
+    tma_prefetch_desc(&tm_do);
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+  grid_wait();
+
+  if (kKey && kQuery) {
+    uint32_t item = blockIdx.x, y, z;
+    bool more = true;
+    while (more) {
+      const bool ok = item < a.items ? window_bwd_run<true>(tm_qkv, tm_do, tm_dqkv, a, smem, tmem, item)
+                                     : window_bwd_run<false>(tm_qkv, tm_do, tm_dqkv, a, smem, tmem, item);
+      more = ok && clc_read(clc_resp, item, y, z);
+      fence_proxy_async_smem();             // this read before the next response overwrites it
+    }
+  } else {
+    window_bwd_run<kKey>(tm_qkv, tm_do, tm_dqkv, a, smem, tmem, blockIdx.x);
+  }
+  if (warp >= 2 && warp < 2 + kBwdWarps && lane == 0) bulk_wait_all<0>();
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// The shared-memory attribute is per device: set it once on every device that launches.
+cudaError_t configure_device() {
+  static bool configured[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 0 && dev < 64 && configured[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(window_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFwdSmem);
+  if (e != cudaSuccess) return e;
+  for (auto kernel : {window_bwd_kernel<true, true>, window_bwd_kernel<true, false>, window_bwd_kernel<false, true>}) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem);
+    if (e != cudaSuccess) return e;
+  }
+  if (dev >= 0 && dev < 64) configured[dev] = true;
+  return cudaSuccess;
+}
+
+int sm_count() {
+  static int count[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (count[dev] == 0 && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return count[dev];
+}
+
+// Rows of items dealt together: the largest divisor of their number that is at most 32.
+int deal(int n) {
+  int g = 1;
+  for (int d = 1; d <= 32; ++d)
+    if (n % d == 0) g = d;
+  return g;
+}
+
+bool off(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0; }
+int blocks_of(int seq) { return (seq + kBlk - 1) / kBlk; }
+cudaError_t check(const WindowShape& s) {
+  if (s.batch <= 0 || s.seq <= 0 || s.kv <= 0 || s.group <= 0 || s.window < 0 || s.sinks < 0) return cudaErrorInvalidValue;
+  const int64_t rows = (int64_t)s.batch * s.kv * s.group, width = (int64_t)s.kv * (s.group + 2) * kD;
+  if (rows > 65535 || blocks_of(s.seq) > 65535 || width > 1 << 24) return cudaErrorInvalidValue;
+  return rows * blocks_of(s.seq) > 1 << 26 ? cudaErrorInvalidValue : cudaSuccess;
+}
+
+}  // namespace
+
+cudaError_t window_attention_fwd(const void* qkv, void* out, float* lse, const WindowShape& s, uint32_t* status, cudaStream_t stream) {
+  cudaError_t e = check(s);
+  if (e != cudaSuccess) return e;
+  if (off(qkv, 16) || off(out, 16)) return cudaErrorInvalidValue;
+  e = configure_device();
+  if (e != cudaSuccess) return e;
+  const int heads = s.kv * s.group, nblk = blocks_of(s.seq);
+  CUtensorMap tq, to;
+  if (make_tensor_map_seq(&tq, qkv, (uint64_t)s.kv * (s.group + 2) * kD, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
+  if (make_tensor_map_seq(&to, out, (uint64_t)heads * kD, s.seq, s.batch, 64, 32) != 0) return cudaErrorInvalidValue;
+  WinArgs a{};
+  a.batch = s.batch; a.seq = s.seq; a.kv = s.kv; a.group = s.group; a.heads = heads;
+  a.window = s.window == 0 || s.window > s.seq ? s.seq : s.window;
+  a.sinks = s.sinks < s.seq ? s.sinks : s.seq;
+  a.scale = s.scale;
+  a.lse = lse;
+  a.status = status;
+  a.timeout_ns = 2000000000ull;
+  // With no more tiles than SMs a tile per CTA leaves none idle; beyond that pairs share K and V and overlap.
+  a.tiles_per_item = (int64_t)s.batch * heads * nblk <= sm_count() ? 1 : 2;
+  const int grp = deal(s.batch * heads);
+  const dim3 grid(grp, (nblk + a.tiles_per_item - 1) / a.tiles_per_item, s.batch * heads / grp);
+  return launch_dependent(window_fwd_kernel, grid, kFwdThreads, kFwdSmem, stream, tq, to, a);
+}
+
+int64_t window_attention_scratch(const WindowShape& s) { return 2 * (int64_t)s.batch * s.kv * s.group * blocks_of(s.seq) * kBlk; }
+
+cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* dout, const float* lse, void* dqkv, float* scratch,
+                                 const WindowShape& s, uint32_t* status, cudaStream_t stream) {
+  cudaError_t e = check(s);
+  if (e != cudaSuccess) return e;
+  if (off(qkv, 16) || off(out, 16) || off(dout, 16) || off(dqkv, 16) || off(scratch, 16)) return cudaErrorInvalidValue;
+  e = configure_device();
+  if (e != cudaSuccess) return e;
+  const int heads = s.kv * s.group, nblk = blocks_of(s.seq);
+  const uint64_t width = (uint64_t)s.kv * (s.group + 2) * kD;
+  CUtensorMap tq, td, tg;
+  if (make_tensor_map_seq(&tq, qkv, width, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
+  if (make_tensor_map_seq(&td, dout, (uint64_t)heads * kD, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
+  if (make_tensor_map_seq(&tg, dqkv, width, s.seq, s.batch, kBwdCols, 32) != 0) return cudaErrorInvalidValue;
+  WinBwdArgs g{};
+  float* delta = scratch + (int64_t)s.batch * heads * nblk * kBlk;
+  {
+    const uint32_t groups = (uint32_t)((int64_t)s.batch * heads * nblk * (kBlk / kDeltaRows));
+    e = launch_dependent(window_delta_kernel, (groups + 15) / 16, 256, 0, stream, reinterpret_cast<const uint4*>(out),
+                         reinterpret_cast<const uint4*>(dout), delta, groups, (uint32_t)s.seq, (uint32_t)(nblk * kBlk), (uint32_t)heads,
+                         lse, scratch, s.scale);
+    if (e != cudaSuccess) return e;
+  }
+  g.lse2 = scratch;
+  g.delta = delta;
+  g.batch = s.batch; g.seq = s.seq; g.kv = s.kv; g.group = s.group; g.heads = heads;
+  g.window = s.window == 0 || s.window > s.seq ? s.seq : s.window;
+  g.sinks = s.sinks < s.seq ? s.sinks : s.seq;
+  g.scale = s.scale;
+  g.status = status;
+  g.timeout_ns = 2000000000ull;
+  g.key_group = deal(s.batch * s.kv);
+  g.query_group = deal(s.batch * heads);
+  const uint32_t keys = (uint32_t)(s.batch * s.kv) * nblk, queries = (uint32_t)(s.batch * heads) * nblk;
+  g.items = keys;
+  // Both kinds in one launch where the longer kind leaves SMs free, two beyond: the kernel of both needs more registers.
+  if (queries <= (uint32_t)sm_count())
+    return launch_dependent(window_bwd_kernel<true, true>, keys + queries, kBwdThreads, kBwdSmem, stream, tq, td, tg, g);
+  e = launch_dependent(window_bwd_kernel<true, false>, keys, kBwdThreads, kBwdSmem, stream, tq, td, tg, g);
+  if (e != cudaSuccess) return e;
+  g.items = 0;
+  return launch_dependent(window_bwd_kernel<false, true>, queries, kBwdThreads, kBwdSmem, stream, tq, td, tg, g);
+}
+
+}  // namespace msb

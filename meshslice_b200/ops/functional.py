@@ -12,7 +12,7 @@ import torch
 from .. import _native
 from .distill import distill_grad, distill_loss_grad, distill_partial  # noqa: F401  (ops of this module's callers)
 from .rotary import Rotary, RotaryConfig, rotary_qkv  # noqa: F401
-from .window import WindowCache, window_attention_decode  # noqa: F401
+from .window import WindowCache, window_attention_bwd, window_attention_decode, window_attention_fwd  # noqa: F401
 
 GELU_K0 = 0.7978845608028654
 GELU_K1 = 0.044715

@@ -26,6 +26,83 @@ def _width(qkv, kv_heads: int, group: int, batch_rows: Optional[int]) -> int:
 
 
 # ----------------------------------------------------------------------------------------------
+# whole sequences
+# ----------------------------------------------------------------------------------------------
+def _check(qkv, batch: int, seq: int, kv_heads: int, group: int, window: int, sinks: int) -> int:
+    if batch < 0 or seq < 1 or window < 0 or sinks < 0:
+        raise ValueError(f"attention needs seq >= 1, window >= 0 (0: no window) and sinks >= 0 (got batch {batch}, seq {seq}, "
+                         f"window {window}, sinks {sinks})")
+    D = _width(qkv, kv_heads, group, batch * seq)
+    if qkv.is_cuda:
+        if qkv.dtype != torch.bfloat16 or D != HEAD_DIM:
+            raise ValueError(f"the window attention kernel needs bf16 rows with head_dim {HEAD_DIM} (got {qkv.dtype}, {D})")
+        _native.check_device(qkv)
+    return D
+
+
+def _dense(t):
+    """``t`` as one block of memory on a 16-byte boundary: the kernels address whole rows without a pitch."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _formulation(qkv, batch, seq, kv_heads, group, window, sinks, D):
+    """fp32 q [b, kv, g, s, D], k and v [b, kv, 1, s, D] and the masked scores."""
+    x = qkv.float().view(batch, seq, kv_heads, group + 2, D).permute(0, 2, 3, 1, 4)
+    q, k, v = x[:, :, :group], x[:, :, group:group + 1], x[:, :, group + 1:]
+    i, j = torch.arange(seq)[:, None], torch.arange(seq)[None, :]
+    hidden = (j > i) | ((i - j >= (window or seq)) & (j >= sinks))
+    return q, k, v, (q @ k.transpose(-1, -2) / math.sqrt(D)).masked_fill(hidden, -math.inf)
+
+
+def window_attention_fwd(qkv, batch: int, seq: int, kv_heads: int, group: int = 1, window: int = 0, sinks: int = 0):
+    """softmax over what a query sees of (q k^T / sqrt(D)), times v: query i sees key j <= i where i - j < ``window`` or j <
+    ``sinks`` (``window`` 0: all).  ``qkv`` [batch * seq, kv_heads * (group + 2) * D], any ``seq``.  Returns
+    (out [batch * seq, kv_heads * group * D], lse [batch, kv_heads * group, seq])."""
+    D = _check(qkv, batch, seq, kv_heads, group, window, sinks)
+    heads = kv_heads * group
+    if qkv.is_cuda:
+        out = torch.empty(batch * seq, heads * D, dtype=qkv.dtype, device=qkv.device)
+        lse = torch.empty(batch, heads, seq, dtype=torch.float32, device=qkv.device)
+        if batch:
+            x = _dense(qkv)
+            _native.load().window_attention_fwd(x.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, seq, kv_heads, group, window, sinks,
+                                                1.0 / math.sqrt(D), _native.status().dev, _native.stream_ptr())
+        return out, lse
+    q, k, v, s = _formulation(qkv, batch, seq, kv_heads, group, window, sinks, D)
+    o = torch.softmax(s, -1) @ v
+    return o.permute(0, 3, 1, 2, 4).reshape(batch * seq, heads * D).to(qkv.dtype), torch.logsumexp(s, -1).view(batch, heads, seq)
+
+
+def window_attention_bwd(dout, qkv, out, lse, batch: int, seq: int, kv_heads: int, group: int = 1, window: int = 0, sinks: int = 0):
+    """Gradient of ``qkv`` in its layout; shared key/value heads get the sum over their query heads."""
+    D = _check(qkv, batch, seq, kv_heads, group, window, sinks)
+    heads = kv_heads * group
+    for name, t in (("dout", dout), ("out", out)):
+        if t.shape != (batch * seq, heads * D) or t.dtype != qkv.dtype or t.device != qkv.device:
+            raise ValueError(f"{name} must be {qkv.dtype} [{batch * seq}, {heads * D}] beside qkv (got {t.dtype} {tuple(t.shape)} on {t.device})")
+    if lse.shape != (batch, heads, seq) or lse.dtype != torch.float32 or lse.device != qkv.device:
+        raise ValueError(f"lse must be fp32 [{batch}, {heads}, {seq}] beside qkv (got {lse.dtype} {tuple(lse.shape)} on {lse.device})")
+    if qkv.is_cuda:
+        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        if batch:
+            C = _native.load()
+            scratch = torch.empty(C.window_attention_scratch(batch, seq, kv_heads, group, window, sinks), dtype=torch.float32,
+                                  device=qkv.device)
+            x, o, do, l = _dense(qkv), _dense(out), _dense(dout), _dense(lse)
+            C.window_attention_bwd(x.data_ptr(), o.data_ptr(), do.data_ptr(), l.data_ptr(), dqkv.data_ptr(), scratch.data_ptr(), batch,
+                                   seq, kv_heads, group, window, sinks, 1.0 / math.sqrt(D), _native.status().dev, _native.stream_ptr())
+        return dqkv
+    q, k, v, s = _formulation(qkv, batch, seq, kv_heads, group, window, sinks, D)
+    rows_of = lambda t: t.float().view(batch, seq, kv_heads, group, D).permute(0, 2, 3, 1, 4)
+    do, o, scale = rows_of(dout), rows_of(out), 1.0 / math.sqrt(D)
+    p = torch.exp(s - lse.view(batch, kv_heads, group, seq, 1))
+    dv = (p.transpose(-1, -2) @ do).sum(2, keepdim=True)
+    ds = p * (do @ v.transpose(-1, -2) - (do * o).sum(-1, keepdim=True)) * scale
+    dk = (ds.transpose(-1, -2) @ q).sum(2, keepdim=True)
+    return torch.cat([ds @ k, dk, dv], 2).permute(0, 3, 1, 2, 4).reshape(qkv.shape).to(qkv.dtype)
+
+
+# ----------------------------------------------------------------------------------------------
 # single tokens over a cache of fixed size
 # ----------------------------------------------------------------------------------------------
 class WindowCache:

@@ -3,7 +3,8 @@ import pytest
 
 import test_dependent_launches_cpu as rules
 
-SOURCES = [rules.CSRC / "ops/rotary.cu", rules.CSRC / "ops/distill.cu", rules.CSRC / "ops/window_decode.cu"]
+SOURCES = [rules.CSRC / "ops/rotary.cu", rules.CSRC / "ops/distill.cu", rules.CSRC / "ops/window_decode.cu",
+           rules.CSRC / "ops/window_attention.cu"]
 CHECKS = [rules.test_inputs_of_dependent_kernels_are_read_coherently, rules.test_dependent_launches_wait,
           rules.test_dependent_kernels_wait_before_they_touch_memory, rules.test_kernels_of_a_row_exchange_do_not_let_the_next_one_start]
 
