@@ -1220,7 +1220,7 @@ __global__ void embedding_fwd_kernel(const int64_t* tokens,
         const int v = v0 + j * blockDim.x;
         if (v < nvec) {
           u[j] = row[v];
-          w[j] = at[v];
+          w[j] = pos_table != nullptr ? at[v] : make_uint4(0u, 0u, 0u, 0u);
         }
       }
 #pragma unroll
@@ -1619,7 +1619,7 @@ cudaError_t embedding_bwd(const int64_t* tokens, const void* dout, float* dtok, 
   if (cols % 8 || n_tokens % seq) return cudaErrorInvalidValue;
   const int grid = n_tokens < 148 * 16 ? n_tokens : 148 * 16;
   const cudaError_t e = launch_dependent(embedding_bwd_tok_kernel, grid, 128, 0, stream, tokens, reinterpret_cast<const uint4*>(dout), dtok, n_tokens, cols / 8);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || dpos == nullptr) return e;
   return launch_dependent(embedding_bwd_pos_kernel, grid_for((int64_t)seq * (cols / 8), 256), 256, 0, stream, reinterpret_cast<const uint4*>(dout), dpos, n_tokens, seq, cols / 8);
 }
 

@@ -109,10 +109,10 @@ cudaError_t ce_grad(void* logits, int64_t ld, const int64_t* targets, int rows, 
                     const RowExchange* exch = nullptr, const float* tgt_logit = nullptr);
 
 // ---- embedding ----------------------------------------------------------------------------
-// out[t, :] = tok_table[token[t], :] + pos_table[t % seq, :]   (tables bf16 [*, cols])
+// out[t, :] = tok_table[token[t], :] + pos_table[t % seq, :]   (tables bf16 [*, cols]; pos_table null: without)
 cudaError_t embedding_fwd(const int64_t* tokens, const void* tok_table, const void* pos_table,
                           void* out, int n_tokens, int seq, int cols, cudaStream_t stream);
-// dtok[token[t], :] += dout[t, :]; dpos[t % seq, :] += dout[t, :]   (fp32 accumulators)
+// dtok[token[t], :] += dout[t, :]; dpos[t % seq, :] += dout[t, :]   (fp32 accumulators; dpos null: without)
 cudaError_t embedding_bwd(const int64_t* tokens, const void* dout, float* dtok, float* dpos,
                           int n_tokens, int seq, int cols, cudaStream_t stream);
 

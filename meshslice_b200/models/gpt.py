@@ -18,10 +18,12 @@ from typing import List, Optional, Tuple
 import torch
 
 from ..ops import functional as F
+from ..ops.distill import distill_rescale
+from ..ops.rotary import RotaryConfig
 from ..parallel.mesh import Mesh, ShardedTensor
 from ..parallel.tensor_parallel import init_block
 from . import sharded_layers
-from .sharded_layers import GeLU, ShardedAttention, ShardedFFLayer, ShardedLayerNorm, _add
+from .sharded_layers import GeLU, ShardedAttention, ShardedFFLayer, ShardedLayerNorm, ShardedWindowAttention, _add
 
 
 @dataclass
@@ -41,6 +43,31 @@ class GPTConfig:
     init_std: float = 0.02
     vocab_pad: int = 2048          # the vocabulary is padded to a multiple of this
     dtype: torch.dtype = torch.bfloat16
+    # long contexts: key/value heads shared by query heads (0: one each), attention to the last ``window`` tokens (0: all) and the first
+    # ``sinks``, rotary positions in place of the learned ones
+    kv_heads: int = 0
+    window: int = 0
+    sinks: int = 0
+    rotary: Optional[RotaryConfig] = None
+
+    def __post_init__(self):
+        if self.window < 0 or self.sinks < 0 or (self.kv_heads and self.n_heads % self.kv_heads):
+            raise ValueError(f"window and sinks are not negative and query heads a multiple of key/value heads (got window {self.window}, "
+                             f"sinks {self.sinks}, {self.n_heads} on {self.kv_heads})")
+        if self.windowed and not self.causal:
+            raise ValueError("shared heads, windows and rotary positions are for causal attention")
+        if self.rotary is not None and self.rotary.head_dim * self.n_heads != self.d_model:
+            raise ValueError(f"rotary positions are for heads of {self.rotary.head_dim} features, the model has {self.d_model // self.n_heads}")
+
+    @property
+    def windowed(self) -> bool:
+        """The attention is ``ShardedWindowAttention``."""
+        return bool(self.kv_heads or self.window or self.sinks or self.rotary is not None)
+
+    @property
+    def qkv_dim(self) -> int:
+        """Output features of the attention's input projection."""
+        return self.d_model + 2 * (self.kv_heads or self.n_heads) * (self.d_model // self.n_heads)
 
     @property
     def vocab_padded(self) -> int:
@@ -48,15 +75,18 @@ class GPTConfig:
 
     def n_params(self) -> int:
         d = self.d_model
-        per_layer = 3 * d * d + d * d + 2 * d * self.ffn + 4 * d
-        return self.n_layers * per_layer + (self.vocab_padded + self.seq) * d + d * self.vocab_padded + 2 * d
+        per_layer = d * self.qkv_dim + d * d + 2 * d * self.ffn + 4 * d
+        positions = 0 if self.rotary is not None else self.seq
+        return self.n_layers * per_layer + (self.vocab_padded + positions) * d + d * self.vocab_padded + 2 * d
 
     def flops_per_token(self) -> float:
         """Model FLOPs of one training step per token (forward + backward = 3x forward GEMMs,
-        attention counted with its full S x S score matrix as the reference's block does)."""
+        attention counted with its full S x S score matrix as the reference's block does; a window's with its pairs)."""
         d = self.d_model
-        gemm = 2 * (3 * d * d + d * d + 2 * d * self.ffn) * self.n_layers + 2 * d * self.vocab_padded
+        gemm = 2 * (d * self.qkv_dim + d * d + 2 * d * self.ffn) * self.n_layers + 2 * d * self.vocab_padded
         attn = 4 * self.seq * d * self.n_layers * (0.5 if self.causal else 1.0)
+        if self.window and self.window < self.seq:
+            attn *= min(1.0, 2.0 * (self.window + self.sinks) / self.seq)
         return 3.0 * (gemm + attn)
 
 
@@ -72,8 +102,11 @@ class GPTBlock:
         s = idx * 16
         self.ln1 = ShardedLayerNorm(mesh, d, affine=True, eps=cfg.eps, dtype=cfg.dtype, device=device, alloc=alloc_rep,
                                     grad_alloc=grad_rep)
-        self.in_proj = ShardedFFLayer(mesh, cfg.algorithm, df[0], ks[0], d, 3 * d, seed=s + 1, **kw)
-        self.attn = ShardedAttention(mesh, cfg.n_heads, cfg.seq, causal=cfg.causal)
+        self.in_proj = ShardedFFLayer(mesh, cfg.algorithm, df[0], ks[0], d, cfg.qkv_dim, seed=s + 1, **kw)
+        if cfg.windowed:
+            self.attn = ShardedWindowAttention(mesh, cfg.n_heads, cfg.seq, cfg.kv_heads, cfg.window, cfg.sinks, cfg.rotary, device)
+        else:
+            self.attn = ShardedAttention(mesh, cfg.n_heads, cfg.seq, causal=cfg.causal)
         self.out_proj = ShardedFFLayer(mesh, cfg.algorithm, df[1], ks[1], d, d, seed=s + 2, **kw)
         self.ln2 = ShardedLayerNorm(mesh, d, affine=True, eps=cfg.eps, dtype=cfg.dtype, device=device, alloc=alloc_rep,
                                     grad_alloc=grad_rep)
@@ -125,6 +158,16 @@ class GPTBlock:
         return [self.ln1, self.in_proj, self.out_proj, self.ln2, self.ff1, self.ff2]
 
 
+@dataclass
+class DistillTargets:
+    """What a teacher says about the tokens of a micro-batch: per coordinate its top logits [local_tokens, top] and their ids (an id
+    outside the vocabulary is no entry), and how the loss is made of them: ``hard_weight`` of it from the labels."""
+    ids: ShardedTensor
+    logits: ShardedTensor
+    temperature: float = 1.0
+    hard_weight: float = 0.0
+
+
 class GPTModel:
     def __init__(self, mesh: Mesh, cfg: GPTConfig, device=None, alloc_sharded=None, alloc_rep=None,
                  grad_sharded=None, grad_rep=None):
@@ -134,20 +177,24 @@ class GPTModel:
         d, C = cfg.d_model, mesh.C
         a_rep = alloc_rep or (lambda shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
         g_rep = grad_rep or (lambda shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
-        self.tok, self.pos = ShardedTensor(mesh, {}), ShardedTensor(mesh, {})
-        self.dtok, self.dpos = ShardedTensor(mesh, {}), ShardedTensor(mesh, {})
+        learned = cfg.rotary is None
+        self.tok, self.pos = ShardedTensor(mesh, {}), ShardedTensor(mesh, {}) if learned else None
+        self.dtok, self.dpos = ShardedTensor(mesh, {}), ShardedTensor(mesh, {}) if learned else None
         # parameters and their gradients are carved in the same order, so a parameter and its
         # gradient sit at the same offset of the flat parameter / gradient buffers
         for (r, c) in mesh.coords():
             t = a_rep((cfg.vocab_padded, d // C), cfg.dtype, device)
             t.copy_(init_block((cfg.vocab_padded, d), cfg.init_std, 900001, 0, cfg.vocab_padded,
                                c * (d // C), (c + 1) * (d // C), device=device).to(cfg.dtype))
-            p = a_rep((cfg.seq, d // C), cfg.dtype, device)
-            p.copy_(init_block((cfg.seq, d), cfg.init_std, 900002, 0, cfg.seq,
-                               c * (d // C), (c + 1) * (d // C), device=device).to(cfg.dtype))
-            self.tok.shards[(r, c)], self.pos.shards[(r, c)] = t, p
+            self.tok.shards[(r, c)] = t
+            if learned:
+                p = a_rep((cfg.seq, d // C), cfg.dtype, device)
+                p.copy_(init_block((cfg.seq, d), cfg.init_std, 900002, 0, cfg.seq,
+                                   c * (d // C), (c + 1) * (d // C), device=device).to(cfg.dtype))
+                self.pos.shards[(r, c)] = p
             self.dtok.shards[(r, c)] = g_rep((cfg.vocab_padded, d // C), torch.float32, device).zero_()
-            self.dpos.shards[(r, c)] = g_rep((cfg.seq, d // C), torch.float32, device).zero_()
+            if learned:
+                self.dpos.shards[(r, c)] = g_rep((cfg.seq, d // C), torch.float32, device).zero_()
         self.blocks = [GPTBlock(mesh, cfg, i, device, alloc_sharded, alloc_rep, grad_sharded, grad_rep)
                        for i in range(cfg.n_layers)]
         self.ln_f = ShardedLayerNorm(mesh, d, affine=True, eps=cfg.eps, dtype=cfg.dtype, device=device, alloc=alloc_rep,
@@ -161,7 +208,9 @@ class GPTModel:
     def parameters(self):
         """[(name, param ShardedTensor, grad ShardedTensor, kind)] with kind 'sharded' (unique per
         rank) or 'row_replicated' (same value along a mesh column; gradients are summed there)."""
-        out = [("tok", self.tok, self.dtok, "row_replicated"), ("pos", self.pos, self.dpos, "row_replicated")]
+        out = [("tok", self.tok, self.dtok, "row_replicated")]
+        if self.pos is not None:
+            out.append(("pos", self.pos, self.dpos, "row_replicated"))
         for i, b in enumerate(self.blocks):
             for j, l in enumerate(b.layers()):
                 out += [(f"block{i}.{type(l).__name__}{j}.{n}", p, g, kind) for n, p, g, kind in l.parameters()]
@@ -175,25 +224,61 @@ class GPTModel:
                 t.zero_()
 
     # ------------------------------------------------------------------ training step pieces
-    def forward_backward(self, tokens: ShardedTensor, targets: ShardedTensor, n_tokens_global: int):
-        """One micro-batch: forward, loss, backward; gradients accumulate.  ``tokens`` / ``targets``
-        hold, per coordinate, the int64 ids of the sequences of that mesh row [local_tokens].
-        Returns the ShardedTensor of per-coordinate loss contributions (sum over local tokens of
-        the token loss divided by n_tokens_global; summing over the mesh rows gives the mean)."""
+    def forward(self, tokens: ShardedTensor) -> ShardedTensor:
+        """Logits [local tokens, padded vocabulary / C] of whole sequences."""
         m, cfg = self.mesh, self.cfg
-        x = ShardedTensor(m, {k: F.embedding_fwd(tokens.shards[k], self.tok.shards[k], self.pos.shards[k], cfg.seq)
-                              for k in m.coords()})
+        pos = lambda k: None if self.pos is None else self.pos.shards[k]
+        x = ShardedTensor(m, {k: F.embedding_fwd(tokens.shards[k], self.tok.shards[k], pos(k), cfg.seq) for k in m.coords()})
         delta = None
         for b in self.blocks:
             x, delta = b.forward(x, delta)
         y = self.ln_f.forward(x, delta)
-        logits = self.head.forward(y)                                    # [T/R, Vp/C]
+        return self.head.forward(y)                                      # [T/R, Vp/C]
+
+    def top_logits(self, tokens: ShardedTensor, top: int, temperature: float = 1.0, hard_weight: float = 0.0) -> DistillTargets:
+        """This model as a teacher: its ``top`` largest logits per token (whole rows on every device)."""
+        if self.mesh.C != 1:
+            raise ValueError("a teacher's rows of logits are whole: its mesh has one column")
+        best = {k: l[:, :self.cfg.vocab].float().topk(top, dim=1) for k, l in self.forward(tokens).shards.items()}
+        return DistillTargets(ShardedTensor(self.mesh, {k: v.indices for k, v in best.items()}),
+                              ShardedTensor(self.mesh, {k: v.values for k, v in best.items()}), temperature, hard_weight)
+
+    def _distill(self, logits: ShardedTensor, targets: ShardedTensor, n_tokens: int, t: DistillTargets) -> ShardedTensor:
+        """Loss contributions of a teacher's targets; the logits become their gradient."""
+        m, cfg = self.mesh, self.cfg
+        a = lambda k: (logits.shards[k], t.ids.shards[k], t.logits.shards[k])
+        if m.C == 1:
+            rows = {k: F.distill_loss_grad(*a(k), cfg.vocab, 1.0 / n_tokens, t.temperature, targets.shards[k], t.hard_weight,
+                                           out=logits.shards[k])[0] for k in m.coords()}
+        else:
+            vc = cfg.vocab_padded // m.C
+            parts = {k: F.distill_partial(*a(k), k[1] * vc, cfg.vocab, t.temperature, targets.shards[k]) for k in m.coords()}
+            gmax = m.all_reduce(ShardedTensor(m, {k: p[:, 0].contiguous() for k, p in parts.items()}), "col", op="max")
+            total = m.all_reduce(ShardedTensor(m, {k: distill_rescale(p, gmax.shards[k], t.temperature) for k, p in parts.items()}), "col")
+            rows = {}
+            for k in m.coords():
+                stats = torch.cat([gmax.shards[k][:, None], total.shards[k][:, 1:]], 1)
+                rows[k] = F.distill_grad(*a(k), k[1] * vc, cfg.vocab, 1.0 / n_tokens, stats, t.temperature, targets.shards[k],
+                                         t.hard_weight, out=logits.shards[k])[0]
+        return ShardedTensor(m, {k: F.sum_over(r, n_tokens) for k, r in rows.items()})
+
+    def forward_backward(self, tokens: ShardedTensor, targets: ShardedTensor, n_tokens_global: int,
+                         teacher: Optional[DistillTargets] = None):
+        """One micro-batch: forward, loss, backward; gradients accumulate.  ``tokens`` / ``targets``
+        hold, per coordinate, the int64 ids of the sequences of that mesh row [local_tokens].  With ``teacher`` the loss is
+        the distillation loss of its targets.
+        Returns the ShardedTensor of per-coordinate loss contributions (sum over local tokens of
+        the token loss divided by n_tokens_global; summing over the mesh rows gives the mean)."""
+        m, cfg = self.mesh, self.cfg
+        logits = self.forward(tokens)
         vc = cfg.vocab_padded // m.C
         ex = getattr(getattr(m, "engine", None), "row_exchange", None)
         k0 = l0 = None
         if len(logits.shards) == 1:
             (k0, l0), = logits.shards.items()
-        if ex is not None and l0 is not None and l0.is_cuda:
+        if teacher is not None:
+            loss = self._distill(logits, targets, n_tokens_global, teacher)
+        elif ex is not None and l0 is not None and l0.is_cuda:
             # max / sum-exp / target logit of the vocabulary slices travel inside the two kernels
             from .. import _native
             prod, cons = ex.next(l0.shape[0], _native.load().ce_grid(l0.shape[0]))
@@ -224,7 +309,8 @@ class GPTModel:
         for b in reversed(self.blocks):
             dh, dm = b.backward(dh, dm)
         for k in m.coords():
-            F.embedding_bwd(tokens.shards[k], dh.shards[k], self.dtok.shards[k], self.dpos.shards[k], cfg.seq)
+            F.embedding_bwd(tokens.shards[k], dh.shards[k], self.dtok.shards[k], None if self.dpos is None else self.dpos.shards[k],
+                            cfg.seq)
         return loss
 
     def sync_replicated_grads(self):

@@ -26,6 +26,7 @@ import torch
 
 from .._native import zero_, zero_both_
 from ..ops import functional as F
+from ..ops.rotary import Rotary, RotaryConfig
 from ..parallel.mesh import Mesh, ShardedTensor
 from ..parallel.tensor_parallel import SPMD, createMultihostMatrix
 
@@ -287,6 +288,51 @@ class ShardedAttention:
         return ShardedTensor(self.mesh, {
             k: F.attention_bwd(dy.shards[k], t, outs[k][0], outs[k][1], t.shape[0] // self.seqlen, self.seqlen,
                                self.heads_per_shard, self.causal, allow_fallback=self.allow_fallback)
+            for k, t in x.shards.items()})
+
+    def parameters(self):
+        return []
+
+
+class ShardedWindowAttention:
+    """Causal attention with sequences on mesh rows and key/value heads (with their query heads) on mesh columns: no communication.
+    Per key/value head the columns are [q_0 | .. | q_group-1 | k | v].  A query sees the last ``window`` tokens (0: all) and the first
+    ``sinks``; ``rotary`` turns queries and keys to their positions first."""
+
+    def __init__(self, mesh: Mesh, n_heads: int, seqlen: int, kv_heads: int = 0, window: int = 0, sinks: int = 0,
+                 rotary: Optional[RotaryConfig] = None, device=None):
+        kv_heads = kv_heads or n_heads
+        if kv_heads < 1 or n_heads % kv_heads:
+            raise ValueError(f"query heads ({n_heads}) must be a multiple of key/value heads ({kv_heads})")
+        if kv_heads % mesh.C:
+            raise ValueError("key/value heads must divide over the mesh columns")
+        self.mesh, self.seqlen, self.window, self.sinks = mesh, seqlen, window, sinks
+        self.kv_per_shard, self.group = kv_heads // mesh.C, n_heads // kv_heads
+        self.rotary = Rotary(rotary, device=device) if rotary is not None else None
+        self._saved = None
+
+    def _shape(self, t):
+        if t.shape[0] % self.seqlen:
+            raise ValueError("local tokens must be whole sequences (batch divisible by mesh rows)")
+        return t.shape[0] // self.seqlen, self.seqlen, self.kv_per_shard, self.group, self.window, self.sinks
+
+    def _turn(self, t, inverse: bool):
+        """In place: queries and keys of the rows are only ever wanted turned, their gradients turned back."""
+        if self.rotary is not None:
+            F.rotary_qkv(t, self.rotary, self.kv_per_shard, self.group, seq=self.seqlen, inverse=inverse, out=t)
+        return t
+
+    def forward(self, x: ShardedTensor) -> ShardedTensor:
+        """With ``rotary``, ``x`` is turned in place."""
+        outs = {k: F.window_attention_fwd(self._turn(t, False), *self._shape(t)) for k, t in x.shards.items()}
+        self._saved = (x, outs)
+        return ShardedTensor(self.mesh, {k: v[0] for k, v in outs.items()})
+
+    def backward(self, dy: ShardedTensor) -> ShardedTensor:
+        x, outs = self._saved
+        self._saved = None
+        return ShardedTensor(self.mesh, {
+            k: self._turn(F.window_attention_bwd(dy.shards[k], t, outs[k][0], outs[k][1], *self._shape(t)), True)
             for k, t in x.shards.items()})
 
     def parameters(self):

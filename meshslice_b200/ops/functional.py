@@ -347,24 +347,28 @@ def ce_grad_(logits, targets, col_offset: int, vocab: int, gmax, gsum, scale: fl
 # embedding
 # ----------------------------------------------------------------------------------------------
 def embedding_fwd(tokens, tok_table, pos_table, seq: int):
+    """``pos_table`` None: no learned positions."""
     n = tokens.numel()
     cols = tok_table.shape[1]
     if tok_table.is_cuda:
         out = torch.empty(n, cols, dtype=tok_table.dtype, device=tok_table.device)
-        _C().embedding_fwd(tokens.data_ptr(), tok_table.data_ptr(), pos_table.data_ptr(), out.data_ptr(),
+        _C().embedding_fwd(tokens.data_ptr(), tok_table.data_ptr(), _p(pos_table), out.data_ptr(),
                            n, seq, cols, _st())
         return out
+    if pos_table is None:
+        return tok_table[tokens.view(-1)]
     pos = torch.arange(n) % seq
     return (tok_table.float()[tokens.view(-1)] + pos_table.float()[pos]).to(tok_table.dtype)
 
 
 def embedding_bwd(tokens, dout, dtok, dpos, seq: int):
-    """dtok / dpos: fp32 accumulators."""
+    """dtok / dpos: fp32 accumulators (dpos None: no learned positions)."""
     n = tokens.numel()
     cols = dout.shape[1]
     if dout.is_cuda:
-        _C().embedding_bwd(tokens.data_ptr(), dout.data_ptr(), dtok.data_ptr(), dpos.data_ptr(), n, seq,
+        _C().embedding_bwd(tokens.data_ptr(), dout.data_ptr(), dtok.data_ptr(), _p(dpos), n, seq,
                            cols, _st())
         return
     dtok.index_add_(0, tokens.view(-1), dout.float())
-    dpos += dout.float().view(n // seq, seq, cols).sum(0)
+    if dpos is not None:
+        dpos += dout.float().view(n // seq, seq, cols).sum(0)

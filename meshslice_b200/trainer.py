@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import os
 from dataclasses import dataclass
-from typing import Optional, Tuple
+from typing import Callable, Optional, Tuple
 
 import torch
 
@@ -40,9 +40,9 @@ def param_elems(cfg: GPTConfig, R: int, C: int) -> Tuple[int, int]:
     """Elements (with alignment padding) of the sharded and row-replicated buffers of one rank."""
     pad = lambda n: (n + 127) // 128 * 128
     d, f, V = cfg.d_model, cfg.ffn, cfg.vocab_padded
-    per_layer = pad(d * 3 * d // (R * C)) + pad(d * d // (R * C)) + 2 * pad(d * f // (R * C))
+    per_layer = pad(d * cfg.qkv_dim // (R * C)) + pad(d * d // (R * C)) + 2 * pad(d * f // (R * C))
     sharded = cfg.n_layers * per_layer + pad(d * V // (R * C))
-    rep = pad(V * d // C) + pad(cfg.seq * d // C) + (2 * cfg.n_layers + 1) * 2 * pad(d // C)
+    rep = pad(V * d // C) + (pad(cfg.seq * d // C) if cfg.rotary is None else 0) + (2 * cfg.n_layers + 1) * 2 * pad(d // C)
     return sharded, rep
 
 
@@ -69,7 +69,7 @@ def workspace_bytes(cfg, micro_batch: int, R: int, C: int):
     under its dataflow (m = tokens per mesh row and micro-batch).  Returns (stage_a, stage_b, slots)."""
     m = micro_batch * cfg.seq
     d, f, V = cfg.d_model, cfg.ffn, cfg.vocab_padded
-    lin = [(d, 3 * d, cfg.dataflows[0]), (d, d, cfg.dataflows[1]), (d, f, cfg.dataflows[2]),
+    lin = [(d, cfg.qkv_dim, cfg.dataflows[0]), (d, d, cfg.dataflows[1]), (d, f, cfg.dataflows[2]),
            (f, d, cfg.dataflows[3]), (d, V, "os")]
     sa = sb = sl = 0
     for i, o, df in lin:
@@ -145,9 +145,10 @@ class Trainer:
         return ids_global[self.r * self.rows_batch:(self.r + 1) * self.rows_batch]
 
     # ------------------------------------------------------------------ step
-    def train_step(self, ids_row: torch.Tensor, read_loss: bool = True):
+    def train_step(self, ids_row: torch.Tensor, read_loss: bool = True, teacher: Optional[Callable] = None):
         """One optimizer step.  ``ids_row``: [global_batch / R, seq + 1] int64 token ids of this
-        rank's mesh row, in pinned host memory or on the device.  Returns the mean token loss as a
+        rank's mesh row, in pinned host memory or on the device.  ``teacher``: gives the ``DistillTargets`` of a micro-batch's tokens
+        (for instance another model's ``top_logits``); the loss is then that of ``GPTModel.forward_backward`` with them.  Returns the mean token loss as a
         float when ``read_loss`` (a device-to-host read), else the device scalar."""
         cfg, mb = self.cfg, self.tcfg.micro_batch
         if ids_row.device != self.device:
@@ -161,7 +162,7 @@ class Trainer:
             chunk = ids[i * mb:(i + 1) * mb]
             tok = ShardedTensor(self.mesh, {key: chunk[:, :-1].reshape(-1)})
             tgt = ShardedTensor(self.mesh, {key: chunk[:, 1:].reshape(-1)})
-            loss = self.model.forward_backward(tok, tgt, self.n_tokens)
+            loss = self.model.forward_backward(tok, tgt, self.n_tokens, None if teacher is None else teacher(tok))
             self._loss_dev += loss.shards[key]
         self.model.sync_replicated_grads()
         self.opt.step()

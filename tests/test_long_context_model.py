@@ -1,0 +1,154 @@
+"""A windowed GPT with rotary positions and shared heads: training on emulated meshes against a dense model, distillation, token by token."""
+import math
+
+import pytest
+import torch
+
+from meshslice_b200.models.decode import GPTDecoder
+from meshslice_b200.models.gpt import DistillTargets, GPTConfig, GPTModel
+from meshslice_b200.ops import functional as F
+from meshslice_b200.ops.rotary import Rotary, RotaryConfig
+from meshslice_b200.parallel.mesh import EmuMesh, ShardedTensor
+from meshslice_b200.trainer import param_elems
+
+ROT = RotaryConfig(head_dim=16, rot_dim=16, layout="interleaved", scaling="by_parts", factor=4.0, original_len=16)
+CFG = GPTConfig(n_layers=2, d_model=128, n_heads=8, kv_heads=4, ffn=256, vocab=500, seq=37, ksplits=(2, 2, 2, 2), head_ksplit=2,
+                vocab_pad=256, dtype=torch.float32, window=9, sinks=2, rotary=ROT)
+
+
+def _cols(mesh, st):
+    return torch.cat([st.shards[(0, c)] for c in range(mesh.C)], dim=-1)
+
+
+def _dense_logits(model, mesh, cfg, ids, leaf):
+    """Plain forward of the same network; ``ids`` [batch, n]."""
+    B, n = ids.shape
+    kv, g, D = cfg.kv_heads, cfg.n_heads // cfg.kv_heads, cfg.d_model // cfg.n_heads
+    x = leaf("tok", _cols(mesh, model.tok))[ids.reshape(-1)]
+    ln = lambda v, l, t: torch.nn.functional.layer_norm(v, (cfg.d_model,), leaf(t + ".g", _cols(mesh, l.gamma)), leaf(t + ".b", _cols(mesh, l.bias)), cfg.eps)
+
+    def lin(v, layer, t):
+        w = leaf(t, mesh.unshard(layer.weight))
+        return v @ (w.t() if layer.dataflow == "ls" else w)
+    cos, sin = Rotary(cfg.rotary).cos_sin(torch.arange(n))
+    i, j = torch.arange(n)[:, None], torch.arange(n)[None, :]
+    hidden = (j > i) | ((i - j >= cfg.window) & (j >= cfg.sinks))
+    for b, blk in enumerate(model.blocks):
+        qkv = lin(ln(x, blk.ln1, f"{b}.ln1"), blk.in_proj, f"{b}.in").view(B, n, kv, g + 2, D)
+        c, s = cos[:, None, None], sin[:, None, None]
+        u, v = qkv[..., 0::2], qkv[..., 1::2]
+        turned = torch.stack([u * c - v * s, v * c + u * s], -1).flatten(-2)
+        q, k, v = turned[:, :, :, :g], turned[:, :, :, g], qkv[:, :, :, g + 1]
+        sc = torch.einsum("bnhgd,bmhd->bhgnm", q, k) / math.sqrt(D)
+        a = torch.einsum("bhgnm,bmhd->bnhgd", torch.softmax(sc.masked_fill(hidden, -math.inf), -1), v).reshape(B * n, -1)
+        x = x + lin(a, blk.out_proj, f"{b}.out")
+        m = torch.nn.functional.gelu(lin(ln(x, blk.ln2, f"{b}.ln2"), blk.ff1, f"{b}.ff1"), approximate="tanh")
+        x = x + lin(m, blk.ff2, f"{b}.ff2")
+    return lin(ln(x, model.ln_f, "lnf"), model.head, "head")[:, :cfg.vocab]
+
+
+@pytest.mark.parametrize("distill", [False, True])
+@pytest.mark.parametrize("shape", [(1, 1), (2, 2), (1, 4)])
+def test_loss_and_gradients_match_dense_model(shape, distill):
+    R, C = shape
+    mesh = EmuMesh(R, C)
+    model, B, n, K, T, w = GPTModel(mesh, CFG), 4, CFG.seq, 5, 2.0, 0.25
+    gen = torch.Generator().manual_seed(1)
+    ids = torch.randint(0, CFG.vocab, (B, n + 1), generator=gen)
+    tid = torch.stack([torch.randperm(CFG.vocab, generator=gen)[:K] for _ in range(B * n)])
+    tval = torch.randn(B * n, K, generator=gen)
+    per = B // R
+    rows = lambda t: ShardedTensor(mesh, {(r, c): t[r * per * n:(r + 1) * per * n].clone() for (r, c) in mesh.coords()})
+    teacher = DistillTargets(rows(tid), rows(tval), T, w) if distill else None
+    tok, tgt = ids[:, :-1].reshape(-1), ids[:, 1:].reshape(-1)
+    loss = model.forward_backward(rows(tok), rows(tgt), B * n, teacher)
+    model.sync_replicated_grads()
+    P = {}
+
+    def leaf(name, t):
+        P[name] = t.clone().float().requires_grad_(True)
+        return P[name]
+    z = _dense_logits(model, mesh, CFG, ids[:, :-1], leaf)
+    want = torch.nn.functional.cross_entropy(z, tgt)
+    if distill:
+        p = torch.softmax(tval / T, 1)
+        kl = (p * (p.log() - torch.log_softmax(z / T, 1).gather(1, tid))).sum(1).mean()
+        want = w * want + (1 - w) * T * T * kl
+    want.backward()
+    assert abs(sum(loss.shards[(r, 0)] for r in range(R)).item() - want.item()) < 1e-4
+    b0 = model.blocks[0]
+    for layer, tag in ((b0.in_proj, "0.in"), (b0.out_proj, "0.out"), (b0.ff1, "0.ff1"), (model.blocks[1].in_proj, "1.in"), (model.head, "head")):
+        assert torch.allclose(mesh.unshard(layer.grad), P[tag].grad, atol=2e-5, rtol=1e-3), tag
+    assert torch.allclose(_cols(mesh, model.dtok), P["tok"].grad, atol=2e-5, rtol=1e-3)
+
+
+def test_parameters_and_sizes():
+    """Rotary models have no learned positions; buffers and counts follow the shared heads."""
+    mesh = EmuMesh(1, 1)
+    model = GPTModel(mesh, CFG)
+    params = model.parameters()
+    assert model.pos is None and "pos" not in [n for n, *_ in params]
+    total = sum(p.shards[(0, 0)].numel() for _, p, _, _ in params)
+    assert total == CFG.n_params()
+    sharded, rep = param_elems(CFG, 1, 1)
+    pad = lambda v: (v + 127) // 128 * 128
+    for kind, n in (("sharded", sharded), ("row_replicated", rep)):
+        assert n == sum(pad(p.shards[(0, 0)].numel()) for _, p, _, k in params if k == kind)
+    for bad in (dict(kv_heads=3), dict(window=-1), dict(causal=False), dict(rotary=RotaryConfig(head_dim=32))):
+        with pytest.raises(ValueError):
+            GPTConfig(**{**dict(n_layers=1, d_model=128, n_heads=8, window=4), **bad})
+    with pytest.raises(ValueError):
+        GPTModel(EmuMesh(1, 8), CFG)
+
+
+@pytest.mark.parametrize("prompt", [1, 8, 30])
+@pytest.mark.parametrize("rotary", [ROT, None])
+def test_token_by_token_is_the_whole_sequence(rotary, prompt):
+    cfg = GPTConfig(**{**CFG.__dict__, "rotary": rotary})
+    mesh = EmuMesh(1, 1)
+    model = GPTModel(mesh, cfg)
+    ids = torch.randint(0, cfg.vocab, (2, cfg.seq), generator=torch.Generator().manual_seed(2))
+    want = model.forward(ShardedTensor(mesh, {(0, 0): ids.reshape(-1)})).shards[(0, 0)][:, :cfg.vocab].view(2, cfg.seq, -1)
+    d = GPTDecoder(model, 2)
+    got = [d.prefill(ids[:, :prompt])]
+    got += [d.step(ids[:, p], torch.full((2,), p)) for p in range(prompt, cfg.seq)]
+    assert torch.allclose(torch.stack(got, 1), want[:, prompt - 1:], atol=1e-4, rtol=1e-4)
+    with pytest.raises(ValueError):
+        d.step(ids[:1, 0], torch.zeros(2))
+    with pytest.raises(ValueError):
+        GPTDecoder(GPTModel(mesh, GPTConfig(**{**cfg.__dict__, "window": 0})), 2)
+
+
+# ---------------------------------------------------------------------------------------------- on a GPU
+@pytest.mark.gpu
+def test_example_runs_and_learns():
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parent.parent / "bench" / "distill_window.py"
+    spec = importlib.util.spec_from_file_location("distill_window", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    losses, written = mod.main(["--steps", "12", "--seqlen", "333", "--window", "64", "--scale-factor", "2"])
+    assert losses[-1] < losses[0] and all(math.isfinite(v) for v in losses)
+    assert len(written) == 4 and all(0 <= t < 1000 for row in written for t in row)
+
+
+@pytest.mark.gpu
+def test_decoding_on_a_gpu_is_the_whole_sequence():
+    """Logits of 32 tokens written one by one against those of the whole sequence: both paths round activations to bf16 at the same
+    places, but sum in different orders, so the streams differ by the rounding of each block's outputs: 2 blocks and the head, each
+    2^-8 of values of the residual stream's size, whose effect on the logits is bounded by their own size."""
+    from meshslice_b200 import _native
+    from meshslice_b200.parallel.engine import LocalGemmEngine
+    mesh = EmuMesh(1, 1)
+    LocalGemmEngine(mesh)
+    cfg = GPTConfig(n_layers=2, d_model=512, n_heads=4, kv_heads=2, ffn=1024, vocab=777, seq=200, vocab_pad=256, window=50, sinks=3,
+                    rotary=RotaryConfig(), init_std=0.05)
+    model = GPTModel(mesh, cfg, device=torch.device("cuda", 0))
+    ids = torch.randint(0, cfg.vocab, (3, cfg.seq), generator=torch.Generator().manual_seed(2)).cuda()
+    want = model.forward(ShardedTensor(mesh, {(0, 0): ids.reshape(-1)})).shards[(0, 0)][:, :cfg.vocab].view(3, cfg.seq, -1).float()
+    d = GPTDecoder(model, 3)
+    got = [d.prefill(ids[:, :169])] + [d.step(ids[:, p], torch.full((3,), p, device="cuda")) for p in range(169, cfg.seq)]
+    _native.check_status()
+    diff = torch.stack(got, 1).float() - want[:, 168:]
+    assert diff.norm() < 6 * 2.0 ** -8 * want[:, 168:].norm()
