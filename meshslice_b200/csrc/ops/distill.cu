@@ -14,7 +14,6 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr uint32_t kNegInf2 = 0xff80ff80u;       // two bf16 -inf
 constexpr int kVec = 4;                          // vectors of a thread that are worked on together
-constexpr int kAhead = 4;                        // groups of kVec that are on their way
 constexpr int kRowBytes = 200 * 1024;            // most of a row that is kept
 
 __device__ __forceinline__ float lo(uint32_t v) { return __uint_as_float(v << 16); }
@@ -66,18 +65,21 @@ __device__ __forceinline__ uint4 cut(uint4 u, int v, int valid) {
   return u;
 }
 
-// Which exponentials a row needs: those of z / T, of z, or both (one kind serves both where T = 1).
-enum Kind { kSoft = 1, kHard = 2, kTwo = 3 };
+// Which exponentials a row needs: those of z / T, of z (one kind serves both where T = 1), both, or, where T = 2, those of z as the
+// squares of those of z / T: the special-function unit gives 16 a cycle and SM, so that four of them an element would take 180 us for
+// 4096 rows of 50257 (148 SMs), two 90.
+enum Kind { kSoft = 1, kHard = 2, kTwo = 3, kSquare = 5 };
 
 // A thread's running maximum m, and sums of exp(z - m) and exp((z - m) / T).  Differences are taken first: they are exact where they
-// matter, and a rounded m / T would shift the whole row.
+// matter, and a rounded m / T would shift the whole row.  (Behind the exponentials scalar sums: packing their results takes moves.)
 template <int K>
 struct Sums {
+  static constexpr bool soft_exp = K & kSoft, hard_exp = K == kHard || K == kTwo, squares = K == kSquare;
   float m = -INFINITY, soft = 0.f, hard = 0.f;
   __device__ __forceinline__ void raise(float to, float c) {
     if (to > m) {
-      if (K & kSoft) soft *= exp2_ftz((m - to) * c);      // (0 while m is -inf: the sums are 0)
-      if (K & kHard) hard *= exp2_ftz((m - to) * kLog2e);
+      soft *= exp2_ftz((m - to) * c);                     // (0 while m is -inf: the sums are 0)
+      hard *= exp2_ftz((m - to) * kLog2e);
       m = to;
     }
   }
@@ -87,34 +89,36 @@ struct Sums {
     for (int j = 0; j < kVec; ++j) top = max_bf16x2(max_bf16x2(max_bf16x2(top, u[j].x), max_bf16x2(u[j].y, u[j].z)), u[j].w);
     raise(fmaxf(lo(top), hi(top)), c);
     if (m > -INFINITY) {
-      const uint64_t neg_m = both(-m), cs = both(c), ch = both(kLog2e);
-      uint64_t ps[kVec] = {}, ph[kVec] = {};
+      const uint64_t neg_m = both(-m), cs = both(soft_exp ? c : kLog2e), ch = both(kLog2e);
+      float ps[4] = {}, ph[4] = {};
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint64_t d = add2(unpack2(w[i]), neg_m);
+          const int at = (i & 1) * 2;
           float a, b;
-          if (K & kSoft) {
-            split(mul2(d, cs), a, b);
-            ps[j] = add2(ps[j], f32x2(exp2_ftz(a), exp2_ftz(b)));
+          split(mul2(d, cs), a, b);
+          a = exp2_ftz(a);
+          b = exp2_ftz(b);
+          ps[at] += a;
+          ps[at + 1] += b;
+          if (squares) {
+            ph[at] = fmaf(a, a, ph[at]);
+            ph[at + 1] = fmaf(b, b, ph[at + 1]);
           }
-          if (K & kHard) {
+          if (K == kTwo) {
             split(mul2(d, ch), a, b);
-            ph[j] = add2(ph[j], f32x2(exp2_ftz(a), exp2_ftz(b)));
+            ph[at] += exp2_ftz(a);
+            ph[at + 1] += exp2_ftz(b);
           }
         }
       }
-      float a, b;
-      if (K & kSoft) {
-        split(add2(add2(ps[0], ps[1]), add2(ps[2], ps[3])), a, b);
-        soft += a + b;
-      }
-      if (K & kHard) {
-        split(add2(add2(ph[0], ph[1]), add2(ph[2], ph[3])), a, b);
-        hard += a + b;
-      }
+      const float p = (ps[0] + ps[1]) + (ps[2] + ps[3]);
+      if (soft_exp) soft += p;
+      else hard += p;
+      if (K == kTwo || squares) hard += (ph[0] + ph[1]) + (ph[2] + ph[3]);
     } else {
       // while everything seen is -inf nothing counts, except that a NaN has to show
 #pragma unroll
@@ -129,82 +133,109 @@ struct Sums {
       }
     }
   }
-  // Maximum and sums of the CTA, for every thread.  red: 3 * 32 floats.
-  __device__ __forceinline__ void block(float c, float* red) {
-    const int w = threadIdx.x >> 5, l = threadIdx.x & 31, nw = blockDim.x >> 5;
-    // (a warp of threads without an element has sums of 0, or NaN)
+  // Those of the warp's lanes, left in red (3 * 32 floats) by each warp / those of `warps` warps, for every thread that comes to read.
+  __device__ __forceinline__ void leave(float c, float* red) {
     const float mw = warp_max(m);
-    const float s = m == -INFINITY && mw > -INFINITY ? soft : soft * exp2_ftz((m - mw) * c);
-    const float h = m == -INFINITY && mw > -INFINITY ? hard : hard * exp2_ftz((m - mw) * kLog2e);
-    soft = warp_sum(mw == -INFINITY ? soft : s);
-    hard = warp_sum(mw == -INFINITY ? hard : h);
-    __syncthreads();
-    if (l == 0) { red[w] = mw; red[32 + w] = soft; red[64 + w] = hard; }
-    __syncthreads();
-    const float mine = l < nw ? red[l] : -INFINITY;
+    // (a thread that has seen nothing but -inf has sums of 0, or NaN)
+    const float fs = m == mw || m == -INFINITY ? 1.f : exp2_ftz((m - mw) * c), fh = m == mw || m == -INFINITY ? 1.f : exp2_ftz((m - mw) * kLog2e);
+    soft = warp_sum(soft * fs);
+    hard = warp_sum(hard * fh);
+    const int w = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) { red[w] = mw; red[32 + w] = soft; red[64 + w] = hard; }
+  }
+  __device__ __forceinline__ void join(float c, const float* red, int warps) {
+    const int l = threadIdx.x & 31;
+    const float mine = l < warps ? red[l] : -INFINITY;
     m = warp_max(mine);
-    soft = l < nw ? red[32 + l] : 0.f;
-    hard = l < nw ? red[64 + l] : 0.f;
-    if (mine > -INFINITY) {
-      soft *= exp2_ftz((mine - m) * c);
-      hard *= exp2_ftz((mine - m) * kLog2e);
-    }
-    soft = warp_sum(soft);
-    hard = warp_sum(hard);
+    const bool as_is = mine == m || mine == -INFINITY;
+    soft = warp_sum(l < warps ? red[32 + l] * (as_is ? 1.f : exp2_ftz((mine - m) * c)) : 0.f);
+    hard = warp_sum(l < warps ? red[64 + l] * (as_is ? 1.f : exp2_ftz((mine - m) * kLog2e)) : 0.f);
+    if (K == kSoft) hard = soft;             // T = 1, or the labels have no weight
+    if (K == kHard) soft = hard;
   }
 };
 
-// The teacher's entries of a row in shared memory: id - col_offset, or -1 for no entry; probability.  Entry `top` is the label.
+// The teacher's entries of a row in shared memory: the column of each (id in the vocabulary) and its probability.  Where a column has
+// several entries the first has their sum, in their order, and the others column -1; no entry has -1 too.  Entry `top` is the label's
+// column, with no probability of its own, unless an entry has it.
 struct Entries {
-  int* id;
+  int* at;
   float* p;
 };
 __host__ __device__ constexpr int entry_bytes(int top) { return (top + 1 + 3) / 4 * 4 * 8; }
 __device__ __forceinline__ Entries entries_at(void* at, int top) {
   Entries e;
-  e.id = reinterpret_cast<int*>(at);
-  e.p = reinterpret_cast<float*>(e.id + (top + 1 + 3) / 4 * 4);
+  e.at = reinterpret_cast<int*>(at);
+  e.p = reinterpret_cast<float*>(e.at + (top + 1 + 3) / 4 * 4);
   return e;
 }
 __device__ __forceinline__ float value_at(const DistillArgs& a, int64_t i) {
   return a.values_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.values)[i]) : reinterpret_cast<const float*>(a.values)[i];
 }
-// By one warp.  Returns whether the row has an entry of any weight, and sum p log p.
-__device__ __forceinline__ bool read_entries(const DistillArgs& a, int row, const Entries& e, float& plogp) {
+// By one warp, through `raw`.  Whether the row has an entry of any weight, its label's column or -1, and sum p log p.
+struct RowTarget {
+  bool some;
+  int label;
+  float plogp;
+};
+__device__ __forceinline__ RowTarget read_entries(const DistillArgs& a, int row, const Entries& raw, const Entries& e) {
   const int l = threadIdx.x & 31;
   const int64_t base = (int64_t)row * a.top;
   const float c = kLog2e / a.temperature;
+  RowTarget t;
+  const int64_t y = a.targets != nullptr ? a.targets[row] : -1;
+  t.label = y >= 0 && y < a.vocab ? (int)y : -1;
   float mx = -INFINITY;
   for (int k = l; k < a.top; k += 32) {
     const int64_t id = a.ids[base + k];
     const bool there = id >= 0 && id < a.vocab;
     const float v = there ? value_at(a, base + k) : -INFINITY;
-    e.id[k] = there ? (int)id : -1;
-    e.p[k] = v;
+    raw.at[k] = there ? (int)id : -1;
+    raw.p[k] = v;
     mx = v > mx || v != v ? v : mx;
   }
   mx = warp_max(mx);
   float sum = 0.f;
   for (int k = l; k < a.top; k += 32) {
-    const float x = e.p[k] == -INFINITY ? 0.f : exp2_ftz((e.p[k] - mx) * c);
+    const float x = raw.p[k] == -INFINITY ? 0.f : exp2_ftz((raw.p[k] - mx) * c);
     sum += x;
-    e.p[k] = x;
+    raw.p[k] = x;
   }
   sum = warp_sum(sum);
-  plogp = 0.f;
+  t.some = sum != 0.f;
+  t.plogp = 0.f;
   for (int k = l; k < a.top; k += 32) {
-    const float p = sum == 0.f ? 0.f : e.p[k] / sum;
-    if (p != 0.f) plogp += p * logf(p);
-    e.p[k] = p;
+    const float p = t.some ? raw.p[k] / sum : 0.f;
+    if (p != 0.f) t.plogp += p * logf(p);
+    raw.p[k] = p;
   }
-  plogp = warp_sum(plogp);
-  if (l == 0) {
-    const int64_t y = a.targets != nullptr ? a.targets[row] : -1;
-    e.id[a.top] = y >= 0 && y < a.vocab ? (int)y : -1;
-    e.p[a.top] = 0.f;
+  t.plogp = warp_sum(t.plogp);
+  if (l < 4 && a.top + l < (a.top + 4) / 4 * 4) {       // the label, and what pads to whole vectors
+    raw.at[a.top + l] = l == 0 ? t.label : -1;
+    raw.p[a.top + l] = 0.f;
   }
   __syncwarp();
-  return sum != 0.f;
+  const int4* quads = reinterpret_cast<const int4*>(raw.at);
+  for (int k = l; k <= a.top; k += 32) {
+    const int id = raw.at[k];
+    float p = raw.p[k];
+    bool first = id >= 0;
+    for (int q = 0; first && q < (a.top + 4) / 4; ++q) {
+      const int4 o = quads[q];
+      if (o.x != id && o.y != id && o.z != id && o.w != id) continue;
+      const int js[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int j = q * 4 + i;
+        if (js[i] == id && j < k) first = false;
+        if (js[i] == id && j > k) p += raw.p[j];
+      }
+    }
+    e.at[k] = first ? id : -1;
+    e.p[k] = p;
+  }
+  __syncwarp();
+  return t;
 }
 
 // What the gradient of a row is made of: soft * exp((z - m) / T) + hard * exp(z - m), less `drop` times an entry's probability and
@@ -219,35 +250,34 @@ __device__ __forceinline__ Weights weights_of(const DistillArgs& a, float m, flo
   w.label = label ? a.hard * a.scale : 0.f;
   w.soft = w.drop / soft;
   w.hard = w.label / hard;
+  if (a.temperature == 1.f) w.soft = w.hard = w.soft + w.hard;      // one kind of exponentials
   return w;
+}
+template <int K>
+__device__ __forceinline__ float grad_of(float soft_or_only, float hard, const Weights& w) {
+  if (K == kSoft) return soft_or_only * w.soft;
+  if (K == kHard) return soft_or_only * w.hard;
+  if (K == kSquare) return soft_or_only * fmaf(soft_or_only, w.hard, w.soft);
+  return fmaf(soft_or_only, w.soft, hard * w.hard);
 }
 template <int K>
 __device__ __forceinline__ uint32_t grad_pair(uint32_t z, const Weights& w, float c) {
   const uint64_t d = add2(unpack2(z), both(-w.m));
-  float a, b;
-  uint64_t g = 0;
-  if (K & kSoft) {
-    split(mul2(d, both(c)), a, b);
-    g = mul2(f32x2(exp2_ftz(a), exp2_ftz(b)), both(w.soft));
+  float a, b, x = 0.f, y = 0.f;
+  split(mul2(d, both(K == kHard ? kLog2e : c)), a, b);
+  if (K == kTwo) {
+    split(mul2(d, both(kLog2e)), x, y);
+    x = exp2_ftz(x);
+    y = exp2_ftz(y);
   }
-  if (K & kHard) {
-    split(mul2(d, both(kLog2e)), a, b);
-    g = fma2(f32x2(exp2_ftz(a), exp2_ftz(b)), both(w.hard), g);
-  }
-  split(g, a, b);
-  return pack(a, b);
+  return pack(grad_of<K>(exp2_ftz(a), x, w), grad_of<K>(exp2_ftz(b), y, w));
 }
 template <int K>
 __device__ __forceinline__ float grad_one(float z, const Weights& w, float c) {
-  float g = 0.f;
-  if (K & kSoft) g = exp2_ftz((z - w.m) * c) * w.soft;
-  if (K & kHard) g += exp2_ftz((z - w.m) * kLog2e) * w.hard;
-  return g;
+  return grad_of<K>(exp2_ftz((z - w.m) * (K == kHard ? kLog2e : c)), K == kTwo ? exp2_ftz((z - w.m) * kLog2e) : 0.f, w);
 }
 template <int K>
 __device__ __forceinline__ uint4 grad_vector(uint4 u, int v, int valid, const Weights& w, float c) {
-  // (rows that nothing is learnt from get zeros, whatever their logits are)
-  if (v * 8 >= valid || (w.drop == 0.f && w.label == 0.f)) return make_uint4(0u, 0u, 0u, 0u);
   const uint4 g = make_uint4(grad_pair<K>(u.x, w, c), grad_pair<K>(u.y, w, c), grad_pair<K>(u.z, w, c), grad_pair<K>(u.w, w, c));
   if (v * 8 + 8 <= valid) return g;
   uint32_t r[4] = {g.x, g.y, g.z, g.w};
@@ -255,91 +285,132 @@ __device__ __forceinline__ uint4 grad_vector(uint4 u, int v, int valid, const We
   for (int i = 0; i < 4; ++i) r[i] = v * 8 + 2 * i >= valid ? 0u : v * 8 + 2 * i + 1 >= valid ? r[i] & 0xffffu : r[i];
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
-// What entry k takes off its column's gradient; false where an earlier entry has the column (and takes it all).  In entry order.
-__device__ __forceinline__ bool entry_drop(const Entries& e, int top, int k, const Weights& w, float& drop) {
-  const int id = e.id[k];
-  if (id < 0) return false;
-  for (int j = 0; j < k; ++j)
-    if (e.id[j] == id) return false;
-  float p = 0.f;
-  for (int j = k; j < top; ++j)
-    if (e.id[j] == id) p += e.p[j];
-  drop = w.drop * p + (e.id[top] == id ? w.label : 0.f);
-  return true;
+// What an entry takes off its column's gradient.
+__device__ __forceinline__ float drop_of(const Weights& w, int at, float p, int label) {
+  return w.drop * p + (at == label ? w.label : 0.f);
 }
-// A row's loss by one warp, from z of its entries.
-template <class Z>
-__device__ __forceinline__ float loss_of(const DistillArgs& a, const Entries& e, float m, float soft, float hard, bool some, float plogp, Z z) {
-  float cross = 0.f;                       // sum p (z - m)
-  for (int k = threadIdx.x & 31; k < a.top; k += 32)
-    if (e.id[k] >= 0 && e.p[k] != 0.f) cross += e.p[k] * (z(e.id[k]) - m);
-  cross = warp_sum(cross);
+// A row's loss from its statistics: cross = sum p (z - m) over its entries, zy = z - m of its label.
+__device__ __forceinline__ float loss_of(const DistillArgs& a, const RowTarget& t, float soft, float hard, float cross, float zy) {
   float loss = 0.f;
-  if (some && a.hard != 1.f) loss = (1.f - a.hard) * a.temperature * (a.temperature * (plogp + logf(soft)) - cross);
-  if (e.id[a.top] >= 0 && a.hard != 0.f) loss += a.hard * (logf(hard) - (z(e.id[a.top]) - m));
+  if (t.some && a.hard != 1.f) loss = (1.f - a.hard) * a.temperature * (a.temperature * (t.plogp + logf(soft)) - cross);
+  if (t.label >= 0 && a.hard != 0.f) loss += a.hard * (logf(hard) - zy);
   return loss;
 }
 
-// Whole rows: a row waits in shared memory between the sums and the gradient, so the logits are read once.
+// The rows' barriers.
+enum { kSums = 1, kTaken = 2, kWritten = 3 };
+__device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+__device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_left(int left) {        // for all but the last `left` <= N groups
+  if (left == N) cp_async_wait<N>();
+  else if constexpr (N > 0) wait_left<N - 1>(left);
+}
+
+// Whole rows: a row waits in shared memory between the sums and the gradient, so the logits are read once.  Persistent CTAs: a thread
+// reads its own vectors in both passes, and as the gradient of one leaves, the same place takes that vector of the CTA's next row: loads
+// run under both passes.  A warp more, the clerk, reads the next row's entries meanwhile, takes their logits out of the row before it is
+// overwritten (kTaken), and writes their columns again once the row's gradient is written (kWritten).
+constexpr int kGroups = kRowBytes / (512 * kVec * 16) + 1;   // groups of vectors of a thread
 template <int K>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(544, 2)
 distill_row_kernel(const __grid_constant__ DistillArgs a) {
   extern __shared__ uint4 ring[];
-  __shared__ float red[96];
-  __shared__ int has;
-  const int T = blockDim.x, row = blockIdx.x, nvec = a.cols >> 3, valid = min(a.cols, a.vocab), nv = (valid + 7) >> 3;
+  __shared__ float red[2][96];
+  __shared__ int has[2], labels[2];
+  const int T = blockDim.x - 32, nvec = a.cols >> 3, valid = min(a.cols, a.vocab), nv = (valid + 7) >> 3;
   const float c = kLog2e / a.temperature;
-  const uint4* z = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld);
-  __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.grad) + (int64_t)row * a.ldg;
-  const Entries e = entries_at(ring + nv, a.top);
+  const __nv_bfloat16* kept = reinterpret_cast<const __nv_bfloat16*>(ring);
+  auto out_row = [&](int row) { return reinterpret_cast<__nv_bfloat16*>(a.grad) + (int64_t)row * a.ldg; };
   grid_trigger();
   grid_wait();
-  auto prefetch = [&](int v0) {
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const int v = v0 + j * T;
-      if (v < nv) cp_async16(ring + v, z + v);
+  int parity = 0;
+  if (threadIdx.x >= T) {
+    const int l = threadIdx.x & 31;
+    const Entries raw = entries_at(ring + nv, a.top);
+    uint8_t* buffers = reinterpret_cast<uint8_t*>(ring + nv) + entry_bytes(a.top);
+    auto rewrite = [&](int row, int buf) {
+      bar_sync(kWritten, T + 32);
+      const Entries e = entries_at(buffers + buf * entry_bytes(a.top), a.top);
+      __nv_bfloat16* out = out_row(row);
+      for (int k = l; k <= a.top; k += 32)
+        if (e.at[k] >= 0) out[e.at[k]] = __float2bfloat16(e.p[k]);
+    };
+    for (int row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+      const Entries e = entries_at(buffers + parity * entry_bytes(a.top), a.top);
+      const RowTarget t = read_entries(a, row, raw, e);
+      if (l == 0) {
+        has[parity] = t.some;
+        labels[parity] = t.label;
+      }
+      if (row != (int)blockIdx.x) rewrite(row - gridDim.x, parity ^ 1);
+      bar_sync(kSums, T + 32);
+      Sums<K> sum;
+      sum.join(c, red[parity], T >> 5);
+      const Weights w = weights_of(a, sum.m, sum.soft, sum.hard, t.some, t.label >= 0);
+      float cross = 0.f;
+      for (int k = l; k <= a.top; k += 32) {
+        const int at = e.at[k];
+        if (at < 0) continue;
+        const float z = __bfloat162float(kept[at]), p = e.p[k], drop = drop_of(w, at, p, t.label);
+        if (p != 0.f) cross += p * (z - sum.m);
+        if (drop == 0.f) e.at[k] = -1;                       // (its column is as the others)
+        else e.p[k] = grad_one<K>(z, w, c) - drop;
+      }
+      const float zy = t.label >= 0 ? __bfloat162float(kept[t.label]) - sum.m : 0.f;
+      __syncwarp();
+      bar_arrive(kTaken, T + 32);
+      cross = warp_sum(cross);
+      if (l == 0) a.loss[row] = loss_of(a, t, sum.soft, sum.hard, cross, zy);
     }
+    const int rows = (a.rows - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
+    rewrite(blockIdx.x + (rows - 1) * gridDim.x, parity ^ 1);
+    return;
+  }
+  const int groups = (nv + T * kVec - 1) / (T * kVec);
+  auto logits_row = [&](int row) {
+    return reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld);
+  };
+  auto fetch = [&](const uint4* z, int v0) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+      if (v0 + j * T < nv) cp_async16(ring + v0 + j * T, z + v0 + j * T);
     cp_async_commit();
   };
+  for (int g = 0; g < groups; ++g) fetch(logits_row(blockIdx.x), threadIdx.x + g * T * kVec);
+  for (int row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
+    Sums<K> sum;
+    for (int g = 0; g < groups; ++g) {
+      wait_left<kGroups>(groups - 1 - g);
+      uint4 u[kVec];
 #pragma unroll
-  for (int i = 0; i < kAhead; ++i) prefetch(threadIdx.x + i * T * kVec);
-  float plogp = 0.f;
-  if (threadIdx.x < 32) {
-    const bool some = read_entries(a, row, e, plogp);
-    if (threadIdx.x == 0) has = some;
-  }
-  Sums<K> sum;
-  for (int v0 = threadIdx.x; v0 < nv; v0 += T * kVec) {
-    prefetch(v0 + kAhead * T * kVec);
-    cp_async_wait<kAhead>();
-    uint4 u[kVec];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const int v = v0 + j * T;
-      u[j] = v < nv ? cut(ring[v], v, valid) : make_uint4(kNegInf2, kNegInf2, kNegInf2, kNegInf2);
+      for (int j = 0; j < kVec; ++j) {
+        const int v = threadIdx.x + (g * kVec + j) * T;
+        u[j] = v < nv ? cut(ring[v], v, valid) : make_uint4(kNegInf2, kNegInf2, kNegInf2, kNegInf2);
+      }
+      sum.add(u, c);
     }
-    sum.add(u, c);
-  }
-  cp_async_wait<0>();
-  sum.block(c, red);                       // (its barriers make the row and its entries visible to every thread)
-  if (K == kSoft) sum.hard = sum.soft;     // T = 1, or nothing of weight
-  if (K == kHard) sum.soft = sum.hard;
-  const bool some = has != 0;
-  Weights w = weights_of(a, sum.m, sum.soft, sum.hard, some, e.id[a.top] >= 0);
-  if (K == kSoft) w.soft += a.temperature == 1.f ? w.hard : 0.f;
-  const __nv_bfloat16* kept = reinterpret_cast<const __nv_bfloat16*>(ring);
-  for (int v = threadIdx.x; v < nvec; v += T)
-    reinterpret_cast<uint4*>(out)[v] = grad_vector<K>(v < nv ? ring[v] : make_uint4(0u, 0u, 0u, 0u), v, valid, w, c);
-  if (threadIdx.x < 32) {
-    const float loss = loss_of(a, e, sum.m, sum.soft, sum.hard, some, plogp, [&](int id) { return __bfloat162float(kept[id]); });
-    if (threadIdx.x == 0) a.loss[row] = loss;
-  }
-  __syncthreads();                         // the row's gradient is written: its entries' columns are written again
-  for (int k = threadIdx.x; k <= a.top; k += T) {
-    float drop;
-    if (entry_drop(e, a.top, k, w, drop) && drop != 0.f)
-      out[e.id[k]] = __float2bfloat16(grad_one<K>(__bfloat162float(kept[e.id[k]]), w, c) - drop);
+    sum.leave(c, red[parity]);
+    bar_sync(kSums, T + 32);
+    sum.join(c, red[parity], T >> 5);
+    const Weights w = weights_of(a, sum.m, sum.soft, sum.hard, has[parity] != 0, labels[parity] >= 0);
+    // (rows that nothing is learnt from get zeros, whatever their logits are)
+    const int learnt = w.drop == 0.f && w.label == 0.f ? 0 : nv;
+    const bool more = row + (int)gridDim.x < a.rows;
+    const uint4* next = logits_row(row + gridDim.x);
+    uint4* out = reinterpret_cast<uint4*>(out_row(row));
+    bar_sync(kTaken, T + 32);
+    for (int g = 0; g < groups; ++g) {
+      const int v0 = threadIdx.x + g * kVec * T;
+#pragma unroll
+      for (int j = 0; j < kVec; ++j) {
+        const int v = v0 + j * T;
+        if (v < nv) out[v] = v < learnt ? grad_vector<K>(ring[v], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+      }
+      if (more) fetch(next, v0);
+    }
+    for (int v = nv + threadIdx.x; v < nvec; v += T) out[v] = make_uint4(0u, 0u, 0u, 0u);
+    bar_arrive(kWritten, T + 32);
   }
 }
 
@@ -352,11 +423,8 @@ distill_partial_kernel(const __grid_constant__ DistillArgs a) {
   const float c = kLog2e / a.temperature;
   const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld;
   const uint4* zv = reinterpret_cast<const uint4*>(z);
-  const Entries e = entries_at(ring, a.top);
   grid_trigger();
   grid_wait();
-  float plogp = 0.f;
-  if (threadIdx.x < 32) read_entries(a, row, e, plogp);
   Sums<kTwo> sum;
   for (int v0 = threadIdx.x; v0 < nv; v0 += T * kVec) {
     uint4 u[kVec];
@@ -367,22 +435,26 @@ distill_partial_kernel(const __grid_constant__ DistillArgs a) {
     }
     sum.add(u, c);
   }
-  sum.block(c, red);
+  sum.leave(c, red);
+  __syncthreads();
   if (threadIdx.x < 32) {
+    sum.join(c, red, T >> 5);
+    const Entries raw = entries_at(ring, a.top), e = entries_at(reinterpret_cast<uint8_t*>(ring) + entry_bytes(a.top), a.top);
+    const RowTarget t = read_entries(a, row, raw, e);
     float dot = 0.f;
-    for (int k = threadIdx.x; k < a.top; k += 32) {
-      const int id = e.id[k] - a.col_offset;
-      if (e.id[k] >= 0 && id >= 0 && id < valid && e.p[k] != 0.f) dot += e.p[k] * __bfloat162float(z[id]);
+    for (int k = threadIdx.x; k <= a.top; k += 32) {
+      const int at = e.at[k] - a.col_offset;
+      if (e.at[k] >= 0 && at >= 0 && at < valid && e.p[k] != 0.f) dot += e.p[k] * __bfloat162float(z[at]);
     }
     dot = warp_sum(dot);
     if (threadIdx.x == 0) {
-      const int y = e.id[a.top] - a.col_offset;
+      const int y = t.label - a.col_offset;
       float* s = a.stats + (int64_t)row * 5;
       s[0] = sum.m;
       s[1] = sum.hard;
       s[2] = sum.soft;
       s[3] = dot;
-      s[4] = e.id[a.top] >= 0 && y >= 0 && y < valid ? __bfloat162float(z[y]) : 0.f;
+      s[4] = t.label >= 0 && y >= 0 && y < valid ? __bfloat162float(z[y]) : 0.f;
     }
   }
 }
@@ -392,57 +464,51 @@ template <int K>
 __global__ void __launch_bounds__(512)
 distill_grad_kernel(const __grid_constant__ DistillArgs a) {
   extern __shared__ uint4 ring[];
-  __shared__ int has;
+  __shared__ RowTarget target;
   const int T = blockDim.x, row = blockIdx.x, nvec = a.cols >> 3, valid = max(0, min(a.cols, a.vocab - a.col_offset));
   const float c = kLog2e / a.temperature;
   const __nv_bfloat16* z = reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(a.grad) + (int64_t)row * a.ldg;
-  const Entries e = entries_at(ring, a.top);
-  float* ze = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(ring) + entry_bytes(a.top));   // z of the entries in this slice
+  const Entries raw = entries_at(ring, a.top), e = entries_at(reinterpret_cast<uint8_t*>(ring) + entry_bytes(a.top), a.top);
   grid_trigger();
   grid_wait();
   const float* s = a.stats + (int64_t)row * 5;
   const float m = s[0], hard = s[1], soft = s[2];
   if (threadIdx.x < 32) {
-    float plogp;
-    const bool some = read_entries(a, row, e, plogp);
+    const RowTarget t = read_entries(a, row, raw, e);
     float total = 0.f;
-    for (int k = threadIdx.x; k < a.top; k += 32) total += e.p[k];
+    for (int k = threadIdx.x; k <= a.top; k += 32) total += e.at[k] >= 0 ? e.p[k] : 0.f;
     total = warp_sum(total);
     if (threadIdx.x == 0) {
-      has = some;
-      if (a.loss != nullptr) {
-        float loss = 0.f;
-        if (some && a.hard != 1.f) loss = (1.f - a.hard) * a.temperature * (a.temperature * (plogp + logf(soft)) - (s[3] - total * m));
-        if (e.id[a.top] >= 0 && a.hard != 0.f) loss += a.hard * (logf(hard) - (s[4] - m));
-        a.loss[row] = loss;
-      }
+      target = t;
+      if (a.loss != nullptr) a.loss[row] = loss_of(a, t, soft, hard, s[3] - total * m, s[4] - m);
     }
   }
   __syncthreads();
+  const Weights w = weights_of(a, m, soft, hard, target.some, target.label >= 0);
   for (int k = threadIdx.x; k <= a.top; k += T) {          // before the gradient may overwrite the logits
-    const int id = e.id[k] - a.col_offset;
-    ze[k] = e.id[k] >= 0 && id >= 0 && id < valid ? __bfloat162float(z[id]) : 0.f;
+    const int at = e.at[k] - a.col_offset;
+    const bool here = e.at[k] >= 0 && at >= 0 && at < valid;
+    const float drop = here ? drop_of(w, e.at[k], e.p[k], target.label) : 0.f;
+    if (drop != 0.f) e.p[k] = grad_one<K>(__bfloat162float(z[at]), w, c) - drop;
+    else e.at[k] = -1;
   }
   __syncthreads();
-  Weights w = weights_of(a, m, soft, hard, has != 0, e.id[a.top] >= 0);
-  if (K == kSoft) w.soft += a.temperature == 1.f ? w.hard : 0.f;
+  const int learnt = w.drop == 0.f && w.label == 0.f ? 0 : (valid + 7) >> 3;
   for (int v0 = threadIdx.x; v0 < nvec; v0 += T * kVec) {
     uint4 u[kVec];
 #pragma unroll
     for (int j = 0; j < kVec; ++j)
-      if (v0 + j * T < nvec) u[j] = reinterpret_cast<const uint4*>(z)[v0 + j * T];
+      if (v0 + j * T < learnt) u[j] = reinterpret_cast<const uint4*>(z)[v0 + j * T];
 #pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (v0 + j * T < nvec) reinterpret_cast<uint4*>(out)[v0 + j * T] = grad_vector<K>(u[j], v0 + j * T, valid, w, c);
+    for (int j = 0; j < kVec; ++j) {
+      const int v = v0 + j * T;
+      if (v < nvec) reinterpret_cast<uint4*>(out)[v] = v < learnt ? grad_vector<K>(u[j], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+    }
   }
   __syncthreads();
-  for (int k = threadIdx.x; k <= a.top; k += T) {
-    const int id = e.id[k] - a.col_offset;
-    float drop;
-    if (e.id[k] >= 0 && id >= 0 && id < valid && entry_drop(e, a.top, k, w, drop) && drop != 0.f)
-      out[id] = __float2bfloat16(grad_one<K>(ze[k], w, c) - drop);
-  }
+  for (int k = threadIdx.x; k <= a.top; k += T)
+    if (e.at[k] >= 0) out[e.at[k] - a.col_offset] = __float2bfloat16(e.p[k]);
 }
 
 cudaError_t check(const DistillArgs& a) {
@@ -458,7 +524,7 @@ cudaError_t check_grad(const DistillArgs& a) {
 }
 int kind_of(const DistillArgs& a) {
   if (a.hard == 0.f || a.temperature == 1.f) return kSoft;
-  return a.hard == 1.f ? kHard : kTwo;
+  return a.hard == 1.f ? kHard : a.temperature == 2.f ? kSquare : kTwo;
 }
 template <class Kernel>
 cudaError_t allow(Kernel kernel, int bytes) {
@@ -475,23 +541,31 @@ cudaError_t distill_row(const DistillArgs& a, cudaStream_t stream) {
   const int valid = a.cols < a.vocab ? a.cols : a.vocab, nv = (valid + 7) / 8;
   if (e != cudaSuccess) return e;
   if (valid > distill_row_cols() || a.col_offset != 0 || a.cols < a.vocab) return cudaErrorInvalidValue;
-  const int smem = nv * 16 + entry_bytes(a.top), kind = kind_of(a);
-  auto kernel = kind == kSoft ? distill_row_kernel<kSoft> : kind == kHard ? distill_row_kernel<kHard> : distill_row_kernel<kTwo>;
+  const int smem = nv * 16 + 3 * entry_bytes(a.top), kind = kind_of(a);
+  auto kernel = kind == kSoft ? distill_row_kernel<kSoft> : kind == kHard ? distill_row_kernel<kHard>
+              : kind == kSquare ? distill_row_kernel<kSquare> : distill_row_kernel<kTwo>;
   e = allow(kernel, smem);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kernel, a.rows, nv > 2048 ? 512 : 256, smem, stream, a);
+  // As many CTAs as are resident at a time: by shared memory (228 KiB, 2 KiB a CTA beside the row) and registers (56 a thread).
+  // Sixteen warps a row where no more than two rows fit, else eight.
+  int sms = 148, dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+  const int fit = 228 * 1024 / (smem + 2048), threads = (fit > 2 ? 256 : 512) + 32, by_registers = 65536 / (56 * threads);
+  const int64_t most = (int64_t)sms * (fit < 1 ? 1 : fit < by_registers ? fit : by_registers);
+  return launch_dependent(kernel, (unsigned)(a.rows < most ? a.rows : most), threads, smem, stream, a);
 }
 cudaError_t distill_partial(const DistillArgs& a, cudaStream_t stream) {
   const cudaError_t e = check(a);
   if (e != cudaSuccess) return e;
-  return launch_dependent(distill_partial_kernel, a.rows, 512, entry_bytes(a.top), stream, a);
+  return launch_dependent(distill_partial_kernel, a.rows, 512, 2 * entry_bytes(a.top), stream, a);
 }
 cudaError_t distill_grad(const DistillArgs& a, cudaStream_t stream) {
   const cudaError_t e = check_grad(a);
   if (e != cudaSuccess) return e;
   const int kind = kind_of(a);
-  auto kernel = kind == kSoft ? distill_grad_kernel<kSoft> : kind == kHard ? distill_grad_kernel<kHard> : distill_grad_kernel<kTwo>;
-  return launch_dependent(kernel, a.rows, 512, entry_bytes(a.top) + 4 * (a.top + 1), stream, a);
+  auto kernel = kind == kSoft ? distill_grad_kernel<kSoft> : kind == kHard ? distill_grad_kernel<kHard>
+              : kind == kSquare ? distill_grad_kernel<kSquare> : distill_grad_kernel<kTwo>;
+  return launch_dependent(kernel, a.rows, 512, 2 * entry_bytes(a.top), stream, a);
 }
 
 }  // namespace msb
