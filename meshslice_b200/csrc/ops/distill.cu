@@ -12,6 +12,7 @@ namespace msb {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr uint32_t kNegInf2 = 0xff80ff80u;       // two bf16 -inf
 constexpr int kVec = 4;                          // vectors of a thread that are worked on together
 constexpr int kRowBytes = 200 * 1024;            // most of a row that is kept
@@ -70,36 +71,47 @@ __device__ __forceinline__ uint4 cut(uint4 u, int v, int valid) {
 // 4096 rows of 50257 (148 SMs), two 90.
 enum Kind { kSoft = 1, kHard = 2, kTwo = 3, kSquare = 5 };
 
-// A thread's running maximum m, and sums of exp(z - m) and exp((z - m) / T).  Differences are taken first: they are exact where they
-// matter, and a rounded m / T would shift the whole row.  (Behind the exponentials scalar sums: packing their results takes moves.)
+// 2^x exponents of z over a temperature: z c - m c with the product z c exact (one rounding, of the result) and m c rounded once for
+// the whole row: `ref`, the same wherever m is.  Sums are relative to 2^ref; that ref is not quite m c cancels in every ratio, and the
+// loss takes ref itself.
+__device__ __forceinline__ float ref_of(float m, float c) { return __fmul_rn(m, c); }
+
+// A thread's running maximum m, and sums of exp(z) and exp(z / T) relative to it.  (Behind the exponentials scalar sums: packing their
+// results takes moves.)
 template <int K>
 struct Sums {
-  static constexpr bool soft_exp = K & kSoft, hard_exp = K == kHard || K == kTwo, squares = K == kSquare;
+  static constexpr bool soft_exp = K & kSoft, squares = K == kSquare;
   float m = -INFINITY, soft = 0.f, hard = 0.f;
+  // What the sums are relative to; where T = 2 the hard one's is twice the soft one's.
+  __device__ __forceinline__ float soft_ref(float c) const { return ref_of(m, c); }
+  __device__ __forceinline__ float hard_ref(float c) const { return squares ? 2.f * ref_of(m, c) : ref_of(m, kLog2e); }
   __device__ __forceinline__ void raise(float to, float c) {
     if (to > m) {
-      soft *= exp2_ftz((m - to) * c);                     // (0 while m is -inf: the sums are 0)
-      hard *= exp2_ftz((m - to) * kLog2e);
+      const float s0 = soft_ref(c), h0 = hard_ref(c);
       m = to;
+      soft *= exp2_ftz(s0 - soft_ref(c));                 // (0 while m is -inf: the sums are 0)
+      hard *= exp2_ftz(h0 - hard_ref(c));
     }
   }
-  __device__ __forceinline__ void add(const uint4 (&u)[kVec], float c) {
+  template <int N>
+  __device__ __forceinline__ void add(const uint4 (&u)[N], float c) {
     uint32_t top = kNegInf2;
 #pragma unroll
-    for (int j = 0; j < kVec; ++j) top = max_bf16x2(max_bf16x2(max_bf16x2(top, u[j].x), max_bf16x2(u[j].y, u[j].z)), u[j].w);
+    for (int j = 0; j < N; ++j) top = max_bf16x2(max_bf16x2(max_bf16x2(top, u[j].x), max_bf16x2(u[j].y, u[j].z)), u[j].w);
     raise(fmaxf(lo(top), hi(top)), c);
     if (m > -INFINITY) {
-      const uint64_t neg_m = both(-m), cs = both(soft_exp ? c : kLog2e), ch = both(kLog2e);
+      const float c0 = soft_exp ? c : kLog2e;
+      const uint64_t cs = both(c0), rs = both(-ref_of(m, c0)), ch = both(kLog2e), rh = both(-ref_of(m, kLog2e));
       float ps[4] = {}, ph[4] = {};
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
+      for (int j = 0; j < N; ++j) {
         const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint64_t d = add2(unpack2(w[i]), neg_m);
+          const uint64_t z = unpack2(w[i]);
           const int at = (i & 1) * 2;
           float a, b;
-          split(mul2(d, cs), a, b);
+          split(fma2(z, cs, rs), a, b);
           a = exp2_ftz(a);
           b = exp2_ftz(b);
           ps[at] += a;
@@ -109,7 +121,7 @@ struct Sums {
             ph[at + 1] = fmaf(b, b, ph[at + 1]);
           }
           if (K == kTwo) {
-            split(mul2(d, ch), a, b);
+            split(fma2(z, ch, rh), a, b);
             ph[at] += exp2_ftz(a);
             ph[at + 1] += exp2_ftz(b);
           }
@@ -122,7 +134,7 @@ struct Sums {
     } else {
       // while everything seen is -inf nothing counts, except that a NaN has to show
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
+      for (int j = 0; j < N; ++j) {
         const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -135,21 +147,23 @@ struct Sums {
   }
   // Those of the warp's lanes, left in red (3 * 32 floats) by each warp / those of `warps` warps, for every thread that comes to read.
   __device__ __forceinline__ void leave(float c, float* red) {
-    const float mw = warp_max(m);
+    const float s0 = soft_ref(c), h0 = hard_ref(c), mine = m;
+    m = warp_max(m);
     // (a thread that has seen nothing but -inf has sums of 0, or NaN)
-    const float fs = m == mw || m == -INFINITY ? 1.f : exp2_ftz((m - mw) * c), fh = m == mw || m == -INFINITY ? 1.f : exp2_ftz((m - mw) * kLog2e);
-    soft = warp_sum(soft * fs);
-    hard = warp_sum(hard * fh);
+    const bool as_is = mine == m || mine == -INFINITY;
+    soft = warp_sum(as_is ? soft : soft * exp2_ftz(s0 - soft_ref(c)));
+    hard = warp_sum(as_is ? hard : hard * exp2_ftz(h0 - hard_ref(c)));
     const int w = threadIdx.x >> 5;
-    if ((threadIdx.x & 31) == 0) { red[w] = mw; red[32 + w] = soft; red[64 + w] = hard; }
+    if ((threadIdx.x & 31) == 0) { red[w] = m; red[32 + w] = soft; red[64 + w] = hard; }
   }
   __device__ __forceinline__ void join(float c, const float* red, int warps) {
     const int l = threadIdx.x & 31;
-    const float mine = l < warps ? red[l] : -INFINITY;
-    m = warp_max(mine);
+    m = l < warps ? red[l] : -INFINITY;
+    const float s0 = soft_ref(c), h0 = hard_ref(c), mine = m;
+    m = warp_max(m);
     const bool as_is = mine == m || mine == -INFINITY;
-    soft = warp_sum(l < warps ? red[32 + l] * (as_is ? 1.f : exp2_ftz((mine - m) * c)) : 0.f);
-    hard = warp_sum(l < warps ? red[64 + l] * (as_is ? 1.f : exp2_ftz((mine - m) * kLog2e)) : 0.f);
+    soft = warp_sum(l < warps ? red[32 + l] * (as_is ? 1.f : exp2_ftz(s0 - soft_ref(c))) : 0.f);
+    hard = warp_sum(l < warps ? red[64 + l] * (as_is ? 1.f : exp2_ftz(h0 - hard_ref(c))) : 0.f);
     if (K == kSoft) hard = soft;             // T = 1, or the labels have no weight
     if (K == kHard) soft = hard;
   }
@@ -172,42 +186,108 @@ __device__ __forceinline__ Entries entries_at(void* at, int top) {
 __device__ __forceinline__ float value_at(const DistillArgs& a, int64_t i) {
   return a.values_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.values)[i]) : reinterpret_cast<const float*>(a.values)[i];
 }
-// By one warp, through `raw`.  Whether the row has an entry of any weight, its label's column or -1, and sum p log p.
+// Whether a row has an entry of any weight, its label's column or -1, and sum p log p.
 struct RowTarget {
   bool some;
   int label;
   float plogp;
 };
-__device__ __forceinline__ RowTarget read_entries(const DistillArgs& a, int row, const Entries& raw, const Entries& e) {
+// What a lane has of a row on its way from memory: entries lane + 32 j, all of them where the teacher kept no more than 32 kHeld.
+constexpr int kHeld = 4;
+struct Held {
+  int64_t id[kHeld], label;
+  float value[kHeld];
+};
+__device__ __forceinline__ Held hold(const DistillArgs& a, int row) {
   const int l = threadIdx.x & 31;
   const int64_t base = (int64_t)row * a.top;
+  Held h;
+  h.label = a.targets != nullptr ? a.targets[row] : -1;
+  if (a.top <= 32 * kHeld) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const int k = l + 32 * j;
+      h.id[j] = k < a.top ? a.ids[base + k] : -1;
+      h.value[j] = k < a.top ? value_at(a, base + k) : -INFINITY;
+    }
+  }
+  return h;
+}
+// Entry k of a row whose ids are in raw: the first of its column?  Adds what later ones of the column have.
+__device__ __forceinline__ bool first_of(const Entries& raw, int top, int k, float& p) {
+  const int id = raw.at[k];
+  if (id < 0) return false;
+  const int4* quads = reinterpret_cast<const int4*>(raw.at);
+  int same = 0;
+#pragma unroll 4
+  for (int q = 0; q < (top + 4) / 4; ++q) {
+    const int4 o = quads[q];
+    same += (o.x == id) + (o.y == id) + (o.z == id) + (o.w == id);
+  }
+  if (same == 1) return true;
+  for (int j = 0; j <= top; ++j) {
+    if (raw.at[j] != id || j == k) continue;
+    if (j < k) return false;
+    p += raw.p[j];
+  }
+  return true;
+}
+// By one warp: the entries of `row` (h: what is held of it), through `raw`.
+__device__ __forceinline__ RowTarget read_entries(const DistillArgs& a, int row, const Held& h, const Entries& raw, const Entries& e) {
+  const int l = threadIdx.x & 31;
   const float c = kLog2e / a.temperature;
   RowTarget t;
-  const int64_t y = a.targets != nullptr ? a.targets[row] : -1;
-  t.label = y >= 0 && y < a.vocab ? (int)y : -1;
-  float mx = -INFINITY;
-  for (int k = l; k < a.top; k += 32) {
-    const int64_t id = a.ids[base + k];
-    const bool there = id >= 0 && id < a.vocab;
-    const float v = there ? value_at(a, base + k) : -INFINITY;
-    raw.at[k] = there ? (int)id : -1;
-    raw.p[k] = v;
-    mx = v > mx || v != v ? v : mx;
-  }
-  mx = warp_max(mx);
-  float sum = 0.f;
-  for (int k = l; k < a.top; k += 32) {
-    const float x = raw.p[k] == -INFINITY ? 0.f : exp2_ftz((raw.p[k] - mx) * c);
-    sum += x;
-    raw.p[k] = x;
-  }
-  sum = warp_sum(sum);
-  t.some = sum != 0.f;
+  t.label = h.label >= 0 && h.label < a.vocab ? (int)h.label : -1;
   t.plogp = 0.f;
-  for (int k = l; k < a.top; k += 32) {
-    const float p = t.some ? raw.p[k] / sum : 0.f;
-    if (p != 0.f) t.plogp += p * logf(p);
-    raw.p[k] = p;
+  float mx = -INFINITY, sum = 0.f;
+  if (a.top <= 32 * kHeld) {
+    float p[kHeld];
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      p[j] = h.id[j] >= 0 && h.id[j] < a.vocab ? h.value[j] : -INFINITY;
+      mx = p[j] > mx || p[j] != p[j] ? p[j] : mx;
+    }
+    mx = warp_max(mx);
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      p[j] = p[j] == -INFINITY ? 0.f : exp2_ftz((p[j] - mx) * c);
+      sum += p[j];
+    }
+    sum = warp_sum(sum);
+    t.some = sum != 0.f;
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j) {
+      const int k = l + 32 * j;
+      if (j * 32 > a.top) break;
+      p[j] = t.some ? p[j] / sum : 0.f;
+      if (p[j] != 0.f) t.plogp += p[j] * logf(p[j]);
+      if (k < a.top) {
+        raw.at[k] = h.id[j] >= 0 && h.id[j] < a.vocab ? (int)h.id[j] : -1;
+        raw.p[k] = p[j];
+      }
+    }
+  } else {
+    const int64_t base = (int64_t)row * a.top;
+    for (int k = l; k < a.top; k += 32) {
+      const int64_t id = a.ids[base + k];
+      const float v = value_at(a, base + k), x = id >= 0 && id < a.vocab ? v : -INFINITY;
+      raw.at[k] = id >= 0 && id < a.vocab ? (int)id : -1;
+      raw.p[k] = x;
+      mx = x > mx || x != x ? x : mx;
+    }
+    mx = warp_max(mx);
+    for (int k = l; k < a.top; k += 32) {
+      const float x = raw.p[k] == -INFINITY ? 0.f : exp2_ftz((raw.p[k] - mx) * c);
+      sum += x;
+      raw.p[k] = x;
+    }
+    sum = warp_sum(sum);
+    t.some = sum != 0.f;
+    for (int k = l; k < a.top; k += 32) {
+      const float p = t.some ? raw.p[k] / sum : 0.f;
+      if (p != 0.f) t.plogp += p * logf(p);
+      raw.p[k] = p;
+    }
   }
   t.plogp = warp_sum(t.plogp);
   if (l < 4 && a.top + l < (a.top + 4) / 4 * 4) {       // the label, and what pads to whole vectors
@@ -215,58 +295,45 @@ __device__ __forceinline__ RowTarget read_entries(const DistillArgs& a, int row,
     raw.p[a.top + l] = 0.f;
   }
   __syncwarp();
-  const int4* quads = reinterpret_cast<const int4*>(raw.at);
   for (int k = l; k <= a.top; k += 32) {
-    const int id = raw.at[k];
     float p = raw.p[k];
-    bool first = id >= 0;
-    for (int q = 0; first && q < (a.top + 4) / 4; ++q) {
-      const int4 o = quads[q];
-      if (o.x != id && o.y != id && o.z != id && o.w != id) continue;
-      const int js[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int j = q * 4 + i;
-        if (js[i] == id && j < k) first = false;
-        if (js[i] == id && j > k) p += raw.p[j];
-      }
-    }
-    e.at[k] = first ? id : -1;
+    e.at[k] = first_of(raw, a.top, k, p) ? raw.at[k] : -1;
     e.p[k] = p;
   }
   __syncwarp();
   return t;
 }
 
-// What the gradient of a row is made of: soft * exp((z - m) / T) + hard * exp(z - m), less `drop` times an entry's probability and
-// `label` at the label.
+// What the gradient of a row is made of: soft * 2^(z c - ref) + hard * 2^(z log2(e) - hard_ref), less `drop` times an entry's
+// probability and `label` at the label.  From sums relative to the same references.
 struct Weights {
-  float m, soft, hard, drop, label;
+  float ref, hard_ref, soft, hard, drop, label;
 };
+template <int K>
 __device__ __forceinline__ Weights weights_of(const DistillArgs& a, float m, float soft, float hard, bool some, bool label) {
   Weights w;
-  w.m = m;
+  w.ref = ref_of(m, K == kHard ? kLog2e : kLog2e / a.temperature);
+  w.hard_ref = ref_of(m, kLog2e);
   w.drop = some ? (1.f - a.hard) * a.temperature * a.scale : 0.f;
   w.label = label ? a.hard * a.scale : 0.f;
   w.soft = w.drop / soft;
   w.hard = w.label / hard;
-  if (a.temperature == 1.f) w.soft = w.hard = w.soft + w.hard;      // one kind of exponentials
+  if (K == kSoft) w.soft = a.temperature == 1.f ? w.soft + w.hard : w.soft;      // one kind of exponentials
   return w;
 }
 template <int K>
-__device__ __forceinline__ float grad_of(float soft_or_only, float hard, const Weights& w) {
-  if (K == kSoft) return soft_or_only * w.soft;
-  if (K == kHard) return soft_or_only * w.hard;
-  if (K == kSquare) return soft_or_only * fmaf(soft_or_only, w.hard, w.soft);
-  return fmaf(soft_or_only, w.soft, hard * w.hard);
+__device__ __forceinline__ float grad_of(float e, float hard, const Weights& w) {
+  if (K == kSoft) return e * w.soft;
+  if (K == kHard) return e * w.hard;
+  if (K == kSquare) return e * fmaf(e, w.hard, w.soft);
+  return fmaf(e, w.soft, hard * w.hard);
 }
 template <int K>
 __device__ __forceinline__ uint32_t grad_pair(uint32_t z, const Weights& w, float c) {
-  const uint64_t d = add2(unpack2(z), both(-w.m));
   float a, b, x = 0.f, y = 0.f;
-  split(mul2(d, both(K == kHard ? kLog2e : c)), a, b);
+  split(fma2(unpack2(z), both(K == kHard ? kLog2e : c), both(-w.ref)), a, b);
   if (K == kTwo) {
-    split(mul2(d, both(kLog2e)), x, y);
+    split(fma2(unpack2(z), both(kLog2e), both(-w.hard_ref)), x, y);
     x = exp2_ftz(x);
     y = exp2_ftz(y);
   }
@@ -274,11 +341,15 @@ __device__ __forceinline__ uint32_t grad_pair(uint32_t z, const Weights& w, floa
 }
 template <int K>
 __device__ __forceinline__ float grad_one(float z, const Weights& w, float c) {
-  return grad_of<K>(exp2_ftz((z - w.m) * (K == kHard ? kLog2e : c)), K == kTwo ? exp2_ftz((z - w.m) * kLog2e) : 0.f, w);
+  return grad_of<K>(exp2_ftz(fmaf(z, K == kHard ? kLog2e : c, -w.ref)), K == kTwo ? exp2_ftz(fmaf(z, kLog2e, -w.hard_ref)) : 0.f, w);
+}
+template <int K>
+__device__ __forceinline__ uint4 grad_whole(uint4 u, const Weights& w, float c) {
+  return make_uint4(grad_pair<K>(u.x, w, c), grad_pair<K>(u.y, w, c), grad_pair<K>(u.z, w, c), grad_pair<K>(u.w, w, c));
 }
 template <int K>
 __device__ __forceinline__ uint4 grad_vector(uint4 u, int v, int valid, const Weights& w, float c) {
-  const uint4 g = make_uint4(grad_pair<K>(u.x, w, c), grad_pair<K>(u.y, w, c), grad_pair<K>(u.z, w, c), grad_pair<K>(u.w, w, c));
+  const uint4 g = grad_whole<K>(u, w, c);
   if (v * 8 + 8 <= valid) return g;
   uint32_t r[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
@@ -289,10 +360,11 @@ __device__ __forceinline__ uint4 grad_vector(uint4 u, int v, int valid, const We
 __device__ __forceinline__ float drop_of(const Weights& w, int at, float p, int label) {
   return w.drop * p + (at == label ? w.label : 0.f);
 }
-// A row's loss from its statistics: cross = sum p (z - m) over its entries, zy = z - m of its label.
-__device__ __forceinline__ float loss_of(const DistillArgs& a, const RowTarget& t, float soft, float hard, float cross, float zy) {
+// A row's loss: cross = sum p (z / T - r) over its entries and their sum `total`, zy = z - h of its label, where r and h are what the
+// sums are relative to.
+__device__ __forceinline__ float loss_of(const DistillArgs& a, const RowTarget& t, float soft, float hard, float cross, float total, float zy) {
   float loss = 0.f;
-  if (t.some && a.hard != 1.f) loss = (1.f - a.hard) * a.temperature * (a.temperature * (t.plogp + logf(soft)) - cross);
+  if (t.some && a.hard != 1.f) loss = (1.f - a.hard) * a.temperature * a.temperature * (t.plogp + total * logf(soft) - cross);
   if (t.label >= 0 && a.hard != 0.f) loss += a.hard * (logf(hard) - zy);
   return loss;
 }
@@ -312,13 +384,13 @@ __device__ __forceinline__ void wait_left(int left) {        // for all but the 
 // run under both passes.  A warp more, the clerk, reads the next row's entries meanwhile, takes their logits out of the row before it is
 // overwritten (kTaken), and writes their columns again once the row's gradient is written (kWritten).
 constexpr int kGroups = kRowBytes / (512 * kVec * 16) + 1;   // groups of vectors of a thread
-template <int K>
-__global__ void __launch_bounds__(544, 2)
+template <int K, int T>
+__global__ void __launch_bounds__(T + 32, T == 512 ? 2 : 4)
 distill_row_kernel(const __grid_constant__ DistillArgs a) {
   extern __shared__ uint4 ring[];
   __shared__ float red[2][96];
   __shared__ int has[2], labels[2];
-  const int T = blockDim.x - 32, nvec = a.cols >> 3, valid = min(a.cols, a.vocab), nv = (valid + 7) >> 3;
+  const int nvec = a.cols >> 3, valid = min(a.cols, a.vocab), nv = (valid + 7) >> 3;
   const float c = kLog2e / a.temperature;
   const __nv_bfloat16* kept = reinterpret_cast<const __nv_bfloat16*>(ring);
   auto out_row = [&](int row) { return reinterpret_cast<__nv_bfloat16*>(a.grad) + (int64_t)row * a.ldg; };
@@ -336,83 +408,115 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
       for (int k = l; k <= a.top; k += 32)
         if (e.at[k] >= 0) out[e.at[k]] = __float2bfloat16(e.p[k]);
     };
+    Held held = hold(a, blockIdx.x);
     for (int row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
       const Entries e = entries_at(buffers + parity * entry_bytes(a.top), a.top);
-      const RowTarget t = read_entries(a, row, raw, e);
+      const RowTarget t = read_entries(a, row, held, raw, e);
+      if (row + (int)gridDim.x < a.rows) held = hold(a, row + gridDim.x);
       if (l == 0) {
         has[parity] = t.some;
         labels[parity] = t.label;
       }
       if (row != (int)blockIdx.x) rewrite(row - gridDim.x, parity ^ 1);
       bar_sync(kSums, T + 32);
+      // the logits of the entries first: the other warps wait for it before the next row arrives
+      for (int k = l; k <= a.top; k += 32) raw.p[k] = e.at[k] >= 0 ? __bfloat162float(kept[e.at[k]]) : 0.f;
+      const float y = t.label >= 0 ? __bfloat162float(kept[t.label]) : 0.f;
+      __syncwarp();
+      bar_arrive(kTaken, T + 32);
       Sums<K> sum;
       sum.join(c, red[parity], T >> 5);
-      const Weights w = weights_of(a, sum.m, sum.soft, sum.hard, t.some, t.label >= 0);
-      float cross = 0.f;
+      const Weights w = weights_of<K>(a, sum.m, sum.soft, sum.hard, t.some, t.label >= 0);
+      const float rs = sum.soft_ref(c), rh = sum.hard_ref(c);
+      float cross = 0.f, total = 0.f;
       for (int k = l; k <= a.top; k += 32) {
         const int at = e.at[k];
         if (at < 0) continue;
-        const float z = __bfloat162float(kept[at]), p = e.p[k], drop = drop_of(w, at, p, t.label);
-        if (p != 0.f) cross += p * (z - sum.m);
+        const float z = raw.p[k], p = e.p[k], drop = drop_of(w, at, p, t.label);
+        if (p != 0.f) {
+          cross += p * (fmaf(z, c, -rs) * kLn2);
+          total += p;
+        }
         if (drop == 0.f) e.at[k] = -1;                       // (its column is as the others)
         else e.p[k] = grad_one<K>(z, w, c) - drop;
       }
-      const float zy = t.label >= 0 ? __bfloat162float(kept[t.label]) - sum.m : 0.f;
-      __syncwarp();
-      bar_arrive(kTaken, T + 32);
       cross = warp_sum(cross);
-      if (l == 0) a.loss[row] = loss_of(a, t, sum.soft, sum.hard, cross, zy);
+      total = warp_sum(total);
+      if (l == 0) a.loss[row] = loss_of(a, t, sum.soft, sum.hard, cross, total, t.label >= 0 ? fmaf(y, kLog2e, -rh) * kLn2 : 0.f);
     }
     const int rows = (a.rows - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     rewrite(blockIdx.x + (rows - 1) * gridDim.x, parity ^ 1);
     return;
   }
-  const int groups = (nv + T * kVec - 1) / (T * kVec);
+  const int groups = (nv + T * kVec - 1) / (T * kVec), whole = valid / (8 * T * kVec);   // whole groups need no tests
+  uint4* mine = ring + threadIdx.x;
   auto logits_row = [&](int row) {
-    return reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld);
+    return reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld) + threadIdx.x;
   };
-  auto fetch = [&](const uint4* z, int v0) {
+  auto fetch = [&](const uint4* z, int g) {
+    uint4* to = mine + g * (kVec * T);
+    z += g * (kVec * T);
+    if (g < whole) {
 #pragma unroll
-    for (int j = 0; j < kVec; ++j)
-      if (v0 + j * T < nv) cp_async16(ring + v0 + j * T, z + v0 + j * T);
+      for (int j = 0; j < kVec; ++j) cp_async16(to + j * T, z + j * T);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+        if (threadIdx.x + (g * kVec + j) * T < nv) cp_async16(to + j * T, z + j * T);
+    }
     cp_async_commit();
   };
-  for (int g = 0; g < groups; ++g) fetch(logits_row(blockIdx.x), threadIdx.x + g * T * kVec);
+  for (int g = 0; g < groups; ++g) fetch(logits_row(blockIdx.x), g);
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
     Sums<K> sum;
     for (int g = 0; g < groups; ++g) {
       wait_left<kGroups>(groups - 1 - g);
-      uint4 u[kVec];
+      const uint4* at = mine + g * (kVec * T);
+      if (g < whole) {
+        uint4 u[kVec];
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const int v = threadIdx.x + (g * kVec + j) * T;
-        u[j] = v < nv ? cut(ring[v], v, valid) : make_uint4(kNegInf2, kNegInf2, kNegInf2, kNegInf2);
+        for (int j = 0; j < kVec; ++j) u[j] = at[j * T];
+        sum.add(u, c);
+      } else {
+        // what does not fill a group is worked on by the warps that have something of it
+#pragma unroll 1
+        for (int v = threadIdx.x + g * kVec * T; v < nv; v += T) {
+          const uint4 u[1] = {cut(ring[v], v, valid)};
+          sum.add(u, c);
+        }
       }
-      sum.add(u, c);
     }
     sum.leave(c, red[parity]);
     bar_sync(kSums, T + 32);
     sum.join(c, red[parity], T >> 5);
-    const Weights w = weights_of(a, sum.m, sum.soft, sum.hard, has[parity] != 0, labels[parity] >= 0);
+    const Weights w = weights_of<K>(a, sum.m, sum.soft, sum.hard, has[parity] != 0, labels[parity] >= 0);
     // (rows that nothing is learnt from get zeros, whatever their logits are)
-    const int learnt = w.drop == 0.f && w.label == 0.f ? 0 : nv;
-    const bool more = row + (int)gridDim.x < a.rows;
+    const bool learnt = w.drop != 0.f || w.label != 0.f, more = row + (int)gridDim.x < a.rows;
     const uint4* next = logits_row(row + gridDim.x);
-    uint4* out = reinterpret_cast<uint4*>(out_row(row));
-    bar_sync(kTaken, T + 32);
+    uint4* out = reinterpret_cast<uint4*>(out_row(row)) + threadIdx.x;
     for (int g = 0; g < groups; ++g) {
-      const int v0 = threadIdx.x + g * kVec * T;
+      const uint4* at = mine + g * (kVec * T);
+      uint4* to = out + g * (kVec * T);
+      if (g < whole && learnt) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) {
-        const int v = v0 + j * T;
-        if (v < nv) out[v] = v < learnt ? grad_vector<K>(ring[v], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+        for (int j = 0; j < kVec; ++j) to[j * T] = grad_whole<K>(at[j * T], w, c);
+      } else {
+#pragma unroll
+        for (int j = 0; j < kVec; ++j) {
+          const int v = threadIdx.x + (g * kVec + j) * T;
+          if (v < nv) to[j * T] = learnt ? grad_vector<K>(at[j * T], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+        }
       }
-      if (more) fetch(next, v0);
+      if (g == 0) bar_sync(kTaken, T + 32);
+      if (more) fetch(next, g);
     }
-    for (int v = nv + threadIdx.x; v < nvec; v += T) out[v] = make_uint4(0u, 0u, 0u, 0u);
+    for (int v = nv + threadIdx.x; v < nvec; v += T) out[v - threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
     bar_arrive(kWritten, T + 32);
   }
 }
+
+// Of sums relative to 2^ref, relative to 2^(m c): times 2^(ref - m c), whose exponent fma gives exactly.
+__device__ __forceinline__ float shift(float m, float c) { return m == -INFINITY ? 1.f : exp2f(fmaf(-m, c, ref_of(m, c))); }
 
 // Statistics of a slice.
 __global__ void __launch_bounds__(512)
@@ -440,7 +544,7 @@ distill_partial_kernel(const __grid_constant__ DistillArgs a) {
   if (threadIdx.x < 32) {
     sum.join(c, red, T >> 5);
     const Entries raw = entries_at(ring, a.top), e = entries_at(reinterpret_cast<uint8_t*>(ring) + entry_bytes(a.top), a.top);
-    const RowTarget t = read_entries(a, row, raw, e);
+    const RowTarget t = read_entries(a, row, hold(a, row), raw, e);
     float dot = 0.f;
     for (int k = threadIdx.x; k <= a.top; k += 32) {
       const int at = e.at[k] - a.col_offset;
@@ -451,8 +555,8 @@ distill_partial_kernel(const __grid_constant__ DistillArgs a) {
       const int y = t.label - a.col_offset;
       float* s = a.stats + (int64_t)row * 5;
       s[0] = sum.m;
-      s[1] = sum.hard;
-      s[2] = sum.soft;
+      s[1] = sum.hard * shift(sum.m, kLog2e);       // relative to the maximum itself
+      s[2] = sum.soft * shift(sum.m, c);
       s[3] = dot;
       s[4] = t.label >= 0 && y >= 0 && y < valid ? __bfloat162float(z[y]) : 0.f;
     }
@@ -475,17 +579,18 @@ distill_grad_kernel(const __grid_constant__ DistillArgs a) {
   const float* s = a.stats + (int64_t)row * 5;
   const float m = s[0], hard = s[1], soft = s[2];
   if (threadIdx.x < 32) {
-    const RowTarget t = read_entries(a, row, raw, e);
+    const RowTarget t = read_entries(a, row, hold(a, row), raw, e);
     float total = 0.f;
     for (int k = threadIdx.x; k <= a.top; k += 32) total += e.at[k] >= 0 ? e.p[k] : 0.f;
     total = warp_sum(total);
     if (threadIdx.x == 0) {
       target = t;
-      if (a.loss != nullptr) a.loss[row] = loss_of(a, t, soft, hard, s[3] - total * m, s[4] - m);
+      if (a.loss != nullptr) a.loss[row] = loss_of(a, t, soft, hard, (s[3] - total * m) / a.temperature, total, s[4] - m);
     }
   }
   __syncthreads();
-  const Weights w = weights_of(a, m, soft, hard, target.some, target.label >= 0);
+  const Weights w = weights_of<K>(a, m, soft / shift(m, c), hard / (K == kSquare ? shift(m, c) * shift(m, c) : shift(m, kLog2e)),
+                                  target.some, target.label >= 0);
   for (int k = threadIdx.x; k <= a.top; k += T) {          // before the gradient may overwrite the logits
     const int at = e.at[k] - a.col_offset;
     const bool here = e.at[k] >= 0 && at >= 0 && at < valid;
@@ -542,15 +647,17 @@ cudaError_t distill_row(const DistillArgs& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   if (valid > distill_row_cols() || a.col_offset != 0 || a.cols < a.vocab) return cudaErrorInvalidValue;
   const int smem = nv * 16 + 3 * entry_bytes(a.top), kind = kind_of(a);
-  auto kernel = kind == kSoft ? distill_row_kernel<kSoft> : kind == kHard ? distill_row_kernel<kHard>
-              : kind == kSquare ? distill_row_kernel<kSquare> : distill_row_kernel<kTwo>;
-  e = allow(kernel, smem);
-  if (e != cudaSuccess) return e;
   // As many CTAs as are resident at a time: by shared memory (228 KiB, 2 KiB a CTA beside the row) and registers (56 a thread).
   // Sixteen warps a row where no more than two rows fit, else eight.
   int sms = 148, dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
   const int fit = 228 * 1024 / (smem + 2048), threads = (fit > 2 ? 256 : 512) + 32, by_registers = 65536 / (56 * threads);
+  auto kernel = fit > 2 ? (kind == kSoft ? distill_row_kernel<kSoft, 256> : kind == kHard ? distill_row_kernel<kHard, 256>
+                           : kind == kSquare ? distill_row_kernel<kSquare, 256> : distill_row_kernel<kTwo, 256>)
+                        : (kind == kSoft ? distill_row_kernel<kSoft, 512> : kind == kHard ? distill_row_kernel<kHard, 512>
+                           : kind == kSquare ? distill_row_kernel<kSquare, 512> : distill_row_kernel<kTwo, 512>);
+  e = allow(kernel, smem);
+  if (e != cudaSuccess) return e;
   const int64_t most = (int64_t)sms * (fit < 1 ? 1 : fit < by_registers ? fit : by_registers);
   return launch_dependent(kernel, (unsigned)(a.rows < most ? a.rows : most), threads, smem, stream, a);
 }
