@@ -500,6 +500,208 @@ window_delta_kernel(const uint4* out, const uint4* dout, float* delta, uint32_t 
   }
 }
 
+// Few first tokens (up to kThinKeys) beyond the window: what far queries add to their dK and dV comes from here, with the row sums, so that
+// no key-major item streams a whole sequence for a handful of keys.  Queries come in tiles of 16 rows, a warp's ring filled by itself
+// (cp.async); the first tokens are the 8 (or twice 8) columns of matrix fragments: S = Q K^T and dP = dO V^T, then dV^T += dO^T P and
+// dK^T += Q^T dS, whose B operands are the score fragments transposed.  A CTA takes a run of the tiles of one key head (of all query
+// heads that share it) and leaves its sums in `parts`; the key-major item of block 0 adds their sum before it rounds.  mma.sync: 32
+// instructions a tile of 8 or 12 KiB and 8 first tokens.
+// Bound by HBM: it reads O, dO and, of far queries, Q once.
+constexpr int kThinKeys = 16;
+constexpr int kRowsWarps = 4, kRowsStages = 2, kRowsTile = 16 * kD * 2;
+constexpr int kRowsSmem = kRowsWarps * kRowsStages * 3 * kRowsTile;
+constexpr int kRowsPart = 2 * kThinKeys * kD;      // floats of a CTA: dV, dK
+static_assert(kRowsWarps * kRowsPart * 4 <= kRowsSmem, "the warps' sums take the place of the tiles");
+struct RowsArgs {
+  const __nv_bfloat16 *qkv, *out, *dout;
+  const float* lse;
+  float *lse2, *delta, *parts;
+  int seq, padded, kv, group, window, sinks, per;   // per: tiles of a CTA
+  float scale;
+};
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void load4(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load4_trans(uint32_t (&r)[4], uint32_t at) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  return t;
+}
+// kCols: groups of 8 first tokens.
+template <int kCols>
+__global__ void __launch_bounds__(kRowsWarps * 32, 2)
+window_rows_kernel(const __grid_constant__ RowsArgs a) {
+  extern __shared__ __align__(128) uint8_t rows_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int b = blockIdx.y / a.kv, h = blockIdx.y - b * a.kv, heads = a.kv * a.group, width = a.kv * (a.group + 2) * kD;
+  const int per_head = a.padded / 16, t0 = blockIdx.x * a.per, t1 = min(t0 + a.per, a.group * per_head);
+  const uint32_t ring = smem_u32(rows_smem) + warp * kRowsStages * 3 * kRowsTile;
+  const __nv_bfloat16* first = a.qkv + (int64_t)b * a.seq * width + h * (a.group + 2) * kD;   // row 0, query head 0 of this key head
+  grid_trigger();
+  grid_wait();
+  // chunk c of row r of a tile lies at c ^ (r % 8): fragments are read without conflicts
+  auto fetch = [&](int t, int stage) {
+    if (t < t1) {
+      const int m = t / per_head, q0 = (t - m * per_head) * 16;
+      const bool far = q0 + 15 >= a.window;
+      const uint32_t at = ring + stage * 3 * kRowsTile;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = i * 2 + (lane >> 4), c = lane & 15;
+        const bool there = q0 + r < a.seq;
+        const int64_t tok = there ? q0 + r : 0;
+        const int64_t o = (((int64_t)b * a.seq + tok) * heads + h * a.group + m) * kD + c * 8;
+        const uint32_t to = at + r * 256 + ((c ^ (r & 7)) << 4);
+        copy16(to, a.out + o, there);
+        copy16(to + kRowsTile, a.dout + o, there);
+        if (far) copy16(to + 2 * kRowsTile, first + tok * width + m * kD + c * 8, there);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fetch(t0 + warp, 0);
+  // first tokens as B fragments: column lane / 4 of each 8, rows (features) 2 (lane % 4) and + 8 of each 16
+  uint32_t kb[kCols][8][2], vb[kCols][8][2];
+#pragma unroll
+  for (int n = 0; n < kCols; ++n)
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = n * 8 + (lane >> 2), col = ks * 16 + i * 8 + (lane & 3) * 2;
+        const __nv_bfloat16* k = first + (int64_t)key * width + a.group * kD + col;
+        kb[n][ks][i] = key < a.sinks ? *reinterpret_cast<const uint32_t*>(k) : 0u;
+        vb[n][ks][i] = key < a.sinks ? *reinterpret_cast<const uint32_t*>(k + kD) : 0u;
+      }
+  float dv[kCols][8][4] = {}, dk[kCols][8][4] = {};   // [features of 16][first tokens of 8]
+  const float sl2 = a.scale * kLog2e;
+  int stage = 0;
+  for (int t = t0 + warp; t < t1; t += kRowsWarps) {
+    fetch(t + kRowsWarps, stage ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+    const uint32_t to = ring + stage * 3 * kRowsTile, td = to + kRowsTile, tq = td + kRowsTile;
+    const int m = t / per_head, q0 = (t - m * per_head) * 16;
+    const int64_t head = (int64_t)b * heads + h * a.group + m;
+    // row sums: two lanes a row, whose chunks are taken in orders that do not meet in a bank
+    float mine = 0.f;
+    {
+      const int r = lane >> 1, half = lane & 1, q = q0 + r;
+      const float lse = q < a.seq ? a.lse[head * a.seq + q] : INFINITY;
+      const uint8_t* row = rows_smem + (to - smem_u32(rows_smem)) + r * 256;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int c = (half * 8 + (i ^ (half * 4))) ^ (r & 7);
+        const uint4 o = *reinterpret_cast<const uint4*>(row + c * 16), d = *reinterpret_cast<const uint4*>(row + kRowsTile + c * 16);
+        const uint32_t ov[4] = {o.x, o.y, o.z, o.w}, dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mine += __uint_as_float(ov[k] << 16) * __uint_as_float(dd[k] << 16) +
+                  __uint_as_float(ov[k] & 0xffff0000u) * __uint_as_float(dd[k] & 0xffff0000u);
+      }
+      mine += __shfl_xor_sync(0xffffffffu, mine, 1);
+      mine = half ? -lse * kLog2e : -mine * a.scale;               // (beyond the end: -inf, 0)
+      (half ? a.lse2 : a.delta)[head * a.padded + q] = mine;
+    }
+    if (q0 + 15 >= a.window) {
+      float s[kCols][4] = {}, dp[kCols][4] = {};
+      const int r = lane & 15;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        uint32_t x[4];
+        const uint32_t at = r * 256 + (((ks * 2 + (lane >> 4)) ^ (r & 7)) << 4);
+        load4(x, tq + at);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) mma(s[n], x, kb[n][ks][0], kb[n][ks][1]);
+        load4(x, td + at);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) mma(dp[n], x, vb[n][ks][0], vb[n][ks][1]);
+      }
+      uint32_t p[kCols][2], g[kCols][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int q = (lane >> 2) + i * 8;
+        const float delta = __shfl_sync(0xffffffffu, mine, 2 * q), lse2 = __shfl_sync(0xffffffffu, mine, 2 * q + 1);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) {
+          float e[2], d[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int key = n * 8 + (lane & 3) * 2 + j;
+            const bool seen = key < a.sinks && q0 + q - key >= a.window;
+            e[j] = seen ? fast_exp2(fmaf(s[n][i * 2 + j], sl2, lse2)) : 0.f;
+            d[j] = seen ? e[j] * fmaf(dp[n][i * 2 + j], a.scale, delta) : 0.f;
+          }
+          p[n][i] = transpose8(pack_bf16(e[0], e[1]));
+          g[n][i] = transpose8(pack_bf16(d[0], d[1]));
+        }
+      }
+#pragma unroll
+      for (int f = 0; f < 8; ++f) {
+        // 16 features of the 16 queries, transposed: rows 0-7 and 8-15 of the fragment are features, its columns queries
+        uint32_t x[4];
+        const int q = (lane & 7) + (lane >> 4) * 8;
+        const uint32_t at = q * 256 + (((f * 2 + (lane >> 3 & 1)) ^ (q & 7)) << 4);
+        load4_trans(x, td + at);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) mma(dv[n][f], x, p[n][0], p[n][1]);
+        load4_trans(x, tq + at);
+#pragma unroll
+        for (int n = 0; n < kCols; ++n) mma(dk[n][f], x, g[n][0], g[n][1]);
+      }
+    }
+    __syncwarp();                                  // the stage has been read
+    stage ^= 1;
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float* sums = reinterpret_cast<float*>(rows_smem) + warp * kRowsPart;
+#pragma unroll
+  for (int n = 0; n < kCols; ++n)
+#pragma unroll
+    for (int f = 0; f < 8; ++f)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float* at = sums + (n * 8 + (lane & 3) * 2 + (i & 1)) * kD + f * 16 + (lane >> 2) + (i >> 1) * 8;
+        at[0] = dv[n][f][i];
+        at[kThinKeys * kD] = dk[n][f][i];
+      }
+  __syncthreads();
+  float* part = a.parts + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kRowsPart;
+  for (int i = threadIdx.x; i < kRowsPart; i += kRowsWarps * 32) {
+    float v = 0.f;
+    if ((i / kD) % kThinKeys < kCols * 8)
+#pragma unroll
+      for (int w = 0; w < kRowsWarps; ++w) v += reinterpret_cast<const float*>(rows_smem)[w * kRowsPart + i];
+    part[i] = v;
+  }
+}
+
+// The CTAs' sums of each key head, added up in their order: a key-major item that added them itself would wait for memory once for each.
+__global__ void __launch_bounds__(128)
+window_parts_kernel(const float* parts, float* sums, int chunks) {
+  grid_trigger();
+  grid_wait();
+  const int64_t at = blockIdx.x * 128 + threadIdx.x;
+  const float* p = parts + (int64_t)blockIdx.y * chunks * kRowsPart + at;
+  float v = 0.f;
+#pragma unroll 8
+  for (int c = 0; c < chunks; ++c) v += p[(int64_t)c * kRowsPart];
+  sums[(int64_t)blockIdx.y * kRowsPart + at] = v;
+}
+
 // Key-major items accumulate dV and dK of 128 keys over the query blocks that see them, of every head of the group; query-major
 // items dQ of 128 queries over their list of key blocks.  Roles, rings and tensor memory as in attn_bwd2_kernel.
 constexpr int kBwdWarps = 16;               // element-wise warps
@@ -519,6 +721,8 @@ struct WinBwdArgs {
   uint32_t items;       // item i < items is key-major, items + i query-major
   int key_group, query_group;   // rows of items (sequence, head) that are dealt together
   int batch, seq, kv, group, heads, window, sinks;
+  int key_sinks;        // first tokens whose keys key-major items stream every later query for: none of the few (`far` has them)
+  const float* far;     // [batch * kv][dV, dK][kThinKeys][128] of the few, or null
   float scale;
   uint32_t* status;
   uint64_t timeout_ns;
@@ -559,7 +763,7 @@ __device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) 
   // the longest items of a group first: key block 0, the last query block
   w.blk = kKeyMajor ? y : nblk - 1 - y;
   if (kKeyMajor) {
-    const int last = w.blk * kBlk < a.sinks ? nblk - 1 : min(nblk - 1, (w.blk * kBlk + kBlk - 1 + a.window - 1) / kBlk);
+    const int last = w.blk * kBlk < a.key_sinks ? nblk - 1 : min(nblk - 1, (w.blk * kBlk + kBlk - 1 + a.window - 1) / kBlk);
     w.i0 = w.blk;
     w.per = last - w.blk + 1;
     w.n_it = w.per * a.group;
@@ -868,7 +1072,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         const float* my_lse = sLse + st0 * kBlk + part * kBwdCols + (lane & 3) * 2;
         const float* my_dlt = sDelta + (g & 1) * kBlk + part * kBwdCols + (lane & 3) * 2;
         // only pairs on the diagonal or the window's edge, and far ones with first tokens among the keys, pay for the mask
-        const bool masked = kKeyMajor ? c0 < me0 + 24 || (c0 + kBwdCols - 1 - me0 >= a.window && me0 + 24 >= a.sinks)
+        const bool masked = kKeyMajor ? c0 < me0 + 24 || (c0 + kBwdCols - 1 - me0 >= a.window && me0 + 24 >= a.key_sinks)
                                       : c0 + kBwdCols - 1 > me || (me - c0 >= a.window && c0 + kBwdCols > a.sinks);
         float e[kBwdCols];                                // P of this thread's columns
         // ---- phase 1: P = exp2(S * scale * log2(e) - lse2) ----
@@ -915,7 +1119,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
                 const int k = kKeyMajor ? (i >> 3) * 16 + hp * 8 + (i & 7) : hp * 16 + i;
                 if (kKeyMajor) {
                   const int key = me0 + (k >> 4) * 16 + (k >> 1 & 1) * 8, query = c0 + (k >> 2 & 3) * 8 + (lane & 3) * 2 + (k & 1);
-                  if (key > query || (query - key >= a.window && key >= a.sinks)) e[k] = 0.f;
+                  if (key > query || (query - key >= a.window && key >= a.key_sinks)) e[k] = 0.f;
                 } else if (c0 + k > me || (me - c0 - k >= a.window && c0 + k >= a.sinks)) {
                   e[k] = 0.f;
                 }
@@ -982,6 +1186,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       // Accumulators -> bf16 rows of dqkv: a warp's 32 rows x kBwdCols columns leave through shared memory as a TMA store
       // (with plain stores the warps stall for 4000 cycles when all SMs write their items at the same time).
       const int col = (kKeyMajor ? col_k(a, w.h) : col_q(a, w.h)) + part * kBwdCols, orow = w.blk * kBlk + q4 * 32, ob = w.b;
+      // what far queries add to a first token's gradients: this lane's row
+      const float* far = kKeyMajor && a.far != nullptr && orow + lane < a.sinks
+                             ? a.far + ((int64_t)w.b * a.kv + w.h) * kRowsPart + (orow + lane) * kD + part * kBwdCols : nullptr;
       const uint32_t phase = items & 1;
       const uint32_t out_st = (g - 1) & 1;
       uint8_t* stage = sS1 + out_st * kTile + (warp - 2) * kBwdStage;   // where the item's last dO or V was
@@ -1001,6 +1208,17 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         tmem_ld_32x32((kKeyMajor && which ? t_acc1 : t_acc0) + lane_off + part * kBwdCols, r);
         warp_stage_free();
         tmem_ld_wait();
+        if (kKeyMajor && far != nullptr) {
+          const float4* add = reinterpret_cast<const float4*>(far + which * kThinKeys * kD);
+#pragma unroll
+          for (int i = 0; i < kBwdCols / 4; ++i) {
+            const float4 v = add[i];
+            r[4 * i] = __float_as_uint(__uint_as_float(r[4 * i]) + v.x);
+            r[4 * i + 1] = __float_as_uint(__uint_as_float(r[4 * i + 1]) + v.y);
+            r[4 * i + 2] = __float_as_uint(__uint_as_float(r[4 * i + 2]) + v.z);
+            r[4 * i + 3] = __float_as_uint(__uint_as_float(r[4 * i + 3]) + v.w);
+          }
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           uint4 v;
@@ -1090,6 +1308,10 @@ cudaError_t configure_device() {
   if (dev >= 0 && dev < 64 && configured[dev]) return cudaSuccess;
   e = cudaFuncSetAttribute(window_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kFwdSmem);
   if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(window_rows_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
+  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(window_rows_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem);
+  if (e != cudaSuccess) return e;
   for (auto kernel : {window_bwd_kernel<true, true>, window_bwd_kernel<true, false>, window_bwd_kernel<false, true>}) {
     e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBwdSmem);
     if (e != cudaSuccess) return e;
@@ -1150,7 +1372,21 @@ cudaError_t window_attention_fwd(const void* qkv, void* out, float* lse, const W
   return launch_dependent(window_fwd_kernel, grid, kFwdThreads, kFwdSmem, stream, tq, to, a);
 }
 
-int64_t window_attention_scratch(const WindowShape& s) { return 2 * (int64_t)s.batch * s.kv * s.group * blocks_of(s.seq) * kBlk; }
+namespace {
+// Few first tokens beyond a window: CTAs of window_rows_kernel per key head (0: the general way).  One wave of two CTAs an SM, each with
+// a tile or more for every warp.
+int thin_chunks(const WindowShape& s) {
+  if (s.sinks == 0 || s.sinks > kThinKeys || s.window == 0 || s.window >= s.seq) return 0;
+  const int units = s.batch * s.kv, tiles = s.group * blocks_of(s.seq) * (kBlk / 16);
+  int n = 148 * 2 / units;
+  n = n < tiles / kRowsWarps ? n : tiles / kRowsWarps;
+  return n < 1 ? 1 : n;
+}
+}  // namespace
+
+int64_t window_attention_scratch(const WindowShape& s) {
+  return 2 * (int64_t)s.batch * s.kv * s.group * blocks_of(s.seq) * kBlk + (int64_t)s.batch * s.kv * (thin_chunks(s) + 1) * kRowsPart;
+}
 
 cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* dout, const float* lse, void* dqkv, float* scratch,
                                  const WindowShape& s, uint32_t* status, cudaStream_t stream) {
@@ -1167,7 +1403,31 @@ cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* d
   if (make_tensor_map_seq(&tg, dqkv, width, s.seq, s.batch, kBwdCols, 32) != 0) return cudaErrorInvalidValue;
   WinBwdArgs g{};
   float* delta = scratch + (int64_t)s.batch * heads * nblk * kBlk;
-  {
+  const int chunks = thin_chunks(s);
+  if (chunks > 0) {
+    const int tiles = s.group * nblk * (kBlk / 16);
+    RowsArgs r{};
+    r.qkv = reinterpret_cast<const __nv_bfloat16*>(qkv);
+    r.out = reinterpret_cast<const __nv_bfloat16*>(out);
+    r.dout = reinterpret_cast<const __nv_bfloat16*>(dout);
+    r.lse = lse;
+    r.lse2 = scratch;
+    r.delta = delta;
+    r.parts = delta + (int64_t)s.batch * heads * nblk * kBlk;
+    r.seq = s.seq; r.padded = nblk * kBlk; r.kv = s.kv; r.group = s.group; r.window = s.window; r.sinks = s.sinks < s.seq ? s.sinks : s.seq;
+    r.per = (tiles + chunks - 1) / chunks;
+    r.scale = s.scale;
+    auto kernel = r.sinks > 8 ? window_rows_kernel<2> : window_rows_kernel<1>;
+    e = launch_dependent(kernel, dim3((unsigned)chunks, (unsigned)(s.batch * s.kv)), kRowsWarps * 32, kRowsSmem, stream, r);
+    if (e != cudaSuccess) return e;
+    g.far = r.parts;
+    if (chunks > 1) {
+      float* sums = r.parts + (int64_t)s.batch * s.kv * chunks * kRowsPart;
+      e = launch_dependent(window_parts_kernel, dim3(kRowsPart / 128, (unsigned)(s.batch * s.kv)), 128, 0, stream, r.parts, sums, chunks);
+      if (e != cudaSuccess) return e;
+      g.far = sums;
+    }
+  } else {
     const uint32_t groups = (uint32_t)((int64_t)s.batch * heads * nblk * (kBlk / kDeltaRows));
     e = launch_dependent(window_delta_kernel, (groups + 15) / 16, 256, 0, stream, reinterpret_cast<const uint4*>(out),
                          reinterpret_cast<const uint4*>(dout), delta, groups, (uint32_t)s.seq, (uint32_t)(nblk * kBlk), (uint32_t)heads,
@@ -1179,6 +1439,7 @@ cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* d
   g.batch = s.batch; g.seq = s.seq; g.kv = s.kv; g.group = s.group; g.heads = heads;
   g.window = s.window == 0 || s.window > s.seq ? s.seq : s.window;
   g.sinks = s.sinks < s.seq ? s.sinks : s.seq;
+  g.key_sinks = chunks > 0 ? 0 : g.sinks;
   g.scale = s.scale;
   g.status = status;
   g.timeout_ns = 2000000000ull;
