@@ -49,6 +49,28 @@ __device__ __forceinline__ int sink_blocks(const A& a) { return (a.sinks + kBlk 
 // n low bits, for any n.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
+// 2^x of two lanes on the FMA pipe, for the share of the exponentials that would queue for the special-function unit: x = n + f with n
+// the nearest whole number, 2^f by the polynomial of degree 5 with the smallest largest relative error on [-1/2, 1/2] (Remez exchange;
+// 2^-23.7, with fp32 rounding 2^-22.2), n added to the exponent.  Below -125 the result is about 2^-125 and not zero; NaN stays NaN.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
+  split(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-125.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-125.0f));
+  const uint64_t t = f32x2(a, b), big = f32x2(12582912.0f, 12582912.0f);   // 1.5 * 2^23: n in the low bits
+  const uint64_t r = add2(t, big), n = add2(r, f32x2(-12582912.0f, -12582912.0f)), f = fma2(n, f32x2(-1.f, -1.f), t);
+  uint64_t p = f32x2(1.327647245e-03f, 1.327647245e-03f);
+  p = fma2(p, f, f32x2(9.675540961e-03f, 9.675540961e-03f));
+  p = fma2(p, f, f32x2(5.550713092e-02f, 5.550713092e-02f));
+  p = fma2(p, f, f32x2(2.402212024e-01f, 2.402212024e-01f));
+  p = fma2(p, f, f32x2(6.931469440e-01f, 6.931469440e-01f));
+  p = fma2(p, f, f32x2(1.000000119e+00f, 1.000000119e+00f));
+  float ra, rb;
+  split(p, a, b);
+  split(r, ra, rb);
+  a = __int_as_float(__float_as_int(a) + (__float_as_int(ra) << 23));
+  b = __int_as_float(__float_as_int(b) + (__float_as_int(rb) << 23));
+}
+
 __device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int b) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
@@ -704,6 +726,7 @@ window_parts_kernel(const float* parts, float* sums, int chunks) {
 
 // Key-major items accumulate dV and dK of 128 keys over the query blocks that see them, of every head of the group; query-major
 // items dQ of 128 queries over their list of key blocks.  Roles, rings and tensor memory as in attn_bwd2_kernel.
+constexpr int kBwdPoly = 2;                 // key-major: exponentials of every eight that run on the FMA pipe
 constexpr int kBwdWarps = 16;               // element-wise warps
 constexpr int kBwdCols = kBlk * 4 / kBwdWarps;   // columns of a row per element-wise thread
 constexpr int kBwdStage = 32 * kBwdCols * 2;     // output staging per element-wise warp
@@ -1109,9 +1132,14 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
 #pragma unroll
             for (int i = 0; i < kBwdCols / 2; i += 2) {
               const int k = kKeyMajor ? (i >> 3) * 16 + hp * 8 + (i & 7) : hp * 16 + i;
-              split(fma2(f32x2(__uint_as_float(rs[k]), __uint_as_float(rs[k + 1])), sl2, st[(k >> 2) & 3]), e[k], e[k + 1]);
-              e[k] = fast_exp2(e[k]);
-              e[k + 1] = fast_exp2(e[k + 1]);
+              const uint64_t x = fma2(f32x2(__uint_as_float(rs[k]), __uint_as_float(rs[k + 1])), sl2, st[(k >> 2) & 3]);
+              if (kKeyMajor && i % 8 < kBwdPoly) {
+                exp2_poly(x, e[k], e[k + 1]);
+              } else {
+                split(x, e[k], e[k + 1]);
+                e[k] = fast_exp2(e[k]);
+                e[k + 1] = fast_exp2(e[k + 1]);
+              }
             }
             if (masked) {
 #pragma unroll
