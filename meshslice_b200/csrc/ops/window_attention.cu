@@ -39,6 +39,8 @@ __device__ __forceinline__ int col_q(const A& a, int h) {
   return (kv * (a.group + 2) + h - kv * a.group) * kD;
 }
 template <class A>
+__device__ __forceinline__ int col_q(const A& a, int kv, int h) { return (kv * (a.group + 2) + h - kv * a.group) * kD; }
+template <class A>
 __device__ __forceinline__ int col_k(const A& a, int kv) { return (kv * (a.group + 2) + a.group) * kD; }
 // First key block of query block i's window, blocks that hold first tokens.
 template <class A>
@@ -731,9 +733,9 @@ constexpr int kBwdWarps = 16;               // element-wise warps
 constexpr int kBwdCols = kBlk * 4 / kBwdWarps;   // columns of a row per element-wise thread
 constexpr int kBwdStage = 32 * kBwdCols * 2;     // output staging per element-wise warp
 constexpr int kStatBytes = kBlk * 4;        // lse2 or delta of 128 queries
-constexpr int kBwdAlignSlack = 256;
+constexpr int kBwdAlignSlack = 192;
 constexpr size_t kBwdBars = 7 * kTile + 5 * kStatBytes;   // where the barriers are
-constexpr size_t kBwdSmem = kBwdBars + 256 + kBwdAlignSlack;
+constexpr size_t kBwdSmem = kBwdBars + 320 + kBwdAlignSlack;
 static_assert(kBwdWarps * kBwdStage == kTile, "an item's staged output takes the place of a tile");
 static_assert(kBwdSmem <= 232448, "shared memory of a CTA");
 constexpr int kBwdThreads = 96 + 32 * kBwdWarps;
@@ -755,24 +757,29 @@ __device__ __forceinline__ int64_t stat_at(const WinBwdArgs& a, int b, int h, in
   return (((int64_t)b * a.heads + h) * nblk + blk) * kBlk;
 }
 
-struct Streamed {
-  int h, blk;           // query head and block of a streamed tile
-};
 struct BwdItem {
   int b, h, blk, n_it;  // sequence, key head (key-major) or query head, owned block, streamed blocks
   int i0, per;          // key-major: first query block, query blocks of a head; query-major: blocks with first tokens, first of the window
-  template <bool kKeyMajor>
-  __device__ __forceinline__ Streamed streamed(const WinBwdArgs& a, int it) const {
-    Streamed s;
+  int kv;               // key head
+  int more;             // there is such an item
+};
+static_assert(sizeof(BwdItem) == 32, "two vectors");
+// The streamed blocks of an item one after another.
+template <bool kKeyMajor>
+struct Streamed {
+  int h, blk;           // query head and block
+  __device__ __forceinline__ Streamed(const WinBwdArgs& a, const BwdItem& w)
+      : h(kKeyMajor ? w.h * a.group : w.h), blk(kKeyMajor ? w.i0 : w.i0 > 0 ? 0 : w.per) {}
+  __device__ __forceinline__ void next(const BwdItem& w) {
+    ++blk;
     if (kKeyMajor) {
-      const int m = it / per;
-      s.h = h * a.group + m;
-      s.blk = i0 + it - m * per;
-    } else {
-      s.h = h;
-      s.blk = it < i0 ? it : per + it - i0;
+      if (blk == w.i0 + w.per) {
+        blk = w.i0;
+        ++h;
+      }
+    } else if (blk == w.i0) {
+      blk = w.per;
     }
-    return s;
   }
 };
 template <bool kKeyMajor>
@@ -795,6 +802,8 @@ __device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) 
     w.per = max(w.i0, window_block(a, w.blk));
     w.n_it = w.i0 + max(0, w.blk + 1 - w.per);
   }
+  w.kv = kKeyMajor ? w.h : w.h / a.group;
+  w.more = 1;
   return w;
 }
 
@@ -818,7 +827,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
   // key-major: lse2 travels with Q, delta with dO.  delta(i+2) takes the slot of delta(i): its producer waits for dS(i).
   float* sLse = reinterpret_cast<float*>(smem + 7 * kTile);   // [3][128]
   float* sDelta = sLse + 3 * kBlk;                            // [2][128]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBwdBars);   // up to 30: the tensor-memory address is behind them
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kBwdBars);   // 30 is the tensor-memory address
   uint8_t* clc_resp = reinterpret_cast<uint8_t*>(bars);   // 16 bytes
   uint64_t* clc_full = bars + 2;
   uint64_t* clc_empty = bars + 3;
@@ -835,16 +844,21 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
   uint64_t* p_ready = bars + 24;            // [2] key-major: the first / second 16 columns of every warp's P^T
   uint64_t* acc_done = bars + 26;           // [2] key-major: dV / dK; query-major: [1] dQ
   uint64_t* out_read = bars + 28;           // [2] the copy engine has read the output staged in a stage of ring 1
+  uint64_t* item_full = bars + 31;          // the next item, as the producer of ring 0 has worked it out
+  uint64_t* out_read0 = bars + 32;          // [3] key-major: as out_read, of ring 0
+  int4* item_slot = reinterpret_cast<int4*>(bars + 36);   // [2]
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint64_t tmo = a.timeout_ns;
 
   if (threadIdx.x == 0) {
     mbar_init(clc_full, 1);
-    mbar_init(clc_empty, 3 + kBwdWarps);    // producers and MMA thread, element-wise warps
+    mbar_init(item_full, 1);
+    mbar_init(clc_empty, 2 + kBwdWarps);    // producer of ring 1 and MMA thread, element-wise warps
     for (int i = 0; i < 3; ++i) {
       mbar_init(full0 + i, 1);
       mbar_init(empty0 + i, 1);
+      mbar_init(out_read0 + i, kBwdWarps);
     }
     mbar_init(s_full, 1);
     mbar_init(s_free, kBwdWarps);
@@ -871,20 +885,20 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
 
   BwdItem w = bwd_item<kKeyMajor>(a, item);
   bool ok = true;
-  // The next item as the producer got it: false when there is none of this kind (or on a timeout).
+  // The next item, which the producer of ring 0 has worked out for all: false when there is none of this kind (or on a timeout).
   uint32_t items = 0;                       // items finished by this thread
   auto next_item = [&]() -> bool {
-    uint32_t x, y, z;
-    if (!mbar_wait(clc_full, items & 1, 8 * tmo)) {
+    if (!mbar_wait(item_full, items & 1, 8 * tmo)) {
       report(a.status, kErrWindow + 18, items, 0);
       ok = false;
       return false;
     }
     ++items;
-    const bool more = clc_read(clc_resp, x, y, z) && (x < a.items) == kKeyMajor;
-    fence_proxy_async_smem();               // this read before the next response overwrites it
-    if (more) w = bwd_item<kKeyMajor>(a, x);
-    return more;
+    const int4 lo = item_slot[0], hi = item_slot[1];
+    if (hi.w == 0) return false;
+    w.b = lo.x; w.h = lo.y; w.blk = lo.z; w.n_it = lo.w;
+    w.i0 = hi.x; w.per = hi.y; w.kv = hi.z;
+    return true;
   };
   uint32_t g = 0;                           // streamed blocks so far: stages and phases of the rings and the hand-overs
 
@@ -892,28 +906,42 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
     // resident tile of S, ring of Q or K, next items
     if (elect_one()) {
       bool more = true;
+      uint32_t outs[3] = {0, 0, 0};           // key-major: outputs staged in each stage so far
+      bool staged[3] = {false, false, false}; // the last user of the stage was an item's output
       while (ok && more) {
         // the resident tile of S first, then the item's first streamed tile: S needs no more
-        for (int it = -1; it < w.n_it && ok; ++it) {
-          if (it < 0) {
-            if (!(ok = mbar_wait(res_empty, (items & 1) ^ 1, 8 * tmo))) break;
-            mbar_expect_tx(res_full, kTile);
-            load_tile(sR0, &tm_qkv, res_full, kKeyMajor ? col_k(a, w.h) : col_q(a, w.h), w.blk * kBlk, w.b);           // K or Q
-            continue;
-          }
+        if (!(ok = mbar_wait(res_empty, (items & 1) ^ 1, 8 * tmo))) break;
+        mbar_expect_tx(res_full, kTile);
+        load_tile(sR0, &tm_qkv, res_full, kKeyMajor ? col_k(a, w.h) : col_q(a, w.kv, w.h), w.blk * kBlk, w.b);           // K or Q
+        Streamed<kKeyMajor> s(a, w);
+        for (int it = 0; it < w.n_it && ok; ++it, ++g, s.next(w)) {
           const uint32_t st = g % kRing0;
-          const Streamed s = w.template streamed<kKeyMajor>(a, it);
           if (!(ok = mbar_wait(empty0 + st, ((g / kRing0) & 1) ^ 1, 8 * tmo))) break;
+          if (kKeyMajor && staged[st] && !(ok = mbar_wait(out_read0 + st, (outs[st] - 1) & 1, 8 * tmo))) break;
+          staged[st] = false;
           mbar_expect_tx(full0 + st, kTile + (kKeyMajor ? kStatBytes : 0));
-          load_tile(sS0 + st * kTile, &tm_qkv, full0 + st, kKeyMajor ? col_q(a, s.h) : col_k(a, s.h / a.group), s.blk * kBlk, w.b);
+          load_tile(sS0 + st * kTile, &tm_qkv, full0 + st, kKeyMajor ? col_q(a, w.h, s.h) : col_k(a, w.kv), s.blk * kBlk, w.b);
           if (kKeyMajor) bulk_g2s(sLse + st * kBlk, a.lse2 + stat_at(a, w.b, s.h, s.blk), kStatBytes, full0 + st);
-          ++g;
         }
+        if (ok) {
+          const uint32_t st = (g - 1) % kRing0;
+          staged[st] = kKeyMajor;
+          ++outs[st];
+        }
+        // every thread has the item that the slot holds: ask for the next and work it out
         if (ok && (ok = mbar_wait(clc_empty, (items & 1) ^ 1, 8 * tmo))) {
           mbar_expect_tx(clc_full, 16);
           clc_try_cancel(clc_resp, clc_full);
-          more = next_item();
-          mbar_arrive(clc_empty);
+          uint32_t x, y, z;
+          if ((ok = mbar_wait(clc_full, items & 1, 8 * tmo))) {
+            more = clc_read(clc_resp, x, y, z) && (x < a.items) == kKeyMajor;
+            fence_proxy_async_smem();         // this read before the next response overwrites it
+            if (more) w = bwd_item<kKeyMajor>(a, x);
+            item_slot[0] = make_int4(w.b, w.h, w.blk, w.n_it);
+            item_slot[1] = make_int4(w.i0, w.per, w.kv, more ? 1 : 0);
+            mbar_arrive(item_full);
+            ++items;
+          }
         }
       }
       // what is still under way (a timeout above is reported here too)
@@ -933,9 +961,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           if (kKeyMajor) load_tile(sR1, &tm_qkv, res_full + 1, col_k(a, w.h) + kD, w.blk * kBlk, w.b);     // V
           else load_tile(sR1, &tm_do, res_full + 1, w.h * kD, w.blk * kBlk, w.b);                            // dO
         }
-        for (int it = 0; it < w.n_it && ok; ++it, ++g) {
+        Streamed<kKeyMajor> s(a, w);
+        for (int it = 0; it < w.n_it && ok; ++it, ++g, s.next(w)) {
           const uint32_t st = g % kRing1;
-          const Streamed s = w.template streamed<kKeyMajor>(a, it);
           if (!(ok = mbar_wait(empty1 + st, ((g / kRing1) & 1) ^ 1, 8 * tmo))) break;
           if (staged[st] && !(ok = mbar_wait(out_read + st, (outs[st] - 1) & 1, 8 * tmo))) break;
           staged[st] = false;
@@ -945,7 +973,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
             if (g > 1 && !(ok = mbar_wait(ds_ready + st, ((g - 2) >> 1) & 1, 8 * tmo))) break;
             bulk_g2s(sDelta + st * kBlk, a.delta + stat_at(a, w.b, s.h, s.blk), kStatBytes, full1 + st);
           } else {
-            load_tile(sS1 + st * kTile, &tm_qkv, full1 + st, col_k(a, s.h / a.group) + kD, s.blk * kBlk, w.b);                  // V
+            load_tile(sS1 + st * kTile, &tm_qkv, full1 + st, col_k(a, w.kv) + kD, s.blk * kBlk, w.b);                  // V
           }
         }
         if (ok) {
@@ -1030,6 +1058,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       // Blocks follow one another across items: the next item's first S is issued where the next block's would be, and its
       // first dP behind this item's last product.
       ok = first_s(g) && first_dp(g);
+      bool early = false;                                 // the next item's first S went before this item's last product
       while (ok && more) {
         const int n = w.n_it;
         for (int it = 0; it < n && ok; ++it, ++g) {
@@ -1054,7 +1083,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           } else {
             more = next_item();                           // w is the next item's from here on
             mbar_arrive(clc_empty);
-            if (more && !(ok = first_s(g + 1))) break;
+            // query-major, where the next item's tiles are there already: the element-wise warps get its scores behind their output
+            early = !kKeyMajor && more && mbar_test(res_full, items & 1) && mbar_test(full0 + (g + 1) % kRing0, ((g + 1) / kRing0) & 1);
+            if (early && !(ok = first_s(g + 1))) break;
           }
           if (!(ok = wait(ds_ready + (g & 1), (g >> 1) & 1, 14))) break;
           const uint32_t acc = kKeyMajor ? t_acc1 : t_acc0, ds = t_dp + dp_buf(g) * 128;
@@ -1063,6 +1094,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           umma_commit(empty0 + st0);
           if (last) umma_commit(acc_done + 1);
           if (last) {
+            if (more && !early && !(ok = first_s(g + 1))) break;
             if (more && !(ok = first_dp(g + 1))) break;
           } else if (kKeyMajor) {
             if (!(ok = issue_dp(g + 1))) break;
@@ -1078,18 +1110,23 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
     const uint32_t lane_off = static_cast<uint32_t>(q4 * 32) << 16;
     const uint64_t sl2 = f32x2(a.scale * kLog2e, a.scale * kLog2e), sc2 = f32x2(a.scale, a.scale);
     bool more = true;
+    float lse2 = 0.f, delta = 0.f;                        // query-major: this lane's statistics, asked for an item ahead
+    auto ask = [&]() {
+      if (!kKeyMajor) {
+        const int64_t at = stat_at(a, w.b, w.h, w.blk) + row;
+        lse2 = a.lse2[at];
+        delta = a.delta[at];
+      }
+    };
+    ask();
     while (more) {
       const int me = w.blk * kBlk + row;                  // query-major: this lane's query
       const int me0 = w.blk * kBlk + q4 * 32 + (lane >> 2);   // key-major: the first of this thread's keys
-      uint64_t my_lse2 = 0, my_delta = 0;
-      if (!kKeyMajor) {
-        const int64_t at = stat_at(a, w.b, w.h, w.blk) + row;
-        my_lse2 = f32x2(a.lse2[at], a.lse2[at]);
-        my_delta = f32x2(a.delta[at], a.delta[at]);
-      }
-      for (int it = 0; it < w.n_it; ++it, ++g) {
+      const uint64_t my_lse2 = f32x2(lse2, lse2), my_delta = f32x2(delta, delta);
+      Streamed<kKeyMajor> s(a, w);
+      for (int it = 0; it < w.n_it; ++it, ++g, s.next(w)) {
         const uint32_t ts = tmem + lane_off + part * kBwdCols, tdp = ts + 128 + dp_buf(g) * 128;
-        const int c0 = w.template streamed<kKeyMajor>(a, it).blk * kBlk + part * kBwdCols;   // first streamed index of this thread's columns
+        const int c0 = s.blk * kBlk + part * kBwdCols;   // first streamed index of this thread's columns
         const uint32_t st0 = g % kRing0;
         // key-major: lse2 / delta of this thread's columns
         const float* my_lse = sLse + st0 * kBlk + part * kBwdCols + (lane & 3) * 2;
@@ -1213,15 +1250,18 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       if (!ok) break;
       // Accumulators -> bf16 rows of dqkv: a warp's 32 rows x kBwdCols columns leave through shared memory as a TMA store
       // (with plain stores the warps stall for 4000 cycles when all SMs write their items at the same time).
-      const int col = (kKeyMajor ? col_k(a, w.h) : col_q(a, w.h)) + part * kBwdCols, orow = w.blk * kBlk + q4 * 32, ob = w.b;
+      const int col = (kKeyMajor ? col_k(a, w.h) : col_q(a, w.kv, w.h)) + part * kBwdCols, orow = w.blk * kBlk + q4 * 32, ob = w.b;
       // what far queries add to a first token's gradients: this lane's row
       const float* far = kKeyMajor && a.far != nullptr && orow + lane < a.sinks
                              ? a.far + ((int64_t)w.b * a.kv + w.h) * kRowsPart + (orow + lane) * kD + part * kBwdCols : nullptr;
       const uint32_t phase = items & 1;
-      const uint32_t out_st = (g - 1) & 1;
-      uint8_t* stage = sS1 + out_st * kTile + (warp - 2) * kBwdStage;   // where the item's last dO or V was
+      // where the item's last dO or V was; dK: where its last Q was
+      const uint32_t out_st = (g - 1) & 1, out_st0 = (g - 1) % kRing0;
+      uint8_t* const stages[2] = {sS1 + out_st * kTile + (warp - 2) * kBwdStage,
+                                  (kKeyMajor ? sS0 + out_st0 * kTile : sS1 + out_st * kTile) + (warp - 2) * kBwdStage};
       more = next_item();                        // w is the next item's from here on
-      __syncwarp();                              // every lane has read the response: the one after may be asked for now
+      if (more) ask();
+      __syncwarp();                              // every lane has read the slot: the one after may be asked for now
       if (lane == 0) mbar_arrive(clc_empty);
 #pragma unroll 1
       for (int which = kKeyMajor ? 0 : 1; which < 2; ++which) {
@@ -1234,7 +1274,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         // key-major: acc0 = dV, acc1 = dK;  query-major: acc0 = dQ
         uint32_t r[kBwdCols];
         tmem_ld_32x32((kKeyMajor && which ? t_acc1 : t_acc0) + lane_off + part * kBwdCols, r);
-        warp_stage_free();
+        uint8_t* stage = stages[which];
         tmem_ld_wait();
         if (kKeyMajor && far != nullptr) {
           const float4* add = reinterpret_cast<const float4*>(far + which * kThinKeys * kD);
@@ -1259,9 +1299,16 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         warp_store_box(&tm_dqkv, stage, col + (kKeyMajor && which == 0 ? kD : 0), orow, ob, a.seq);
       }
       if (!ok) break;
-      if (lane == 0) {
-        bulk_wait_read<0>();
-        mbar_arrive(out_read + out_st);          // the stage may take a tile again
+      if (lane == 0) {                           // the stages may take tiles again
+        if (kKeyMajor) {
+          bulk_wait_read<1>();
+          mbar_arrive(out_read + out_st);
+          bulk_wait_read<0>();
+          mbar_arrive(out_read0 + out_st0);
+        } else {
+          bulk_wait_read<0>();
+          mbar_arrive(out_read + out_st);
+        }
       }
       tc_fence_before_sync();                    // the accumulators are read before the next P / dS is announced
       __syncwarp();
@@ -1272,7 +1319,8 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
   const bool all = __syncthreads_and(ok) != 0;
   tc_fence_after_sync();
   if (threadIdx.x == 0 && all)
-    for (int i = 2; i < 30; ++i) mbar_inval(bars + i);
+    for (int i = 2; i < 35; ++i)
+      if (i != 30) mbar_inval(bars + i);
   return all;
 }
 
