@@ -807,6 +807,9 @@ __device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) 
   return w;
 }
 
+// How many of the distances 8 t + (0 or 1), t = -3 .. 3, are below d.
+__device__ __forceinline__ int below(int d) { return d <= -24 ? 0 : ((d + 24) >> 3) * 2 + min((d + 24) & 7, 2); }
+
 // A CTA's run of items of one kind, from `item` on, until cluster launch control has none left or one of the other kind (the
 // response stays in shared memory).  False after a timeout.  At its end every copy and every tcgen05 operation has arrived
 // where it was announced, so the barriers can be set up anew for the next run.
@@ -1162,6 +1165,17 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
 #pragma unroll
             for (int n = 0; n < 4; ++n) st[n] = *reinterpret_cast<const uint64_t*>(my_lse + n * 8);
           }
+          // What is seen, as bits.  key-major: of query - key = base + 8 (n - r) + (0 or 1), in rising order; what is seen lies between
+          // 0 and the window, for first tokens of any number above.
+          uint32_t seen[4] = {};
+          if (masked && kKeyMajor) {
+            const int base = c0 + (lane & 3) * 2 - me0;
+            const uint32_t from = ~low_bits(below(-base)), upto = low_bits(below(a.window - base));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) seen[r] = me0 + r * 8 < a.key_sinks ? from : from & upto;
+          }
+          if (masked && !kKeyMajor)
+            seen[0] = low_bits(me - c0 + 1) & (~low_bits(me - c0 + 1 - a.window) | low_bits(a.sinks - c0));
           // key-major: columns of a fragment are in groups n of 8, elements 4 n + {0, 1} of this thread's first row of a
           // lane half, + {2, 3} of its second; by halves of 16 columns, so that P^T can be handed over in two parts
 #pragma unroll
@@ -1182,12 +1196,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
 #pragma unroll
               for (int i = 0; i < kBwdCols / 2; ++i) {
                 const int k = kKeyMajor ? (i >> 3) * 16 + hp * 8 + (i & 7) : hp * 16 + i;
-                if (kKeyMajor) {
-                  const int key = me0 + (k >> 4) * 16 + (k >> 1 & 1) * 8, query = c0 + (k >> 2 & 3) * 8 + (lane & 3) * 2 + (k & 1);
-                  if (key > query || (query - key >= a.window && key >= a.key_sinks)) e[k] = 0.f;
-                } else if (c0 + k > me || (me - c0 - k >= a.window && c0 + k >= a.sinks)) {
-                  e[k] = 0.f;
-                }
+                // key-major: row r of four (keys + 8 r), column group n of four (queries + 8 n): distance t = n - r
+                const int r = (k >> 4) * 2 + (k >> 1 & 1), bit = kKeyMajor ? ((k >> 2 & 3) - r + 3) * 2 + (k & 1) : k;
+                if (!(seen[kKeyMajor ? r : 0] >> bit & 1)) e[k] = 0.f;
               }
             }
             if (kKeyMajor) {
