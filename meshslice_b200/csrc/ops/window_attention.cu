@@ -21,6 +21,7 @@ namespace msb {
 namespace {
 
 constexpr uint32_t kErrWindow = 40;
+constexpr int kThinKeys = 16;       // few first tokens: the narrowest product with 128 rows
 
 struct WinArgs {
   int batch, seq, kv, group, heads;   // heads = kv * group
@@ -28,6 +29,7 @@ struct WinArgs {
   float scale;
   float* lse;
   int tiles_per_item;                 // query tiles that a CTA works on at a time (1 or 2)
+  int thin;                           // no more than kThinKeys first tokens
   uint32_t* status;
   uint64_t timeout_ns;
 };
@@ -47,6 +49,22 @@ template <class A>
 __device__ __forceinline__ int window_block(const A& a, int i) { return max(0, i * kBlk - a.window + 1) / kBlk; }
 template <class A>
 __device__ __forceinline__ int sink_blocks(const A& a) { return (a.sinks + kBlk - 1) / kBlk; }
+
+// 32 lanes x 16 / 8 consecutive 32-bit columns: thread t of the warp has row (lane base + t).
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 
 // n low bits, for any n.
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
@@ -109,15 +127,16 @@ constexpr int kFwdRegsLow = 96, kFwdRegsHigh = 200;
 static_assert(kFwdRegsLow + 2 * kFwdRegsHigh <= 3 * 168, "register shares exceed what the CTA is launched with");
 
 // One or two neighbouring tiles (tile 0 the later one, block hi) of a head, and the list of key blocks that either sees: `ns` blocks
-// with first tokens, then from `lo` to hi.  Tile 0 sees all but entry `skip` (the window of tile 1 begins a block earlier, or not),
-// tile 1 all but the last, which is tile 0's diagonal.
+// with first tokens, what both have of the window from `lo` on, block hi, which tile 1 does not see, and (extra) the block before `lo`,
+// which tile 0 does not see, so that each tile has one of the last two while the other has the other.  thin bit t: entry 0 holds nothing
+// but first tokens, at most kThinKeys, for tile t, which takes its first kThinKeys keys only.
 struct FwdItem {
-  int b, h, hi, two, ns, lo, n, skip;
-  __device__ __forceinline__ int block(int x) const { return x < ns ? x : lo + x - ns; }
-  __device__ __forceinline__ bool uses(int t, int x) const { return t == 0 ? x != skip : two && x + 1 < n; }
-  __device__ __forceinline__ int first(int t) const { return t == 0 && skip == 0 ? 1 : 0; }
-  __device__ __forceinline__ int last(int t) const { return t == 0 ? n - 1 : n - 2; }
-  __device__ __forceinline__ int next(int t, int x) const { return t == 0 && x + 1 == skip ? x + 2 : x + 1; }
+  int b, h, hi, two, ns, lo, n, extra, thin;
+  __device__ __forceinline__ int block(int x) const { return x < ns ? x : x + extra == n ? lo - 1 : lo + x - ns; }
+  __device__ __forceinline__ bool uses(int t, int x) const { return t == 0 ? x + extra < n : two && x + 1 + extra != n; }
+  __device__ __forceinline__ int first(int t) const { return t == 1 && n == 2 && extra ? 1 : 0; }
+  __device__ __forceinline__ int last(int t) const { return t == 0 ? n - 1 - extra : extra ? n - 1 : n - 2; }
+  __device__ __forceinline__ int next(int t, int x) const { return t == 1 && x + 2 + extra == n ? x + 2 : x + 1; }
 };
 __device__ __forceinline__ FwdItem fwd_item(const WinArgs& a, uint32_t x, uint32_t y, uint32_t z, int group) {
   FwdItem w;
@@ -127,16 +146,17 @@ __device__ __forceinline__ FwdItem fwd_item(const WinArgs& a, uint32_t x, uint32
   w.hi = nblk - 1 - (int)y * a.tiles_per_item;
   w.two = a.tiles_per_item == 2 && w.hi > 0 ? 1 : 0;
   w.ns = min(sink_blocks(a), w.hi + 1);
-  const int lo0 = window_block(a, w.hi);
-  w.lo = max(w.ns, w.two ? window_block(a, w.hi - 1) : lo0);
-  w.n = w.ns + max(0, w.hi + 1 - w.lo);
-  w.skip = w.lo < lo0 ? w.ns : -1;
+  const int lo0 = window_block(a, w.hi), lo1 = window_block(a, max(w.hi - 1, 0));
+  w.lo = max(w.ns, lo0);
+  w.extra = w.two && max(w.ns, lo1) < w.lo ? 1 : 0;
+  w.n = w.ns + max(0, w.hi + 1 - w.lo) + w.extra;
+  w.thin = a.thin && w.ns == 1 ? (lo0 > 0 ? 1 : 0) | (w.two && lo1 > 0 ? 2 : 0) : 0;
   return w;
 }
 
 __global__ void __launch_bounds__(kFwdThreads, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_out,
-                 const __grid_constant__ WinArgs a) {
+                  const __grid_constant__ CUtensorMap tm_thin, const __grid_constant__ WinArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -158,6 +178,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
   uint64_t* o_done = bars + 18;
   uint64_t* p_ready = bars + 20;      // [2 * tile + part]: columns [0,96) / [96,128) of P
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+  uint64_t* item_full = bars + 25;    // the next item, as the producer has worked it out
+  int4* item_slot = reinterpret_cast<int4*>(bars + 26);   // [3]
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint64_t tmo = a.timeout_ns;
@@ -166,7 +188,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
   if (threadIdx.x == 0) {
     tma_prefetch_desc(&tm_qkv);
     mbar_init(clc_full, 1);
-    mbar_init(clc_empty, 10);         // producer and MMA thread, 8 softmax warps
+    mbar_init(item_full, 1);
+    mbar_init(clc_empty, 9);          // MMA thread, 8 softmax warps
     for (int i = 0; i < 2; ++i) {
       mbar_init(q_full + i, 1);
       mbar_init(q_empty + i, 1);
@@ -192,19 +215,19 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
   grid_trigger();
   grid_wait();
 
-  // The next item as the producer got it: false when there is none (or on a timeout).
-  uint32_t clc_phase = 0;
+  // The next item, which the producer has worked out for all: false when there is none (or on a timeout).
+  uint32_t items = 0;
   auto next_item = [&](FwdItem& w) -> bool {
-    uint32_t x, y, z;
-    if (!mbar_wait(clc_full, clc_phase, 8 * tmo)) {
+    if (!mbar_wait(item_full, items & 1, 8 * tmo)) {
       report(a.status, kErrWindow + 6, 0, 0);
       return false;
     }
-    clc_phase ^= 1;
-    const bool more = clc_read(clc_resp, x, y, z);
-    fence_proxy_async_smem();         // this read before the next response overwrites it
-    if (more) w = fwd_item(a, x, y, z, group);
-    return more;
+    ++items;
+    const int4 i0 = item_slot[0], i1 = item_slot[1], i2 = item_slot[2];
+    w.b = i0.x; w.h = i0.y; w.hi = i0.z; w.two = i0.w;
+    w.ns = i1.x; w.lo = i1.y; w.n = i1.z; w.extra = i1.w;
+    w.thin = i2.x;
+    return i2.y != 0;
   };
 
   if (warp < 4) {
@@ -225,20 +248,32 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
         for (int x = 0; x < w.n && ok; ++x, ++c) {
           const uint32_t st = c & 1, ph = ((c >> 1) & 1) ^ 1;
           const int krow = w.block(x) * kBlk;
+          const bool thin = x == 0 && w.thin == (w.two ? 3 : 1);        // for all that use it
+          const CUtensorMap* map = thin ? &tm_thin : &tm_qkv;
+          const uint32_t bytes = thin ? kThinKeys * kD * 2 : kTile;
           if (!(ok = mbar_wait(k_empty + st, ph, 8 * tmo))) break;
-          mbar_expect_tx(k_full + st, kTile);
-          load_tile(sK + st * kTile, &tm_qkv, k_full + st, colk, krow, w.b);
+          mbar_expect_tx(k_full + st, bytes);
+          load_tile(sK + st * kTile, map, k_full + st, colk, krow, w.b);
           if (!(ok = mbar_wait(v_empty + st, ph, 8 * tmo))) break;
-          mbar_expect_tx(v_full + st, kTile);
-          load_tile(sV + st * kTile, &tm_qkv, v_full + st, colk + kD, krow, w.b);
+          mbar_expect_tx(v_full + st, bytes);
+          load_tile(sV + st * kTile, map, v_full + st, colk + kD, krow, w.b);
         }
         // Only now, with the item's last loads on their way, ask for the next item: a CTA that took one item ahead
         // would hold it back from a CTA that is free sooner.
-        if (ok && (ok = mbar_wait(clc_empty, clc_phase ^ 1, 8 * tmo))) {
+        if (ok && (ok = mbar_wait(clc_empty, (items & 1) ^ 1, 8 * tmo))) {
           mbar_expect_tx(clc_full, 16);
           clc_try_cancel(clc_resp, clc_full);
-          more = next_item(w);
-          mbar_arrive(clc_empty);
+          uint32_t x, y, z;
+          if ((ok = mbar_wait(clc_full, items & 1, 8 * tmo))) {
+            more = clc_read(clc_resp, x, y, z);
+            fence_proxy_async_smem();         // this read before the next response overwrites it
+            if (more) w = fwd_item(a, x, y, z, group);
+            item_slot[0] = make_int4(w.b, w.h, w.hi, w.two);
+            item_slot[1] = make_int4(w.ns, w.lo, w.n, w.extra);
+            item_slot[2] = make_int4(w.thin, more ? 1 : 0, 0, 0);
+            mbar_arrive(item_full);
+            ++items;
+          }
         }
         if (!ok) report(a.status, kErrWindow + 1, w.hi, c);
       }
@@ -259,16 +294,17 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
         report(a.status, kErrWindow + code, d, base);
         return false;
       };
-      // Scores of tile t against entry x of the list.  The later tile that uses an entry gives its K back: tile 1 where both do (it
-      // leaves out none but the last, and its turn comes after tile 0's).
+      const uint32_t idesc_thin = make_idesc_bf16(128, kThinKeys, 0, 0);
+      // Scores of tile t against entry x of the list.  The later tile that uses an entry gives its K back: tile 1 where both do.
       auto issue_s = [&](int t, int x) -> bool {
         const uint32_t at = base + x;
         if (!wait(k_full + (at & 1), (at >> 1) & 1, 3, t)) return false;
         const uint64_t dqt = dq + t * kTileOff, dkt = dk + (at & 1) * kTileOff;
+        const uint32_t idesc = x == 0 && (w.thin >> t & 1) ? idesc_thin : idesc_s;
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
           const uint64_t off = (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4);
-          umma_f16(tmem + t * 128, dqt + off, dkt + off, idesc_s, k != 0);
+          umma_f16(tmem + t * 128, dqt + off, dkt + off, idesc, k != 0);
         }
         umma_commit(s_full + t);
         if (x == w.last(t)) umma_commit(q_empty + t);
@@ -287,14 +323,16 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
           const uint64_t dvs = dv + (at & 1) * kTileOff;
           for (int t = 0; t < 2; ++t) {
             if (!w.uses(t, x)) continue;
+            const bool thin = x == 0 && (w.thin >> t & 1);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               if (ok) ok = wait(p_ready + 2 * t + half, pc[t] & 1, 4, t);
               if (ok) {
 #pragma unroll
                 for (int k = half * 6; k < 6 + half * 2; ++k)   // 16 bf16 of a row of P = 8 TMEM columns per step
-                  umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, dvs + (uint64_t)((k * 2048) >> 4), idesc_pv,
-                              x != w.first(t) || k != 0);
+                  if (k == 0 || !thin)
+                    umma_f16_ts(tmem + 256 + t * 128, tmem + t * 128 + k * 8, dvs + (uint64_t)((k * 2048) >> 4), idesc_pv,
+                                x != w.first(t) || k != 0);
               }
             }
             if (!ok) break;
@@ -339,6 +377,33 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
         }
         tc_fence_after_sync();
         ++sc;
+        if (x == 0 && (w.thin >> t & 1)) {
+          // nothing but the first tokens, which the whole tile sees
+          uint32_t r[16], pk[8];
+          tmem_ld_32x16(ts, r);
+          tmem_ld_wait();
+          float m = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < kThinKeys; ++i) {
+            if (i >= a.sinks) r[i] = 0xff800000u;
+            m = fmaxf(m, __uint_as_float(r[i]));
+          }
+          first = false;
+          m_used = m * sl2;
+          const float m_here = m_used == -INFINITY ? 0.f : m_used;
+#pragma unroll
+          for (int i = 0; i < kThinKeys; i += 2) {
+            const float x0 = fast_exp2(fmaf(__uint_as_float(r[i]), sl2, -m_here)), x1 = fast_exp2(fmaf(__uint_as_float(r[i + 1]), sl2, -m_here));
+            l += x0 + x1;
+            pk[i >> 1] = pack_bf16(x0, x1);
+          }
+          tmem_st_32x8(ts, pk);
+          tmem_st_wait();
+          tc_fence_before_sync();
+          mbar_arrive(p_ready + 2 * t);
+          mbar_arrive(p_ready + 2 * t + 1);
+          continue;
+        }
         const int key0 = w.block(x) * kBlk;
         // only blocks on the diagonal and on the window's edge, and far ones with first tokens, carry mask arithmetic
         const bool masked = key0 == i_blk * kBlk || (i_blk * kBlk + kBlk - 1 - key0 >= a.window && key0 + kBlk > a.sinks);
@@ -468,7 +533,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
         if (query < a.seq) a.lse[((int64_t)w.b * a.heads + w.h) * a.seq + query] = m_used * kLn2 + logf(l);
       }
       more = next_item(w);
-      __syncwarp();                              // every lane has read the response
+      __syncwarp();                              // every lane has read the slot
       if (lane == 0) mbar_arrive(clc_empty);
     }
     if (lane == 0) bulk_wait_all<0>();
@@ -531,7 +596,6 @@ window_delta_kernel(const uint4* out, const uint4* dout, float* delta, uint32_t 
 // heads that share it) and leaves its sums in `parts`; the key-major item of block 0 adds their sum before it rounds.  mma.sync: 32
 // instructions a tile of 8 or 12 KiB and 8 first tokens.
 // Bound by HBM: it reads O, dO and, of far queries, Q once.
-constexpr int kThinKeys = 16;
 constexpr int kRowsWarps = 4, kRowsStages = 2, kRowsTile = 16 * kD * 2;
 constexpr int kRowsSmem = kRowsWarps * kRowsStages * 3 * kRowsTile;
 constexpr int kRowsPart = 2 * kThinKeys * kD;      // floats of a CTA: dV, dK
@@ -1441,13 +1505,16 @@ cudaError_t window_attention_fwd(const void* qkv, void* out, float* lse, const W
   e = configure_device();
   if (e != cudaSuccess) return e;
   const int heads = s.kv * s.group, nblk = blocks_of(s.seq);
-  CUtensorMap tq, to;
-  if (make_tensor_map_seq(&tq, qkv, (uint64_t)s.kv * (s.group + 2) * kD, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
+  CUtensorMap tq, to, tt;
+  const uint64_t width = (uint64_t)s.kv * (s.group + 2) * kD;
+  if (make_tensor_map_seq(&tq, qkv, width, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
+  if (make_tensor_map_seq(&tt, qkv, width, s.seq, s.batch, 64, kThinKeys) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&to, out, (uint64_t)heads * kD, s.seq, s.batch, 64, 32) != 0) return cudaErrorInvalidValue;
   WinArgs a{};
   a.batch = s.batch; a.seq = s.seq; a.kv = s.kv; a.group = s.group; a.heads = heads;
   a.window = s.window == 0 || s.window > s.seq ? s.seq : s.window;
   a.sinks = s.sinks < s.seq ? s.sinks : s.seq;
+  a.thin = a.sinks <= kThinKeys ? 1 : 0;
   a.scale = s.scale;
   a.lse = lse;
   a.status = status;
@@ -1456,7 +1523,7 @@ cudaError_t window_attention_fwd(const void* qkv, void* out, float* lse, const W
   a.tiles_per_item = (int64_t)s.batch * heads * nblk <= sm_count() ? 1 : 2;
   const int grp = deal(s.batch * heads);
   const dim3 grid(grp, (nblk + a.tiles_per_item - 1) / a.tiles_per_item, s.batch * heads / grp);
-  return launch_dependent(window_fwd_kernel, grid, kFwdThreads, kFwdSmem, stream, tq, to, a);
+  return launch_dependent(window_fwd_kernel, grid, kFwdThreads, kFwdSmem, stream, tq, to, tt, a);
 }
 
 namespace {
