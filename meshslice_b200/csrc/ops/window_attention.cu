@@ -797,6 +797,7 @@ constexpr int kBwdWarps = 16;               // element-wise warps
 constexpr int kBwdCols = kBlk * 4 / kBwdWarps;   // columns of a row per element-wise thread
 constexpr int kBwdStage = 32 * kBwdCols * 2;     // output staging per element-wise warp
 constexpr int kStatBytes = kBlk * 4;        // lse2 or delta of 128 queries
+constexpr int kThinBytes = kThinKeys * kD * 2;
 constexpr int kBwdAlignSlack = 192;
 constexpr size_t kBwdBars = 7 * kTile + 5 * kStatBytes;   // where the barriers are
 constexpr size_t kBwdSmem = kBwdBars + 320 + kBwdAlignSlack;
@@ -825,8 +826,9 @@ struct BwdItem {
   int b, h, blk, n_it;  // sequence, key head (key-major) or query head, owned block, streamed blocks
   int i0, per;          // key-major: first query block, query blocks of a head; query-major: blocks with first tokens, first of the window
   int kv;               // key head
-  int more;             // there is such an item
+  int flags;            // kMore: there is such an item; kThin: query-major, the first block streams no more than its kThinKeys first tokens
 };
+enum { kMore = 1, kThin = 2 };
 static_assert(sizeof(BwdItem) == 32, "two vectors");
 // The streamed blocks of an item one after another.
 template <bool kKeyMajor>
@@ -867,7 +869,7 @@ __device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) 
     w.n_it = w.i0 + max(0, w.blk + 1 - w.per);
   }
   w.kv = kKeyMajor ? w.h : w.h / a.group;
-  w.more = 1;
+  w.flags = kMore | (!kKeyMajor && w.i0 == 1 && a.sinks <= kThinKeys && window_block(a, w.blk) > 0 ? kThin : 0);
   return w;
 }
 
@@ -883,6 +885,7 @@ __device__ __forceinline__ int below(int d) { return d <= -24 ? 0 : ((d + 24) >>
 //                    TMEM lanes = queries, columns = keys: lse / delta are per thread.
 template <bool kKeyMajor>
 __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const CUtensorMap& tm_dqkv,
+                                               const CUtensorMap& tm_thin,
                                               const WinBwdArgs& a, uint8_t* smem, uint32_t tmem, uint32_t item) {
   uint8_t* sR0 = smem;                      // resident: K (key-major) or Q
   uint8_t* sR1 = smem + kTile;              // resident: V (key-major) or dO
@@ -963,6 +966,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
     ++items;
     const int4 lo = item_slot[0], hi = item_slot[1];
     if (hi.w == 0) return false;
+    w.flags = hi.w;
     w.b = lo.x; w.h = lo.y; w.blk = lo.z; w.n_it = lo.w;
     w.i0 = hi.x; w.per = hi.y; w.kv = hi.z;
     return true;
@@ -986,8 +990,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           if (!(ok = mbar_wait(empty0 + st, ((g / kRing0) & 1) ^ 1, 8 * tmo))) break;
           if (kKeyMajor && staged[st] && !(ok = mbar_wait(out_read0 + st, (outs[st] - 1) & 1, 8 * tmo))) break;
           staged[st] = false;
-          mbar_expect_tx(full0 + st, kTile + (kKeyMajor ? kStatBytes : 0));
-          load_tile(sS0 + st * kTile, &tm_qkv, full0 + st, kKeyMajor ? col_q(a, w.h, s.h) : col_k(a, w.kv), s.blk * kBlk, w.b);
+          const bool thin = !kKeyMajor && it == 0 && (w.flags & kThin);
+          mbar_expect_tx(full0 + st, thin ? kThinBytes : kTile + (kKeyMajor ? kStatBytes : 0));
+          load_tile(sS0 + st * kTile, thin ? &tm_thin : &tm_qkv, full0 + st, kKeyMajor ? col_q(a, w.h, s.h) : col_k(a, w.kv), s.blk * kBlk, w.b);
           if (kKeyMajor) bulk_g2s(sLse + st * kBlk, a.lse2 + stat_at(a, w.b, s.h, s.blk), kStatBytes, full0 + st);
         }
         if (ok) {
@@ -1005,7 +1010,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
             fence_proxy_async_smem();         // this read before the next response overwrites it
             if (more) w = bwd_item<kKeyMajor>(a, x);
             item_slot[0] = make_int4(w.b, w.h, w.blk, w.n_it);
-            item_slot[1] = make_int4(w.i0, w.per, w.kv, more ? 1 : 0);
+            item_slot[1] = make_int4(w.i0, w.per, w.kv, more ? w.flags : 0);
             mbar_arrive(item_full);
             ++items;
           }
@@ -1034,13 +1039,14 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           if (!(ok = mbar_wait(empty1 + st, ((g / kRing1) & 1) ^ 1, 8 * tmo))) break;
           if (staged[st] && !(ok = mbar_wait(out_read + st, (outs[st] - 1) & 1, 8 * tmo))) break;
           staged[st] = false;
-          mbar_expect_tx(full1 + st, kTile + (kKeyMajor ? kStatBytes : 0));
+          const bool thin = !kKeyMajor && it == 0 && (w.flags & kThin);
+          mbar_expect_tx(full1 + st, thin ? kThinBytes : kTile + (kKeyMajor ? kStatBytes : 0));
           if (kKeyMajor) {
             load_tile(sS1 + st * kTile, &tm_do, full1 + st, s.h * kD, s.blk * kBlk, w.b);                                // dO
             if (g > 1 && !(ok = mbar_wait(ds_ready + st, ((g - 2) >> 1) & 1, 8 * tmo))) break;
             bulk_g2s(sDelta + st * kBlk, a.delta + stat_at(a, w.b, s.h, s.blk), kStatBytes, full1 + st);
           } else {
-            load_tile(sS1 + st * kTile, &tm_qkv, full1 + st, col_k(a, w.kv) + kD, s.blk * kBlk, w.b);                  // V
+            load_tile(sS1 + st * kTile, thin ? &tm_thin : &tm_qkv, full1 + st, col_k(a, w.kv) + kD, s.blk * kBlk, w.b);                  // V
           }
         }
         if (ok) {
@@ -1077,7 +1083,8 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       };
       // S (or S^T) / dP (or dP^T) of streamed block number q, once its tile is there and the block before is out of S (key-major:
       // the products that read its P^T were issued before)
-      auto issue_s = [&](uint32_t q) -> bool {
+      const uint32_t id_thin = make_idesc_bf16(128, kThinKeys, 0, 0);
+      auto issue_s = [&](uint32_t q, uint32_t id_s) -> bool {
         const uint32_t st = q % kRing0;
         if (!kKeyMajor && q > 0 && !wait(s_free, (q - 1) & 1, 19)) return false;
         if (!wait(full0 + st, (q / kRing0) & 1, 13)) return false;
@@ -1090,7 +1097,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         umma_commit(s_full);
         return true;
       };
-      auto issue_dp = [&](uint32_t q) -> bool {
+      auto issue_dp = [&](uint32_t q, uint32_t id_s) -> bool {
         const uint32_t st = q % kRing1;
         if (!wait(full1 + st, (q / kRing1) & 1, 13)) return false;
         const uint64_t tile = ds1k + st * kStageOff;
@@ -1105,12 +1112,12 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       };
       // The first blocks of an item also wait for its resident tiles.  An item's last products of either kind free them.
       auto first_s = [&](uint32_t q) -> bool {
-        if (!(wait(res_full, items & 1, 12) && issue_s(q))) return false;
+        if (!(wait(res_full, items & 1, 12) && issue_s(q, w.flags & kThin ? id_thin : id_s))) return false;
         if (w.n_it == 1) umma_commit(res_empty);
         return true;
       };
       auto first_dp = [&](uint32_t q) -> bool {
-        if (!(wait(res_full + 1, items & 1, 12) && issue_dp(q))) return false;
+        if (!(wait(res_full + 1, items & 1, 12) && issue_dp(q, w.flags & kThin ? id_thin : id_s))) return false;
         if (w.n_it == 1) umma_commit(res_empty + 1);
         return true;
       };
@@ -1128,6 +1135,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       bool early = false;                                 // the next item's first S went before this item's last product
       while (ok && more) {
         const int n = w.n_it;
+        const bool thin_item = !kKeyMajor && (w.flags & kThin);
         for (int it = 0; it < n && ok; ++it, ++g) {
           const bool last = it + 1 == n;
           const uint32_t st0 = g % kRing0, st1 = g % kRing1;
@@ -1141,10 +1149,10 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
             if (last) umma_commit(acc_done);
           }
           if (!last) {
-            if (!(ok = issue_s(g + 1))) break;
+            if (!(ok = issue_s(g + 1, id_s))) break;
             if (it + 2 == n) umma_commit(res_empty);
             if (!kKeyMajor) {
-              if (!(ok = issue_dp(g + 1))) break;
+              if (!(ok = issue_dp(g + 1, id_s))) break;
               if (it + 2 == n) umma_commit(res_empty + 1);
             }
           } else {
@@ -1156,15 +1164,19 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           }
           if (!(ok = wait(ds_ready + (g & 1), (g >> 1) & 1, 14))) break;
           const uint32_t acc = kKeyMajor ? t_acc1 : t_acc0, ds = t_dp + dp_buf(g) * 128;
-          issue_grad(acc, ds, ds0m + st0 * kStageOff, 0, it == 0);     // dK += dS^T Q / dQ += dS K
-          issue_grad(acc, ds, ds0m + st0 * kStageOff, 1, false);
+          if (it == 0 && thin_item) {
+            umma_f16_ts(acc, ds, ds0m + st0 * kStageOff, id_g, false);
+          } else {
+            issue_grad(acc, ds, ds0m + st0 * kStageOff, 0, it == 0);   // dK += dS^T Q / dQ += dS K
+            issue_grad(acc, ds, ds0m + st0 * kStageOff, 1, false);
+          }
           umma_commit(empty0 + st0);
           if (last) umma_commit(acc_done + 1);
           if (last) {
             if (more && !early && !(ok = first_s(g + 1))) break;
             if (more && !(ok = first_dp(g + 1))) break;
           } else if (kKeyMajor) {
-            if (!(ok = issue_dp(g + 1))) break;
+            if (!(ok = issue_dp(g + 1, id_s))) break;
             if (it + 2 == n) umma_commit(res_empty + 1);
           }
         }
@@ -1201,6 +1213,8 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         // only pairs on the diagonal or the window's edge, and far ones with first tokens among the keys, pay for the mask
         const bool masked = kKeyMajor ? c0 < me0 + 24 || (c0 + kBwdCols - 1 - me0 >= a.window && me0 + 24 >= a.key_sinks)
                                       : c0 + kBwdCols - 1 > me || (me - c0 >= a.window && c0 + kBwdCols > a.sinks);
+        // of a thin block only the first columns are there
+        const bool mine = kKeyMajor || it > 0 || part == 0 || !(w.flags & kThin);
         float e[kBwdCols];                                // P of this thread's columns
         // ---- phase 1: P = exp2(S * scale * log2(e) - lse2) ----
         // (key-major: lse2 comes with Q and delta with dO, whose barriers order them for this thread)
@@ -1210,7 +1224,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           break;
         }
         tc_fence_after_sync();
-        {
+        if (!mine) {
+          if (lane == 0) mbar_arrive(s_free);
+        } else {
           uint32_t rs[kBwdCols];
           if (kKeyMajor) {
             tmem_ld_16x32_frag(ts, rs);
@@ -1290,7 +1306,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           break;
         }
         tc_fence_after_sync();
-        {
+        if (!mine) {
+          if (lane == 0) mbar_arrive(ds_ready + (g & 1));
+        } else {
           uint32_t rp[kBwdCols], dk[16];
           uint64_t st[4] = {my_delta, my_delta, my_delta, my_delta};
           if (kKeyMajor) {
@@ -1404,7 +1422,8 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
 template <bool kKey, bool kQuery>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 window_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_constant__ CUtensorMap tm_do,
-                 const __grid_constant__ CUtensorMap tm_dqkv, const __grid_constant__ WinBwdArgs a) {
+                  const __grid_constant__ CUtensorMap tm_dqkv, const __grid_constant__ CUtensorMap tm_thin,
+                  const __grid_constant__ WinBwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
@@ -1435,13 +1454,13 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
     uint32_t item = blockIdx.x, y, z;
     bool more = true;
     while (more) {
-      const bool ok = item < a.items ? window_bwd_run<true>(tm_qkv, tm_do, tm_dqkv, a, smem, tmem, item)
-                                     : window_bwd_run<false>(tm_qkv, tm_do, tm_dqkv, a, smem, tmem, item);
+      const bool ok = item < a.items ? window_bwd_run<true>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, item)
+                                     : window_bwd_run<false>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, item);
       more = ok && clc_read(clc_resp, item, y, z);
       fence_proxy_async_smem();             // this read before the next response overwrites it
     }
   } else {
-    window_bwd_run<kKey>(tm_qkv, tm_do, tm_dqkv, a, smem, tmem, blockIdx.x);
+    window_bwd_run<kKey>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, blockIdx.x);
   }
   if (warp >= 2 && warp < 2 + kBwdWarps && lane == 0) bulk_wait_all<0>();
   tc_fence_before_sync();
@@ -1551,7 +1570,8 @@ cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* d
   if (e != cudaSuccess) return e;
   const int heads = s.kv * s.group, nblk = blocks_of(s.seq);
   const uint64_t width = (uint64_t)s.kv * (s.group + 2) * kD;
-  CUtensorMap tq, td, tg;
+  CUtensorMap tq, td, tg, tt;
+  if (make_tensor_map_seq(&tt, qkv, width, s.seq, s.batch, 64, kThinKeys) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&tq, qkv, width, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&td, dout, (uint64_t)heads * kD, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&tg, dqkv, width, s.seq, s.batch, kBwdCols, 32) != 0) return cudaErrorInvalidValue;
@@ -1603,11 +1623,11 @@ cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* d
   g.items = keys;
   // Both kinds in one launch where the longer kind leaves SMs free, two beyond: the kernel of both needs more registers.
   if (queries <= (uint32_t)sm_count())
-    return launch_dependent(window_bwd_kernel<true, true>, keys + queries, kBwdThreads, kBwdSmem, stream, tq, td, tg, g);
-  e = launch_dependent(window_bwd_kernel<true, false>, keys, kBwdThreads, kBwdSmem, stream, tq, td, tg, g);
+    return launch_dependent(window_bwd_kernel<true, true>, keys + queries, kBwdThreads, kBwdSmem, stream, tq, td, tg, tt, g);
+  e = launch_dependent(window_bwd_kernel<true, false>, keys, kBwdThreads, kBwdSmem, stream, tq, td, tg, tt, g);
   if (e != cudaSuccess) return e;
   g.items = 0;
-  return launch_dependent(window_bwd_kernel<false, true>, queries, kBwdThreads, kBwdSmem, stream, tq, td, tg, g);
+  return launch_dependent(window_bwd_kernel<false, true>, queries, kBwdThreads, kBwdSmem, stream, tq, td, tg, tt, g);
 }
 
 }  // namespace msb
