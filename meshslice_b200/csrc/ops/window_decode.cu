@@ -280,8 +280,16 @@ cudaError_t window_decode(const WindowDecodeArgs& a, int splits, cudaStream_t st
   if (slots > 1 << 30 || rows > 65535 || a.batch > 65535) return cudaErrorInvalidValue;
   const int steps = kWarps * kKeys, per = (int)((slots + splits - 1) / splits + steps - 1) / steps * steps;
   auto kernel = a.group > 8 ? window_decode_kernel<true> : window_decode_kernel<false>;
-  const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  // the attribute is per device: set it once on every device that launches
+  static bool configured[64][2] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64 || !configured[dev][a.group > 8]) {
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev >= 0 && dev < 64) configured[dev][a.group > 8] = true;
+  }
   return launch_dependent(kernel, dim3((unsigned)splits, (unsigned)rows, (unsigned)a.batch), kWarps * 32, kSmem, stream, a, splits, per);
 }
 

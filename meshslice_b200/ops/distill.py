@@ -20,13 +20,16 @@ from .. import _native
 from . import rows
 
 
+_VALUES = {torch.float32: 0, torch.bfloat16: 1}     # types of the teacher's logits
+
+
 def _check(logits, ids, values, vocab: int, temperature: float, targets, hard_weight: float):
     if logits.dim() != 2:
         raise ValueError(f"logits must be [rows, columns] (got {tuple(logits.shape)})")
     n = logits.shape[0]
     if ids.dim() != 2 or ids.shape[0] != n or ids.dtype != torch.int64:
         raise ValueError(f"teacher ids must be int64 [rows, top] (got {ids.dtype} {tuple(ids.shape)})")
-    if values.shape != ids.shape or values.dtype not in (torch.float32, torch.bfloat16):
+    if values.shape != ids.shape or values.dtype not in _VALUES:
         raise ValueError(f"teacher logits must be fp32 or bf16 of the ids' shape (got {values.dtype} {tuple(values.shape)})")
     if targets is not None and (targets.shape != (n,) or targets.dtype != torch.int64):
         raise ValueError(f"targets must be int64 [rows] (got {targets.dtype} {tuple(targets.shape)})")
@@ -68,7 +71,7 @@ def _launch(step: int, logits, grad, ids, values, targets, col_offset: int, voca
     targets = None if targets is None else targets.contiguous()
     p = lambda t: 0 if t is None else t.data_ptr()
     _native.load().distill(step, z.data_ptr(), rows.pitch(z), p(grad), 0 if grad is None else rows.pitch(grad), ids.data_ptr(),
-                           values.data_ptr(), 1 if values.dtype == torch.bfloat16 else 0, p(targets), z.shape[0], z.shape[1], col_offset,
+                           values.data_ptr(), _VALUES[values.dtype], p(targets), z.shape[0], z.shape[1], col_offset,
                            vocab, ids.shape[1], temperature, hard_weight, scale, p(loss), p(stats), _native.stream_ptr())
 
 
@@ -77,6 +80,24 @@ def distill_loss_grad(logits, teacher_ids, teacher_logits, vocab: int, scale: fl
     """Loss [rows] (fp32, not scaled) and gradient times ``scale`` of whole rows of logits [rows, columns >= vocab]; columns from
     ``vocab`` on are padding and get 0.  ``teacher_ids`` int64 and ``teacher_logits`` fp32 or bf16 [rows, top].  The gradient goes to
     ``out`` (``out=logits`` works in place) or a new tensor."""
+    # the common call, checked in a few steps: a kernel of a few us is over before a longer list of them
+    if (logits.is_cuda and out is None and logits.dtype is torch.bfloat16 and logits.is_contiguous() and logits.data_ptr() & 15 == 0
+            and teacher_ids.dtype is torch.int64 and teacher_ids.shape == teacher_logits.shape and teacher_ids.dim() == logits.dim() == 2
+            and teacher_logits.dtype in _VALUES and teacher_ids.is_contiguous() and teacher_logits.is_contiguous()
+            and (hard_weight == 0.0 if targets is None else targets.dtype is torch.int64 and targets.shape == logits.shape[:1]
+                 and targets.is_contiguous() and targets.get_device() == logits.get_device())
+            and logits.get_device() == teacher_ids.get_device() == teacher_logits.get_device()
+            and 0.0 <= hard_weight <= 1.0 and 0.0 < temperature < math.inf):
+        n, cols = logits.shape
+        C = _native.load()
+        m, top = teacher_ids.shape
+        if m == n > 0 and cols % 8 == 0 and 0 < vocab <= min(cols, C.DISTILL_ROW_COLS) and top <= C.DISTILL_TOP:
+            _native.check_device(logits)
+            grad, loss = torch.empty_like(logits), torch.empty(n, dtype=torch.float32, device=logits.device)
+            C.distill(0, logits.data_ptr(), cols, grad.data_ptr(), cols, teacher_ids.data_ptr(), teacher_logits.data_ptr(),
+                      _VALUES[teacher_logits.dtype], 0 if targets is None else targets.data_ptr(), n, cols, 0, vocab, top, temperature,
+                      hard_weight, scale, loss.data_ptr(), 0, _native.stream_ptr())
+            return loss, grad
     _check(logits, teacher_ids, teacher_logits, vocab, temperature, targets, hard_weight)
     if logits.shape[1] < vocab:
         raise ValueError(f"whole rows have at least vocab = {vocab} columns (got {logits.shape[1]})")

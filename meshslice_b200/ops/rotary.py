@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from functools import cached_property
 from typing import List, Optional
 
 import torch
@@ -52,7 +53,7 @@ class RotaryConfig:
         if self.scaling == "by_parts" and not (self.original_len > 0 and self.beta_fast > self.beta_slow):
             raise ValueError("scaling by parts needs original_len > 0 and beta_fast > beta_slow")
 
-    @property
+    @cached_property
     def cos_factor(self) -> float:
         if self.attention_factor is not None:
             return float(self.attention_factor)
@@ -82,6 +83,7 @@ class Rotary:
         # turns per position in units of 2^-64, as two's complement
         turns = [round(math.fmod(v / (2 * math.pi), 1.0) * 2.0 ** 64) % (1 << 64) for v in freq]
         self.turns = torch.tensor([t - (1 << 64) if t >= 1 << 63 else t for t in turns], dtype=torch.int64, device=device)
+        self._kernel = (config.head_dim, config.rot_dim, 1 if config.layout == "half" else 0)
         self._freq = torch.tensor(freq, dtype=torch.float64) if not self.turns.is_cuda else None
 
     def cos_sin(self, positions):
@@ -114,9 +116,23 @@ def rotary_qkv(qkv, rotary: Rotary, kv_heads: int, group: int = 1, seq: Optional
     they are.  ``positions``: int64 [tokens]; without them token t is at t % ``seq``.  ``inverse`` turns back: the gradient of the
     unrotated rows from that of the rotated ones (times the same factor of cosines and sines).  ``out=qkv`` works in place.
     """
-    _check(qkv, rotary, kv_heads, group, seq, positions, out)
     c = rotary.config
     if qkv.is_cuda:
+        # the common call, checked in a few steps: a kernel of 3 us is over before a longer list of them
+        if (out is None and qkv.dtype is torch.bfloat16 and kv_heads > 0 and group > 0 and qkv.is_contiguous() and qkv.data_ptr() & 15 == 0
+                and qkv.shape[1:] == (kv_heads * (group + 2) * c.head_dim,) and qkv.get_device() == rotary.turns.get_device()
+                and (seq is not None and seq > 0 if positions is None else
+                     positions.dtype is torch.int64 and positions.shape == qkv.shape[:1] and positions.is_contiguous()
+                     and positions.get_device() == qkv.get_device())):
+            _native.check_device(qkv)
+            y = torch.empty_like(qkv)
+            n, width = qkv.shape
+            if n:
+                _native.load().rotary(qkv.data_ptr(), y.data_ptr(), width, width, 0 if positions is None else positions.data_ptr(),
+                                      rotary.turns.data_ptr(), n, seq or 1, kv_heads, group, *rotary._kernel, -1.0 if inverse else 1.0,
+                                      c.cos_factor, _native.stream_ptr())
+            return y
+        _check(qkv, rotary, kv_heads, group, seq, positions, out)
         if qkv.dtype != torch.bfloat16:
             raise ValueError(f"the rotary kernel needs bf16 rows (got {qkv.dtype})")
         _native.check_device(qkv)
@@ -133,12 +149,13 @@ def rotary_qkv(qkv, rotary: Rotary, kv_heads: int, group: int = 1, seq: Optional
         if qkv.shape[0]:
             _native.load().rotary(x.data_ptr(), y.data_ptr(), rows.pitch(x), rows.pitch(y),
                                   0 if positions is None else positions.data_ptr(), rotary.turns.data_ptr(), qkv.shape[0],
-                                  1 if seq is None else seq, kv_heads, group, c.head_dim, c.rot_dim, 1 if c.layout == "half" else 0,
+                                  1 if seq is None else seq, kv_heads, group, *rotary._kernel,
                                   -1.0 if inverse else 1.0, c.cos_factor, _native.stream_ptr())
         if out is not None and y is not out:
             out.copy_(y)
             return out
         return y
+    _check(qkv, rotary, kv_heads, group, seq, positions, out)
     pos = torch.arange(qkv.shape[0]) % seq if positions is None else positions
     cos, sin = rotary.cos_sin(pos)
     cos, sin = cos[:, None, None], (-sin if inverse else sin)[:, None, None]

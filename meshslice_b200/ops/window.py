@@ -4,6 +4,7 @@ formulation for CPU tensors."""
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -28,6 +29,14 @@ def _width(qkv, kv_heads: int, group: int, batch_rows: Optional[int]) -> int:
 # ----------------------------------------------------------------------------------------------
 # whole sequences
 # ----------------------------------------------------------------------------------------------
+@lru_cache(maxsize=256)
+def _scratch(batch: int, seq: int, kv_heads: int, group: int, window: int, sinks: int) -> int:
+    return _native.load().window_attention_scratch(batch, seq, kv_heads, group, window, sinks)
+
+
+_SCALE = 1.0 / math.sqrt(HEAD_DIM)
+
+
 def _check(qkv, batch: int, seq: int, kv_heads: int, group: int, window: int, sinks: int) -> int:
     if batch < 0 or seq < 1 or window < 0 or sinks < 0:
         raise ValueError(f"attention needs seq >= 1, window >= 0 (0: no window) and sinks >= 0 (got batch {batch}, seq {seq}, "
@@ -66,7 +75,7 @@ def window_attention_fwd(qkv, batch: int, seq: int, kv_heads: int, group: int = 
         if batch:
             x = _dense(qkv)
             _native.load().window_attention_fwd(x.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, seq, kv_heads, group, window, sinks,
-                                                1.0 / math.sqrt(D), _native.status().dev, _native.stream_ptr())
+                                                _SCALE, _native.status().dev, _native.stream_ptr())
         return out, lse
     q, k, v, s = _formulation(qkv, batch, seq, kv_heads, group, window, sinks, D)
     o = torch.softmax(s, -1) @ v
@@ -78,19 +87,18 @@ def window_attention_bwd(dout, qkv, out, lse, batch: int, seq: int, kv_heads: in
     D = _check(qkv, batch, seq, kv_heads, group, window, sinks)
     heads = kv_heads * group
     for name, t in (("dout", dout), ("out", out)):
-        if t.shape != (batch * seq, heads * D) or t.dtype != qkv.dtype or t.device != qkv.device:
+        if t.shape != (batch * seq, heads * D) or t.dtype is not qkv.dtype or t.get_device() != qkv.get_device():
             raise ValueError(f"{name} must be {qkv.dtype} [{batch * seq}, {heads * D}] beside qkv (got {t.dtype} {tuple(t.shape)} on {t.device})")
-    if lse.shape != (batch, heads, seq) or lse.dtype != torch.float32 or lse.device != qkv.device:
+    if lse.shape != (batch, heads, seq) or lse.dtype is not torch.float32 or lse.get_device() != qkv.get_device():
         raise ValueError(f"lse must be fp32 [{batch}, {heads}, {seq}] beside qkv (got {lse.dtype} {tuple(lse.shape)} on {lse.device})")
     if qkv.is_cuda:
-        dqkv = torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
+        dqkv = torch.empty_like(qkv, memory_format=torch.contiguous_format)
         if batch:
-            C = _native.load()
-            scratch = torch.empty(C.window_attention_scratch(batch, seq, kv_heads, group, window, sinks), dtype=torch.float32,
-                                  device=qkv.device)
+            scratch = torch.empty(_scratch(batch, seq, kv_heads, group, window, sinks), dtype=torch.float32, device=qkv.device)
             x, o, do, l = _dense(qkv), _dense(out), _dense(dout), _dense(lse)
-            C.window_attention_bwd(x.data_ptr(), o.data_ptr(), do.data_ptr(), l.data_ptr(), dqkv.data_ptr(), scratch.data_ptr(), batch,
-                                   seq, kv_heads, group, window, sinks, 1.0 / math.sqrt(D), _native.status().dev, _native.stream_ptr())
+            _native.load().window_attention_bwd(x.data_ptr(), o.data_ptr(), do.data_ptr(), l.data_ptr(), dqkv.data_ptr(), scratch.data_ptr(),
+                                                batch, seq, kv_heads, group, window, sinks, _SCALE, _native.status().dev,
+                                                _native.stream_ptr())
         return dqkv
     q, k, v, s = _formulation(qkv, batch, seq, kv_heads, group, window, sinks, D)
     rows_of = lambda t: t.float().view(batch, seq, kv_heads, group, D).permute(0, 2, 3, 1, 4)
@@ -123,6 +131,7 @@ class WindowCache:
                 raise ValueError("the kernel needs contiguous caches on 16-byte boundaries")
         self.k, self.v, self.window, self.sinks = k, v, window, sinks
         self._work = {}
+        self._scale = 1.0 / math.sqrt(k.shape[3])
 
     @classmethod
     def new(cls, batch: int, kv_heads: int, window: int, sinks: int = 0, head_dim: int = HEAD_DIM, dtype=torch.bfloat16, device=None):
@@ -159,11 +168,27 @@ class WindowCache:
         return self._work[group]
 
 
+def _decode(x, pitch: int, cache: WindowCache, positions, batch: int, kv: int, group: int, D: int):
+    out = torch.empty(batch, kv * group * D, dtype=x.dtype, device=x.device)
+    splits, parts, counters = cache.workspace(group)
+    _native.load().window_decode(x.data_ptr(), pitch, cache.k.data_ptr(), cache.v.data_ptr(), positions.data_ptr(), out.data_ptr(), batch,
+                                 kv, group, cache.window, cache.sinks, cache._scale, parts.data_ptr(), counters.data_ptr(), splits,
+                                 _native.stream_ptr())
+    return out
+
+
 def window_attention_decode(qkv, cache: WindowCache, positions, group: int = 1):
     """Attention of one token per sequence, ``qkv`` [batch, kv_heads * (group + 2) * D], at ``positions`` (int64 [batch]) over what
     it sees, itself included.  Stores its key and value in the cache.  A negative position is an idle sequence: nothing is
     stored, its output is zero.  Returns [batch, kv_heads * group * D]."""
-    batch, kv, slots, D = cache.k.shape
+    k = cache.k
+    batch, kv, slots, D = k.shape
+    # the common call, checked in a few steps: a kernel of a few us is over before a longer list of them
+    if (k.is_cuda and group > 0 and qkv.shape == (batch, kv * (group + 2) * D) and qkv.dtype is k.dtype and qkv.is_contiguous()
+            and qkv.data_ptr() & 15 == 0 and positions.dtype is torch.int64 and positions.shape == (batch,) and positions.is_contiguous()
+            and qkv.get_device() == positions.get_device() == k.get_device() and batch):
+        _native.check_device(qkv)
+        return _decode(qkv, qkv.shape[1], cache, positions, batch, kv, group, D)
     if _width(qkv, kv, group, batch) != D:
         raise ValueError(f"the cache holds {D} features per head, the rows {qkv.shape[1] // (kv * (group + 2))}")
     if positions.shape != (batch,) or positions.dtype != torch.int64 or positions.device != qkv.device:
@@ -173,14 +198,10 @@ def window_attention_decode(qkv, cache: WindowCache, positions, group: int = 1):
         raise ValueError(f"rows are {qkv.dtype} on {qkv.device}, the cache {cache.k.dtype} on {cache.k.device}")
     if qkv.is_cuda:
         _native.check_device(qkv)
-        out = torch.empty(batch, kv * group * D, dtype=qkv.dtype, device=qkv.device)
-        if batch:
-            x, positions = rows.as_aligned(qkv), positions.contiguous()
-            splits, parts, counters = cache.workspace(group)
-            _native.load().window_decode(x.data_ptr(), rows.pitch(x), cache.k.data_ptr(), cache.v.data_ptr(), positions.data_ptr(),
-                                         out.data_ptr(), batch, kv, group, cache.window, cache.sinks, 1.0 / math.sqrt(D),
-                                         parts.data_ptr(), counters.data_ptr(), splits, _native.stream_ptr())
-        return out
+        if batch == 0:
+            return qkv.new_empty(0, kv * group * D)
+        x = rows.as_aligned(qkv)
+        return _decode(x, rows.pitch(x), cache, positions.contiguous(), batch, kv, group, D)
     x = qkv.view(batch, kv, group + 2, D)
     out = torch.zeros(batch, kv, group, D, dtype=torch.float32)
     for b, p in enumerate(positions.tolist()):
