@@ -20,7 +20,8 @@ constexpr int kSmem = kWarps * kStages * 2 * kTile;
 constexpr int kPart = kWindowDecodePart;           // floats of a split: O, m, l
 static_assert(kPart == kHeads * (kD + 2), "what a split leaves");
 constexpr float kLog2e = 1.4426950408889634f;
-static_assert(kWarps * kHeads * (kD + 2) * 4 <= kSmem, "the warps' results take the place of the tiles");
+constexpr int kShares = 128;                       // splits that are joined together
+static_assert(kWarps * kHeads * (kD + 2) * 4 <= kSmem && kHeads * (kShares + kD) * 4 <= kSmem, "results take the place of the tiles");
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   // what is not there is filled with zeros: the cache may hold anything beyond the last position
@@ -79,7 +80,7 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
     return;
   }
   const int held = pos < slots ? (int)pos + 1 : slots;
-  const int own = pos < a.sinks ? (int)pos : a.sinks + (int)((pos - a.sinks) % a.window);
+  const int own = pos < a.sinks ? (int)pos : a.sinks + (int)(pos < 1ll << 31 ? (uint32_t)(pos - a.sinks) % (uint32_t)a.window : (pos - a.sinks) % a.window);
   const int s0 = split * per_split, s1 = min(held, s0 + per_split);
   if (s0 >= held) return;
   const int64_t base = ((int64_t)b * a.kv + h) * slots * kD;
@@ -249,17 +250,32 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
   __syncthreads();
   if (!last) return;
   __threadfence();
+  // The shares of the splits first, a warp a head, then their sums, a feature a thread: nothing waits for one split after another.
   const float* parts = a.parts + unit * splits * kPart;
-  for (int head = 0; head < heads; ++head) {
-    float top = -INFINITY;
-    for (int s = 0; s < live; ++s) top = fmaxf(top, __ldcg(parts + s * kPart + kHeads * kD + head));
-    float sum = 0.f, acc = 0.f;
-    for (int s = 0; s < live; ++s) {
-      const float f = exp2_ftz(__ldcg(parts + s * kPart + kHeads * kD + head) - top);
-      sum += f * __ldcg(parts + s * kPart + kHeads * kD + kHeads + head);
-      acc += f * __ldcg(parts + s * kPart + head * kD + d);
+  float *share = so, *rest = so + kHeads * kShares;   // [head][kShares], [head][kD]
+  for (int s0 = 0; s0 < live; s0 += kShares) {     // (all at once for up to kShares splits)
+    const int n = min(kShares, live - s0);
+    __syncthreads();
+    for (int head = warp; head < heads; head += kWarps) {
+      float top = -INFINITY, sum = 0.f;
+      for (int s = lane; s < live; s += 32) top = fmaxf(top, __ldcg(parts + s * kPart + kHeads * kD + head));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int s = lane; s < live; s += 32)
+        sum += exp2_ftz(__ldcg(parts + s * kPart + kHeads * kD + head) - top) * __ldcg(parts + s * kPart + kHeads * kD + kHeads + head);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int s = lane; s < n; s += 32)
+        share[head * kShares + s] = exp2_ftz(__ldcg(parts + (s0 + s) * kPart + kHeads * kD + head) - top) / sum;
     }
-    out[head * kD + d] = __float2bfloat16(acc / sum);
+    __syncthreads();
+    for (int head = 0; head < heads; ++head) {
+      float acc = s0 == 0 ? 0.f : rest[head * kD + d];
+#pragma unroll 8
+      for (int s = 0; s < n; ++s) acc += share[head * kShares + s] * __ldcg(parts + (s0 + s) * kPart + head * kD + d);
+      if (s0 + n == live) out[head * kD + d] = __float2bfloat16(acc);
+      else rest[head * kD + d] = acc;
+    }
   }
 }
 
