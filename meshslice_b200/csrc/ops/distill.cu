@@ -3,6 +3,8 @@
 
 #include <cuda_bf16.h>
 
+#include <type_traits>
+
 #include "../common/f32x2.cuh"
 #include "../common/pdl.cuh"
 #include "../common/ptx.cuh"
@@ -383,9 +385,11 @@ __device__ __forceinline__ void wait_left(int left) {        // for all but the 
 // reads its own vectors in both passes, and as the gradient of one leaves, the same place takes that vector of the CTA's next row: loads
 // run under both passes.  A warp more, the clerk, reads the next row's entries meanwhile, takes their logits out of the row before it is
 // overwritten (kTaken), and writes their columns again once the row's gradient is written (kWritten).
-constexpr int kGroups = kRowBytes / (512 * kVec * 16) + 1;   // groups of vectors of a thread
+// CTAs of an SM by width: a row that fills shared memory alone has sixteen warps, one of up to 8192 columns four; between, eight (4096 rows of
+// 50257, two CTAs an SM: 16 warps 182 us, 12 175, 8 172, 4 200; 8192 of 8000: 8 warps 89 us, 4 78).
+constexpr int row_ctas(int T) { return T == 512 ? 1 : T == 256 ? 3 : 7; }
 template <int K, int T>
-__global__ void __launch_bounds__(T + 32, T == 512 ? 2 : 4)
+__global__ void __launch_bounds__(T + 32, row_ctas(T))
 distill_row_kernel(const __grid_constant__ DistillArgs a) {
   extern __shared__ uint4 ring[];
   __shared__ float red[2][96];
@@ -448,6 +452,7 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
     rewrite(blockIdx.x + (rows - 1) * gridDim.x, parity ^ 1);
     return;
   }
+  constexpr int kGroups = (T == 512 ? kRowBytes : T == 256 ? kRowBytes / 2 + 16 * 1024 : 16 * 1024) / (T * kVec * 16) + 1;   // most groups of a row
   const int groups = (nv + T * kVec - 1) / (T * kVec), whole = valid / (8 * T * kVec);   // whole groups need no tests
   uint4* mine = ring + threadIdx.x;
   auto logits_row = [&](int row) {
@@ -647,19 +652,21 @@ cudaError_t distill_row(const DistillArgs& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   if (valid > distill_row_cols() || a.col_offset != 0 || a.cols < a.vocab) return cudaErrorInvalidValue;
   const int smem = nv * 16 + 3 * entry_bytes(a.top), kind = kind_of(a);
-  // As many CTAs as are resident at a time: by shared memory (228 KiB, 2 KiB a CTA beside the row) and registers (56 a thread).
-  // Sixteen warps a row where no more than two rows fit, else eight.
+  // As many CTAs as are resident at a time: by shared memory (228 KiB, 2 KiB a CTA beside the row) and registers.
   int sms = 148, dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
-  const int fit = 228 * 1024 / (smem + 2048), threads = (fit > 2 ? 256 : 512) + 32, by_registers = 65536 / (56 * threads);
-  auto kernel = fit > 2 ? (kind == kSoft ? distill_row_kernel<kSoft, 256> : kind == kHard ? distill_row_kernel<kHard, 256>
-                           : kind == kSquare ? distill_row_kernel<kSquare, 256> : distill_row_kernel<kTwo, 256>)
-                        : (kind == kSoft ? distill_row_kernel<kSoft, 512> : kind == kHard ? distill_row_kernel<kHard, 512>
-                           : kind == kSquare ? distill_row_kernel<kSquare, 512> : distill_row_kernel<kTwo, 512>);
+  const int fit = 228 * 1024 / (smem + 2048), T = fit < 2 ? 512 : nv > 1024 ? 256 : 128;
+  const auto of_kind = [&](auto width) {
+    constexpr int W = decltype(width)::value;
+    return kind == kSoft ? distill_row_kernel<kSoft, W> : kind == kHard ? distill_row_kernel<kHard, W>
+         : kind == kSquare ? distill_row_kernel<kSquare, W> : distill_row_kernel<kTwo, W>;
+  };
+  auto kernel = T == 512 ? of_kind(std::integral_constant<int, 512>()) : T == 256 ? of_kind(std::integral_constant<int, 256>())
+                                                                                 : of_kind(std::integral_constant<int, 128>());
   e = allow(kernel, smem);
   if (e != cudaSuccess) return e;
-  const int64_t most = (int64_t)sms * (fit < 1 ? 1 : fit < by_registers ? fit : by_registers);
-  return launch_dependent(kernel, (unsigned)(a.rows < most ? a.rows : most), threads, smem, stream, a);
+  const int64_t most = (int64_t)sms * (fit < 1 ? 1 : fit < row_ctas(T) ? fit : row_ctas(T));
+  return launch_dependent(kernel, (unsigned)(a.rows < most ? a.rows : most), T + 32, smem, stream, a);
 }
 cudaError_t distill_partial(const DistillArgs& a, cudaStream_t stream) {
   const cudaError_t e = check(a);
