@@ -11,7 +11,7 @@ namespace msb {
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kUnit = 16;        // features per step of a thread: two 16-byte vectors, eight pairs
 constexpr int kAhead = 4;        // steps whose loads are on their way together
 constexpr int kMaxTokens = 32;   // per CTA
@@ -61,8 +61,8 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s) {
 // A CTA takes a few tokens: first the cosines and sines of their positions, once for all heads, into shared memory, then the
 // rows, 32 bytes a step.  The angle is counted in turns of 2^-64, where position * frequency wraps by itself and keeps 2^-32 of a
 // turn at any position (in fp32 radians a position of 100000 is off by 0.004).
-// Bound by HBM: it reads and writes the rows once (in place: the query and key heads).  8192 tokens of 96 heads of 128: 71 us, 5.6 TB/s
-// (copy: 62).
+// Bound by HBM: it reads and writes the rows once (in place: the query and key heads).  8192 tokens of 96 heads of 128: 63.5 us, 6.3 TB/s
+// (the tensor library's copy 63.7; with 256 threads a CTA 70.5, 512 72.4), in place 45; 16384 tokens of 24 heads 33.7 (copy 34.4).
 template <bool kHalf>
 __global__ void __launch_bounds__(kThreads)
 rotary_kernel(const __grid_constant__ Rows w) {
