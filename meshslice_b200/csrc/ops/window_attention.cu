@@ -848,7 +848,8 @@ struct Streamed {
     }
   }
 };
-template <bool kKeyMajor>
+// kThinItems: few first tokens are streamed alone (not by the kernel of both kinds, which has no registers left for it).
+template <bool kKeyMajor, bool kThinItems>
 __device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) {
   BwdItem w;
   const int nblk = (a.seq + kBlk - 1) / kBlk, group = kKeyMajor ? a.key_group : a.query_group, heads = kKeyMajor ? a.kv : a.heads;
@@ -869,7 +870,7 @@ __device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) 
     w.n_it = w.i0 + max(0, w.blk + 1 - w.per);
   }
   w.kv = kKeyMajor ? w.h : w.h / a.group;
-  w.flags = kMore | (!kKeyMajor && w.i0 == 1 && a.sinks <= kThinKeys && window_block(a, w.blk) > 0 ? kThin : 0);
+  w.flags = kMore | (kThinItems && w.i0 == 1 && a.sinks <= kThinKeys && window_block(a, w.blk) > 0 ? kThin : 0);
   return w;
 }
 
@@ -883,7 +884,7 @@ __device__ __forceinline__ int below(int d) { return d <= -24 ? 0 : ((d + 24) >>
 //                    TMEM lanes = keys, columns = queries: lse / delta vary along the columns.
 // kKeyMajor = false: resident tiles Q, dO (this item's 128 queries), streamed K, V; accumulator dQ.
 //                    TMEM lanes = queries, columns = keys: lse / delta are per thread.
-template <bool kKeyMajor>
+template <bool kKeyMajor, bool kThinItems>
 __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const CUtensorMap& tm_do, const CUtensorMap& tm_dqkv,
                                                const CUtensorMap& tm_thin,
                                               const WinBwdArgs& a, uint8_t* smem, uint32_t tmem, uint32_t item) {
@@ -953,7 +954,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
   const auto dp_phase = [](uint32_t q) -> uint32_t { return (kKeyMajor ? q : q >> 1) & 1; };
   const uint32_t t_acc0 = tmem + (kKeyMajor ? 256 : 384), t_acc1 = tmem + 384;
 
-  BwdItem w = bwd_item<kKeyMajor>(a, item);
+  BwdItem w = bwd_item<kKeyMajor, kThinItems>(a, item);
   bool ok = true;
   // The next item, which the producer of ring 0 has worked out for all: false when there is none of this kind (or on a timeout).
   uint32_t items = 0;                       // items finished by this thread
@@ -990,7 +991,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           if (!(ok = mbar_wait(empty0 + st, ((g / kRing0) & 1) ^ 1, 8 * tmo))) break;
           if (kKeyMajor && staged[st] && !(ok = mbar_wait(out_read0 + st, (outs[st] - 1) & 1, 8 * tmo))) break;
           staged[st] = false;
-          const bool thin = !kKeyMajor && it == 0 && (w.flags & kThin);
+          const bool thin = kThinItems && it == 0 && (w.flags & kThin);
           mbar_expect_tx(full0 + st, thin ? kThinBytes : kTile + (kKeyMajor ? kStatBytes : 0));
           load_tile(sS0 + st * kTile, thin ? &tm_thin : &tm_qkv, full0 + st, kKeyMajor ? col_q(a, w.h, s.h) : col_k(a, w.kv), s.blk * kBlk, w.b);
           if (kKeyMajor) bulk_g2s(sLse + st * kBlk, a.lse2 + stat_at(a, w.b, s.h, s.blk), kStatBytes, full0 + st);
@@ -1008,7 +1009,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           if ((ok = mbar_wait(clc_full, items & 1, 8 * tmo))) {
             more = clc_read(clc_resp, x, y, z) && (x < a.items) == kKeyMajor;
             fence_proxy_async_smem();         // this read before the next response overwrites it
-            if (more) w = bwd_item<kKeyMajor>(a, x);
+            if (more) w = bwd_item<kKeyMajor, kThinItems>(a, x);
             item_slot[0] = make_int4(w.b, w.h, w.blk, w.n_it);
             item_slot[1] = make_int4(w.i0, w.per, w.kv, more ? w.flags : 0);
             mbar_arrive(item_full);
@@ -1039,7 +1040,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
           if (!(ok = mbar_wait(empty1 + st, ((g / kRing1) & 1) ^ 1, 8 * tmo))) break;
           if (staged[st] && !(ok = mbar_wait(out_read + st, (outs[st] - 1) & 1, 8 * tmo))) break;
           staged[st] = false;
-          const bool thin = !kKeyMajor && it == 0 && (w.flags & kThin);
+          const bool thin = kThinItems && it == 0 && (w.flags & kThin);
           mbar_expect_tx(full1 + st, thin ? kThinBytes : kTile + (kKeyMajor ? kStatBytes : 0));
           if (kKeyMajor) {
             load_tile(sS1 + st * kTile, &tm_do, full1 + st, s.h * kD, s.blk * kBlk, w.b);                                // dO
@@ -1112,12 +1113,12 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       };
       // The first blocks of an item also wait for its resident tiles.  An item's last products of either kind free them.
       auto first_s = [&](uint32_t q) -> bool {
-        if (!(wait(res_full, items & 1, 12) && issue_s(q, w.flags & kThin ? id_thin : id_s))) return false;
+        if (!(wait(res_full, items & 1, 12) && issue_s(q, kThinItems && (w.flags & kThin) ? id_thin : id_s))) return false;
         if (w.n_it == 1) umma_commit(res_empty);
         return true;
       };
       auto first_dp = [&](uint32_t q) -> bool {
-        if (!(wait(res_full + 1, items & 1, 12) && issue_dp(q, w.flags & kThin ? id_thin : id_s))) return false;
+        if (!(wait(res_full + 1, items & 1, 12) && issue_dp(q, kThinItems && (w.flags & kThin) ? id_thin : id_s))) return false;
         if (w.n_it == 1) umma_commit(res_empty + 1);
         return true;
       };
@@ -1135,7 +1136,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
       bool early = false;                                 // the next item's first S went before this item's last product
       while (ok && more) {
         const int n = w.n_it;
-        const bool thin_item = !kKeyMajor && (w.flags & kThin);
+        const bool thin_item = kThinItems && (w.flags & kThin);
         for (int it = 0; it < n && ok; ++it, ++g) {
           const bool last = it + 1 == n;
           const uint32_t st0 = g % kRing0, st1 = g % kRing1;
@@ -1214,7 +1215,7 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         const bool masked = kKeyMajor ? c0 < me0 + 24 || (c0 + kBwdCols - 1 - me0 >= a.window && me0 + 24 >= a.key_sinks)
                                       : c0 + kBwdCols - 1 > me || (me - c0 >= a.window && c0 + kBwdCols > a.sinks);
         // of a thin block only the first columns are there
-        const bool mine = kKeyMajor || it > 0 || part == 0 || !(w.flags & kThin);
+        const bool mine = !kThinItems || it > 0 || part == 0 || !(w.flags & kThin);
         float e[kBwdCols];                                // P of this thread's columns
         // ---- phase 1: P = exp2(S * scale * log2(e) - lse2) ----
         // (key-major: lse2 comes with Q and delta with dO, whose barriers order them for this thread)
@@ -1454,13 +1455,13 @@ window_bwd_kernel(const __grid_constant__ CUtensorMap tm_qkv, const __grid_const
     uint32_t item = blockIdx.x, y, z;
     bool more = true;
     while (more) {
-      const bool ok = item < a.items ? window_bwd_run<true>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, item)
-                                     : window_bwd_run<false>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, item);
+      const bool ok = item < a.items ? window_bwd_run<true, false>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, item)
+                                     : window_bwd_run<false, false>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, item);
       more = ok && clc_read(clc_resp, item, y, z);
       fence_proxy_async_smem();             // this read before the next response overwrites it
     }
   } else {
-    window_bwd_run<kKey>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, blockIdx.x);
+    window_bwd_run<kKey, !kKey>(tm_qkv, tm_do, tm_dqkv, tm_thin, a, smem, tmem, blockIdx.x);
   }
   if (warp >= 2 && warp < 2 + kBwdWarps && lane == 0) bulk_wait_all<0>();
   tc_fence_before_sync();
