@@ -20,8 +20,7 @@ constexpr int kSmem = kWarps * kStages * 2 * kTile;
 constexpr int kPart = kWindowDecodePart;           // floats of a split: O, m, l
 static_assert(kPart == kHeads * (kD + 2), "what a split leaves");
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kShares = 128;                       // splits that are joined together
-static_assert(kWarps * kHeads * (kD + 2) * 4 <= kSmem && kHeads * (kShares + kD) * 4 <= kSmem, "results take the place of the tiles");
+static_assert(kWarps * kHeads * (kD + 2) * 4 <= kSmem, "the warps' results take the place of the tiles");
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
   // what is not there is filled with zeros: the cache may hold anything beyond the last position
@@ -213,30 +212,36 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
     }
   }
   __syncthreads();
+  // A warp a head from here on, four features a lane.
   const int live = (held + per_split - 1) / per_split;
-  const int64_t unit = ((int64_t)b * gridDim.y + blockIdx.y);
-  const int d = threadIdx.x;                       // one feature per thread
-  static_assert(kWarps * 32 == kD, "a thread per feature");
+  const int64_t unit = (int64_t)b * gridDim.y + blockIdx.y;
+  const auto store = [&](int head, const float4& v, float by) {
+    *reinterpret_cast<uint2*>(out + head * kD + lane * 4) = make_uint2(pack(v.x * by, v.y * by), pack(v.z * by, v.w * by));
+  };
+  const auto add = [](float4& acc, float f, const float4& v) {
+    acc.x += f * v.x;
+    acc.y += f * v.y;
+    acc.z += f * v.z;
+    acc.w += f * v.w;
+  };
   float* part = a.parts + (unit * splits + split) * kPart;
-  for (int head = 0; head < heads; ++head) {
+  for (int head = warp; head < heads; head += kWarps) {
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) top = fmaxf(top, sm[w * kHeads + head]);
-    float sum = 0.f, acc = 0.f;
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float mw = sm[w * kHeads + head], f = w < tiles ? exp2_ftz(mw - top) : 0.f;   // a warp without a tile has nothing
+      const float f = w < tiles ? exp2_ftz(sm[w * kHeads + head] - top) : 0.f;            // a warp without a tile has nothing
       sum += f * sl[w * kHeads + head];
-      acc += f * so[(w * kHeads + head) * kD + d];
+      add(acc, f, *reinterpret_cast<const float4*>(so + (w * kHeads + head) * kD + lane * 4));
     }
     if (live == 1) {
-      out[head * kD + d] = __float2bfloat16(acc / sum);
+      store(head, acc, 1.f / sum);
     } else {
-      part[head * kD + d] = acc;
-      if (d == 0) {
-        part[kHeads * kD + head] = top;
-        part[kHeads * kD + kHeads + head] = sum;
-      }
+      __stcg(reinterpret_cast<float4*>(part + head * kD + lane * 4), acc);
+      if (lane == 0) __stcg(reinterpret_cast<float2*>(part + kHeads * kD + head * 2), make_float2(top, sum));
     }
   }
   if (live == 1) return;
@@ -250,32 +255,31 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
   __syncthreads();
   if (!last) return;
   __threadfence();
-  // The shares of the splits first, a warp a head, then their sums, a feature a thread: nothing waits for one split after another.
+  // The CTA that finishes last joins them, in their order: a lane has the statistics of every 32nd split.
   const float* parts = a.parts + unit * splits * kPart;
-  float *share = so, *rest = so + kHeads * kShares;   // [head][kShares], [head][kD]
-  for (int s0 = 0; s0 < live; s0 += kShares) {     // (all at once for up to kShares splits)
-    const int n = min(kShares, live - s0);
-    __syncthreads();
-    for (int head = warp; head < heads; head += kWarps) {
-      float top = -INFINITY, sum = 0.f;
-      for (int s = lane; s < live; s += 32) top = fmaxf(top, __ldcg(parts + s * kPart + kHeads * kD + head));
+  const auto stats = [&](int s, int head) {
+    return s < live ? __ldcg(reinterpret_cast<const float2*>(parts + s * kPart + kHeads * kD + head * 2)) : make_float2(-INFINITY, 0.f);
+  };
+  for (int head = warp; head < heads; head += kWarps) {
+    const float2 mine = stats(lane, head);
+    float top = mine.x;
+    for (int s = lane + 32; s < live; s += 32) top = fmaxf(top, stats(s, head).x);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      for (int s = lane; s < live; s += 32)
-        sum += exp2_ftz(__ldcg(parts + s * kPart + kHeads * kD + head) - top) * __ldcg(parts + s * kPart + kHeads * kD + kHeads + head);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      for (int s = lane; s < n; s += 32)
-        share[head * kShares + s] = exp2_ftz(__ldcg(parts + (s0 + s) * kPart + kHeads * kD + head) - top) / sum;
-    }
-    __syncthreads();
-    for (int head = 0; head < heads; ++head) {
-      float acc = s0 == 0 ? 0.f : rest[head * kD + d];
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < live; s0 += 32) {
+      const float2 st = s0 == 0 ? mine : stats(s0 + lane, head);
+      const float f = s0 + lane < live ? exp2_ftz(st.x - top) : 0.f;
+      sum += f * st.y;
+      const int n = min(32, live - s0);
+      const float* from = parts + (int64_t)s0 * kPart + head * kD + lane * 4;
 #pragma unroll 8
-      for (int s = 0; s < n; ++s) acc += share[head * kShares + s] * __ldcg(parts + (s0 + s) * kPart + head * kD + d);
-      if (s0 + n == live) out[head * kD + d] = __float2bfloat16(acc);
-      else rest[head * kD + d] = acc;
+      for (int s = 0; s < n; ++s) add(acc, __shfl_sync(0xffffffffu, f, s), __ldcg(reinterpret_cast<const float4*>(from + (int64_t)s * kPart)));
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    store(head, acc, 1.f / sum);
   }
 }
 
