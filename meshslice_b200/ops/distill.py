@@ -81,22 +81,24 @@ def distill_loss_grad(logits, teacher_ids, teacher_logits, vocab: int, scale: fl
     ``vocab`` on are padding and get 0.  ``teacher_ids`` int64 and ``teacher_logits`` fp32 or bf16 [rows, top].  The gradient goes to
     ``out`` (``out=logits`` works in place) or a new tensor."""
     # the common call, checked in a few steps: a kernel of a few us is over before a longer list of them
-    if (logits.is_cuda and out is None and logits.dtype is torch.bfloat16 and logits.is_contiguous() and logits.data_ptr() & 15 == 0
-            and teacher_ids.dtype is torch.int64 and teacher_ids.shape == teacher_logits.shape and teacher_ids.dim() == logits.dim() == 2
-            and teacher_logits.dtype in _VALUES and teacher_ids.is_contiguous() and teacher_logits.is_contiguous()
-            and (hard_weight == 0.0 if targets is None else targets.dtype is torch.int64 and targets.shape == logits.shape[:1]
-                 and targets.is_contiguous() and targets.get_device() == logits.get_device())
-            and logits.get_device() == teacher_ids.get_device() == teacher_logits.get_device()
-            and 0.0 <= hard_weight <= 1.0 and 0.0 < temperature < math.inf):
+    if (logits.is_cuda and out is None and logits.dtype is torch.bfloat16 and logits.dim() == 2 and logits.is_contiguous()
+            and teacher_ids.dtype is torch.int64 and teacher_ids.dim() == 2 and teacher_ids.is_contiguous()
+            and teacher_logits.dtype in _VALUES and teacher_logits.is_contiguous() and 0.0 <= hard_weight <= 1.0
+            and 0.0 < temperature < math.inf):
         n, cols = logits.shape
-        C = _native.load()
-        m, top = teacher_ids.shape
-        if m == n > 0 and cols % 8 == 0 and 0 < vocab <= min(cols, C.DISTILL_ROW_COLS) and top <= C.DISTILL_TOP:
+        shape, dev, z, C = teacher_ids.shape, logits.get_device(), logits.data_ptr(), _native.load()
+        top = shape[1]
+        if targets is None:
+            y, fine = 0, hard_weight == 0.0
+        else:
+            y, fine = targets.data_ptr(), (targets.dtype is torch.int64 and targets.dim() == 1 and targets.shape[0] == n
+                                           and targets.is_contiguous() and targets.get_device() == dev)
+        if (fine and shape[0] == n > 0 and teacher_logits.shape == shape and teacher_ids.get_device() == dev == teacher_logits.get_device()
+                and cols % 8 == 0 and z & 15 == 0 and 0 < vocab <= cols and vocab <= C.DISTILL_ROW_COLS and top <= C.DISTILL_TOP):
             _native.check_device(logits)
             grad, loss = torch.empty_like(logits), torch.empty(n, dtype=torch.float32, device=logits.device)
-            C.distill(0, logits.data_ptr(), cols, grad.data_ptr(), cols, teacher_ids.data_ptr(), teacher_logits.data_ptr(),
-                      _VALUES[teacher_logits.dtype], 0 if targets is None else targets.data_ptr(), n, cols, 0, vocab, top, temperature,
-                      hard_weight, scale, loss.data_ptr(), 0, _native.stream_ptr())
+            C.distill(0, z, cols, grad.data_ptr(), cols, teacher_ids.data_ptr(), teacher_logits.data_ptr(), _VALUES[teacher_logits.dtype],
+                      y, n, cols, 0, vocab, top, temperature, hard_weight, scale, loss.data_ptr(), 0, _native.stream_ptr())
             return loss, grad
     _check(logits, teacher_ids, teacher_logits, vocab, temperature, targets, hard_weight)
     if logits.shape[1] < vocab:

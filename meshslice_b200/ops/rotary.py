@@ -119,19 +119,20 @@ def rotary_qkv(qkv, rotary: Rotary, kv_heads: int, group: int = 1, seq: Optional
     c = rotary.config
     if qkv.is_cuda:
         # the common call, checked in a few steps: a kernel of 3 us is over before a longer list of them
-        if (out is None and qkv.dtype is torch.bfloat16 and kv_heads > 0 and group > 0 and qkv.is_contiguous() and qkv.data_ptr() & 15 == 0
-                and qkv.shape[1:] == (kv_heads * (group + 2) * c.head_dim,) and qkv.get_device() == rotary.turns.get_device()
-                and (seq is not None and seq > 0 if positions is None else
-                     positions.dtype is torch.int64 and positions.shape == qkv.shape[:1] and positions.is_contiguous()
-                     and positions.get_device() == qkv.get_device())):
-            _native.check_device(qkv)
-            y = torch.empty_like(qkv)
+        if out is None and qkv.dtype is torch.bfloat16 and qkv.dim() == 2 and qkv.is_contiguous() and kv_heads > 0 and group > 0:
             n, width = qkv.shape
-            if n:
-                _native.load().rotary(qkv.data_ptr(), y.data_ptr(), width, width, 0 if positions is None else positions.data_ptr(),
-                                      rotary.turns.data_ptr(), n, seq or 1, kv_heads, group, *rotary._kernel, -1.0 if inverse else 1.0,
-                                      c.cos_factor, _native.stream_ptr())
-            return y
+            turns, dev, x = rotary.turns, qkv.get_device(), qkv.data_ptr()
+            if positions is None:
+                at, fine = 0, seq is not None and seq > 0
+            else:
+                at, fine = positions.data_ptr(), (positions.dtype is torch.int64 and positions.dim() == 1 and positions.shape[0] == n
+                                                  and positions.is_contiguous() and positions.get_device() == dev)
+            if fine and n and x & 15 == 0 and width == kv_heads * (group + 2) * c.head_dim and turns.get_device() == dev:
+                _native.check_device(qkv)
+                y = torch.empty_like(qkv)
+                _native.load().rotary(x, y.data_ptr(), width, width, at, turns.data_ptr(), n, seq or 1, kv_heads, group, *rotary._kernel,
+                                      -1.0 if inverse else 1.0, c.cos_factor, _native.stream_ptr())
+                return y
         _check(qkv, rotary, kv_heads, group, seq, positions, out)
         if qkv.dtype != torch.bfloat16:
             raise ValueError(f"the rotary kernel needs bf16 rows (got {qkv.dtype})")
