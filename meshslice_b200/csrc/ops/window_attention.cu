@@ -1622,8 +1622,11 @@ cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* d
   g.query_group = deal(s.batch * heads);
   const uint32_t keys = (uint32_t)(s.batch * s.kv) * nblk, queries = (uint32_t)(s.batch * heads) * nblk;
   g.items = keys;
-  // Both kinds in one launch where the longer kind leaves SMs free, two beyond: the kernel of both needs more registers.
-  if (queries <= (uint32_t)sm_count())
+  // Both kinds in one launch up to six query-major items an SM, two launches beyond: in one, items of the second kind take the SMs that the
+  // last of the first leave, but the kernel of both is slower by a few per cent.  Two / one, us: 1 x 2048, 12 heads, window 512 (192 items)
+  // 43.1 / 36.4, 8 heads on 4 (256) 57.4 / 50.5; 2 x 3000, 16 on 8, window 500 (768) 127 / 119; 4 x 2048, 16 heads, window 512
+  // (1024) 156 / 158; 2 x 5003, 16 on 4, window 1000 (1280) 271 / 276.
+  if (queries <= 6u * sm_count())
     return launch_dependent(window_bwd_kernel<true, true>, keys + queries, kBwdThreads, kBwdSmem, stream, tq, td, tg, tt, g);
   e = launch_dependent(window_bwd_kernel<true, false>, keys, kBwdThreads, kBwdSmem, stream, tq, td, tg, tt, g);
   if (e != cudaSuccess) return e;
