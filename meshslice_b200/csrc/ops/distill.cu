@@ -68,10 +68,11 @@ __device__ __forceinline__ uint4 cut(uint4 u, int v, int valid) {
   return u;
 }
 
-// Which exponentials a row needs: those of z / T, of z (one kind serves both where T = 1), both, or, where T = 2, those of z as the
-// squares of those of z / T: the special-function unit gives 16 a cycle and SM, so that four of them an element would take 180 us for
-// 4096 rows of 50257 (148 SMs), two 90.
-enum Kind { kSoft = 1, kHard = 2, kTwo = 3, kSquare = 5 };
+// Which exponentials a row needs: those of z / T, of z (one kind serves both where T = 1), both, or, where T = 2 or 4, those of z as the
+// squares of those of z / T, or the squares of these: the special-function unit gives 16 a cycle and SM, so that four of them an element
+// take 180 us for 4096 rows of 50257 (148 SMs), two 90 (temperature 3: 251 us, 2: 172).
+enum Kind { kSoft = 1, kHard = 2, kTwo = 3, kSquare = 5, kFourth = 9 };
+constexpr int powers(int K) { return K == kSquare ? 2 : K == kFourth ? 4 : 1; }
 
 // 2^x exponents of z over a temperature: z c - m c with the product z c exact (one rounding, of the result) and m c rounded once for
 // the whole row: `ref`, the same wherever m is.  Sums are relative to 2^ref; that ref is not quite m c cancels in every ratio, and the
@@ -82,11 +83,11 @@ __device__ __forceinline__ float ref_of(float m, float c) { return __fmul_rn(m, 
 // results takes moves.)
 template <int K>
 struct Sums {
-  static constexpr bool soft_exp = K & kSoft, squares = K == kSquare;
+  static constexpr bool soft_exp = K & kSoft, squares = powers(K) > 1;
   float m = -INFINITY, soft = 0.f, hard = 0.f;
-  // What the sums are relative to; where T = 2 the hard one's is twice the soft one's.
+  // What the sums are relative to; where T = 2 or 4 the hard one's is that times the soft one's.
   __device__ __forceinline__ float soft_ref(float c) const { return ref_of(m, c); }
-  __device__ __forceinline__ float hard_ref(float c) const { return squares ? 2.f * ref_of(m, c) : ref_of(m, kLog2e); }
+  __device__ __forceinline__ float hard_ref(float c) const { return squares ? powers(K) * ref_of(m, c) : ref_of(m, kLog2e); }
   __device__ __forceinline__ void raise(float to, float c) {
     if (to > m) {
       const float s0 = soft_ref(c), h0 = hard_ref(c);
@@ -119,6 +120,10 @@ struct Sums {
           ps[at] += a;
           ps[at + 1] += b;
           if (squares) {
+            if (K == kFourth) {
+              a *= a;
+              b *= b;
+            }
             ph[at] = fmaf(a, a, ph[at]);
             ph[at + 1] = fmaf(b, b, ph[at + 1]);
           }
@@ -328,6 +333,7 @@ __device__ __forceinline__ float grad_of(float e, float hard, const Weights& w) 
   if (K == kSoft) return e * w.soft;
   if (K == kHard) return e * w.hard;
   if (K == kSquare) return e * fmaf(e, w.hard, w.soft);
+  if (K == kFourth) return e * fmaf(e * e, e * w.hard, w.soft);
   return fmaf(e, w.soft, hard * w.hard);
 }
 template <int K>
@@ -594,7 +600,7 @@ distill_grad_kernel(const __grid_constant__ DistillArgs a) {
     }
   }
   __syncthreads();
-  const Weights w = weights_of<K>(a, m, soft / shift(m, c), hard / (K == kSquare ? shift(m, c) * shift(m, c) : shift(m, kLog2e)),
+  const Weights w = weights_of<K>(a, m, soft / shift(m, c), hard / (powers(K) > 1 ? powf(shift(m, c), powers(K)) : shift(m, kLog2e)),
                                   target.some, target.label >= 0);
   for (int k = threadIdx.x; k <= a.top; k += T) {          // before the gradient may overwrite the logits
     const int at = e.at[k] - a.col_offset;
@@ -634,7 +640,7 @@ cudaError_t check_grad(const DistillArgs& a) {
 }
 int kind_of(const DistillArgs& a) {
   if (a.hard == 0.f || a.temperature == 1.f) return kSoft;
-  return a.hard == 1.f ? kHard : a.temperature == 2.f ? kSquare : kTwo;
+  return a.hard == 1.f ? kHard : a.temperature == 2.f ? kSquare : a.temperature == 4.f ? kFourth : kTwo;
 }
 template <class Kernel>
 cudaError_t allow(Kernel kernel, int bytes) {
@@ -659,7 +665,7 @@ cudaError_t distill_row(const DistillArgs& a, cudaStream_t stream) {
   const auto of_kind = [&](auto width) {
     constexpr int W = decltype(width)::value;
     return kind == kSoft ? distill_row_kernel<kSoft, W> : kind == kHard ? distill_row_kernel<kHard, W>
-         : kind == kSquare ? distill_row_kernel<kSquare, W> : distill_row_kernel<kTwo, W>;
+         : kind == kSquare ? distill_row_kernel<kSquare, W> : kind == kFourth ? distill_row_kernel<kFourth, W> : distill_row_kernel<kTwo, W>;
   };
   auto kernel = T == 512 ? of_kind(std::integral_constant<int, 512>()) : T == 256 ? of_kind(std::integral_constant<int, 256>())
                                                                                  : of_kind(std::integral_constant<int, 128>());
@@ -678,7 +684,7 @@ cudaError_t distill_grad(const DistillArgs& a, cudaStream_t stream) {
   if (e != cudaSuccess) return e;
   const int kind = kind_of(a);
   auto kernel = kind == kSoft ? distill_grad_kernel<kSoft> : kind == kHard ? distill_grad_kernel<kHard>
-              : kind == kSquare ? distill_grad_kernel<kSquare> : distill_grad_kernel<kTwo>;
+              : kind == kSquare ? distill_grad_kernel<kSquare> : kind == kFourth ? distill_grad_kernel<kFourth> : distill_grad_kernel<kTwo>;
   return launch_dependent(kernel, a.rows, 512, 2 * entry_bytes(a.top), stream, a);
 }
 
