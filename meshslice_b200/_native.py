@@ -20,6 +20,16 @@ STATUS_NAMES = {
     5: "timeout: waiting for a gathered chunk", 6: "timeout: bulk copy of the communication warp",
     7: "timeout: entry barrier with peers", 8: "timeout: exit barrier with peers",
     9: "timeout: reduce phase waiting for peers' partial tiles", 10: "timeout: waiting for the local go flag",
+    # window attention: forward from 41, backward from 50
+    41: "timeout: window attention, loads", 42: "timeout: window attention, MMA waiting for Q", 43: "timeout: window attention, MMA waiting for K",
+    44: "timeout: window attention, MMA waiting for V or probabilities", 45: "timeout: window attention, softmax waiting for scores",
+    46: "timeout: window attention, next item", 47: "timeout: window attention, output waiting for its sums",
+    50: "window attention backward: shared memory not aligned", 51: "timeout: window attention backward, loads",
+    52: "timeout: window attention backward, MMA waiting for resident tiles",
+    53: "timeout: window attention backward, MMA waiting for streamed tiles", 54: "timeout: window attention backward, MMA waiting for P or dS",
+    55: "timeout: window attention backward, waiting for scores", 56: "timeout: window attention backward, waiting for dP",
+    57: "timeout: window attention backward, output waiting for its sums", 58: "timeout: window attention backward, next item",
+    59: "timeout: window attention backward, MMA waiting for S to be read",
 }
 
 

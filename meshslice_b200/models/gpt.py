@@ -86,7 +86,11 @@ class GPTConfig:
         gemm = 2 * (d * self.qkv_dim + d * d + 2 * d * self.ffn) * self.n_layers + 2 * d * self.vocab_padded
         attn = 4 * self.seq * d * self.n_layers * (0.5 if self.causal else 1.0)
         if self.window and self.window < self.seq:
-            attn *= min(1.0, 2.0 * (self.window + self.sinks) / self.seq)
+            # (query, key) pairs of a window: the triangle of its first queries, whole windows, first tokens beyond them
+            w, far = self.window, self.seq - self.window
+            first = min(far, self.sinks)
+            pairs = w * (w + 1) / 2 + far * w + first * (first + 1) / 2 + (far - first) * min(self.sinks, far)
+            attn *= pairs / (self.seq * self.seq / 2)
         return 3.0 * (gemm + attn)
 
 

@@ -129,9 +129,18 @@ class WindowCache:
                 raise ValueError(f"the kernel needs a bf16 cache with head_dim {HEAD_DIM} (got {k.dtype}, {k.shape[3]})")
             if not (k.is_contiguous() and v.is_contiguous()) or k.data_ptr() % 16 or v.data_ptr() % 16:
                 raise ValueError("the kernel needs contiguous caches on 16-byte boundaries")
-        self.k, self.v, self.window, self.sinks = k, v, window, sinks
+        self._k, self._v, self.window, self.sinks = k, v, window, sinks
         self._work = {}
         self._scale = 1.0 / math.sqrt(k.shape[3])
+
+    # (the tensors stay those that were checked)
+    @property
+    def k(self):
+        return self._k
+
+    @property
+    def v(self):
+        return self._v
 
     @classmethod
     def new(cls, batch: int, kv_heads: int, window: int, sinks: int = 0, head_dim: int = HEAD_DIM, dtype=torch.bfloat16, device=None):

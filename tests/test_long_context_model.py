@@ -152,3 +152,13 @@ def test_decoding_on_a_gpu_is_the_whole_sequence():
     _native.check_status()
     diff = torch.stack(got, 1).float() - want[:, 168:]
     assert diff.norm() < 6 * 2.0 ** -8 * want[:, 168:].norm()
+
+
+def test_operations_of_a_window():
+    """Attention's share of the operations counts the pairs that a window and its first tokens leave."""
+    base = dict(n_layers=3, d_model=128, n_heads=8, ffn=256, vocab=500, vocab_pad=256)
+    for seq, window, sinks in ((50, 7, 0), (50, 7, 3), (64, 60, 30), (40, 1, 1)):
+        pairs = sum(1 for i in range(seq) for j in range(i + 1) if i - j < window or j < sinks)
+        rest = GPTConfig(**base, seq=seq).flops_per_token() - 3 * 4 * seq * 128 * 3 * 0.5
+        got = GPTConfig(**base, seq=seq, window=window, sinks=sinks).flops_per_token() - rest
+        assert abs(got - 3 * 4 * 128 * 3 * pairs / seq) < 1e-6 * got

@@ -143,6 +143,38 @@ def test_kernel(shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(4, 2000, 16, 1, 300, 4), (5, 1500, 16, 1, 200, 20), (3, 1700, 8, 3, 260, 16), (4, 1921, 16, 1, 0, 0),
+                                   (2, 1800, 33, 1, 128, 9)])
+def test_kernel_many_items(shape):
+    """More than six query-major items an SM: the two kinds of gradient items in launches of their own."""
+    test_kernel(shape)
+
+
+@pytest.mark.gpu
+def test_kernel_on_another_stream_and_in_a_graph():
+    shape = (2, 333, 2, 2, 90, 4)
+    qkv, dout, out, lse, dqkv = on_gpu(shape)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x, d = qkv.clone().mul_(1), dout.clone().mul_(1)
+        o, l = F.window_attention_fwd(x, *shape)
+        g = F.window_attention_bwd(d, x, o, l, *shape)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(o, out) and torch.equal(g, dqkv)
+    x, d = torch.zeros_like(qkv), torch.zeros_like(dout)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, l = F.window_attention_fwd(x, *shape)
+        g = F.window_attention_bwd(d, x, o, l, *shape)
+    for times in (1, 2):
+        x.copy_(qkv)
+        d.copy_(dout)
+        graph.replay()
+        assert torch.equal(o, out) and torch.equal(l, lse) and torch.equal(g, dqkv)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(2, 300, 2, 2, 100, 4), (3, 1100, 9, 2, 256, 4)])
 def test_kernel_is_deterministic_and_reads_strided_tensors(shape):
     batch, seq, kv, group, window, sinks = shape

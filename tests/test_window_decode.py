@@ -66,6 +66,8 @@ def refusals(dev):
             F.window_attention_decode(*args)
     with pytest.raises(ValueError):
         cache.fill(x, 2)
+    with pytest.raises(AttributeError):
+        cache.k = k
 
 
 def test_refusals():
@@ -74,7 +76,7 @@ def test_refusals():
 
 # ---------------------------------------------------------------------------------------------- on a GPU
 @pytest.mark.gpu
-@pytest.mark.parametrize("size", SIZES + [(2, 2, 4, 300, 4), (1, 1, 1, 2000, 0)])
+@pytest.mark.parametrize("size", SIZES + [(2, 2, 4, 300, 4), (1, 1, 1, 2000, 0), (1, 1, 3, 6000, 5)])
 def test_kernel(size):
     """Positions from the first to far beyond the window; every slot that holds nothing yet is NaN."""
     batch, kv, group, window, sinks = size
