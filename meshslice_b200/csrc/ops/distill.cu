@@ -391,6 +391,9 @@ __device__ __forceinline__ void wait_left(int left) {        // for all but the 
 // reads its own vectors in both passes, and as the gradient of one leaves, the same place takes that vector of the CTA's next row: loads
 // run under both passes.  A warp more, the clerk, reads the next row's entries meanwhile, takes their logits out of the row before it is
 // overwritten (kTaken), and writes their columns again once the row's gradient is written (kWritten).
+// 4096 rows of 50257 at temperature 2: 172 us (4.8 TB/s; without arithmetic 142: the rows of an SM take turns between the passes).  One CTA a
+// row that begins when the one before it ends 514; persistent with sixteen warps 216; entries held a row ahead and no work on vectors
+// that are not there 183.
 // CTAs of an SM by width: a row that fills shared memory alone has sixteen warps, one of up to 8192 columns four; between, eight (4096 rows of
 // 50257, two CTAs an SM: 16 warps 182 us, 12 175, 8 172, 4 200; 8192 of 8000: 8 warps 89 us, 4 78).
 constexpr int row_ctas(int T) { return T == 512 ? 1 : T == 256 ? 3 : 7; }

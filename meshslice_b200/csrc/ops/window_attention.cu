@@ -117,8 +117,14 @@ __device__ __forceinline__ void warp_store_box(const CUtensorMap* map, const voi
 // ==========================================================================================
 // forward
 // ==========================================================================================
+// softmax(q k^T scale) v with the running maximum and sum of each row, in the log2 domain: m and l rescaled when the maximum grows by more
+// than 2^8, one division at the end.  P is rounded to bf16 as the operand of P V (its sum l is not), the output once.
 // Roles and tensor memory as in attn_fwd2_kernel: producer, MMA issuer, a softmax warpgroup for each of two neighbouring query
 // tiles.  Both tiles walk one list of key blocks through the same K / V rings; each leaves out what it does not see.
+// What bounds it: a step of both tiles takes 3260 cycles (2048 of the special-function unit, 1024 of products a tile), a masked block 650
+// more, an item's end 2900 in which the output leaves and nothing is multiplied; below windows of about 200, HBM.  4 x 2048, 32 heads: window
+// 128 54 us (6.2 TB/s), 512 with 4 first tokens 90; 1 x 16384, 16 heads on 4, window 4096 405 us (1190 TFLOP/s; under the power cap 468).
+// First tokens as whole blocks took 102 us of the 90; tile 1's own block at the head of the list 97.
 constexpr int kFwdWarpStage = 32 * 128;   // output staging per softmax warp: 32 rows x 64 columns
 constexpr size_t kFwdSmem = 6 * kTile + 8 * kFwdWarpStage + 256 + 1024;
 constexpr int kFwdThreads = 384;
@@ -791,7 +797,12 @@ window_parts_kernel(const float* parts, float* sums, int chunks) {
 }
 
 // Key-major items accumulate dV and dK of 128 keys over the query blocks that see them, of every head of the group; query-major
-// items dQ of 128 queries over their list of key blocks.  Roles, rings and tensor memory as in attn_bwd2_kernel.
+// items dQ of 128 queries over their list of key blocks.  Roles, rings and tensor memory as in attn_bwd2_kernel.  P (for dV) and dS
+// are rounded to bf16 as operands; dS is formed from P in fp32.
+// What bounds it: a key-major pair takes 2650 cycles (2048 of products), an item about 5000 more in which its output leaves and the next
+// one's tiles arrive; over long runs the power cap (1.5 GHz), which gives back in clock about half of what a cycle saved brings.
+// 4 x 2048, 32 heads, window 512, 4 first tokens: 299 us (key-major 150, query-major 110, row sums and first tokens 37; first tokens in items of
+// their own kind 327); 2 x 5003, 16 heads on 4, window 1000, 16 first tokens: 271 (418).
 constexpr int kBwdPoly = 2;                 // key-major: exponentials of every eight that run on the FMA pipe
 constexpr int kBwdWarps = 16;               // element-wise warps
 constexpr int kBwdCols = kBlk * 4 / kBwdWarps;   // columns of a row per element-wise thread
