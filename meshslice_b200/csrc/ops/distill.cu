@@ -70,7 +70,7 @@ __device__ __forceinline__ uint4 cut(uint4 u, int v, int valid) {
 
 // Which exponentials a row needs: those of z / T, of z (one kind serves both where T = 1), both, or, where T = 2 or 4, those of z as the
 // squares of those of z / T, or the squares of these: the special-function unit gives 16 a cycle and SM, so that four of them an element
-// take 180 us for 4096 rows of 50257 (148 SMs), two 90 (temperature 3: 251 us, 2: 172).
+// take 180 us for 4096 rows of 50257 (148 SMs), two 90 (temperature 3: 239 us, 2: 165).
 enum Kind { kSoft = 1, kHard = 2, kTwo = 3, kSquare = 5, kFourth = 9 };
 constexpr int powers(int K) { return K == kSquare ? 2 : K == kFourth ? 4 : 1; }
 
@@ -381,19 +381,13 @@ __device__ __forceinline__ float loss_of(const DistillArgs& a, const RowTarget& 
 enum { kSums = 1, kTaken = 2, kWritten = 3 };
 __device__ __forceinline__ void bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 __device__ __forceinline__ void bar_arrive(int id, int threads) { asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-template <int N>
-__device__ __forceinline__ void wait_left(int left) {        // for all but the last `left` <= N groups
-  if (left == N) cp_async_wait<N>();
-  else if constexpr (N > 0) wait_left<N - 1>(left);
-}
-
 // Whole rows: a row waits in shared memory between the sums and the gradient, so the logits are read once.  Persistent CTAs: a thread
 // reads its own vectors in both passes, and as the gradient of one leaves, the same place takes that vector of the CTA's next row: loads
 // run under both passes.  A warp more, the clerk, reads the next row's entries meanwhile, takes their logits out of the row before it is
 // overwritten (kTaken), and writes their columns again once the row's gradient is written (kWritten).
-// 4096 rows of 50257 at temperature 2: 172 us (4.8 TB/s; without arithmetic 142: the rows of an SM take turns between the passes).  One CTA a
+// 4096 rows of 50257 at temperature 2: 165 us (5.1 TB/s; without arithmetic 142: the rows of an SM take turns between the passes).  One CTA a
 // row that begins when the one before it ends 514; persistent with sixteen warps 216; entries held a row ahead and no work on vectors
-// that are not there 183.
+// that are not there 183; by the widths below 172, with a row's copies in two groups instead of one for every four vectors 165.
 // CTAs of an SM by width: a row that fills shared memory alone has sixteen warps, one of up to 8192 columns four; between, eight (4096 rows of
 // 50257, two CTAs an SM: 16 warps 182 us, 12 175, 8 172, 4 200; 8192 of 8000: 8 warps 89 us, 4 78).
 constexpr int row_ctas(int T) { return T == 512 ? 1 : T == 256 ? 3 : 7; }
@@ -461,43 +455,41 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
     rewrite(blockIdx.x + (rows - 1) * gridDim.x, parity ^ 1);
     return;
   }
-  constexpr int kGroups = (T == 512 ? kRowBytes : T == 256 ? kRowBytes / 2 + 16 * 1024 : 16 * 1024) / (T * kVec * 16) + 1;   // most groups of a row
-  const int groups = (nv + T * kVec - 1) / (T * kVec), whole = valid / (8 * T * kVec);   // whole groups need no tests
+  // Whole groups of kVec vectors a thread need no tests; what is left is worked on by the warps that have something of it.  A row's copies
+  // are two groups to wait for: the first `half` whole groups, the others.
+  constexpr int kStep = kVec * T;
+  const int whole = valid / (8 * kStep), half = whole >> 1, rest = threadIdx.x + whole * kStep;
   uint4* mine = ring + threadIdx.x;
   auto logits_row = [&](int row) {
-    return reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld) + threadIdx.x;
+    return reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(a.logits) + (int64_t)row * a.ld);
   };
-  auto fetch = [&](const uint4* z, int g) {
-    uint4* to = mine + g * (kVec * T);
-    z += g * (kVec * T);
-    if (g < whole) {
+  {
+    const uint4* z = logits_row(blockIdx.x);
+    for (int g = 0; g < whole; ++g) {
 #pragma unroll
-      for (int j = 0; j < kVec; ++j) cp_async16(to + j * T, z + j * T);
-    } else {
-#pragma unroll
-      for (int j = 0; j < kVec; ++j)
-        if (threadIdx.x + (g * kVec + j) * T < nv) cp_async16(to + j * T, z + j * T);
+      for (int j = 0; j < kVec; ++j) cp_async16(mine + g * kStep + j * T, z + threadIdx.x + g * kStep + j * T);
+      if (g + 1 == half) cp_async_commit();
     }
+    for (int v = rest; v < nv; v += T) cp_async16(ring + v, z + v);
     cp_async_commit();
-  };
-  for (int g = 0; g < groups; ++g) fetch(logits_row(blockIdx.x), g);
+  }
   for (int row = blockIdx.x; row < a.rows; row += gridDim.x, parity ^= 1) {
     Sums<K> sum;
-    for (int g = 0; g < groups; ++g) {
-      wait_left<kGroups>(groups - 1 - g);
-      const uint4* at = mine + g * (kVec * T);
-      if (g < whole) {
+    {
+      const uint4* at = mine;
+      if (half > 0) cp_async_wait<1>();
+      for (int g = 0; g < whole; ++g, at += kStep) {
+        if (g == half) cp_async_wait<0>();
         uint4 u[kVec];
 #pragma unroll
         for (int j = 0; j < kVec; ++j) u[j] = at[j * T];
         sum.add(u, c);
-      } else {
-        // what does not fill a group is worked on by the warps that have something of it
+      }
+      if (whole == 0) cp_async_wait<0>();
 #pragma unroll 1
-        for (int v = threadIdx.x + g * kVec * T; v < nv; v += T) {
-          const uint4 u[1] = {cut(ring[v], v, valid)};
-          sum.add(u, c);
-        }
+      for (int v = rest; v < nv; v += T) {
+        const uint4 u[1] = {cut(ring[v], v, valid)};
+        sum.add(u, c);
       }
     }
     sum.leave(c, red[parity]);
@@ -506,25 +498,35 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
     const Weights w = weights_of<K>(a, sum.m, sum.soft, sum.hard, has[parity] != 0, labels[parity] >= 0);
     // (rows that nothing is learnt from get zeros, whatever their logits are)
     const bool learnt = w.drop != 0.f || w.label != 0.f, more = row + (int)gridDim.x < a.rows;
-    const uint4* next = logits_row(row + gridDim.x);
-    uint4* out = reinterpret_cast<uint4*>(out_row(row)) + threadIdx.x;
-    for (int g = 0; g < groups; ++g) {
-      const uint4* at = mine + g * (kVec * T);
-      uint4* to = out + g * (kVec * T);
-      if (g < whole && learnt) {
+    const uint4* z = logits_row(more ? row + gridDim.x : row);
+    uint4* out = reinterpret_cast<uint4*>(out_row(row));
+    {
+      const uint4 *at = mine, *next = z + threadIdx.x;
+      uint4* to = out + threadIdx.x;
+      for (int g = 0; g < whole; ++g, at += kStep, to += kStep, next += kStep) {
+        if (learnt) {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) to[j * T] = grad_whole<K>(at[j * T], w, c);
-      } else {
+          for (int j = 0; j < kVec; ++j) to[j * T] = grad_whole<K>(at[j * T], w, c);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kVec; ++j) {
-          const int v = threadIdx.x + (g * kVec + j) * T;
-          if (v < nv) to[j * T] = learnt ? grad_vector<K>(at[j * T], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+          for (int j = 0; j < kVec; ++j) to[j * T] = make_uint4(0u, 0u, 0u, 0u);
         }
+        if (g == 0) bar_sync(kTaken, T + 32);      // the clerk has what it wants of this row
+        if (more) {
+#pragma unroll
+          for (int j = 0; j < kVec; ++j) cp_async16(const_cast<uint4*>(at) + j * T, next + j * T);
+        }
+        if (g + 1 == half) cp_async_commit();
       }
-      if (g == 0) bar_sync(kTaken, T + 32);
-      if (more) fetch(next, g);
     }
-    for (int v = nv + threadIdx.x; v < nvec; v += T) out[v - threadIdx.x] = make_uint4(0u, 0u, 0u, 0u);
+    if (whole == 0) bar_sync(kTaken, T + 32);
+#pragma unroll 1
+    for (int v = rest; v < nv; v += T) {
+      out[v] = learnt ? grad_vector<K>(ring[v], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+      if (more) cp_async16(ring + v, z + v);
+    }
+    cp_async_commit();
+    for (int v = nv + threadIdx.x; v < nvec; v += T) out[v] = make_uint4(0u, 0u, 0u, 0u);
     bar_arrive(kWritten, T + 32);
   }
 }
