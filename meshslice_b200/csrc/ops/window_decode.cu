@@ -58,7 +58,7 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
 // sixth of what that path does beside the memory, and the operands come as rows of any number and origin.
 // The token's own k and v are taken from `qkv` in place of their slot, which the CTA that has it writes.
 // Splits of a sequence are joined, in their order, by the CTA that finishes last.  P is rounded to bf16 as the operand of P V.
-// Bound by HBM: 64 sequences of up to 4100 slots, 8 x 4 heads, 160 us (6.0 TB/s); one sequence of 700 tokens by the launch and three
+// Bound by HBM: 64 sequences of up to 4100 slots, 8 x 4 heads, 145 us (6.6 TB/s); one sequence of 700 tokens by the launch and three
 // trips to memory (position, tiles, splits): 6.7 us, 14.7 when the splits were joined one after another.
 // kWide: more than 8 query heads (rows 8 to 15 of the fragments are in use).
 template <bool kWide>
@@ -262,36 +262,56 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
   const auto stats = [&](int s, int head) {
     return s < live ? __ldcg(reinterpret_cast<const float2*>(parts + s * kPart + kHeads * kD + head * 2)) : make_float2(-INFINITY, 0.f);
   };
-  for (int head = warp; head < heads; head += kWarps) {
-    const float2 mine = stats(lane, head);
-    float top = mine.x;
-    for (int s = lane + 32; s < live; s += 32) top = fmaxf(top, stats(s, head).x);
+  // (the heads of a warp together: their splits are on their way at the same time)
+  constexpr int kEach = (kWide ? kHeads : 8) / kWarps;
+  float top[kEach], sum[kEach];
+  float4 acc[kEach];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < live; s0 += 32) {
-      const float2 st = s0 == 0 ? mine : stats(s0 + lane, head);
-      const float f = s0 + lane < live ? exp2_ftz(st.x - top) : 0.f;
-      sum += f * st.y;
-      const int n = min(32, live - s0);
-      const float* from = parts + (int64_t)s0 * kPart + head * kD + lane * 4;
-#pragma unroll 8
-      for (int s = 0; s < n; ++s) add(acc, __shfl_sync(0xffffffffu, f, s), __ldcg(reinterpret_cast<const float4*>(from + (int64_t)s * kPart)));
+  for (int i = 0; i < kEach; ++i) {
+    const int head = min(warp + i * kWarps, heads - 1);
+    float t = -INFINITY;
+    for (int s = lane; s < live; s += 32) t = fmaxf(t, stats(s, head).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+    top[i] = t;
+    sum[i] = 0.f;
+    acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int s0 = 0; s0 < live; s0 += 32) {
+    float f[kEach];
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const float2 st = stats(s0 + lane, min(warp + i * kWarps, heads - 1));
+      f[i] = s0 + lane < live ? exp2_ftz(st.x - top[i]) : 0.f;
+      sum[i] += f[i] * st.y;
     }
+    const int n = min(32, live - s0);
+    const float* from = parts + (int64_t)s0 * kPart + lane * 4;
+#pragma unroll 4
+    for (int s = 0; s < n; ++s)
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    store(head, acc, 1.f / sum);
+      for (int i = 0; i < kEach; ++i)
+        add(acc[i], __shfl_sync(0xffffffffu, f[i], s),
+            __ldcg(reinterpret_cast<const float4*>(from + (int64_t)s * kPart + min(warp + i * kWarps, heads - 1) * kD)));
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    float t = sum[i];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+    if (warp + i * kWarps < heads) store(warp + i * kWarps, acc[i], 1.f / t);
   }
 }
 
 }  // namespace
 
+// One wave of two CTAs an SM, each with three tiles or more for every warp: a split more costs every sequence a trip through memory (8 us) and
+// every CTA its start.  us by splits: 64 sequences of 8 key heads, 4100 slots, 1 143, 2 152, 6 148; 256 of 8, 512 slots, 1 85, 2 119; 16 of 8,
+// 4100, 1 58, 2 50, 4 49, 12 58; 8 of 2, 8196, 6 30, 12 22.6, 18 22.8, 37 32; 1 of 8, 4100, 6 15, 18 12.7, 37 15.
 int window_decode_splits(int batch, int kv, int group, int slots, int sms) {
   const int64_t units = (int64_t)batch * kv * ((group + kHeads - 1) / kHeads);
-  const int64_t most = (slots + kWarps * kKeys - 1) / (kWarps * kKeys);        // a tile for every warp
-  const int64_t want = ((int64_t)sms * 4 + units - 1) / units;
-  return (int)(want < most ? want : most);
+  const int64_t most = (slots + 3 * kWarps * kKeys - 1) / (3 * kWarps * kKeys), want = (int64_t)sms * 2 / units;
+  return (int)(want < 1 ? 1 : want < most ? want : most);
 }
 
 cudaError_t window_decode(const WindowDecodeArgs& a, int splits, cudaStream_t stream) {
