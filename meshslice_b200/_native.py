@@ -83,10 +83,17 @@ def _init_cuda():
 
 def check_device(t) -> None:
     """Refuse a tensor of another GPU than the current one, whose stream the launch would go to."""
+    stream_on(t.get_device())
+
+
+def stream_on(device: int) -> int:
+    """``stream_ptr()`` for tensors on GPU ``device``, which has to be the current one."""
     if _cuda is None:
         _init_cuda()
-    if t.get_device() != _cuda._cuda_getDevice():
-        raise ValueError(f"the tensor is on {t.device}, the current GPU is cuda:{_cuda._cuda_getDevice()}")
+    here = _cuda._cuda_getDevice()
+    if device != here:
+        raise ValueError(f"the tensors are on cuda:{device}, the current GPU is cuda:{here}")
+    return _cuda._cuda_getCurrentRawStream(here)
 
 
 def _block_here(t) -> bool:

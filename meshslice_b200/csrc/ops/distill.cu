@@ -664,8 +664,12 @@ cudaError_t distill_row(const DistillArgs& a, cudaStream_t stream) {
   if (valid > distill_row_cols() || a.col_offset != 0 || a.cols < a.vocab) return cudaErrorInvalidValue;
   const int smem = nv * 16 + 3 * entry_bytes(a.top), kind = kind_of(a);
   // As many CTAs as are resident at a time: by shared memory (228 KiB, 2 KiB a CTA beside the row) and registers.
+  static int counts[64] = {0};
   int sms = 148, dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev >= 0 && dev < 64) {
+    if (counts[dev] == 0 && cudaDeviceGetAttribute(&counts[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) counts[dev] = 148;
+    sms = counts[dev];
+  }
   const int fit = 228 * 1024 / (smem + 2048), T = fit < 2 ? 512 : nv > 1024 ? 256 : 128;
   const auto of_kind = [&](auto width) {
     constexpr int W = decltype(width)::value;

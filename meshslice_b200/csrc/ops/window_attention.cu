@@ -881,7 +881,7 @@ __device__ __forceinline__ BwdItem bwd_item(const WinBwdArgs& a, uint32_t item) 
     w.n_it = w.i0 + max(0, w.blk + 1 - w.per);
   }
   w.kv = kKeyMajor ? w.h : w.h / a.group;
-  w.flags = kMore | (kThinItems && w.i0 == 1 && a.sinks <= kThinKeys && window_block(a, w.blk) > 0 ? kThin : 0);
+  w.flags = kMore | (kThinItems && w.i0 == 1 && a.far != nullptr && window_block(a, w.blk) > 0 ? kThin : 0);
   return w;
 }
 
@@ -1539,13 +1539,15 @@ cudaError_t window_attention_fwd(const void* qkv, void* out, float* lse, const W
   CUtensorMap tq, to, tt;
   const uint64_t width = (uint64_t)s.kv * (s.group + 2) * kD;
   if (make_tensor_map_seq(&tq, qkv, width, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
-  if (make_tensor_map_seq(&tt, qkv, width, s.seq, s.batch, 64, kThinKeys) != 0) return cudaErrorInvalidValue;
+  const bool thin = s.sinks > 0 && s.sinks <= kThinKeys && s.seq > kBlk;
+  if (!thin) tt = tq;
+  else if (make_tensor_map_seq(&tt, qkv, width, s.seq, s.batch, 64, kThinKeys) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&to, out, (uint64_t)heads * kD, s.seq, s.batch, 64, 32) != 0) return cudaErrorInvalidValue;
   WinArgs a{};
   a.batch = s.batch; a.seq = s.seq; a.kv = s.kv; a.group = s.group; a.heads = heads;
   a.window = s.window == 0 || s.window > s.seq ? s.seq : s.window;
   a.sinks = s.sinks < s.seq ? s.sinks : s.seq;
-  a.thin = a.sinks <= kThinKeys ? 1 : 0;
+  a.thin = thin ? 1 : 0;
   a.scale = s.scale;
   a.lse = lse;
   a.status = status;
@@ -1583,10 +1585,11 @@ cudaError_t window_attention_bwd(const void* qkv, const void* out, const void* d
   const int heads = s.kv * s.group, nblk = blocks_of(s.seq);
   const uint64_t width = (uint64_t)s.kv * (s.group + 2) * kD;
   CUtensorMap tq, td, tg, tt;
-  if (make_tensor_map_seq(&tt, qkv, width, s.seq, s.batch, 64, kThinKeys) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&tq, qkv, width, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&td, dout, (uint64_t)heads * kD, s.seq, s.batch, 64, kBlk) != 0) return cudaErrorInvalidValue;
   if (make_tensor_map_seq(&tg, dqkv, width, s.seq, s.batch, kBwdCols, 32) != 0) return cudaErrorInvalidValue;
+  tt = tq;
+  if (thin_chunks(s) > 0 && make_tensor_map_seq(&tt, qkv, width, s.seq, s.batch, 64, kThinKeys) != 0) return cudaErrorInvalidValue;
   WinBwdArgs g{};
   float* delta = scratch + (int64_t)s.batch * heads * nblk * kBlk;
   const int chunks = thin_chunks(s);

@@ -95,10 +95,10 @@ def distill_loss_grad(logits, teacher_ids, teacher_logits, vocab: int, scale: fl
                                            and targets.is_contiguous() and targets.get_device() == dev)
         if (fine and shape[0] == n > 0 and teacher_logits.shape == shape and teacher_ids.get_device() == dev == teacher_logits.get_device()
                 and cols % 8 == 0 and z & 15 == 0 and 0 < vocab <= cols and vocab <= C.DISTILL_ROW_COLS and top <= C.DISTILL_TOP):
-            _native.check_device(logits)
+            stream = _native.stream_on(dev)
             grad, loss = torch.empty_like(logits), torch.empty(n, dtype=torch.float32, device=logits.device)
             C.distill(0, z, cols, grad.data_ptr(), cols, teacher_ids.data_ptr(), teacher_logits.data_ptr(), _VALUES[teacher_logits.dtype],
-                      y, n, cols, 0, vocab, top, temperature, hard_weight, scale, loss.data_ptr(), 0, _native.stream_ptr())
+                      y, n, cols, 0, vocab, top, temperature, hard_weight, scale, loss.data_ptr(), 0, stream)
             return loss, grad
     _check(logits, teacher_ids, teacher_logits, vocab, temperature, targets, hard_weight)
     if logits.shape[1] < vocab:

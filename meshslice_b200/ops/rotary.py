@@ -127,11 +127,12 @@ def rotary_qkv(qkv, rotary: Rotary, kv_heads: int, group: int = 1, seq: Optional
             else:
                 at, fine = positions.data_ptr(), (positions.dtype is torch.int64 and positions.dim() == 1 and positions.shape[0] == n
                                                   and positions.is_contiguous() and positions.get_device() == dev)
-            if fine and n and x & 15 == 0 and width == kv_heads * (group + 2) * c.head_dim and turns.get_device() == dev:
-                _native.check_device(qkv)
+            D, rot, half = rotary._kernel
+            if fine and n and x & 15 == 0 and width == kv_heads * (group + 2) * D and turns.get_device() == dev:
+                stream = _native.stream_on(dev)
                 y = torch.empty_like(qkv)
-                _native.load().rotary(x, y.data_ptr(), width, width, at, turns.data_ptr(), n, seq or 1, kv_heads, group, *rotary._kernel,
-                                      -1.0 if inverse else 1.0, c.cos_factor, _native.stream_ptr())
+                _native.load().rotary(x, y.data_ptr(), width, width, at, turns.data_ptr(), n, seq or 1, kv_heads, group, D, rot, half,
+                                      -1.0 if inverse else 1.0, c.cos_factor, stream)
                 return y
         _check(qkv, rotary, kv_heads, group, seq, positions, out)
         if qkv.dtype != torch.bfloat16:

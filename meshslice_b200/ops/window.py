@@ -38,6 +38,9 @@ _SCALE = 1.0 / math.sqrt(HEAD_DIM)
 
 
 def _check(qkv, batch: int, seq: int, kv_heads: int, group: int, window: int, sinks: int) -> int:
+    if (qkv.is_cuda and qkv.dtype is torch.bfloat16 and batch >= 0 and seq > 0 and kv_heads > 0 and group > 0 and window >= 0 and sinks >= 0
+            and qkv.shape == (batch * seq, kv_heads * (group + 2) * HEAD_DIM)):
+        return HEAD_DIM
     if batch < 0 or seq < 1 or window < 0 or sinks < 0:
         raise ValueError(f"attention needs seq >= 1, window >= 0 (0: no window) and sinks >= 0 (got batch {batch}, seq {seq}, "
                          f"window {window}, sinks {sinks})")
@@ -45,7 +48,6 @@ def _check(qkv, batch: int, seq: int, kv_heads: int, group: int, window: int, si
     if qkv.is_cuda:
         if qkv.dtype != torch.bfloat16 or D != HEAD_DIM:
             raise ValueError(f"the window attention kernel needs bf16 rows with head_dim {HEAD_DIM} (got {qkv.dtype}, {D})")
-        _native.check_device(qkv)
     return D
 
 
@@ -70,12 +72,13 @@ def window_attention_fwd(qkv, batch: int, seq: int, kv_heads: int, group: int = 
     D = _check(qkv, batch, seq, kv_heads, group, window, sinks)
     heads = kv_heads * group
     if qkv.is_cuda:
-        out = torch.empty(batch * seq, heads * D, dtype=qkv.dtype, device=qkv.device)
-        lse = torch.empty(batch, heads, seq, dtype=torch.float32, device=qkv.device)
+        stream, device = _native.stream_on(qkv.get_device()), qkv.device
+        out = torch.empty(batch * seq, heads * D, dtype=qkv.dtype, device=device)
+        lse = torch.empty(batch, heads, seq, dtype=torch.float32, device=device)
         if batch:
             x = _dense(qkv)
             _native.load().window_attention_fwd(x.data_ptr(), out.data_ptr(), lse.data_ptr(), batch, seq, kv_heads, group, window, sinks,
-                                                _SCALE, _native.status().dev, _native.stream_ptr())
+                                                _SCALE, _native.status().dev, stream)
         return out, lse
     q, k, v, s = _formulation(qkv, batch, seq, kv_heads, group, window, sinks, D)
     o = torch.softmax(s, -1) @ v
@@ -92,13 +95,13 @@ def window_attention_bwd(dout, qkv, out, lse, batch: int, seq: int, kv_heads: in
     if lse.shape != (batch, heads, seq) or lse.dtype is not torch.float32 or lse.get_device() != qkv.get_device():
         raise ValueError(f"lse must be fp32 [{batch}, {heads}, {seq}] beside qkv (got {lse.dtype} {tuple(lse.shape)} on {lse.device})")
     if qkv.is_cuda:
-        dqkv = torch.empty_like(qkv, memory_format=torch.contiguous_format)
+        stream = _native.stream_on(qkv.get_device())
+        dqkv = torch.empty_like(qkv) if qkv.is_contiguous() else torch.empty(qkv.shape, dtype=qkv.dtype, device=qkv.device)
         if batch:
             scratch = torch.empty(_scratch(batch, seq, kv_heads, group, window, sinks), dtype=torch.float32, device=qkv.device)
             x, o, do, l = _dense(qkv), _dense(out), _dense(dout), _dense(lse)
             _native.load().window_attention_bwd(x.data_ptr(), o.data_ptr(), do.data_ptr(), l.data_ptr(), dqkv.data_ptr(), scratch.data_ptr(),
-                                                batch, seq, kv_heads, group, window, sinks, _SCALE, _native.status().dev,
-                                                _native.stream_ptr())
+                                                batch, seq, kv_heads, group, window, sinks, _SCALE, _native.status().dev, stream)
         return dqkv
     q, k, v, s = _formulation(qkv, batch, seq, kv_heads, group, window, sinks, D)
     rows_of = lambda t: t.float().view(batch, seq, kv_heads, group, D).permute(0, 2, 3, 1, 4)
@@ -178,11 +181,12 @@ class WindowCache:
 
 
 def _decode(x, pitch: int, cache: WindowCache, positions, batch: int, kv: int, group: int, D: int):
+    stream = _native.stream_on(x.get_device())
     out = torch.empty(batch, kv * group * D, dtype=x.dtype, device=x.device)
     splits, parts, counters = cache.workspace(group)
     _native.load().window_decode(x.data_ptr(), pitch, cache.k.data_ptr(), cache.v.data_ptr(), positions.data_ptr(), out.data_ptr(), batch,
                                  kv, group, cache.window, cache.sinks, cache._scale, parts.data_ptr(), counters.data_ptr(), splits,
-                                 _native.stream_ptr())
+                                 stream)
     return out
 
 
@@ -196,7 +200,6 @@ def window_attention_decode(qkv, cache: WindowCache, positions, group: int = 1):
     if (k.is_cuda and group > 0 and qkv.shape == (batch, kv * (group + 2) * D) and qkv.dtype is k.dtype and qkv.is_contiguous()
             and qkv.data_ptr() & 15 == 0 and positions.dtype is torch.int64 and positions.shape == (batch,) and positions.is_contiguous()
             and qkv.get_device() == positions.get_device() == k.get_device() and batch):
-        _native.check_device(qkv)
         return _decode(qkv, qkv.shape[1], cache, positions, batch, kv, group, D)
     if _width(qkv, kv, group, batch) != D:
         raise ValueError(f"the cache holds {D} features per head, the rows {qkv.shape[1] // (kv * (group + 2))}")
@@ -206,7 +209,6 @@ def window_attention_decode(qkv, cache: WindowCache, positions, group: int = 1):
     if qkv.dtype != cache.k.dtype or qkv.device != cache.k.device:
         raise ValueError(f"rows are {qkv.dtype} on {qkv.device}, the cache {cache.k.dtype} on {cache.k.device}")
     if qkv.is_cuda:
-        _native.check_device(qkv)
         if batch == 0:
             return qkv.new_empty(0, kv * group * D)
         x = rows.as_aligned(qkv)
