@@ -34,6 +34,8 @@ __device__ __forceinline__ float exp2_ftz(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// A maximum to subtract: where all scores so far are -inf, -inf - 0 gives the probability 0 that -inf + inf would not.
+__device__ __forceinline__ float finite(float m) { return m == -INFINITY ? 0.f : m; }
 __device__ __forceinline__ uint32_t pack(float a, float b) {
   __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<uint32_t*>(&v);
@@ -156,7 +158,7 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
       float t = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
       t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
       t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-      up[r] = fmaxf(m[r], t);                      // a tile has a slot in it: finite unless a score is not
+      up[r] = fmaxf(m[r], t);
       grown |= up[r] > m[r];
     }
     if (__any_sync(0xffffffffu, grown)) {
@@ -177,7 +179,7 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int r = 0; r < (kWide ? 2 : 1); ++r) {
-        const float x = exp2_ftz(s[n][2 * r] - m[r]), y = exp2_ftz(s[n][2 * r + 1] - m[r]);
+        const float at = finite(m[r]), x = exp2_ftz(s[n][2 * r] - at), y = exp2_ftz(s[n][2 * r + 1] - at);
         l[r] += x + y;
         p[n * 2 + r] = pack(x, y);
       }
@@ -235,7 +237,7 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = w < tiles ? exp2_ftz(sm[w * kHeads + head] - top) : 0.f;            // a warp without a tile has nothing
+      const float f = w < tiles ? exp2_ftz(sm[w * kHeads + head] - finite(top)) : 0.f;            // a warp without a tile has nothing
       sum += f * sl[w * kHeads + head];
       add(acc, f, *reinterpret_cast<const float4*>(so + (w * kHeads + head) * kD + lane * 4));
     }
@@ -282,7 +284,7 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       const float2 st = stats(s0 + lane, min(warp + i * kWarps, heads - 1));
-      f[i] = s0 + lane < live ? exp2_ftz(st.x - top[i]) : 0.f;
+      f[i] = s0 + lane < live ? exp2_ftz(st.x - finite(top[i])) : 0.f;
       sum[i] += f[i] * st.y;
     }
     const int n = min(32, live - s0);

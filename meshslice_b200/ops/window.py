@@ -167,8 +167,10 @@ class WindowCache:
         self.v[:, :, at] = x[:, :, :, group + 1].transpose(1, 2)
 
     def workspace(self, group: int):
-        """(splits, partial results, counters) of the decoding kernel, laid out once."""
-        if group not in self._work:
+        """(splits, partial results, counters) of the decoding kernel, laid out once (for a call in a graph that is being captured,
+        where nothing is laid out yet, by the graph itself: its counters are zeroed when it runs, not now)."""
+        work = self._work.get(group)
+        if work is None:
             batch, kv, slots = self.k.shape[:3]
             C = _native.load()
             sms = torch.cuda.get_device_properties(self.k.device).multi_processor_count
@@ -176,8 +178,10 @@ class WindowCache:
             units = batch * kv * -(-group // 16)
             parts = torch.empty(units * splits * C.WINDOW_DECODE_PART if splits > 1 else 0, dtype=torch.float32, device=self.k.device)
             counters = torch.zeros(units, dtype=torch.int32, device=self.k.device)
-            self._work[group] = (splits, parts, counters)
-        return self._work[group]
+            work = (splits, parts, counters)
+            if not torch.cuda.is_current_stream_capturing():
+                self._work[group] = work
+        return work
 
 
 def _decode(x, pitch: int, cache: WindowCache, positions, batch: int, kv: int, group: int, D: int):

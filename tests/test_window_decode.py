@@ -165,3 +165,38 @@ def test_kernel_in_a_graph_and_refusals():
         WindowCache(cache.k.transpose(0, 1), cache.v.transpose(0, 1), 30, 2)
     with pytest.raises(ValueError):
         WindowCache.new(1, 1, 4, head_dim=64, device="cuda")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [3, 12])
+@pytest.mark.parametrize("batch,window", [(1, 700), (40, 700), (1, 20000)])
+def test_kernel_keys_of_minus_infinity(batch, window, group):
+    """Keys whose score is -inf have probability 0, also where a warp's first tiles, or all of a split, have no other."""
+    n = window + 1
+    x = history(1, n, 1, group, 128)
+    x[..., :group, 0] = 1.0
+    x[:, 1:window // 2, :, group, 0] = -math.inf
+    cache = WindowCache.new(batch, 1, window, 0, device="cuda")
+    cache.fill(x[0, : n - 1].reshape(n - 1, -1).repeat(batch, 1).cuda(), n - 1, group)
+    got = F.window_attention_decode(x[:, n - 1].reshape(1, -1).repeat(batch, 1).cuda(), cache, torch.full((batch,), n - 1, device="cuda"), group)
+    assert torch.equal(got, got[:1].expand_as(got))
+    check(got[0], *definition(x[0], n - 1, window, 0))
+
+
+@pytest.mark.gpu
+def test_kernel_whose_first_call_is_captured():
+    """The workspace that a graph lays out is the graph's own: calls outside of it, before its first run too, are right."""
+    x = history(1, 3000, 1, 2, 128)
+    cache = WindowCache.new(1, 1, 2900, 2, device="cuda")
+    cache.fill(x[0, :2999].reshape(2999, -1).cuda(), 2999, 2)
+    row, pos = x[:, 2999].reshape(1, -1).cuda(), torch.full((1,), 2999, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = F.window_attention_decode(row, cache, pos, 2)
+    want = definition(x[0], 2999, 2900, 2)
+    check(F.window_attention_decode(row, cache, pos, 2)[0], *want)
+    for _ in range(2):
+        graph.replay()
+        check(out[0], *want)
+    del graph
+    check(F.window_attention_decode(row, cache, pos, 2)[0], *want)
