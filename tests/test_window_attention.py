@@ -233,3 +233,20 @@ def test_kernel_matches_causal_attention_and_refusals():
     with pytest.raises(ValueError):
         F.window_attention_fwd(qkv, 2, 512, 6)
     assert F.window_attention_fwd(qkv[:0], 0, 512, 3)[0].shape == (0, 384)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sinks,dead", [(4, range(1, 301)), (4, range(4)), (40, range(39)), (0, range(1, 301))])
+def test_kernel_keys_of_minus_infinity(sinks, dead):
+    """Keys whose score is -inf have probability 0, where a query's first tiles have no others too; a query without any other is NaN."""
+    shape = (1, 700, 1, 2, 200, sinks)
+    qkv, _ = inputs(1, 700, 1, 2)
+    x = qkv.view(700, 4, 128)
+    x[:, :2, 0] = 1.0
+    x[list(dead), 2, 0] = -math.inf
+    out, _ = F.window_attention_fwd(qkv.cuda(), *shape)
+    want, _, _ = definition(qkv, torch.zeros(700, 256), *shape)
+    held = ~want.isnan().any(1)
+    assert held.sum() >= 300 and (~held).any() == (0 in dead or sinks == 0)
+    got = out.double().cpu()
+    assert rel(got[held], want[held]) < OUT and got[~held].isnan().any(1).all()
