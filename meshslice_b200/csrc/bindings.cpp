@@ -649,6 +649,7 @@ PYBIND11_MODULE(_C, m) {
   m.attr("DISTILL_ROW_COLS") = distill_row_cols();
   m.attr("DISTILL_TOP") = kDistillTop;
   m.attr("WINDOW_DECODE_PART") = kWindowDecodePart;
+  m.attr("WINDOW_DECODE_CLUSTER") = kWindowDecodeCluster;
   m.def("window_attention_scratch", [](int batch, int seq, int kv, int group, int window, int sinks) {
     return window_attention_scratch({batch, seq, kv, group, window, sinks, 1.f});
   }, "fp32 values of the backward pass's scratch");

@@ -2,6 +2,7 @@
 #include "window_decode.h"
 
 #include <cuda_bf16.h>
+#include <math.h>
 
 #include "../common/pdl.cuh"
 #include "../common/ptx.cuh"
@@ -19,6 +20,7 @@ constexpr int kHeads = 16;                         // query heads of a CTA: rows
 constexpr int kSmem = kWarps * kStages * 2 * kTile;
 constexpr int kPart = kWindowDecodePart;           // floats of a split: O, m, l
 static_assert(kPart == kHeads * (kD + 2), "what a split leaves");
+constexpr int kClusterSplits = kWindowDecodeCluster;
 constexpr float kLog2e = 1.4426950408889634f;
 static_assert(kWarps * kHeads * (kD + 2) * 4 <= kSmem, "the warps' results take the place of the tiles");
 
@@ -54,16 +56,38 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ uint32_t of_rank(uint32_t at, int rank) {       // the same place of another CTA of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(at), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float load_of(uint32_t at) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 load4_of(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+  return v;
+}
+// What the CTAs of the cluster that have not left wrote to their shared memory before this is seen after it.
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
 // A CTA works on a run of slots of one (sequence, key/value head, 16 of its query heads); each warp on every fourth tile of 16
 // slots, with running maximum and sum of its own, through a ring that it fills itself (cp.async; no barrier).  The query heads
 // are the rows of the matrix fragments, so that all heads of a group share a pass over K and V.  mma.sync: a token's products are a
 // sixth of what that path does beside the memory, and the operands come as rows of any number and origin.
 // The token's own k and v are taken from `qkv` in place of their slot, which the CTA that has it writes.
-// Splits of a sequence are joined, in their order, by the CTA that finishes last.  P is rounded to bf16 as the operand of P V.
-// Bound by HBM: 64 sequences of up to 4100 slots, 8 x 4 heads, 145 us (6.6 TB/s); one sequence of 700 tokens by the launch and three
-// trips to memory (position, tiles, splits): 6.7 us, 14.7 when the splits were joined one after another.
+// Splits of a sequence are joined in their order: up to 8 are a cluster, whose CTAs take the heads by turns from the shared memory of
+// all, more by the CTA that finishes last, through memory.  P is rounded to bf16 as the operand of P V.
+// Bound by HBM: 64 sequences of up to 4100 slots, 8 x 4 heads, 145 us (6.6 TB/s); one sequence of 700 tokens by the launch and two
+// trips to memory (position, tiles): 6.7 us (8.2 where its splits were joined through memory).
 // kWide: more than 8 query heads (rows 8 to 15 of the fragments are in use).
-template <bool kWide>
+// kCluster: the splits of a sequence are a cluster, and each CTA joins some of its heads from the shared memory of all.
+template <bool kWide, bool kCluster>
 __global__ void __launch_bounds__(kWarps * 32)
 window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int per_split) {
   extern __shared__ __align__(128) uint8_t smem[];
@@ -243,12 +267,44 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
     }
     if (live == 1) {
       store(head, acc, 1.f / sum);
+    } else if constexpr (kCluster) {
+      __syncwarp();
+      *reinterpret_cast<float4*>(so + head * kD + lane * 4) = acc;                       // (read by this warp alone)
+      if (lane == 0) {
+        sm[head] = top;
+        sl[head] = sum;
+      }
     } else {
       __stcg(reinterpret_cast<float4*>(part + head * kD + lane * 4), acc);
       if (lane == 0) __stcg(reinterpret_cast<float2*>(part + kHeads * kD + head * 2), make_float2(top, sum));
     }
   }
-  if (live == 1) return;
+  if (live == 1) return;                           // (CTAs without a slot have left: the barriers do not count them)
+  if constexpr (kCluster) {
+    cluster_barrier();
+    const uint32_t at_o = smem_u32(so), at_m = smem_u32(sm), at_l = smem_u32(sl);
+    for (int head = warp * live + split; head < heads; head += kWarps * live) {
+      const int rank = min(lane, live - 1);
+      const float m1 = load_of(of_rank(at_m + head * 4, rank)), l1 = load_of(of_rank(at_l + head * 4, rank));
+      float4 v[kClusterSplits];
+#pragma unroll
+      for (int s = 0; s < kClusterSplits; ++s) v[s] = load4_of(of_rank(at_o + head * (kD * 4) + lane * 16, min(s, live - 1)));
+      float t = m1;
+#pragma unroll
+      for (int o = kClusterSplits / 2; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+      const float f = lane < live ? exp2_ftz(m1 - finite(t)) : 0.f;
+      float sum = f * l1;
+#pragma unroll
+      for (int o = kClusterSplits / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < kClusterSplits; ++s)
+        if (s < live) add(acc, __shfl_sync(0xffffffffu, f, s), v[s]);
+      store(head, acc, 1.f / __shfl_sync(0xffffffffu, sum, 0));
+    }
+    cluster_barrier();                             // until here the others read this CTA's memory
+    return;
+  }
   __threadfence();
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -307,13 +363,19 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
 
 }  // namespace
 
-// One wave of two CTAs an SM, each with three tiles or more for every warp: a split more costs every sequence a trip through memory (8 us) and
-// every CTA its start.  us by splits: 64 sequences of 8 key heads, 4100 slots, 1 143, 2 152, 6 148; 256 of 8, 512 slots, 1 85, 2 119; 16 of 8,
-// 4100, 1 58, 2 50, 4 49, 12 58; 8 of 2, 8196, 6 30, 12 22.6, 18 22.8, 37 32; 1 of 8, 4100, 6 15, 18 12.7, 37 15.
+// One wave of two CTAs an SM, in clusters of up to 8 with a tile or more for every warp.  A wide launch of long caches goes beyond a
+// cluster: s splits cost slots / s for the tiles and s for the join through memory, least at a multiple of the root of slots.  us by splits:
+// 64 sequences of 8 key heads, 4100 slots, 1 143, 2 155, 6 167; 256 of 8, 512 slots, 1 87, 2 118; 16 of 8, 4100, 1 56, 2 48, 4 49, 8 58; 1 of 8,
+// 128 slots, 1 4.4, 2 4.8; 260, 1 5.7, 2 6.3, 5 5.0; 1028, 1 9.3, 4 8.3, 8 6.7, 12 9.0; 8196, 8 18.3, 18 16.6, 37 17.8; 65536, 8 106, 18 57, 24 52,
+// 37 54; 3 of 8, 65536, 8 124, 12 130, 24 130; 1 of 1, 4096, 8 10.6, 12 14.3, 22 13.9; 8192, 8 15.8, 18 15.7, 43 20; 131072, 8 186, 37 45, 74 35, 148 40,
+// 296 61.
 int window_decode_splits(int batch, int kv, int group, int slots, int sms) {
-  const int64_t units = (int64_t)batch * kv * ((group + kHeads - 1) / kHeads);
-  const int64_t most = (slots + 3 * kWarps * kKeys - 1) / (3 * kWarps * kKeys), want = (int64_t)sms * 2 / units;
-  return (int)(want < 1 ? 1 : want < most ? want : most);
+  const int64_t units = (int64_t)batch * kv * ((group + kHeads - 1) / kHeads), want = (int64_t)sms * 2 / units;
+  const int tiles = kWarps * kKeys, most = slots <= 2 * tiles ? 1 : (slots + tiles - 1) / tiles;
+  const int64_t wide = (int64_t)sqrt(slots / 24.);
+  if (want >= 2 * kClusterSplits && wide >= 2 * kClusterSplits) return (int)(want < wide ? want : wide);
+  const int64_t n = want < kClusterSplits ? want : kClusterSplits;
+  return (int)(n < 1 ? 1 : n < most ? n : most);
 }
 
 cudaError_t window_decode(const WindowDecodeArgs& a, int splits, cudaStream_t stream) {
@@ -323,18 +385,22 @@ cudaError_t window_decode(const WindowDecodeArgs& a, int splits, cudaStream_t st
   const int64_t slots = (int64_t)a.sinks + a.window, rows = (int64_t)a.kv * ((a.group + kHeads - 1) / kHeads);
   if (slots > 1 << 30 || rows > 65535 || a.batch > 65535) return cudaErrorInvalidValue;
   const int steps = kWarps * kKeys, per = (int)((slots + splits - 1) / splits + steps - 1) / steps * steps;
-  auto kernel = a.group > 8 ? window_decode_kernel<true> : window_decode_kernel<false>;
+  if (splits > kClusterSplits && (a.parts == nullptr || off(a.parts) || a.counters == nullptr)) return cudaErrorInvalidValue;
+  const bool wide = a.group > 8, cluster = splits > 1 && splits <= kClusterSplits;
+  auto kernel = wide ? cluster ? window_decode_kernel<true, true> : window_decode_kernel<true, false>
+                     : cluster ? window_decode_kernel<false, true> : window_decode_kernel<false, false>;
   // the attribute is per device: set it once on every device that launches
-  static bool configured[64][2] = {};
+  static bool configured[64][4] = {};
+  const int which = wide * 2 + cluster;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev < 0 || dev >= 64 || !configured[dev][a.group > 8]) {
+  if (dev < 0 || dev >= 64 || !configured[dev][which]) {
     e = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
-    if (dev >= 0 && dev < 64) configured[dev][a.group > 8] = true;
+    if (dev >= 0 && dev < 64) configured[dev][which] = true;
   }
-  return launch_dependent(kernel, dim3((unsigned)splits, (unsigned)rows, (unsigned)a.batch), kWarps * 32, kSmem, stream, a, splits, per);
+  return launch_dependent_clusters(kernel, cluster ? splits : 1, dim3((unsigned)splits, (unsigned)rows, (unsigned)a.batch), kWarps * 32, kSmem, stream, a, splits, per);
 }
 
 }  // namespace msb

@@ -13,10 +13,12 @@ struct WindowDecodeArgs {
   void* out;                   // bf16 [batch, kv * group * 128], contiguous
   int batch, kv, group, window, sinks;
   float scale;
-  float* parts;                // fp32 [batch * kv * passes * splits * 16 * 130], passes = ceil(group / 16); unused for one split
+  // unused up to kWindowDecodeCluster splits:
+  float* parts;                // fp32 [batch * kv * passes * splits * 16 * 130], passes = ceil(group / 16)
   uint32_t* counters;          // [batch * kv * passes], zero before the first launch and after each
 };
 constexpr int kWindowDecodePart = 16 * 130;   // floats of a split
+constexpr int kWindowDecodeCluster = 8;       // splits that are joined within a cluster: the largest that every GPU of this kind has room for
 // Splits of a sequence's slots that a launch uses on a GPU of `sms` SMs: sizes of `parts`.
 int window_decode_splits(int batch, int kv, int group, int slots, int sms);
 // Position p lies in slot p below `sinks` and in slot sinks + (p - sinks) % window from there on, so that the first

@@ -167,19 +167,19 @@ class WindowCache:
         self.v[:, :, at] = x[:, :, :, group + 1].transpose(1, 2)
 
     def workspace(self, group: int):
-        """(splits, partial results, counters) of the decoding kernel, laid out once (for a call in a graph that is being captured,
-        where nothing is laid out yet, by the graph itself: its counters are zeroed when it runs, not now)."""
+        """(splits, partial results, counters) of the decoding kernel, laid out once (by a graph that is being captured, where nothing
+        is laid out yet, for itself: its counters are zeroed when it runs, not now)."""
         work = self._work.get(group)
         if work is None:
             batch, kv, slots = self.k.shape[:3]
             C = _native.load()
             sms = torch.cuda.get_device_properties(self.k.device).multi_processor_count
             splits = C.window_decode_splits(batch, kv, group, slots, sms)
-            units = batch * kv * -(-group // 16)
-            parts = torch.empty(units * splits * C.WINDOW_DECODE_PART if splits > 1 else 0, dtype=torch.float32, device=self.k.device)
+            units = batch * kv * -(-group // 16) if splits > C.WINDOW_DECODE_CLUSTER else 0      # (fewer are joined without)
+            parts = torch.empty(units * splits * C.WINDOW_DECODE_PART, dtype=torch.float32, device=self.k.device)
             counters = torch.zeros(units, dtype=torch.int32, device=self.k.device)
             work = (splits, parts, counters)
-            if not torch.cuda.is_current_stream_capturing():
+            if units == 0 or not torch.cuda.is_current_stream_capturing():
                 self._work[group] = work
         return work
 

@@ -184,19 +184,43 @@ def test_kernel_keys_of_minus_infinity(batch, window, group):
 
 
 @pytest.mark.gpu
-def test_kernel_whose_first_call_is_captured():
+@pytest.mark.parametrize("window", [2900, 7000])
+def test_kernel_whose_first_call_is_captured(window):
     """The workspace that a graph lays out is the graph's own: calls outside of it, before its first run too, are right."""
-    x = history(1, 3000, 1, 2, 128)
-    cache = WindowCache.new(1, 1, 2900, 2, device="cuda")
-    cache.fill(x[0, :2999].reshape(2999, -1).cuda(), 2999, 2)
-    row, pos = x[:, 2999].reshape(1, -1).cuda(), torch.full((1,), 2999, device="cuda")
+    x = history(1, window + 100, 1, 2, 128)
+    cache = WindowCache.new(1, 1, window, 2, device="cuda")
+    cache.fill(x[0, :window + 99].reshape(window + 99, -1).cuda(), window + 99, 2)
+    row, pos = x[:, window + 99].reshape(1, -1).cuda(), torch.full((1,), window + 99, device="cuda")
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = F.window_attention_decode(row, cache, pos, 2)
-    want = definition(x[0], 2999, 2900, 2)
+    want = definition(x[0], window + 99, window, 2)
     check(F.window_attention_decode(row, cache, pos, 2)[0], *want)
     for _ in range(2):
         graph.replay()
         check(out[0], *want)
     del graph
     check(F.window_attention_decode(row, cache, pos, 2)[0], *want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kv,group", [(1, 1), (2, 4), (1, 8), (1, 11), (1, 33)])
+@pytest.mark.parametrize("window", [190, 250, 400, 1000, 1400, 1600, 7000])
+def test_kernel_splits_that_hold_nothing_yet(kv, group, window):
+    """Sequences of every number of splits in use, up to all of them, beside one another."""
+    stops = [0, -1, window - 1] + list(range(63, 2 * window, window // 7 + 1))
+    x = history(1, 2 * window, kv, group, 128)
+    rows = x[0, [max(p, 0) for p in stops]].reshape(len(stops), -1).cuda()
+    cache = WindowCache.new(len(stops), kv, window, 3, device="cuda")
+    whole = x[0].reshape(2 * window, -1).cuda()
+    for b, p in enumerate(stops):
+        if p > 0:
+            one = WindowCache.new(1, kv, window, 3, device="cuda")
+            one.fill(whole[:p], p, group)
+            cache.k[b], cache.v[b] = one.k[0], one.v[0]
+    got = F.window_attention_decode(rows, cache, torch.tensor(stops, device="cuda"), group)
+    for b, p in enumerate(stops):
+        if p < 0:
+            assert got[b].count_nonzero() == 0
+        else:
+            check(got[b], *definition(x[0], p, window, 3))
