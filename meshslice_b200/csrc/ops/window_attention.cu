@@ -124,7 +124,7 @@ __device__ __forceinline__ void warp_store_box(const CUtensorMap* map, const voi
 // What bounds it: a step of both tiles takes 3260 cycles (2048 of the special-function unit, 1024 of products a tile), a masked block 650
 // more, an item's end 2900 in which the output leaves and nothing is multiplied; below windows of about 200, HBM.  4 x 2048, 32 heads: window
 // 128 54 us (6.2 TB/s), 512 with 4 first tokens 90; 1 x 16384, 16 heads on 4, window 4096 405 us (1190 TFLOP/s; under the power cap 468).
-// First tokens as whole blocks took 102 us of the 90; tile 1's own block at the head of the list 97.
+// The 90 us were 102 with first tokens as whole blocks, 97 with tile 1's own block at the head of the list.
 constexpr int kFwdWarpStage = 32 * 128;   // output staging per softmax warp: 32 rows x 64 columns
 constexpr size_t kFwdSmem = 6 * kTile + 8 * kFwdWarpStage + 256 + 1024;
 constexpr int kFwdThreads = 384;
