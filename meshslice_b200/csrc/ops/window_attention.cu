@@ -1561,7 +1561,8 @@ cudaError_t window_attention_fwd(const void* qkv, void* out, float* lse, const W
 
 namespace {
 // Few first tokens beyond a window: CTAs of window_rows_kernel per key head (0: the general way).  One wave of two CTAs an SM, each with
-// a tile or more for every warp.
+// a tile or more for every warp (the whole backward of 4 x 2048, 32 heads by CTAs an SM: 2 293 us, 3 299, 4 296, 7 300; 2 x 5003, 16 heads on 4: 267, 273,
+// 275, 286).
 int thin_chunks(const WindowShape& s) {
   if (s.sinks == 0 || s.sinks > kThinKeys || s.window == 0 || s.window >= s.seq) return 0;
   const int units = s.batch * s.kv, tiles = s.group * blocks_of(s.seq) * (kBlk / 16);
