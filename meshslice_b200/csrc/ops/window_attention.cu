@@ -1564,6 +1564,7 @@ namespace {
 // a tile or more for every warp (the whole backward of 4 x 2048, 32 heads by CTAs an SM: 2 293 us, 3 299, 4 296, 7 300; 2 x 5003, 16 heads on 4: 267, 273,
 // 275, 286).
 int thin_chunks(const WindowShape& s) {
+  if (s.batch <= 0 || s.kv <= 0) return 0;           // (such a launch is refused)
   if (s.sinks == 0 || s.sinks > kThinKeys || s.window == 0 || s.window >= s.seq) return 0;
   const int units = s.batch * s.kv, tiles = s.group * blocks_of(s.seq) * (kBlk / 16);
   int n = 148 * 2 / units;

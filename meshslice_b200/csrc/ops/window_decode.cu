@@ -370,6 +370,7 @@ window_decode_kernel(const __grid_constant__ WindowDecodeArgs a, int splits, int
 // 37 54; 3 of 8, 65536, 8 124, 12 130, 24 130; 1 of 1, 4096, 8 10.6, 12 14.3, 22 13.9; 8192, 8 15.8, 18 15.7, 43 20; 131072, 8 186, 37 45, 74 35, 148 40,
 // 296 61.
 int window_decode_splits(int batch, int kv, int group, int slots, int sms) {
+  if (batch <= 0 || kv <= 0 || group <= 0 || slots <= 0 || sms <= 0) return 1;      // (nothing to deal out; such a launch is refused)
   const int64_t units = (int64_t)batch * kv * ((group + kHeads - 1) / kHeads), want = (int64_t)sms * 2 / units;
   const int tiles = kWarps * kKeys, most = slots <= 2 * tiles ? 1 : (slots + tiles - 1) / tiles;
   const int64_t wide = (int64_t)sqrt(slots / 24.);

@@ -124,8 +124,9 @@ class WindowCache:
     def __init__(self, k, v, window: int, sinks: int = 0):
         if window < 1 or sinks < 0:
             raise ValueError(f"a cache needs window >= 1 and sinks >= 0 (got {window}, {sinks})")
-        if k.dim() != 4 or k.shape[2] != window + sinks or v.shape != k.shape or v.dtype != k.dtype or v.device != k.device:
-            raise ValueError(f"keys and values must both be [batch, kv_heads, {window + sinks}, head_dim] (got {tuple(k.shape)} {k.dtype} "
+        if (k.dim() != 4 or k.shape[1] < 1 or k.shape[2] != window + sinks or k.shape[3] < 1 or v.shape != k.shape or v.dtype != k.dtype
+                or v.device != k.device):
+            raise ValueError(f"keys and values must both be [batch, kv_heads >= 1, {window + sinks}, head_dim >= 1] (got {tuple(k.shape)} {k.dtype} "
                              f"and {tuple(v.shape)} {v.dtype})")
         if k.is_cuda:
             if k.dtype != torch.bfloat16 or k.shape[3] != HEAD_DIM:

@@ -224,3 +224,22 @@ def test_kernel_splits_that_hold_nothing_yet(kv, group, window):
             assert got[b].count_nonzero() == 0
         else:
             check(got[b], *definition(x[0], p, window, 3))
+
+
+def test_sizes_without_heads_sequences_or_slots():
+    """The sizes that a launch lays out are worked out before anything checks its arguments: nothing to deal out is an answer, and no
+    division by it; a cache without heads or features is refused."""
+    from meshslice_b200 import _native
+    C = _native.load()
+    for args in ((1, 0, 1, 8, 148), (0, 4, 1, 8, 148), (1, 4, 0, 8, 148), (1, 4, 1, 0, 148), (1, -1, 1, 8, 148), (1, 4, 1, 8, 0)):
+        assert C.window_decode_splits(*args) == 1
+    assert C.window_decode_splits(1, 1, 1, 131072, 148) > 8
+    for batch, kv in ((0, 1), (1, 0), (0, 0), (-1, 1)):
+        assert C.window_attention_scratch(batch, 200, kv, 1, 64, 4) <= 0
+    assert C.window_attention_scratch(1, 200, 1, 1, 64, 4) > 0
+    for shape in ((2, 0, 6, 128), (2, 1, 6, 0)):
+        k = torch.zeros(shape, dtype=torch.bfloat16)
+        with pytest.raises(ValueError):
+            WindowCache(k, k.clone(), 5, 1)
+    with pytest.raises(ValueError):
+        WindowCache.new(2, 0, 5, 1)
