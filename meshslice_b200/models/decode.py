@@ -11,7 +11,11 @@ from .gpt import GPTModel
 
 class GPTDecoder:
     """``prefill`` takes prompts of one length, ``step`` a token of each sequence at its own position; both return logits
-    [batch, vocab] of the next tokens.  A negative position is an idle sequence, whose logits mean nothing."""
+    [batch, vocab] of the next tokens.  A negative position is an idle sequence, whose token and logits mean nothing.
+
+    Tokens and positions are int64 on the model's device.  What they hold is checked on the CPU; on a GPU, where that would wait for the
+    device, a token outside the vocabulary counts as the nearest one in it, and a position that a model with learned positions has
+    no vector for (``cfg.seq`` and beyond) makes the logits of its sequence NaN."""
 
     def __init__(self, model: GPTModel, batch: int):
         cfg, mesh = model.cfg, model.mesh
@@ -46,17 +50,34 @@ class GPTDecoder:
     def _logits(self, x, delta):
         return self._linear(self.model.head, self._norm(self.model.ln_f, x, delta)[1])[:, :self.cfg.vocab]
 
+    def _check(self, name, t, shape):
+        device = self.model.tok.shards[self.key].device
+        if t.shape != shape or t.dtype != torch.int64 or t.device != device:
+            raise ValueError(f"{name} must be int64 {list(shape)} on {device} (got {t.dtype} {list(t.shape)} on {t.device})")
+
     def _embed(self, tokens, positions):
         tok = self.model.tok.shards[self.key]
+        rows = tok.shape[0]
+        if not tok.is_cuda and ((tokens < 0) | (tokens >= rows))[positions >= 0].any():
+            raise ValueError(f"tokens must be in [0, {rows})")
+        tokens = tokens.clamp(0, rows - 1).contiguous()
         if self.model.pos is None:
-            return F.embedding_fwd(tokens.contiguous(), tok, None, 1)
-        return (tok[tokens].float() + self.model.pos.shards[self.key][positions.clamp_min(0)].float()).to(tok.dtype)
+            return F.embedding_fwd(tokens, tok, None, 1)
+        pos = self.model.pos.shards[self.key]
+        beyond = positions >= pos.shape[0]
+        if not tok.is_cuda and beyond.any():
+            raise ValueError(f"the model has learned positions below {pos.shape[0]} (got {int(positions.max())})")
+        x = (tok[tokens].float() + pos[positions.clamp(0, pos.shape[0] - 1)].float()).to(tok.dtype)
+        return x.masked_fill_(beyond[:, None], float("nan"))
 
     def prefill(self, tokens):
         """``tokens`` [batch, n], positions 0 .. n - 1."""
         if tokens.dim() != 2 or tokens.shape[0] != self.batch or tokens.shape[1] < 1:
             raise ValueError(f"prompts must be [{self.batch}, n >= 1] (got {tuple(tokens.shape)})")
         n, cfg = tokens.shape[1], self.cfg
+        self._check("prompts", tokens, (self.batch, n))
+        if self.model.pos is not None and n > cfg.seq:
+            raise ValueError(f"the model has learned positions of {cfg.seq} tokens (got a prompt of {n})")
         pos = torch.arange(n, device=tokens.device).repeat(self.batch)
 
         def attend(i, qkv):
@@ -72,9 +93,8 @@ class GPTDecoder:
 
     def step(self, tokens, positions):
         """``tokens``, ``positions`` int64 [batch]."""
-        if tokens.shape != (self.batch,) or positions.shape != (self.batch,):
-            raise ValueError(f"a step takes a token and a position of each of {self.batch} sequences (got {tuple(tokens.shape)}, "
-                             f"{tuple(positions.shape)})")
+        self._check("tokens", tokens, (self.batch,))
+        self._check("positions", positions, (self.batch,))
 
         def attend(i, qkv):
             rot = self.model.blocks[i].attn.rotary

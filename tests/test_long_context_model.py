@@ -162,3 +162,66 @@ def test_operations_of_a_window():
         rest = GPTConfig(**base, seq=seq).flops_per_token() - 3 * 4 * seq * 128 * 3 * 0.5
         got = GPTConfig(**base, seq=seq, window=window, sinks=sinks).flops_per_token() - rest
         assert abs(got - 3 * 4 * 128 * 3 * pairs / seq) < 1e-6 * got
+
+
+@pytest.mark.parametrize("rotary", [ROT, None])
+def test_decoder_refuses_tokens_and_positions_that_it_has_nothing_for(rotary):
+    """Types, devices, ids outside the vocabulary, prompts and positions beyond the learned ones (of which decoding with a cache of fixed
+    size is free otherwise)."""
+    cfg = GPTConfig(**{**CFG.__dict__, "rotary": rotary, "seq": 12})
+    model = GPTModel(EmuMesh(1, 1), cfg)
+    d = GPTDecoder(model, 2)
+    ids = torch.randint(0, cfg.vocab, (2, 20), generator=torch.Generator().manual_seed(3))
+    at = lambda p: torch.full((2,), p)
+    if rotary is None:
+        for call in (lambda: d.prefill(ids[:, :13]), lambda: d.step(ids[:, 0], at(12)), lambda: d.step(ids[:, 0], torch.tensor([1, 400]))):
+            with pytest.raises(ValueError):
+                call()
+    else:
+        assert d.prefill(ids[:, :13]).isfinite().all() and d.step(ids[:, 13], at(13)).isfinite().all()
+    d.prefill(ids[:, :11])
+    for tokens, positions in ((ids[:, 11].int(), at(11)), (ids[:, 11], at(11).int()), (ids[:, 11], at(11).float()), (ids[:, 11].float(), at(11)),
+                              (ids[:, 11].to("meta"), at(11)), (ids[:, 11], at(11).to("meta")), (torch.tensor([0, -1]), at(11)),
+                              (torch.tensor([cfg.vocab_padded, 0]), at(11))):
+        with pytest.raises(ValueError):
+            d.step(tokens, positions)
+    for prompts in (ids[:, :5].int(), ids[:, :5].float(), ids[:, :5].to("meta"), ids[:, :5] - cfg.vocab):
+        with pytest.raises(ValueError):
+            d.prefill(prompts)
+    want = d.step(ids[:, 11], at(11))
+    d.prefill(ids[:, :11])
+    got = d.step(torch.tensor([int(ids[0, 11]), -1]), torch.tensor([11, -1]))          # an idle sequence's token is not looked at
+    assert torch.equal(got[0], want[0])
+
+
+@pytest.mark.gpu
+def test_decoder_on_a_gpu_reads_nothing_outside_its_tables():
+    """Ids outside the vocabulary count as the nearest one; positions without a learned vector show as NaN in their own sequence."""
+    from meshslice_b200 import _native
+    from meshslice_b200.parallel.engine import LocalGemmEngine
+    mesh = EmuMesh(1, 1)
+    LocalGemmEngine(mesh)
+    for rotary in (RotaryConfig(), None):
+        cfg = GPTConfig(n_layers=1, d_model=256, n_heads=2, ffn=512, vocab=250, seq=40, vocab_pad=256, window=16, rotary=rotary)
+        model = GPTModel(mesh, cfg, device=torch.device("cuda", 0))
+        d = GPTDecoder(model, 3)
+        ids = torch.randint(0, cfg.vocab, (3, 41), generator=torch.Generator().manual_seed(4)).cuda()
+        with pytest.raises(ValueError):
+            d.step(ids[:, 0].int(), ids[:, 0])
+        with pytest.raises(ValueError):
+            d.step(ids[:, 0], ids[:, 0].cpu())
+        if rotary is None:
+            with pytest.raises(ValueError):
+                d.prefill(ids)
+        d.prefill(ids[:, :39])
+        want = d.step(ids[:, 39], torch.tensor([39, 39, -1], device="cuda"))
+        d.prefill(ids[:, :39])
+        tokens = ids[:, 39].clone()
+        tokens[2] = -(1 << 40)
+        got = d.step(tokens, torch.tensor([39, 1 << 20, -1], device="cuda"))
+        assert torch.equal(got[0], want[0]) and bool(got[1].isnan().all()) == (rotary is None)
+        d.prefill(ids[:, :39])
+        tokens[1], tokens[0] = 1 << 40, cfg.vocab_padded - 1
+        same = d.step(tokens, torch.full((3,), 39, device="cuda"))
+        assert same[1].isfinite().all() and same[0].isfinite().all()
+    _native.check_status()
