@@ -32,7 +32,7 @@ class GPTDecoder:
                        for _ in model.blocks]
 
     def _linear(self, layer, x):
-        return layer.forward(ShardedTensor(self.model.mesh, {self.key: x})).shards[self.key]
+        return layer.forward(ShardedTensor(self.model.mesh, {self.key: x}), keep=False).shards[self.key]
 
     def _norm(self, layer, x, res):
         return F.ln_full(x, res, layer.gamma.shards[self.key], layer.bias.shards[self.key], layer.eps)[:2]

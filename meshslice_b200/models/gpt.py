@@ -122,27 +122,35 @@ class GPTBlock:
     # [in, tokens] with the features over the mesh rows; its output and the gradient it returns are
     # in the usual / the transposed orientation respectively (ShardedLayers.py:69-81).  The block keeps
     # activations [tokens, features] and re-orients around such a layer.
-    def _lin(self, layer, x: ShardedTensor) -> ShardedTensor:
-        return layer.forward(self.mesh.transpose(x) if layer.dataflow == "rs" else x)
+    def _lin(self, layer, x: ShardedTensor, keep: bool = True) -> ShardedTensor:
+        return layer.forward(self.mesh.transpose(x) if layer.dataflow == "rs" else x, keep)
+
+    @staticmethod
+    def _norm(layer, x: ShardedTensor, res: Optional[ShardedTensor], keep: bool):
+        """The residual stream behind ``layer`` and its output."""
+        y = layer.forward(x, res, keep)
+        h = layer.h
+        if not keep:
+            layer.h = None
+        return h, y
 
     def _lin_bwd(self, layer, dy: ShardedTensor) -> ShardedTensor:
         d = layer.backward(dy)
         return self.mesh.transpose(d) if layer.dataflow == "rs" else d
 
-    def forward(self, x: ShardedTensor, delta: Optional[ShardedTensor]):
+    def forward(self, x: ShardedTensor, delta: Optional[ShardedTensor], keep: bool = True):
         """Input: residual stream x and a pending branch output ``delta`` (added inside LN1).
-        Returns (h, mlp_out): the caller's next LayerNorm adds them."""
-        y = self.ln1.forward(x, delta)            # residual stream becomes x + delta
-        x = self.ln1.h
-        a = self._lin(self.out_proj, self.attn.forward(self._lin(self.in_proj, y)))
-        y = self.ln2.forward(a, x)                # h = x + a
-        h = self.ln2.h
+        Returns (h, mlp_out): the caller's next LayerNorm adds them.  ``keep``: hold what ``backward`` needs."""
+        x, y = self._norm(self.ln1, x, delta, keep)            # residual stream becomes x + delta
+        a = self._lin(self.out_proj, self.attn.forward(self._lin(self.in_proj, y, keep), keep), keep)
+        h, y = self._norm(self.ln2, a, x, keep)                # h = x + a
         if self.ff1._fused and self.ff1.dataflow == "os" and sharded_layers.FUSE_GELU:
-            g, pre = self.ff1.forward_gelu(y)          # GeLU in the GEMM epilogue
-            self.gelu.remember(pre)
+            g, pre = self.ff1.forward_gelu(y, keep)            # GeLU in the GEMM epilogue
+            if keep:
+                self.gelu.remember(pre)
         else:
-            g = self.gelu.forward(self._lin(self.ff1, y))
-        m = self._lin(self.ff2, g)
+            g = self.gelu.forward(self._lin(self.ff1, y, keep), keep)
+        m = self._lin(self.ff2, g, keep)
         return h, m
 
     def backward(self, dh: ShardedTensor, dm: ShardedTensor):
@@ -228,22 +236,23 @@ class GPTModel:
                 t.zero_()
 
     # ------------------------------------------------------------------ training step pieces
-    def forward(self, tokens: ShardedTensor) -> ShardedTensor:
-        """Logits [local tokens, padded vocabulary / C] of whole sequences."""
+    def forward(self, tokens: ShardedTensor, keep: bool = True) -> ShardedTensor:
+        """Logits [local tokens, padded vocabulary / C] of whole sequences.  ``keep``: hold what the backward pass needs; without it
+        the activations are free as soon as they are used, and those that an earlier forward pass holds stay as they are."""
         m, cfg = self.mesh, self.cfg
         pos = lambda k: None if self.pos is None else self.pos.shards[k]
         x = ShardedTensor(m, {k: F.embedding_fwd(tokens.shards[k], self.tok.shards[k], pos(k), cfg.seq) for k in m.coords()})
         delta = None
         for b in self.blocks:
-            x, delta = b.forward(x, delta)
-        y = self.ln_f.forward(x, delta)
-        return self.head.forward(y)                                      # [T/R, Vp/C]
+            x, delta = b.forward(x, delta, keep)
+        _, y = GPTBlock._norm(self.ln_f, x, delta, keep)
+        return self.head.forward(y, keep)                                # [T/R, Vp/C]
 
     def top_logits(self, tokens: ShardedTensor, top: int, temperature: float = 1.0, hard_weight: float = 0.0) -> DistillTargets:
         """This model as a teacher: its ``top`` largest logits per token (whole rows on every device)."""
         if self.mesh.C != 1:
             raise ValueError("a teacher's rows of logits are whole: its mesh has one column")
-        best = {k: l[:, :self.cfg.vocab].float().topk(top, dim=1) for k, l in self.forward(tokens).shards.items()}
+        best = {k: l[:, :self.cfg.vocab].float().topk(top, dim=1) for k, l in self.forward(tokens, keep=False).shards.items()}
         return DistillTargets(ShardedTensor(self.mesh, {k: v.indices for k, v in best.items()}),
                               ShardedTensor(self.mesh, {k: v.values for k, v in best.items()}), temperature, hard_weight)
 

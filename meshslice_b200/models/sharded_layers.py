@@ -83,20 +83,24 @@ class ShardedFFLayer:
         for k, g in self.grad.shards.items():
             g += dw.shards[k]
 
-    def forward_gelu(self, x: ShardedTensor):
+    def forward_gelu(self, x: ShardedTensor, keep: bool = True):
         """y = gelu(x @ W) with the activation applied in the GEMM epilogue (fused 'os' layers
         only).  Returns (gelu output, pre-activation); the caller keeps the latter for backward."""
         if not (self._fused and self.dataflow == "os"):
             raise RuntimeError("forward_gelu needs a fused 'os' layer")
-        self._x = x
+        if keep:
+            self._x = x
         (key, xl), = x.shards.items()
         m, n = xl.shape[0], self.weight.shards[key].shape[1]
         pre = torch.empty(m, n, dtype=xl.dtype, device=xl.device)
         y = self._OS(x, self.weight, act="gelu", pre_act=pre)
         return y, ShardedTensor(self.mesh, {key: pre})
 
-    def forward(self, x: ShardedTensor) -> ShardedTensor:
-        self._x = x
+    def forward(self, x: ShardedTensor, keep: bool = True) -> ShardedTensor:
+        """``keep``, here and in the layers below: hold what ``backward`` needs.  Without it nothing is held, and what an earlier
+        forward pass holds stays as it is."""
+        if keep:
+            self._x = x
         w = self.weight
         if self.dataflow == "os":
             return self._OS(x, w)
@@ -159,11 +163,11 @@ class ShardedLayerNorm:
             self.dgamma, self.dbias = z(), z()
         self._saved = None
 
-    def forward(self, x: ShardedTensor, res: Optional[ShardedTensor] = None):
+    def forward(self, x: ShardedTensor, res: Optional[ShardedTensor] = None, keep: bool = True):
         """Returns y; ``self.h`` holds x + res (the new residual stream)."""
         m = self.mesh
         if m.C == 1:
-            return self._forward_rows(x, res)
+            return self._forward_rows(x, res, keep)
         g = self.gamma if self.affine else None
         b = self.bias if self.affine else None
         G = lambda k: g.shards[k] if g is not None else None
@@ -187,17 +191,19 @@ class ShardedLayerNorm:
             y = ShardedTensor(m, {k: v[0] for k, v in outs.items()})
             mr = ShardedTensor(m, {k: v[1] for k, v in outs.items()})
         self.h = h
-        self._saved = (h, mr)
+        if keep:
+            self._saved = (h, mr)
         return y
 
-    def _forward_rows(self, x: ShardedTensor, res: Optional[ShardedTensor]) -> ShardedTensor:
+    def _forward_rows(self, x: ShardedTensor, res: Optional[ShardedTensor], keep: bool) -> ShardedTensor:
         """Whole rows on every device: one kernel per shard."""
         h, y, mr = {}, {}, {}
         for k in self.mesh.coords():
             g, b = (self.gamma.shards[k], self.bias.shards[k]) if self.affine else (None, None)
             h[k], y[k], mr[k] = F.ln_full(x.shards[k], None if res is None else res.shards[k], g, b, self.eps)
         self.h = ShardedTensor(self.mesh, h)
-        self._saved = (self.h, ShardedTensor(self.mesh, mr))
+        if keep:
+            self._saved = (self.h, ShardedTensor(self.mesh, mr))
         return ShardedTensor(self.mesh, y)
 
     def _exchanger(self, t: ShardedTensor):
@@ -272,14 +278,15 @@ class ShardedAttention:
         self.heads_per_shard = n_heads // mesh.C
         self._saved = None
 
-    def forward(self, x: ShardedTensor) -> ShardedTensor:
+    def forward(self, x: ShardedTensor, keep: bool = True) -> ShardedTensor:
         outs = {}
         for k, t in x.shards.items():
             if t.shape[0] % self.seqlen:
                 raise ValueError("local tokens must be whole sequences (batch divisible by mesh rows)")
             outs[k] = F.attention_fwd(t, t.shape[0] // self.seqlen, self.seqlen, self.heads_per_shard, self.causal,
                                       allow_fallback=self.allow_fallback)
-        self._saved = (x, {k: v for k, v in outs.items()})
+        if keep:
+            self._saved = (x, {k: v for k, v in outs.items()})
         return ShardedTensor(self.mesh, {k: v[0] for k, v in outs.items()})
 
     def backward(self, dy: ShardedTensor) -> ShardedTensor:
@@ -322,10 +329,11 @@ class ShardedWindowAttention:
             F.rotary_qkv(t, self.rotary, self.kv_per_shard, self.group, seq=self.seqlen, inverse=inverse, out=t)
         return t
 
-    def forward(self, x: ShardedTensor) -> ShardedTensor:
+    def forward(self, x: ShardedTensor, keep: bool = True) -> ShardedTensor:
         """With ``rotary``, ``x`` is turned in place."""
         outs = {k: F.window_attention_fwd(self._turn(t, False), *self._shape(t)) for k, t in x.shards.items()}
-        self._saved = (x, outs)
+        if keep:
+            self._saved = (x, outs)
         return ShardedTensor(self.mesh, {k: v[0] for k, v in outs.items()})
 
     def backward(self, dy: ShardedTensor) -> ShardedTensor:
@@ -359,8 +367,9 @@ class GeLU:
         a, b = self._x.local(), y.local()
         return a.is_cuda and a.shape == b.shape and a.dtype == b.dtype == torch.bfloat16
 
-    def forward(self, x: ShardedTensor) -> ShardedTensor:
-        self._x = x
+    def forward(self, x: ShardedTensor, keep: bool = True) -> ShardedTensor:
+        if keep:
+            self._x = x
         return x.map(F.gelu)
 
     def backward(self, dy: ShardedTensor) -> ShardedTensor:

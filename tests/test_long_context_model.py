@@ -225,3 +225,48 @@ def test_decoder_on_a_gpu_reads_nothing_outside_its_tables():
         same = d.step(tokens, torch.full((3,), 39, device="cuda"))
         assert same[1].isfinite().all() and same[0].isfinite().all()
     _native.check_status()
+
+
+def _held(model):
+    """What the layers hold for a backward pass, by identity."""
+    layers = [l for b in model.blocks for l in (*b.layers(), b.attn, b.gelu)] + [model.ln_f, model.head]
+    return [(type(l).__name__, getattr(l, "_x", None), getattr(l, "_saved", None)) for l in layers]
+
+
+@pytest.mark.parametrize("change", [{}, dict(rotary=None), dict(window=0, kv_heads=0, sinks=0, rotary=None)])
+def test_teacher_and_decoder_hold_nothing_and_disturb_nothing(change):
+    """Without a backward pass to come no activation is held; what a forward pass holds is there when the decoder or a teacher's logits
+    were asked for in between, and its gradients are the same."""
+    cfg = GPTConfig(**{**CFG.__dict__, **change})
+    mesh = EmuMesh(1, 1)
+    model = GPTModel(mesh, cfg)
+    gen = torch.Generator().manual_seed(5)
+    ids = torch.randint(0, cfg.vocab, (2 * cfg.seq,), generator=gen)
+    tokens = ShardedTensor(mesh, {(0, 0): ids})
+
+    def between():
+        model.top_logits(tokens, 3)
+        if cfg.window:
+            d = GPTDecoder(model, 2)
+            d.prefill(ids.view(2, -1)[:, :4])
+            d.step(ids[:2], torch.full((2,), 4))
+    between()
+    assert all(x is None and saved is None for _, x, saved in _held(model))
+    assert all(l.h is None for b in model.blocks for l in (b.ln1, b.ln2)) and model.ln_f.h is None
+
+    block = model.blocks[0]
+    x, dh, dm = (torch.randn(2 * cfg.seq, cfg.d_model, generator=gen) for _ in range(3))
+    grads = []
+    for disturb in (False, True):
+        model.zero_grad()
+        st = lambda t: ShardedTensor(mesh, {(0, 0): t.clone()})
+        h, _ = block.forward(st(x), None)
+        held, residual = _held(model), h.shards[(0, 0)].clone()
+        assert any(v is not None for _, v, _ in held)
+        if disturb:
+            between()
+            assert all(a[1] is b[1] and a[2] is b[2] for a, b in zip(held, _held(model)))
+            assert torch.equal(h.shards[(0, 0)], residual)
+        dx, _ = block.backward(st(dh), st(dm))
+        grads.append([dx.shards[(0, 0)]] + [g.shards[(0, 0)].clone() for _, _, g, _ in model.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
