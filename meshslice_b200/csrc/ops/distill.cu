@@ -2,6 +2,7 @@
 #include "distill.h"
 
 #include <cuda_bf16.h>
+#include <float.h>
 
 #include <type_traits>
 
@@ -70,14 +71,35 @@ __device__ __forceinline__ uint4 cut(uint4 u, int v, int valid) {
 
 // Which exponentials a row needs: those of z / T, of z (one kind serves both where T = 1), both, or, where T = 2 or 4, those of z as the
 // squares of those of z / T, or the squares of these: the special-function unit gives 16 a cycle and SM, so that four of them an element
-// take 180 us for 4096 rows of 50257 (148 SMs), two 90 (temperature 3: 239 us, 2: 165).
+// take 180 us for 4096 rows of 50257 (148 SMs), two 90 (temperature 3: 244 us, 2: 165).
 enum Kind { kSoft = 1, kHard = 2, kTwo = 3, kSquare = 5, kFourth = 9 };
 constexpr int powers(int K) { return K == kSquare ? 2 : K == kFourth ? 4 : 1; }
 
 // 2^x exponents of z over a temperature: z c - m c with the product z c exact (one rounding, of the result) and m c rounded once for
 // the whole row: `ref`, the same wherever m is.  Sums are relative to 2^ref; that ref is not quite m c cancels in every ratio, and the
 // loss takes ref itself.
+// That holds while ref is off by little (1 at kNear).  From there on, where masks of the type's lowest value or of -1e30 are, neighbours of
+// bf16 are 2^16 or more apart in exponent: a term is 1, where z is m, or nothing.  Then c gives way to a power of two that brings m to
+// 2^17: z and m scaled by it are exact, and neighbours still 2^9 apart.  Sums are relative to m itself.
+constexpr float kNear = 16777216.f;
 __device__ __forceinline__ float ref_of(float m, float c) { return __fmul_rn(m, c); }
+__device__ __forceinline__ bool near(float ref) { return fabsf(ref) < kNear; }
+struct Exponent {
+  float c, ref;
+};
+__device__ __forceinline__ Exponent exponent_of(float m, float c) {
+  Exponent e{c, ref_of(m, c)};
+  if (!near(e.ref)) {
+    e.c = __uint_as_float(min(271u - ((__float_as_uint(m) >> 23) & 255u), 254u) << 23);
+    e.ref = m * e.c;
+  }
+  return e;
+}
+// What sums relative to m0 are times, relative to m1 > m0 (of the p-th powers of the terms).  From or to a far one nothing is left, also where
+// both references are beyond fp32.
+__device__ __forceinline__ float lowered(float m0, float m1, float c, float p = 1.f) {
+  return exp2_ftz(fmaxf(p * ref_of(m0, c) - p * ref_of(m1, c), -200.f));
+}
 
 // A thread's running maximum m, and sums of exp(z) and exp(z / T) relative to it.  (Behind the exponentials scalar sums: packing their
 // results takes moves.)
@@ -85,15 +107,25 @@ template <int K>
 struct Sums {
   static constexpr bool soft_exp = K & kSoft, squares = powers(K) > 1;
   float m = -INFINITY, soft = 0.f, hard = 0.f;
-  // What the sums are relative to; where T = 2 or 4 the hard one's is that times the soft one's.
-  __device__ __forceinline__ float soft_ref(float c) const { return ref_of(m, c); }
-  __device__ __forceinline__ float hard_ref(float c) const { return squares ? powers(K) * ref_of(m, c) : ref_of(m, kLog2e); }
+  // Where T = 2 or 4 what the hard one is relative to is a power of what the soft one is.
+  static __device__ __forceinline__ float soft_lowered(float m0, float m1, float c) { return lowered(m0, m1, c); }
+  static __device__ __forceinline__ float hard_lowered(float m0, float m1, float c) {
+    return squares ? lowered(m0, m1, c, powers(K)) : lowered(m0, m1, kLog2e);
+  }
+  // z less what the sums are relative to, of z / T and of z.
+  __device__ __forceinline__ float soft_above(float z, float c) const {
+    const float r = ref_of(m, c);
+    return (near(r) ? fmaf(z, c, -r) : (z - m) * c) * kLn2;
+  }
+  __device__ __forceinline__ float hard_above(float z, float c) const {
+    const float r = ref_of(m, squares ? c : kLog2e);
+    return (near(r) ? fmaf(z, kLog2e, squares ? -powers(K) * r : -r) : (z - m) * kLog2e) * kLn2;
+  }
   __device__ __forceinline__ void raise(float to, float c) {
     if (to > m) {
-      const float s0 = soft_ref(c), h0 = hard_ref(c);
+      soft *= soft_lowered(m, to, c);                     // (while m is -inf the sums are 0)
+      hard *= hard_lowered(m, to, c);
       m = to;
-      soft *= exp2_ftz(s0 - soft_ref(c));                 // (0 while m is -inf: the sums are 0)
-      hard *= exp2_ftz(h0 - hard_ref(c));
     }
   }
   template <int N>
@@ -102,9 +134,9 @@ struct Sums {
 #pragma unroll
     for (int j = 0; j < N; ++j) top = max_bf16x2(max_bf16x2(max_bf16x2(top, u[j].x), max_bf16x2(u[j].y, u[j].z)), u[j].w);
     raise(fmaxf(lo(top), hi(top)), c);
-    if (m > -INFINITY) {
-      const float c0 = soft_exp ? c : kLog2e;
-      const uint64_t cs = both(c0), rs = both(-ref_of(m, c0)), ch = both(kLog2e), rh = both(-ref_of(m, kLog2e));
+    const float c0 = soft_exp ? c : kLog2e, r0 = ref_of(m, c0), r1 = ref_of(m, kLog2e);
+    if (near(K == kTwo ? fmaxf(fabsf(r0), fabsf(r1)) : r0)) {
+      const uint64_t cs = both(c0), rs = both(-r0), ch = both(kLog2e), rh = both(-r1);
       float ps[4] = {}, ph[4] = {};
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -139,38 +171,41 @@ struct Sums {
       else hard += p;
       if (K == kTwo || squares) hard += (ph[0] + ph[1]) + (ph[2] + ph[3]);
     } else {
-      // while everything seen is -inf nothing counts, except that a NaN has to show
+      // far from zero, or everything seen is -inf: then nothing counts, except that a NaN has to show
+      Exponent es = exponent_of(m, c0), eh = exponent_of(m, kLog2e);
+      if (m == -INFINITY) es.ref = eh.ref = 0.f;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const uint32_t w[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float a = lo(w[i]), b = hi(w[i]), n = (a == a ? 0.f : a) + (b == b ? 0.f : b);
-          soft += n;
-          hard += n;
+          const float a = exp2_ftz(fmaf(lo(w[i]), es.c, -es.ref)), b = exp2_ftz(fmaf(hi(w[i]), es.c, -es.ref));
+          if (soft_exp) soft += a + b;
+          if (K == kTwo) hard += exp2_ftz(fmaf(lo(w[i]), eh.c, -eh.ref)) + exp2_ftz(fmaf(hi(w[i]), eh.c, -eh.ref));
+          else if (!soft_exp || squares) hard += a + b;        // (powers of 1 and of nothing)
         }
       }
     }
   }
   // Those of the warp's lanes, left in red (3 * 32 floats) by each warp / those of `warps` warps, for every thread that comes to read.
   __device__ __forceinline__ void leave(float c, float* red) {
-    const float s0 = soft_ref(c), h0 = hard_ref(c), mine = m;
+    const float mine = m;
     m = warp_max(m);
     // (a thread that has seen nothing but -inf has sums of 0, or NaN)
     const bool as_is = mine == m || mine == -INFINITY;
-    soft = warp_sum(as_is ? soft : soft * exp2_ftz(s0 - soft_ref(c)));
-    hard = warp_sum(as_is ? hard : hard * exp2_ftz(h0 - hard_ref(c)));
+    soft = warp_sum(as_is ? soft : soft * soft_lowered(mine, m, c));
+    hard = warp_sum(as_is ? hard : hard * hard_lowered(mine, m, c));
     const int w = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) { red[w] = m; red[32 + w] = soft; red[64 + w] = hard; }
   }
   __device__ __forceinline__ void join(float c, const float* red, int warps) {
     const int l = threadIdx.x & 31;
     m = l < warps ? red[l] : -INFINITY;
-    const float s0 = soft_ref(c), h0 = hard_ref(c), mine = m;
+    const float mine = m;
     m = warp_max(m);
     const bool as_is = mine == m || mine == -INFINITY;
-    soft = warp_sum(l < warps ? red[32 + l] * (as_is ? 1.f : exp2_ftz(s0 - soft_ref(c))) : 0.f);
-    hard = warp_sum(l < warps ? red[64 + l] * (as_is ? 1.f : exp2_ftz(h0 - hard_ref(c))) : 0.f);
+    soft = warp_sum(l < warps ? red[32 + l] * (as_is ? 1.f : soft_lowered(mine, m, c)) : 0.f);
+    hard = warp_sum(l < warps ? red[64 + l] * (as_is ? 1.f : hard_lowered(mine, m, c)) : 0.f);
     if (K == kSoft) hard = soft;             // T = 1, or the labels have no weight
     if (K == kHard) soft = hard;
   }
@@ -311,16 +346,19 @@ __device__ __forceinline__ RowTarget read_entries(const DistillArgs& a, int row,
   return t;
 }
 
-// What the gradient of a row is made of: soft * 2^(z c - ref) + hard * 2^(z log2(e) - hard_ref), less `drop` times an entry's
+// What the gradient of a row is made of: soft * 2^(z c - ref) + hard * 2^(z hard_c - hard_ref), less `drop` times an entry's
 // probability and `label` at the label.  From sums relative to the same references.
 struct Weights {
-  float ref, hard_ref, soft, hard, drop, label;
+  float c, ref, hard_c, hard_ref, soft, hard, drop, label;
 };
 template <int K>
 __device__ __forceinline__ Weights weights_of(const DistillArgs& a, float m, float soft, float hard, bool some, bool label) {
   Weights w;
-  w.ref = ref_of(m, K == kHard ? kLog2e : kLog2e / a.temperature);
-  w.hard_ref = ref_of(m, kLog2e);
+  const Exponent es = exponent_of(m, K == kHard ? kLog2e : kLog2e / a.temperature), eh = exponent_of(m, kLog2e);
+  w.c = es.c;
+  w.ref = es.ref;
+  w.hard_c = eh.c;
+  w.hard_ref = eh.ref;
   w.drop = some ? (1.f - a.hard) * a.temperature * a.scale : 0.f;
   w.label = label ? a.hard * a.scale : 0.f;
   w.soft = w.drop / soft;
@@ -337,27 +375,27 @@ __device__ __forceinline__ float grad_of(float e, float hard, const Weights& w) 
   return fmaf(e, w.soft, hard * w.hard);
 }
 template <int K>
-__device__ __forceinline__ uint32_t grad_pair(uint32_t z, const Weights& w, float c) {
+__device__ __forceinline__ uint32_t grad_pair(uint32_t z, const Weights& w) {
   float a, b, x = 0.f, y = 0.f;
-  split(fma2(unpack2(z), both(K == kHard ? kLog2e : c), both(-w.ref)), a, b);
+  split(fma2(unpack2(z), both(w.c), both(-w.ref)), a, b);
   if (K == kTwo) {
-    split(fma2(unpack2(z), both(kLog2e), both(-w.hard_ref)), x, y);
+    split(fma2(unpack2(z), both(w.hard_c), both(-w.hard_ref)), x, y);
     x = exp2_ftz(x);
     y = exp2_ftz(y);
   }
   return pack(grad_of<K>(exp2_ftz(a), x, w), grad_of<K>(exp2_ftz(b), y, w));
 }
 template <int K>
-__device__ __forceinline__ float grad_one(float z, const Weights& w, float c) {
-  return grad_of<K>(exp2_ftz(fmaf(z, K == kHard ? kLog2e : c, -w.ref)), K == kTwo ? exp2_ftz(fmaf(z, kLog2e, -w.hard_ref)) : 0.f, w);
+__device__ __forceinline__ float grad_one(float z, const Weights& w) {
+  return grad_of<K>(exp2_ftz(fmaf(z, w.c, -w.ref)), K == kTwo ? exp2_ftz(fmaf(z, w.hard_c, -w.hard_ref)) : 0.f, w);
 }
 template <int K>
-__device__ __forceinline__ uint4 grad_whole(uint4 u, const Weights& w, float c) {
-  return make_uint4(grad_pair<K>(u.x, w, c), grad_pair<K>(u.y, w, c), grad_pair<K>(u.z, w, c), grad_pair<K>(u.w, w, c));
+__device__ __forceinline__ uint4 grad_whole(uint4 u, const Weights& w) {
+  return make_uint4(grad_pair<K>(u.x, w), grad_pair<K>(u.y, w), grad_pair<K>(u.z, w), grad_pair<K>(u.w, w));
 }
 template <int K>
-__device__ __forceinline__ uint4 grad_vector(uint4 u, int v, int valid, const Weights& w, float c) {
-  const uint4 g = grad_whole<K>(u, w, c);
+__device__ __forceinline__ uint4 grad_vector(uint4 u, int v, int valid, const Weights& w) {
+  const uint4 g = grad_whole<K>(u, w);
   if (v * 8 + 8 <= valid) return g;
   uint32_t r[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
@@ -434,22 +472,21 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
       Sums<K> sum;
       sum.join(c, red[parity], T >> 5);
       const Weights w = weights_of<K>(a, sum.m, sum.soft, sum.hard, t.some, t.label >= 0);
-      const float rs = sum.soft_ref(c), rh = sum.hard_ref(c);
       float cross = 0.f, total = 0.f;
       for (int k = l; k <= a.top; k += 32) {
         const int at = e.at[k];
         if (at < 0) continue;
         const float z = raw.p[k], p = e.p[k], drop = drop_of(w, at, p, t.label);
         if (p != 0.f) {
-          cross += p * (fmaf(z, c, -rs) * kLn2);
+          cross += p * sum.soft_above(z, c);
           total += p;
         }
         if (drop == 0.f) e.at[k] = -1;                       // (its column is as the others)
-        else e.p[k] = grad_one<K>(z, w, c) - drop;
+        else e.p[k] = grad_one<K>(z, w) - drop;
       }
       cross = warp_sum(cross);
       total = warp_sum(total);
-      if (l == 0) a.loss[row] = loss_of(a, t, sum.soft, sum.hard, cross, total, t.label >= 0 ? fmaf(y, kLog2e, -rh) * kLn2 : 0.f);
+      if (l == 0) a.loss[row] = loss_of(a, t, sum.soft, sum.hard, cross, total, t.label >= 0 ? sum.hard_above(y, c) : 0.f);
     }
     const int rows = (a.rows - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x;
     rewrite(blockIdx.x + (rows - 1) * gridDim.x, parity ^ 1);
@@ -506,7 +543,7 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
       for (int g = 0; g < whole; ++g, at += kStep, to += kStep, next += kStep) {
         if (learnt) {
 #pragma unroll
-          for (int j = 0; j < kVec; ++j) to[j * T] = grad_whole<K>(at[j * T], w, c);
+          for (int j = 0; j < kVec; ++j) to[j * T] = grad_whole<K>(at[j * T], w);
         } else {
 #pragma unroll
           for (int j = 0; j < kVec; ++j) to[j * T] = make_uint4(0u, 0u, 0u, 0u);
@@ -522,7 +559,7 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
     if (whole == 0) bar_sync(kTaken, T + 32);
 #pragma unroll 1
     for (int v = rest; v < nv; v += T) {
-      out[v] = learnt ? grad_vector<K>(ring[v], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+      out[v] = learnt ? grad_vector<K>(ring[v], v, valid, w) : make_uint4(0u, 0u, 0u, 0u);
       if (more) cp_async16(ring + v, z + v);
     }
     cp_async_commit();
@@ -532,7 +569,13 @@ distill_row_kernel(const __grid_constant__ DistillArgs a) {
 }
 
 // Of sums relative to 2^ref, relative to 2^(m c): times 2^(ref - m c), whose exponent fma gives exactly.
-__device__ __forceinline__ float shift(float m, float c) { return m == -INFINITY ? 1.f : exp2f(fmaf(-m, c, ref_of(m, c))); }
+__device__ __forceinline__ float shift(float m, float c) { return near(ref_of(m, c)) ? exp2f(fmaf(-m, c, ref_of(m, c))) : 1.f; }
+// sum p (z - m) over the entries, from the sum of p z: of logits whose differences are far below their size, what the sums' rounding
+// (2^-18 of it: up to 1024 entries in fp32) cannot tell from 0 is 0.
+__device__ __forceinline__ float above(float dot, float total, float m, float c) {
+  const float d = dot - total * m;
+  return !near(ref_of(m, c)) && fabsf(d) <= fminf(fabsf(m), FLT_MAX) * 3.814697265625e-6f ? 0.f : d;
+}
 
 // Statistics of a slice.
 __global__ void __launch_bounds__(512)
@@ -601,7 +644,7 @@ distill_grad_kernel(const __grid_constant__ DistillArgs a) {
     total = warp_sum(total);
     if (threadIdx.x == 0) {
       target = t;
-      if (a.loss != nullptr) a.loss[row] = loss_of(a, t, soft, hard, (s[3] - total * m) / a.temperature, total, s[4] - m);
+      if (a.loss != nullptr) a.loss[row] = loss_of(a, t, soft, hard, above(s[3], total, m, c) / a.temperature, total, s[4] - m);
     }
   }
   __syncthreads();
@@ -611,7 +654,7 @@ distill_grad_kernel(const __grid_constant__ DistillArgs a) {
     const int at = e.at[k] - a.col_offset;
     const bool here = e.at[k] >= 0 && at >= 0 && at < valid;
     const float drop = here ? drop_of(w, e.at[k], e.p[k], target.label) : 0.f;
-    if (drop != 0.f) e.p[k] = grad_one<K>(__bfloat162float(z[at]), w, c) - drop;
+    if (drop != 0.f) e.p[k] = grad_one<K>(__bfloat162float(z[at]), w) - drop;
     else e.at[k] = -1;
   }
   __syncthreads();
@@ -624,7 +667,7 @@ distill_grad_kernel(const __grid_constant__ DistillArgs a) {
 #pragma unroll
     for (int j = 0; j < kVec; ++j) {
       const int v = v0 + j * T;
-      if (v < nvec) reinterpret_cast<uint4*>(out)[v] = v < learnt ? grad_vector<K>(u[j], v, valid, w, c) : make_uint4(0u, 0u, 0u, 0u);
+      if (v < nvec) reinterpret_cast<uint4*>(out)[v] = v < learnt ? grad_vector<K>(u[j], v, valid, w) : make_uint4(0u, 0u, 0u, 0u);
     }
   }
   __syncthreads();

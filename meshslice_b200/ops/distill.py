@@ -186,7 +186,12 @@ def distill_grad(logits, teacher_ids, teacher_logits, col_offset: int, vocab: in
     plogp = torch.where(p != 0, p * torch.log(torch.where(p != 0, p, 1.0)), 0.0).sum(1)
     loss = torch.zeros(n)
     if w != 1.0:
-        loss = loss + torch.where(some, (1 - w) * T * (T * (plogp + torch.log(soft)) - (dot - p.sum(1) * m)), 0.0)
+        # sum p (z - m): of logits far beyond their differences (masks of the type's lowest value) what the sums' rounding cannot tell
+        # from 0 is 0
+        above = dot - p.sum(1) * m
+        far = (m * (math.log2(math.e) / T)).abs() >= 2.0 ** 24
+        above = torch.where(far & (above.abs() <= m.abs().clamp_max(torch.finfo(torch.float32).max) * 2.0 ** -18), 0.0, above)
+        loss = loss + torch.where(some, (1 - w) * T * (T * (plogp + torch.log(soft)) - above), 0.0)
     if w != 0.0:
         loss = loss + torch.where(label, w * (torch.log(hard) - (zy - m)), 0.0)
     valid = max(0, min(cols, vocab - col_offset))

@@ -253,3 +253,53 @@ def test_kernel_refusals():
         F.distill_loss_grad(z, ids.cpu(), values, 50, 1.0)
     with pytest.raises(ValueError):
         F.distill_loss_grad(z, ids.repeat(1, 200), values.repeat(1, 200), 50, 1.0)
+
+
+LOWEST = torch.finfo(torch.bfloat16).min
+FILLS = [LOWEST, -1e30, -1e10, -1e4]
+
+
+def masked(dev, vocab, fill, T, w, how):
+    """Logits that a mask has filled: a run of columns longer than what a thread sums at a time, a few, all of a row, all but one; and one
+    that is as far above the others.  The teacher's entries and the label are beside the mask, in the third row inside it."""
+    n, cols, top = 5, -(-vocab // 8) * 8, 6
+    z, ids, values, targets = data(n, vocab, cols, top, seed=3)
+    ids = vocab - 1 - torch.arange(top).repeat(n, 1) * max(1, vocab // 40)
+    targets = ids[:, 2].clone()
+    z[0, : vocab * 3 // 4] = fill
+    z[1, 8:40] = fill
+    z[2] = fill
+    z[3] = fill
+    z[3, vocab - 1] = 1.5
+    ids[3], targets[3] = torch.tensor([vocab - 1] + [-1] * (top - 1)), vocab - 1
+    z[4, 3] = -fill
+    ids[4], targets[4] = torch.tensor([3] + [-1] * (top - 1)), 3
+    want = definition(z, ids, values, targets, vocab, T, w)
+    a = [t.to(dev) for t in (z, ids, values, targets)]
+    got = how(a, vocab, T, w)
+    assert got[0].isfinite().all() and got[1].isfinite().all()
+    check(got, want, 0.5)
+    # beyond 2^24 T not by the size of the logits, but by that of their differences (below, sums of p z are rounded to their own size)
+    for r in (2, 3, 4) if abs(fill) >= 2.0 ** 24 * T else ():
+        p = torch.softmax(values[r][(ids[r] >= 0)].double() / T, 0)
+        rest = math.log(vocab) + 1 + (p * p.log()).sum().abs()
+        assert abs(got[0][r].double().cpu() - want[0][r]) <= 2.0 ** -19 * ((1 - w) * T * T + w) * rest
+
+
+WAYS = {"rows": lambda a, vocab, T, w: F.distill_loss_grad(a[0], a[1], a[2], vocab, 0.5, T, a[3], w),
+        "slices": lambda a, vocab, T, w: slices(*a, vocab, T, w, [0, vocab // 32 * 8, vocab // 16 * 8, a[0].shape[1]], 0.5)}
+
+
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("T,w", SETTINGS)
+@pytest.mark.parametrize("fill", FILLS)
+def test_cpu_masked_logits(fill, T, w, way):
+    masked("cpu", 203, fill, T, w, WAYS[way])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,way", [(203, "rows"), (6000, "rows"), (30011, "rows"), (104000, "rows"), (6000, "slices")])
+@pytest.mark.parametrize("T,w", SETTINGS + [(3.0, 0.5), (40.0, 0.5)])
+@pytest.mark.parametrize("fill", FILLS)
+def test_kernel_masked_logits(fill, T, w, vocab, way):
+    masked("cuda", vocab, fill, T, w, WAYS[way])
