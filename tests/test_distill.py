@@ -303,3 +303,90 @@ def test_cpu_masked_logits(fill, T, w, way):
 @pytest.mark.parametrize("fill", FILLS)
 def test_kernel_masked_logits(fill, T, w, vocab, way):
     masked("cuda", vocab, fill, T, w, WAYS[way])
+
+
+def dense(z, ids, values, targets, vocab, T, w):
+    """``definition`` for many rows at a time, on the tensors' device; every id occurs once."""
+    x, n = z[:, :vocab].double(), z.shape[0]
+    there = (ids >= 0) & (ids < vocab) & (values.float() != -math.inf)
+    r, k = there.nonzero(as_tuple=True)
+    t = torch.full_like(x, -math.inf)
+    t[r, ids[r, k]] = values[r, k].double()
+    p = torch.softmax(t / T, 1).nan_to_num_(0.0)                       # (rows without entries)
+    some = there.any(1)
+    plogp = (p * p.clamp_min(1e-300).log()).sum(1)
+    logq, m, far = torch.log_softmax(x / T, 1), x.amax(1), (x - x.amax(1, keepdim=True)).abs()
+    loss = torch.where(some, (1 - w) * T * T * (plogp - (p * logq).sum(1)), 0.0)
+    parts_of_loss = T * T * (1 + plogp.abs() + torch.logsumexp(x / T, 1).abs() + m.abs()) + T * (p * far).sum(1)
+    size = 1 + torch.where(some, parts_of_loss if w != 1.0 else 0.0, 0.0)
+    q = logq.exp_() * some[:, None] * ((1 - w) * T)
+    grad, parts = q - (1 - w) * T * p, q + (1 - w) * T * p
+    label = ((targets >= 0) & (targets < vocab)).nonzero()[:, 0]
+    y = targets[label]
+    if w != 0.0:
+        logq = torch.log_softmax(x, 1)
+        loss[label] -= w * logq[label, y]
+        size[label] += torch.logsumexp(x, 1)[label].abs() + far[label, y] + m[label].abs()
+        hard = torch.zeros_like(x)
+        hard[label] = w * logq[label].exp()
+        grad += hard
+        parts += hard
+        grad[label, y] -= w
+        parts[label, y] += w
+    pad = lambda v: torch.nn.functional.pad(v, (0, z.shape[1] - vocab)).cpu()
+    return loss.cpu(), pad(grad), size.cpu(), pad(parts)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("T,w", [(1.0, 0.3), (0.7, 1.0), (2.0, 0.5), (4.0, 0.1), (3.0, 0.5)])
+@pytest.mark.parametrize("rows,vocab,top", [(3200, 1003, 9), (1100, 8200, 200), (900, 12003, 20), (700, 45007, 33), (450, 60001, 64)])
+def test_kernel_rows_of_a_cta_follow_one_another(rows, vocab, top, T, w, in_place):
+    """Two to four rows for every CTA that is resident, of each width: entries, labels, neither and NaN by turns.  Every row is what it is
+    among a few others, bit by bit, and what the definition says."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    cols = -(-vocab // 16) * 16
+    z = torch.empty(rows, cols, device="cuda", dtype=torch.bfloat16).normal_(0, 2, generator=g)
+    values, ids = torch.rand(rows, vocab, device="cuda", generator=g).topk(top, 1)
+    values = (values - 0.9) * 40 + torch.empty_like(values).normal_(0, 3, generator=g)
+    targets = torch.randint(0, vocab, (rows,), device="cuda", generator=g)
+    targets[::2] = ids[::2, 0]
+    of = torch.randint(0, 6, (rows,), device="cuda", generator=g)      # 0, 1: all; 2: no label; 3: no entry; 4: some entries; 5: neither
+    targets[(of == 2) | (of == 5)] = -1
+    ids[(of == 3) | (of == 5)] = -1
+    ids[of == 4, top // 2:] = vocab
+    nan = (of == 5) & (torch.arange(rows, device="cuda") % 2 == 0)
+    z[nan] = float("nan")
+    a = (ids, values, vocab, 0.25, T, targets, w)
+    few = [F.distill_loss_grad(z[i:i + 90], ids[i:i + 90], values[i:i + 90], vocab, 0.25, T, targets[i:i + 90], w) for i in range(0, rows, 90)]
+    x = z.clone() if in_place else z
+    loss, grad = F.distill_loss_grad(x, *a, out=x if in_place else None)
+    assert torch.equal(loss, torch.cat([l for l, _ in few])) and torch.equal(grad, torch.cat([g for _, g in few]))
+    assert loss[of == 5].count_nonzero() == 0 and grad[of == 5].count_nonzero() == 0 and grad[:, vocab:].count_nonzero() == 0
+    check((loss, grad), dense(z.masked_fill(nan[:, None], 0.0), ids, values, targets, vocab, T, w), 0.25)
+
+
+@pytest.mark.gpu
+def test_kernel_on_another_stream_and_in_a_graph():
+    z, ids, values, targets = (t.cuda() for t in data(2500, 1003, 1008, 9, True))
+    a = (1003, 0.5, 2.0, targets, 0.5)
+    want = F.distill_loss_grad(z, ids, values, *a)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = z.clone().mul_(1)
+        got = F.distill_loss_grad(x, ids, values, *a, out=x)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got[0], want[0]) and torch.equal(x, want[1])
+    x = torch.zeros_like(z)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss, grad = F.distill_loss_grad(x, ids, values, *a)
+        stats = F.distill_partial(x, ids, values, 0, 1003, 2.0, targets)
+        by_slices = F.distill_grad(x, ids, values, 0, 1003, 0.5, stats, 2.0, targets, 0.5)
+    for _ in range(2):
+        x.copy_(z)
+        graph.replay()
+        assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
+        assert torch.allclose(by_slices[0], loss, rtol=1e-4, atol=1e-4) and torch.allclose(by_slices[1].float(), grad.float(), rtol=2 ** -6, atol=2.5e-5)
+        x.zero_()
