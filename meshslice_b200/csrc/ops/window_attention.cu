@@ -71,7 +71,8 @@ __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xfffffff
 
 // 2^x of two lanes on the FMA pipe, for the share of the exponentials that would queue for the special-function unit: x = n + f with n
 // the nearest whole number, 2^f by the polynomial of degree 5 with the smallest largest relative error on [-1/2, 1/2] (Remez exchange;
-// 2^-23.7, with fp32 rounding 2^-22.2), n added to the exponent.  Below -125 the result is about 2^-125 and not zero; NaN stays NaN.
+// 2^-23.7, with fp32 rounding 2^-22.2), times 2^n.  (n added to the exponent's bits would make a NaN the largest number.)  Below -125
+// the result is about 2^-125 and not zero; NaN stays NaN.  x stays below 127 wherever the result is used.
 __device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
   split(x, a, b);
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-125.0f));
@@ -84,11 +85,8 @@ __device__ __forceinline__ void exp2_poly(uint64_t x, float& a, float& b) {
   p = fma2(p, f, f32x2(2.402212024e-01f, 2.402212024e-01f));
   p = fma2(p, f, f32x2(6.931469440e-01f, 6.931469440e-01f));
   p = fma2(p, f, f32x2(1.000000119e+00f, 1.000000119e+00f));
-  float ra, rb;
-  split(p, a, b);
-  split(r, ra, rb);
-  a = __int_as_float(__float_as_int(a) + (__float_as_int(ra) << 23));
-  b = __int_as_float(__float_as_int(b) + (__float_as_int(rb) << 23));
+  split(r, a, b);
+  split(mul2(p, f32x2(__int_as_float((__float_as_int(a) << 23) + 0x3f800000), __int_as_float((__float_as_int(b) << 23) + 0x3f800000))), a, b);
 }
 
 __device__ __forceinline__ void load_half(uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int col, int row, int b) {

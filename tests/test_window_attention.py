@@ -250,3 +250,23 @@ def test_kernel_keys_of_minus_infinity(sinks, dead):
     assert held.sum() >= 300 and (~held).any() == (0 in dead or sinks == 0)
     got = out.double().cpu()
     assert rel(got[held], want[held]) < OUT and got[~held].isnan().any(1).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 300, 2, 2, 100, 0), (1, 700, 1, 1, 0, 0), (1, 640, 1, 2, 200, 4)])
+def test_kernel_nan_in_the_scores_of_a_query(shape):
+    """A NaN in a query is a NaN in every gradient of the keys and values that it sees, whichever unit made the exponential, and in its
+    own; sequences and heads beside it stay as they are."""
+    batch, seq, kv, group, window, sinks = shape
+    qkv, dout, out, lse, dqkv = on_gpu(shape)
+    dout = dout.masked_fill(dout == 0, 0.01)
+    j = torch.arange(seq, device="cuda")
+    for bad in list(range(seq - 40, seq)) + [0, 1, 130, 131, 147]:
+        x = qkv.clone()
+        x[bad, 3] = float("nan")                                # the first query head of the first key head
+        o, l = F.window_attention_fwd(x, *shape)
+        g = F.window_attention_bwd(dout, x, o, l, *shape).view(seq, kv, group + 2, 128)
+        seen = (j <= bad) & ((bad - j < (window or seq)) | (j < sinks))
+        assert g[seen, 0, group:].isnan().all() and g[bad, 0, 0].isnan().all() and l[0, 0, bad].isnan()
+        if kv > 1:
+            assert torch.equal(g[:, 1], F.window_attention_bwd(dout, qkv, out, lse, *shape).view_as(g)[:, 1])
