@@ -71,6 +71,7 @@ def window_attention_fwd(qkv, batch: int, seq: int, kv_heads: int, group: int = 
     (out [batch * seq, kv_heads * group * D], lse [batch, kv_heads * group, seq])."""
     D = _check(qkv, batch, seq, kv_heads, group, window, sinks)
     heads = kv_heads * group
+    window, sinks = min(window, seq), min(sinks, seq)          # (more is the whole sequence, and might not fit the kernels' 32 bits)
     if qkv.is_cuda:
         stream, device = _native.stream_on(qkv.get_device()), qkv.device
         out = torch.empty(batch * seq, heads * D, dtype=qkv.dtype, device=device)
@@ -89,6 +90,7 @@ def window_attention_bwd(dout, qkv, out, lse, batch: int, seq: int, kv_heads: in
     """Gradient of ``qkv`` in its layout; shared key/value heads get the sum over their query heads."""
     D = _check(qkv, batch, seq, kv_heads, group, window, sinks)
     heads = kv_heads * group
+    window, sinks = min(window, seq), min(sinks, seq)
     for name, t in (("dout", dout), ("out", out)):
         if t.shape != (batch * seq, heads * D) or t.dtype is not qkv.dtype or t.get_device() != qkv.get_device():
             raise ValueError(f"{name} must be {qkv.dtype} [{batch * seq}, {heads * D}] beside qkv (got {t.dtype} {tuple(t.shape)} on {t.device})")

@@ -270,3 +270,24 @@ def test_kernel_nan_in_the_scores_of_a_query(shape):
         assert g[seen, 0, group:].isnan().all() and g[bad, 0, 0].isnan().all() and l[0, 0, bad].isnan()
         if kv > 1:
             assert torch.equal(g[:, 1], F.window_attention_bwd(dout, qkv, out, lse, *shape).view_as(g)[:, 1])
+
+
+def long_window(dev, D):
+    qkv, dout = (t.to(dev) for t in inputs(1, 150, 1, 1, D))
+    a = (1, 150, 1, 1)
+    out, lse = F.window_attention_fwd(qkv, *a, 150, 0)
+    grad = F.window_attention_bwd(dout, qkv, out, lse, *a, 150, 0)
+    for window, sinks in ((1 << 31, 0), (1 << 70, 0), (1 << 32, 1 << 32), (1, 1 << 40)):
+        o, l = F.window_attention_fwd(qkv, *a, window, sinks)
+        assert torch.equal(o, out) and torch.equal(l, lse)
+        assert torch.equal(F.window_attention_bwd(dout, qkv, o, l, *a, window, sinks), grad)
+
+
+def test_window_beyond_32_bits():
+    """A window or a number of first tokens beyond the sequence is the whole sequence, however large."""
+    long_window("cpu", 16)
+
+
+@pytest.mark.gpu
+def test_kernel_window_beyond_32_bits():
+    long_window("cuda", 128)
