@@ -67,7 +67,7 @@ class GPTConfig:
     @property
     def qkv_dim(self) -> int:
         """Output features of the attention's input projection."""
-        return self.d_model + 2 * (self.kv_heads or self.n_heads) * (self.d_model // self.n_heads)
+        return self.d_model + 2 * self.kv_heads * (self.d_model // self.n_heads) if self.kv_heads else 3 * self.d_model
 
     @property
     def vocab_padded(self) -> int:

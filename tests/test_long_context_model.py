@@ -270,3 +270,15 @@ def test_teacher_and_decoder_hold_nothing_and_disturb_nothing(change):
         dx, _ = block.backward(st(dh), st(dm))
         grads.append([dx.shards[(0, 0)]] + [g.shards[(0, 0)].clone() for _, _, g, _ in model.parameters()])
     assert all(torch.equal(a, b) for a, b in zip(*grads))
+
+
+def test_counts_without_shared_heads_are_those_of_three_widths():
+    """The input projection of a model whose heads each have a key and a value is three widths wide, whether or not the heads divide it
+    (counts are asked of sizes that no device has run yet)."""
+    for d, heads in ((128, 8), (100, 8), (1000, 3), (12, 24)):
+        cfg = GPTConfig(n_layers=2, d_model=d, n_heads=heads, ffn=4 * d, vocab=500, seq=64, vocab_pad=256)
+        per_layer = 3 * d * d + d * d + 2 * d * 4 * d + 4 * d
+        assert cfg.n_params() == 2 * per_layer + (512 + 64) * d + d * 512 + 2 * d
+        assert cfg.flops_per_token() == 3.0 * (2 * (3 * d * d + d * d + 8 * d * d) * 2 + 2 * d * 512 + 4 * 64 * d * 2 * 0.5)
+    assert GPTConfig(n_layers=1, d_model=128, n_heads=8, kv_heads=8).qkv_dim == 384
+    assert GPTConfig(n_layers=1, d_model=128, n_heads=8, kv_heads=2).qkv_dim == 192
