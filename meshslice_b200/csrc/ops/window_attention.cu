@@ -732,7 +732,8 @@ window_rows_kernel(const __grid_constant__ RowsArgs a) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const int key = n * 8 + (lane & 3) * 2 + j;
-            const bool seen = key < a.sinks && q0 + q - key >= a.window;
+            // (a query beyond the end is zeros, whose score for an infinite key is NaN)
+            const bool seen = key < a.sinks && q0 + q - key >= a.window && q0 + q < a.seq;
             e[j] = seen ? fast_exp2(fmaf(s[n][i * 2 + j], sl2, lse2)) : 0.f;
             d[j] = seen ? e[j] * fmaf(dp[n][i * 2 + j], a.scale, delta) : 0.f;
           }
@@ -1220,8 +1221,9 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
         // key-major: lse2 / delta of this thread's columns
         const float* my_lse = sLse + st0 * kBlk + part * kBwdCols + (lane & 3) * 2;
         const float* my_dlt = sDelta + (g & 1) * kBlk + part * kBwdCols + (lane & 3) * 2;
-        // only pairs on the diagonal or the window's edge, and far ones with first tokens among the keys, pay for the mask
-        const bool masked = kKeyMajor ? c0 < me0 + 24 || (c0 + kBwdCols - 1 - me0 >= a.window && me0 + 24 >= a.key_sinks)
+        // only pairs on the diagonal or the window's edge, far ones with first tokens among the keys, and (key-major) those with queries
+        // beyond the end, zeros whose score for an infinite key is NaN, pay for the mask
+        const bool masked = kKeyMajor ? c0 < me0 + 24 || (c0 + kBwdCols - 1 - me0 >= a.window && me0 + 24 >= a.key_sinks) || c0 + kBwdCols > a.seq
                                       : c0 + kBwdCols - 1 > me || (me - c0 >= a.window && c0 + kBwdCols > a.sinks);
         // of a thin block only the first columns are there
         const bool mine = !kThinItems || it > 0 || part == 0 || !(w.flags & kThin);
@@ -1263,6 +1265,10 @@ __device__ __forceinline__ bool window_bwd_run(const CUtensorMap& tm_qkv, const 
             const uint32_t from = ~low_bits(below(-base)), upto = low_bits(below(a.window - base));
 #pragma unroll
             for (int r = 0; r < 4; ++r) seen[r] = me0 + r * 8 < a.key_sinks ? from : from & upto;
+            if (c0 + kBwdCols > a.seq) {
+#pragma unroll
+              for (int r = 0; r < 4; ++r) seen[r] &= low_bits(below(a.seq - c0 - (lane & 3) * 2 - r * 8));
+            }
           }
           if (masked && !kKeyMajor)
             seen[0] = low_bits(me - c0 + 1) & (~low_bits(me - c0 + 1 - a.window) | low_bits(a.sinks - c0));

@@ -291,3 +291,52 @@ def test_window_beyond_32_bits():
 @pytest.mark.gpu
 def test_kernel_window_beyond_32_bits():
     long_window("cuda", 128)
+
+
+def check_gradient(shape, qkv, dout, dqkv, wg):
+    batch, seq, kv, group, window, sinks = shape
+    part = lambda t: t.double().view(batch, seq, kv, group + 2, 128).split([group, 1, 1], 3)
+    got, ref = part(dqkv), part(wg)
+    assert rel(got[2], ref[2]) < GRAD
+    for a, b, e in zip(got[:2], ref[:2], propagated(qkv, dout, *shape)):
+        assert (a - b).norm() < 1.5 * U * (e + b.square().sum()).sqrt()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 700, 1, 2, 200, 4), (2, 500, 2, 1, 0, 0), (1, 900, 1, 2, 130, 20)])
+def test_kernel_gradient_of_large_scores(shape):
+    """Scores of several hundred: most probabilities are 0 or 1.  A score is off by some 2^-22 of the sum of its terms' sizes, of about a
+    thousand: 2^-12 of a probability, beside 2^-9.3 for its rounding."""
+    batch, seq, kv, group, window, sinks = shape
+    qkv, dout = (t.cuda() for t in inputs(batch, seq, kv, group))
+    qkv = (qkv.float() * 12).bfloat16()
+    for _ in range(2):
+        out, lse = F.window_attention_fwd(qkv, *shape)
+        _, _, wg = definition(qkv, dout, *shape)
+        check_gradient(shape, qkv, dout, F.window_attention_bwd(dout, qkv, out, lse, *shape), wg)
+        x = qkv.view(batch * seq, kv, group + 2, 128)           # then every query against its own key: the diagonal is the lowest score
+        x[:, :, :group] = -x[:, :, group:group + 1]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("sinks,dead", [(4, range(1, 301)), (40, range(1, 39)), (40, range(1, 301)), (1, range(300, 420))])
+def test_kernel_gradient_of_keys_of_minus_infinity(sinks, dead):
+    """Keys whose score is -inf for every query get no gradient and disturb nobody else's; only the queries' feature that meets the
+    infinity is NaN, by the definition too."""
+    shape = (1, 700, 1, 2, 200, sinks)
+    qkv, dout = (t.cuda() for t in inputs(1, 700, 1, 2))
+    x = qkv.view(700, 4, 128)
+    x[:, :2, 0] = 1.0
+    x[list(dead), 2, 0] = -math.inf
+    out, lse = F.window_attention_fwd(qkv, *shape)
+    g = F.window_attention_bwd(dout, qkv, out, lse, *shape).double().view(700, 4, 128)
+    want = definition(qkv, dout, *shape)[2].view(700, 4, 128)
+    assert g[:, 2:].isfinite().all() and want[:, 2:].isfinite().all() and g[:, :2, 1:].isfinite().all()
+    assert (g[list(dead), 2:].abs() < 2.0 ** -100).all()
+    # (the errors that go into dQ and dK, with the dead keys' infinity out of the sums: they have no probability)
+    y = qkv.clone()
+    y.view(700, 4, 128)[list(dead), 2, 0] = -20000.0
+    assert rel(g[:, 3], want[:, 3]) < GRAD
+    dq, dk = propagated(y, dout, *shape)
+    for a, b, e in ((g[:, :2, 1:], want[:, :2, 1:], dq), (g[:, 2], want[:, 2], dk)):
+        assert (a - b).norm() < 1.5 * U * (e + b.square().sum()).sqrt()
