@@ -7,9 +7,10 @@ namespace msb {
 
 // Per row, with z the student's logits, p = softmax(t / T) over the entries the teacher kept (id in [0, vocab), the others are no
 // entries) and y the label (outside [0, vocab): no label):
-//   loss = w (log sum exp z - z_y) + (1 - w) T^2 KL(p || softmax(z / T))
+//   loss = w (log sum exp z - z_y) + (1 - w) T^2 sum_k p_k (log p_k - log softmax(z / T) at id_k)
 //   grad = scale ( w (softmax z - onehot y) + (1 - w) T (softmax(z / T) - p) )
-// A term without a label or without entries is zero.  Ids that occur more than once count with all their entries.
+// A term without a label or without entries is zero.  The second term of the loss is a Kullback-Leibler divergence where every id occurs once;
+// entries that share an id count as an event each, which takes a constant of the teacher off the loss and leaves the gradient as it is.
 struct DistillArgs {
   const void* logits;          // bf16 [rows, cols]: columns [col_offset, col_offset + cols) of the vocabulary, pitch ld
   void* grad;                  // bf16 [rows, cols], pitch ldg; may be the logits

@@ -3,8 +3,12 @@ formulation for CPU tensors.
 
 Per row, with z the student's logits over the vocabulary, p = softmax(t / T) over the teacher's entries, y the label:
 
-    loss = w (log sum exp z - z_y) + (1 - w) T^2 KL(p || softmax(z / T))
+    loss = w (log sum exp z - z_y) + (1 - w) T^2 sum_k p_k (log p_k - log softmax(z / T) at id_k)
     d loss / d z = w (softmax z - onehot y) + (1 - w) T (softmax(z / T) - p)
+
+The second term is KL(p || softmax(z / T)) where every id occurs once.  Entries that share an id count as an event each: beside one entry of
+their joint probability the loss is lower by (1 - w) T^2 times what they are uncertain among themselves, which depends on the teacher alone
+(so the loss may be negative); the gradient is the same.
 
 An id outside [0, vocab) is no entry (teachers that kept fewer than others), a target outside is no label; a term without entries or
 label is zero, in the loss and in the gradient.  T^2 keeps the gradient's size as T grows.

@@ -390,3 +390,34 @@ def test_kernel_on_another_stream_and_in_a_graph():
         assert torch.equal(loss, want[0]) and torch.equal(grad, want[1])
         assert torch.allclose(by_slices[0], loss, rtol=1e-4, atol=1e-4) and torch.allclose(by_slices[1].float(), grad.float(), rtol=2 ** -6, atol=2.5e-5)
         x.zero_()
+
+
+def shared_ids(dev):
+    """Entries of one id against one entry of their joint probability: the same gradient, and a loss that differs by what they are
+    uncertain among themselves, whatever the logits are."""
+    z, ids, values, targets = data(6, 203, 208, 4, seed=9)
+    for T, w in ((1.0, 0.0), (2.0, 0.5), (3.0, 0.3)):
+        twice = torch.cat([ids, ids[:, :1], ids[:, :2]], 1)
+        more = torch.cat([values, values[:, :1] + 0.5, values[:, :2] - 1.0], 1)
+        p = torch.softmax(more.double() / T, 1)
+        joint = p[:, :4].clone()
+        joint[:, 0] += p[:, 4] + p[:, 5]
+        joint[:, 1] += p[:, 6]
+        among = (joint * joint.log()).sum(1) - (p * p.log()).sum(1)
+        assert (among > 0).all() and among.max() > 0.1
+        for x in (z, (z.float() * 0.3 + 1.0).bfloat16()):
+            a = [t.to(dev) for t in (x, twice, more, targets, ids, (T * joint.log()).float())]
+            loss, grad = F.distill_loss_grad(a[0], a[1], a[2], 203, 1.0, T, a[3], w)
+            one, same = F.distill_loss_grad(a[0], a[4], a[5], 203, 1.0, T, a[3], w)
+            assert ((one - loss).double().cpu() - (1 - w) * T * T * among).abs().max() < 1e-4
+            # (p of either is rounded to 24 bits, the gradient to bf16)
+            assert ((grad - same).float().abs() <= 2.0 ** -7 * same.float().abs() + 1e-5).all()
+
+
+def test_cpu_entries_that_share_an_id():
+    shared_ids("cpu")
+
+
+@pytest.mark.gpu
+def test_kernel_entries_that_share_an_id():
+    shared_ids("cuda")
