@@ -71,7 +71,7 @@ __device__ __forceinline__ uint4 cut(uint4 u, int v, int valid) {
 
 // Which exponentials a row needs: those of z / T, of z (one kind serves both where T = 1), both, or, where T = 2 or 4, those of z as the
 // squares of those of z / T, or the squares of these: the special-function unit gives 16 a cycle and SM, so that four of them an element
-// take 180 us for 4096 rows of 50257 (148 SMs), two 90 (temperature 3: 244 us, 2: 165).
+// take 180 us for 4096 rows of 50257 (148 SMs), two 90 (temperature 3: 244 us, 2: 162).
 enum Kind { kSoft = 1, kHard = 2, kTwo = 3, kSquare = 5, kFourth = 9 };
 constexpr int powers(int K) { return K == kSquare ? 2 : K == kFourth ? 4 : 1; }
 

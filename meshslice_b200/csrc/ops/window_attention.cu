@@ -599,7 +599,7 @@ window_delta_kernel(const uint4* out, const uint4* dout, float* delta, uint32_t 
 // dK^T += Q^T dS, whose B operands are the score fragments transposed.  A CTA takes a run of the tiles of one key head (of all query
 // heads that share it) and leaves its sums in `parts`; the key-major item of block 0 adds their sum before it rounds.  mma.sync: 32
 // instructions a tile of 8 or 12 KiB and 8 first tokens.
-// Bound by HBM: it reads O, dO and, of far queries, Q once.
+// It reads O, dO and, of far queries, Q once: 186 MB in 43 us with cold caches (4 x 2048, 32 heads, window 512), 55 % of DRAM where a copy reaches 85.
 constexpr int kRowsWarps = 4, kRowsStages = 2, kRowsTile = 16 * kD * 2;
 constexpr int kRowsSmem = kRowsWarps * kRowsStages * 3 * kRowsTile;
 constexpr int kRowsPart = 2 * kThinKeys * kD;      // floats of a CTA: dV, dK
@@ -799,9 +799,10 @@ window_parts_kernel(const float* parts, float* sums, int chunks) {
 // items dQ of 128 queries over their list of key blocks.  Roles, rings and tensor memory as in attn_bwd2_kernel.  P (for dV) and dS
 // are rounded to bf16 as operands; dS is formed from P in fp32.
 // What bounds it: a key-major pair takes 2650 cycles (2048 of products), an item about 5000 more in which its output leaves and the next
-// one's tiles arrive; over long runs the power cap (1.5 GHz), which gives back in clock about half of what a cycle saved brings.
-// 4 x 2048, 32 heads, window 512, 4 first tokens: 299 us (key-major 150, query-major 110, row sums and first tokens 37; first tokens in items of
-// their own kind 327); 2 x 5003, 16 heads on 4, window 1000, 16 first tokens: 271 (418).
+// one's tiles arrive (30 % of that pass at a window of 512); over long runs the power cap (1.5 GHz), which gives back in clock about half of
+// what a cycle saved brings.
+// 4 x 2048, 32 heads, window 512, 4 first tokens: 300 us (key-major 150, query-major 110, row sums and first tokens 37; first tokens in items of
+// their own kind 327); 2 x 5003, 16 heads on 4, window 1000, 16 first tokens: 270 (418).
 constexpr int kBwdPoly = 2;                 // key-major: exponentials of every eight that run on the FMA pipe
 constexpr int kBwdWarps = 16;               // element-wise warps
 constexpr int kBwdCols = kBlk * 4 / kBwdWarps;   // columns of a row per element-wise thread
