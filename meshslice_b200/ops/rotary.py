@@ -123,15 +123,16 @@ def rotary_qkv(qkv, rotary: Rotary, kv_heads: int, group: int = 1, seq: Optional
             n, width = qkv.shape
             turns, dev, x = rotary.turns, qkv.get_device(), qkv.data_ptr()
             if positions is None:
-                at, fine = 0, seq is not None and seq > 0
+                at, fine, length = 0, seq is not None and seq > 0, seq
             else:
-                at, fine = positions.data_ptr(), (positions.dtype is torch.int64 and positions.dim() == 1 and positions.shape[0] == n
-                                                  and positions.is_contiguous() and positions.get_device() == dev)
+                at, length = positions.data_ptr(), 1
+                fine = (positions.dtype is torch.int64 and positions.dim() == 1 and positions.shape[0] == n
+                        and positions.is_contiguous() and positions.get_device() == dev)
             D, rot, half = rotary._kernel
             if fine and n and x & 15 == 0 and width == kv_heads * (group + 2) * D and turns.get_device() == dev:
                 stream = _native.stream_on(dev)
                 y = torch.empty_like(qkv)
-                _native.load().rotary(x, y.data_ptr(), width, width, at, turns.data_ptr(), n, seq or 1, kv_heads, group, D, rot, half,
+                _native.load().rotary(x, y.data_ptr(), width, width, at, turns.data_ptr(), n, length, kv_heads, group, D, rot, half,
                                       -1.0 if inverse else 1.0, c.cos_factor, stream)
                 return y
         _check(qkv, rotary, kv_heads, group, seq, positions, out)
@@ -151,7 +152,7 @@ def rotary_qkv(qkv, rotary: Rotary, kv_heads: int, group: int = 1, seq: Optional
         if qkv.shape[0]:
             _native.load().rotary(x.data_ptr(), y.data_ptr(), rows.pitch(x), rows.pitch(y),
                                   0 if positions is None else positions.data_ptr(), rotary.turns.data_ptr(), qkv.shape[0],
-                                  1 if seq is None else seq, kv_heads, group, *rotary._kernel,
+                                  seq if positions is None else 1, kv_heads, group, *rotary._kernel,
                                   -1.0 if inverse else 1.0, c.cos_factor, _native.stream_ptr())
         if out is not None and y is not out:
             out.copy_(y)

@@ -179,3 +179,23 @@ def test_kernel_on_another_stream_and_refusals():
         F.rotary_qkv(x, Rotary(RotaryConfig()), 2, seq=50)
     with pytest.raises(ValueError):
         F.rotary_qkv(x, r, 2, positions=torch.arange(50))
+
+
+def length_beside_positions(dev):
+    """With positions given the length of a sequence is not looked at, whatever it is and wherever the result goes."""
+    x, pos = rows(5, 1, 2, 128).to(dev), torch.tensor([3, 0, 9, 70000, 2], device=dev)
+    rot = Rotary(RotaryConfig(head_dim=128), device=dev)
+    want = F.rotary_qkv(x, rot, 1, 2, positions=pos)
+    for seq in (None, 0, -3, 7, 1 << 40):
+        assert torch.equal(F.rotary_qkv(x, rot, 1, 2, seq=seq, positions=pos), want)
+        y = x.clone()
+        assert torch.equal(F.rotary_qkv(y, rot, 1, 2, seq=seq, positions=pos, out=y), want)
+
+
+def test_length_beside_positions():
+    length_beside_positions("cpu")
+
+
+@pytest.mark.gpu
+def test_kernel_length_beside_positions():
+    length_beside_positions("cuda")
