@@ -22,11 +22,15 @@ OBJ = PKG / "csrc" / "build"
 CU_SOURCES = [
     "gemm/sm100_gemm.cu",
     "gemm/sm100_gemm2.cu",
+    "gemm/sm100_products.cu",
     "ops/ops.cu",
     "ops/attention.cu",
     "ops/attention_noalloc.cu",
     "ops/rotary.cu",
     "ops/distill.cu",
+    "ops/gated.cu",
+    "ops/head.cu",
+    "ops/orthogonal.cu",
     "ops/window_attention.cu",
     "ops/window_decode.cu",
     "comm/p2p.cu",

@@ -17,8 +17,12 @@
 
 #include "comm/p2p.h"
 #include "gemm/sm100_gemm.h"
+#include "gemm/sm100_products.h"
 #include "ops/attention.h"
 #include "ops/distill.h"
+#include "ops/gated.h"
+#include "ops/head.h"
+#include "ops/orthogonal.h"
 #include "ops/ops.h"
 #include "ops/rotary.h"
 #include "ops/window_attention.h"
@@ -385,6 +389,191 @@ void gemm_pair(const std::array<int64_t, 30>& v) {
 }
 
 // ---------------------------------------------------------------------------------------
+// products with an epilogue of their own
+// ---------------------------------------------------------------------------------------
+void products_ok(int r, const char* what) {
+  if (r != 0) throw std::runtime_error(std::string(what) + ": tensor map failed, code " + std::to_string(r));
+}
+void order_of(Product& p, int64_t K, int tile_n) {
+  const Gemm2Order o = gemm2_order(p.M, p.N, K, tile_n);
+  p.group = o.group;
+  p.along_n = o.along_n;
+}
+void run_products(ProductArgs& a, int k0, int k1, int problems, int tile_n, int sms, uint64_t status, uint64_t stream, const char* what) {
+  a.status = P<uint32_t>(status);
+  a.timeout_ns = kLocalTimeoutNs;
+  check(launch_sm100_products(a, k0, k1, problems, tile_n, sms, S(stream)), what);
+}
+// Columns of a tile for a product of this kind: a tile of 128 counts three quarters of one of 256 (gemm2_tile_n).
+int64_t products_waves(int kind, int64_t M, int64_t N, int64_t items, int tile_n, int sms) {
+  Product p;
+  std::memset(static_cast<void*>(&p), 0, sizeof(p));
+  p.M = (int)M;
+  p.N = (int)N;
+  p.items = (int)items;
+  const int64_t pairs = sms > 1 ? sms / 2 : 1;
+  return (product_tiles(p, kind, tile_n) + pairs - 1) / pairs;
+}
+int products_tile_n(int kind, int64_t M, int64_t N, int64_t items, int sms) {
+  return 3 * products_waves(kind, M, N, items, 128, sms) < 4 * products_waves(kind, M, N, items, 256, sms) ? 128 : 256;
+}
+
+// tokens, width, ffn, x, ldx, gate, ld, up, ld, mn_major, h, g, u, exps, act, keep, sms, status, stream
+void gated_fwd(const std::array<int64_t, 19>& v) {
+  static thread_local ProductArgs a;
+  Product& p = a.p[0];
+  p.M = (int)v[0];
+  p.N = (int)v[2];
+  p.items = 1;
+  p.a_item = p.b_item = 0;
+  const int tile_n = products_tile_n(kGated, v[0], v[2], 1, (int)v[16]);
+  const ProductOperand x{P<void>(v[3]), v[4], 0, 0}, w[2] = {{P<void>(v[5]), v[6], (int)v[9], 0}, {P<void>(v[7]), v[8], (int)v[9], 0}};
+  products_ok(product_operands(&p, kGated, tile_n, &x, w, 1, v[0], v[2], &v[1]), "gated_fwd");
+  p.act = (int)v[14];
+  p.keep = (int)v[15];
+  products_ok(product_output(&p, 0, P<void>(v[10]), v[2], v[0], v[2], false), "gated_fwd");
+  if (p.keep) {
+    products_ok(product_output(&p, 1, P<void>(v[11]), v[2], v[0], v[2], false), "gated_fwd");
+    products_ok(product_output(&p, 2, P<void>(v[12]), v[2], v[0], v[2], false), "gated_fwd");
+  }
+  p.exps = P<uint16_t>(v[13]);
+  order_of(p, v[1], tile_n);
+  run_products(a, kGated, kNone, 1, tile_n, (int)v[16], (uint64_t)v[17], (uint64_t)v[18], "gated_fwd");
+}
+// tokens, ffn, outputs, dy, ld, down, ld, mn_major, g, u, exps, dg, du, act, sms, status, stream
+void gated_grad(const std::array<int64_t, 17>& v) {
+  static thread_local ProductArgs a;
+  Product& p = a.p[0];
+  p.M = (int)v[0];
+  p.N = (int)v[1];
+  p.items = 1;
+  p.a_item = p.b_item = 0;
+  const int tile_n = products_tile_n(kGatedGrad, v[0], v[1], 1, (int)v[14]);
+  const ProductOperand dy{P<void>(v[3]), v[4], 0, 0}, w{P<void>(v[5]), v[6], (int)v[7], 0};
+  products_ok(product_operands(&p, kGatedGrad, tile_n, &dy, &w, 1, v[0], v[1], &v[2]), "gated_grad");
+  p.g = P<void>(v[8]);
+  p.u = P<void>(v[9]);
+  p.exps = P<uint16_t>(v[10]);
+  p.act = (int)v[13];
+  for (int i = 0; i < 2; ++i) products_ok(product_output(&p, i, P<void>(v[11 + i]), v[1], v[0], v[1], false), "gated_grad");
+  order_of(p, v[2], tile_n);
+  run_products(a, kGatedGrad, kNone, 1, tile_n, (int)v[14], (uint64_t)v[15], (uint64_t)v[16], "gated_grad");
+}
+// C = A0 B0 + A1 B1: M, N, K0, K1, A0, ld, A1, ld, a_mn_major, B0, ld, B1, ld, b_mn_major, C, ld, sms, status, stream
+void gemm_sum(const std::array<int64_t, 19>& v) {
+  static thread_local ProductArgs a;
+  Product& p = a.p[0];
+  p.M = (int)v[0];
+  p.N = (int)v[1];
+  p.items = 1;
+  p.a_item = p.b_item = 0;
+  const int tile_n = products_tile_n(kPlain, v[0], v[1], 1, (int)v[16]);
+  const ProductOperand x[2] = {{P<void>(v[4]), v[5], (int)v[8], 0}, {P<void>(v[6]), v[7], (int)v[8], 0}};
+  const ProductOperand w[2] = {{P<void>(v[9]), v[10], (int)v[13], 0}, {P<void>(v[11]), v[12], (int)v[13], 0}};
+  products_ok(product_operands(&p, kPlain, tile_n, x, w, 2, v[0], v[1], &v[2]), "gemm_sum");
+  products_ok(product_output(&p, 0, P<void>(v[14]), v[1], v[0], v[15], false), "gemm_sum");
+  order_of(p, v[2] + v[3], tile_n);
+  run_products(a, kPlain, kNone, 1, tile_n, (int)v[16], (uint64_t)v[17], (uint64_t)v[18], "gemm_sum");
+}
+// rows, width, vocab, columns, x, ldx, w, ldw, mn_major, e (0: losses alone), lde, stats, label, targets, tile_n, sms, status, stream
+void head_partial(const std::array<int64_t, 18>& v) {
+  static thread_local ProductArgs a;
+  Product& p = a.p[0];
+  p.M = (int)v[0];
+  p.N = (int)v[3];
+  p.items = 1;
+  p.a_item = p.b_item = 0;
+  const int tile_n = (int)v[14];
+  const ProductOperand x{P<void>(v[4]), v[5], 0, 0}, w{P<void>(v[6]), v[7], (int)v[8], 0};
+  products_ok(product_operands(&p, kHead, tile_n, &x, &w, 1, v[0], v[2], &v[1]), "head_partial");
+  p.write = v[9] != 0;
+  if (p.write) products_ok(product_output(&p, 0, P<void>(v[9]), v[3], v[0], v[10], false), "head_partial");
+  p.stats = P<float2>(v[11]);
+  p.label = P<float>(v[12]);
+  p.targets = P<int64_t>(v[13]);
+  p.vocab = (int)v[2];
+  order_of(p, v[1], tile_n);
+  run_products(a, kHead, kNone, 1, tile_n, (int)v[15], (uint64_t)v[16], (uint64_t)v[17], "head_partial");
+}
+void py_head_rows(uint64_t e, int64_t ld, uint64_t stats, uint64_t label, uint64_t targets, int rows, int cols, int tiles, int tile_n, int vocab,
+                  float scale, uint64_t loss, uint64_t stream) {
+  check(head_rows({P<void>(e), ld, P<float2>(stats), P<float>(label), P<int64_t>(targets), rows, cols, tiles, tile_n, vocab, scale,
+                   P<float>(loss)}, S(stream)), "head_rows");
+}
+// The unit matrix and its fp16 copy: g, bf16, stride, items, rows, cols, transpose, partial, x, xs, mp, np, scale, stream
+void unit_load(uint64_t g, int bf16, int64_t stride, int items, int rows, int cols, int transpose, uint64_t partial, uint64_t x, uint64_t xs,
+               int mp, int np, float scale, uint64_t stream) {
+  const int64_t n = (int64_t)rows * cols;
+  check(square_sums(P<void>(g), bf16, items, n, stride, P<double>(partial), S(stream)), "square_sums");
+  check(load_unit({P<void>(g), bf16, stride, items, rows, cols, transpose, P<double>(partial), norm_parts(n), P<float>(x), P<void>(xs), mp, np,
+                   scale}, S(stream)), "load_unit");
+}
+void py_gated_act(uint64_t g, uint64_t u, uint64_t h, int64_t n, int act, uint64_t stream) {
+  check(gated_act(P<void>(g), P<void>(u), P<void>(h), n, act, S(stream)), "gated_act");
+}
+void py_gated_act_bwd(uint64_t dh, uint64_t g, uint64_t u, uint64_t dg, uint64_t du, int64_t n, int act, uint64_t stream) {
+  check(gated_act_bwd(P<void>(dh), P<void>(g), P<void>(u), P<void>(dg), P<void>(du), n, act, S(stream)), "gated_act_bwd");
+}
+void py_momentum_step(uint64_t grad, int grad_fp32, uint64_t m, uint64_t u, int64_t items, int64_t n, int64_t stride, float momentum,
+                      int nesterov, uint64_t grad_scale, uint64_t stream) {
+  check(momentum_step(P<void>(grad), grad_fp32, P<float>(m), P<float>(u), items, n, stride, momentum, nesterov, P<float>(grad_scale), S(stream)),
+        "momentum_step");
+}
+void py_apply_update(uint64_t o, uint64_t master, uint64_t param, int64_t items, int64_t n, int64_t stride, float lr, float size, float wd,
+                     uint64_t stream) {
+  check(apply_update(P<float>(o), P<float>(master), P<void>(param), items, n, stride, lr, size, wd, S(stream)), "apply_update");
+}
+// alpha A A^T + beta C of a batch: items, m, k, a, out, c, alpha, beta, sms, status, stream
+void gram(int items, int m, int k, uint64_t src, uint64_t out, uint64_t c, float alpha, float beta, int sms, uint64_t status, uint64_t stream) {
+  static thread_local ProductArgs a;
+  Product& p = a.p[0];
+  p.M = p.N = m;
+  p.items = items;
+  p.a_item = p.b_item = m;
+  const int tile_n = products_tile_n(kGram, m, m, items, sms);
+  const ProductOperand o{P<void>(src), k, 0, 0};
+  const int64_t K = k, rows = (int64_t)items * m;
+  products_ok(product_operands(&p, kGram, tile_n, &o, &o, 1, rows, rows, &K), "gram");
+  products_ok(product_output(&p, 0, P<void>(out), m, rows, m, false), "gram");
+  p.out = P<void>(out);
+  p.c = P<void>(c);
+  p.alpha = alpha;
+  p.beta = beta;
+  run_products(a, kGram, kNone, 1, tile_n, sms, status, stream, "gram");
+}
+// alpha X + beta B X of a batch: items, m, n, b, xs, x, xs_out, scale, alpha, beta, out (0: x and xs_out), rows, cols, item, row and column
+// strides of out, out_fp32, sms, status, stream
+void ortho_step(int items, int m, int n, uint64_t b, uint64_t xs, uint64_t x, uint64_t xs_out, float scale, float alpha, float beta,
+                uint64_t out, int rows, int cols, int64_t s_item, int64_t s_row, int64_t s_col, int out_fp32, int sms, uint64_t status,
+                uint64_t stream) {
+  static thread_local ProductArgs a;
+  Product& p = a.p[0];
+  p.M = m;
+  p.N = n;
+  p.items = items;
+  p.a_item = p.b_item = m;
+  const int tile_n = products_tile_n(kStep, m, n, items, sms);
+  const int64_t rows_all = (int64_t)items * m, K = m;
+  const ProductOperand B{P<void>(b), m, 0, 0}, X{P<void>(xs), n, 1, rows_all};
+  products_ok(product_operands(&p, kStep, tile_n, &B, &X, 1, rows_all, n, &K), "ortho_step");
+  products_ok(product_output(&p, 0, P<void>(x), n, rows_all, n, true), "ortho_step");
+  if (out == 0) products_ok(product_output(&p, 1, P<void>(xs_out), n, rows_all, n, false), "ortho_step");
+  p.out = P<void>(out);
+  p.c = P<void>(x);
+  p.scale = scale;
+  p.alpha = alpha;
+  p.beta = beta;
+  p.rows = rows;
+  p.cols = cols;
+  p.out_item = s_item;
+  p.out_row = s_row;
+  p.out_col = s_col;
+  p.out_fp32 = out_fp32;
+  order_of(p, m, tile_n);
+  run_products(a, kStep, kNone, 1, tile_n, sms, status, stream, "ortho_step");
+}
+
+// ---------------------------------------------------------------------------------------
 // runtime: IPC-shared device memory, host-mapped status words
 // ---------------------------------------------------------------------------------------
 py::tuple symm_alloc(size_t bytes) {
@@ -586,6 +775,11 @@ PYBIND11_MODULE(_C, m) {
   m.attr("PUSH_JOB_BYTES") = (int)sizeof(PushJob);
   m.attr("CHUNK_DESC_BYTES") = (int)sizeof(ChunkDesc);
 
+  m.attr("GATED_CHUNK") = (int)kGatedChunk;
+  m.attr("NORM_PARTS") = (int)kNormParts;
+  m.def("products_tile_n", &products_tile_n, "columns of a tile: kind, M, N, items, sms");
+  m.attr("PRODUCT_HEAD") = (int)kHead;
+
   m.def("gemm_run", &gemm_run, "persistent tcgen05 GEMM with optional fused gather / push");
   m.def("symm_alloc", &symm_alloc);
   m.def("symm_open", &symm_open);
@@ -700,6 +894,26 @@ PYBIND11_MODULE(_C, m) {
       {"gemm_pair", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&direct_values<&gemm_pair, 30>)), METH_FASTCALL,
        "two independent plain GEMMs in one launch: M, N, K, A, lda, a_mn_major, B, ldb, b_mn_major, C, ldc, c_fp32, accumulate "
        "of either, sms, status, stream, gelu_pre"},
+#define MSB_VALUES(name, fn, n, doc) \
+  {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&direct_values<&fn, n>)), METH_FASTCALL, doc}
+      MSB_VALUES("gated_fwd", gated_fwd, 19, "tokens, width, ffn, x, ldx, gate, ld, up, ld, mn_major, h, g, u, exps, act, keep, sms, status, "
+                 "stream"),
+      MSB_VALUES("gated_grad", gated_grad, 17, "tokens, ffn, outputs, dy, ld, down, ld, mn_major, g, u, exps, dg, du, act, sms, status, "
+                 "stream"),
+      MSB_VALUES("gemm_sum", gemm_sum, 19, "two products summed: M, N, K0, K1, A0, ld, A1, ld, a_mn_major, B0, ld, B1, ld, b_mn_major, C, ld, "
+                 "sms, status, stream"),
+      MSB_VALUES("head_partial", head_partial, 18, "rows, width, vocab, columns, x, ldx, w, ldw, mn_major, e, lde, stats, label, targets, "
+                 "tile_n, sms, status, stream"),
+#undef MSB_VALUES
+      MSB_DIRECT("head_rows", py_head_rows, "e, ld, stats, label, targets, rows, cols, tiles, tile_n, vocab, scale, loss, stream"),
+      MSB_DIRECT("unit_load", unit_load, "g, bf16, stride, items, rows, cols, transpose, partial, x, xs, mp, np, scale, stream"),
+      MSB_DIRECT("gated_act", py_gated_act, "g, u, h, n, act, stream"),
+      MSB_DIRECT("gated_act_bwd", py_gated_act_bwd, "dh, g, u, dg, du, n, act, stream"),
+      MSB_DIRECT("momentum_step", py_momentum_step, "grad, grad_fp32, m, u, items, n, stride, momentum, nesterov, grad_scale, stream"),
+      MSB_DIRECT("apply_update", py_apply_update, "o, master, param, items, n, stride, lr, size, wd, stream"),
+      MSB_DIRECT("gram", gram, "items, m, k, a, out, c, alpha, beta, sms, status, stream"),
+      MSB_DIRECT("ortho_step", ortho_step, "items, m, n, b, xs, x, xs_out, scale, alpha, beta, out, rows, cols, item, row and column strides "
+                 "of out, out_fp32, sms, status, stream"),
       MSB_DIRECT("memset_zero", memset_zero, "ptr, bytes, stream"),
       MSB_DIRECT("ln_fwd_local", ln_fwd_local, "x, res, h_out, y, gamma, beta, mean_rstd, rows, cols, eps, stream"),
       MSB_DIRECT("ln_bwd_local", ln_bwd_local, "dy, h, gamma, mean_rstd, dres, dx, dgamma, dbeta, rows, cols, stream"),

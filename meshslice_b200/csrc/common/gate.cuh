@@ -1,0 +1,22 @@
+// Activations of gated feed-forward blocks in fp32.  Both are x sigmoid(q(x)): q(x) = x (silu), 2 sqrt(2 / pi) (x + 0.044715 x^3) (tanh-GeLU, since
+// 1 + tanh(y) = 2 sigmoid(2 y)), with ex2.approx and a division of 2 units in the last place: some 2^-21 of the value, where tanh.approx
+// would leave 2^-11.
+#pragma once
+#include <cuda_runtime.h>
+
+namespace msb {
+
+// act 0: silu, 1: GeLU.  sigmoid(q(x))
+__device__ __forceinline__ float gate_sigmoid(float x, int act) {
+  const float q = act == 0 ? x : 1.5957691216057308f * (x + 0.044715f * x * x * x);
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.4426950408889634f * q));
+  return __fdividef(1.f, 1.f + e);
+}
+// The activation's derivative, with s = sigmoid(q(x)).
+__device__ __forceinline__ float gate_slope(float x, float s, int act) {
+  const float dq = act == 0 ? 1.f : 1.5957691216057308f * (1.f + 3.f * 0.044715f * x * x);
+  return s + x * s * (1.f - s) * dq;
+}
+
+}  // namespace msb

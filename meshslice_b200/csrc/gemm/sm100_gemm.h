@@ -248,6 +248,9 @@ int make_tensor_map_seq(CUtensorMap* map, const void* base, uint64_t cols, uint6
 // swizzle.  Returns non-zero where TMA cannot address it (base or pitch not a multiple of 16 bytes).
 int make_tensor_map_out(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, bool fp32);
 
+// The same for boxes of 32 rows x 32 columns, of 16 bits (64-byte swizzle) or fp32 (128-byte swizzle).
+int make_tensor_map_chunk(CUtensorMap* map, const void* base, int64_t cols, int64_t rows, int64_t ld, bool fp32);
+
 // Tensor map of an MN-major operand (stored [k_rows, mn_extent] row-major, mn_extent % 64 == 0) as
 // {64 elements, k_rows, mn_extent / 64 blocks}: one box of {64, kBK, blocks_per_box} fills the
 // shared-memory layout of `blocks_per_box` consecutive 64-wide blocks with ONE TMA instruction.

@@ -1,0 +1,199 @@
+"""Gated feed-forward block  y = (act(x Wg) * (x Wu)) Wd  with its gradients.  Native kernels for CUDA tensors, fp32 formulation for
+CPU tensors.
+
+act is 'silu' (x sigmoid(x)) or 'gelu' (tanh form).  Gate and up weights lie as [inputs, features] (layout 'nn') or [features, inputs]
+('nt'), the down weight as [features, outputs] ('nn') or [outputs, features] ('nt').
+
+    dh = dy Wd^T     du = dh act(g)     dg = dh u act'(g)        g = x Wg, u = x Wu, h = act(g) u
+    dWd = h^T dy     dWg = x^T dg       dWu = x^T du             dx = dg Wg^T + du Wu^T
+
+On a GPU both projections, the activation and the product are one kernel; what it keeps of g and u for the gradient has 11 significant
+bits, in a range that 32 features of a token share.  h, dg and du are rounded to bf16, as inputs of products are.
+"""
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+from typing import Optional, Sequence, Tuple
+
+import torch
+
+from .. import _native
+from . import rows
+from .gemm import gemm, gemm_pair, sm_count
+
+ACTS = {"silu": 0, "gelu": 1}
+_LAYOUTS = ("nn", "nt")
+
+
+@dataclass
+class GatedSaved:
+    """What a forward pass keeps for the backward one: h, and gate and up (on a GPU fp16 with an exponent for 32 features)."""
+    h: torch.Tensor
+    gate: torch.Tensor
+    up: torch.Tensor
+    exponents: Optional[torch.Tensor] = None
+
+
+def _sizes(x, w_gate, w_up, w_down, act: str, up_layout: str, down_layout: str) -> Tuple[int, int, int, int]:
+    """(tokens, inputs, features, outputs) after all checks that do not depend on the direction."""
+    if act not in ACTS:
+        raise ValueError(f"unknown activation {act!r}: one of {sorted(ACTS)}")
+    if up_layout not in _LAYOUTS or down_layout not in _LAYOUTS:
+        raise ValueError(f"weights lie as 'nn' or 'nt' (got {up_layout!r}, {down_layout!r})")
+    if any(t.dim() != 2 for t in (x, w_gate, w_up, w_down)):
+        raise ValueError("x and the weights are matrices")
+    n, d = x.shape
+    i, f = w_gate.shape if up_layout == "nn" else w_gate.shape[::-1]
+    j, o = w_down.shape if down_layout == "nn" else w_down.shape[::-1]
+    if w_up.shape != w_gate.shape or i != d or j != f:
+        raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, gate {tuple(w_gate.shape)}, up {tuple(w_up.shape)} ({up_layout}), "
+                         f"down {tuple(w_down.shape)} ({down_layout})")
+    if min(d, f, o) < 1:
+        raise ValueError(f"inputs, features and outputs must not be empty (got {d}, {f}, {o})")
+    for t in (w_gate, w_up, w_down):
+        if t.device != x.device or t.dtype != x.dtype:
+            raise ValueError(f"x is {x.dtype} on {x.device}, a weight {t.dtype} on {t.device}")
+    if x.is_cuda:
+        if x.dtype != torch.bfloat16:
+            raise ValueError(f"the gated kernels need bf16 (got {x.dtype})")
+        if d % 8 or f % 8 or o % 8:
+            raise ValueError(f"the gated kernels need multiples of 8 features (got {d}, {f}, {o})")
+        if n >= 1 << 31:
+            raise ValueError(f"the gated kernels take fewer than 2^31 tokens (got {n})")
+        _native.check_device(x)
+    return n, d, f, o
+
+
+def gated_ff_fwd(x, w_gate, w_up, w_down, act: str = "silu", up_layout: str = "nn", down_layout: str = "nn", keep: bool = True):
+    """(y [tokens, outputs], what ``gated_ff_bwd`` needs, None without ``keep``)."""
+    n, d, f, o = _sizes(x, w_gate, w_up, w_down, act, up_layout, down_layout)
+    if not x.is_cuda:
+        xf = x.float()
+        g, u = (xf @ (w.float() if up_layout == "nn" else w.float().T) for w in (w_gate, w_up))
+        h = _act(g, act)[0] * u
+        y = h @ (w_down.float() if down_layout == "nn" else w_down.float().T)
+        return y.to(x.dtype), GatedSaved(h, g, u) if keep else None
+    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=x.device)
+    h, y = new(x.dtype, n, f), new(x.dtype, n, o)
+    saved = GatedSaved(h, new(torch.float16, n, f), new(torch.float16, n, f), new(torch.int16, n, -(-f // _native.load().GATED_CHUNK))) if keep else None
+    if n == 0:
+        return y, saved
+    xa, wg, wu, wd = (rows.as_aligned(t) for t in (x, w_gate, w_up, w_down))
+    p = lambda name: getattr(saved, name).data_ptr() if keep else 0
+    _native.load().gated_fwd(n, d, f, xa.data_ptr(), rows.pitch(xa), wg.data_ptr(), rows.pitch(wg), wu.data_ptr(), rows.pitch(wu),
+                             1 if up_layout == "nn" else 0, h.data_ptr(), p("gate"), p("up"), p("exponents"), ACTS[act], 1 if keep else 0,
+                             sm_count(x.device), _native.status().dev, _native.stream_ptr())
+    gemm(h, wd, down_layout, out=y)
+    return y, saved
+
+
+def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "silu", up_layout: str = "nn", down_layout: str = "nn",
+                 grads: Optional[Sequence[torch.Tensor]] = None):
+    """(dx, (gradients of gate, up and down weight)).  The weights' gradients are new tensors, or are added to ``grads`` (fp32 or the
+    weights' type, in the weights' layouts)."""
+    n, d, f, o = _sizes(x, w_gate, w_up, w_down, act, up_layout, down_layout)
+    if dy.shape != (n, o) or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError(f"dy must be {x.dtype} [{n}, {o}] on {x.device} (got {dy.dtype} {tuple(dy.shape)} on {dy.device})")
+    if saved is None or saved.h.shape != (n, f) or saved.h.device != x.device or (saved.exponents is not None) != x.is_cuda:
+        raise ValueError("the backward pass needs what the forward pass kept")
+    weights = (w_gate, w_up, w_down)
+    add = grads is not None
+    if add:
+        if len(grads) != 3:
+            raise ValueError("grads are those of gate, up and down weight")
+        for g, w in zip(grads, weights):
+            if g.shape != w.shape or g.device != w.device or g.dtype not in (torch.float32, w.dtype):
+                raise ValueError(f"a gradient must be fp32 or {w.dtype} {tuple(w.shape)} on {w.device} (got {g.dtype} {tuple(g.shape)} on {g.device})")
+            if x.is_cuda and not (rows.aligned(g) and rows.pitch(g) % 8 == 0):
+                raise ValueError("gradients that are added to need neighbouring columns and rows on 16-byte boundaries")
+    if not x.is_cuda:
+        g, u, xf, dyf = saved.gate, saved.up, x.float(), dy.float()
+        a, da = _act(g, act)
+        dh = dyf @ (w_down.float().T if down_layout == "nn" else w_down.float())
+        dg, du, h = dh * u * da, dh * a, saved.h
+        back = lambda t, w: t @ (w.float().T if up_layout == "nn" else w.float())
+        dx = (back(dg, w_gate) + back(du, w_up)).to(x.dtype)
+        new = [xf.T @ dg, xf.T @ du] if up_layout == "nn" else [dg.T @ xf, du.T @ xf]
+        new.append(h.T @ dyf if down_layout == "nn" else dyf.T @ h)
+        if not add:
+            return dx, tuple(t.to(x.dtype) for t in new)
+        for t, v in zip(grads, new):
+            t += v.to(t.dtype)
+        return dx, tuple(grads)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if not add:
+        grads = tuple(torch.empty(w.shape, dtype=w.dtype, device=w.device) for w in weights)
+    if n == 0:
+        if not add:
+            for t in grads:
+                t.zero_()
+        return dx, tuple(grads)
+    xa, dya, wg, wu, wd = (rows.as_aligned(t) for t in (x, dy, *weights))
+    dg, du = torch.empty_like(saved.h), torch.empty_like(saved.h)
+    C, sms, status, stream = _native.load(), sm_count(x.device), _native.status().dev, _native.stream_ptr()
+    C.gated_grad(n, f, o, dya.data_ptr(), rows.pitch(dya), wd.data_ptr(), rows.pitch(wd), 0 if down_layout == "nn" else 1,
+                 saved.gate.data_ptr(), saved.up.data_ptr(), saved.exponents.data_ptr(), dg.data_ptr(), du.data_ptr(), ACTS[act], sms, status,
+                 stream)
+    product = lambda a, b, first: (a, b, "tn") if first else (b, a, "tn")
+    gemm(*product(saved.h, dya, down_layout == "nn"), out=grads[2], accumulate=add)
+    a0, a1 = product(xa, dg, up_layout == "nn"), product(xa, du, up_layout == "nn")
+    gemm_pair(*a0, grads[0], add, *a1, grads[1], add)
+    C.gemm_sum(n, d, f, f, dg.data_ptr(), f, du.data_ptr(), f, 0, wg.data_ptr(), rows.pitch(wg), wu.data_ptr(), rows.pitch(wu),
+               0 if up_layout == "nn" else 1, dx.data_ptr(), d, sms, status, stream)
+    return dx, tuple(grads)
+
+
+def _same(act: str, *tensors):
+    first = tensors[0]
+    if act not in ACTS:
+        raise ValueError(f"unknown activation {act!r}: one of {sorted(ACTS)}")
+    for t in tensors[1:]:
+        if t.shape != first.shape or t.dtype != first.dtype or t.device != first.device:
+            raise ValueError(f"operands of one shape, type and device (got {first.dtype} {tuple(first.shape)} on {first.device}, "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device})")
+    if first.is_cuda:
+        if first.dtype != torch.bfloat16 or first.numel() % 8:
+            raise ValueError(f"the gated kernels need bf16 and a multiple of 8 elements (got {first.dtype} {tuple(first.shape)})")
+        _native.check_device(first)
+
+
+def _block(t):
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def gated_act(gate, up, act: str = "silu"):
+    """act(gate) * up of projections that are there already."""
+    _same(act, gate, up)
+    if not gate.is_cuda:
+        return (_act(gate.float(), act)[0] * up.float()).to(gate.dtype)
+    h = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    if gate.numel():
+        gate, up = _block(gate), _block(up)
+        _native.load().gated_act(gate.data_ptr(), up.data_ptr(), h.data_ptr(), h.numel(), ACTS[act], _native.stream_ptr())
+    return h
+
+
+def gated_act_bwd(dh, gate, up, act: str = "silu"):
+    """Gradients of ``gated_act`` for gate and up."""
+    _same(act, dh, gate, up)
+    if not dh.is_cuda:
+        a, da = _act(gate.float(), act)
+        return (dh.float() * up.float() * da).to(dh.dtype), (dh.float() * a).to(dh.dtype)
+    dg, du = (torch.empty(dh.shape, dtype=dh.dtype, device=dh.device) for _ in range(2))
+    if dh.numel():
+        dh, gate, up = _block(dh), _block(gate), _block(up)
+        _native.load().gated_act_bwd(dh.data_ptr(), gate.data_ptr(), up.data_ptr(), dg.data_ptr(), du.data_ptr(), dg.numel(), ACTS[act],
+                                     _native.stream_ptr())
+    return dg, du
+
+
+def _act(g, act: str):
+    """Activation and derivative in g's precision."""
+    if act == "silu":
+        s = torch.sigmoid(g)
+        return g * s, s * (1 + g * (1 - s))
+    c = math.sqrt(2 / math.pi)
+    t = torch.tanh(c * (g + 0.044715 * g ** 3))
+    return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * c * (1 + 3 * 0.044715 * g * g)
