@@ -33,6 +33,9 @@ def main():
     p.add_argument("--ksplit", type=int, nargs=4, default=[4, 4, 4, 4])
     p.add_argument("--alg", default="meshflow", choices=["meshflow", "collective"])
     p.add_argument("--tuned-json", default="", help="autotuner output: per-layer dataflow and slice count")
+    p.add_argument("--gated", default="", choices=["", "silu", "gelu"], help="gated feed-forward blocks with this activation")
+    p.add_argument("--head-rows", type=int, default=-1, help="loss without logits in memory: tokens at a time (0: chosen; one GPU)")
+    p.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"], help="muon: orthogonal updates of the blocks' matrices (one GPU)")
     p.add_argument("--log", default="")
     p.add_argument("--ckpt-dir", default="")
     p.add_argument("--ckpt-every", type=int, default=0)
@@ -62,11 +65,11 @@ def main():
             dataflows = tuple(l["dataflow"] for l in tuned["layers"])
             ksplits = tuple(int(l["ksplit"] or 1) for l in tuned["layers"])
     cfg = GPTConfig(n_layers=a.layers, d_model=a.d_model, n_heads=a.nheads, ffn=a.ffn, vocab=a.vocab, seq=a.seqlen,
-                    dataflows=dataflows, ksplits=ksplits)
+                    dataflows=dataflows, ksplits=ksplits, gated=a.gated, head_rows=None if a.head_rows < 0 else a.head_rows)
     rows_batch = a.batchsize // R
     mb = a.micro_batch or min(rows_batch, 4 * C)
     tr = Trainer(cfg, TrainConfig(global_batch=a.batchsize, micro_batch=mb, lr=a.lr,
-                                  backend="fused" if a.alg == "meshflow" else "collective"), mesh_shape=(R, C))
+                                  backend="fused" if a.alg == "meshflow" else "collective", optimizer=a.optimizer), mesh_shape=(R, C))
     log = RunLogger(a.log or None, rank)
     log.log("config", mesh=f"{R}x{C}", layers=a.layers, d_model=a.d_model, params=cfg.n_params(),
             global_batch=a.batchsize, micro_batch=mb, dataflows=str(dataflows), ksplits=str(ksplits))

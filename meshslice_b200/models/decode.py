@@ -44,7 +44,10 @@ class GPTDecoder:
             h, y = self._norm(b.ln1, x, delta)
             a = self._linear(b.out_proj, attend(i, self._linear(b.in_proj, y)))
             x, y = self._norm(b.ln2, a, h)
-            delta = self._linear(b.ff2, F.gelu(self._linear(b.ff1, y)))
+            if b.ff is not None:
+                delta = self._linear(b.ff, y)
+            else:
+                delta = self._linear(b.ff2, F.gelu(self._linear(b.ff1, y)))
         return x, delta
 
     def _logits(self, x, delta):

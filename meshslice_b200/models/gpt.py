@@ -23,7 +23,7 @@ from ..ops.rotary import RotaryConfig
 from ..parallel.mesh import Mesh, ShardedTensor
 from ..parallel.tensor_parallel import init_block
 from . import sharded_layers
-from .sharded_layers import GeLU, ShardedAttention, ShardedFFLayer, ShardedLayerNorm, ShardedWindowAttention, _add
+from .sharded_layers import GeLU, ShardedAttention, ShardedFFLayer, ShardedGatedFF, ShardedLayerNorm, ShardedWindowAttention, _add
 
 
 @dataclass
@@ -49,8 +49,17 @@ class GPTConfig:
     window: int = 0
     sinks: int = 0
     rotary: Optional[RotaryConfig] = None
+    # feed-forward block of gate and up projection ('silu' or 'gelu' of the gate) in place of the GeLU one; ``ffn`` features each
+    gated: str = ""
+    # the loss without the logits of a micro-batch in memory: this many tokens' at a time (0: chosen); whole matrices only (a 1 x 1 mesh)
+    head_rows: Optional[int] = None
 
     def __post_init__(self):
+        if self.gated and (self.gated not in F.GATED_ACTS or "rs" in self.dataflows[2:]):
+            raise ValueError(f"a gated feed-forward block has one of the activations {sorted(F.GATED_ACTS)} and 'os' and 'ls' layers "
+                             f"(got {self.gated!r}, {self.dataflows[2:]})")
+        if self.head_rows is not None and self.head_rows < 0:
+            raise ValueError(f"the tokens of the head at a time are not negative (got {self.head_rows})")
         if self.window < 0 or self.sinks < 0 or (self.kv_heads and self.n_heads % self.kv_heads):
             raise ValueError(f"window and sinks are not negative and query heads a multiple of key/value heads (got window {self.window}, "
                              f"sinks {self.sinks}, {self.n_heads} on {self.kv_heads})")
@@ -70,12 +79,17 @@ class GPTConfig:
         return self.d_model + 2 * self.kv_heads * (self.d_model // self.n_heads) if self.kv_heads else 3 * self.d_model
 
     @property
+    def ff_matrices(self) -> int:
+        """Matrices of d_model x ffn in a block."""
+        return 3 if self.gated else 2
+
+    @property
     def vocab_padded(self) -> int:
         return (self.vocab + self.vocab_pad - 1) // self.vocab_pad * self.vocab_pad
 
     def n_params(self) -> int:
         d = self.d_model
-        per_layer = d * self.qkv_dim + d * d + 2 * d * self.ffn + 4 * d
+        per_layer = d * self.qkv_dim + d * d + self.ff_matrices * d * self.ffn + 4 * d
         positions = 0 if self.rotary is not None else self.seq
         return self.n_layers * per_layer + (self.vocab_padded + positions) * d + d * self.vocab_padded + 2 * d
 
@@ -83,7 +97,7 @@ class GPTConfig:
         """Model FLOPs of one training step per token (forward + backward = 3x forward GEMMs,
         attention counted with its full S x S score matrix as the reference's block does; a window's with its pairs)."""
         d = self.d_model
-        gemm = 2 * (d * self.qkv_dim + d * d + 2 * d * self.ffn) * self.n_layers + 2 * d * self.vocab_padded
+        gemm = 2 * (d * self.qkv_dim + d * d + self.ff_matrices * d * self.ffn) * self.n_layers + 2 * d * self.vocab_padded
         attn = 4 * self.seq * d * self.n_layers * (0.5 if self.causal else 1.0)
         if self.window and self.window < self.seq:
             # (query, key) pairs of a window: the triangle of its first queries, whole windows, first tokens beyond them
@@ -95,7 +109,7 @@ class GPTConfig:
 
 
 class GPTBlock:
-    """Pre-LN decoder block: x + out_proj(attn(in_proj(LN1 x)));  h + ff2(gelu(ff1(LN2 h)))."""
+    """Pre-LN decoder block: x + out_proj(attn(in_proj(LN1 x)));  h + ff2(gelu(ff1(LN2 h))), or h + ff(LN2 h) with a gated block."""
 
     def __init__(self, mesh: Mesh, cfg: GPTConfig, idx: int, device, alloc_sharded, alloc_rep, grad_sharded,
                  grad_rep=None):
@@ -114,6 +128,10 @@ class GPTBlock:
         self.out_proj = ShardedFFLayer(mesh, cfg.algorithm, df[1], ks[1], d, d, seed=s + 2, **kw)
         self.ln2 = ShardedLayerNorm(mesh, d, affine=True, eps=cfg.eps, dtype=cfg.dtype, device=device, alloc=alloc_rep,
                                     grad_alloc=grad_rep)
+        if cfg.gated:
+            self.ff = ShardedGatedFF(mesh, cfg.algorithm, df[2:], ks[2:], d, cfg.ffn, cfg.gated, seeds=(s + 3, s + 5, s + 4), **kw)
+            return
+        self.ff = None
         self.ff1 = ShardedFFLayer(mesh, cfg.algorithm, df[2], ks[2], d, cfg.ffn, seed=s + 3, **kw)
         self.gelu = GeLU()
         self.ff2 = ShardedFFLayer(mesh, cfg.algorithm, df[3], ks[3], cfg.ffn, d, seed=s + 4, **kw)
@@ -144,6 +162,8 @@ class GPTBlock:
         x, y = self._norm(self.ln1, x, delta, keep)            # residual stream becomes x + delta
         a = self._lin(self.out_proj, self.attn.forward(self._lin(self.in_proj, y, keep), keep), keep)
         h, y = self._norm(self.ln2, a, x, keep)                # h = x + a
+        if self.ff is not None:
+            return h, self.ff.forward(y, keep)
         if self.ff1._fused and self.ff1.dataflow == "os" and sharded_layers.FUSE_GELU:
             g, pre = self.ff1.forward_gelu(y, keep)            # GeLU in the GEMM epilogue
             if keep:
@@ -156,18 +176,25 @@ class GPTBlock:
     def backward(self, dh: ShardedTensor, dm: ShardedTensor):
         """dh: gradient of the residual stream after this block, dm: gradient of the MLP output.
         Returns (dx, ddelta) for the block below."""
-        if self.ff2.dataflow != "rs":
+        if self.ff is not None:
+            d = self.ff.backward(dm)
+        elif self.ff2.dataflow != "rs":
             d = self.ff2.backward_gelu(dm, self.gelu)     # GeLU's derivative in the GEMM epilogue
+            d = self._lin_bwd(self.ff1, d)
         else:
             d = self.gelu.backward(self._lin_bwd(self.ff2, dm))
-        d = self._lin_bwd(self.ff1, d)
+            d = self._lin_bwd(self.ff1, d)
         dh2 = self.ln2.backward(d, dh)            # gradient of h = x + a
         d = self._lin_bwd(self.in_proj, self.attn.backward(self._lin_bwd(self.out_proj, dh2)))
         dx = self.ln1.backward(d, dh2)            # gradient of x + delta
         return dx, dx
 
     def layers(self):
-        return [self.ln1, self.in_proj, self.out_proj, self.ln2, self.ff1, self.ff2]
+        return [self.ln1, self.in_proj, self.out_proj, self.ln2, *(self.ff.layers() if self.ff is not None else (self.ff1, self.ff2))]
+
+    def matrices(self):
+        """The weights of the block's linear layers."""
+        return [l.weight for l in self.layers() if isinstance(l, ShardedFFLayer)]
 
 
 @dataclass
@@ -186,6 +213,8 @@ class GPTModel:
         self.mesh, self.cfg, self.device = mesh, cfg, device
         if cfg.d_model % mesh.C or cfg.vocab_padded % mesh.C or cfg.n_heads % mesh.C:
             raise ValueError("model width / heads / vocabulary must divide over the mesh columns")
+        if cfg.head_rows is not None and mesh.R * mesh.C != 1:
+            raise ValueError("a head without logits in memory has whole matrices: a 1 x 1 mesh")
         d, C = cfg.d_model, mesh.C
         a_rep = alloc_rep or (lambda shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
         g_rep = grad_rep or (lambda shape, dtype, dev: torch.empty(shape, dtype=dtype, device=dev))
@@ -239,14 +268,26 @@ class GPTModel:
     def forward(self, tokens: ShardedTensor, keep: bool = True) -> ShardedTensor:
         """Logits [local tokens, padded vocabulary / C] of whole sequences.  ``keep``: hold what the backward pass needs; without it
         the activations are free as soon as they are used, and those that an earlier forward pass holds stay as they are."""
+        return self.head.forward(self._features(tokens, keep), keep)     # [T/R, Vp/C]
+
+    def _features(self, tokens: ShardedTensor, keep: bool) -> ShardedTensor:
+        """What the head reads."""
         m, cfg = self.mesh, self.cfg
         pos = lambda k: None if self.pos is None else self.pos.shards[k]
         x = ShardedTensor(m, {k: F.embedding_fwd(tokens.shards[k], self.tok.shards[k], pos(k), cfg.seq) for k in m.coords()})
         delta = None
         for b in self.blocks:
             x, delta = b.forward(x, delta, keep)
-        _, y = GPTBlock._norm(self.ln_f, x, delta, keep)
-        return self.head.forward(y, keep)                                # [T/R, Vp/C]
+        return GPTBlock._norm(self.ln_f, x, delta, keep)[1]
+
+    def token_losses(self, tokens: ShardedTensor, targets: ShardedTensor) -> ShardedTensor:
+        """Loss [tokens] of every token of whole sequences, without logits in memory and without holding anything (a 1 x 1 mesh; a target
+        outside the vocabulary has loss 0)."""
+        if self.mesh.R * self.mesh.C != 1:
+            raise ValueError("a head without logits in memory has whole matrices: a 1 x 1 mesh")
+        y = self._features(tokens, keep=False)
+        return ShardedTensor(self.mesh, {k: F.head_loss(t, self.head.weight.shards[k], targets.shards[k], self.cfg.vocab)
+                                         for k, t in y.shards.items()})
 
     def top_logits(self, tokens: ShardedTensor, top: int, temperature: float = 1.0, hard_weight: float = 0.0) -> DistillTargets:
         """This model as a teacher: its ``top`` largest logits per token (whole rows on every device)."""
@@ -283,6 +324,12 @@ class GPTModel:
         Returns the ShardedTensor of per-coordinate loss contributions (sum over local tokens of
         the token loss divided by n_tokens_global; summing over the mesh rows gives the mean)."""
         m, cfg = self.mesh, self.cfg
+        if cfg.head_rows is not None and teacher is None:      # a teacher's targets are compared with logits
+            (k, y), = self._features(tokens, keep=True).shards.items()
+            rows, dy, _ = F.head_loss_grad(y, self.head.weight.shards[k], targets.shards[k], cfg.vocab, 1.0 / n_tokens_global,
+                                           dw=self.head.grad.shards[k], rows=cfg.head_rows)
+            self._backward(tokens, ShardedTensor(m, {k: dy}))
+            return ShardedTensor(m, {k: F.sum_over(rows, n_tokens_global)})
         logits = self.forward(tokens)
         vc = cfg.vocab_padded // m.C
         ex = getattr(getattr(m, "engine", None), "row_exchange", None)
@@ -316,7 +363,12 @@ class GPTModel:
             for k in m.coords():
                 F.ce_grad_(logits.shards[k], targets.shards[k], k[1] * vc, cfg.vocab, gmax.shards[k],
                            packed.shards[k][0].contiguous(), 1.0 / n_tokens_global)
-        d = self.head.backward(logits)
+        self._backward(tokens, self.head.backward(logits))
+        return loss
+
+    def _backward(self, tokens: ShardedTensor, d: ShardedTensor):
+        """From the gradient of what the head reads."""
+        m, cfg = self.mesh, self.cfg
         dx = self.ln_f.backward(d)                                       # gradient of x + delta
         dh, dm = dx, dx
         for b in reversed(self.blocks):
@@ -324,7 +376,6 @@ class GPTModel:
         for k in m.coords():
             F.embedding_bwd(tokens.shards[k], dh.shards[k], self.dtok.shards[k], None if self.dpos is None else self.dpos.shards[k],
                             cfg.seq)
-        return loss
 
     def sync_replicated_grads(self):
         """Sum the gradients of row-replicated parameters over the mesh rows."""

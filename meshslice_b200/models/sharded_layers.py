@@ -377,6 +377,63 @@ class GeLU:
         return ShardedTensor(x.mesh, {k: F.gelu_bwd(dy.shards[k], v) for k, v in x.shards.items()})
 
 
+class ShardedGatedFF:
+    """Gated feed-forward block (act(x Wg) * (x Wu)) Wd of three sharded linears; the features between them are sharded as those of
+    ``ShardedFFLayer`` are.  Where whole matrices are on one GPU the two projections, the activation and the product are one kernel."""
+
+    def __init__(self, mesh: Mesh, algorithm: str, dataflows, ksplits, dim: int, ffn: int, act: str = "silu", seeds=(0, 1, 2), **kw):
+        """``dataflows`` / ``ksplits``: of gate and up, of down; ``kw``: as ``ShardedFFLayer`` takes them."""
+        if "rs" in dataflows:
+            raise ValueError("a gated feed-forward block takes 'os' and 'ls' layers")
+        if act not in F.GATED_ACTS:
+            raise ValueError(f"unknown activation {act!r}: one of {sorted(F.GATED_ACTS)}")
+        self.mesh, self.act = mesh, act
+        self.gate = ShardedFFLayer(mesh, algorithm, dataflows[0], ksplits[0], dim, ffn, seed=seeds[0], **kw)
+        self.up = ShardedFFLayer(mesh, algorithm, dataflows[0], ksplits[0], dim, ffn, seed=seeds[1], **kw)
+        self.down = ShardedFFLayer(mesh, algorithm, dataflows[1], ksplits[1], ffn, dim, seed=seeds[2], **kw)
+        self._saved = None
+
+    def _whole(self, x: ShardedTensor) -> bool:
+        return self.gate._dw_dx is not None and x.local().is_cuda
+
+    def _layouts(self):
+        return tuple("nt" if layer.dataflow == "ls" else "nn" for layer in (self.up, self.down))
+
+    def _weights(self, key):
+        return tuple(layer.weight.shards[key] for layer in (self.gate, self.up, self.down))
+
+    def forward(self, x: ShardedTensor, keep: bool = True) -> ShardedTensor:
+        if self._whole(x):
+            (key, t), = x.shards.items()
+            up, down = self._layouts()
+            y, saved = F.gated_ff_fwd(t, *self._weights(key), act=self.act, up_layout=up, down_layout=down, keep=keep)
+            if keep:
+                self._saved = (x, saved)
+            return ShardedTensor(self.mesh, {key: y})
+        g, u = self.gate.forward(x, keep), self.up.forward(x, keep)
+        if keep:
+            self._saved = (g, u)
+        h = ShardedTensor(self.mesh, {k: F.gated_act(v, u.shards[k], self.act) for k, v in g.shards.items()})
+        return self.down.forward(h, keep)
+
+    def backward(self, dy: ShardedTensor) -> ShardedTensor:
+        a, b = self._saved
+        self._saved = None
+        if isinstance(b, F.GatedSaved):
+            (key, t), = a.shards.items()
+            up, down = self._layouts()
+            grads = tuple(layer.grad.shards[key] for layer in (self.gate, self.up, self.down))
+            dx, _ = F.gated_ff_bwd(dy.shards[key], t, *self._weights(key), b, act=self.act, up_layout=up, down_layout=down, grads=grads)
+            return ShardedTensor(self.mesh, {key: dx})
+        dh = self.down.backward(dy)
+        both = {k: F.gated_act_bwd(v, a.shards[k], b.shards[k], self.act) for k, v in dh.shards.items()}
+        dg, du = (ShardedTensor(self.mesh, {k: v[i] for k, v in both.items()}) for i in (0, 1))
+        return _add(self.gate.backward(dg), self.up.backward(du))
+
+    def layers(self):
+        return [self.gate, self.up, self.down]
+
+
 def _add(a: ShardedTensor, b: ShardedTensor) -> ShardedTensor:
     return ShardedTensor(a.mesh, {k: F.add(a.shards[k], b.shards[k]) for k in a.shards})
 

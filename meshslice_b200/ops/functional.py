@@ -11,7 +11,7 @@ import torch
 
 from .. import _native
 from .distill import distill_grad, distill_loss_grad, distill_partial  # noqa: F401  (ops of this module's callers)
-from .gated import GatedSaved, gated_act, gated_act_bwd, gated_ff_bwd, gated_ff_fwd  # noqa: F401
+from .gated import ACTS as GATED_ACTS, GatedSaved, gated_act, gated_act_bwd, gated_ff_bwd, gated_ff_fwd  # noqa: F401
 from .head import head_loss, head_loss_grad  # noqa: F401
 from .orthogonal import orthogonalize  # noqa: F401
 from .rotary import Rotary, RotaryConfig, rotary_qkv  # noqa: F401

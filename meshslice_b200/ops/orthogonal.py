@@ -21,7 +21,7 @@ from .. import _native
 from .gemm import sm_count
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
-WORKSPACE_BYTES = 8 << 30       # matrices of a batch are taken some at a time beyond it
+WORKSPACE_BYTES = 2 << 30       # matrices of a batch are taken some at a time beyond it
 # powers of two that the fp16 copies are scaled by: their largest values are below 4, 16 and 255 (what the coefficients are checked for)
 _SX, _SA, _SB = 2.0 ** 10, 2.0 ** 10, 2.0 ** 8
 

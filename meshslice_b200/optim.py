@@ -14,6 +14,7 @@ from typing import List, Optional
 import torch
 
 from . import _native
+from .ops.orthogonal import COEFFICIENTS, orthogonalize
 
 
 class FlatGroup:
@@ -69,23 +70,36 @@ class AdamW:
         return self._scale
 
     def step(self):
+        self._step()
+
+    def _step(self):
+        """AdamW on the spans of the groups; returns the gradients' scale."""
         self.step_count += 1
         b1, b2 = self.betas
         bc1, bc2 = 1 - b1 ** self.step_count, 1 - b2 ** self.step_count
         scale = self._grad_scale()
         for g in self.groups:
-            if g.param.is_cuda:
-                _native.load().adamw_step(g.param.data_ptr(), g.master.data_ptr(), g.m.data_ptr(), g.v.data_ptr(),
-                                          g.grad.data_ptr(), 1 if g.grad.dtype == torch.float32 else 0,
-                                          g.param.numel(), self.lr, b1, b2, self.eps, self.wd, bc1, bc2,
-                                          0 if scale is None else scale.data_ptr(), _native.stream_ptr())
-            else:
-                gr = g.grad.float() * (1.0 if scale is None else scale.item())
-                g.m.mul_(b1).add_(gr, alpha=1 - b1)
-                g.v.mul_(b2).addcmul_(gr, gr, value=1 - b2)
-                upd = (g.m / bc1) / ((g.v / bc2).sqrt() + self.eps) + self.wd * g.master
-                g.master.add_(upd, alpha=-self.lr)
-                g.param.copy_(g.master.to(g.param.dtype))
+            for a, b in self._spans(g):
+                param, grad, master, m, v = g.param, g.grad, g.master, g.m, g.v
+                if b - a != param.numel():
+                    param, grad, master, m, v = (t[a:b] for t in (param, grad, master, m, v))
+                if param.is_cuda:
+                    _native.load().adamw_step(param.data_ptr(), master.data_ptr(), m.data_ptr(), v.data_ptr(),
+                                              grad.data_ptr(), 1 if grad.dtype == torch.float32 else 0,
+                                              param.numel(), self.lr, b1, b2, self.eps, self.wd, bc1, bc2,
+                                              0 if scale is None else scale.data_ptr(), _native.stream_ptr())
+                else:
+                    gr = grad.float() * (1.0 if scale is None else scale.item())
+                    m.mul_(b1).add_(gr, alpha=1 - b1)
+                    v.mul_(b2).addcmul_(gr, gr, value=1 - b2)
+                    upd = (m / bc1) / ((v / bc2).sqrt() + self.eps) + self.wd * master
+                    master.add_(upd, alpha=-self.lr)
+                    param.copy_(master.to(param.dtype))
+        return scale
+
+    def _spans(self, g: FlatGroup):
+        """The elements of a group that this step updates, as (first, end) pairs."""
+        return [(0, g.param.numel())]
 
     def zero_grad(self):
         for g in self.groups:
@@ -140,3 +154,94 @@ class AdamW:
             g.m.copy_(s["m"])
             g.v.copy_(s["v"])
             g.param.copy_(g.master.to(g.param.dtype))
+
+
+UPDATE_BYTES = 1 << 30      # of updates that are in memory at a time
+
+
+class Muon(AdamW):
+    """Orthogonal updates of matrices, AdamW for everything else in the flat buffers.  Per matrix, with its gradient g (clipped by the norm of
+    all gradients):
+
+        m <- momentum m + g        u = g + momentum m (nesterov) or m
+        w <- w - lr (0.2 sqrt(max(rows, columns)) orthogonalize(u) + weight_decay w)
+
+    whose elements are of the size of AdamW's, so that one learning rate serves both.  ``matrices``: whole 2-D views of the groups'
+    parameters; those of one shape that lie at equal distances are updated together.  Their m is kept in the group's first
+    moment, and the second one stays 0.
+    """
+
+    def __init__(self, groups: List[FlatGroup], matrices: List[torch.Tensor], momentum: float = 0.95, nesterov: bool = True, steps: int = 5,
+                 coefficients=COEFFICIENTS, **kw):
+        super().__init__(groups, **kw)
+        if self.mesh is not None and self.mesh.R * self.mesh.C > 1:
+            raise ValueError("orthogonal updates are of whole matrices: a 1 x 1 mesh")
+        if not 0.0 <= momentum < 1.0:
+            raise ValueError(f"momentum must be in [0, 1) (got {momentum})")
+        self.momentum, self.nesterov, self.steps, self.coefficients = momentum, nesterov, steps, coefficients
+        self._stacks = []                 # (group, first element, distance, count, rows, columns)
+        self._rest = {}                   # of the groups, by identity of the group: spans that AdamW updates
+        taken = {id(g): [] for g in groups}
+        found = sorted((self._place(w) + tuple(w.shape) for w in matrices), key=lambda t: (t[0], t[2:], t[1]))
+        for k, at, r, c in found:
+            taken[id(groups[k])].append((at, at + r * c))
+            last = self._stacks[-1] if self._stacks else None
+            if last is not None and (last[0], *last[4:]) == (k, r, c):
+                first, gap, n = last[1:4]
+                if (n == 1 and at >= first + r * c) or (n > 1 and at == first + n * gap):
+                    self._stacks[-1] = (k, first, at - first if n == 1 else gap, n + 1, r, c)
+                    continue
+            self._stacks.append((k, at, r * c, 1, r, c))
+        for g in groups:
+            at, rest = 0, []
+            for a, b in sorted(taken[id(g)]) + [(g.param.numel(), g.param.numel())]:
+                if a < at:
+                    raise ValueError("two of the matrices share elements")
+                if a > at:
+                    rest.append((at, a))
+                at = b
+            self._rest[id(g)] = rest
+
+    def _place(self, w: torch.Tensor):
+        if w.dim() != 2 or not w.is_contiguous() or w.numel() % 4:
+            raise ValueError(f"matrices are contiguous, of a multiple of 4 elements (got {tuple(w.shape)})")
+        for k, g in enumerate(self.groups):
+            at = w.data_ptr() - g.param.data_ptr()
+            if w.dtype == g.param.dtype and 0 <= at < g.param.numel() * g.param.element_size():
+                at //= g.param.element_size()
+                if at % 4 or at + w.numel() > g.param.numel():
+                    raise ValueError("a matrix begins at a multiple of 4 elements of its flat buffer and ends in it")
+                return k, at
+        raise ValueError("a matrix lies outside the optimizer's flat buffers")
+
+    def _spans(self, g: FlatGroup):
+        return self._rest[id(g)]
+
+    def step(self):
+        scale = self._step()
+        for k, first, gap, count, r, c in self._stacks:
+            some = max(1, min(count, UPDATE_BYTES // (4 * r * c)))
+            for i in range(0, count, some):
+                self._update(k, first + i * gap, gap, min(some, count - i), r, c, scale)
+
+    def _update(self, k: int, at: int, gap: int, n: int, r: int, c: int, scale):
+        """``n`` matrices of group ``k``, ``gap`` elements apart from element ``at`` on."""
+        g, size = self.groups[k], 0.2 * math.sqrt(max(r, c))
+        if g.param.is_cuda:
+            _native.check_device(g.param)
+            C, stream = _native.load(), _native.stream_ptr()
+            u = torch.empty(n, r, c, dtype=torch.float32, device=g.param.device)
+            wide = g.grad.element_size()
+            C.momentum_step(g.grad.data_ptr() + at * wide, 1 if wide == 4 else 0, g.m.data_ptr() + at * 4, u.data_ptr(), n, r * c, gap,
+                            self.momentum, 1 if self.nesterov else 0, 0 if scale is None else scale.data_ptr(), stream)
+            orthogonalize(u, self.steps, self.coefficients, out=u)
+            C.apply_update(u.data_ptr(), g.master.data_ptr() + at * 4, g.param.data_ptr() + at * g.param.element_size(), n, r * c, gap,
+                           self.lr, size, self.wd, stream)
+            return
+        view = lambda t: t.as_strided((n, r, c), (gap, c, 1), t.storage_offset() + at)
+        grad = view(g.grad).float() * (1.0 if scale is None else scale.item())
+        m, master = view(g.m), view(g.master)
+        m.mul_(self.momentum).add_(grad)
+        u = grad + self.momentum * m if self.nesterov else m
+        master.sub_(self.lr * (size * orthogonalize(u, self.steps, self.coefficients, out_dtype=torch.float32) + self.wd * master))
+        view(g.param).copy_(master.to(g.param.dtype))

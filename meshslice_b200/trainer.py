@@ -16,7 +16,7 @@ import torch
 
 from . import _native
 from .models.gpt import GPTConfig, GPTModel
-from .optim import AdamW, FlatGroup
+from .optim import AdamW, FlatGroup, Muon
 from .parallel.mesh import DistMesh, EmuMesh, Mesh, ShardedTensor
 
 
@@ -40,7 +40,7 @@ def param_elems(cfg: GPTConfig, R: int, C: int) -> Tuple[int, int]:
     """Elements (with alignment padding) of the sharded and row-replicated buffers of one rank."""
     pad = lambda n: (n + 127) // 128 * 128
     d, f, V = cfg.d_model, cfg.ffn, cfg.vocab_padded
-    per_layer = pad(d * cfg.qkv_dim // (R * C)) + pad(d * d // (R * C)) + 2 * pad(d * f // (R * C))
+    per_layer = pad(d * cfg.qkv_dim // (R * C)) + pad(d * d // (R * C)) + cfg.ff_matrices * pad(d * f // (R * C))
     sharded = cfg.n_layers * per_layer + pad(d * V // (R * C))
     rep = pad(V * d // C) + (pad(cfg.seq * d // C) if cfg.rotary is None else 0) + (2 * cfg.n_layers + 1) * 2 * pad(d // C)
     return sharded, rep
@@ -61,6 +61,8 @@ class TrainConfig:
     max_grad_norm: Optional[float] = 1.0
     backend: str = "fused"        # 'fused' (tcgen05 + in-kernel NVLink) or 'collective' (NCCL + library GEMM)
     timeout_ns: int = 20_000_000_000
+    optimizer: str = "adamw"      # or 'muon': orthogonal updates of the blocks' matrices, AdamW for the rest (a 1 x 1 mesh)
+    momentum: float = 0.95        # of 'muon'
 
 
 def workspace_bytes(cfg, micro_batch: int, R: int, C: int):
@@ -92,6 +94,10 @@ class Trainer:
         self.world = dist.get_world_size() if self.distributed else 1
         self.rank = dist.get_rank() if self.distributed else 0
         R, C = mesh_shape or choose_mesh(self.world)
+        if tcfg.optimizer not in ("adamw", "muon"):
+            raise ValueError(f"unknown optimizer {tcfg.optimizer!r}")
+        if tcfg.optimizer == "muon" and R * C != 1:
+            raise ValueError("orthogonal updates are of whole matrices: a 1 x 1 mesh")
         self.device = device or torch.device("cuda", torch.cuda.current_device())
         if self.distributed and self.world > 1:
             self.mesh = DistMesh(R, C)
@@ -127,9 +133,13 @@ class Trainer:
         a_sh, a_gsh, a_rep, a_grep = Arena(self.p_sh), Arena(self.g_sh), Arena(self.p_rep), Arena(self.g_rep)
         self.model = GPTModel(self.mesh, cfg, device=self.device, alloc_sharded=a_sh.alloc, alloc_rep=a_rep.alloc,
                               grad_sharded=a_gsh.alloc, grad_rep=a_grep.alloc)
-        self.opt = AdamW([FlatGroup(self.p_sh, self.g_sh, "sharded"), FlatGroup(self.p_rep, self.g_rep, "row_replicated")],
-                         lr=tcfg.lr, betas=tcfg.betas, weight_decay=tcfg.weight_decay,
-                         max_grad_norm=tcfg.max_grad_norm, mesh=self.mesh if self.world > 1 else None)
+        groups = [FlatGroup(self.p_sh, self.g_sh, "sharded"), FlatGroup(self.p_rep, self.g_rep, "row_replicated")]
+        kw = dict(lr=tcfg.lr, betas=tcfg.betas, weight_decay=tcfg.weight_decay, max_grad_norm=tcfg.max_grad_norm,
+                  mesh=self.mesh if self.world > 1 else None)
+        if tcfg.optimizer == "muon":
+            self.opt = Muon(groups, [w.local() for b in self.model.blocks for w in b.matrices()], momentum=tcfg.momentum, **kw)
+        else:
+            self.opt = AdamW(groups, **kw)
         self.n_tokens = tcfg.global_batch * cfg.seq
         self._ids_dev = torch.empty(self.rows_batch, cfg.seq + 1, dtype=torch.int64, device=self.device)
         self._loss_dev = torch.zeros(1, dtype=torch.float32, device=self.device)
