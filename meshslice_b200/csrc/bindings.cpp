@@ -18,6 +18,7 @@
 #include "comm/p2p.h"
 #include "gemm/sm100_gemm.h"
 #include "gemm/sm100_products.h"
+#include "gemm/tile_walk.h"
 #include "ops/attention.h"
 #include "ops/distill.h"
 #include "ops/gated.h"
@@ -399,115 +400,163 @@ void order_of(Product& p, int64_t K, int tile_n) {
   p.group = o.group;
   p.along_n = o.along_n;
 }
-void run_products(ProductArgs& a, int k0, int k1, int problems, int tile_n, int sms, uint64_t status, uint64_t stream, const char* what) {
+
+Product& plain_problem(Product& p, int64_t M, int64_t N) {
+  p.M = (int)M;
+  p.N = (int)N;
+  p.items = 1;
+  p.a_item = p.b_item = 0;
+  return p;
+}
+// C (+)= A0 B0 (+ A1 B1)
+void plain_product(Product& p, int tile_n, int64_t M, int64_t N, const int64_t* K, const ProductOperand* a, const ProductOperand* b, int ranges,
+                   uint64_t C, int64_t ldc, int fp32, int accumulate, const char* what) {
+  plain_problem(p, M, N);
+  products_ok(product_operands(&p, kPlain, tile_n, a, b, ranges, M, N, K), what);
+  products_ok(product_output(&p, 0, P<void>(C), N, M, ldc, fp32 != 0), what);
+  p.c = P<void>(C);
+  p.ldc = ldc;
+  p.out_fp32 = fp32;
+  p.accumulate = accumulate;
+  order_of(p, K[0] + (ranges > 1 ? K[1] : 0), tile_n);
+}
+void run_products(ProductArgs& a, int k0, int k1, int problems, int longer, int tile_n, int sms, uint64_t status, uint64_t stream, const char* what) {
   a.status = P<uint32_t>(status);
   a.timeout_ns = kLocalTimeoutNs;
-  check(launch_sm100_products(a, k0, k1, problems, tile_n, sms, S(stream)), what);
+  check(launch_sm100_products(a, k0, k1, problems, longer, tile_n, sms, S(stream)), what);
 }
-// Columns of a tile for a product of this kind: a tile of 128 counts three quarters of one of 256 (gemm2_tile_n).
-int64_t products_waves(int kind, int64_t M, int64_t N, int64_t items, int tile_n, int sms) {
+int64_t products_tiles(int kind, int64_t M, int64_t N, int64_t items, int tile_n) {
   Product p;
-  std::memset(static_cast<void*>(&p), 0, sizeof(p));
   p.M = (int)M;
   p.N = (int)N;
   p.items = (int)items;
-  const int64_t pairs = sms > 1 ? sms / 2 : 1;
-  return (product_tiles(p, kind, tile_n) + pairs - 1) / pairs;
+  return product_tiles(p, kind, tile_n);
 }
+// Columns of a tile: one of 128 counts three quarters of one of 256 (gemm2_tile_n).
 int products_tile_n(int kind, int64_t M, int64_t N, int64_t items, int sms) {
-  return 3 * products_waves(kind, M, N, items, 128, sms) < 4 * products_waves(kind, M, N, items, 256, sms) ? 128 : 256;
+  const int64_t pairs = sms > 1 ? sms / 2 : 1;
+  const auto waves = [&](int tile_n) { return (products_tiles(kind, M, N, items, tile_n) + pairs - 1) / pairs; };
+  return 3 * waves(128) < 4 * waves(256) ? 128 : 256;
+}
+// The same for two groups of problems: tiles of the longer and of the shorter contraction.
+template <class F>
+int joint_tile_n(F tiles, int64_t k0, int64_t k1, int sms) {
+  const int64_t pairs = sms > 1 ? sms / 2 : 1;
+  const auto end = [&](int tile_n) { return walk_end(tiles(0, tile_n), k0, tiles(1, tile_n), k1, pairs); };
+  return 3 * end(128) < 4 * end(256) ? 128 : 256;
 }
 
-// tokens, width, ffn, x, ldx, gate, ld, up, ld, mn_major, h, g, u, exps, act, keep, sms, status, stream
-void gated_fwd(const std::array<int64_t, 19>& v) {
+// tokens, inputs, features, outputs, x, ld, gate, ld, up, ld, up_nt, down, ld, down_nt, y, h, g, u, exps, act, keep, sms, status, stream
+void gated_fwd(const std::array<int64_t, 24>& v) {
   static thread_local ProductArgs a;
-  Product& p = a.p[0];
-  p.M = (int)v[0];
-  p.N = (int)v[2];
-  p.items = 1;
-  p.a_item = p.b_item = 0;
-  const int tile_n = products_tile_n(kGated, v[0], v[2], 1, (int)v[16]);
-  const ProductOperand x{P<void>(v[3]), v[4], 0, 0}, w[2] = {{P<void>(v[5]), v[6], (int)v[9], 0}, {P<void>(v[7]), v[8], (int)v[9], 0}};
-  products_ok(product_operands(&p, kGated, tile_n, &x, w, 1, v[0], v[2], &v[1]), "gated_fwd");
-  p.act = (int)v[14];
-  p.keep = (int)v[15];
-  products_ok(product_output(&p, 0, P<void>(v[10]), v[2], v[0], v[2], false), "gated_fwd");
-  if (p.keep) {
-    products_ok(product_output(&p, 1, P<void>(v[11]), v[2], v[0], v[2], false), "gated_fwd");
-    products_ok(product_output(&p, 2, P<void>(v[12]), v[2], v[0], v[2], false), "gated_fwd");
+  const int64_t n = v[0], d = v[1], f = v[2], o = v[3];
+  const int sms = (int)v[21];
+  const uint64_t status = (uint64_t)v[22], stream = (uint64_t)v[23];
+  Product& p = plain_problem(a.p[0], n, f);
+  const int tile_n = products_tile_n(kGated, n, f, 1, sms), up_mn = v[10] ? 0 : 1;
+  const ProductOperand x{P<void>(v[4]), v[5], 0, 0}, w[2] = {{P<void>(v[6]), v[7], up_mn, 0}, {P<void>(v[8]), v[9], up_mn, 0}};
+  products_ok(product_operands(&p, kGated, tile_n, &x, w, 1, n, f, &d), "gated_fwd");
+  p.act = (int)v[19];
+  p.keep = (int)v[20];
+  for (int i = 0; i < (p.keep ? 3 : 1); ++i) products_ok(product_output(&p, i, P<void>(v[15 + i]), f, n, f, false), "gated_fwd");
+  p.exps = P<uint16_t>(v[18]);
+  order_of(p, d, tile_n);
+  run_products(a, kGated, kNone, 1, 1, tile_n, sms, status, stream, "gated_fwd");
+  const Gemm2Operands y = local_operands(n, o, f, (uint64_t)v[15], f, 0, (uint64_t)v[11], v[12], v[13] ? 0 : 1, (uint64_t)v[14], o, 0, 0, status);
+  run_gemm2(&y, 1, gemm2_tile_n(&y, 1, sms), sms, P<uint32_t>(status), kLocalTimeoutNs, stream);
+}
+// tokens, inputs, features, outputs, dy, ld, x, ld, gate, ld, up, ld, up_nt, down, ld, down_nt, h, g, u, exps, dg, du, dx, dgate, ld, dup, ld,
+// ddown, ld, their types (bit i: fp32), accumulate, act, sms, status, stream
+void gated_bwd(const std::array<int64_t, 35>& v) {
+  static thread_local ProductArgs a;
+  const int64_t n = v[0], d = v[1], f = v[2], o = v[3];
+  const int sms = (int)v[32], add = (int)v[30], types = (int)v[29];
+  const uint64_t status = (uint64_t)v[33], stream = (uint64_t)v[34];
+  const bool up_nt = v[12] != 0, down_nt = v[15] != 0;
+  // dh = dy Wd^T with dg and du, and dWd = h^T dy (or its transpose), which does not need them
+  {
+    const int64_t kd = (o + kBK - 1) / kBK, kw = (n + kBK - 1) / kBK, wm = down_nt ? o : f, wn = down_nt ? f : o;
+    const bool grad_first = kd >= kw;
+    const int tile_n = joint_tile_n([&](int i, int t) { return (i == 0) == grad_first ? products_tiles(kGatedGrad, n, f, 1, t) : products_tiles(kPlain, wm, wn, 1, t); },
+                                    grad_first ? kd : kw, grad_first ? kw : kd, sms);
+    Product& p = plain_problem(a.p[grad_first ? 0 : 1], n, f);
+    const ProductOperand dy{P<void>(v[4]), v[5], 0, 0}, w{P<void>(v[13]), v[14], down_nt ? 1 : 0, 0};
+    products_ok(product_operands(&p, kGatedGrad, tile_n, &dy, &w, 1, n, f, &o), "gated_bwd");
+    p.g = P<void>(v[17]);
+    p.u = P<void>(v[18]);
+    p.exps = P<uint16_t>(v[19]);
+    p.act = (int)v[31];
+    for (int i = 0; i < 2; ++i) products_ok(product_output(&p, i, P<void>(v[20 + i]), f, n, f, false), "gated_bwd");
+    order_of(p, o, tile_n);
+    const ProductOperand h{P<void>(v[16]), f, 1, 0}, dyt{P<void>(v[4]), v[5], 1, 0};
+    plain_product(a.p[grad_first ? 1 : 0], tile_n, wm, wn, &n, down_nt ? &dyt : &h, down_nt ? &h : &dyt, 1, (uint64_t)v[27], v[28], types >> 2 & 1, add,
+                  "gated_bwd");
+    run_products(a, grad_first ? kGatedGrad : kPlain, grad_first ? kPlain : kGatedGrad, 2, 1, tile_n, sms, status, stream, "gated_bwd");
   }
-  p.exps = P<uint16_t>(v[13]);
-  order_of(p, v[1], tile_n);
-  run_products(a, kGated, kNone, 1, tile_n, (int)v[16], (uint64_t)v[17], (uint64_t)v[18], "gated_fwd");
+  // dx = dg Wg^T + du Wu^T, dWg = x^T dg, dWu = x^T du (or their transposes)
+  {
+    const int64_t kx = 2 * ((f + kBK - 1) / kBK), kw = (n + kBK - 1) / kBK, wm = up_nt ? f : d, wn = up_nt ? d : f, ff[2] = {f, f};
+    const bool dx_first = kx >= kw;
+    const int tile_n = joint_tile_n([&](int i, int t) { return (i == 0) == dx_first ? products_tiles(kPlain, n, d, 1, t) : 2 * products_tiles(kPlain, wm, wn, 1, t); },
+                                    dx_first ? kx : kw, dx_first ? kw : kx, sms);
+    const ProductOperand g[2] = {{P<void>(v[20]), f, 0, 0}, {P<void>(v[21]), f, 0, 0}};
+    const ProductOperand w[2] = {{P<void>(v[8]), v[9], up_nt ? 1 : 0, 0}, {P<void>(v[10]), v[11], up_nt ? 1 : 0, 0}};
+    plain_product(a.p[dx_first ? 0 : 2], tile_n, n, d, ff, g, w, 2, (uint64_t)v[22], d, 0, 0, "gated_bwd");
+    const ProductOperand xt{P<void>(v[6]), v[7], 1, 0};
+    for (int i = 0; i < 2; ++i) {
+      const ProductOperand gt{P<void>(v[20 + i]), f, 1, 0};
+      plain_product(a.p[dx_first ? 1 + i : i], tile_n, wm, wn, &n, up_nt ? &gt : &xt, up_nt ? &xt : &gt, 1, (uint64_t)v[23 + 2 * i], v[24 + 2 * i],
+                    types >> i & 1, add, "gated_bwd");
+    }
+    run_products(a, kPlain, kPlain, 3, dx_first ? 1 : 2, tile_n, sms, status, stream, "gated_bwd");
+  }
 }
-// tokens, ffn, outputs, dy, ld, down, ld, mn_major, g, u, exps, dg, du, act, sms, status, stream
-void gated_grad(const std::array<int64_t, 17>& v) {
+
+// Statistics of the logits' tiles, and their exponentials where `e` is given.
+void head_partial(int64_t rows, int64_t width, int64_t vocab, int64_t columns, uint64_t x, int64_t ldx, uint64_t w, int64_t ldw, int mn, uint64_t e,
+                  uint64_t stats, uint64_t label, uint64_t targets, int tile_n, int sms, uint64_t status, uint64_t stream) {
   static thread_local ProductArgs a;
-  Product& p = a.p[0];
-  p.M = (int)v[0];
-  p.N = (int)v[1];
-  p.items = 1;
-  p.a_item = p.b_item = 0;
-  const int tile_n = products_tile_n(kGatedGrad, v[0], v[1], 1, (int)v[14]);
-  const ProductOperand dy{P<void>(v[3]), v[4], 0, 0}, w{P<void>(v[5]), v[6], (int)v[7], 0};
-  products_ok(product_operands(&p, kGatedGrad, tile_n, &dy, &w, 1, v[0], v[1], &v[2]), "gated_grad");
-  p.g = P<void>(v[8]);
-  p.u = P<void>(v[9]);
-  p.exps = P<uint16_t>(v[10]);
-  p.act = (int)v[13];
-  for (int i = 0; i < 2; ++i) products_ok(product_output(&p, i, P<void>(v[11 + i]), v[1], v[0], v[1], false), "gated_grad");
-  order_of(p, v[2], tile_n);
-  run_products(a, kGatedGrad, kNone, 1, tile_n, (int)v[14], (uint64_t)v[15], (uint64_t)v[16], "gated_grad");
+  Product& p = plain_problem(a.p[0], rows, columns);
+  const ProductOperand A{P<void>(x), ldx, 0, 0}, B{P<void>(w), ldw, mn, 0};
+  products_ok(product_operands(&p, kHead, tile_n, &A, &B, 1, rows, vocab, &width), "head");
+  p.write = e != 0;
+  if (p.write) products_ok(product_output(&p, 0, P<void>(e), columns, rows, columns, false), "head");
+  p.stats = P<float2>(stats);
+  p.label = P<float>(label);
+  p.targets = P<int64_t>(targets);
+  p.vocab = (int)vocab;
+  order_of(p, width, tile_n);
+  run_products(a, kHead, kNone, 1, 1, tile_n, sms, status, stream, "head");
 }
-// C = A0 B0 + A1 B1: M, N, K0, K1, A0, ld, A1, ld, a_mn_major, B0, ld, B1, ld, b_mn_major, C, ld, sms, status, stream
-void gemm_sum(const std::array<int64_t, 19>& v) {
-  static thread_local ProductArgs a;
-  Product& p = a.p[0];
-  p.M = (int)v[0];
-  p.N = (int)v[1];
-  p.items = 1;
-  p.a_item = p.b_item = 0;
-  const int tile_n = products_tile_n(kPlain, v[0], v[1], 1, (int)v[16]);
-  const ProductOperand x[2] = {{P<void>(v[4]), v[5], (int)v[8], 0}, {P<void>(v[6]), v[7], (int)v[8], 0}};
-  const ProductOperand w[2] = {{P<void>(v[9]), v[10], (int)v[13], 0}, {P<void>(v[11]), v[12], (int)v[13], 0}};
-  products_ok(product_operands(&p, kPlain, tile_n, x, w, 2, v[0], v[1], &v[2]), "gemm_sum");
-  products_ok(product_output(&p, 0, P<void>(v[14]), v[1], v[0], v[15], false), "gemm_sum");
-  order_of(p, v[2] + v[3], tile_n);
-  run_products(a, kPlain, kNone, 1, tile_n, (int)v[16], (uint64_t)v[17], (uint64_t)v[18], "gemm_sum");
+// Losses of `rows` tokens: nt: the weight lies as [columns, inputs]; stats [blocks, rows, 2] and label [rows]: fp32 scratch
+void head_losses(int64_t rows, int64_t width, int64_t vocab, uint64_t x, int64_t ldx, uint64_t w, int64_t ldw, int nt, uint64_t targets,
+                 uint64_t stats, uint64_t label, int tile_n, uint64_t loss, int sms, uint64_t status, uint64_t stream) {
+  head_partial(rows, width, vocab, vocab, x, ldx, w, ldw, nt ? 0 : 1, 0, stats, label, targets, tile_n, sms, status, stream);
+  const int half = tile_n / 2, blocks = (int)((vocab + half - 1) / half);
+  check(head_rows({nullptr, 0, P<float2>(stats), P<float>(label), P<int64_t>(targets), (int)rows, 0, blocks, half, (int)vocab, 0.f, P<float>(loss)},
+                  S(stream)), "head_rows");
 }
-// rows, width, vocab, columns, x, ldx, w, ldw, mn_major, e (0: losses alone), lde, stats, label, targets, tile_n, sms, status, stream
-void head_partial(const std::array<int64_t, 18>& v) {
-  static thread_local ProductArgs a;
-  Product& p = a.p[0];
-  p.M = (int)v[0];
-  p.N = (int)v[3];
-  p.items = 1;
-  p.a_item = p.b_item = 0;
-  const int tile_n = (int)v[14];
-  const ProductOperand x{P<void>(v[4]), v[5], 0, 0}, w{P<void>(v[6]), v[7], (int)v[8], 0};
-  products_ok(product_operands(&p, kHead, tile_n, &x, &w, 1, v[0], v[2], &v[1]), "head_partial");
-  p.write = v[9] != 0;
-  if (p.write) products_ok(product_output(&p, 0, P<void>(v[9]), v[3], v[0], v[10], false), "head_partial");
-  p.stats = P<float2>(v[11]);
-  p.label = P<float>(v[12]);
-  p.targets = P<int64_t>(v[13]);
-  p.vocab = (int)v[2];
-  order_of(p, v[1], tile_n);
-  run_products(a, kHead, kNone, 1, tile_n, (int)v[15], (uint64_t)v[16], (uint64_t)v[17], "head_partial");
+// Losses and gradients of `rows` tokens: e [rows, columns] is scratch too; dw is written or added to as far as `wide` of its columns, and
+// `pad_height` rows of `pad_width` bytes from `pad` on, `pad_pitch` apart, are cleared.
+void head_grads(int64_t rows, int64_t width, int64_t vocab, int64_t columns, int64_t wide, uint64_t x, int64_t ldx, uint64_t w, int64_t ldw,
+                int nt, uint64_t targets, float scale, uint64_t e, uint64_t stats, uint64_t label, int tile_n, uint64_t loss, uint64_t dx,
+                uint64_t dw, int64_t lddw, int dw_fp32, int accumulate, uint64_t pad, int64_t pad_pitch, int64_t pad_width, int64_t pad_height,
+                int sms, uint64_t status, uint64_t stream) {
+  head_partial(rows, width, vocab, columns, x, ldx, w, ldw, nt ? 0 : 1, e, stats, label, targets, tile_n, sms, status, stream);
+  const int half = tile_n / 2, blocks = (int)((columns + half - 1) / half);
+  check(head_rows({P<void>(e), columns, P<float2>(stats), P<float>(label), P<int64_t>(targets), (int)rows, (int)columns, blocks, half, (int)vocab,
+                   scale, P<float>(loss)}, S(stream)), "head_rows");
+  Gemm2Operands o[2];
+  if (nt) o[0] = local_operands(wide, width, rows, e, columns, 1, x, ldx, 1, dw, lddw, dw_fp32, accumulate, status);
+  else o[0] = local_operands(width, wide, rows, x, ldx, 1, e, columns, 1, dw, lddw, dw_fp32, accumulate, status);
+  o[1] = local_operands(rows, width, vocab, e, columns, 0, w, ldw, nt ? 1 : 0, dx, width, 0, 0, status);
+  if (o[1].K > o[0].K) std::swap(o[0], o[1]);
+  run_gemm2(o, 2, gemm2_tile_n(o, 2, sms), sms, P<uint32_t>(status), kLocalTimeoutNs, stream);
+  if (pad_height > 0 && pad_width > 0)
+    check(cudaMemset2DAsync(P<void>(pad), pad_pitch, 0, pad_width, pad_height, reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream))),
+          "cudaMemset2DAsync");
 }
-void py_head_rows(uint64_t e, int64_t ld, uint64_t stats, uint64_t label, uint64_t targets, int rows, int cols, int tiles, int tile_n, int vocab,
-                  float scale, uint64_t loss, uint64_t stream) {
-  check(head_rows({P<void>(e), ld, P<float2>(stats), P<float>(label), P<int64_t>(targets), rows, cols, tiles, tile_n, vocab, scale,
-                   P<float>(loss)}, S(stream)), "head_rows");
-}
-// The unit matrix and its fp16 copy: g, bf16, stride, items, rows, cols, transpose, partial, x, xs, mp, np, scale, stream
-void unit_load(uint64_t g, int bf16, int64_t stride, int items, int rows, int cols, int transpose, uint64_t partial, uint64_t x, uint64_t xs,
-               int mp, int np, float scale, uint64_t stream) {
-  const int64_t n = (int64_t)rows * cols;
-  check(square_sums(P<void>(g), bf16, items, n, stride, P<double>(partial), S(stream)), "square_sums");
-  check(load_unit({P<void>(g), bf16, stride, items, rows, cols, transpose, P<double>(partial), norm_parts(n), P<float>(x), P<void>(xs), mp, np,
-                   scale}, S(stream)), "load_unit");
-}
+
 void py_gated_act(uint64_t g, uint64_t u, uint64_t h, int64_t n, int act, uint64_t stream) {
   check(gated_act(P<void>(g), P<void>(u), P<void>(h), n, act, S(stream)), "gated_act");
 }
@@ -523,11 +572,10 @@ void py_apply_update(uint64_t o, uint64_t master, uint64_t param, int64_t items,
                      uint64_t stream) {
   check(apply_update(P<float>(o), P<float>(master), P<void>(param), items, n, stride, lr, size, wd, S(stream)), "apply_update");
 }
-// alpha A A^T + beta C of a batch: items, m, k, a, out, c, alpha, beta, sms, status, stream
+// alpha A A^T + beta C of a batch [items, m, k]
 void gram(int items, int m, int k, uint64_t src, uint64_t out, uint64_t c, float alpha, float beta, int sms, uint64_t status, uint64_t stream) {
   static thread_local ProductArgs a;
-  Product& p = a.p[0];
-  p.M = p.N = m;
+  Product& p = plain_problem(a.p[0], m, m);
   p.items = items;
   p.a_item = p.b_item = m;
   const int tile_n = products_tile_n(kGram, m, m, items, sms);
@@ -539,17 +587,19 @@ void gram(int items, int m, int k, uint64_t src, uint64_t out, uint64_t c, float
   p.c = P<void>(c);
   p.alpha = alpha;
   p.beta = beta;
-  run_products(a, kGram, kNone, 1, tile_n, sms, status, stream, "gram");
+  run_products(a, kGram, kNone, 1, 1, tile_n, sms, status, stream, "gram");
 }
-// alpha X + beta B X of a batch: items, m, n, b, xs, x, xs_out, scale, alpha, beta, out (0: x and xs_out), rows, cols, item, row and column
-// strides of out, out_fp32, sms, status, stream
+struct OrthoOut {
+  uint64_t out;      // 0: x and xs_out
+  int rows, cols;    // of the result, as X lies
+  int64_t item, row, col;
+  int fp32;
+};
+// alpha X + beta B X of a batch [items, m, n]
 void ortho_step(int items, int m, int n, uint64_t b, uint64_t xs, uint64_t x, uint64_t xs_out, float scale, float alpha, float beta,
-                uint64_t out, int rows, int cols, int64_t s_item, int64_t s_row, int64_t s_col, int out_fp32, int sms, uint64_t status,
-                uint64_t stream) {
+                const OrthoOut& r, int sms, uint64_t status, uint64_t stream) {
   static thread_local ProductArgs a;
-  Product& p = a.p[0];
-  p.M = m;
-  p.N = n;
+  Product& p = plain_problem(a.p[0], m, n);
   p.items = items;
   p.a_item = p.b_item = m;
   const int tile_n = products_tile_n(kStep, m, n, items, sms);
@@ -557,20 +607,45 @@ void ortho_step(int items, int m, int n, uint64_t b, uint64_t xs, uint64_t x, ui
   const ProductOperand B{P<void>(b), m, 0, 0}, X{P<void>(xs), n, 1, rows_all};
   products_ok(product_operands(&p, kStep, tile_n, &B, &X, 1, rows_all, n, &K), "ortho_step");
   products_ok(product_output(&p, 0, P<void>(x), n, rows_all, n, true), "ortho_step");
-  if (out == 0) products_ok(product_output(&p, 1, P<void>(xs_out), n, rows_all, n, false), "ortho_step");
-  p.out = P<void>(out);
+  if (r.out == 0) products_ok(product_output(&p, 1, P<void>(xs_out), n, rows_all, n, false), "ortho_step");
+  p.out = P<void>(r.out);
   p.c = P<void>(x);
   p.scale = scale;
   p.alpha = alpha;
   p.beta = beta;
-  p.rows = rows;
-  p.cols = cols;
-  p.out_item = s_item;
-  p.out_row = s_row;
-  p.out_col = s_col;
-  p.out_fp32 = out_fp32;
+  p.rows = r.rows;
+  p.cols = r.cols;
+  p.out_item = r.item;
+  p.out_row = r.row;
+  p.out_col = r.col;
+  p.out_fp32 = r.fp32;
   order_of(p, m, tile_n);
-  run_products(a, kStep, kNone, 1, tile_n, sms, status, stream, "ortho_step");
+  run_products(a, kStep, kNone, 1, 1, tile_n, sms, status, stream, "ortho_step");
+}
+// `steps` steps of a batch of matrices [rows, cols], `stride` elements apart, in `space` (unit_space() bytes): X [m, n] in fp32, its copies
+// for the products twice, two matrices [m, m] and the partial sums of the norms.
+int64_t unit_space(int64_t m, int64_t n) { return 8 * m * n + 4 * m * m + 8 * kNormParts; }
+void orthogonalize(uint64_t g, int bf16, int64_t stride, int items, int rows, int cols, int steps, float a, float b, float c, uint64_t space, int m,
+                   int n, uint64_t out, int out_fp32, int64_t out_item, int64_t out_row, int64_t out_col, int sms, uint64_t status,
+                   uint64_t stream) {
+  // powers of two that the fp16 copies are scaled by: their largest values are below 4, 16 and 200 (what the coefficients are checked for)
+  constexpr float sx = 1024.f, sa = 1024.f, sb = 256.f;
+  const bool tall = rows > cols;
+  const int64_t count = (int64_t)rows * cols, mn = (int64_t)items * m * n, mm = (int64_t)items * m * m;
+  const uint64_t x = space, q = space + 8 * mn, p = q + 2 * mm, norms = p + 2 * mm;
+  uint64_t xs = space + 4 * mn, ys = space + 6 * mn;
+  check(square_sums(P<void>(g), bf16, items, count, stride, P<double>(norms), S(stream)), "square_sums");
+  check(load_unit({P<void>(g), bf16, stride, items, rows, cols, tall ? 1 : 0, P<double>(norms), norm_parts(count), P<float>(x), P<void>(xs), m, n, sx},
+                  S(stream)), "load_unit");
+  for (int k = 0; k < steps; ++k) {
+    const bool last = k + 1 == steps;
+    gram(items, m, n, xs, q, 0, sa / (sx * sx), 0.f, sms, status, stream);
+    gram(items, m, m, q, p, q, sb * c / (sa * sa), sb * b / sa, sms, status, stream);
+    ortho_step(items, m, n, p, xs, x, ys, sx, a, 1.f / (sb * sx),
+               {last ? out : 0, std::min(rows, cols), std::max(rows, cols), out_item, tall ? out_col : out_row, tall ? out_row : out_col, out_fp32}, sms,
+               status, stream);
+    std::swap(xs, ys);
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -776,7 +851,7 @@ PYBIND11_MODULE(_C, m) {
   m.attr("CHUNK_DESC_BYTES") = (int)sizeof(ChunkDesc);
 
   m.attr("GATED_CHUNK") = (int)kGatedChunk;
-  m.attr("NORM_PARTS") = (int)kNormParts;
+  m.def("unit_space", &unit_space, "bytes of workspace of a matrix: m, n");
   m.def("products_tile_n", &products_tile_n, "columns of a tile: kind, M, N, items, sms");
   m.attr("PRODUCT_HEAD") = (int)kHead;
 
@@ -896,24 +971,20 @@ PYBIND11_MODULE(_C, m) {
        "of either, sms, status, stream, gelu_pre"},
 #define MSB_VALUES(name, fn, n, doc) \
   {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&direct_values<&fn, n>)), METH_FASTCALL, doc}
-      MSB_VALUES("gated_fwd", gated_fwd, 19, "tokens, width, ffn, x, ldx, gate, ld, up, ld, mn_major, h, g, u, exps, act, keep, sms, status, "
-                 "stream"),
-      MSB_VALUES("gated_grad", gated_grad, 17, "tokens, ffn, outputs, dy, ld, down, ld, mn_major, g, u, exps, dg, du, act, sms, status, "
-                 "stream"),
-      MSB_VALUES("gemm_sum", gemm_sum, 19, "two products summed: M, N, K0, K1, A0, ld, A1, ld, a_mn_major, B0, ld, B1, ld, b_mn_major, C, ld, "
-                 "sms, status, stream"),
-      MSB_VALUES("head_partial", head_partial, 18, "rows, width, vocab, columns, x, ldx, w, ldw, mn_major, e, lde, stats, label, targets, "
-                 "tile_n, sms, status, stream"),
+      MSB_VALUES("gated_fwd", gated_fwd, 24, "tokens, inputs, features, outputs, x, ld, gate, ld, up, ld, up_nt, down, ld, down_nt, y, h, g, u, "
+                 "exps, act, keep, sms, status, stream"),
+      MSB_VALUES("gated_bwd", gated_bwd, 35, "tokens, inputs, features, outputs, dy, ld, x, ld, gate, ld, up, ld, up_nt, down, ld, down_nt, h, g, "
+                 "u, exps, dg, du, dx, dgate, ld, dup, ld, ddown, ld, types (bit i: fp32), accumulate, act, sms, status, stream"),
 #undef MSB_VALUES
-      MSB_DIRECT("head_rows", py_head_rows, "e, ld, stats, label, targets, rows, cols, tiles, tile_n, vocab, scale, loss, stream"),
-      MSB_DIRECT("unit_load", unit_load, "g, bf16, stride, items, rows, cols, transpose, partial, x, xs, mp, np, scale, stream"),
+      MSB_DIRECT("head_losses", head_losses, "rows, width, vocab, x, ldx, w, ldw, nt, targets, stats, label, tile_n, loss, sms, status, stream"),
+      MSB_DIRECT("head_grads", head_grads, "rows, width, vocab, columns, wide, x, ldx, w, ldw, nt, targets, scale, e, stats, label, tile_n, loss, dx, "
+                 "dw, lddw, dw_fp32, accumulate, pad, pad_pitch, pad_width, pad_height, sms, status, stream"),
+      MSB_DIRECT("orthogonalize", orthogonalize, "g, bf16, stride, items, rows, cols, steps, a, b, c, space, m, n, out, out_fp32, item, row and column "
+                 "strides of out, sms, status, stream"),
       MSB_DIRECT("gated_act", py_gated_act, "g, u, h, n, act, stream"),
       MSB_DIRECT("gated_act_bwd", py_gated_act_bwd, "dh, g, u, dg, du, n, act, stream"),
       MSB_DIRECT("momentum_step", py_momentum_step, "grad, grad_fp32, m, u, items, n, stride, momentum, nesterov, grad_scale, stream"),
       MSB_DIRECT("apply_update", py_apply_update, "o, master, param, items, n, stride, lr, size, wd, stream"),
-      MSB_DIRECT("gram", gram, "items, m, k, a, out, c, alpha, beta, sms, status, stream"),
-      MSB_DIRECT("ortho_step", ortho_step, "items, m, n, b, xs, x, xs_out, scale, alpha, beta, out, rows, cols, item, row and column strides "
-                 "of out, out_fp32, sms, status, stream"),
       MSB_DIRECT("memset_zero", memset_zero, "ptr, bytes, stream"),
       MSB_DIRECT("ln_fwd_local", ln_fwd_local, "x, res, h_out, y, gamma, beta, mean_rstd, rows, cols, eps, stream"),
       MSB_DIRECT("ln_bwd_local", ln_bwd_local, "dy, h, gamma, mean_rstd, dres, dx, dgamma, dbeta, rows, cols, stream"),

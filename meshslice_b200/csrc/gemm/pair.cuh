@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "../common/ptx.cuh"
+#include "tile_walk.h"
 
 namespace msb {
 

@@ -222,6 +222,7 @@ struct Gemm2Problem {
 struct Gemm2Args {
   Gemm2Problem p[2];
   int tiles[2];                // tiles of the first problem, of both (set by the launcher)
+  int rounds;                  // of the second problem's tiles for the pairs with fewer of the first (set by the launcher)
   uint32_t* status;            // [4]: code, blockIdx, detail, detail2
   uint64_t timeout_ns;
 };

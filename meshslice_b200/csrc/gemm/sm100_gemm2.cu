@@ -189,8 +189,7 @@ sm100_gemm2_kernel(const __grid_constant__ Gemm2Args a) {
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();      // 0: leader
   const uint64_t tmo = a.timeout_ns;
-  const int num_tiles = a.tiles[1];
-  const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+  const TileWalk first_walk(blockIdx.x >> 1, gridDim.x >> 1, a.tiles[0], a.tiles[1], a.rounds);
   // Tile t: its problem and its place in it.
   const auto place = [&](int t, bool& second, int& m2, int& nb) {
     second = t >= a.tiles[0];
@@ -237,7 +236,8 @@ sm100_gemm2_kernel(const __grid_constant__ Gemm2Args a) {
       const uint32_t full0 = mapa_u32(smem_u32(full_bar), 0);     // the leader's barriers
       uint32_t stage = 0, phase = 0;
       bool ok = true, free = true;                                // `free`: the next stage was seen empty
-      for (int t = cluster_id; t < num_tiles && ok; t += n_clusters) {
+      for (TileWalk walk = first_walk; walk.more() && ok; walk.next()) {
+        const int t = walk.t;
         bool second;
         int m2, nb;
         place(t, second, m2, nb);
@@ -282,7 +282,8 @@ sm100_gemm2_kernel(const __grid_constant__ Gemm2Args a) {
       uint32_t stage = 0, phase = 0;
       bool ok = true, full = false;                               // `full`: the next stage was seen complete
       int it = 0;
-      for (int t = cluster_id; t < num_tiles && ok; t += n_clusters, ++it) {
+      for (TileWalk walk = first_walk; walk.more() && ok; walk.next(), ++it) {
+        const int t = walk.t;
         const uint32_t acc = it & 1, acc_phase = (it >> 1) & 1;
         if (!mbar_wait(tempty_bar + acc, acc_phase ^ 1, 6 * tmo)) {
           report2(a, kTimeoutTmemEmpty, t, acc);
@@ -326,7 +327,8 @@ sm100_gemm2_kernel(const __grid_constant__ Gemm2Args a) {
     OutStage out{smem + kSmemOut2 + q * 2 * kOutBox, {0}};
     bool ok = true;
     int it = 0;
-    for (int t = cluster_id; t < num_tiles && ok; t += n_clusters, ++it) {
+    for (TileWalk walk = first_walk; walk.more() && ok; walk.next(), ++it) {
+      const int t = walk.t;
       bool second;
       int m2, nb;
       place(t, second, m2, nb);
@@ -461,14 +463,7 @@ static int64_t last_end(const Gemm2Operands* o, int problems, int tile_n, int64_
     tiles[i] = ((o[i].M + 2 * kBM - 1) / (2 * kBM)) * ((o[i].N + tile_n - 1) / tile_n);
     kb[i] = (o[i].K + kBK - 1) / kBK;
   }
-  const int64_t all = tiles[0] + tiles[1], at[3] = {0, tiles[0] % pairs, all % pairs};
-  int64_t last = 0;
-  for (int64_t i : at) {
-    const int64_t n0 = (tiles[0] - i + pairs - 1) / pairs, n = (all - i + pairs - 1) / pairs;
-    const int64_t end = n0 * kb[0] + (n - n0) * kb[1];
-    last = end > last ? end : last;
-  }
-  return last;
+  return walk_end(tiles[0], kb[0], tiles[1], kb[1], pairs);
 }
 int gemm2_tile_n(const Gemm2Operands* o, int problems, int sms) {
   const int64_t pairs = sms > 1 ? sms / 2 : 1;
@@ -523,18 +518,20 @@ int gemm2_problem(Gemm2Problem* p, const Gemm2Operands& o, int tile_n) {
 }
 
 cudaError_t launch_sm100_gemm2(Gemm2Args& args, int problems, int tile_n, int sms, cudaStream_t stream) {
-  int64_t tiles = 0;
+  int64_t tiles = 0, of[2] = {0, 0}, kb[2] = {0, 0};
   bool dgelu = false;
   for (int i = 0; i < 2; ++i) {
     if (i < problems) {
       const Gemm2Problem& p = args.p[i];
       dgelu = dgelu || p.act == 2;
-      tiles += (int64_t)((p.M + 2 * kBM - 1) / (2 * kBM)) * ((p.N + tile_n - 1) / tile_n);
+      kb[i] = (p.K + kBK - 1) / kBK;
+      tiles += of[i] = (int64_t)((p.M + 2 * kBM - 1) / (2 * kBM)) * ((p.N + tile_n - 1) / tile_n);
     }
     args.tiles[i] = (int)tiles;
   }
   int grid = (int)(2 * tiles < (sms & ~1) ? 2 * tiles : (sms & ~1));
   if (grid < 2) grid = 2;
+  args.rounds = (int)walk_rounds(of[0], kb[0], of[1], kb[1], grid / 2);
   if (dgelu) return tile_n == 128 ? launch2<128, true>(args, grid, stream) : launch2<256, true>(args, grid, stream);
   return tile_n == 128 ? launch2<128, false>(args, grid, stream) : launch2<256, false>(args, grid, stream);
 }

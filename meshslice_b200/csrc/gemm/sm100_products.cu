@@ -1,10 +1,12 @@
 // Products with an epilogue of their own.  The roles are those of the plain GEMM of CTA pairs (sm100_gemm2.cu): a TMA producer warp
-// per operand, one thread that issues every tcgen05.mma, four epilogue warps that drain one accumulator while the next tile is
+// per operand, one thread that issues every tcgen05.mma, epilogue warps that drain one accumulator while the next tile is
 // multiplied.  What differs is what the epilogue warps do with the fp32 sums, and where a tile's operands lie.
 //
-// Outputs leave in chunks of 32 rows x 32 columns: an epilogue warp stages up to 6 KiB of a chunk (three 16-bit boxes, or an fp32 and a
-// 16-bit one) and has two such sets, so that the copy engine reads one while the other is written.  That takes one of the plain
-// GEMM's pipeline stages.
+// There are eight epilogue warps, two for every 32 rows, which take half of a tile's columns each: the arithmetic of a chunk (32 rows x
+// 32 columns) is a chain of latencies, and one warp a scheduler leaves it idle.  Outputs leave chunk by chunk as TMA stores from 6 or 8 KiB
+// of staging a warp: as many sets of boxes as fit, written in turn (three 16-bit boxes, or an fp32 and a 16-bit one, are one set).  The staging
+// takes one of the plain GEMM's pipeline stages.  What an epilogue reads of memory it asks for one chunk ahead, for the first chunk
+// before the accumulator is complete.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math_constants.h>
@@ -24,11 +26,11 @@ namespace {
 constexpr uint32_t kAStageP = kBM * kBK * 2;
 constexpr uint32_t b_stage_p(int bn) { return (bn / 2) * kBK * 2; }
 constexpr uint32_t kBox16 = 32 * 64, kBox32 = 32 * 128;   // 32 x 32 of 16 and of 32 bits
-constexpr uint32_t kSet = 3 * kBox16;                     // what a chunk stages at most
-constexpr uint32_t kOutStageP = 4 * 2 * kSet;
+constexpr int kEpiWarps = 8;
+constexpr uint32_t staging(int bn) { return (bn == 256 ? 4 : 3) * kBox16; }       // of an epilogue warp
 constexpr int stages_p(int bn) { return bn == 256 ? 5 : 7; }
-constexpr uint32_t smem_alloc_p(int bn) { return stages_p(bn) * (kAStageP + b_stage_p(bn)) + kOutStageP + 256 + 1024; }
-constexpr int kThreadsP = 224;   // warps: A producer, MMA, 4x epilogue, B producer
+constexpr uint32_t smem_alloc_p(int bn) { return stages_p(bn) * (kAStageP + b_stage_p(bn)) + kEpiWarps * staging(bn) + 256 + 1024; }
+constexpr int kThreadsP = 32 * (3 + kEpiWarps);   // warps: A producer, MMA, epilogue, B producer
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void report_p(const ProductArgs& a, uint32_t code, uint32_t d0, uint32_t d1) {
@@ -50,20 +52,23 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
-// The staging of an epilogue warp: two sets of boxes, written in turn.
+// The staging of an epilogue warp: sets of `kBytes`, written in turn.
+template <uint32_t kStaging, uint32_t kBytes>
 struct ChunkStage {
+  static constexpr int kSets = kStaging / kBytes;
   uint8_t* base;
   int turn;
-  // The next set, free again: of the chunks sent so far only the last may still be read.
+  // The next set, free again: of the chunks sent so far only the last kSets - 1 may still be read.
   __device__ __forceinline__ uint8_t* take(int lane) {
-    if (lane == 0) bulk_wait_read<1>();
+    if (lane == 0) bulk_wait_read<kSets - 1>();
     __syncwarp();
-    return base + (turn & 1) * kSet;
+    uint8_t* set = base + turn * kBytes;
+    turn = turn + 1 == kSets ? 0 : turn + 1;
+    return set;
   }
   __device__ __forceinline__ void written() {
     fence_proxy_async_smem();
     __syncwarp();
-    ++turn;
   }
 };
 // 32 x 32 of 16 bits with a 64-byte swizzle, of 32 bits with a 128-byte one; a lane holds a row.
@@ -111,36 +116,51 @@ __device__ __forceinline__ uint32_t shared_exponent(const float (&v)[32]) {
 __device__ __forceinline__ float to_shared(uint32_t e) { return __uint_as_float((268u - e) << 23); }     // 2^(141 - e)
 __device__ __forceinline__ float from_shared(uint32_t e) { return __uint_as_float((e - 14u) << 23); }    // 2^(e - 141)
 
-// What an epilogue warp knows of its tile.
+// What an epilogue warp knows of its tile, and the half of the columns that is its own.
 struct TileAt {
   int item, m2, nb;        // item of the batch, 256-row block, column block
   int row0;                // first of this warp's 32 rows, in the item
-  uint32_t taddr;          // its accumulator
-  uint32_t drained;        // barrier to arrive at once it has been read
+  int half;
+  uint32_t taddr;          // the accumulator of its rows
+  uint64_t* full;          // the accumulator is complete
+  uint32_t phase;
+  uint32_t drained;        // barrier to arrive at once this warp has read it
+  uint64_t timeout_ns;
   int lane;
+
+  // Bounded; false: given up.
+  __device__ __forceinline__ bool wait() const {
+    int ok = 1;
+    if (lane == 0) ok = mbar_wait(full, phase, 7 * timeout_ns) ? 1 : 0;
+    if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
+    mbar_wait(full, phase, timeout_ns);
+    tc_fence_after_sync();
+    return true;
+  }
+  __device__ __forceinline__ void read() const {
+    tc_fence_before_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(drained);
+  }
 };
-__device__ __forceinline__ void acc_drained(const TileAt& at) {
-  tc_fence_before_sync();
-  __syncwarp();
-  if (at.lane == 0) mbar_arrive_cluster(at.drained);
-}
 __device__ __forceinline__ void send(const CUtensorMap* map, const uint8_t* box, int x, int y) { tma_store_box(map, box, x, y, false); }
 
 // ---- kGated: columns [0, BN / 2) of the accumulator are the gate, the others the up projection of the same features ----
 template <int BN>
-__device__ __forceinline__ void epilogue_gated(const Product& p, const TileAt& at, ChunkStage& out) {
-  constexpr int kChunks = BN / 2 / 32;
+__device__ __forceinline__ bool epilogue_gated(const Product& p, const TileAt& at, ChunkStage<staging(BN), 3 * kBox16>& out) {
+  constexpr int kChunks = BN / 2 / 32 / 2;                     // of this warp
   const int chunks = (p.N + 31) / 32;
+  if (!at.wait()) return false;
 #pragma unroll 1
-  for (int c = 0; c < kChunks; ++c) {
+  for (int c = at.half * kChunks; c < (at.half + 1) * kChunks; ++c) {
     float g[32], u[32];
     load_acc(at.taddr + c * 32, g);
     load_acc(at.taddr + BN / 2 + c * 32, u);
-    if (c == kChunks - 1) acc_drained(at);
+    if (c == (at.half + 1) * kChunks - 1) at.read();
     const int col0 = at.nb * (BN / 2) + c * 32;
     if (at.row0 >= p.M || col0 >= p.N) continue;
-    uint8_t* box = out.take(at.lane);
     uint32_t w[16];
+    uint8_t* box = out.take(at.lane);
     if (p.keep) {
       const uint32_t eg = shared_exponent(g), eu = shared_exponent(u);
       const float fg = to_shared(eg), fu = to_shared(eu);
@@ -153,8 +173,9 @@ __device__ __forceinline__ void epilogue_gated(const Product& p, const TileAt& a
       if (at.row0 + at.lane < p.M) p.exps[(int64_t)(at.row0 + at.lane) * chunks + (col0 >> 5)] = (uint16_t)(eg | eu << 8);
     }
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-      w[i] = pk2(g[2 * i] * gate_sigmoid(g[2 * i], p.act) * u[2 * i], g[2 * i + 1] * gate_sigmoid(g[2 * i + 1], p.act) * u[2 * i + 1]);
+    for (int i = 0; i < 32; ++i) u[i] *= g[i] * gate_sigmoid(g[i], p.act);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = pk2(u[2 * i], u[2 * i + 1]);
     stage16(box, at.lane, w);
     out.written();
     if (at.lane == 0) {
@@ -166,11 +187,13 @@ __device__ __forceinline__ void epilogue_gated(const Product& p, const TileAt& a
       bulk_commit();
     }
   }
+  return true;
 }
 
 // ---- kGatedGrad: the accumulator is dh; du = dh act(g), dg = dh u act'(g) ----
 template <int BN>
-__device__ __forceinline__ void epilogue_gated_grad(const Product& p, const TileAt& at, ChunkStage& out) {
+__device__ __forceinline__ bool epilogue_gated_grad(const Product& p, const TileAt& at, ChunkStage<staging(BN), 2 * kBox16>& out) {
+  constexpr int kChunks = BN / 32 / 2;
   const int chunks = (p.N + 31) / 32;
   const int64_t row = at.row0 + at.lane;
   const bool live = row < p.M;
@@ -181,13 +204,15 @@ __device__ __forceinline__ void epilogue_gated_grad(const Product& p, const Tile
     load_row16(reinterpret_cast<const __half*>(p.u) + row * p.N + col0, nvalid, xu);
     e = nvalid > 0 ? p.exps[row * chunks + (col0 >> 5)] : 0x1010u;
   };
-  ask(at.nb * BN);
+  const int first = at.nb * BN + at.half * (BN / 2);
+  ask(first);
+  if (!at.wait()) return false;
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
+  for (int c = 0; c < kChunks; ++c) {
     float v[32];
-    load_acc(at.taddr + c * 32, v);
-    if (c == BN / 32 - 1) acc_drained(at);
-    const int col0 = at.nb * BN + c * 32;
+    load_acc(at.taddr + at.half * (BN / 2) + c * 32, v);
+    if (c == kChunks - 1) at.read();
+    const int col0 = first + c * 32;
     if (at.row0 >= p.M || col0 >= p.N) continue;
     const float fg = from_shared(e & 255u), fu = from_shared(e >> 8);
     uint32_t wg[16], wu[16];
@@ -199,7 +224,7 @@ __device__ __forceinline__ void epilogue_gated_grad(const Product& p, const Tile
       wu[i] = pk2(v[2 * i] * g.x * s0, v[2 * i + 1] * g.y * s1);
       wg[i] = pk2(v[2 * i] * u.x * gate_slope(g.x, s0, p.act), v[2 * i + 1] * u.y * gate_slope(g.y, s1, p.act));
     }
-    if (c + 1 < BN / 32 && col0 + 32 < p.N) ask(col0 + 32);      // one chunk ahead
+    if (c + 1 < kChunks && col0 + 32 < p.N) ask(col0 + 32);
     uint8_t* box = out.take(at.lane);
     stage16(box, at.lane, wg);
     stage16(box + kBox16, at.lane, wu);
@@ -210,53 +235,79 @@ __device__ __forceinline__ void epilogue_gated_grad(const Product& p, const Tile
       bulk_commit();
     }
   }
+  return true;
 }
 
-// ---- kPlain ----
+// ---- kPlain: bf16 or fp32, stored or added to what is there ----
 template <int BN>
-__device__ __forceinline__ void epilogue_plain(const Product& p, const TileAt& at, ChunkStage& out) {
+__device__ __forceinline__ bool epilogue_plain(const Product& p, const TileAt& at, ChunkStage<staging(BN), kBox32>& out) {
+  constexpr int kChunks = BN / 32 / 2;
+  const int64_t row = at.row0 + at.lane;
+  const bool read = p.accumulate && !p.out_fp32;               // the copy engine adds fp32 values; bf16 ones are added before the rounding
+  const int first = at.nb * BN + at.half * (BN / 2);
+  uint32_t x[16];
+  const auto ask = [&](int col0) {
+    load_row16(reinterpret_cast<const __nv_bfloat16*>(p.c) + row * p.ldc + col0, read && row < p.M ? p.N - col0 : 0, x);
+  };
+  ask(first);
+  if (!at.wait()) return false;
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
+  for (int c = 0; c < kChunks; ++c) {
     float v[32];
-    load_acc(at.taddr + c * 32, v);
-    if (c == BN / 32 - 1) acc_drained(at);
-    const int col0 = at.nb * BN + c * 32;
+    load_acc(at.taddr + at.half * (BN / 2) + c * 32, v);
+    if (c == kChunks - 1) at.read();
+    const int col0 = first + c * 32;
     if (at.row0 >= p.M || col0 >= p.N) continue;
-    uint32_t w[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) w[i] = pk2(v[2 * i], v[2 * i + 1]);
     uint8_t* box = out.take(at.lane);
-    stage16(box, at.lane, w);
+    if (p.out_fp32) {
+      stage32(box, at.lane, v);
+    } else {
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) w[i] = read ? pk2(v[2 * i] + blo(x[i]), v[2 * i + 1] + bhi(x[i])) : pk2(v[2 * i], v[2 * i + 1]);
+      if (read && c + 1 < kChunks) ask(col0 + 32);
+      stage16(box, at.lane, w);
+    }
     out.written();
     if (at.lane == 0) {
-      send(&p.o[0], box, col0, at.row0);
+      tma_store_box(&p.o[0], box, col0, at.row0, p.out_fp32 && p.accumulate);
       bulk_commit();
     }
   }
+  return true;
 }
 
-// ---- kHead: a row's maximum over the tile's columns of the vocabulary, then its exponentials relative to that, which fp16 holds with
+// ---- kHead: a row's maximum over this warp's columns of the vocabulary, then its exponentials relative to that, which fp16 holds with
 // 11 significant bits down to 2^-14 of the largest (in bf16 the second rounding, of the probabilities, would add to a first as large) ----
 template <int BN>
-__device__ __forceinline__ void epilogue_head(const Product& p, const TileAt& at, ChunkStage& out) {
+__device__ __forceinline__ bool epilogue_head(const Product& p, const TileAt& at, ChunkStage<staging(BN), kBox16>& out) {
+  constexpr int kChunks = BN / 32 / 2;
   const int row = at.row0 + at.lane;
-  const int first = at.nb * BN, valid = min(BN, p.vocab - first);      // may be negative: a tile of padding
+  const int first = at.nb * BN + at.half * (BN / 2);
+  const int valid = min(BN / 2, p.vocab - first);              // may be negative: padding alone
+  const uint32_t taddr = at.taddr + at.half * (BN / 2);
   const bool live = at.row0 < p.M;
   int64_t y = -1;
   if (row < p.M) {
     const int64_t t = p.targets[row];
     y = t >= 0 && t < p.vocab ? t - first : -1;
   }
+  if (!at.wait()) return false;
   float m = -CUDART_INF_F;
   if (live) {
 #pragma unroll 1
-    for (int c = 0; c < BN / 32; ++c) {
+    for (int c = 0; c < kChunks; ++c) {
       if (c * 32 >= valid) break;
       float v[32];
-      load_acc(at.taddr + c * 32, v);
+      load_acc(taddr + c * 32, v);
       if (valid - c * 32 >= 32) {
+        float a = fmaxf(v[0], v[1]), b = fmaxf(v[2], v[3]);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) m = fmaxf(m, v[i]);
+        for (int i = 4; i < 32; i += 4) {
+          a = fmaxf(a, fmaxf(v[i], v[i + 1]));
+          b = fmaxf(b, fmaxf(v[i + 2], v[i + 3]));
+        }
+        m = fmaxf(m, fmaxf(a, b));
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i) m = c * 32 + i < valid ? fmaxf(m, v[i]) : m;
@@ -272,69 +323,69 @@ __device__ __forceinline__ void epilogue_head(const Product& p, const TileAt& at
   const float ref = m == -CUDART_INF_F ? 0.f : m;               // nothing above -inf: exponentials of zero, not of NaN
   float s = 0.f;
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
+  for (int c = 0; c < kChunks; ++c) {
     const int col0 = first + c * 32;
-    const bool wanted = live && (c * 32 < valid || (p.write && col0 < p.N));
-    if (wanted) {
-      float v[32];
-      load_acc(at.taddr + c * 32, v);
+    if (!live || !(c * 32 < valid || (p.write && col0 < p.N))) break;
+    float v[32];
+    load_acc(taddr + c * 32, v);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = ex2((v[i] - ref) * kLog2e);   // the difference first: logits down to the type's lowest value
-      if (valid - c * 32 < 32) {
+    for (int i = 0; i < 32; ++i) v[i] = ex2((v[i] - ref) * kLog2e);   // the difference first: logits down to the type's lowest value
+    if (valid - c * 32 < 32) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = c * 32 + i < valid ? v[i] : 0.f;
-      }
+      for (int i = 0; i < 32; ++i) v[i] = c * 32 + i < valid ? v[i] : 0.f;
+    }
+    float part[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) s += (v[i] + v[i + 1]) + (v[i + 2] + v[i + 3]);
-      if (p.write) {
-        uint32_t w[16];
+    for (int i = 0; i < 32; ++i) part[i & 3] += v[i];
+    s += (part[0] + part[1]) + (part[2] + part[3]);
+    if (p.write) {
+      uint32_t w[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) w[i] = pkh(v[2 * i], v[2 * i + 1]);
-        uint8_t* box = out.take(at.lane);
-        stage16(box, at.lane, w);
-        out.written();
-        if (at.lane == 0) {
-          send(&p.o[0], box, col0, at.row0);
-          bulk_commit();
-        }
+      for (int i = 0; i < 16; ++i) w[i] = pkh(v[2 * i], v[2 * i + 1]);
+      uint8_t* box = out.take(at.lane);
+      stage16(box, at.lane, w);
+      out.written();
+      if (at.lane == 0) {
+        send(&p.o[0], box, col0, at.row0);
+        bulk_commit();
       }
     }
   }
-  acc_drained(at);
-  if (row < p.M) p.stats[(int64_t)at.nb * p.M + row] = make_float2(m, s);
+  at.read();
+  if (row < p.M && first < p.N) p.stats[(int64_t)(2 * at.nb + at.half) * p.M + row] = make_float2(m, s);
+  return true;
 }
 
 // ---- kGram: alpha acc + beta C in fp16; below the diagonal the tile is written a second time, mirrored ----
 template <int BN>
-__device__ __forceinline__ void epilogue_gram(const Product& p, const TileAt& at, ChunkStage& out) {
+__device__ __forceinline__ bool epilogue_gram(const Product& p, const TileAt& at, ChunkStage<staging(BN), kBox16>& out) {
+  constexpr int kChunks = BN / 32 / 2;
   const int64_t item0 = (int64_t)at.item * p.M;
   const int row = at.row0 + at.lane;
   const bool mirror = at.nb * BN + BN <= at.m2 * 2 * kBM;      // the tile has nothing on the diagonal
   __half* const whole = reinterpret_cast<__half*>(p.out) + item0 * p.M;
+  const int first = at.nb * BN + at.half * (BN / 2);
+  uint32_t x[16];
+  const auto ask = [&](int col0) {
+    const int nvalid = p.c != nullptr && at.row0 < p.M ? p.M - col0 : 0;
+    load_row16(reinterpret_cast<const __half*>(p.c) + (item0 + row) * p.M + col0, nvalid, x);
+  };
+  ask(first);
+  if (!at.wait()) return false;
 #pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
-    const int col0 = at.nb * BN + c * 32;
-    const bool live = at.row0 < p.M && col0 < p.M;
-    uint32_t x[16];
-    if (live && p.c != nullptr) load_row16(reinterpret_cast<const __half*>(p.c) + (item0 + row) * p.M + col0, p.M - col0, x);
+  for (int c = 0; c < kChunks; ++c) {
+    const int col0 = first + c * 32;
     float v[32];
-    load_acc(at.taddr + c * 32, v);
-    if (c == BN / 32 - 1) acc_drained(at);
-    if (!live) continue;
+    load_acc(at.taddr + at.half * (BN / 2) + c * 32, v);
+    if (c == kChunks - 1) at.read();
+    if (at.row0 >= p.M || col0 >= p.M) continue;
     uint32_t w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float2 t = p.c != nullptr ? unh(x[i]) : make_float2(0.f, 0.f);
+      const float2 t = unh(x[i]);
       w[i] = pkh(fmaf(p.beta, t.x, p.alpha * v[2 * i]), fmaf(p.beta, t.y, p.alpha * v[2 * i + 1]));
     }
-    if (mirror) {
-      unsigned short* at_t = reinterpret_cast<unsigned short*>(whole) + (int64_t)col0 * p.M + row;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        at_t[(int64_t)(2 * i) * p.M] = (unsigned short)(w[i] & 0xffffu);
-        at_t[(int64_t)(2 * i + 1) * p.M] = (unsigned short)(w[i] >> 16);
-      }
-    }
+    if (c + 1 < kChunks) ask(col0 + 32);
     uint8_t* box = out.take(at.lane);
     stage16(box, at.lane, w);
     out.written();
@@ -342,28 +393,44 @@ __device__ __forceinline__ void epilogue_gram(const Product& p, const TileAt& at
       send(&p.o[0], box, col0, (int)item0 + at.row0);
       bulk_commit();
     }
+    if (mirror) {
+      unsigned short* to = reinterpret_cast<unsigned short*>(whole) + (int64_t)col0 * p.M + row;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        to[(int64_t)(2 * i) * p.M] = (unsigned short)(w[i] & 0xffffu);
+        to[(int64_t)(2 * i + 1) * p.M] = (unsigned short)(w[i] >> 16);
+      }
+    }
   }
+  return true;
 }
 
 // ---- kStep: alpha X + beta acc ----
 template <int BN>
-__device__ __forceinline__ void epilogue_step(const Product& p, const TileAt& at, ChunkStage& out) {
+__device__ __forceinline__ bool epilogue_step(const Product& p, const TileAt& at, ChunkStage<staging(BN), kBox32 + kBox16>& out) {
+  constexpr int kChunks = BN / 32 / 2;
   const int64_t item0 = (int64_t)at.item * p.M;
   const int row = at.row0 + at.lane;
-#pragma unroll 1
-  for (int c = 0; c < BN / 32; ++c) {
-    const int col0 = at.nb * BN + c * 32;
-    const bool live = at.row0 < p.M && col0 < p.N;             // M and N are multiples of 64: whole chunks
-    float4 x[8];
-    if (live) {
-      const float4* from = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p.c) + (item0 + row) * p.N + col0);
+  const int first = at.nb * BN + at.half * (BN / 2);
+  float4 x[8];
+  const auto ask = [&](int col0) {                               // M and N are multiples of 64: whole chunks
+    if (at.row0 >= p.M || col0 >= p.N) return;
+    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.c) + (item0 + row) * p.N + col0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = from[i];
+    for (int i = 0; i < 8; ++i) {
+      const uint4 u = ld_stream(from + i);
+      x[i] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
     }
+  };
+  ask(first);
+  if (!at.wait()) return false;
+#pragma unroll 1
+  for (int c = 0; c < kChunks; ++c) {
+    const int col0 = first + c * 32;
     float v[32];
-    load_acc(at.taddr + c * 32, v);
-    if (c == BN / 32 - 1) acc_drained(at);
-    if (!live) continue;
+    load_acc(at.taddr + at.half * (BN / 2) + c * 32, v);
+    if (c == kChunks - 1) at.read();
+    if (at.row0 >= p.M || col0 >= p.N) continue;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       v[4 * i] = fmaf(p.alpha, x[i].x, p.beta * v[4 * i]);
@@ -371,6 +438,7 @@ __device__ __forceinline__ void epilogue_step(const Product& p, const TileAt& at
       v[4 * i + 2] = fmaf(p.alpha, x[i].z, p.beta * v[4 * i + 2]);
       v[4 * i + 3] = fmaf(p.alpha, x[i].w, p.beta * v[4 * i + 3]);
     }
+    if (c + 1 < kChunks) ask(col0 + 32);
     if (p.out == nullptr) {
       uint32_t w[16];
 #pragma unroll
@@ -413,16 +481,22 @@ __device__ __forceinline__ void epilogue_step(const Product& p, const TileAt& at
       }
     }
   }
+  return true;
 }
 
+// Bytes of a chunk's boxes.
+constexpr uint32_t set_bytes(int kind) {
+  return kind == kGated || kind == kStep ? 3 * kBox16 : kind == kGatedGrad || kind == kPlain ? 2 * kBox16 : kBox16;
+}
 template <int Kind, int BN>
-__device__ __forceinline__ void epilogue(const Product& p, const TileAt& at, ChunkStage& out) {
-  if constexpr (Kind == kGated) epilogue_gated<BN>(p, at, out);
-  if constexpr (Kind == kGatedGrad) epilogue_gated_grad<BN>(p, at, out);
-  if constexpr (Kind == kPlain) epilogue_plain<BN>(p, at, out);
-  if constexpr (Kind == kHead) epilogue_head<BN>(p, at, out);
-  if constexpr (Kind == kGram) epilogue_gram<BN>(p, at, out);
-  if constexpr (Kind == kStep) epilogue_step<BN>(p, at, out);
+__device__ __forceinline__ bool epilogue(const Product& p, const TileAt& at, ChunkStage<staging(BN), set_bytes(Kind)>& out) {
+  if constexpr (Kind == kGated) return epilogue_gated<BN>(p, at, out);
+  if constexpr (Kind == kGatedGrad) return epilogue_gated_grad<BN>(p, at, out);
+  if constexpr (Kind == kPlain) return epilogue_plain<BN>(p, at, out);
+  if constexpr (Kind == kHead) return epilogue_head<BN>(p, at, out);
+  if constexpr (Kind == kGram) return epilogue_gram<BN>(p, at, out);
+  if constexpr (Kind == kStep) return epilogue_step<BN>(p, at, out);
+  return false;
 }
 
 // Blocks of columns of an item: tiles of kGated have gate and up of half as many features.
@@ -466,7 +540,7 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
   constexpr uint32_t kSmemOut = kSmemB + kStagesP * kBStageP;
   uint8_t* sA = smem;
   uint8_t* sB = smem + kSmemB;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kSmemOut + kOutStageP);    // [kStagesP], used in the leader
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kSmemOut + kEpiWarps * staging(BN));    // [kStagesP], used in the leader
   uint64_t* empty_bar = full_bar + kStagesP;     // [kStagesP], one set per CTA
   uint64_t* tfull_bar = empty_bar + kStagesP;    // [2], one set per CTA
   uint64_t* tempty_bar = tfull_bar + 2;          // [2], used in the leader
@@ -475,8 +549,7 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();      // 0: leader
   const uint64_t tmo = a.timeout_ns;
-  const int num_tiles = a.tiles[2];
-  const int cluster_id = blockIdx.x >> 1, n_clusters = gridDim.x >> 1;
+  const TileWalk first_walk(blockIdx.x >> 1, gridDim.x >> 1, a.lead, a.tiles[2], a.rounds);
   // Tile t: its problem and its place in it.
   const auto where = [&](int t, int& which, int& item, int& m2, int& nb) {
     which = 0;
@@ -494,7 +567,7 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(tfull_bar + i, 1);
-      mbar_init(tempty_bar + i, 8);  // a lane of each epilogue warp of both CTAs
+      mbar_init(tempty_bar + i, 2 * kEpiWarps);  // a lane of each epilogue warp of both CTAs
     }
     mbar_fence_init();
   }
@@ -509,14 +582,15 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
   grid_trigger();
   grid_wait();
 
-  if (warp == 0 || warp == 6) {
-    // ===================== TMA producers (both CTAs): warp 0 loads A, warp 6 loads B ==========
+  if (warp == 0 || warp == 2 + kEpiWarps) {
+    // ===================== TMA producers (both CTAs): warp 0 loads A, the last one B ==========
     if (elect_one()) {
       const bool is_a = warp == 0;
       const uint32_t full0 = mapa_u32(smem_u32(full_bar), 0);     // the leader's barriers
       uint32_t stage = 0, phase = 0;
       bool ok = true, free = true;                                // `free`: the next stage was seen empty
-      for (int t = cluster_id; t < num_tiles && ok; t += n_clusters) {
+      for (TileWalk walk = first_walk; walk.more() && ok; walk.next()) {
+        const int t = walk.t;
         int which, item, m2, nb;
         where(t, which, item, m2, nb);
         const Product& p = a.p[which];
@@ -559,7 +633,8 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
       uint32_t stage = 0, phase = 0;
       bool ok = true, full = false;                               // `full`: the next stage was seen complete
       int it = 0;
-      for (int t = cluster_id; t < num_tiles && ok; t += n_clusters, ++it) {
+      for (TileWalk walk = first_walk; walk.more() && ok; walk.next(), ++it) {
+        const int t = walk.t;
         const uint32_t acc = it & 1, acc_phase = (it >> 1) & 1;
         if (!mbar_wait(tempty_bar + acc, acc_phase ^ 1, 6 * tmo)) {
           report_p(a, kTimeoutTmemEmpty, t, acc);
@@ -598,26 +673,36 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
     }
   } else {
     // ===================== epilogue (both CTAs, own 128 rows) =====================
-    const int q = warp & 3;
-    ChunkStage out{smem + kSmemOut + q * 2 * kSet, 0};
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    // a warp's chunks of either kind, in the same staging: all of one problem's are read before the next one's first is written
+    uint8_t* const boxes = smem + kSmemOut + (warp - 2) * staging(BN);
+    ChunkStage<staging(BN), set_bytes(K0)> out0{boxes, 0};
+    ChunkStage<staging(BN), set_bytes(K1 == kNone ? K0 : K1)> out1{boxes, 0};
+    int last = 0;
     int it = 0;
-    for (int t = cluster_id; t < num_tiles; t += n_clusters, ++it) {
+    for (TileWalk walk = first_walk; walk.more(); walk.next(), ++it) {
+      const int t = walk.t;
       int which, item, m2, nb;
       where(t, which, item, m2, nb);
       const uint32_t acc = it & 1, acc_phase = (it >> 1) & 1;
-      int okw = 1;
-      if (lane == 0) okw = mbar_wait(tfull_bar + acc, acc_phase, 7 * tmo) ? 1 : 0;
-      okw = __shfl_sync(0xffffffffu, okw, 0);
-      if (!okw) {
+      const TileAt at{item, m2, nb, (2 * m2 + (int)rank) * kBM + q * 32, half,
+                      tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, tfull_bar + acc, acc_phase,
+                      mapa_u32(smem_u32(tempty_bar + acc), 0), tmo, lane};
+      bool done;
+      if (K1 == kNone || which == 0) {
+        done = epilogue<K0, BN>(a.p[0], at, out0);
+      } else {
+        if (last == 0) {
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+        }
+        done = epilogue<K1 == kNone ? K0 : K1, BN>(a.p[which], at, out1);
+      }
+      last = which;
+      if (!done) {
         if (lane == 0) report_p(a, kTimeoutTmemFull, t, acc);
         break;
       }
-      mbar_wait(tfull_bar + acc, acc_phase, tmo);
-      tc_fence_after_sync();
-      const TileAt at{item, m2, nb, (2 * m2 + (int)rank) * kBM + q * 32, tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN,
-                      mapa_u32(smem_u32(tempty_bar + acc), 0), lane};
-      if (K1 == kNone || which == 0) epilogue<K0, BN>(a.p[0], at, out);
-      else epilogue<K1, BN>(a.p[which], at, out);
     }
     if (lane == 0) bulk_wait_all<0>();
   }
@@ -682,7 +767,7 @@ int64_t product_tiles(const Product& p, int kind, int tile_n) {
   return p.items * tm * ((p.N + cols - 1) / cols);
 }
 
-cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problems, int tile_n, int sms, cudaStream_t stream) {
+cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problems, int longer, int tile_n, int sms, cudaStream_t stream) {
   int64_t tiles = 0;
   for (int i = 0; i < 3; ++i) {
     if (i < problems) tiles += product_tiles(args.p[i], i == 0 ? k0 : k1, tile_n);
@@ -691,12 +776,16 @@ cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problem
   }
   if (tiles == 0) return cudaSuccess;
   const int most = sms & ~1, grid = (int)(2 * tiles < most ? 2 * tiles : most);
+  const auto kblocks = [&](int i) { return (int64_t)args.p[i].kblocks[0] + args.p[i].kblocks[1]; };
+  args.lead = args.tiles[longer - 1];
+  args.rounds = longer == problems ? 0 : (int)walk_rounds(args.lead, kblocks(0), args.tiles[2] - args.lead, kblocks(longer), grid / 2);
 #define MSB_PRODUCTS(A, B)                                                                           \
   if (k0 == A && k1 == B)                                                                            \
     return tile_n == 128 ? launch_as<A, B, 128>(args, grid, stream) : launch_as<A, B, 256>(args, grid, stream);
   MSB_PRODUCTS(kGated, kNone)
-  MSB_PRODUCTS(kGatedGrad, kNone)
-  MSB_PRODUCTS(kPlain, kNone)
+  MSB_PRODUCTS(kGatedGrad, kPlain)
+  MSB_PRODUCTS(kPlain, kGatedGrad)
+  MSB_PRODUCTS(kPlain, kPlain)
   MSB_PRODUCTS(kHead, kNone)
   MSB_PRODUCTS(kGram, kNone)
   MSB_PRODUCTS(kStep, kNone)

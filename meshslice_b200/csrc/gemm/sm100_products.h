@@ -1,7 +1,7 @@
 // Local products whose epilogue is more than a conversion, on the tcgen05 core of the plain GEMM (CTA pairs, 256-row tiles):
 //   kGated       h = act(x Wg) * (x Wu), and what its gradient needs
 //   kGatedGrad   dg, du from dh = dy Wd^T
-//   kPlain       C = A0 B0 (+ A1 B1), bf16
+//   kPlain       C (+)= A0 B0 (+ A1 B1), bf16 or fp32
 //   kHead        logits of a tile as statistics and exponentials relative to the tile's maximum
 //   kGram        alpha A A^T + beta C of a batch, symmetric: half of the tiles, mirrored (fp16)
 //   kStep        a X + gamma B X of a batch (fp32, with an fp16 copy, or the last one as the result)
@@ -33,23 +33,27 @@ struct Product {
   const void* u;
   uint16_t* exps;              // [M, chunks]: exponents of gate (low byte) and up
   // ---- kHead ----
-  float2* stats;               // [tiles_n, M]: maximum, sum of exp(z - maximum)
+  float2* stats;               // [2 tiles_n, M], of each half of a tile's columns: maximum, sum of exp(z - maximum)
   float* label;                // [M]: the label's logit, where there is one
   const int64_t* targets;
   int vocab;
   int write;                   // exponentials are written
-  // ---- kGram, kStep ----
+  // ---- kPlain ----
+  int accumulate;              // add to what is there: c (bf16) is read, fp32 is added by the copy engine
+  int64_t ldc;
+  // ---- kPlain, kGram, kStep ----
   void* out;                   // kGram: fp16 [items, M, M]; kStep: the last step's result, or null
-  const void* c;               // kGram: fp16 [items, M, M] or null; kStep: X in fp32 [items, M, N]
+  const void* c;               // kPlain: the output; kGram: fp16 [items, M, M] or null; kStep: X in fp32 [items, M, N]
   float alpha, beta;
   float scale;                 // kStep: of the fp16 copy
   int rows, cols;              // kStep: extent of the result that is wanted
   int64_t out_item, out_row, out_col;   // its strides in elements, one of the last two 1
-  int out_fp32;
+  int out_fp32;                // kPlain too
 };
 struct ProductArgs {
   Product p[3];
-  int tiles[3];                // tiles of the first problem, of the first two, of all
+  int tiles[3];                // tiles of the first problem, of the first two, of all (set by the launcher)
+  int lead, rounds;            // tiles of the longer contraction, and of tile_walk.h (set by the launcher)
   uint32_t* status;            // [4]: code, blockIdx, detail, detail2
   uint64_t timeout_ns;
 };
@@ -71,8 +75,9 @@ int product_output(Product* p, int which, const void* base, int64_t cols, int64_
 // Tiles of a problem.
 int64_t product_tiles(const Product& p, int kind, int tile_n);
 
-// `problems` problems: the first of kind k0, the others of kind k1, on at most `sms` SMs.  Supported: (kGated, kNone), (kGatedGrad, kNone),
-// (kGatedGrad, kPlain), (kPlain, kPlain), (kHead, kNone), (kGram, kNone), (kStep, kNone).
-cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problems, int tile_n, int sms, cudaStream_t stream);
+// `problems` problems: the first of kind k0, the others of kind k1, on at most `sms` SMs.  The first `longer` of them have one contraction, not
+// shorter than the one of the others.  Supported: kGated, kHead, kGram, kStep alone (k1 kNone); (kGatedGrad, kPlain), (kPlain, kGatedGrad),
+// (kPlain, kPlain).
+cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problems, int longer, int tile_n, int sms, cudaStream_t stream);
 
 }  // namespace msb

@@ -20,19 +20,29 @@ import torch
 
 from .. import _native
 from . import rows
-from .gemm import gemm, gemm_pair, sm_count
+from .gemm import _SM_COUNT, sm_count
 
 ACTS = {"silu": 0, "gelu": 1}
 _LAYOUTS = ("nn", "nt")
+_BF16, _F32 = torch.bfloat16, torch.float32
 
 
 @dataclass
 class GatedSaved:
-    """What a forward pass keeps for the backward one: h, and gate and up (on a GPU fp16 with an exponent for 32 features)."""
-    h: torch.Tensor
-    gate: torch.Tensor
-    up: torch.Tensor
-    exponents: Optional[torch.Tensor] = None
+    """What a forward pass keeps for the backward one: h, gate and up.  On a GPU in one block of bytes: h (bf16), gate and up (fp16 beside an
+    exponent for 32 features), the exponents."""
+    tokens: int
+    features: int
+    device: torch.device
+    block: Optional[torch.Tensor] = None
+    h: Optional[torch.Tensor] = None
+    gate: Optional[torch.Tensor] = None
+    up: Optional[torch.Tensor] = None
+
+
+def _plain(t, device: int) -> bool:
+    """A matrix that the kernels can address as it lies, on GPU ``device``."""
+    return t.dtype is _BF16 and t.dim() == 2 and t.is_contiguous() and t.get_device() == device and t.data_ptr() & 15 == 0
 
 
 def _sizes(x, w_gate, w_up, w_down, act: str, up_layout: str, down_layout: str) -> Tuple[int, int, int, int]:
@@ -49,13 +59,14 @@ def _sizes(x, w_gate, w_up, w_down, act: str, up_layout: str, down_layout: str) 
     if w_up.shape != w_gate.shape or i != d or j != f:
         raise ValueError(f"shapes do not fit: x {tuple(x.shape)}, gate {tuple(w_gate.shape)}, up {tuple(w_up.shape)} ({up_layout}), "
                          f"down {tuple(w_down.shape)} ({down_layout})")
-    if min(d, f, o) < 1:
+    if d < 1 or f < 1 or o < 1:
         raise ValueError(f"inputs, features and outputs must not be empty (got {d}, {f}, {o})")
+    dtype, at = x.dtype, x.get_device()
     for t in (w_gate, w_up, w_down):
-        if t.device != x.device or t.dtype != x.dtype:
+        if t.dtype is not dtype or t.get_device() != at:
             raise ValueError(f"x is {x.dtype} on {x.device}, a weight {t.dtype} on {t.device}")
     if x.is_cuda:
-        if x.dtype != torch.bfloat16:
+        if dtype is not _BF16:
             raise ValueError(f"the gated kernels need bf16 (got {x.dtype})")
         if d % 8 or f % 8 or o % 8:
             raise ValueError(f"the gated kernels need multiples of 8 features (got {d}, {f}, {o})")
@@ -63,6 +74,12 @@ def _sizes(x, w_gate, w_up, w_down, act: str, up_layout: str, down_layout: str) 
             raise ValueError(f"the gated kernels take fewer than 2^31 tokens (got {n})")
         _native.check_device(x)
     return n, d, f, o
+
+
+def _reachable(*tensors):
+    """The tensors, those that the kernels cannot address as copies."""
+    at = tensors[0].get_device()
+    return tensors if all(_plain(t, at) for t in tensors) else tuple(rows.as_aligned(t) for t in tensors)
 
 
 def gated_ff_fwd(x, w_gate, w_up, w_down, act: str = "silu", up_layout: str = "nn", down_layout: str = "nn", keep: bool = True):
@@ -73,18 +90,20 @@ def gated_ff_fwd(x, w_gate, w_up, w_down, act: str = "silu", up_layout: str = "n
         g, u = (xf @ (w.float() if up_layout == "nn" else w.float().T) for w in (w_gate, w_up))
         h = _act(g, act)[0] * u
         y = h @ (w_down.float() if down_layout == "nn" else w_down.float().T)
-        return y.to(x.dtype), GatedSaved(h, g, u) if keep else None
-    new = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=x.device)
-    h, y = new(x.dtype, n, f), new(x.dtype, n, o)
-    saved = GatedSaved(h, new(torch.float16, n, f), new(torch.float16, n, f), new(torch.int16, n, -(-f // _native.load().GATED_CHUNK))) if keep else None
+        return y.to(x.dtype), GatedSaved(n, f, x.device, h=h, gate=g, up=u) if keep else None
+    C = _native.load()
+    y = torch.empty(n, o, dtype=_BF16, device=x.device)
+    part = 2 * n * f
+    block = torch.empty(3 * part + 2 * n * -(-f // C.GATED_CHUNK) if keep else part, dtype=torch.uint8, device=x.device)
+    saved = GatedSaved(n, f, x.device, block) if keep else None
     if n == 0:
         return y, saved
-    xa, wg, wu, wd = (rows.as_aligned(t) for t in (x, w_gate, w_up, w_down))
-    p = lambda name: getattr(saved, name).data_ptr() if keep else 0
-    _native.load().gated_fwd(n, d, f, xa.data_ptr(), rows.pitch(xa), wg.data_ptr(), rows.pitch(wg), wu.data_ptr(), rows.pitch(wu),
-                             1 if up_layout == "nn" else 0, h.data_ptr(), p("gate"), p("up"), p("exponents"), ACTS[act], 1 if keep else 0,
-                             sm_count(x.device), _native.status().dev, _native.stream_ptr())
-    gemm(h, wd, down_layout, out=y)
+    x, w_gate, w_up, w_down = _reachable(x, w_gate, w_up, w_down)
+    at = block.data_ptr()
+    C.gated_fwd(n, d, f, o, x.data_ptr(), rows.pitch(x), w_gate.data_ptr(), rows.pitch(w_gate), w_up.data_ptr(), rows.pitch(w_up),
+                1 if up_layout == "nt" else 0, w_down.data_ptr(), rows.pitch(w_down), 1 if down_layout == "nt" else 0, y.data_ptr(), at, at + part,
+                at + 2 * part, at + 3 * part, ACTS[act], 1 if keep else 0, _SM_COUNT.get(x.get_device()) or sm_count(x.device),
+                _native.status().dev, _native.stream_ptr())
     return y, saved
 
 
@@ -93,9 +112,9 @@ def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "sil
     """(dx, (gradients of gate, up and down weight)).  The weights' gradients are new tensors, or are added to ``grads`` (fp32 or the
     weights' type, in the weights' layouts)."""
     n, d, f, o = _sizes(x, w_gate, w_up, w_down, act, up_layout, down_layout)
-    if dy.shape != (n, o) or dy.dtype != x.dtype or dy.device != x.device:
+    if dy.shape != (n, o) or dy.dtype is not x.dtype or dy.get_device() != x.get_device():
         raise ValueError(f"dy must be {x.dtype} [{n}, {o}] on {x.device} (got {dy.dtype} {tuple(dy.shape)} on {dy.device})")
-    if saved is None or saved.h.shape != (n, f) or saved.h.device != x.device or (saved.exponents is not None) != x.is_cuda:
+    if saved is None or (saved.tokens, saved.features, saved.device) != (n, f, x.device):
         raise ValueError("the backward pass needs what the forward pass kept")
     weights = (w_gate, w_up, w_down)
     add = grads is not None
@@ -103,7 +122,7 @@ def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "sil
         if len(grads) != 3:
             raise ValueError("grads are those of gate, up and down weight")
         for g, w in zip(grads, weights):
-            if g.shape != w.shape or g.device != w.device or g.dtype not in (torch.float32, w.dtype):
+            if g.shape != w.shape or g.device != w.device or g.dtype not in (_F32, w.dtype):
                 raise ValueError(f"a gradient must be fp32 or {w.dtype} {tuple(w.shape)} on {w.device} (got {g.dtype} {tuple(g.shape)} on {g.device})")
             if x.is_cuda and not (rows.aligned(g) and rows.pitch(g) % 8 == 0):
                 raise ValueError("gradients that are added to need neighbouring columns and rows on 16-byte boundaries")
@@ -121,26 +140,25 @@ def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "sil
         for t, v in zip(grads, new):
             t += v.to(t.dtype)
         return dx, tuple(grads)
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dx = torch.empty(n, d, dtype=_BF16, device=x.device)
     if not add:
-        grads = tuple(torch.empty(w.shape, dtype=w.dtype, device=w.device) for w in weights)
+        grads = tuple(torch.empty(w.shape, dtype=_BF16, device=x.device) for w in weights)
     if n == 0:
         if not add:
             for t in grads:
                 t.zero_()
         return dx, tuple(grads)
-    xa, dya, wg, wu, wd = (rows.as_aligned(t) for t in (x, dy, *weights))
-    dg, du = torch.empty_like(saved.h), torch.empty_like(saved.h)
-    C, sms, status, stream = _native.load(), sm_count(x.device), _native.status().dev, _native.stream_ptr()
-    C.gated_grad(n, f, o, dya.data_ptr(), rows.pitch(dya), wd.data_ptr(), rows.pitch(wd), 0 if down_layout == "nn" else 1,
-                 saved.gate.data_ptr(), saved.up.data_ptr(), saved.exponents.data_ptr(), dg.data_ptr(), du.data_ptr(), ACTS[act], sms, status,
-                 stream)
-    product = lambda a, b, first: (a, b, "tn") if first else (b, a, "tn")
-    gemm(*product(saved.h, dya, down_layout == "nn"), out=grads[2], accumulate=add)
-    a0, a1 = product(xa, dg, up_layout == "nn"), product(xa, du, up_layout == "nn")
-    gemm_pair(*a0, grads[0], add, *a1, grads[1], add)
-    C.gemm_sum(n, d, f, f, dg.data_ptr(), f, du.data_ptr(), f, 0, wg.data_ptr(), rows.pitch(wg), wu.data_ptr(), rows.pitch(wu),
-               0 if up_layout == "nn" else 1, dx.data_ptr(), d, sms, status, stream)
+    dy, x, w_gate, w_up, w_down = _reachable(dy, x, *weights)
+    part = 2 * n * f
+    space = torch.empty(2 * part, dtype=torch.uint8, device=x.device)           # dg, du
+    at, to = saved.block.data_ptr(), space.data_ptr()
+    gg, gu, gd = grads
+    types = sum(1 << i for i, g in enumerate(grads) if g.dtype is _F32)
+    _native.load().gated_bwd(n, d, f, o, dy.data_ptr(), rows.pitch(dy), x.data_ptr(), rows.pitch(x), w_gate.data_ptr(), rows.pitch(w_gate),
+                             w_up.data_ptr(), rows.pitch(w_up), 1 if up_layout == "nt" else 0, w_down.data_ptr(), rows.pitch(w_down),
+                             1 if down_layout == "nt" else 0, at, at + part, at + 2 * part, at + 3 * part, to, to + part, dx.data_ptr(),
+                             gg.data_ptr(), rows.pitch(gg), gu.data_ptr(), rows.pitch(gu), gd.data_ptr(), rows.pitch(gd), types, 1 if add else 0,
+                             ACTS[act], _SM_COUNT.get(x.get_device()) or sm_count(x.device), _native.status().dev, _native.stream_ptr())
     return dx, tuple(grads)
 
 

@@ -6,7 +6,7 @@ fp32 formulation for CPU tensors.
 The weight lies as [inputs, columns] (layout 'nn') or [columns, inputs] ('nt', as an embedding table); columns from ``vocab`` on are
 padding: they have no probability and their gradient is 0.  A target outside [0, vocab) is no label: loss and gradient of the token are 0.
 
-On a GPU the product's epilogue takes the maximum of every row over the 128 or 256 columns of a tile from the fp32 sums, and the sum of
+On a GPU the product's epilogue takes the maximum of every row over half the columns of a tile, 64 or 128, from the fp32 sums, and the sum of
 the exponentials relative to it; the joined maxima and sums give the loss.  For the gradient the exponentials are kept for some rows
 at a time, become dz where they lie, and go into the two products of the gradients.
 """
@@ -18,7 +18,7 @@ import torch
 
 from .. import _native
 from . import rows as _rows
-from .gemm import gemm_pair, sm_count
+from .gemm import _SM_COUNT, sm_count
 
 PIECE_BYTES = 1 << 29      # of exponentials that are in memory at a time, unless the caller says how many rows
 
@@ -37,48 +37,44 @@ def _check(x, w, targets, vocab: int, layout: str) -> Tuple[int, int, int]:
         raise ValueError(f"the vocabulary must have a token, and at most the weight's {cols} columns (got {vocab})")
     if targets.shape != (n,) or targets.dtype != torch.int64:
         raise ValueError(f"targets must be int64 [{n}] (got {targets.dtype} {tuple(targets.shape)})")
-    if w.dtype != x.dtype or w.device != x.device or targets.device != x.device:
+    if w.dtype is not x.dtype or w.get_device() != x.get_device() or targets.get_device() != x.get_device():
         raise ValueError(f"x is {x.dtype} on {x.device}, the weight {w.dtype} on {w.device}, targets on {targets.device}")
     if x.is_cuda:
         if x.dtype != torch.bfloat16:
             raise ValueError(f"the kernels need bf16 (got {x.dtype})")
         if d % 8 or (layout == "nn" and cols % 8):
             raise ValueError(f"the kernels need rows of a multiple of 8 elements (got {d} inputs, {cols} columns, {layout})")
-        if n >= 1 << 31 or cols > 1 << 20:
-            raise ValueError(f"the kernels take fewer than 2^31 tokens and at most 2^20 columns (got {n}, {cols})")
+        if n >= 1 << 31 or vocab > 1 << 18:
+            raise ValueError(f"the kernels take fewer than 2^31 tokens and a vocabulary of at most 2^18 (got {n}, {vocab})")
         _native.check_device(x)
     return n, d, cols
 
 
-def _partial(x, w, targets, vocab: int, layout: str, e, columns: int, stats, label, tile_n: int):
-    _native.load().head_partial(x.shape[0], x.shape[1], vocab, columns, x.data_ptr(), _rows.pitch(x), w.data_ptr(), _rows.pitch(w),
-                                1 if layout == "nn" else 0, 0 if e is None else e.data_ptr(), columns, stats.data_ptr(), label.data_ptr(),
-                                targets.data_ptr(), tile_n, sm_count(x.device), _native.status().dev, _native.stream_ptr())
-
-
-def _join(e, columns: int, stats, label, targets, vocab: int, tile_n: int, scale: float, loss):
-    _native.load().head_rows(0 if e is None else e.data_ptr(), columns, stats.data_ptr(), label.data_ptr(), targets.data_ptr(),
-                             targets.shape[0], columns, stats.shape[0], tile_n, vocab, scale, loss.data_ptr(), _native.stream_ptr())
-
-
-def _plan(n: int, columns: int, device) -> int:
+def _tile_n(n: int, columns: int, sms: int) -> int:
     C = _native.load()
-    return C.products_tile_n(C.PRODUCT_HEAD, n, columns, 1, sm_count(device))
+    return C.products_tile_n(C.PRODUCT_HEAD, n, columns, 1, sms)
+
+
+def _reachable(x, w, targets):
+    return _rows.as_aligned(x), _rows.as_aligned(w), targets if targets.is_contiguous() else targets.contiguous()
 
 
 def head_loss(x, w, targets, vocab: int, layout: str = "nn") -> torch.Tensor:
     """Loss [tokens] (fp32) of ``x`` [tokens, inputs] under the head ``w``."""
-    n, _, _ = _check(x, w, targets, vocab, layout)
+    n, d, _ = _check(x, w, targets, vocab, layout)
     if not x.is_cuda:
         return _reference(x, w, targets, vocab, layout)[0]
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
     if n:
-        x, w, targets = _rows.as_aligned(x), _rows.as_aligned(w), targets.contiguous()
-        tile_n = _plan(n, vocab, x.device)
-        stats = torch.empty(-(-vocab // tile_n), n, 2, dtype=torch.float32, device=x.device)
-        label = torch.empty(n, dtype=torch.float32, device=x.device)
-        _partial(x, w, targets, vocab, layout, None, vocab, stats, label, tile_n)
-        _join(None, 0, stats, label, targets, vocab, tile_n, 0.0, loss)
+        x, w, targets = _reachable(x, w, targets)
+        sms = _SM_COUNT.get(x.get_device()) or sm_count(x.device)
+        tile_n = _tile_n(n, vocab, sms)
+        blocks = -(-vocab * 2 // tile_n)                  # statistics are of half a tile's columns
+        space = torch.empty((2 * blocks + 1) * n, dtype=torch.float32, device=x.device)
+        at = space.data_ptr()
+        _native.load().head_losses(n, d, vocab, x.data_ptr(), _rows.pitch(x), w.data_ptr(), _rows.pitch(w), 1 if layout == "nt" else 0,
+                                   targets.data_ptr(), at, at + 8 * blocks * n, tile_n, loss.data_ptr(), sms, _native.status().dev,
+                                   _native.stream_ptr())
     return loss
 
 
@@ -107,35 +103,43 @@ def head_loss_grad(x, w, targets, vocab: int, scale: float, layout: str = "nn", 
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     if n == 0:
         return loss, dx, dw if add else torch.zeros(w.shape, dtype=w.dtype, device=w.device)
-    x, w, targets = _rows.as_aligned(x), _rows.as_aligned(w), targets.contiguous()
+    x, w, targets = _reachable(x, w, targets)
+    nt = layout == "nt"
     columns = -(-vocab // 64) * 64                        # of the exponentials: zeros from vocab on
     wide = min(columns, cols)                             # those of the weight's gradient that a product writes
-    most = rows or max(256, PIECE_BYTES // (2 * columns) // 256 * 256)
-    pieces = -(-n // most)
-    piece = min(n, rows or -(-n // pieces // 256) * 256)     # equal ones, of whole tiles
-    tile_n = _plan(piece, columns, x.device)
-    e = torch.empty(piece, columns, dtype=x.dtype, device=x.device)
-    stats = torch.empty(-(-columns // tile_n) * piece * 2, dtype=torch.float32, device=x.device)
-    label = torch.empty(piece, dtype=torch.float32, device=x.device)
     if not add:
         dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
-    # sums over several pieces are held in fp32
-    total = dw if dw.dtype == torch.float32 or pieces == 1 else torch.empty(w.shape, dtype=torch.float32, device=w.device)
-    part = (lambda t: t[:, :wide]) if layout == "nn" else (lambda t: t[:wide])
-    given, known = (w[:, :vocab], "nt") if layout == "nn" else (w[:vocab], "nn")
-    for k, i in enumerate(range(0, n, piece)):
-        xi, ti = x[i:i + piece], targets[i:i + piece]
-        m = xi.shape[0]
-        ei, si = e[:m], stats[:-(-columns // tile_n) * m * 2].view(-1, m, 2)
-        _partial(xi, w, ti, vocab, layout, ei, columns, si, label, tile_n)
-        _join(ei, columns, si, label, ti, vocab, tile_n, scale, loss[i:i + piece])
-        first = (xi, ei[:, :wide], "tn") if layout == "nn" else (ei[:, :wide], xi, "tn")
-        gemm_pair(*first, part(total), k > 0 or (add and total is dw), ei[:, :vocab], given, known, dx[i:i + piece])
-    if wide < cols and not (add and total is dw):
-        (total[:, wide:] if layout == "nn" else total[wide:]).zero_()
+    # Sums over several pieces are held in fp32; where that would take a matrix of its own, as much memory is better spent on a larger piece.
+    limit = PIECE_BYTES + (0 if dw.dtype is torch.float32 else 4 * w.numel())
+    most = rows or max(256, limit // (2 * columns) // 256 * 256)
+    if not rows and most < n:
+        most = max(256, PIECE_BYTES // (2 * columns) // 256 * 256)
+    pieces = -(-n // most)
+    piece = min(n, rows or -(-n // pieces // 256) * 256)     # equal ones, of whole tiles
+    total = dw if dw.dtype is torch.float32 or piece == n else torch.empty(w.shape, dtype=torch.float32, device=w.device)
+    C, sms, status, stream = _native.load(), _SM_COUNT.get(x.get_device()) or sm_count(x.device), _native.status().dev, _native.stream_ptr()
+    tile_n = _tile_n(piece, columns, sms)
+    blocks = -(-columns * 2 // tile_n)
+    space = torch.empty((2 * columns + 8 * blocks + 4) * piece, dtype=torch.uint8, device=x.device)
+    e = space.data_ptr()
+    stats, label = e + 2 * columns * piece, e + (2 * columns + 8 * blocks) * piece
+    wide_bytes, pitch = total.element_size() * wide, _rows.pitch(total)
+    clear = wide < cols and not (add and total is dw)
+    if not clear:
+        pad = (0, 0, 0, 0)
+    elif nt:
+        pad = (total.data_ptr() + total.element_size() * wide * pitch, total.element_size() * pitch, total.element_size() * d, cols - wide)
+    else:
+        pad = (total.data_ptr() + wide_bytes, total.element_size() * pitch, total.element_size() * (cols - wide), d)
+    for i in range(0, n, piece):
+        m = min(piece, n - i)
+        C.head_grads(m, d, vocab, columns, wide, x.data_ptr() + 2 * i * _rows.pitch(x), _rows.pitch(x), w.data_ptr(), _rows.pitch(w),
+                     1 if nt else 0, targets.data_ptr() + 8 * i, scale, e, stats, label, tile_n, loss.data_ptr() + 4 * i,
+                     dx.data_ptr() + 2 * i * d, total.data_ptr(), pitch, 1 if total.dtype is torch.float32 else 0,
+                     1 if i or (add and total is dw) else 0, *(pad if i == 0 else (0, 0, 0, 0)), sms, status, stream)
     if total is not dw:
         if dw.is_contiguous() and dw.numel() % 4 == 0:
-            _native.load().cast_f32_to_bf16(total.data_ptr(), dw.data_ptr(), dw.numel(), 1 if add else 0, _native.stream_ptr())
+            C.cast_f32_to_bf16(total.data_ptr(), dw.data_ptr(), dw.numel(), 1 if add else 0, stream)
         elif add:
             dw += total
         else:

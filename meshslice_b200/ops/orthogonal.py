@@ -18,16 +18,15 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _native
-from .gemm import sm_count
+from .gemm import _SM_COUNT, sm_count
 
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 WORKSPACE_BYTES = 2 << 30       # matrices of a batch are taken some at a time beyond it
-# powers of two that the fp16 copies are scaled by: their largest values are below 4, 16 and 255 (what the coefficients are checked for)
-_SX, _SA, _SB = 2.0 ** 10, 2.0 ** 10, 2.0 ** 8
 
 
 @lru_cache(maxsize=64)
 def _check_coefficients(steps: int, coefficients: Tuple[float, float, float]):
+    """The fp16 copies of X, A and b A + c A^2 are scaled for singular values of up to 4 and a polynomial of up to 200."""
     a, b, c = coefficients
     s = [i / 1000 for i in range(1001)]
     for _ in range(steps):
@@ -71,38 +70,19 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
     if min(target.stride(1), target.stride(2)) != 1 or (r > 1 and c > 1 and target.stride(1) == target.stride(2)):
         result = torch.empty(target.shape, dtype=target.dtype, device=target.device)
     m, n = -(-min(r, c) // 64) * 64, -(-max(r, c) // 64) * 64
-    each = 8 * m * n + 4 * m * m + 8 * _native.load().NORM_PARTS
-    most = int(max(1, min(items, WORKSPACE_BYTES // each, (1 << 31) // m - 1)))
+    C, sms, status, stream = _native.load(), _SM_COUNT.get(g.get_device()) or sm_count(g.device), _native.status().dev, _native.stream_ptr()
+    each = C.unit_space(m, n)
+    most = max(1, min(items, WORKSPACE_BYTES // each, (1 << 31) // m - 1))
     space = torch.empty(most * each, dtype=torch.uint8, device=g.device)
+    stride, strides = batch.stride(0) if items > 1 else 0, (result.stride(0) if items > 1 else 0, result.stride(1), result.stride(2))
     for i in range(0, items, most):
-        _some(batch[i:i + most], result[i:i + most], int(steps), coefficients, m, n, space)
-    return out if result is target else _copied(out, target, result)
-
-
-def _copied(out, target, result):
-    target.copy_(result)
+        C.orthogonalize(batch.data_ptr() + i * stride * batch.element_size(), 1 if batch.dtype is torch.bfloat16 else 0, stride,
+                        min(most, items - i), r, c, int(steps), *coefficients, space.data_ptr(), m, n,
+                        result.data_ptr() + i * strides[0] * result.element_size(), 1 if result.dtype is torch.float32 else 0, *strides, sms,
+                        status, stream)
+    if result is not target:
+        target.copy_(result)
     return out
-
-
-def _some(g, out, steps: int, coefficients, m: int, n: int, space):
-    C, sms, status, stream = _native.load(), sm_count(g.device), _native.status().dev, _native.stream_ptr()
-    items, r, c = g.shape
-    tall = r > c
-    a, b, cc = coefficients
-    at = space.data_ptr()
-    x, xs, ys = at, at + 4 * items * m * n, at + 6 * items * m * n
-    q, p = at + 8 * items * m * n, at + 8 * items * m * n + 2 * items * m * m
-    norms = at + 8 * items * m * n + 4 * items * m * m
-    C.unit_load(g.data_ptr(), 1 if g.dtype == torch.bfloat16 else 0, g.stride(0) if items > 1 else 0, items, r, c, 1 if tall else 0, norms, x, xs,
-                m, n, _SX, stream)
-    s_row, s_col = (out.stride(2), out.stride(1)) if tall else (out.stride(1), out.stride(2))
-    for k in range(steps):
-        last = k == steps - 1
-        C.gram(items, m, n, xs, q, 0, _SA / _SX ** 2, 0.0, sms, status, stream)
-        C.gram(items, m, m, q, p, q, _SB * cc / _SA ** 2, _SB * b / _SA, sms, status, stream)
-        C.ortho_step(items, m, n, p, xs, x, ys, _SX, a, 1 / (_SB * _SX), out.data_ptr() if last else 0, min(r, c), max(r, c),
-                     out.stride(0) if items > 1 else 0, s_row, s_col, 1 if out.dtype == torch.float32 else 0, sms, status, stream)
-        xs, ys = ys, xs
 
 
 def _reference(g, steps: int, coefficients):
