@@ -28,6 +28,7 @@ CU_SOURCES = [
     "ops/attention_noalloc.cu",
     "ops/rotary.cu",
     "ops/distill.cu",
+    "ops/few_tokens.cu",
     "ops/gated.cu",
     "ops/head.cu",
     "ops/orthogonal.cu",

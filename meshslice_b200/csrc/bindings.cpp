@@ -21,6 +21,7 @@
 #include "gemm/tile_walk.h"
 #include "ops/attention.h"
 #include "ops/distill.h"
+#include "ops/few_tokens.h"
 #include "ops/gated.h"
 #include "ops/head.h"
 #include "ops/orthogonal.h"
@@ -452,6 +453,13 @@ void gated_fwd(const std::array<int64_t, 24>& v) {
   const int64_t n = v[0], d = v[1], f = v[2], o = v[3];
   const int sms = (int)v[21];
   const uint64_t status = (uint64_t)v[22], stream = (uint64_t)v[23];
+  if (n <= kFewTokens && !v[20]) {
+    const FewTokens h{P<void>(v[4]), v[5], P<void>(v[6]), v[7], P<void>(v[8]), v[9], P<void>(v[15]), f, (int)n, (int)d, (int)f, (int)v[10], (int)v[19]};
+    check(few_tokens(h, S(stream)), "few_tokens");
+    const FewTokens y{P<void>(v[15]), f, P<void>(v[11]), v[12], nullptr, 0, P<void>(v[14]), o, (int)n, (int)f, (int)o, (int)v[13], 0};
+    check(few_tokens(y, S(stream)), "few_tokens");
+    return;
+  }
   Product& p = plain_problem(a.p[0], n, f);
   const int tile_n = products_tile_n(kGated, n, f, 1, sms), up_mn = v[10] ? 0 : 1;
   const ProductOperand x{P<void>(v[4]), v[5], 0, 0}, w[2] = {{P<void>(v[6]), v[7], up_mn, 0}, {P<void>(v[8]), v[9], up_mn, 0}};

@@ -40,9 +40,14 @@ class GatedSaved:
     up: Optional[torch.Tensor] = None
 
 
-def _plain(t, device: int) -> bool:
-    """A matrix that the kernels can address as it lies, on GPU ``device``."""
-    return t.dtype is _BF16 and t.dim() == 2 and t.is_contiguous() and t.get_device() == device and t.data_ptr() & 15 == 0
+def _at(t, pitch: int):
+    """(tensor, address, row pitch) as the kernels take a matrix whose rows are ``pitch`` long; a copy where they cannot address it."""
+    if t.is_contiguous():
+        p = t.data_ptr()
+        if p & 15 == 0:
+            return t, p, pitch
+    t = rows.as_aligned(t)
+    return t, t.data_ptr(), rows.pitch(t)
 
 
 def _sizes(x, w_gate, w_up, w_down, act: str, up_layout: str, down_layout: str) -> Tuple[int, int, int, int]:
@@ -76,12 +81,6 @@ def _sizes(x, w_gate, w_up, w_down, act: str, up_layout: str, down_layout: str) 
     return n, d, f, o
 
 
-def _reachable(*tensors):
-    """The tensors, those that the kernels cannot address as copies."""
-    at = tensors[0].get_device()
-    return tensors if all(_plain(t, at) for t in tensors) else tuple(rows.as_aligned(t) for t in tensors)
-
-
 def gated_ff_fwd(x, w_gate, w_up, w_down, act: str = "silu", up_layout: str = "nn", down_layout: str = "nn", keep: bool = True):
     """(y [tokens, outputs], what ``gated_ff_bwd`` needs, None without ``keep``)."""
     n, d, f, o = _sizes(x, w_gate, w_up, w_down, act, up_layout, down_layout)
@@ -92,18 +91,21 @@ def gated_ff_fwd(x, w_gate, w_up, w_down, act: str = "silu", up_layout: str = "n
         y = h @ (w_down.float() if down_layout == "nn" else w_down.float().T)
         return y.to(x.dtype), GatedSaved(n, f, x.device, h=h, gate=g, up=u) if keep else None
     C = _native.load()
-    y = torch.empty(n, o, dtype=_BF16, device=x.device)
-    part = 2 * n * f
-    block = torch.empty(3 * part + 2 * n * -(-f // C.GATED_CHUNK) if keep else part, dtype=torch.uint8, device=x.device)
+    y = x.new_empty(n, o)
+    part = n * f
+    block = x.new_empty(3 * part + n * -(-f // C.GATED_CHUNK) if keep else part)
     saved = GatedSaved(n, f, x.device, block) if keep else None
     if n == 0:
         return y, saved
-    x, w_gate, w_up, w_down = _reachable(x, w_gate, w_up, w_down)
-    at = block.data_ptr()
-    C.gated_fwd(n, d, f, o, x.data_ptr(), rows.pitch(x), w_gate.data_ptr(), rows.pitch(w_gate), w_up.data_ptr(), rows.pitch(w_up),
-                1 if up_layout == "nt" else 0, w_down.data_ptr(), rows.pitch(w_down), 1 if down_layout == "nt" else 0, y.data_ptr(), at, at + part,
-                at + 2 * part, at + 3 * part, ACTS[act], 1 if keep else 0, _SM_COUNT.get(x.get_device()) or sm_count(x.device),
-                _native.status().dev, _native.stream_ptr())
+    up_nt, down_nt = up_layout == "nt", down_layout == "nt"
+    x, px, lx = _at(x, d)
+    w_gate, pg, lg = _at(w_gate, d if up_nt else f)
+    w_up, pu, lu = _at(w_up, d if up_nt else f)
+    w_down, pd, ld = _at(w_down, f if down_nt else o)
+    at, part = block.data_ptr(), 2 * part
+    C.gated_fwd(n, d, f, o, px, lx, pg, lg, pu, lu, 1 if up_nt else 0, pd, ld, 1 if down_nt else 0, y.data_ptr(), at, at + part, at + 2 * part,
+                at + 3 * part, ACTS[act], 1 if keep else 0, _SM_COUNT.get(x.get_device()) or sm_count(x.device), _native.status().dev,
+                _native.stream_ptr())
     return y, saved
 
 
@@ -140,26 +142,34 @@ def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "sil
         for t, v in zip(grads, new):
             t += v.to(t.dtype)
         return dx, tuple(grads)
-    dx = torch.empty(n, d, dtype=_BF16, device=x.device)
+    dx = x.new_empty(n, d)
     if not add:
-        grads = tuple(torch.empty(w.shape, dtype=_BF16, device=x.device) for w in weights)
+        grads = (x.new_empty(w_gate.shape), x.new_empty(w_up.shape), x.new_empty(w_down.shape))
     if n == 0:
         if not add:
             for t in grads:
                 t.zero_()
         return dx, tuple(grads)
-    dy, x, w_gate, w_up, w_down = _reachable(dy, x, *weights)
-    part = 2 * n * f
-    space = torch.empty(2 * part, dtype=torch.uint8, device=x.device)           # dg, du
-    at, to = saved.block.data_ptr(), space.data_ptr()
+    up_nt, down_nt = up_layout == "nt", down_layout == "nt"
+    dy, py, ly = _at(dy, o)
+    x, px, lx = _at(x, d)
+    w_gate, pg, lg = _at(w_gate, d if up_nt else f)
+    w_up, pu, lu = _at(w_up, d if up_nt else f)
+    w_down, pd, ld = _at(w_down, f if down_nt else o)
     gg, gu, gd = grads
-    types = sum(1 << i for i, g in enumerate(grads) if g.dtype is _F32)
-    _native.load().gated_bwd(n, d, f, o, dy.data_ptr(), rows.pitch(dy), x.data_ptr(), rows.pitch(x), w_gate.data_ptr(), rows.pitch(w_gate),
-                             w_up.data_ptr(), rows.pitch(w_up), 1 if up_layout == "nt" else 0, w_down.data_ptr(), rows.pitch(w_down),
-                             1 if down_layout == "nt" else 0, at, at + part, at + 2 * part, at + 3 * part, to, to + part, dx.data_ptr(),
-                             gg.data_ptr(), rows.pitch(gg), gu.data_ptr(), rows.pitch(gu), gd.data_ptr(), rows.pitch(gd), types, 1 if add else 0,
-                             ACTS[act], _SM_COUNT.get(x.get_device()) or sm_count(x.device), _native.status().dev, _native.stream_ptr())
-    return dx, tuple(grads)
+    if add:
+        lgg, lgu, lgd = rows.pitch(gg), rows.pitch(gu), rows.pitch(gd)
+        types = sum(1 << i for i, g in enumerate(grads) if g.dtype is _F32)
+    else:
+        lgg = lgu = d if up_nt else f
+        lgd, types = f if down_nt else o, 0
+    space = x.new_empty(2 * n * f)                        # dg, du
+    part, at, to = 2 * n * f, saved.block.data_ptr(), space.data_ptr()
+    _native.load().gated_bwd(n, d, f, o, py, ly, px, lx, pg, lg, pu, lu, 1 if up_nt else 0, pd, ld, 1 if down_nt else 0, at, at + part,
+                             at + 2 * part, at + 3 * part, to, to + part, dx.data_ptr(), gg.data_ptr(), lgg, gu.data_ptr(), lgu, gd.data_ptr(), lgd,
+                             types, 1 if add else 0, ACTS[act], _SM_COUNT.get(x.get_device()) or sm_count(x.device), _native.status().dev,
+                             _native.stream_ptr())
+    return dx, grads if type(grads) is tuple else tuple(grads)
 
 
 def _same(act: str, *tensors):

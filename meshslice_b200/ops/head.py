@@ -55,24 +55,32 @@ def _tile_n(n: int, columns: int, sms: int) -> int:
     return C.products_tile_n(C.PRODUCT_HEAD, n, columns, 1, sms)
 
 
-def _reachable(x, w, targets):
-    return _rows.as_aligned(x), _rows.as_aligned(w), targets if targets.is_contiguous() else targets.contiguous()
+def _at(t, pitch: int):
+    """(tensor, address, row pitch) as the kernels take a matrix whose rows are ``pitch`` long; a copy where they cannot address it."""
+    if t.is_contiguous():
+        p = t.data_ptr()
+        if p & 15 == 0:
+            return t, p, pitch
+    t = _rows.as_aligned(t)
+    return t, t.data_ptr(), _rows.pitch(t)
 
 
 def head_loss(x, w, targets, vocab: int, layout: str = "nn") -> torch.Tensor:
     """Loss [tokens] (fp32) of ``x`` [tokens, inputs] under the head ``w``."""
-    n, d, _ = _check(x, w, targets, vocab, layout)
+    n, d, cols = _check(x, w, targets, vocab, layout)
     if not x.is_cuda:
         return _reference(x, w, targets, vocab, layout)[0]
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
     if n:
-        x, w, targets = _reachable(x, w, targets)
+        x, px, lx = _at(x, d)
+        w, pw, lw = _at(w, cols if layout == "nn" else d)
+        targets = targets.contiguous()
         sms = _SM_COUNT.get(x.get_device()) or sm_count(x.device)
         tile_n = _tile_n(n, vocab, sms)
         blocks = -(-vocab * 2 // tile_n)                  # statistics are of half a tile's columns
         space = torch.empty((2 * blocks + 1) * n, dtype=torch.float32, device=x.device)
         at = space.data_ptr()
-        _native.load().head_losses(n, d, vocab, x.data_ptr(), _rows.pitch(x), w.data_ptr(), _rows.pitch(w), 1 if layout == "nt" else 0,
+        _native.load().head_losses(n, d, vocab, px, lx, pw, lw, 1 if layout == "nt" else 0,
                                    targets.data_ptr(), at, at + 8 * blocks * n, tile_n, loss.data_ptr(), sms, _native.status().dev,
                                    _native.stream_ptr())
     return loss
@@ -100,15 +108,17 @@ def head_loss_grad(x, w, targets, vocab: int, scale: float, layout: str = "nn", 
         dw += new.to(dw.dtype)
         return loss, dx.to(x.dtype), dw
     loss = torch.empty(n, dtype=torch.float32, device=x.device)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dx = x.new_empty(n, d)
     if n == 0:
         return loss, dx, dw if add else torch.zeros(w.shape, dtype=w.dtype, device=w.device)
-    x, w, targets = _reachable(x, w, targets)
     nt = layout == "nt"
+    x, px, lx = _at(x, d)
+    w, pw, lw = _at(w, d if nt else cols)
+    targets = targets.contiguous()
     columns = -(-vocab // 64) * 64                        # of the exponentials: zeros from vocab on
     wide = min(columns, cols)                             # those of the weight's gradient that a product writes
     if not add:
-        dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+        dw = w.new_empty(w.shape)
     # Sums over several pieces are held in fp32; where that would take a matrix of its own, as much memory is better spent on a larger piece.
     limit = PIECE_BYTES + (0 if dw.dtype is torch.float32 else 4 * w.numel())
     most = rows or max(256, limit // (2 * columns) // 256 * 256)
@@ -120,23 +130,18 @@ def head_loss_grad(x, w, targets, vocab: int, scale: float, layout: str = "nn", 
     C, sms, status, stream = _native.load(), _SM_COUNT.get(x.get_device()) or sm_count(x.device), _native.status().dev, _native.stream_ptr()
     tile_n = _tile_n(piece, columns, sms)
     blocks = -(-columns * 2 // tile_n)
-    space = torch.empty((2 * columns + 8 * blocks + 4) * piece, dtype=torch.uint8, device=x.device)
+    space = x.new_empty((columns + 4 * blocks + 2) * piece)
     e = space.data_ptr()
     stats, label = e + 2 * columns * piece, e + (2 * columns + 8 * blocks) * piece
-    wide_bytes, pitch = total.element_size() * wide, _rows.pitch(total)
-    clear = wide < cols and not (add and total is dw)
-    if not clear:
-        pad = (0, 0, 0, 0)
-    elif nt:
-        pad = (total.data_ptr() + total.element_size() * wide * pitch, total.element_size() * pitch, total.element_size() * d, cols - wide)
-    else:
-        pad = (total.data_ptr() + wide_bytes, total.element_size() * pitch, total.element_size() * (cols - wide), d)
+    pitch, size = _rows.pitch(total) if add else (d if nt else cols), total.element_size()
+    at, fp32, onto = total.data_ptr(), 1 if size == 4 else 0, add and total is dw
+    pad = (0, 0, 0, 0)
+    if wide < cols and not onto:
+        pad = (at + size * wide * pitch, size * pitch, size * d, cols - wide) if nt else (at + size * wide, size * pitch, size * (cols - wide), d)
     for i in range(0, n, piece):
-        m = min(piece, n - i)
-        C.head_grads(m, d, vocab, columns, wide, x.data_ptr() + 2 * i * _rows.pitch(x), _rows.pitch(x), w.data_ptr(), _rows.pitch(w),
-                     1 if nt else 0, targets.data_ptr() + 8 * i, scale, e, stats, label, tile_n, loss.data_ptr() + 4 * i,
-                     dx.data_ptr() + 2 * i * d, total.data_ptr(), pitch, 1 if total.dtype is torch.float32 else 0,
-                     1 if i or (add and total is dw) else 0, *(pad if i == 0 else (0, 0, 0, 0)), sms, status, stream)
+        C.head_grads(min(piece, n - i), d, vocab, columns, wide, px + 2 * i * lx, lx, pw, lw, 1 if nt else 0, targets.data_ptr() + 8 * i, scale, e,
+                     stats, label, tile_n, loss.data_ptr() + 4 * i, dx.data_ptr() + 2 * i * d, at, pitch, fp32, 1 if i or onto else 0,
+                     *(pad if i == 0 else (0, 0, 0, 0)), sms, status, stream)
     if total is not dw:
         if dw.is_contiguous() and dw.numel() % 4 == 0:
             C.cast_f32_to_bf16(total.data_ptr(), dw.data_ptr(), dw.numel(), 1 if add else 0, stream)

@@ -7,7 +7,7 @@ import test_dependent_launches_cpu as rules
 import test_dependent_launches_operators_cpu as operators
 import test_dependent_launches_strict_cpu as strict
 
-SMALL = [rules.CSRC / "ops" / n for n in ("gated.cu", "head.cu", "orthogonal.cu")]
+SMALL = [rules.CSRC / "ops" / n for n in ("few_tokens.cu", "gated.cu", "head.cu", "orthogonal.cu")]
 
 
 @pytest.mark.parametrize("check", operators.CHECKS, ids=lambda f: f.__name__[5:])
@@ -23,5 +23,5 @@ def test_strict_rules(path):
 
 def test_every_kernel_is_known():
     names = {k for p in SMALL + [rules.CSRC / "gemm/sm100_products.cu"] for k in rules.functions(rules._code(p), "__global__")}
-    assert names == {"gated_act_kernel", "gated_act_bwd_kernel", "head_rows_kernel", "square_sums_kernel", "load_unit_kernel", "load_unit_transposed_kernel", "head_losses_kernel", "momentum_kernel",
+    assert names == {"few_nn_kernel", "few_nt_kernel", "gated_act_kernel", "gated_act_bwd_kernel", "head_rows_kernel", "square_sums_kernel", "load_unit_kernel", "load_unit_transposed_kernel", "head_losses_kernel", "momentum_kernel",
                      "apply_update_kernel", "sm100_products_kernel"}
