@@ -30,6 +30,7 @@ STATUS_NAMES = {
     55: "timeout: window attention backward, waiting for scores", 56: "timeout: window attention backward, waiting for dP",
     57: "timeout: window attention backward, output waiting for its sums", 58: "timeout: window attention backward, next item",
     59: "timeout: window attention backward, MMA waiting for S to be read",
+    60: "timeout: orthogonal update of a small matrix, waiting for a product",
 }
 
 

@@ -32,6 +32,7 @@ CU_SOURCES = [
     "ops/gated.cu",
     "ops/head.cu",
     "ops/orthogonal.cu",
+    "ops/orthogonal_small.cu",
     "ops/window_attention.cu",
     "ops/window_decode.cu",
     "comm/p2p.cu",

@@ -638,6 +638,11 @@ void orthogonalize(uint64_t g, int bf16, int64_t stride, int items, int rows, in
                    uint64_t stream) {
   // powers of two that the fp16 copies are scaled by: their largest values are below 4, 16 and 200 (what the coefficients are checked for)
   constexpr float sx = 1024.f, sa = 1024.f, sb = 256.f;
+  if (rows <= kUnitSide && cols <= kUnitSide) {
+    check(orthogonal_small({P<void>(g), bf16, stride, items, rows, cols, steps, a, b, c, P<void>(out), out_fp32, out_item, out_row, out_col,
+                            P<uint32_t>(status), kLocalTimeoutNs}, S(stream)), "orthogonal_small");
+    return;
+  }
   const bool tall = rows > cols;
   const int64_t count = (int64_t)rows * cols, mn = (int64_t)items * m * n, mm = (int64_t)items * m * m;
   const uint64_t x = space, q = space + 8 * mn, p = q + 2 * mm, norms = p + 2 * mm;
@@ -859,6 +864,7 @@ PYBIND11_MODULE(_C, m) {
   m.attr("CHUNK_DESC_BYTES") = (int)sizeof(ChunkDesc);
 
   m.attr("GATED_CHUNK") = (int)kGatedChunk;
+  m.attr("UNIT_SIDE") = (int)kUnitSide;
   m.def("unit_space", &unit_space, "bytes of workspace of a matrix: m, n");
   m.def("products_tile_n", &products_tile_n, "columns of a tile: kind, M, N, items, sms");
   m.attr("PRODUCT_HEAD") = (int)kHead;

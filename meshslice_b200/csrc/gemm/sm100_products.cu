@@ -15,6 +15,7 @@
 #include "../common/gate.cuh"
 #include "../common/pdl.cuh"
 #include "../common/ptx.cuh"
+#include "../common/store_row.cuh"
 #include "pair.cuh"
 #include "sm100_gemm.h"
 #include "sm100_products.h"
@@ -455,31 +456,7 @@ __device__ __forceinline__ bool epilogue_step(const Product& p, const TileAt& at
       continue;
     }
     if (row >= p.rows) continue;
-    const int64_t at0 = at.item * p.out_item + row * p.out_row + col0 * p.out_col;
-    const int n = min(32, p.cols - col0);
-    if (p.out_fp32) {
-      float* o = reinterpret_cast<float*>(p.out) + at0;
-      if (n == 32 && p.out_col == 1 && aligned16(o)) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < n) o[i * p.out_col] = v[i];
-      }
-    } else {
-      __nv_bfloat16* o = reinterpret_cast<__nv_bfloat16*>(p.out) + at0;
-      if (n == 32 && p.out_col == 1 && aligned16(o)) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          reinterpret_cast<uint4*>(o)[i] = make_uint4(pk2(v[8 * i], v[8 * i + 1]), pk2(v[8 * i + 2], v[8 * i + 3]),
-                                                      pk2(v[8 * i + 4], v[8 * i + 5]), pk2(v[8 * i + 6], v[8 * i + 7]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < n) o[i * p.out_col] = __float2bfloat16_rn(v[i]);
-      }
-    }
+    store_row32(p.out, at.item * p.out_item + row * p.out_row + col0 * p.out_col, p.out_col, min(32, p.cols - col0), p.out_fp32 != 0, v);
   }
   return true;
 }

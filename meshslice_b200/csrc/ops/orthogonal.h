@@ -26,6 +26,23 @@ struct LoadUnit {
 };
 cudaError_t load_unit(const LoadUnit& a, cudaStream_t stream);
 
+// All of it for matrices of up to kUnitSide rows and columns, in one launch.
+constexpr int kUnitSide = 256;
+constexpr uint32_t kUnitTimeout = 60;        // status: waited too long for a product
+struct UnitSmall {
+  const void* g;
+  int bf16;
+  int64_t stride;              // elements from one matrix to the next
+  int items, rows, cols, steps;
+  float a, b, c;
+  void* out;
+  int out_fp32;
+  int64_t out_item, out_row, out_col;        // strides in elements
+  uint32_t* status;
+  uint64_t timeout_ns;
+};
+cudaError_t orthogonal_small(const UnitSmall& a, cudaStream_t stream);
+
 // The optimizer step around it, on `items` matrices of n elements (a multiple of 4) that lie `stride` elements apart in the flat buffers:
 //   m <- momentum m + s g,   u = s g + momentum m (nesterov) or m            s: *grad_scale, 1 for null
 //   master <- master - lr (size o + wd master), param = bf16(master)         u, o: [items, n], fp32

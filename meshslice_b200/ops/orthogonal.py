@@ -20,6 +20,7 @@ import torch
 from .. import _native
 from .gemm import _SM_COUNT, sm_count
 
+_TYPES = (torch.float32, torch.bfloat16)
 COEFFICIENTS = (3.4445, -4.7750, 2.0315)
 WORKSPACE_BYTES = 2 << 30       # matrices of a batch are taken some at a time beyond it
 
@@ -40,19 +41,19 @@ def _check_coefficients(steps: int, coefficients: Tuple[float, float, float]):
 def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16):
     """``g`` [rows, cols] or a batch of them [n, rows, cols], fp32 or bf16; the result, of the same shape, goes to ``out`` (fp32 or bf16, which may
     be ``g``) or a new tensor of ``out_dtype``."""
-    if g.dim() not in (2, 3) or g.dtype not in (torch.float32, torch.bfloat16):
+    if g.dim() not in (2, 3) or g.dtype not in _TYPES:
         raise ValueError(f"matrices are fp32 or bf16 [rows, cols] or [n, rows, cols] (got {g.dtype} {tuple(g.shape)})")
     if steps < 1 or int(steps) != steps:
         raise ValueError(f"the number of steps is positive (got {steps})")
-    coefficients = tuple(float(v) for v in coefficients)
-    if len(coefficients) != 3 or not all(math.isfinite(v) for v in coefficients):
+    coefficients = tuple(coefficients)
+    if len(coefficients) != 3 or not all(map(math.isfinite, coefficients)):
         raise ValueError(f"three finite coefficients (got {coefficients})")
     _check_coefficients(int(steps), coefficients)
     if out is None:
-        if out_dtype not in (torch.float32, torch.bfloat16):
+        if out_dtype not in _TYPES:
             raise ValueError(f"the result is fp32 or bf16 (got {out_dtype})")
         out = torch.empty(g.shape, dtype=out_dtype, device=g.device)
-    elif out.shape != g.shape or out.dtype not in (torch.float32, torch.bfloat16) or out.device != g.device:
+    elif out.shape != g.shape or out.dtype not in _TYPES or out.device != g.device:
         raise ValueError(f"out must be fp32 or bf16 {tuple(g.shape)} on {g.device} (got {out.dtype} {tuple(out.shape)} on {out.device})")
     if g.is_cuda:
         _native.check_device(g)
@@ -71,13 +72,17 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
         result = torch.empty(target.shape, dtype=target.dtype, device=target.device)
     m, n = -(-min(r, c) // 64) * 64, -(-max(r, c) // 64) * 64
     C, sms, status, stream = _native.load(), _SM_COUNT.get(g.get_device()) or sm_count(g.device), _native.status().dev, _native.stream_ptr()
-    each = C.unit_space(m, n)
-    most = max(1, min(items, WORKSPACE_BYTES // each, (1 << 31) // m - 1))
-    space = torch.empty(most * each, dtype=torch.uint8, device=g.device)
+    if r <= C.UNIT_SIDE and c <= C.UNIT_SIDE:      # in one launch, without a workspace
+        most, space = items, 0
+    else:
+        each = C.unit_space(m, n)
+        most = max(1, min(items, WORKSPACE_BYTES // each, (1 << 31) // m - 1))
+        block = torch.empty(most * each, dtype=torch.uint8, device=g.device)
+        space = block.data_ptr()
     stride, strides = batch.stride(0) if items > 1 else 0, (result.stride(0) if items > 1 else 0, result.stride(1), result.stride(2))
     for i in range(0, items, most):
         C.orthogonalize(batch.data_ptr() + i * stride * batch.element_size(), 1 if batch.dtype is torch.bfloat16 else 0, stride,
-                        min(most, items - i), r, c, int(steps), *coefficients, space.data_ptr(), m, n,
+                        min(most, items - i), r, c, int(steps), *coefficients, space, m, n,
                         result.data_ptr() + i * strides[0] * result.element_size(), 1 if result.dtype is torch.float32 else 0, *strides, sms,
                         status, stream)
     if result is not target:

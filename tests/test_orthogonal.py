@@ -53,7 +53,8 @@ def check(got, g, **kw):
     assert off.le(allowed).all(), (off / allowed)
 
 
-SIZES = [(1, 1, 1), (1, 8, 8), (2, 1, 100), (3, 100, 1), (1, 64, 64), (2, 65, 63), (1, 130, 300), (2, 300, 130), (1, 257, 513), (3, 40, 1000)]
+SIZES = [(1, 1, 1), (1, 8, 8), (2, 1, 100), (3, 100, 1), (1, 64, 64), (2, 65, 63), (1, 130, 300), (2, 300, 130), (1, 257, 513), (3, 40, 1000),
+         (2, 256, 256), (1, 255, 129), (1, 257, 256), (2, 20, 257), (2, 300, 1), (80, 33, 17)]
 
 
 @pytest.mark.parametrize("size", SIZES[:8])
@@ -93,21 +94,24 @@ def test_gpu_many_tiles(size):
 @gpu
 @pytest.mark.parametrize("steps,coefficients", [(1, COEFFICIENTS), (2, (1.5, -0.5, 0.0)), (3, (1.875, -1.25, 0.375)), (12, COEFFICIENTS)])
 def test_gpu_other_polynomials(steps, coefficients):
-    g = matrices("noise", 2, 100, 180)
-    check(F.orthogonalize(g.cuda(), steps=steps, coefficients=coefficients, out_dtype=torch.float32), g, steps=steps, coefficients=coefficients)
+    for n in (180, 280):
+        g = matrices("noise", 2, 100, n)
+        check(F.orthogonalize(g.cuda(), steps=steps, coefficients=coefficients, out_dtype=torch.float32), g, steps=steps, coefficients=coefficients)
 
 
 @gpu
 @pytest.mark.parametrize("size", [1e-30, 1e-18, 1e18, 1e30])
 def test_gpu_range(size):
     """Squares of the values are beyond fp32."""
-    g = matrices("noise", 2, 70, 130) * size
-    check(F.orthogonalize(g.cuda()), g)
+    for n in (130, 290):
+        g = matrices("noise", 2, 70, n) * size
+        check(F.orthogonalize(g.cuda()), g)
 
 
 @gpu
-def test_gpu_zeros_and_bad_values():
-    g = matrices("noise", 4, 70, 130)
+@pytest.mark.parametrize("n", [130, 290])
+def test_gpu_zeros_and_bad_values(n):
+    g = matrices("noise", 4, 70, n)
     g[1] = 0
     g[2, 3, 5] = float("nan")
     got = F.orthogonalize(g.cuda())
@@ -117,22 +121,23 @@ def test_gpu_zeros_and_bad_values():
 
 
 @gpu
-def test_gpu_layouts():
-    """Strided batches, results in other layouts and in place."""
-    g = matrices("noise", 3, 70, 130)
+@pytest.mark.parametrize("n", [130, 290])
+def test_gpu_layouts(n):
+    """Strided batches, results in other layouts and in place; in one launch and in several."""
+    g = matrices("noise", 3, 70, n)
     plain = F.orthogonalize(g.cuda())
-    flat = torch.zeros(3, 70 * 130 + 28, device="cuda")
-    view = flat.as_strided((3, 70, 130), (70 * 130 + 28, 130, 1))
+    flat = torch.zeros(3, 70 * n + 28, device="cuda")
+    view = flat.as_strided((3, 70, n), (70 * n + 28, n, 1))
     view.copy_(g)
     assert torch.equal(F.orthogonalize(view), plain)
     assert torch.equal(F.orthogonalize(g.mT.contiguous().mT.cuda()), plain)
     assert torch.equal(F.orthogonalize(g.mT.contiguous().cuda()).mT, plain)
-    out = torch.zeros(3, 80, 140, dtype=torch.bfloat16, device="cuda")
-    assert F.orthogonalize(g.cuda(), out=out[:, 5:75, 3:133]).data_ptr() == out[:, 5:75, 3:133].data_ptr()
-    assert torch.equal(out[:, 5:75, 3:133], plain)
-    out[:, 5:75, 3:133] = 0
+    out = torch.zeros(3, 80, n + 10, dtype=torch.bfloat16, device="cuda")
+    part = out[:, 5:75, 3:n + 3]
+    assert F.orthogonalize(g.cuda(), out=part) is part and torch.equal(part, plain)
+    part.zero_()
     assert out.count_nonzero() == 0
-    out = torch.zeros(130, 70, 3, dtype=torch.bfloat16, device="cuda").permute(2, 1, 0)
+    out = torch.zeros(n, 70, 3, dtype=torch.bfloat16, device="cuda").permute(2, 1, 0)
     assert F.orthogonalize(g.cuda(), out=out) is out and torch.equal(out, plain)
     own = g.cuda()
     whole = F.orthogonalize(own, out_dtype=torch.float32)
@@ -143,9 +148,9 @@ def test_gpu_layouts():
 def test_gpu_some_at_a_time(monkeypatch):
     """A batch that the workspace does not hold, on another stream; every matrix gets the same bits."""
     from meshslice_b200.ops import orthogonal
-    g = matrices("noise", 5, 70, 130).cuda()
+    g = matrices("noise", 5, 70, 290).cuda()
     plain = F.orthogonalize(g)
-    monkeypatch.setattr(orthogonal, "WORKSPACE_BYTES", 400000)
+    monkeypatch.setattr(orthogonal, "WORKSPACE_BYTES", 900000)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
@@ -156,10 +161,11 @@ def test_gpu_some_at_a_time(monkeypatch):
 
 
 @gpu
-def test_gpu_graphs():
+@pytest.mark.parametrize("m", [130, 290])
+def test_gpu_graphs(m):
     built = []
     for seed in (0, 1):
-        g = matrices("noise", 2, 130, 70, seed=seed).cuda()
+        g = matrices("noise", 2, m, 70, seed=seed).cuda()
         graph = torch.cuda.CUDAGraph()
         F.orthogonalize(g)
         torch.cuda.synchronize()
@@ -167,7 +173,7 @@ def test_gpu_graphs():
             out = F.orthogonalize(g)
         built.append((g, graph, out))
     for k, (g, _, _) in enumerate(built):
-        g.copy_(matrices("noise", 2, 130, 70, seed=5 + k))
+        g.copy_(matrices("noise", 2, m, 70, seed=5 + k))
     for _, graph, _ in built:
         graph.replay()
     torch.cuda.synchronize()
