@@ -581,63 +581,45 @@ void py_apply_update(uint64_t o, uint64_t master, uint64_t param, int64_t items,
   check(apply_update(P<float>(o), P<float>(master), P<void>(param), items, n, stride, lr, size, wd, S(stream)), "apply_update");
 }
 // alpha A A^T + beta C of a batch [items, m, k]
-void gram(int items, int m, int k, uint64_t src, uint64_t out, uint64_t c, float alpha, float beta, int sms, uint64_t status, uint64_t stream) {
-  static thread_local ProductArgs a;
-  Product& p = plain_problem(a.p[0], m, m);
+void gram_problem(Product& p, int tile_n, int items, int m, int k, uint64_t src, uint64_t out, uint64_t c, float alpha, float beta) {
+  plain_problem(p, m, m);
   p.items = items;
   p.a_item = p.b_item = m;
-  const int tile_n = products_tile_n(kGram, m, m, items, sms);
   const ProductOperand o{P<void>(src), k, 0, 0};
   const int64_t K = k, rows = (int64_t)items * m;
-  products_ok(product_operands(&p, kGram, tile_n, &o, &o, 1, rows, rows, &K), "gram");
-  products_ok(product_output(&p, 0, P<void>(out), m, rows, m, false), "gram");
+  products_ok(product_operands(&p, kGram, tile_n, &o, &o, 1, rows, rows, &K), "orthogonalize");
   p.out = P<void>(out);
   p.c = P<void>(c);
   p.alpha = alpha;
   p.beta = beta;
-  run_products(a, kGram, kNone, 1, 1, tile_n, sms, status, stream, "gram");
 }
-struct OrthoOut {
-  uint64_t out;      // 0: x and xs_out
-  int rows, cols;    // of the result, as X lies
-  int64_t item, row, col;
-  int fp32;
-};
-// alpha X + beta B X of a batch [items, m, n]
-void ortho_step(int items, int m, int n, uint64_t b, uint64_t xs, uint64_t x, uint64_t xs_out, float scale, float alpha, float beta,
-                const OrthoOut& r, int sms, uint64_t status, uint64_t stream) {
-  static thread_local ProductArgs a;
-  Product& p = plain_problem(a.p[0], m, n);
+// alpha X + beta B X of a batch [items, m, n]: to X (fp32) and, times `scale`, its other copy
+void step_problem(Product& p, int tile_n, int items, int m, int n, uint64_t b, uint64_t xs, uint64_t x, uint64_t xs_out, float scale, float alpha,
+                  float beta) {
+  plain_problem(p, m, n);
   p.items = items;
   p.a_item = p.b_item = m;
-  const int tile_n = products_tile_n(kStep, m, n, items, sms);
   const int64_t rows_all = (int64_t)items * m, K = m;
   const ProductOperand B{P<void>(b), m, 0, 0}, X{P<void>(xs), n, 1, rows_all};
-  products_ok(product_operands(&p, kStep, tile_n, &B, &X, 1, rows_all, n, &K), "ortho_step");
-  products_ok(product_output(&p, 0, P<void>(x), n, rows_all, n, true), "ortho_step");
-  if (r.out == 0) products_ok(product_output(&p, 1, P<void>(xs_out), n, rows_all, n, false), "ortho_step");
-  p.out = P<void>(r.out);
+  products_ok(product_operands(&p, kStep, tile_n, &B, &X, 1, rows_all, n, &K), "orthogonalize");
+  p.out = nullptr;
   p.c = P<void>(x);
+  p.copy = P<void>(xs_out);
   p.scale = scale;
   p.alpha = alpha;
   p.beta = beta;
-  p.rows = r.rows;
-  p.cols = r.cols;
-  p.out_item = r.item;
-  p.out_row = r.row;
-  p.out_col = r.col;
-  p.out_fp32 = r.fp32;
   order_of(p, m, tile_n);
-  run_products(a, kStep, kNone, 1, 1, tile_n, sms, status, stream, "ortho_step");
 }
-// `steps` steps of a batch of matrices [rows, cols], `stride` elements apart, in `space` (unit_space() bytes): X [m, n] in fp32, its copies
-// for the products twice, two matrices [m, m] and the partial sums of the norms.
-int64_t unit_space(int64_t m, int64_t n) { return 8 * m * n + 4 * m * m + 8 * kNormParts; }
+// `steps` steps of a batch of matrices [rows, cols], `stride` elements apart, in `space` (unit_space() bytes a matrix): X [m, n] in fp32, its copies
+// for the products twice, two matrices [m, m], the partial sums of the norms and the counters of the chain.
+constexpr int kMostSteps = 64;
+int64_t unit_space(int64_t m, int64_t n) { return 8 * m * n + 4 * m * m + 8 * kNormParts + 4 * 3 * kMostSteps; }
 void orthogonalize(uint64_t g, int bf16, int64_t stride, int items, int rows, int cols, int steps, float a, float b, float c, uint64_t space, int m,
                    int n, uint64_t out, int out_fp32, int64_t out_item, int64_t out_row, int64_t out_col, int sms, uint64_t status,
                    uint64_t stream) {
   // powers of two that the fp16 copies are scaled by: their largest values are below 4, 16 and 200 (what the coefficients are checked for)
   constexpr float sx = 1024.f, sa = 1024.f, sb = 256.f;
+  if (steps > kMostSteps) throw std::runtime_error("orthogonalize: too many steps");
   if (rows <= kUnitSide && cols <= kUnitSide) {
     check(orthogonal_small({P<void>(g), bf16, stride, items, rows, cols, steps, a, b, c, P<void>(out), out_fp32, out_item, out_row, out_col,
                             P<uint32_t>(status), kLocalTimeoutNs}, S(stream)), "orthogonal_small");
@@ -645,20 +627,33 @@ void orthogonalize(uint64_t g, int bf16, int64_t stride, int items, int rows, in
   }
   const bool tall = rows > cols;
   const int64_t count = (int64_t)rows * cols, mn = (int64_t)items * m * n, mm = (int64_t)items * m * m;
-  const uint64_t x = space, q = space + 8 * mn, p = q + 2 * mm, norms = p + 2 * mm;
-  uint64_t xs = space + 4 * mn, ys = space + 6 * mn;
-  check(square_sums(P<void>(g), bf16, items, count, stride, P<double>(norms), S(stream)), "square_sums");
+  const uint64_t x = space, xs = space + 4 * mn, ys = space + 6 * mn, q = space + 8 * mn, p = q + 2 * mm, norms = p + 2 * mm;
+  const uint64_t counters = norms + 8 * (int64_t)kNormParts * items;
+  check(square_sums(P<void>(g), bf16, items, count, stride, P<double>(norms), P<uint32_t>(counters), 3 * steps * items, S(stream)), "square_sums");
   check(load_unit({P<void>(g), bf16, stride, items, rows, cols, tall ? 1 : 0, P<double>(norms), norm_parts(count), P<float>(x), P<void>(xs), m, n, sx},
                   S(stream)), "load_unit");
-  for (int k = 0; k < steps; ++k) {
-    const bool last = k + 1 == steps;
-    gram(items, m, n, xs, q, 0, sa / (sx * sx), 0.f, sms, status, stream);
-    gram(items, m, m, q, p, q, sb * c / (sa * sa), sb * b / sa, sms, status, stream);
-    ortho_step(items, m, n, p, xs, x, ys, sx, a, 1.f / (sb * sx),
-               {last ? out : 0, std::min(rows, cols), std::max(rows, cols), out_item, tall ? out_col : out_row, tall ? out_row : out_col, out_fp32}, sms,
-               status, stream);
-    std::swap(xs, ys);
+  static thread_local ChainArgs chain;
+  const int tile_n = chain_tile_n(m, n, items, sms);
+  for (int i = 0; i < 2; ++i) {
+    gram_problem(chain.gram[i], tile_n, items, m, n, i ? ys : xs, q, 0, sa / (sx * sx), 0.f);
+    step_problem(chain.step[i], tile_n, items, m, n, p, i ? ys : xs, x, i ? xs : ys, sx, a, 1.f / (sb * sx));
   }
+  gram_problem(chain.square, tile_n, items, m, m, q, p, q, sb * c / (sa * sa), sb * b / sa);
+  Product& last = chain.step[2];
+  std::memcpy(static_cast<void*>(&last), static_cast<const void*>(&chain.step[(steps - 1) & 1]), sizeof(Product));
+  last.out = P<void>(out);
+  last.rows = std::min(rows, cols);
+  last.cols = std::max(rows, cols);
+  last.out_item = out_item;
+  last.out_row = tall ? out_col : out_row;
+  last.out_col = tall ? out_row : out_col;
+  last.out_fp32 = out_fp32;
+  chain.items = items;
+  chain.steps = steps;
+  chain.counters = P<uint32_t>(counters);
+  chain.status = P<uint32_t>(status);
+  chain.timeout_ns = kLocalTimeoutNs;
+  check(launch_sm100_chain(chain, tile_n, sms, S(stream)), "orthogonalize");
 }
 
 // ---------------------------------------------------------------------------------------
@@ -865,6 +860,7 @@ PYBIND11_MODULE(_C, m) {
 
   m.attr("GATED_CHUNK") = (int)kGatedChunk;
   m.attr("UNIT_SIDE") = (int)kUnitSide;
+  m.attr("UNIT_STEPS") = (int)kMostSteps;
   m.def("unit_space", &unit_space, "bytes of workspace of a matrix: m, n");
   m.def("products_tile_n", &products_tile_n, "columns of a tile: kind, M, N, items, sms");
   m.attr("PRODUCT_HEAD") = (int)kHead;

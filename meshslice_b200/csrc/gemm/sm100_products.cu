@@ -4,7 +4,7 @@
 //
 // There are eight epilogue warps, two for every 32 rows, which take half of a tile's columns each: the arithmetic of a chunk (32 rows x
 // 32 columns) is a chain of latencies, and one warp a scheduler leaves it idle.  Outputs leave chunk by chunk as TMA stores from 6 or 8 KiB
-// of staging a warp: as many sets of boxes as fit, written in turn (three 16-bit boxes, or an fp32 and a 16-bit one, are one set).  The staging
+// of staging a warp: as many sets of boxes as fit, written in turn (three 16-bit boxes are one set).  The staging
 // takes one of the plain GEMM's pipeline stages.  What an epilogue reads of memory it asks for one chunk ahead, for the first chunk
 // before the accumulator is complete.
 #include <cuda_bf16.h>
@@ -34,7 +34,8 @@ constexpr uint32_t smem_alloc_p(int bn) { return stages_p(bn) * (kAStageP + b_st
 constexpr int kThreadsP = 32 * (3 + kEpiWarps);   // warps: A producer, MMA, epilogue, B producer
 constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ void report_p(const ProductArgs& a, uint32_t code, uint32_t d0, uint32_t d1) {
+template <class Args>
+__device__ __forceinline__ void report_p(const Args& a, uint32_t code, uint32_t d0, uint32_t d1) {
   if (atomicCAS(a.status, 0u, code) == 0u) {
     a.status[1] = blockIdx.x;
     a.status[2] = d0;
@@ -128,7 +129,16 @@ struct TileAt {
   uint32_t drained;        // barrier to arrive at once this warp has read it
   uint64_t timeout_ns;
   int lane;
+  const uint32_t* written;  // of a chain: counter of the product before, and what it comes to; null: there is none
+  uint32_t target;
 
+  // What the product before wrote may be read.  Bounded; false: given up.
+  __device__ __forceinline__ bool before() const {
+    if (written == nullptr) return true;
+    int ok = 1;
+    if (lane == 0) ok = wait_flag_geq_gpu(written, target, 7 * timeout_ns) ? 1 : 0;
+    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+  }
   // Bounded; false: given up.
   __device__ __forceinline__ bool wait() const {
     int ok = 1;
@@ -357,20 +367,41 @@ __device__ __forceinline__ bool epilogue_head(const Product& p, const TileAt& at
   return true;
 }
 
+// A tile of 32 x 32 sums from lanes that hold rows to lanes that hold neighbouring columns: what is read and written of memory beside them then is
+// in whole lines.  (As rows of 128 bytes a lane, the fp32 X of a step took 11 us a tile of 256 x 256; as boxes of the copy engine, with a fence of
+// 550 cycles for each, 12.)
+__device__ __forceinline__ void to_columns(uint8_t* tile, int lane, const float (&v)[32]) {
+  __syncwarp();
+  stage32(tile, lane, v);
+  __syncwarp();
+}
+__device__ __forceinline__ float4 sums_of(const uint8_t* tile, int row, int unit) {
+  return *reinterpret_cast<const float4*>(tile + row * 128 + ((unit ^ (row & 7)) << 4));
+}
+
 // ---- kGram: alpha acc + beta C in fp16; below the diagonal the tile is written a second time, mirrored ----
 template <int BN>
-__device__ __forceinline__ bool epilogue_gram(const Product& p, const TileAt& at, ChunkStage<staging(BN), kBox16>& out) {
+__device__ __forceinline__ bool epilogue_gram(const Product& p, const TileAt& at, uint8_t* tile) {
+  // fields of an argument that is chosen at run time would be read again after every store
+  const int M = p.M;
+  const float alpha = p.alpha, beta = p.beta;
+  const __half* const C = reinterpret_cast<const __half*>(p.c);
   constexpr int kChunks = BN / 32 / 2;
-  const int64_t item0 = (int64_t)at.item * p.M;
-  const int row = at.row0 + at.lane;
+  uint8_t* const mirrored = tile + kBox32;                     // the chunk as fp16
+  const int64_t item0 = (int64_t)at.item * M;
+  const int lr = at.lane >> 2, lu = at.lane & 3;               // rows lr, lr + 8 .., columns 8 lu ..
   const bool mirror = at.nb * BN + BN <= at.m2 * 2 * kBM;      // the tile has nothing on the diagonal
-  __half* const whole = reinterpret_cast<__half*>(p.out) + item0 * p.M;
+  __half* const whole = reinterpret_cast<__half*>(p.out) + item0 * M;
   const int first = at.nb * BN + at.half * (BN / 2);
-  uint32_t x[16];
+  uint4 x[4];
   const auto ask = [&](int col0) {
-    const int nvalid = p.c != nullptr && at.row0 < p.M ? p.M - col0 : 0;
-    load_row16(reinterpret_cast<const __half*>(p.c) + (item0 + row) * p.M + col0, nvalid, x);
+    const bool there = C != nullptr && at.row0 < M && col0 < M;          // M is a multiple of 64: whole chunks
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = there ? ld_stream(reinterpret_cast<const uint4*>(C + (item0 + at.row0 + 8 * i + lr) * M + col0 + 8 * lu))
+                   : make_uint4(0u, 0u, 0u, 0u);
   };
+  if (C != nullptr && !at.before()) return false;
   ask(first);
   if (!at.wait()) return false;
 #pragma unroll 1
@@ -379,27 +410,33 @@ __device__ __forceinline__ bool epilogue_gram(const Product& p, const TileAt& at
     float v[32];
     load_acc(at.taddr + at.half * (BN / 2) + c * 32, v);
     if (c == kChunks - 1) at.read();
-    if (at.row0 >= p.M || col0 >= p.M) continue;
-    uint32_t w[16];
+    if (at.row0 >= M || col0 >= M) continue;
+    to_columns(tile, at.lane, v);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const float2 t = unh(x[i]);
-      w[i] = pkh(fmaf(p.beta, t.x, p.alpha * v[2 * i]), fmaf(p.beta, t.y, p.alpha * v[2 * i + 1]));
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + lr;
+      const float4 s0 = sums_of(tile, r, 2 * lu), s1 = sums_of(tile, r, 2 * lu + 1);
+      const float2 t0 = unh(x[i].x), t1 = unh(x[i].y), t2 = unh(x[i].z), t3 = unh(x[i].w);
+      const uint4 o = make_uint4(pkh(fmaf(beta, t0.x, alpha * s0.x), fmaf(beta, t0.y, alpha * s0.y)),
+                                 pkh(fmaf(beta, t1.x, alpha * s0.z), fmaf(beta, t1.y, alpha * s0.w)),
+                                 pkh(fmaf(beta, t2.x, alpha * s1.x), fmaf(beta, t2.y, alpha * s1.y)),
+                                 pkh(fmaf(beta, t3.x, alpha * s1.z), fmaf(beta, t3.y, alpha * s1.w)));
+      *reinterpret_cast<uint4*>(whole + (int64_t)(at.row0 + r) * M + col0 + 8 * lu) = o;
+      if (mirror) *reinterpret_cast<uint4*>(mirrored + r * 64 + ((lu ^ ((r >> 1) & 3)) << 4)) = o;
     }
     if (c + 1 < kChunks) ask(col0 + 32);
-    uint8_t* box = out.take(at.lane);
-    stage16(box, at.lane, w);
-    out.written();
-    if (at.lane == 0) {
-      send(&p.o[0], box, col0, (int)item0 + at.row0);
-      bulk_commit();
-    }
     if (mirror) {
-      unsigned short* to = reinterpret_cast<unsigned short*>(whole) + (int64_t)col0 * p.M + row;
+      __syncwarp();
+      unsigned short* to = reinterpret_cast<unsigned short*>(whole) + (int64_t)col0 * M + at.row0 + at.lane;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        to[(int64_t)(2 * i) * p.M] = (unsigned short)(w[i] & 0xffffu);
-        to[(int64_t)(2 * i + 1) * p.M] = (unsigned short)(w[i] >> 16);
+      for (int q = 0; q < 4; ++q) {
+        const uint4 o = *reinterpret_cast<const uint4*>(mirrored + at.lane * 64 + ((q ^ ((at.lane >> 1) & 3)) << 4));
+        const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          to[(int64_t)(8 * q + 2 * k) * M] = (unsigned short)(w[k] & 0xffffu);
+          to[(int64_t)(8 * q + 2 * k + 1) * M] = (unsigned short)(w[k] >> 16);
+        }
       }
     }
   }
@@ -408,21 +445,26 @@ __device__ __forceinline__ bool epilogue_gram(const Product& p, const TileAt& at
 
 // ---- kStep: alpha X + beta acc ----
 template <int BN>
-__device__ __forceinline__ bool epilogue_step(const Product& p, const TileAt& at, ChunkStage<staging(BN), kBox32 + kBox16>& out) {
+__device__ __forceinline__ bool epilogue_step(const Product& p, const TileAt& at, uint8_t* tile) {
+  const int M = p.M, N = p.N;
+  const float alpha = p.alpha, beta = p.beta, scale = p.scale;
+  __half* const copy = reinterpret_cast<__half*>(p.copy);
+  const bool last = p.out != nullptr;
   constexpr int kChunks = BN / 32 / 2;
-  const int64_t item0 = (int64_t)at.item * p.M;
-  const int row = at.row0 + at.lane;
+  const int64_t row0 = (int64_t)at.item * M + at.row0;
+  const int lr = at.lane >> 3, lu = at.lane & 7;               // rows lr, lr + 4 .., columns 4 lu ..
   const int first = at.nb * BN + at.half * (BN / 2);
+  float* const whole = const_cast<float*>(reinterpret_cast<const float*>(p.c));
   float4 x[8];
   const auto ask = [&](int col0) {                               // M and N are multiples of 64: whole chunks
-    if (at.row0 >= p.M || col0 >= p.N) return;
-    const uint4* from = reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(p.c) + (item0 + row) * p.N + col0);
+    if (at.row0 >= M || col0 >= N) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint4 u = ld_stream(from + i);
+      const uint4 u = ld_stream(reinterpret_cast<const uint4*>(whole + (row0 + 4 * i + lr) * N + col0 + 4 * lu));
       x[i] = make_float4(__uint_as_float(u.x), __uint_as_float(u.y), __uint_as_float(u.z), __uint_as_float(u.w));
     }
   };
+  if (!at.before()) return false;
   ask(first);
   if (!at.wait()) return false;
 #pragma unroll 1
@@ -431,39 +473,42 @@ __device__ __forceinline__ bool epilogue_step(const Product& p, const TileAt& at
     float v[32];
     load_acc(at.taddr + at.half * (BN / 2) + c * 32, v);
     if (c == kChunks - 1) at.read();
-    if (at.row0 >= p.M || col0 >= p.N) continue;
+    if (at.row0 >= M || col0 >= N) continue;
+    to_columns(tile, at.lane, v);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      v[4 * i] = fmaf(p.alpha, x[i].x, p.beta * v[4 * i]);
-      v[4 * i + 1] = fmaf(p.alpha, x[i].y, p.beta * v[4 * i + 1]);
-      v[4 * i + 2] = fmaf(p.alpha, x[i].z, p.beta * v[4 * i + 2]);
-      v[4 * i + 3] = fmaf(p.alpha, x[i].w, p.beta * v[4 * i + 3]);
+      const int r = 4 * i + lr;
+      const float4 t = sums_of(tile, r, lu);
+      x[i] = make_float4(fmaf(alpha, x[i].x, beta * t.x), fmaf(alpha, x[i].y, beta * t.y), fmaf(alpha, x[i].z, beta * t.z),
+                         fmaf(alpha, x[i].w, beta * t.w));
+      if (!last) {
+        const int64_t to = (row0 + r) * N + col0 + 4 * lu;
+        *reinterpret_cast<float4*>(whole + to) = x[i];
+        *reinterpret_cast<uint2*>(copy + to) =
+            make_uint2(pkh(x[i].x * scale, x[i].y * scale), pkh(x[i].z * scale, x[i].w * scale));
+      } else {
+        *reinterpret_cast<float4*>(tile + r * 128 + ((lu ^ (r & 7)) << 4)) = x[i];
+      }
     }
     if (c + 1 < kChunks) ask(col0 + 32);
-    if (p.out == nullptr) {
-      uint32_t w[16];
+    if (!last) continue;
+    // the result, in any layout: back to lanes that hold rows
+    __syncwarp();
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pkh(v[2 * i] * p.scale, v[2 * i + 1] * p.scale);
-      uint8_t* box = out.take(at.lane);
-      stage32(box, at.lane, v);
-      stage16(box + kBox32, at.lane, w);
-      out.written();
-      if (at.lane == 0) {
-        send(&p.o[0], box, col0, (int)item0 + at.row0);
-        send(&p.o[1], box + kBox32, col0, (int)item0 + at.row0);
-        bulk_commit();
-      }
-      continue;
+    for (int q = 0; q < 8; ++q) {
+      const float4 t = sums_of(tile, at.lane, q);
+      v[4 * q] = t.x; v[4 * q + 1] = t.y; v[4 * q + 2] = t.z; v[4 * q + 3] = t.w;
     }
-    if (row >= p.rows) continue;
-    store_row32(p.out, at.item * p.out_item + row * p.out_row + col0 * p.out_col, p.out_col, min(32, p.cols - col0), p.out_fp32 != 0, v);
+    const int64_t row = at.row0 + at.lane;
+    if (row < p.rows)
+      store_row32(p.out, at.item * p.out_item + row * p.out_row + col0 * p.out_col, p.out_col, min(32, p.cols - col0), p.out_fp32 != 0, v);
   }
   return true;
 }
 
 // Bytes of a chunk's boxes.
 constexpr uint32_t set_bytes(int kind) {
-  return kind == kGated || kind == kStep ? 3 * kBox16 : kind == kGatedGrad || kind == kPlain ? 2 * kBox16 : kBox16;
+  return kind == kGated ? 3 * kBox16 : kind == kGatedGrad || kind == kPlain ? 2 * kBox16 : kBox16;
 }
 template <int Kind, int BN>
 __device__ __forceinline__ bool epilogue(const Product& p, const TileAt& at, ChunkStage<staging(BN), set_bytes(Kind)>& out) {
@@ -471,8 +516,6 @@ __device__ __forceinline__ bool epilogue(const Product& p, const TileAt& at, Chu
   if constexpr (Kind == kGatedGrad) return epilogue_gated_grad<BN>(p, at, out);
   if constexpr (Kind == kPlain) return epilogue_plain<BN>(p, at, out);
   if constexpr (Kind == kHead) return epilogue_head<BN>(p, at, out);
-  if constexpr (Kind == kGram) return epilogue_gram<BN>(p, at, out);
-  if constexpr (Kind == kStep) return epilogue_step<BN>(p, at, out);
   return false;
 }
 
@@ -510,7 +553,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsP, 1)
 sm100_products_kernel(const __grid_constant__ ProductArgs a) {
   constexpr int kStagesP = stages_p(BN);
   constexpr uint32_t kBStageP = b_stage_p(BN);
-  constexpr bool kF16 = K0 == kGram || K0 == kStep;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   constexpr uint32_t kSmemB = kStagesP * kAStageP;
@@ -622,7 +664,7 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
         const Product& p = a.p[K1 == kNone ? 0 : t >= a.tiles[1] ? 2 : t >= a.tiles[0] ? 1 : 0];
         const int kblocks = p.kblocks[0] + p.kblocks[1];
         const bool a_mn = p.a_mn_major != 0, b_mn = p.b_mn_major != 0;
-        const uint32_t idesc = make_idesc_bf16(2 * kBM, BN, a_mn, b_mn) & (kF16 ? ~((1u << 7) | (1u << 10)) : ~0u);
+        const uint32_t idesc = make_idesc_bf16(2 * kBM, BN, a_mn, b_mn);
         const uint64_t da0 = make_smem_desc(smem_u32(sA), a_mn ? kBK * 128 : 16, 1024);
         const uint64_t db0 = make_smem_desc(smem_u32(sB), b_mn ? kBK * 128 : 16, 1024);
         const uint32_t da_hi = (uint32_t)(da0 >> 32), db_hi = (uint32_t)(db0 >> 32);
@@ -664,7 +706,7 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
       const uint32_t acc = it & 1, acc_phase = (it >> 1) & 1;
       const TileAt at{item, m2, nb, (2 * m2 + (int)rank) * kBM + q * 32, half,
                       tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, tfull_bar + acc, acc_phase,
-                      mapa_u32(smem_u32(tempty_bar + acc), 0), tmo, lane};
+                      mapa_u32(smem_u32(tempty_bar + acc), 0), tmo, lane, nullptr, 0};
       bool done;
       if (K1 == kNone || which == 0) {
         done = epilogue<K0, BN>(a.p[0], at, out0);
@@ -685,6 +727,191 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
   }
 
   // both CTAs are done with shared memory, barriers and TMEM of the pair
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2u * BN) : "memory");
+}
+
+// The products of an orthogonal update, one after another for every matrix of a batch, in one launch.  Tiles are numbered step by step, product by
+// product, matrix by matrix, and go round the CTA pairs; a tile's operands are the whole product before it of the same matrix, so its producers
+// wait until every epilogue warp of that product has counted itself done.  A pair comes to its tiles in their order and every tile waits for
+// earlier ones alone, so that with all pairs on the GPU (a cooperative launch) the first unfinished tile can always go on.  What that saves over a
+// launch a product: with several matrices no pair stands idle at the end of a product, where 8 x 1024 x 1024 (80, 80 and 128 tiles of 256 x 256 on
+// 74 pairs) took two rounds each, and no launch between any two of them.
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsP, 1)
+sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
+  constexpr int kStagesP = stages_p(BN);
+  constexpr uint32_t kBStageP = b_stage_p(BN);
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  constexpr uint32_t kSmemB = kStagesP * kAStageP;
+  constexpr uint32_t kSmemOut = kSmemB + kStagesP * kBStageP;
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + kSmemB;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(smem + kSmemOut + kEpiWarps * staging(BN));
+  uint64_t* empty_bar = full_bar + kStagesP;
+  uint64_t* tfull_bar = empty_bar + kStagesP;
+  uint64_t* tempty_bar = tfull_bar + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();      // 0: leader
+  const uint64_t tmo = a.timeout_ns;
+  const int cluster = blockIdx.x >> 1, clusters = gridDim.x >> 1;
+  const int of_gram = a.items * a.tiles[0], of_step = a.items * a.tiles[1], round = 2 * of_gram + of_step, all = a.steps * round;
+  struct Place {
+    const Product* p;
+    int phase;               // 0: X X^T, 1: b A + c A^2, 2: a X + B X
+    int t;                   // of the product
+    int index;               // of the product, 3 a step
+  };
+  const auto where = [&](int t) {
+    const int step = t / round, r = t - step * round;
+    Place w;
+    w.phase = r >= 2 * of_gram ? 2 : r >= of_gram ? 1 : 0;
+    w.t = r - (w.phase == 2 ? 2 * of_gram : w.phase * of_gram);
+    w.index = 3 * step + w.phase;
+    w.p = w.phase == 0 ? &a.gram[step & 1] : w.phase == 1 ? &a.square : &a.step[step + 1 == a.steps ? 2 : step & 1];
+    return w;
+  };
+  const auto counted = [&](int index, int item) { return a.counters + (int64_t)index * a.items + item; };
+  // Epilogue warps of the product before, of one matrix.
+  const auto target = [&](int phase) { return (uint32_t)(a.tiles[phase == 0 ? 1 : 0] * 2 * kEpiWarps); };
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < kStagesP; ++i) {
+      mbar_init(full_bar + i, 2);
+      mbar_init(empty_bar + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(tfull_bar + i, 1);
+      mbar_init(tempty_bar + i, 2 * kEpiWarps);
+    }
+    mbar_fence_init();
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2u * BN) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before_sync();
+  cluster_sync_all();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0 || warp == 2 + kEpiWarps) {
+    // ===================== TMA producers =====================
+    if (elect_one()) {
+      const bool is_a = warp == 0;
+      const uint32_t full0 = mapa_u32(smem_u32(full_bar), 0);
+      uint32_t stage = 0, phase = 0;
+      bool ok = true, free = true;
+      for (int t = cluster; t < all && ok; t += clusters) {
+        const Place w = where(t);
+        const Product& p = *w.p;
+        int item, m2, nb;
+        if (w.phase < 2) place<kGram, BN>(p, w.t, item, m2, nb);
+        else place<kStep, BN>(p, w.t, item, m2, nb);
+        if (w.index > 0) {
+          if (!wait_flag_geq_gpu(counted(w.index - 1, item), target(w.phase), 5 * tmo)) {
+            report_p(a, kTimeoutChunk, t, w.index);
+            break;
+          }
+          asm volatile("fence.proxy.async.global;" ::: "memory");            // what was written by stores is read by copies
+        }
+        const bool mn_major = (is_a ? p.a_mn_major : p.b_mn_major) != 0;      // of a step's X: always the 3-D map
+        const int first = item * (is_a ? p.a_item : p.b_item);
+        const int row = (is_a ? (2 * m2 + (int)rank) * kBM : nb * BN + (int)rank * (BN / 2)) + (mn_major ? 0 : first);
+        const int k_first = mn_major ? first : 0;
+        const uint32_t bytes = is_a ? kAStageP : kBStageP;
+        uint8_t* ring = is_a ? sA : sB;
+        const CUtensorMap* map = is_a ? &p.a[0] : &p.b[0];
+        const int kblocks = p.kblocks[0];
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!free && !mbar_wait(empty_bar + stage, phase ^ 1, 5 * tmo)) {
+            report_p(a, kTimeoutEmpty, t, kb);
+            ok = false;
+            break;
+          }
+          const uint32_t fb = full0 + stage * 8;
+          if (rank == 0) mbar_expect_tx(full_bar + stage, 2 * bytes);
+          uint8_t* dst = ring + stage * bytes;
+          if (!mn_major) tma_load_2d_pair(dst, map, fb, kb * kBK, row);
+          else tma_load_3d_pair(dst, map, fb, 0, k_first + kb * kBK, row >> 6);
+          if (++stage == kStagesP) { stage = 0; phase ^= 1; }
+          free = mbar_test(empty_bar + stage, phase ^ 1);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ===================== MMA issuer (leader only) =====================
+    if (rank == 0 && elect_one()) {
+      uint32_t stage = 0, phase = 0;
+      bool ok = true, full = false;
+      int it = 0;
+      for (int t = cluster; t < all && ok; t += clusters, ++it) {
+        const uint32_t acc = it & 1, acc_phase = (it >> 1) & 1;
+        if (!mbar_wait(tempty_bar + acc, acc_phase ^ 1, 6 * tmo)) {
+          report_p(a, kTimeoutTmemEmpty, t, acc);
+          ok = false;
+          break;
+        }
+        const uint32_t tmem_d = tmem_base + acc * BN;
+        const Product& p = *where(t).p;
+        const bool b_mn = p.b_mn_major != 0;
+        const uint32_t idesc = make_idesc_bf16(2 * kBM, BN, 0, b_mn) & ~((1u << 7) | (1u << 10));      // fp16
+        const uint64_t da0 = make_smem_desc(smem_u32(sA), 16, 1024);
+        const uint64_t db0 = make_smem_desc(smem_u32(sB), b_mn ? kBK * 128 : 16, 1024);
+        const uint32_t da_hi = (uint32_t)(da0 >> 32), db_hi = (uint32_t)(db0 >> 32);
+        const uint32_t b_kstep = (b_mn ? 16 * 128 : 32) >> 4;
+        const int kblocks = p.kblocks[0];
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!full && !mbar_wait(full_bar + stage, phase, 6 * tmo)) {
+            report_p(a, kTimeoutFull, t, kb);
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+          const uint32_t da_lo = (uint32_t)da0 + stage * (kAStageP >> 4);
+          const uint32_t db_lo = (uint32_t)db0 + stage * (kBStageP >> 4);
+          const uint32_t eb = smem_u32(empty_bar + stage);
+          if (++stage == kStagesP) { stage = 0; phase ^= 1; }
+          full = mbar_test(full_bar + stage, phase);
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k)
+            umma_f16_pair(tmem_d, desc_at(da_lo + k * 2, da_hi), desc_at(db_lo + k * b_kstep, db_hi), idesc, (kb | k) != 0 ? 1u : 0u);
+          umma_commit_both(eb);
+        }
+        if (ok) umma_commit_both(smem_u32(tfull_bar + acc));
+      }
+    }
+  } else {
+    // ===================== epilogue =====================
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* const boxes = smem + kSmemOut + (warp - 2) * staging(BN);
+    int it = 0;
+    for (int t = cluster; t < all; t += clusters, ++it) {
+      const Place w = where(t);
+      int item, m2, nb;
+      if (w.phase < 2) place<kGram, BN>(*w.p, w.t, item, m2, nb);
+      else place<kStep, BN>(*w.p, w.t, item, m2, nb);
+      const uint32_t acc = it & 1, acc_phase = (it >> 1) & 1;
+      const TileAt at{item, m2, nb, (2 * m2 + (int)rank) * kBM + q * 32, half,
+                      tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, tfull_bar + acc, acc_phase,
+                      mapa_u32(smem_u32(tempty_bar + acc), 0), tmo, lane,
+                      w.index > 0 ? counted(w.index - 1, item) : nullptr, target(w.phase)};
+      const bool done = w.phase < 2 ? epilogue_gram<BN>(*w.p, at, boxes) : epilogue_step<BN>(*w.p, at, boxes);
+      if (!done) {
+        if (lane == 0) report_p(a, kTimeoutTmemFull, t, acc);
+        break;
+      }
+      // this warp's part is written
+      __syncwarp();
+      if (lane == 0) red_add_release_gpu(counted(w.index, item), 1);
+    }
+  }
+
   tc_fence_before_sync();
   cluster_sync_all();
   tc_fence_after_sync();
@@ -764,10 +991,72 @@ cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problem
   MSB_PRODUCTS(kPlain, kGatedGrad)
   MSB_PRODUCTS(kPlain, kPlain)
   MSB_PRODUCTS(kHead, kNone)
-  MSB_PRODUCTS(kGram, kNone)
-  MSB_PRODUCTS(kStep, kNone)
 #undef MSB_PRODUCTS
   return cudaErrorInvalidValue;
+}
+
+
+template <int BN>
+static cudaError_t launch_chain_as(const ChainArgs& args, int64_t most_tiles, int sms, cudaStream_t stream) {
+  static int resident[64] = {0};          // clusters that fit the GPU at a time, 0: not yet asked
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  constexpr int smem = (int)smem_alloc_p(BN);
+  cudaLaunchAttribute attr[1];
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2);
+  cfg.blockDim = dim3(kThreadsP);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  int clusters = dev < 64 ? resident[dev] : 0;
+  if (clusters == 0) {
+    e = cudaFuncSetAttribute(sm100_chain_kernel<BN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 2;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.numAttrs = 1;
+    e = cudaOccupancyMaxActiveClusters(&clusters, sm100_chain_kernel<BN>, &cfg);
+    if (e != cudaSuccess) return e;
+    if (clusters < 1) return cudaErrorLaunchOutOfResources;
+    if (dev < 64) resident[dev] = clusters;
+  }
+  int64_t n = clusters < sms / 2 ? clusters : sms / 2;
+  n = most_tiles < n ? most_tiles : n;
+  cfg.gridDim = dim3((unsigned)(2 * (n < 1 ? 1 : n)));
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, sm100_chain_kernel<BN>, args);
+  if (e != cudaSuccess) (void)cudaGetLastError();
+  return e;
+}
+
+// The products of a step cannot take less time than one tile each, nor than all tiles on all pairs; a tile of 128 columns counts three quarters of
+// one of 256.
+int chain_tile_n(int64_t m, int64_t n, int64_t items, int sms) {
+  const int64_t pairs = sms > 1 ? sms / 2 : 1;
+  Product gram, step;
+  gram.M = gram.N = step.M = (int)m;
+  step.N = (int)n;
+  gram.items = step.items = (int)items;
+  const auto cost = [&](int tile_n) {
+    const int64_t each = tile_n == 128 ? 3 : 4, tiles = 2 * product_tiles(gram, kGram, tile_n) + product_tiles(step, kStep, tile_n);
+    const int64_t rounds = (tiles + pairs - 1) / pairs;
+    return each * (rounds < 3 ? 3 : rounds);
+  };
+  return cost(128) < cost(256) ? 128 : 256;
+}
+
+cudaError_t launch_sm100_chain(ChainArgs& args, int tile_n, int sms, cudaStream_t stream) {
+  const int64_t gram = product_tiles(args.square, kGram, tile_n), step = product_tiles(args.step[0], kStep, tile_n);
+  if (args.items < 1 || args.steps < 1 || (2 * gram + step) * args.steps > 0x3fffffff) return cudaErrorInvalidValue;
+  args.tiles[0] = (int)(gram / args.items);
+  args.tiles[1] = (int)(step / args.items);
+  const int64_t most = gram > step ? gram : step;
+  return tile_n == 128 ? launch_chain_as<128>(args, most, sms, stream) : launch_chain_as<256>(args, most, sms, stream);
 }
 
 }  // namespace msb

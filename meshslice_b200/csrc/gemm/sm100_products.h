@@ -45,7 +45,8 @@ struct Product {
   void* out;                   // kGram: fp16 [items, M, M]; kStep: the last step's result, or null
   const void* c;               // kPlain: the output; kGram: fp16 [items, M, M] or null; kStep: X in fp32 [items, M, N]
   float alpha, beta;
-  float scale;                 // kStep: of the fp16 copy
+  void* copy;                  // kStep: fp16 copy of X, times
+  float scale;
   int rows, cols;              // kStep: extent of the result that is wanted
   int64_t out_item, out_row, out_col;   // its strides in elements, one of the last two 1
   int out_fp32;                // kPlain too
@@ -76,8 +77,24 @@ int product_output(Product* p, int which, const void* base, int64_t cols, int64_
 int64_t product_tiles(const Product& p, int kind, int tile_n);
 
 // `problems` problems: the first of kind k0, the others of kind k1, on at most `sms` SMs.  The first `longer` of them have one contraction, not
-// shorter than the one of the others.  Supported: kGated, kHead, kGram, kStep alone (k1 kNone); (kGatedGrad, kPlain), (kPlain, kGatedGrad),
+// shorter than the one of the others.  Supported: kGated, kHead alone (k1 kNone); (kGatedGrad, kPlain), (kPlain, kGatedGrad),
 // (kPlain, kPlain).
 cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problems, int longer, int tile_n, int sms, cudaStream_t stream);
+
+// All products of the orthogonal update of a batch in one launch: step by step X X^T, b A + c A^2 and a X + B X, in which a tile waits for the
+// tiles that its matrix's product before it consists of.
+struct ChainArgs {
+  Product gram[2];             // kGram, of either copy of X
+  Product square;              // kGram
+  Product step[3];             // kStep: of either copy of X, and the last
+  int items, steps;
+  int tiles[2];                // of an item, kGram and kStep (set by the launcher)
+  uint32_t* counters;          // [3 steps, items], 0 at launch: epilogue warps that have written their part of a tile
+  uint32_t* status;
+  uint64_t timeout_ns;
+};
+// Columns of a tile, and the launch on at most `sms` SMs.
+int chain_tile_n(int64_t m, int64_t n, int64_t items, int sms);
+cudaError_t launch_sm100_chain(ChainArgs& args, int tile_n, int sms, cudaStream_t stream);
 
 }  // namespace msb

@@ -19,9 +19,11 @@ __device__ __forceinline__ float element(const void* g, int bf16, int64_t i) {
 // In 64 bits: squares of gradients leave the range of fp32 (1e-23), and the order of the parts is fixed.  A thread has four vectors in
 // flight: 4096 x 16384 in fp32 (268 MB) 300 us with four elements, in 128 parts.
 __global__ void __launch_bounds__(kSumThreads)
-square_sums_kernel(const void* g, int bf16, int64_t items, int64_t n, int64_t stride, int64_t per, double* partial) {
+square_sums_kernel(const void* g, int bf16, int64_t items, int64_t n, int64_t stride, int64_t per, double* partial, uint32_t* clear, int zeros) {
   grid_trigger();
   grid_wait();
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int i = threadIdx.x; i < zeros; i += kSumThreads) clear[i] = 0;
   __shared__ double red[kSumThreads / 32];
   const int wide = bf16 ? 8 : 4, bytes = bf16 ? 2 : 4;
   for (int64_t item = blockIdx.y; item < items; item += gridDim.y) {
@@ -222,11 +224,12 @@ int norm_parts(int64_t n) {
   const int64_t want = (n + 16383) / 16384;
   return (int)(want < 1 ? 1 : want > kNormParts ? kNormParts : want);
 }
-cudaError_t square_sums(const void* g, int bf16, int64_t items, int64_t n, int64_t stride, double* partial, cudaStream_t stream) {
+cudaError_t square_sums(const void* g, int bf16, int64_t items, int64_t n, int64_t stride, double* partial, uint32_t* clear, int zeros,
+                        cudaStream_t stream) {
   const int parts = norm_parts(n);
   const int64_t per = ((n + parts - 1) / parts + 7) / 8 * 8;
   return launch_dependent(square_sums_kernel, dim3(parts, (unsigned)(items < 4096 ? items : 4096)), kSumThreads, 0, stream, g, bf16, items, n,
-                          stride, per, partial);
+                          stride, per, partial, clear, zeros);
 }
 cudaError_t load_unit(const LoadUnit& a, cudaStream_t stream) {
   if (a.mp % 32 || a.np % 32 || a.parts > kThreads) return cudaErrorInvalidValue;

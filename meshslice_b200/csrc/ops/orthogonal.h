@@ -9,7 +9,9 @@ constexpr int kNormParts = 256;      // most partial sums of a matrix
 // Sums of squares of `items` matrices of `n` contiguous elements each (fp32 or bf16), `stride` elements apart: partial sums in 64 bits
 // [items, kNormParts], norm_parts(n) of each.
 int norm_parts(int64_t n);
-cudaError_t square_sums(const void* g, int bf16, int64_t items, int64_t n, int64_t stride, double* partial, cudaStream_t stream);
+// Clears `zeros` words at `clear` too.
+cudaError_t square_sums(const void* g, int bf16, int64_t items, int64_t n, int64_t stride, double* partial, uint32_t* clear, int zeros,
+                        cudaStream_t stream);
 // X = G / |G| (0 where G is 0), or its transpose, padded with zeros to [mp, np]: fp32, and `scale` times it in fp16.
 struct LoadUnit {
   const void* g;

@@ -63,8 +63,9 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
         return out.copy_(_reference(g, int(steps), coefficients))
     batch, target = (g[None], out[None]) if g.dim() == 2 else (g, out)
     items, r, c = batch.shape
-    if max(r, c) >= 1 << 24:
-        raise ValueError(f"the kernels take matrices of fewer than 2^24 rows and columns (got {r} x {c})")
+    if max(r, c) >= 1 << 24 or steps > _native.load().UNIT_STEPS:
+        raise ValueError(f"the kernels take matrices of fewer than 2^24 rows and columns and at most {_native.load().UNIT_STEPS} steps "
+                         f"(got {r} x {c}, {steps})")
     if not batch[0].is_contiguous():
         batch = batch.contiguous()
     result = target
