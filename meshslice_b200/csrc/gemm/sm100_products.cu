@@ -129,14 +129,13 @@ struct TileAt {
   uint32_t drained;        // barrier to arrive at once this warp has read it
   uint64_t timeout_ns;
   int lane;
-  const uint32_t* written;  // of a chain: counter of the product before, and what it comes to; null: there is none
-  uint32_t target;
+  uint64_t* written;        // of a chain: what the product before wrote may be read
+  uint32_t written_phase;
 
-  // What the product before wrote may be read.  Bounded; false: given up.
+  // Bounded; false: given up.
   __device__ __forceinline__ bool before() const {
-    if (written == nullptr) return true;
     int ok = 1;
-    if (lane == 0) ok = wait_flag_geq_gpu(written, target, 7 * timeout_ns) ? 1 : 0;
+    if (lane == 0) ok = mbar_wait(written, written_phase, 7 * timeout_ns) ? 1 : 0;
     return __shfl_sync(0xffffffffu, ok, 0) != 0;
   }
   // Bounded; false: given up.
@@ -706,7 +705,7 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
       const uint32_t acc = it & 1, acc_phase = (it >> 1) & 1;
       const TileAt at{item, m2, nb, (2 * m2 + (int)rank) * kBM + q * 32, half,
                       tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, tfull_bar + acc, acc_phase,
-                      mapa_u32(smem_u32(tempty_bar + acc), 0), tmo, lane, nullptr, 0};
+                      mapa_u32(smem_u32(tempty_bar + acc), 0), tmo, lane, nullptr, 0u};
       bool done;
       if (K1 == kNone || which == 0) {
         done = epilogue<K0, BN>(a.p[0], at, out0);
@@ -735,7 +734,8 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
 
 // The products of an orthogonal update, one after another for every matrix of a batch, in one launch.  Tiles are numbered step by step, product by
 // product, matrix by matrix, and go round the CTA pairs; a tile's operands are the whole product before it of the same matrix, so its producers
-// wait until every epilogue warp of that product has counted itself done.  A pair comes to its tiles in their order and every tile waits for
+// wait until all of its CTAs have counted themselves done (one counter a product and matrix, an arrival and a reader a CTA: with one for every
+// warp 3 x 1000 x 520 took 208 us).  A pair comes to its tiles in their order and every tile waits for
 // earlier ones alone, so that with all pairs on the GPU (a cooperative launch) the first unfinished tile can always go on.  What that saves over a
 // launch a product: with several matrices no pair stands idle at the end of a product, where 8 x 1024 x 1024 (80, 80 and 128 tiles of 256 x 256 on
 // 74 pairs) took two rounds each, and no launch between any two of them.
@@ -744,6 +744,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreadsP, 1)
 sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
   constexpr int kStagesP = stages_p(BN);
   constexpr uint32_t kBStageP = b_stage_p(BN);
+  constexpr int kAhead = 16;        // tiles that a producer may be ahead of the epilogue, and more: a stage holds a k-block, the accumulators two tiles
+  static_assert(kStagesP + 3 < kAhead, "");
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   constexpr uint32_t kSmemB = kStagesP * kAStageP;
@@ -754,7 +756,8 @@ sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
   uint64_t* empty_bar = full_bar + kStagesP;
   uint64_t* tfull_bar = empty_bar + kStagesP;
   uint64_t* tempty_bar = tfull_bar + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(tempty_bar + 2);
+  uint64_t* before_bar = tempty_bar + 2;         // [kAhead], one set per CTA: the product before that of a tile has been written
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(before_bar + kAhead);
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();      // 0: leader
@@ -777,8 +780,8 @@ sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
     return w;
   };
   const auto counted = [&](int index, int item) { return a.counters + (int64_t)index * a.items + item; };
-  // Epilogue warps of the product before, of one matrix.
-  const auto target = [&](int phase) { return (uint32_t)(a.tiles[phase == 0 ? 1 : 0] * 2 * kEpiWarps); };
+  // CTAs' parts of the product before, of one matrix.
+  const auto target = [&](int phase) { return (uint32_t)(a.tiles[phase == 0 ? 1 : 0] * 2); };
 
   if (warp == 0 && lane == 0) {
     for (int i = 0; i < kStagesP; ++i) {
@@ -789,6 +792,7 @@ sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
       mbar_init(tfull_bar + i, 1);
       mbar_init(tempty_bar + i, 2 * kEpiWarps);
     }
+    for (int i = 0; i < kAhead; ++i) mbar_init(before_bar + i, 1);
     mbar_fence_init();
   }
   if (warp == 1) {
@@ -807,19 +811,26 @@ sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
       const uint32_t full0 = mapa_u32(smem_u32(full_bar), 0);
       uint32_t stage = 0, phase = 0;
       bool ok = true, free = true;
-      for (int t = cluster; t < all && ok; t += clusters) {
+      int it = 0;
+      for (int t = cluster; t < all && ok; t += clusters, ++it) {
         const Place w = where(t);
         const Product& p = *w.p;
         int item, m2, nb;
         if (w.phase < 2) place<kGram, BN>(p, w.t, item, m2, nb);
         else place<kStep, BN>(p, w.t, item, m2, nb);
-        if (w.index > 0) {
-          if (!wait_flag_geq_gpu(counted(w.index - 1, item), target(w.phase), 5 * tmo)) {
-            report_p(a, kTimeoutChunk, t, w.index);
-            break;
-          }
-          asm volatile("fence.proxy.async.global;" ::: "memory");            // what was written by stores is read by copies
+        // One thread of a CTA looks at the counter, the others at what it saw.
+        uint64_t* const before = before_bar + it % kAhead;
+        if (is_a && w.index > 0 && !wait_flag_geq_gpu(counted(w.index - 1, item), target(w.phase), 5 * tmo)) {
+          report_p(a, kTimeoutChunk, t, w.index);
+          break;
         }
+        if (is_a) {
+          mbar_arrive(before);
+        } else if (!mbar_wait(before, it / kAhead & 1, 6 * tmo)) {
+          report_p(a, kTimeoutChunk, t, w.index);
+          break;
+        }
+        asm volatile("fence.proxy.async.global;" ::: "memory");              // what was written by stores is read by copies
         const bool mn_major = (is_a ? p.a_mn_major : p.b_mn_major) != 0;      // of a step's X: always the 3-D map
         const int first = item * (is_a ? p.a_item : p.b_item);
         const int row = (is_a ? (2 * m2 + (int)rank) * kBM : nb * BN + (int)rank * (BN / 2)) + (mn_major ? 0 : first);
@@ -890,6 +901,7 @@ sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
     // ===================== epilogue =====================
     const int q = warp & 3, half = (warp - 2) >> 2;
     uint8_t* const boxes = smem + kSmemOut + (warp - 2) * staging(BN);
+    bool ok = true;
     int it = 0;
     for (int t = cluster; t < all; t += clusters, ++it) {
       const Place w = where(t);
@@ -900,15 +912,15 @@ sm100_chain_kernel(const __grid_constant__ ChainArgs a) {
       const TileAt at{item, m2, nb, (2 * m2 + (int)rank) * kBM + q * 32, half,
                       tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN, tfull_bar + acc, acc_phase,
                       mapa_u32(smem_u32(tempty_bar + acc), 0), tmo, lane,
-                      w.index > 0 ? counted(w.index - 1, item) : nullptr, target(w.phase)};
-      const bool done = w.phase < 2 ? epilogue_gram<BN>(*w.p, at, boxes) : epilogue_step<BN>(*w.p, at, boxes);
-      if (!done) {
+                      before_bar + it % kAhead, (uint32_t)(it / kAhead & 1)};
+      // a warp that has given up does no more work, and still comes to the barrier of the CTA's epilogue warps
+      if (ok && !(w.phase < 2 ? epilogue_gram<BN>(*w.p, at, boxes) : epilogue_step<BN>(*w.p, at, boxes))) {
         if (lane == 0) report_p(a, kTimeoutTmemFull, t, acc);
-        break;
+        ok = false;
       }
-      // this warp's part is written
       __syncwarp();
-      if (lane == 0) red_add_release_gpu(counted(w.index, item), 1);
+      asm volatile("bar.sync 1, %0;" ::"n"(32 * kEpiWarps) : "memory");      // this CTA's part is written
+      if (warp == 2 && lane == 0) red_add_release_gpu(counted(w.index, item), 1);
     }
   }
 
