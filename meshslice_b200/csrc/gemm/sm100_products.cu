@@ -1046,20 +1046,15 @@ static cudaError_t launch_chain_as(const ChainArgs& args, int64_t most_tiles, in
   return e;
 }
 
-// The products of a step cannot take less time than one tile each, nor than all tiles on all pairs; a tile of 128 columns counts three quarters of
-// one of 256.
+// Columns of a tile: with 256 fewer operand bytes and rounds, with 128 a shorter way from one product to the next.  Us with tiles of 128 and of 256
+// columns, and how many of the latter a pair has in a step: 1024 x 1024 128 and 195 (0.5), 2048 x 2048 222 and 281 (1.8), 8 x 1024 x 1024 262 and
+// 271 (3.9), 4 x 1024 x 4096 472 and 496 (4.5), 4096 x 4096 1318 and 1183 (7.1), 16 x 1024 x 1024 528 and 479 (7.8).
 int chain_tile_n(int64_t m, int64_t n, int64_t items, int sms) {
-  const int64_t pairs = sms > 1 ? sms / 2 : 1;
   Product gram, step;
   gram.M = gram.N = step.M = (int)m;
   step.N = (int)n;
   gram.items = step.items = (int)items;
-  const auto cost = [&](int tile_n) {
-    const int64_t each = tile_n == 128 ? 3 : 4, tiles = 2 * product_tiles(gram, kGram, tile_n) + product_tiles(step, kStep, tile_n);
-    const int64_t rounds = (tiles + pairs - 1) / pairs;
-    return each * (rounds < 3 ? 3 : rounds);
-  };
-  return cost(128) < cost(256) ? 128 : 256;
+  return 2 * product_tiles(gram, kGram, 256) + product_tiles(step, kStep, 256) < 6 * (int64_t)(sms / 2) ? 128 : 256;
 }
 
 cudaError_t launch_sm100_chain(ChainArgs& args, int tile_n, int sms, cudaStream_t stream) {
