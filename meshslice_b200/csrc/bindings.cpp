@@ -409,9 +409,9 @@ Product& plain_problem(Product& p, int64_t M, int64_t N) {
   p.a_item = p.b_item = 0;
   return p;
 }
-// C (+)= A0 B0 (+ A1 B1)
+// C (+)= alpha (A0 B0 (+ A1 B1))
 void plain_product(Product& p, int tile_n, int64_t M, int64_t N, const int64_t* K, const ProductOperand* a, const ProductOperand* b, int ranges,
-                   uint64_t C, int64_t ldc, int fp32, int accumulate, const char* what) {
+                   uint64_t C, int64_t ldc, int fp32, int accumulate, float alpha, const char* what) {
   plain_problem(p, M, N);
   products_ok(product_operands(&p, kPlain, tile_n, a, b, ranges, M, N, K), what);
   products_ok(product_output(&p, 0, P<void>(C), N, M, ldc, fp32 != 0), what);
@@ -419,6 +419,7 @@ void plain_product(Product& p, int tile_n, int64_t M, int64_t N, const int64_t* 
   p.ldc = ldc;
   p.out_fp32 = fp32;
   p.accumulate = accumulate;
+  p.alpha = alpha;
   order_of(p, K[0] + (ranges > 1 ? K[1] : 0), tile_n);
 }
 void run_products(ProductArgs& a, int k0, int k1, int problems, int longer, int tile_n, int sms, uint64_t status, uint64_t stream, const char* what) {
@@ -497,7 +498,7 @@ void gated_bwd(const std::array<int64_t, 35>& v) {
     for (int i = 0; i < 2; ++i) products_ok(product_output(&p, i, P<void>(v[20 + i]), f, n, f, false), "gated_bwd");
     order_of(p, o, tile_n);
     const ProductOperand h{P<void>(v[16]), f, 1, 0}, dyt{P<void>(v[4]), v[5], 1, 0};
-    plain_product(a.p[grad_first ? 1 : 0], tile_n, wm, wn, &n, down_nt ? &dyt : &h, down_nt ? &h : &dyt, 1, (uint64_t)v[27], v[28], types >> 2 & 1, add,
+    plain_product(a.p[grad_first ? 1 : 0], tile_n, wm, wn, &n, down_nt ? &dyt : &h, down_nt ? &h : &dyt, 1, (uint64_t)v[27], v[28], types >> 2 & 1, add, 1.f,
                   "gated_bwd");
     run_products(a, grad_first ? kGatedGrad : kPlain, grad_first ? kPlain : kGatedGrad, 2, 1, tile_n, sms, status, stream, "gated_bwd");
   }
@@ -509,12 +510,12 @@ void gated_bwd(const std::array<int64_t, 35>& v) {
                                     dx_first ? kx : kw, dx_first ? kw : kx, sms);
     const ProductOperand g[2] = {{P<void>(v[20]), f, 0, 0}, {P<void>(v[21]), f, 0, 0}};
     const ProductOperand w[2] = {{P<void>(v[8]), v[9], up_nt ? 1 : 0, 0}, {P<void>(v[10]), v[11], up_nt ? 1 : 0, 0}};
-    plain_product(a.p[dx_first ? 0 : 2], tile_n, n, d, ff, g, w, 2, (uint64_t)v[22], d, 0, 0, "gated_bwd");
+    plain_product(a.p[dx_first ? 0 : 2], tile_n, n, d, ff, g, w, 2, (uint64_t)v[22], d, 0, 0, 1.f, "gated_bwd");
     const ProductOperand xt{P<void>(v[6]), v[7], 1, 0};
     for (int i = 0; i < 2; ++i) {
       const ProductOperand gt{P<void>(v[20 + i]), f, 1, 0};
       plain_product(a.p[dx_first ? 1 + i : i], tile_n, wm, wn, &n, up_nt ? &gt : &xt, up_nt ? &xt : &gt, 1, (uint64_t)v[23 + 2 * i], v[24 + 2 * i],
-                    types >> i & 1, add, "gated_bwd");
+                    types >> i & 1, add, 1.f, "gated_bwd");
     }
     run_products(a, kPlain, kPlain, 3, dx_first ? 1 : 2, tile_n, sms, status, stream, "gated_bwd");
   }
@@ -533,6 +534,9 @@ void head_partial(int64_t rows, int64_t width, int64_t vocab, int64_t columns, u
   p.label = P<float>(label);
   p.targets = P<int64_t>(targets);
   p.vocab = (int)vocab;
+  // parts of at most 1024, as many as are full of equal k-blocks
+  const int parts = (p.kblocks[0] + 15) / 16, per = (p.kblocks[0] + parts - 1) / parts;
+  p.parts = (p.kblocks[0] + per - 1) / per;
   order_of(p, width, tile_n);
   run_products(a, kHead, kNone, 1, 1, tile_n, sms, status, stream, "head");
 }
@@ -552,14 +556,19 @@ void head_grads(int64_t rows, int64_t width, int64_t vocab, int64_t columns, int
                 int sms, uint64_t status, uint64_t stream) {
   head_partial(rows, width, vocab, columns, x, ldx, w, ldw, nt ? 0 : 1, e, stats, label, targets, tile_n, sms, status, stream);
   const int half = tile_n / 2, blocks = (int)((columns + half - 1) / half);
+  // The scale is applied to the sums of the products: softmax - onehot as it is has its largest values near -1, which bf16 holds exactly, where
+  // times 1 / tokens all of them would be off by one and the same share, of up to 2^-8.
   check(head_rows({P<void>(e), columns, P<float2>(stats), P<float>(label), P<int64_t>(targets), (int)rows, (int)columns, blocks, half, (int)vocab,
-                   scale, P<float>(loss)}, S(stream)), "head_rows");
-  Gemm2Operands o[2];
-  if (nt) o[0] = local_operands(wide, width, rows, e, columns, 1, x, ldx, 1, dw, lddw, dw_fp32, accumulate, status);
-  else o[0] = local_operands(width, wide, rows, x, ldx, 1, e, columns, 1, dw, lddw, dw_fp32, accumulate, status);
-  o[1] = local_operands(rows, width, vocab, e, columns, 0, w, ldw, nt ? 1 : 0, dx, width, 0, 0, status);
-  if (o[1].K > o[0].K) std::swap(o[0], o[1]);
-  run_gemm2(o, 2, gemm2_tile_n(o, 2, sms), sms, P<uint32_t>(status), kLocalTimeoutNs, stream);
+                   1.f, P<float>(loss)}, S(stream)), "head_rows");
+  static thread_local ProductArgs a;
+  const int64_t kx = (vocab + kBK - 1) / kBK, kw = (rows + kBK - 1) / kBK, wm = nt ? wide : width, wn = nt ? width : wide;
+  const bool dx_first = kx >= kw;
+  const int tn = joint_tile_n([&](int i, int t) { return (i == 0) == dx_first ? products_tiles(kPlain, rows, width, 1, t) : products_tiles(kPlain, wm, wn, 1, t); },
+                              dx_first ? kx : kw, dx_first ? kw : kx, sms);
+  const ProductOperand ek{P<void>(e), columns, 0, 0}, em{P<void>(e), columns, 1, 0}, xm{P<void>(x), ldx, 1, 0}, wk{P<void>(w), ldw, nt ? 1 : 0, 0};
+  plain_product(a.p[dx_first ? 0 : 1], tn, rows, width, &vocab, &ek, &wk, 1, dx, width, 0, 0, scale, "head");
+  plain_product(a.p[dx_first ? 1 : 0], tn, wm, wn, &rows, nt ? &em : &xm, nt ? &xm : &em, 1, dw, lddw, dw_fp32, accumulate, scale, "head");
+  run_products(a, kPlain, kPlain, 2, 1, tn, sms, status, stream, "head");
   if (pad_height > 0 && pad_width > 0)
     check(cudaMemset2DAsync(P<void>(pad), pad_pitch, 0, pad_width, pad_height, reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream))),
           "cudaMemset2DAsync");

@@ -1,7 +1,7 @@
 // Local products whose epilogue is more than a conversion, on the tcgen05 core of the plain GEMM (CTA pairs, 256-row tiles):
 //   kGated       h = act(x Wg) * (x Wu), and what its gradient needs
 //   kGatedGrad   dg, du from dh = dy Wd^T
-//   kPlain       C (+)= A0 B0 (+ A1 B1), bf16 or fp32
+//   kPlain       C (+)= alpha (A0 B0 (+ A1 B1)), bf16 or fp32
 //   kHead        logits of a tile as statistics and exponentials relative to the tile's maximum
 //   kGram        alpha A A^T + beta C of a batch, symmetric: half of the tiles, mirrored (fp16)
 //   kStep        a X + gamma B X of a batch (fp32, with an fp16 copy, or the last one as the result)
@@ -38,6 +38,7 @@ struct Product {
   const int64_t* targets;
   int vocab;
   int write;                   // exponentials are written
+  int parts;                   // of the contraction, added in fp32 outside the tensor pipe; none is empty
   // ---- kPlain ----
   int accumulate;              // add to what is there: c (bf16) is read, fp32 is added by the copy engine
   int64_t ldc;

@@ -108,6 +108,20 @@ def test_gpu_odd_vocabularies(layout):
 
 
 @gpu
+@pytest.mark.parametrize("d", [1024, 1032, 2056, 4096])
+def test_gpu_contractions_in_parts(d):
+    """Inputs beyond 1024 are summed in several accumulators: a loss is as near as sums in fp32 are, whatever the width."""
+    x, w, t = data(70, d, 300, 320)
+    w[:, t[:35]] += (x[:35].float() * 0.1).bfloat16().T                   # confident ones, whose logits are large
+    z = x.double() @ w.double()[:, :300]
+    want = -torch.log_softmax(z, 1).gather(1, t[:, None])[:, 0]
+    loss = F.head_loss(x.cuda(), w.cuda(), t.cuda(), 300)
+    # 64 sums of 16 products, each cut off by at most 2^-23 of the largest partial sum, and those of the parts: 2^-16 of |x| |w| at the very most,
+    # 2^-21 of the logits in the mean (a quarter of 64 half steps, logits of few units)
+    assert (loss.double().cpu() - want).norm() <= 2.0 ** -20 * (want.norm() + z.amax(1).norm())
+
+
+@gpu
 def test_gpu_many_tiles():
     run("cuda", *data(2100, 64, 5003, 5120), 5003)
 
