@@ -406,7 +406,7 @@ Product& plain_problem(Product& p, int64_t M, int64_t N) {
   p.M = (int)M;
   p.N = (int)N;
   p.items = 1;
-  p.a_item = p.b_item = 0;
+  p.a_item = p.b_item = p.k_item = p.out_item_rows = 0;
   return p;
 }
 // C (+)= alpha (A0 B0 (+ A1 B1))
@@ -548,11 +548,21 @@ void head_losses(int64_t rows, int64_t width, int64_t vocab, uint64_t x, int64_t
   check(head_rows({nullptr, 0, P<float2>(stats), P<float>(label), P<int64_t>(targets), (int)rows, 0, blocks, half, (int)vocab, 0.f, P<float>(loss)},
                   S(stream)), "head_rows");
 }
+// Parts of the contraction over the vocabulary that the gradient of a few tokens is computed in, each by CTA pairs of their own: 1 where its tiles
+// keep the GPU busy, else as many as there are pairs for, of 32 k-blocks or more.  (52 tokens, 632 inputs, vocabulary 82320: five tiles of 1287
+// k-blocks, 334 us with them.)
+int head_parts(int64_t rows, int64_t width, int64_t vocab, int sms) {
+  const int64_t pairs = sms > 1 ? sms / 2 : 1, kb = (vocab + kBK - 1) / kBK, tiles = products_tiles(kPlain, rows, width, 1, 128);
+  const int64_t n = std::min(pairs / tiles, kb / 32);
+  if (n < 2) return 1;
+  const int64_t per = (kb + n - 1) / n;
+  return (int)((kb + per - 1) / per);
+}
 // Losses and gradients of `rows` tokens: e [rows, columns] is scratch too; dw is written or added to as far as `wide` of its columns, and
 // `pad_height` rows of `pad_width` bytes from `pad` on, `pad_pitch` apart, are cleared.
 void head_grads(int64_t rows, int64_t width, int64_t vocab, int64_t columns, int64_t wide, uint64_t x, int64_t ldx, uint64_t w, int64_t ldw,
                 int nt, uint64_t targets, float scale, uint64_t e, uint64_t stats, uint64_t label, int tile_n, uint64_t loss, uint64_t dx,
-                uint64_t dw, int64_t lddw, int dw_fp32, int accumulate, uint64_t pad, int64_t pad_pitch, int64_t pad_width, int64_t pad_height,
+                uint64_t dw, int64_t lddw, int dw_fp32, int accumulate, int parts, uint64_t sums, uint64_t pad, int64_t pad_pitch, int64_t pad_width, int64_t pad_height,
                 int sms, uint64_t status, uint64_t stream) {
   head_partial(rows, width, vocab, columns, x, ldx, w, ldw, nt ? 0 : 1, e, stats, label, targets, tile_n, sms, status, stream);
   const int half = tile_n / 2, blocks = (int)((columns + half - 1) / half);
@@ -562,13 +572,29 @@ void head_grads(int64_t rows, int64_t width, int64_t vocab, int64_t columns, int
                    1.f, P<float>(loss)}, S(stream)), "head_rows");
   static thread_local ProductArgs a;
   const int64_t kx = (vocab + kBK - 1) / kBK, kw = (rows + kBK - 1) / kBK, wm = nt ? wide : width, wn = nt ? width : wide;
-  const bool dx_first = kx >= kw;
-  const int tn = joint_tile_n([&](int i, int t) { return (i == 0) == dx_first ? products_tiles(kPlain, rows, width, 1, t) : products_tiles(kPlain, wm, wn, 1, t); },
-                              dx_first ? kx : kw, dx_first ? kw : kx, sms);
+  const int64_t per = (kx + parts - 1) / parts;
+  const bool dx_first = per >= kw;
+  const int tn = joint_tile_n([&](int i, int t) { return (i == 0) == dx_first ? products_tiles(kPlain, rows, width, parts, t) : products_tiles(kPlain, wm, wn, 1, t); },
+                              dx_first ? per : kw, dx_first ? kw : per, sms);
   const ProductOperand ek{P<void>(e), columns, 0, 0}, em{P<void>(e), columns, 1, 0}, xm{P<void>(x), ldx, 1, 0}, wk{P<void>(w), ldw, nt ? 1 : 0, 0};
-  plain_product(a.p[dx_first ? 0 : 1], tn, rows, width, &vocab, &ek, &wk, 1, dx, width, 0, 0, scale, "head");
+  Product& pd = a.p[dx_first ? 0 : 1];
+  if (parts == 1) {
+    plain_product(pd, tn, rows, width, &vocab, &ek, &wk, 1, dx, width, 0, 0, scale, "head");
+  } else {
+    const int64_t item_rows = (rows + 31) / 32 * 32;
+    plain_product(pd, tn, rows, width, &vocab, &ek, &wk, 1, sums, width, 1, 0, 1.f, "head");
+    products_ok(product_output(&pd, 0, P<void>(sums), width, item_rows * parts, width, true), "head");
+    pd.items = parts;
+    pd.kblocks[0] = (int)per;
+    pd.k_item = (int)per * kBK;
+    pd.out_item_rows = (int)item_rows;
+  }
   plain_product(a.p[dx_first ? 1 : 0], tn, wm, wn, &rows, nt ? &em : &xm, nt ? &xm : &em, 1, dw, lddw, dw_fp32, accumulate, scale, "head");
   run_products(a, kPlain, kPlain, 2, 1, tn, sms, status, stream, "head");
+  if (parts > 1) {
+    const int64_t stride = (rows + 31) / 32 * 32 * width;
+    check(sum_parts(P<float>(sums), stride, parts, P<void>(dx), rows, width, scale, S(stream)), "sum_parts");
+  }
   if (pad_height > 0 && pad_width > 0)
     check(cudaMemset2DAsync(P<void>(pad), pad_pitch, 0, pad_width, pad_height, reinterpret_cast<cudaStream_t>(static_cast<uintptr_t>(stream))),
           "cudaMemset2DAsync");
@@ -872,6 +898,7 @@ PYBIND11_MODULE(_C, m) {
   m.attr("UNIT_STEPS") = (int)kMostSteps;
   m.def("unit_space", &unit_space, "bytes of workspace of a matrix: m, n");
   m.def("products_tile_n", &products_tile_n, "columns of a tile: kind, M, N, items, sms");
+  m.def("head_parts", &head_parts, "parts of the contraction of a few tokens' gradient: rows, width, vocab, sms");
   m.attr("PRODUCT_HEAD") = (int)kHead;
 
   m.def("gemm_run", &gemm_run, "persistent tcgen05 GEMM with optional fused gather / push");
@@ -997,7 +1024,7 @@ PYBIND11_MODULE(_C, m) {
 #undef MSB_VALUES
       MSB_DIRECT("head_losses", head_losses, "rows, width, vocab, x, ldx, w, ldw, nt, targets, stats, label, tile_n, loss, sms, status, stream"),
       MSB_DIRECT("head_grads", head_grads, "rows, width, vocab, columns, wide, x, ldx, w, ldw, nt, targets, scale, e, stats, label, tile_n, loss, dx, "
-                 "dw, lddw, dw_fp32, accumulate, pad, pad_pitch, pad_width, pad_height, sms, status, stream"),
+                 "dw, lddw, dw_fp32, accumulate, parts, sums, pad, pad_pitch, pad_width, pad_height, sms, status, stream"),
       MSB_DIRECT("orthogonalize", orthogonalize, "g, bf16, stride, items, rows, cols, steps, a, b, c, space, m, n, out, out_fp32, item, row and column "
                  "strides of out, sms, status, stream"),
       MSB_DIRECT("gated_act", py_gated_act, "g, u, h, n, act, stream"),

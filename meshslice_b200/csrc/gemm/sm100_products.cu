@@ -298,7 +298,7 @@ __device__ __forceinline__ bool epilogue_plain(const Product& p, const TileAt& a
     }
     out.written();
     if (at.lane == 0) {
-      tma_store_box(&p.o[0], box, col0, at.row0, p.out_fp32 && p.accumulate);
+      tma_store_box(&p.o[0], box, col0, at.item * p.out_item_rows + at.row0, p.out_fp32 && p.accumulate);
       bulk_commit();
     }
   }
@@ -645,7 +645,7 @@ sm100_products_kernel(const __grid_constant__ ProductArgs a) {
         const bool mn_major = (is_a ? p.a_mn_major : p.b_mn_major) != 0, map3d = (is_a ? p.a_map3d : p.b_map3d) != 0;
         const int first = item * (is_a ? p.a_item : p.b_item);    // of the item's rows in the map
         const int row = (is_a ? (2 * m2 + (int)rank) * kBM : gated ? nb * (BN / 2) : nb * BN + (int)rank * (BN / 2)) + (mn_major ? 0 : first);
-        const int k_first = mn_major ? first : 0;
+        const int k_first = (mn_major ? first : 0) + item * p.k_item;
         const uint32_t bytes = is_a ? kAStageP : kBStageP;
         uint8_t* ring = is_a ? sA : sB;
         const int boxes = is_a ? kBM / 64 : BN / 128;

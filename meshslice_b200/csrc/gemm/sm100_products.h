@@ -25,6 +25,7 @@ struct Product {
   int items;                   // batch
   int a_mn_major, a_map3d, b_mn_major, b_map3d;
   int a_item, b_item;          // rows of the operand's map from one item to the next
+  int k_item;                  // of a contraction in parts, which are the items: its length from one to the next
   int group, along_n;          // tile order: panels of `group` blocks along M or N
   // ---- kGated, kGatedGrad ----
   int act;                     // 0: silu, 1: tanh-GeLU
@@ -40,6 +41,7 @@ struct Product {
   int write;                   // exponentials are written
   int parts;                   // of the contraction, added in fp32 outside the tensor pipe; none is empty
   // ---- kPlain ----
+  int out_item_rows;           // rows of the output from one item to the next, a multiple of 32
   int accumulate;              // add to what is there: c (bf16) is read, fp32 is added by the copy engine
   int64_t ldc;
   // ---- kPlain, kGram, kStep ----

@@ -132,6 +132,28 @@ head_losses_kernel(const HeadRows a) {
   a.loss[row] = y >= 0 && y < a.vocab ? logf(s) + (m - a.label[row]) : 0.f;
 }
 
+__global__ void __launch_bounds__(kThreads)
+sum_parts_kernel(const float* parts, int64_t stride, int n, uint2* out, int64_t vectors, float scale) {
+  grid_trigger();
+  grid_wait();
+  const int64_t i = blockIdx.x * (int64_t)kThreads + threadIdx.x;
+  if (i >= vectors) return;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < n; ++k) {
+    const float4 v = reinterpret_cast<const float4*>(parts + k * stride)[i];
+    s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
+  }
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(s.x * scale, s.y * scale), hi = __floats2bfloat162_rn(s.z * scale, s.w * scale);
+  out[i] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+
+cudaError_t sum_parts(const float* parts, int64_t stride, int n, void* out, int64_t rows, int64_t cols, float scale, cudaStream_t stream) {
+  const int64_t vectors = rows * cols / 4;
+  if (cols % 4 || stride % 4 || vectors > (int64_t)1 << 38) return cudaErrorInvalidValue;
+  return launch_dependent(sum_parts_kernel, (unsigned)((vectors + kThreads - 1) / kThreads), kThreads, 0, stream, parts, stride, n,
+                          reinterpret_cast<uint2*>(out), vectors, scale);
+}
 cudaError_t head_rows(const HeadRows& a, cudaStream_t stream) {
   if (a.e == nullptr) return launch_dependent(head_losses_kernel, (a.rows + 31) / 32, 32 * kLossWarps, 0, stream, a);
   if (a.cols % 8 || a.ld % 8 || a.tile_n % 8 || a.tiles > 4096) return cudaErrorInvalidValue;

@@ -20,5 +20,7 @@ struct HeadRows {
   float* loss;               // [rows]
 };
 cudaError_t head_rows(const HeadRows& a, cudaStream_t stream);
+// out [rows, cols] (bf16, cols a multiple of 4) = scale times the sum of `parts` fp32 matrices, `stride` elements apart, in their order.
+cudaError_t sum_parts(const float* parts, int64_t stride, int n, void* out, int64_t rows, int64_t cols, float scale, cudaStream_t stream);
 
 }  // namespace msb

@@ -130,9 +130,12 @@ def head_loss_grad(x, w, targets, vocab: int, scale: float, layout: str = "nn", 
     C, sms, status, stream = _native.load(), _SM_COUNT.get(x.get_device()) or sm_count(x.device), _native.status().dev, _native.stream_ptr()
     tile_n = _tile_n(piece, columns, sms)
     blocks = -(-columns * 2 // tile_n)
-    space = x.new_empty((columns + 4 * blocks + 2) * piece)
+    parts = C.head_parts(piece, d, vocab, sms)            # of the tokens' gradient, held in fp32 beside the others
+    sums = -(-piece // 32) * 32 * d * parts if parts > 1 else 0
+    space = x.new_empty((columns + 4 * blocks + 2) * piece + 2 * sums + 8)
     e = space.data_ptr()
     stats, label = e + 2 * columns * piece, e + (2 * columns + 8 * blocks) * piece
+    partial = (label + 4 * piece + 15) // 16 * 16
     pitch, size = _rows.pitch(total) if add else (d if nt else cols), total.element_size()
     at, fp32, onto = total.data_ptr(), 1 if size == 4 else 0, add and total is dw
     pad = (0, 0, 0, 0)
@@ -140,7 +143,7 @@ def head_loss_grad(x, w, targets, vocab: int, scale: float, layout: str = "nn", 
         pad = (at + size * wide * pitch, size * pitch, size * d, cols - wide) if nt else (at + size * wide, size * pitch, size * (cols - wide), d)
     for i in range(0, n, piece):
         C.head_grads(min(piece, n - i), d, vocab, columns, wide, px + 2 * i * lx, lx, pw, lw, 1 if nt else 0, targets.data_ptr() + 8 * i, scale, e,
-                     stats, label, tile_n, loss.data_ptr() + 4 * i, dx.data_ptr() + 2 * i * d, at, pitch, fp32, 1 if i or onto else 0,
+                     stats, label, tile_n, loss.data_ptr() + 4 * i, dx.data_ptr() + 2 * i * d, at, pitch, fp32, 1 if i or onto else 0, parts, partial,
                      *(pad if i == 0 else (0, 0, 0, 0)), sms, status, stream)
     if total is not dw:
         if dw.is_contiguous() and dw.numel() % 4 == 0:

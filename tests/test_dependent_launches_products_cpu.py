@@ -23,5 +23,5 @@ def test_strict_rules(path):
 
 def test_every_kernel_is_known():
     names = {k for p in SMALL + [rules.CSRC / "gemm/sm100_products.cu", rules.CSRC / "ops/orthogonal_small.cu"] for k in rules.functions(rules._code(p), "__global__")}
-    assert names == {"sm100_chain_kernel", "orthogonal_small_kernel", "few_nn_kernel", "few_nt_kernel", "gated_act_kernel", "gated_act_bwd_kernel", "head_rows_kernel", "square_sums_kernel", "load_unit_kernel", "load_unit_transposed_kernel", "head_losses_kernel", "momentum_kernel",
+    assert names == {"sum_parts_kernel", "sm100_chain_kernel", "orthogonal_small_kernel", "few_nn_kernel", "few_nt_kernel", "gated_act_kernel", "gated_act_bwd_kernel", "head_rows_kernel", "square_sums_kernel", "load_unit_kernel", "load_unit_transposed_kernel", "head_losses_kernel", "momentum_kernel",
                      "apply_update_kernel", "sm100_products_kernel"}

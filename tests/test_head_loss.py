@@ -108,6 +108,14 @@ def test_gpu_odd_vocabularies(layout):
 
 
 @gpu
+@pytest.mark.parametrize("layout", ["nn", "nt"])
+@pytest.mark.parametrize("n,d,vocab,rows", [(1, 24, 9001, 0), (33, 136, 12000, 0), (300, 72, 8200, 0), (100, 72, 8200, 33), (40, 520, 5000, 0)])
+def test_gpu_few_tokens_large_vocabularies(n, d, vocab, rows, layout):
+    """The contraction over the vocabulary in parts, the last of them shorter; with pieces of the tokens, the last of which has fewer."""
+    run("cuda", *data(n, d, vocab, -(-vocab // 8) * 8, missing=n > 10), vocab, layout, rows)
+
+
+@gpu
 @pytest.mark.parametrize("d", [1024, 1032, 2056, 4096])
 def test_gpu_contractions_in_parts(d):
     """Inputs beyond 1024 are summed in several accumulators: a loss is as near as sums in fp32 are, whatever the width."""
