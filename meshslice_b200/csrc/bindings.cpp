@@ -444,7 +444,7 @@ int products_tile_n(int kind, int64_t M, int64_t N, int64_t items, int sms) {
 template <class F>
 int joint_tile_n(F tiles, int64_t k0, int64_t k1, int sms) {
   const int64_t pairs = sms > 1 ? sms / 2 : 1;
-  const auto end = [&](int tile_n) { return walk_end(tiles(0, tile_n), k0, tiles(1, tile_n), k1, pairs); };
+  const auto end = [&](int tile_n) { return walk_end(tiles(0, tile_n), walk_blocks(k0), tiles(1, tile_n), walk_blocks(k1), pairs); };
   return 3 * end(128) < 4 * end(256) ? 128 : 256;
 }
 
@@ -549,8 +549,8 @@ void head_losses(int64_t rows, int64_t width, int64_t vocab, uint64_t x, int64_t
                   S(stream)), "head_rows");
 }
 // Parts of the contraction over the vocabulary that the gradient of a few tokens is computed in, each by CTA pairs of their own: 1 where its tiles
-// keep the GPU busy, else as many as there are pairs for, of 32 k-blocks or more.  (52 tokens, 632 inputs, vocabulary 82320: five tiles of 1287
-// k-blocks, 334 us with them.)
+// keep the GPU busy, else as many as there are pairs for, of 32 k-blocks or more.  (Tokens x inputs x vocabulary without and with them:
+// 52 x 632 x 82320 345 and 168 us, 32 x 2112 x 49461 265 and 217, 500 x 1024 x 50257 261 and 187.)
 int head_parts(int64_t rows, int64_t width, int64_t vocab, int sms) {
   const int64_t pairs = sms > 1 ? sms / 2 : 1, kb = (vocab + kBK - 1) / kBK, tiles = products_tiles(kPlain, rows, width, 1, 128);
   const int64_t n = std::min(pairs / tiles, kb / 32);

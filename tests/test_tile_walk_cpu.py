@@ -41,6 +41,17 @@ int main() {
     const long all = ((long)n0 * k0 + (long)n1 * k1 + n - 1) / n, longest = (long)((n0 + n - 1) / n) * k0;
     if (end > (all > longest ? all : longest) + 2 * k1) fail("uneven", n, n0, n1, k0, k1);
   }
+  // a long contraction's tiles on all pairs but a few, and thousands of one k-block: those few do not get nearly all of them
+  for (int late = 1; late < 74; ++late) {
+    const int n = 74, n1 = 3483, rounds = (int)walk_rounds(late, walk_blocks(194), n1, walk_blocks(1), n);
+    int most = 0;
+    for (int c = 0; c < n; ++c) {
+      int tiles = 0;
+      for (TileWalk w(c, n, late, late + n1, rounds); w.more(); w.next()) tiles += w.t >= late;
+      most = tiles > most ? tiles : most;
+    }
+    if (most > (n1 + n - 1) / n + 194 / 12 + 1) fail("short tiles on few pairs", n, late, n1, 194, 1);
+  }
   printf("ok\n");
 }
 """
