@@ -550,7 +550,7 @@ void head_losses(int64_t rows, int64_t width, int64_t vocab, uint64_t x, int64_t
 }
 // Parts of the contraction over the vocabulary that the gradient of a few tokens is computed in, each by CTA pairs of their own: 1 where its tiles
 // keep the GPU busy, else as many as there are pairs for, of 32 k-blocks or more.  (Tokens x inputs x vocabulary without and with them:
-// 52 x 632 x 82320 345 and 168 us, 32 x 2112 x 49461 265 and 217, 500 x 1024 x 50257 261 and 187.)
+// 52 x 632 x 82320 345 and 165 us, 32 x 2112 x 49464 265 and 210, 500 x 1024 x 50264 261 and 183.)
 int head_parts(int64_t rows, int64_t width, int64_t vocab, int sms) {
   const int64_t pairs = sms > 1 ? sms / 2 : 1, kb = (vocab + kBK - 1) / kBK, tiles = products_tiles(kPlain, rows, width, 1, 128);
   const int64_t n = std::min(pairs / tiles, kb / 32);

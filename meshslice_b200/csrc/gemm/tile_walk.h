@@ -39,10 +39,15 @@ struct TileWalk {
     }
   }
 };
-// What a tile of `k` k-blocks takes, in k-blocks: however short its contraction, its sums are read and stored, which took 2.4 us for
-// 256 x 128 of them, as long as 12 k-blocks.  The gradients of 52 tokens, 632 inputs and 82320 columns, and of 32, 2112 and 49461, with a
-// least of 6, 12 and 24: 174, 168 and 174 us, 223, 217 and 231 us; with none 318 and 530, for a few pairs then get nearly all short tiles.
-inline int64_t walk_blocks(int64_t k) { return k < 12 ? 12 : k; }
+// What a tile of `k` k-blocks takes, in k-blocks: however short its contraction, its sums are read and stored meanwhile, which takes as long as 8, and
+// as 48 where they are added to 16-bit values.  Without that, few pairs get nearly all short tiles.  Gradients of a head (tokens x inputs x
+// vocabulary), us by k-blocks alone and with leasts of 6, 8, 12 and 16: 52 x 632 x 82320 317, 171, 165, 166, 169; 32 x 2112 x 49464 524, 221, 210,
+// 216, 223; 500 x 1024 x 50264 183, 183, 183, 187, 195.  Of a gated block of 512 x 4096 x 10752, added to bf16, by k-blocks alone and with leasts of
+// 12, 24, 36 and 48: 1123, 1118, 1050, 1017, 999.
+inline int64_t walk_blocks(int64_t k, bool adds_16 = false) {
+  const int64_t least = adds_16 ? 48 : 8;
+  return k < least ? least : k;
+}
 // Those rounds, for `n0` tiles of `k0` k-blocks and `n1` of `k1`, and the k-blocks of the pair that ends last.
 inline int64_t walk_rounds(int64_t n0, int64_t k0, int64_t n1, int64_t k1, int64_t clusters) {
   const int64_t late = n0 % clusters;

@@ -50,7 +50,7 @@ int main() {
       for (TileWalk w(c, n, late, late + n1, rounds); w.more(); w.next()) tiles += w.t >= late;
       most = tiles > most ? tiles : most;
     }
-    if (most > (n1 + n - 1) / n + 194 / 12 + 1) fail("short tiles on few pairs", n, late, n1, 194, 1);
+    if (most > (n1 + n - 1) / n + 194 / 8 + 1) fail("short tiles on few pairs", n, late, n1, 194, 1);
   }
   printf("ok\n");
 }
