@@ -123,6 +123,8 @@ def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "sil
     if add:
         if len(grads) != 3:
             raise ValueError("grads are those of gate, up and down weight")
+        if len({g.data_ptr() for g in grads}) != 3:            # two products would add to it at the same time
+            raise ValueError("grads are three tensors: one cannot hold two gradients")
         for g, w in zip(grads, weights):
             if g.shape != w.shape or g.device != w.device or g.dtype not in (_F32, w.dtype):
                 raise ValueError(f"a gradient must be fp32 or {w.dtype} {tuple(w.shape)} on {w.device} (got {g.dtype} {tuple(g.shape)} on {g.device})")

@@ -38,6 +38,15 @@ def _check_coefficients(steps: int, coefficients: Tuple[float, float, float]):
         raise ValueError(f"the polynomial of {coefficients} takes singular values out of range within {steps} steps")
 
 
+def _meet(a, b) -> bool:
+    """The memory of two tensors may have a byte in common."""
+    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
+        return False
+    span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
 def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[torch.Tensor] = None, out_dtype=torch.bfloat16):
     """``g`` [rows, cols] or a batch of them [n, rows, cols], fp32 or bf16; the result, of the same shape, goes to ``out`` (fp32 or bf16, which may
     be ``g``) or a new tensor of ``out_dtype``."""
@@ -55,6 +64,8 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
         out = torch.empty(g.shape, dtype=out_dtype, device=g.device)
     elif out.shape != g.shape or out.dtype not in _TYPES or out.device != g.device:
         raise ValueError(f"out must be fp32 or bf16 {tuple(g.shape)} on {g.device} (got {out.dtype} {tuple(out.shape)} on {out.device})")
+    elif any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError(f"out needs an element for each of the result's (got strides {out.stride()})")
     if g.is_cuda:
         _native.check_device(g)
     if g.numel() == 0:
@@ -68,6 +79,8 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
                          f"(got {r} x {c}, {steps})")
     if not batch[0].is_contiguous():
         batch = batch.contiguous()
+    if out is not g and _meet(batch, target):       # a matrix is read before its own result is written, not before those of others
+        batch = batch.clone()
     result = target
     if min(target.stride(1), target.stride(2)) != 1 or (r > 1 and c > 1 and target.stride(1) == target.stride(2)):
         result = torch.empty(target.shape, dtype=target.dtype, device=target.device)

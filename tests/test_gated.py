@@ -282,6 +282,7 @@ BAD = {
     "kept by another call": lambda a: F.gated_ff_bwd(a[4], *a[:4], F.gated_ff_fwd(a[0][:2], *a[1:4])[1]),
     "gradients": lambda a: F.gated_ff_bwd(a[4], *a[:4], F.gated_ff_fwd(*a[:4])[1], grads=(torch.zeros(1), torch.zeros(1), torch.zeros(1))),
     "two gradients": lambda a: F.gated_ff_bwd(a[4], *a[:4], F.gated_ff_fwd(*a[:4])[1], grads=(torch.zeros_like(a[1]), torch.zeros_like(a[2]))),
+    "one gradient twice": lambda a: F.gated_ff_bwd(a[4], *a[:4], F.gated_ff_fwd(*a[:4])[1], grads=[torch.zeros_like(a[1])] * 2 + [torch.zeros_like(a[3])]),
     "operands": lambda a: F.gated_act(a[0], a[4]),
     "operands' activation": lambda a: F.gated_act(a[0], a[0], "tanh"),
 }

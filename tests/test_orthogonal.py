@@ -120,6 +120,23 @@ def test_gpu_zeros_and_bad_values(n):
         check(got[i:i + 1], g[i:i + 1])
 
 
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("n", [130, 290])
+def test_out_shares_memory_with_other_matrices(n, dev):
+    """Results that lie where matrices that are still to be read are: as without that."""
+    g = matrices("noise", 4, 70, n).to(dev)
+    want = F.orthogonalize(g[:3], out_dtype=torch.float32)
+    for first, to in ((0, 1), (1, 0)):
+        t = torch.zeros(4, 70, n, device=dev)
+        t[first:first + 3] = g[:3]
+        F.orthogonalize(t[first:first + 3], out=t[to:to + 3])
+        assert torch.equal(t[to:to + 3], want)
+    square = matrices("noise", 2, 70, 70).to(dev)
+    want = F.orthogonalize(square, out_dtype=torch.float32)
+    F.orthogonalize(square, out=square.mT)
+    assert torch.equal(square.mT, want)
+
+
 @gpu
 @pytest.mark.parametrize("n", [130, 290])
 def test_gpu_layouts(n):
@@ -197,6 +214,8 @@ BAD = {
     "one that is no number": lambda g: F.orthogonalize(g, coefficients=(1.5, float("nan"), 0.0)),
     "type of the result": lambda g: F.orthogonalize(g, out_dtype=torch.float16),
     "shape of the result": lambda g: F.orthogonalize(g, out=torch.zeros(4, 4, device=g.device)),
+    "an out that lies on itself": lambda g: F.orthogonalize(g, out=torch.zeros(1, 6, device=g.device).expand(4, 6)),
+    "a batch of one out": lambda g: F.orthogonalize(g.expand(3, 4, 6), out=torch.zeros(1, 4, 6, device=g.device).expand(3, 4, 6)),
     "type of out": lambda g: F.orthogonalize(g, out=torch.zeros(4, 6, device=g.device, dtype=torch.float64)),
 }
 
