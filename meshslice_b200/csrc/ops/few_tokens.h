@@ -5,6 +5,8 @@
 
 namespace msb {
 
+// Beyond them tiles of the tcgen05 pipe are faster.  Us here and there, weights [K, N]: 16 tokens of 1024 x 2816 22 and 28, of 4096 x 10752 81 and
+// 89, of 8192 x 28672 300 and 288.
 constexpr int kFewTokens = 16;
 
 // out [tokens, N] = x W, or act(x W) * (x U) with `up`.  bf16, sums in fp32.  nt: the weights lie as [N, K], otherwise as [K, N]; rows begin on
