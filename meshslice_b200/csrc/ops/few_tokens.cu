@@ -196,7 +196,7 @@ few_nn_kernel(const FewTokens a) {
 
 // CTAs of a cluster.  It costs some 2 us beside a plain launch: 8 tokens of 1024 x 2816, weights [K, N], 16.3, 15.8 and 17.4 us with at least 32, 64 and
 // 148 CTAs.  Where every warp keeps two units of the contraction, two CTAs an SM are worth more (one with 9 tokens or more, whose CTAs take twice the
-// registers): one token of 10752 x 4096, down weight [K, N], 97 us with 64 CTAs and 62 with 512, of 28672 x 8192 314 with 128 and 139 with 512.
+// registers): one token of 10752 x 4096, down weight [K, N], 95 us with 64 CTAs and 62 with 512, of 28672 x 8192 314 with 128 and 139 with 512.
 static int cluster_of(int64_t blocks, int64_t units, int64_t most) {
   int size = 1;
   while (size < 8 && ((blocks * size < 64 && 2 * size * kWarps <= units) || (blocks * size < most && 4 * size * kWarps <= units))) size *= 2;
