@@ -15,9 +15,12 @@ Layout on disk: ``<dir>/step_<N>/shard_r<r>_c<c>.pt`` = {name: local block} plus
 optimizer is saved, ``optim/master/<name>``, ``optim/m/<name>``, ``optim/v/<name>`` (fp32, same
 block as the parameter, so the optimizer state re-shards with the parameters) and
 ``optim/step``; ``<dir>/step_<N>/meta.json`` (mesh, per-parameter global shape / kind / dataflow /
-dtype, step, whether optimizer state is present, caller's ``extra`` such as the data position).
+dtype, step, whether optimizer state is present and what updated each parameter, caller's ``extra`` such as the data position).
 meta.json is written last, through a temporary file and an atomic rename: a step directory
 without it is an interrupted save.
+
+Optimizer state is loaded by an optimizer that updates the parameters in the same way (AdamW or orthogonal updates) alone: m and v
+mean other things in the other one.  A checkpoint that does not say what updated its parameters is judged by its moments.
 
 Loading parameters without optimizer state (an older checkpoint, imported weights) rebuilds the
 optimizer's fp32 master copies from the loaded parameters and clears the moments.
@@ -30,6 +33,7 @@ from typing import Dict, List, Optional, Tuple
 
 import torch
 
+from .optim import OTHER_RULE, found_rule
 from .parallel.mesh import Mesh, ShardedTensor
 
 
@@ -73,6 +77,8 @@ def save_checkpoint(root: str, step: int, model, optimizer=None, extra: Optional
     if rank0:
         meta = {"format": "meshslice_b200.ckpt.v1", "mesh": [mesh.R, mesh.C], "step": step,
                 "has_optimizer": optimizer is not None, "extra": extra or {}, "params": {}}
+        if optimizer is not None:
+            meta["update_rules"] = optimizer.update_rules(params)
         dataflows = {}
         for i, b in enumerate(getattr(model, "blocks", [])):
             for j, l in enumerate(b.layers()):
@@ -102,7 +108,8 @@ def _write_json_atomic(path: str, obj):
 
 def load_checkpoint(root: str, step: int, model, optimizer=None) -> dict:
     """Loads the coordinates this process holds.  Raises if the mesh shape or a shard shape
-    does not match (re-shard offline with ``reshard_checkpoint`` first)."""
+    does not match (re-shard offline with ``reshard_checkpoint`` first), or if the optimizer's
+    state is that of another update rule."""
     mesh: Mesh = model.mesh
     d = _step_dir(root, step)
     meta = json.load(open(os.path.join(d, "meta.json")))
@@ -111,6 +118,10 @@ def load_checkpoint(root: str, step: int, model, optimizer=None) -> dict:
     params = model.parameters()
     with_opt = optimizer is not None and bool(meta.get("has_optimizer"))
     named = optimizer.named_state(params) if with_opt else None
+    rules, saved = optimizer.update_rules(params) if with_opt else {}, meta.get("update_rules")
+    for name, rule in rules.items():
+        if saved is not None and saved.get(name, rule) != rule:
+            raise ValueError(f"{name}: {OTHER_RULE}")
     for (r, c) in mesh.coords():
         path = os.path.join(d, f"shard_r{r}_c{c}.pt")
         if not os.path.exists(path):
@@ -119,6 +130,11 @@ def load_checkpoint(root: str, step: int, model, optimizer=None) -> dict:
             blob = torch.load(path, map_location="cpu")
         except Exception as e:
             raise RuntimeError(f"corrupted shard file {path}: {e}") from e
+        if saved is None:
+            for name, rule in rules.items():
+                keys = [f"optim/{k}/{name}" for k in ("m", "v")]
+                if all(k in blob for k in keys) and rule != "both" and found_rule(*(blob[k] for k in keys)) not in (None, rule):
+                    raise ValueError(f"{name}: {OTHER_RULE}")
         for name, p, _, _ in params:
             if name not in blob:
                 raise KeyError(f"{path} has no parameter {name}")

@@ -124,36 +124,68 @@ class AdamW:
         view has the shape of the parameter shard; a parameter that does not live inside one of
         this optimizer's flat buffers is an error.  This is what makes the optimizer state
         save-able and re-shardable with the same rules as the parameters themselves."""
-        out = {}
+        out = {name: {} for name, _, _, _ in params}
+        for name, key, t, g, off in self._located(params):
+            out[name][key] = tuple(b[off:off + t.numel()].view(t.shape) for b in (g.master, g.m, g.v))
+        return out
+
+    def _located(self, params):
+        """(name, coordinate, shard, group, its first element there) of every parameter shard."""
         spans = [(g, g.param.data_ptr(), g.param.data_ptr() + g.param.numel() * g.param.element_size())
                  for g in self.groups]
         for name, p, _, _ in params:
-            per = {}
             for key, t in p.shards.items():
                 for g, lo, hi in spans:
                     if lo <= t.data_ptr() < hi:
                         if not t.is_contiguous():
                             raise ValueError(f"{name}: parameter shard is not contiguous in its flat buffer")
-                        off = (t.data_ptr() - lo) // g.param.element_size()
-                        n = t.numel()
-                        per[key] = tuple(b[off:off + n].view(t.shape) for b in (g.master, g.m, g.v))
+                        yield name, key, t, g, (t.data_ptr() - lo) // g.param.element_size()
                         break
                 else:
                     raise ValueError(f"{name}: parameter shard {key} is outside the optimizer's flat buffers")
-            out[name] = per
+
+    def update_rules(self, params):
+        """{name: 'adamw', 'orthogonal' or 'both'}: what updates a parameter, and so what its m and v mean."""
+        out = {}
+        for name, _, t, g, off in self._located(params):
+            here = sum(max(0, min(b, off + t.numel()) - max(a, off)) for a, b in self._spans(g))
+            out[name] = "adamw" if here == t.numel() else "orthogonal" if here == 0 else "both"
         return out
 
     def state_dict(self):
         return {"step": self.step_count,
-                "groups": [{"master": g.master, "m": g.m, "v": g.v, "kind": g.kind} for g in self.groups]}
+                "groups": [{"master": g.master, "m": g.m, "v": g.v, "kind": g.kind, "adamw": self._spans(g)} for g in self.groups]}
 
     def load_state_dict(self, sd):
+        for i, (g, s) in enumerate(zip(self.groups, sd["groups"])):
+            own, at = self._spans(g), 0
+            if "adamw" in s:
+                same = [tuple(x) for x in s["adamw"]] == own
+            else:
+                same = True
+                for a, b in own + [(g.param.numel(), g.param.numel())]:
+                    same &= found_rule(s["m"][at:a], s["v"][at:a]) in (None, "orthogonal")
+                    same &= found_rule(s["m"][a:b], s["v"][a:b]) in (None, "adamw")
+                    at = b
+            if not same:
+                raise ValueError(f"group {i}: {OTHER_RULE}")
         self.step_count = sd["step"]
         for g, s in zip(self.groups, sd["groups"]):
             g.master.copy_(s["master"])
             g.m.copy_(s["m"])
             g.v.copy_(s["v"])
             g.param.copy_(g.master.to(g.param.dtype))
+
+
+OTHER_RULE = ("the moments are those of another optimizer (AdamW's are means, those of orthogonal updates an undamped sum beside no second one); "
+              "without them the parameters can be loaded alone, and resync_from_params starts the optimizer anew")
+
+
+def found_rule(m, v) -> Optional[str]:
+    """The update rule of a state that does not name it: orthogonal updates leave v at 0, AdamW does not beside a first moment of this
+    size, whose square is far above the smallest fp32 number.  None: nothing that tells."""
+    orthogonal, adamw = bool(((m.abs() > 1e-12) & (v == 0)).any()), bool(v.any())
+    return "both" if orthogonal and adamw else "orthogonal" if orthogonal else "adamw" if adamw else None
 
 
 UPDATE_BYTES = 1 << 30      # of updates that are in memory at a time
@@ -168,7 +200,7 @@ class Muon(AdamW):
 
     whose elements are of the size of AdamW's, so that one learning rate serves both.  ``matrices``: whole 2-D views of the groups'
     parameters; those of one shape that lie at equal distances are updated together.  Their m is kept in the group's first
-    moment, and the second one stays 0.
+    moment, and the second one stays 0: a state saved by one of the two optimizers is refused by the other.
     """
 
     def __init__(self, groups: List[FlatGroup], matrices: List[torch.Tensor], momentum: float = 0.95, nesterov: bool = True, steps: int = 5,
