@@ -112,7 +112,7 @@ def gated_ff_fwd(x, w_gate, w_up, w_down, act: str = "silu", up_layout: str = "n
 def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "silu", up_layout: str = "nn", down_layout: str = "nn",
                  grads: Optional[Sequence[torch.Tensor]] = None):
     """(dx, (gradients of gate, up and down weight)).  The weights' gradients are new tensors, or are added to ``grads`` (fp32 or the
-    weights' type, in the weights' layouts)."""
+    weights' type, in the weights' layouts), which share no memory with one another or with an operand; columns of one wider matrix are fine."""
     n, d, f, o = _sizes(x, w_gate, w_up, w_down, act, up_layout, down_layout)
     if dy.shape != (n, o) or dy.dtype is not x.dtype or dy.get_device() != x.get_device():
         raise ValueError(f"dy must be {x.dtype} [{n}, {o}] on {x.device} (got {dy.dtype} {tuple(dy.shape)} on {dy.device})")
@@ -123,13 +123,12 @@ def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "sil
     if add:
         if len(grads) != 3:
             raise ValueError("grads are those of gate, up and down weight")
-        if len({g.data_ptr() for g in grads}) != 3:            # two products would add to it at the same time
-            raise ValueError("grads are three tensors: one cannot hold two gradients")
         for g, w in zip(grads, weights):
             if g.shape != w.shape or g.device != w.device or g.dtype not in (_F32, w.dtype):
                 raise ValueError(f"a gradient must be fp32 or {w.dtype} {tuple(w.shape)} on {w.device} (got {g.dtype} {tuple(g.shape)} on {g.device})")
-            if x.is_cuda and not (rows.aligned(g) and rows.pitch(g) % 8 == 0):
+            if x.is_cuda and not rows.adds(g):
                 raise ValueError("gradients that are added to need neighbouring columns and rows on 16-byte boundaries")
+        rows.check_apart(grads, (dy, x, *weights), "a gradient")        # products of one launch add to them and read the operands
     if not x.is_cuda:
         g, u, xf, dyf = saved.gate, saved.up, x.float(), dy.float()
         a, da = _act(g, act)
