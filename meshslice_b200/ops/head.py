@@ -88,8 +88,8 @@ def head_loss(x, w, targets, vocab: int, layout: str = "nn") -> torch.Tensor:
 
 def head_loss_grad(x, w, targets, vocab: int, scale: float, layout: str = "nn", dw: Optional[torch.Tensor] = None, rows: int = 0):
     """(loss [tokens] in fp32 and not scaled, dx, dw): the gradients times ``scale``.  ``dw`` (fp32 or the weight's type, the weight's
-    layout) is added to; without it the weight's gradient is a new tensor.  ``rows``: tokens whose exponentials are in memory at a
-    time (0: as many as half a gigabyte holds)."""
+    layout) is added to and shares no memory with an operand; without it the weight's gradient is a new tensor.  ``rows``: tokens whose
+    exponentials are in memory at a time (0: as many as half a gigabyte holds)."""
     n, d, cols = _check(x, w, targets, vocab, layout)
     if rows < 0:
         raise ValueError(f"rows at a time are not negative (got {rows})")
@@ -97,8 +97,9 @@ def head_loss_grad(x, w, targets, vocab: int, scale: float, layout: str = "nn", 
     if add:
         if dw.shape != w.shape or dw.device != w.device or dw.dtype not in (torch.float32, w.dtype):
             raise ValueError(f"dw must be fp32 or {w.dtype} {tuple(w.shape)} on {w.device} (got {dw.dtype} {tuple(dw.shape)} on {dw.device})")
-        if x.is_cuda and not (_rows.aligned(dw) and _rows.pitch(dw) % 8 == 0):
+        if x.is_cuda and not _rows.adds(dw):
             raise ValueError("a gradient that is added to needs neighbouring columns and rows on 16-byte boundaries")
+        _rows.check_apart((dw,), (x, w, targets), "dw")       # pieces of the tokens read the operands after others were added
     if not x.is_cuda:
         loss, dz = _reference(x, w, targets, vocab, layout, scale)
         dx = dz @ (w.float().T if layout == "nn" else w.float())
