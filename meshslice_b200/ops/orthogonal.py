@@ -38,10 +38,18 @@ def _check_coefficients(steps: int, coefficients: Tuple[float, float, float]):
         raise ValueError(f"the polynomial of {coefficients} takes singular values out of range within {steps} steps")
 
 
+def _own_elements(t) -> bool:
+    """Every element has memory of its own: along each dimension a step leads beyond what the shorter steps reach."""
+    reach = 0
+    for step, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if step <= reach:
+            return False
+        reach += step * (n - 1)
+    return True
+
+
 def _meet(a, b) -> bool:
-    """The memory of two tensors may have a byte in common."""
-    if a.untyped_storage().data_ptr() != b.untyped_storage().data_ptr():
-        return False
+    """The memory of two tensors may have a byte in common, in one storage or in several over the same memory."""
     span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
     (a0, a1), (b0, b1) = span(a), span(b)
     return a0 < b1 and b0 < a1
@@ -64,8 +72,8 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
         out = torch.empty(g.shape, dtype=out_dtype, device=g.device)
     elif out.shape != g.shape or out.dtype not in _TYPES or out.device != g.device:
         raise ValueError(f"out must be fp32 or bf16 {tuple(g.shape)} on {g.device} (got {out.dtype} {tuple(out.shape)} on {out.device})")
-    elif any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
-        raise ValueError(f"out needs an element for each of the result's (got strides {out.stride()})")
+    elif not _own_elements(out):
+        raise ValueError(f"out needs an element for each of the result's (got {tuple(out.shape)} with strides {out.stride()})")
     if g.is_cuda:
         _native.check_device(g)
     if g.numel() == 0:
