@@ -28,9 +28,21 @@ class FlatGroup:
         self.v = torch.zeros_like(self.master)
 
 
+def _check_buffers(param, grad):
+    """What the kernels read and write of a group, four elements at a time."""
+    if param.dtype != torch.bfloat16 or grad.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"the optimizer's kernels need bf16 parameters with fp32 or bf16 gradients (got {param.dtype}, {grad.dtype})")
+    for t in (param, grad):
+        if not t.is_contiguous() or t.data_ptr() % (4 * t.element_size()):
+            raise ValueError("the optimizer's kernels need contiguous buffers that begin on a boundary of four elements")
+
+
 class AdamW:
     def __init__(self, groups: List[FlatGroup], lr: float = 1e-4, betas=(0.9, 0.95), eps: float = 1e-8,
                  weight_decay: float = 0.0, max_grad_norm: Optional[float] = 1.0, mesh=None):
+        for g in groups:
+            if g.param.is_cuda:
+                _check_buffers(g.param, g.grad)
         self.groups, self.lr, self.betas, self.eps, self.wd = groups, lr, betas, eps, weight_decay
         self.max_grad_norm, self.mesh = max_grad_norm, mesh
         self.step_count = 0
