@@ -38,6 +38,23 @@ def _check_coefficients(steps: int, coefficients: Tuple[float, float, float]):
         raise ValueError(f"the polynomial of {coefficients} takes singular values out of range within {steps} steps")
 
 
+def check_polynomial(steps, coefficients) -> Tuple[int, Tuple[float, float, float]]:
+    if steps < 1 or int(steps) != steps:
+        raise ValueError(f"the number of steps is positive (got {steps})")
+    coefficients = tuple(coefficients)
+    if len(coefficients) != 3 or not all(map(math.isfinite, coefficients)):
+        raise ValueError(f"three finite coefficients (got {coefficients})")
+    _check_coefficients(int(steps), coefficients)
+    return int(steps), coefficients
+
+
+def check_kernels(rows: int, cols: int, steps: int):
+    """What the kernels take beside it."""
+    if max(rows, cols) >= 1 << 24 or steps > _native.load().UNIT_STEPS:
+        raise ValueError(f"the kernels take matrices of fewer than 2^24 rows and columns and at most {_native.load().UNIT_STEPS} steps "
+                         f"(got {rows} x {cols}, {steps})")
+
+
 def _own_elements(t) -> bool:
     """Every element has memory of its own: along each dimension a step leads beyond what the shorter steps reach."""
     reach = 0
@@ -60,12 +77,7 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
     be ``g``) or a new tensor of ``out_dtype``."""
     if g.dim() not in (2, 3) or g.dtype not in _TYPES:
         raise ValueError(f"matrices are fp32 or bf16 [rows, cols] or [n, rows, cols] (got {g.dtype} {tuple(g.shape)})")
-    if steps < 1 or int(steps) != steps:
-        raise ValueError(f"the number of steps is positive (got {steps})")
-    coefficients = tuple(coefficients)
-    if len(coefficients) != 3 or not all(map(math.isfinite, coefficients)):
-        raise ValueError(f"three finite coefficients (got {coefficients})")
-    _check_coefficients(int(steps), coefficients)
+    steps, coefficients = check_polynomial(steps, coefficients)
     if out is None:
         if out_dtype not in _TYPES:
             raise ValueError(f"the result is fp32 or bf16 (got {out_dtype})")
@@ -79,12 +91,10 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
     if g.numel() == 0:
         return out
     if not g.is_cuda:
-        return out.copy_(_reference(g, int(steps), coefficients))
+        return out.copy_(_reference(g, steps, coefficients))
     batch, target = (g[None], out[None]) if g.dim() == 2 else (g, out)
     items, r, c = batch.shape
-    if max(r, c) >= 1 << 24 or steps > _native.load().UNIT_STEPS:
-        raise ValueError(f"the kernels take matrices of fewer than 2^24 rows and columns and at most {_native.load().UNIT_STEPS} steps "
-                         f"(got {r} x {c}, {steps})")
+    check_kernels(r, c, steps)
     if not batch[0].is_contiguous():
         batch = batch.contiguous()
     if out is not g and _meet(batch, target):       # a matrix is read before its own result is written, not before those of others
@@ -104,7 +114,7 @@ def orthogonalize(g, steps: int = 5, coefficients=COEFFICIENTS, out: Optional[to
     stride, strides = batch.stride(0) if items > 1 else 0, (result.stride(0) if items > 1 else 0, result.stride(1), result.stride(2))
     for i in range(0, items, most):
         C.orthogonalize(batch.data_ptr() + i * stride * batch.element_size(), 1 if batch.dtype is torch.bfloat16 else 0, stride,
-                        min(most, items - i), r, c, int(steps), *coefficients, space, m, n,
+                        min(most, items - i), r, c, steps, *coefficients, space, m, n,
                         result.data_ptr() + i * strides[0] * result.element_size(), 1 if result.dtype is torch.float32 else 0, *strides, sms,
                         status, stream)
     if result is not target:

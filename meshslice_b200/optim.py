@@ -14,7 +14,7 @@ from typing import List, Optional
 import torch
 
 from . import _native
-from .ops.orthogonal import COEFFICIENTS, orthogonalize
+from .ops.orthogonal import COEFFICIENTS, check_kernels, check_polynomial, orthogonalize
 
 
 class FlatGroup:
@@ -222,7 +222,8 @@ class Muon(AdamW):
             raise ValueError("orthogonal updates are of whole matrices: a 1 x 1 mesh")
         if not 0.0 <= momentum < 1.0:
             raise ValueError(f"momentum must be in [0, 1) (got {momentum})")
-        self.momentum, self.nesterov, self.steps, self.coefficients = momentum, nesterov, steps, coefficients
+        self.momentum, self.nesterov = momentum, nesterov
+        self.steps, self.coefficients = check_polynomial(steps, coefficients)
         self._stacks = []                 # (group, first element, distance, count, rows, columns)
         self._rest = {}                   # of the groups, by identity of the group: spans that AdamW updates
         taken = {id(g): [] for g in groups}
@@ -247,8 +248,10 @@ class Muon(AdamW):
             self._rest[id(g)] = rest
 
     def _place(self, w: torch.Tensor):
-        if w.dim() != 2 or not w.is_contiguous() or w.numel() % 4:
-            raise ValueError(f"matrices are contiguous, of a multiple of 4 elements (got {tuple(w.shape)})")
+        if w.dim() != 2 or not w.is_contiguous() or w.numel() % 4 or w.numel() == 0:
+            raise ValueError(f"matrices are contiguous, of a multiple of 4 elements, and not empty (got {tuple(w.shape)})")
+        if w.is_cuda:
+            check_kernels(*w.shape, self.steps)
         for k, g in enumerate(self.groups):
             at = w.data_ptr() - g.param.data_ptr()
             if w.dtype == g.param.dtype and 0 <= at < g.param.numel() * g.param.element_size():

@@ -48,3 +48,36 @@ def test_gpu_steps_stay_in_their_buffers(kind, p, g, i, j):
     opt.step()
     assert torch.equal(group.param, group.master.to(BF)) and (group.param < 1).all()
     assert (param[:i] == 1).all() and (param[i + 256:] == 1).all() and (grad == 1).all()
+
+
+# ----------------------------------------------------------------------------------------------
+# orthogonal updates: before the first step, not in the middle of it
+# ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+@pytest.mark.parametrize("kw", [dict(steps=0), dict(steps=1.5), dict(coefficients=(1.5, -0.5)), dict(coefficients=(1.5, float("nan"), 0.0)),
+                                dict(coefficients=(6.0, 1.0, 1.0)), dict(steps=400, coefficients=(3.0, 0.0, 0.0))], ids=str)
+def test_polynomials_are_refused_when_the_optimizer_is_made(dev, kw):
+    group = FlatGroup(*buffers(dev, (BF, F32), (0, 0)), "sharded")
+    with pytest.raises(ValueError):
+        Muon([group], [group.param[:64].view(8, 8)], **kw)
+
+
+@pytest.mark.parametrize("dev", ["cpu", pytest.param("cuda", marks=gpu)])
+def test_empty_matrices_are_refused(dev):
+    group = FlatGroup(*buffers(dev, (BF, F32), (0, 0)), "sharded")
+    for shape in ((0, 8), (8, 0)):
+        with pytest.raises(ValueError):
+            Muon([group], [group.param[:64].view(8, 8), group.param[64:64].view(shape)])
+
+
+@gpu
+def test_gpu_more_steps_than_the_kernels_take():
+    group = FlatGroup(*buffers("cuda", (BF, F32), (0, 0)), "sharded")
+    with pytest.raises(ValueError, match="steps"):
+        Muon([group], [group.param[:64].view(8, 8)], steps=65, coefficients=(1.5, -0.5, 0.0))
+
+
+def test_other_polynomials_are_taken():
+    group = FlatGroup(*buffers("cpu", (F32, F32), (0, 0)), "sharded")
+    Muon([group], [group.param[:64].view(8, 8)], steps=3, coefficients=[1.875, -1.25, 0.375]).step()
+    assert group.param.isfinite().all()
