@@ -15,7 +15,8 @@ __device__ __forceinline__ float gate_sigmoid(float x, int act) {
 }
 // The activation's derivative, with s = sigmoid(q(x)).
 __device__ __forceinline__ float gate_slope(float x, float s, int act) {
-  const float dq = act == 0 ? 1.f : 1.5957691216057308f * (1.f + 3.f * 0.044715f * x * x);
+  const float c = fminf(fabsf(x), 64.f);       // beyond, s is 0 or 1 and 1 - s or s without a rest, and x x may leave fp32: 0 times infinity
+  const float dq = act == 0 ? 1.f : 1.5957691216057308f * (1.f + 3.f * 0.044715f * c * c);
   return s + x * s * (1.f - s) * dq;
 }
 

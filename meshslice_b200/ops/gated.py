@@ -219,10 +219,11 @@ def gated_act_bwd(dh, gate, up, act: str = "silu"):
 
 
 def _act(g, act: str):
-    """Activation and derivative in g's precision."""
+    """Activation and derivative in g's precision: both activations are g sigmoid(q(g)), whose small values a tanh would lose."""
     if act == "silu":
-        s = torch.sigmoid(g)
-        return g * s, s * (1 + g * (1 - s))
-    c = math.sqrt(2 / math.pi)
-    t = torch.tanh(c * (g + 0.044715 * g ** 3))
-    return 0.5 * g * (1 + t), 0.5 * (1 + t) + 0.5 * g * (1 - t * t) * c * (1 + 3 * 0.044715 * g * g)
+        q, dq = g, 1.0
+    else:
+        c, near = 2 * math.sqrt(2 / math.pi), g.clamp(-64, 64)      # beyond, s (1 - s) is 0, and g g may leave the precision's range
+        q, dq = c * (g + 0.044715 * g ** 3), c * (1 + 3 * 0.044715 * near * near)
+    s = torch.sigmoid(q)
+    return g * s, s + g * s * (1 - s) * dq

@@ -97,3 +97,74 @@ def test_gradients_side_by_side_are_taken(dev, dtype):
     for build in (columns, neighbours):
         got, _ = call(dev, build)
         assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+# ----------------------------------------------------------------------------------------------
+# gates of any size
+# ----------------------------------------------------------------------------------------------
+def tails64(x, act):
+    """Activation and derivative with sigmoids that keep their small values; how far fp32 may be off, as a share of both: the exponent q has up to
+    six roundings, and its product with log2 e two more, each of 2^-24 of q, which are shares of the exponential; exponential, division and the
+    products beside it 16 more of 2^-24.  Below 2^-120 a sigmoid may be 0."""
+    a, cubic = (1.0, 0.0) if act == "silu" else (2 * (2 / torch.pi) ** 0.5, 0.044715)
+    q = a * (x + cubic * x ** 3)
+    s, r = torch.sigmoid(q), torch.sigmoid(-q)
+    share = (8 * q.abs().clamp_max(90) + 16) * 2.0 ** -24
+    dq = a * (1 + 3 * cubic * x ** 2)
+    bend = torch.where(s * r == 0, 0.0, x * dq * s * r)
+    off = share * s + torch.where(s * r == 0, 0.0, (x * dq).abs() * (2 * share * s * r + 2.0 ** -22 * s)).abs()
+    return x * s, s + bend, share * (x * s).abs() + 2.0 ** -120 * x.abs(), off + 2.0 ** -118 * (1 + x.abs())
+
+
+def grid():
+    fine = torch.linspace(-12, 12, 3073)
+    far = torch.tensor([16., 40., 87., 89., 1e3, 1e6, 1e12, 1e13, 2e19, 1e20, 1e25, 1e30, 3e38])
+    return torch.cat([fine, far, -far, torch.zeros(5)]).bfloat16()
+
+
+@both
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_from_far_below_to_far_above(dev, act):
+    x = grid()
+    x = x[:x.numel() // 8 * 8]
+    one = torch.ones_like(x)
+    a, da, ea, eda = tails64(x.double(), act)
+    h = F.gated_act(x.to(dev), one.to(dev), act)
+    dg, du = F.gated_act_bwd(one.to(dev), x.to(dev), one.to(dev), act)
+    for got, want, off in ((h, a, ea), (du, a, ea), (dg, da, eda)):
+        got = got.double().cpu()
+        bad = (got - want).abs() > off + base.BF * want.abs() + 2.0 ** -126
+        assert not bad.any() and got.isfinite().all(), (x[bad], got[bad], want[bad])
+
+
+@both
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("tokens", [3, 24])
+def test_a_block_with_far_gates(dev, act, tokens):
+    """Gates of 1e4 and 2e19 and below -1e4 and -2e19: the activation is the gate or 0, its derivative 1 or 0."""
+    x = torch.zeros(tokens, 8).bfloat16()
+    size = torch.tensor([1e4, 1e-3, 2e19])[torch.arange(tokens) % 3]
+    x[:, 0] = size * torch.where(torch.arange(tokens) // 3 % 2 == 0, 1, -1)
+    wg, wu, wd = torch.zeros(8, 16).bfloat16(), torch.zeros(8, 16).bfloat16(), torch.eye(16).bfloat16()
+    wg[0] = 1
+    wu[0] = 2.0 ** -10
+    dy = torch.ones(tokens, 16).bfloat16()
+    args = [t.to(dev) for t in (x, wg, wu, wd)]
+    y, saved = F.gated_ff_fwd(*args, act=act)
+    alone = F.gated_ff_fwd(*args, act=act, keep=False)[0]
+    dx, grads = F.gated_ff_bwd(dy.to(dev), *args, saved, act=act)
+    g = x[:, :1].double()
+    a, da, _, _ = tails64(g, act)
+    h = a * g * 2.0 ** -10
+    for got in (y, alone):
+        assert (got.double().cpu() - h).abs().le(2.0 ** -7 * h.abs() + 1e-37).all()
+    want = 16 * (g * 2.0 ** -10 * da + a * 2.0 ** -10)                     # 16 features of one kind each
+    assert (dx[:, :1].double().cpu() - want).abs().le(2.0 ** -6 * (g.abs() * da.abs() + a.abs()) * 2.0 ** -6 + 1e-37).all() and dx[:, 1:].count_nonzero() == 0
+    # the up weight's has x a, up to 4e38: beyond fp32 itself
+    assert grads[0].isfinite().all() and grads[2].isfinite().all()
+
+
+@gpu
+@pytest.mark.parametrize("size,weight", [(1e-6, 1.0), (1e5, 1.0), (3e-20, 1e-6), (1e4, 1e4)])
+def test_gpu_range_of_gelu(size, weight):
+    base.run("cuda", base.data(140, 64, 72, 40, size=size, weight=weight), "gelu")
