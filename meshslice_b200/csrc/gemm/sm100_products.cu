@@ -246,8 +246,8 @@ __device__ __forceinline__ bool epilogue_gated_grad(const Product& p, const Tile
       float2 g = unh(xg[i]), u = unh(xu[i]);
       g.x *= fg; g.y *= fg; u.x *= fu; u.y *= fu;
       const float s0 = gate_sigmoid(g.x, p.act), s1 = gate_sigmoid(g.y, p.act);
-      wu[i] = pk2(v[2 * i] * g.x * s0, v[2 * i + 1] * g.y * s1);
-      wg[i] = pk2(v[2 * i] * u.x * gate_slope(g.x, s0, p.act), v[2 * i + 1] * u.y * gate_slope(g.y, s1, p.act));
+      wu[i] = pk2(v[2 * i] * (g.x * s0), v[2 * i + 1] * (g.y * s1));       // the bounded factor first, as in ops/gated.cu
+      wg[i] = pk2(v[2 * i] * (u.x * gate_slope(g.x, s0, p.act)), v[2 * i + 1] * (u.y * gate_slope(g.y, s1, p.act)));
     }
     if (c + 1 < kChunks && col0 + 32 < p.N) ask(col0 + 32);
     uint8_t* box = out.take(at.lane);

@@ -56,8 +56,8 @@ gated_act_bwd_kernel(const uint4* dh, const uint4* g, const uint4* u, uint4* dg,
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const float s = gate_sigmoid(a[k], act);
-      e[k] = d[k] * a[k] * s;
-      d[k] = d[k] * b[k] * gate_slope(a[k], s, act);
+      e[k] = d[k] * (a[k] * s);             // the bounded factor first: without it the others may leave fp32 where it is 0
+      d[k] = d[k] * (b[k] * gate_slope(a[k], s, act));
     }
     dg[i] = pack(d);
     du[i] = pack(e);

@@ -133,7 +133,7 @@ def gated_ff_bwd(dy, x, w_gate, w_up, w_down, saved: GatedSaved, act: str = "sil
         g, u, xf, dyf = saved.gate, saved.up, x.float(), dy.float()
         a, da = _act(g, act)
         dh = dyf @ (w_down.float().T if down_layout == "nn" else w_down.float())
-        dg, du, h = dh * u * da, dh * a, saved.h
+        dg, du, h = dh * (u * da), dh * a, saved.h
         back = lambda t, w: t @ (w.float().T if up_layout == "nn" else w.float())
         dx = (back(dg, w_gate) + back(du, w_up)).to(x.dtype)
         new = [xf.T @ dg, xf.T @ du] if up_layout == "nn" else [dg.T @ xf, du.T @ xf]
@@ -209,7 +209,7 @@ def gated_act_bwd(dh, gate, up, act: str = "silu"):
     _same(act, dh, gate, up)
     if not dh.is_cuda:
         a, da = _act(gate.float(), act)
-        return (dh.float() * up.float() * da).to(dh.dtype), (dh.float() * a).to(dh.dtype)
+        return (dh.float() * (up.float() * da)).to(dh.dtype), (dh.float() * a).to(dh.dtype)
     dg, du = (torch.empty(dh.shape, dtype=dh.dtype, device=dh.device) for _ in range(2))
     if dh.numel():
         dh, gate, up = _block(dh), _block(gate), _block(up)

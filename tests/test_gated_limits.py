@@ -139,6 +139,16 @@ def test_gates_from_far_below_to_far_above(dev, act):
 
 @both
 @pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gates_whose_activation_is_zero_beside_large_factors(dev, act):
+    """The factors' product is beyond fp32, the gradients are not."""
+    x = torch.tensor([-1e30, -1e20, -1e25, -1e30, -1e35, -3e38, -1e21, -1e30]).bfloat16().to(dev)
+    big = torch.full_like(x, 1e19)
+    dg, du = F.gated_act_bwd(big, x, big * 10, act)
+    assert dg.count_nonzero() == 0 and du.count_nonzero() == 0
+
+
+@both
+@pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("tokens", [3, 24])
 def test_a_block_with_far_gates(dev, act, tokens):
     """Gates of 1e4 and 2e19 and below -1e4 and -2e19: the activation is the gate or 0, its derivative 1 or 0."""
