@@ -1,6 +1,8 @@
 // Activations of gated feed-forward blocks in fp32.  Both are x sigmoid(q(x)): q(x) = x (silu), 2 sqrt(2 / pi) (x + 0.044715 x^3) (tanh-GeLU, since
-// 1 + tanh(y) = 2 sigmoid(2 y)), with ex2.approx and a division of 2 units in the last place: some 2^-21 of the value, where tanh.approx
-// would leave 2^-11.
+// 1 + tanh(y) = 2 sigmoid(2 y)), with ex2.approx and a division of 2 units in the last place.  A value is off by at most (8 |q| + 16) 2^-24 of it
+// where q is negative: the roundings of q, up to six, and of its product with log2 e are shares of the exponential there.  That is 2^-20 near 0, 2^-17.5
+// for a GeLU of -4 (q = -11), 2^-14 where the sigmoid leaves fp32 (q = -87), all far below the 2^-9 of a result in bf16; where q is positive 2^-20.
+// tanh.approx would leave 2^-11 everywhere.
 #pragma once
 #include <cuda_runtime.h>
 
