@@ -151,7 +151,9 @@ struct TileAt {
   __device__ __forceinline__ bool before() const {
     int ok = 1;
     if (lane == 0) ok = mbar_wait(written, written_phase, 7 * timeout_ns) ? 1 : 0;
-    return __shfl_sync(0xffffffffu, ok, 0) != 0;
+    ok = __shfl_sync(0xffffffffu, ok, 0);
+    __syncwarp();                          // a shuffle orders no memory: the other lanes read behind the wait too
+    return ok != 0;
   }
   // Bounded; false: given up.
   __device__ __forceinline__ bool wait() const {

@@ -240,6 +240,7 @@ orthogonal_small_kernel(const UnitSmall a) {
     int there = 1;
     if (lane == 0) there = finished(done) ? 1 : 0;
     there = __shfl_sync(0xffffffffu, there, 0);
+    __syncwarp();                          // a shuffle orders no memory: the other lanes read behind the wait too
     tc_fence_after_sync();
     return there != 0;
   };
