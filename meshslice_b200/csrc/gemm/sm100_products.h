@@ -92,7 +92,7 @@ struct ChainArgs {
   Product step[3];             // kStep: of either copy of X, and the last
   int items, steps;
   int tiles[2];                // of an item, kGram and kStep (set by the launcher)
-  uint32_t* counters;          // [3 steps, items], 0 at launch: epilogue warps that have written their part of a tile
+  uint32_t* counters;          // [3 steps, items], 0 at launch: CTAs that have written their part of a tile, two a tile
   uint32_t* status;
   uint64_t timeout_ns;
 };

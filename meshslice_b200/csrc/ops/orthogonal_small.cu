@@ -8,10 +8,12 @@
 //              rows are written to both CTAs.
 // X is held times 32 and A times 32^2, as their products are, so that sums become factors without a multiplication: fp16 has 11 significant
 // bits down to 2^-14 / 32 of X (an element of 256 x 256 is 2^-8 in the mean), and 2^-24 of what is below.
-// Between the products the epilogue warps turn sums into the next factors, where the factors before lie.  Latencies bound it.  A product of 256 takes 16
-// instructions of 128 cycles; what is between two products, even of 16 x 16, 2300 cycles: commit and wait 500, tensor memory, conversion and
-// shared memory 600, the fence to the tensor pipe's view of it 550 (1000 with stores to the other CTA), arrival and wait 300.  256 x 256 in five
-// steps 63 us (101 as seventeen launches), 64 x 64 36.
+// Between the products the epilogue warps turn sums into the next factors, where the factors before lie.  Latencies bound it.  A step of 16 x 16 takes 3.5 us,
+// of 64 x 64 4.9, of 256 x 256 9.7 (from calls of 1 to 20 steps, at 1.9 GHz).  Of the last the tensor pipe has 3.1, 16 instructions of 128 cycles a product;
+// from one product to the next are 2200 cycles of 16 x 16 (commit and wait 500, tensor memory, conversion and shared memory 600, the fence to the tensor
+// pipe's view of it 550, 1000 with stores to the other CTA, arrival and wait 300) and 4300 of 256 x 256, where a warp has 64 columns to
+// convert and to store to both CTAs.  Outside the steps are 17 to 23 us: the launch and its events 6, the rest G's way from memory,
+// |G| in 64 bits, the first factors, the result.  256 x 256 in five steps 66 to 71 us (101 as seventeen launches), 64 x 64 43.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -33,7 +35,9 @@ constexpr int kPart = kSide / (kEpiThreads / 128), kChunks = kPart / 32;   // co
 constexpr uint32_t kBlockRows = kHalf * 128;                       // 64 columns of a CTA's rows
 constexpr uint32_t kBlockCols = kSide * 128;                       // 64 columns of all rows
 constexpr uint32_t kRowBytes = kSide / 64 * kBlockRows, kColBytes = kHalf / 64 * kBlockCols;
-constexpr uint32_t kSmem = 2 * kRowBytes + kColBytes + 1024 + 256;
+// behind them: two barriers, both CTAs' norms, the slot of the tensor memory's address with room for another, the warps' sums
+constexpr uint32_t kTail = 2 * sizeof(uint64_t) + 2 * sizeof(double) + 2 * sizeof(uint32_t) + kEpiThreads / 32 * sizeof(double);
+constexpr uint32_t kSmem = 2 * kRowBytes + kColBytes + 1024 + kTail;          // the first 1024 for alignment
 static_assert(kRowBytes == 65536 && kColBytes == 65536, "");
 
 __device__ __forceinline__ uint32_t half2_of(float a, float b) {
@@ -80,7 +84,7 @@ orthogonal_small_kernel(const UnitSmall a) {
   uint64_t* const ready = done + 1;                                // in the leader: the factors are there; an arrival of every epilogue warp
   double* const norm = reinterpret_cast<double*>(ready + 1);       // [2]: of either CTA's part
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(norm + 2);
-  double* const red = reinterpret_cast<double*>(tmem_slot + 2);    // [8]
+  double* const red = reinterpret_cast<double*>(tmem_slot + 2);    // [kEpiThreads / 32]
 
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
