@@ -178,3 +178,24 @@ def test_a_block_with_far_gates(dev, act, tokens):
 @pytest.mark.parametrize("size,weight", [(1e-6, 1.0), (1e5, 1.0), (3e-20, 1e-6), (1e4, 1e4)])
 def test_gpu_range_of_gelu(size, weight):
     base.run("cuda", base.data(140, 64, 72, 40, size=size, weight=weight), "gelu")
+
+
+# ----------------------------------------------------------------------------------------------
+# few tokens: ends of the units and parts that the contraction is taken in
+# ----------------------------------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("layout,unit", [("nn", 32), ("nt", 128)])
+@pytest.mark.parametrize("ctas", [1, 2, 4, 8])
+@pytest.mark.parametrize("tokens", [5, 12])
+def test_gpu_few_tokens_at_the_ends_of_units(layout, unit, ctas, tokens):
+    """Eight warps of 1 to 8 CTAs take a unit each in turn: one unit less than a round, a round, 8 beyond, and beyond two rounds; as inputs of the gated
+    product and as features of the plain one.  A warp's share is a few instructions, so sums are off as those of 512 products are, twice at most
+    where a warp takes several rounds (an instruction is cut off at 2^-22 of the largest)."""
+    once = 8 * ctas * unit
+    for long in (once - unit, once, once + 8, 2 * once + unit - 8):
+        for d, f, o in ((long, 16, 24), (24, long, 16)):
+            args = base.data(tokens, d, f, o, seed=long)
+            y, off = base.definition(*args, "silu")["y"]
+            x, wg, wu, wd = (t.cuda() for t in (args[0], *(base.lay(w, layout) for w in args[1:4])))
+            got = F.gated_ff_fwd(x, wg, wu, wd, up_layout=layout, down_layout=layout, keep=False)[0]
+            base.near(got, (y, 2 * off))
