@@ -532,10 +532,14 @@ cudaError_t launch_sm100_gemm2(Gemm2Args& args, int problems, int tile_n, int sm
   int grid = (int)(2 * tiles < (sms & ~1) ? 2 * tiles : (sms & ~1));
   if (grid < 2) grid = 2;
   // Linear layers' gradients, added to fp32 and to bf16, in us without
-  // rounds, with rounds by k-blocks alone, and by walk_blocks: 64 tokens of 16384 x 4096 137, 243, 137 and 219, 911, 219; 64 of
-  // 4096 x 16384 150, 142, 143 and 252, 344, 231; 512 of 4096 x 16384 180, 148, 148 and 275, 343, 238.
-  const auto cost = [&](int i) { return walk_blocks(kb[i], args.p[i].accumulate && !args.p[i].c_fp32); };
-  args.rounds = problems > 1 ? (int)walk_rounds(of[0], cost(0), of[1], cost(1), grid / 2) : 0;
+  // rounds, with rounds by k-blocks alone, and by walk_blocks: 64 tokens of 16384 x 4096 131, 243, 133 and 217, 911, 216; 64 of
+  // 4096 x 16384 150, 142, 140 and 252, 344, 233; 512 of 4096 x 16384 176, 148, 146 and 274, 343, 237.
+  const int clusters = grid / 2, early = clusters - (int)(of[0] % clusters);
+  const auto cost = [&](int i) {
+    const Gemm2Problem& p = args.p[i];
+    return walk_blocks(kb[i], !p.accumulate ? kWalkStored : !p.c_fp32 ? kWalkAdded16 : 2 * early < clusters ? kWalkAdded32 : kWalkStored);
+  };
+  args.rounds = problems > 1 ? (int)walk_rounds(of[0], cost(0), of[1], cost(1), clusters) : 0;
   if (dgelu) return tile_n == 128 ? launch2<128, true>(args, grid, stream) : launch2<256, true>(args, grid, stream);
   return tile_n == 128 ? launch2<128, false>(args, grid, stream) : launch2<256, false>(args, grid, stream);
 }

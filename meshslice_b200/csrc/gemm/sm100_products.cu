@@ -1034,7 +1034,7 @@ cudaError_t launch_sm100_products(ProductArgs& args, int k0, int k1, int problem
   const int most = sms & ~1, grid = (int)(2 * tiles < most ? 2 * tiles : most);
   const auto kblocks = [&](int i) {
     const Product& p = args.p[i];
-    return walk_blocks((int64_t)p.kblocks[0] + p.kblocks[1], (i == 0 ? k0 : k1) == kPlain && p.accumulate && !p.out_fp32);
+    return walk_blocks((int64_t)p.kblocks[0] + p.kblocks[1], (i == 0 ? k0 : k1) == kPlain && p.accumulate && !p.out_fp32 ? kWalkAdded16 : kWalkStored);
   };
   args.lead = args.tiles[longer - 1];
   args.rounds = longer == problems ? 0 : (int)walk_rounds(args.lead, kblocks(0), args.tiles[2] - args.lead, kblocks(longer), grid / 2);

@@ -44,10 +44,14 @@ struct TileWalk {
 // vocabulary), us by k-blocks alone and with leasts of 6, 8, 12 and 16: 52 x 632 x 82320 317, 171, 165, 166, 169; 32 x 2112 x 49464 524, 221, 210,
 // 216, 223; 500 x 1024 x 50264 183, 183, 183, 187, 195.  Of a gated block of 512 x 4096 x 10752, added to bf16, by k-blocks alone and with leasts of
 // 12, 24, 36 and 48: 1123, 1118, 1050, 1017, 999.
-inline int64_t walk_blocks(int64_t k, bool adds_16 = false) {
-  const int64_t least = adds_16 ? 48 : 8;
-  return k < least ? least : k;
-}
+// In the plain GEMM, with four epilogue warps, a tile that the copy engine adds to fp32 values takes a pair as long as 24: where fewer than half of the
+// pairs take rounds of them, those end last with a least of 8.  Where more do, memory is what bounds them all, and the more of it happens while
+// others are on long tiles, the better.  Gradients of linear layers (tokens x inputs x outputs; pairs that take rounds), us without rounds and with leasts
+// of 8, 20, 24 and 28: 640 x 4440 x 6992 (20) 94, 109, 92, 91, 90; 408 x 7664 x 7728 (14) 141, 164, 148, 146, 144; 1000 x 4440 x 6992 (2) 111, 123, 115, 110,
+// 110; 736 x 11688 x 7816 (10) 301, 323, 302, 301, 301; 512 x 4096 x 16384 (42) 176, 146, 160, 163, 166; 64 x 4096 x 16384 (58) 150, 140, 144, 145, 145.
+// The products, with eight, stay with 8: 500 x 1024 x 50264 198 us, with 16 and 24 212 and 218.
+constexpr int64_t kWalkStored = 8, kWalkAdded32 = 24, kWalkAdded16 = 48;
+inline int64_t walk_blocks(int64_t k, int64_t least = kWalkStored) { return k < least ? least : k; }
 // Those rounds, for `n0` tiles of `k0` k-blocks and `n1` of `k1`, and the k-blocks of the pair that ends last.
 inline int64_t walk_rounds(int64_t n0, int64_t k0, int64_t n1, int64_t k1, int64_t clusters) {
   const int64_t late = n0 % clusters;
