@@ -452,22 +452,10 @@ static cudaError_t launch2(const Gemm2Args& args, int grid, cudaStream_t stream)
   return launch_dependent(sm100_gemm2_kernel<BN, kDGelu>, grid, kThreads2, smem, stream, args);
 }
 
-// The tile width that ends sooner.  A 64-deep k-block takes about 390 cycles on 128 columns (the loads: 24 KiB
-// a CTA) and 530 on 256 (the tensor pipe: 512), so a narrow tile counts three quarters of a wide one.  A CTA pair takes every
-// n-th tile: the last pair to end is the one with one tile more of either problem (pair 0) or the first without.
-// 2048 x 1024 x 4096 (32 wide tiles): 26.5 us wide, 19.6 narrow; 1024 x 2048 x 1024 11.9 and 8.7; 2048 x 2048 x 2048 (64
-// wide tiles, one wave against two): wide, 16.3 us.
-static int64_t last_end(const Gemm2Operands* o, int problems, int tile_n, int64_t pairs) {
-  int64_t tiles[2] = {0, 0}, kb[2] = {0, 0};
-  for (int i = 0; i < problems; ++i) {
-    tiles[i] = ((o[i].M + 2 * kBM - 1) / (2 * kBM)) * ((o[i].N + tile_n - 1) / tile_n);
-    kb[i] = (o[i].K + kBK - 1) / kBK;
-  }
-  return walk_end(tiles[0], kb[0], tiles[1], kb[1], pairs);
-}
 int gemm2_tile_n(const Gemm2Operands* o, int problems, int sms) {
-  const int64_t pairs = sms > 1 ? sms / 2 : 1;
-  return 3 * last_end(o, problems, 128, pairs) < 4 * last_end(o, problems, 256, pairs) ? 128 : 256;
+  WalkProblem p[2];
+  for (int i = 0; i < problems; ++i) p[i] = {o[i].M, o[i].N, (o[i].K + kBK - 1) / kBK, problems > 1 && o[i].accumulate && !o[i].c_fp32};
+  return walk_tile_n(p, problems, sms > 1 ? sms / 2 : 1);
 }
 
 // The order of the tiles, by what they read from HBM: under the power cap that traffic costs clock.  A panel of sixteen

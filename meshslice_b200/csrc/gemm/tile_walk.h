@@ -67,4 +67,29 @@ inline int64_t walk_end(int64_t n0, int64_t k0, int64_t n1, int64_t k1, int64_t 
   return ends_early > ends_late ? ends_early : ends_late;
 }
 
+
+// The tile width that ends sooner.  A 64-deep k-block takes about 390 cycles on 128 columns (the loads: 24 KiB
+// a CTA) and 530 on 256 (the tensor pipe: 512), so a narrow tile counts three quarters of a wide one.
+// 2048 x 1024 x 4096 (32 wide tiles): 26.5 us wide, 19.6 narrow; 1024 x 2048 x 1024 11.9 and 8.7; 2048 x 2048 x 2048 (64
+// wide tiles, one wave against two): wide, 16.3 us.
+// A tile whose sums are added to 16-bit values costs its epilogue at least, a narrow one half of it, two thirds in its own k-blocks: linear
+// layers' gradients by k-blocks alone and like this 2848 x 2720 x 472 49 and 35 us, 1208 x 1256 x 2400 33 and 31, 64 x 4096 x 16384 233 and 216, 232 x 3696 x
+// 6880 106 and 98, 16 x 1536 x 12944 83 and 88.  For sums that are stored or added to fp32 it does not tell: priced so, wide tiles were chosen for
+// 64 x 4096 x 16384 added to fp32, 169 us instead of 145.
+struct WalkProblem {
+  int64_t M, N, kblocks;
+  bool adds_16;
+};
+inline int64_t walk_end(const WalkProblem* p, int problems, int tile_n, int64_t clusters) {
+  int64_t tiles[2] = {0, 0}, k[2] = {0, 0};
+  for (int i = 0; i < problems; ++i) {
+    tiles[i] = (p[i].M + 255) / 256 * ((p[i].N + tile_n - 1) / tile_n);
+    k[i] = p[i].adds_16 ? walk_blocks(p[i].kblocks, tile_n == 128 ? kWalkAdded16 * 2 / 3 : kWalkAdded16) : p[i].kblocks;
+  }
+  return walk_end(tiles[0], k[0], tiles[1], k[1], clusters);
+}
+inline int walk_tile_n(const WalkProblem* p, int problems, int64_t clusters) {
+  return 3 * walk_end(p, problems, 128, clusters) < 4 * walk_end(p, problems, 256, clusters) ? 128 : 256;
+}
+
 }  // namespace msb
