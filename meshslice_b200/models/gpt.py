@@ -51,7 +51,8 @@ class GPTConfig:
     rotary: Optional[RotaryConfig] = None
     # feed-forward block of gate and up projection ('silu' or 'gelu' of the gate) in place of the GeLU one; ``ffn`` features each
     gated: str = ""
-    # the loss without the logits of a micro-batch in memory: this many tokens' at a time (0: chosen); whole matrices only (a 1 x 1 mesh)
+    # the loss without the logits of a micro-batch in memory: this many tokens' at a time (0: chosen); whole matrices only (a 1 x 1 mesh).  A step
+    # with a teacher compares logits with the teacher's, so there they are in memory all the same
     head_rows: Optional[int] = None
 
     def __post_init__(self):
